@@ -36,13 +36,24 @@ COMMON_FLAGS = [
     "-Xcompiler",
     "-fvisibility=hidden",
     "-shared",
+    "--threads",  # compile the sources side by side
+    "0",
 ]
 
 LIBS = {
-    "libfa_b200.so": ["flash_fwd_sm100.cu", "capi.cu", "capi_static.cu"],
+    "libfa_b200.so": [
+        "flash_fwd_sm100.cu",
+        "cache_append_sm100.cu",
+        "cache_attn_sm100.cu",
+        "window_sm100.cu",
+        "capi.cu",
+        "capi_static.cu",
+        "capi_stream.cu",
+    ],
     "libfa_selftest.so": ["selftest_sm100.cu"],
 }
-HEADERS = ["sm100_ptx.cuh", "softmax_common.cuh", "fa_internal.h", "tma_host.h", "capi_internal.h"]
+HEADERS = ["sm100_ptx.cuh", "softmax_common.cuh", "fa_internal.h", "tma_host.h", "capi_internal.h",
+           "stream_internal.h"]
 
 
 def nvcc_path() -> str:

@@ -51,7 +51,9 @@ __device__ fa_sm100::DeviceStatus g_device_status;
 SymbolCache g_status_cache;
 std::atomic<unsigned> g_epoch{0};
 
-cudaError_t status_ptr_for(int device, fa_sm100::DeviceStatus** out) {
+}  // namespace
+
+cudaError_t device_status_ptr(int device, fa_sm100::DeviceStatus** out) {
     void* p = nullptr;
     const cudaError_t err = g_status_cache.get(device, &p, [](void** dst) {
         return cudaGetSymbolAddress(dst, g_device_status);
@@ -67,8 +69,6 @@ unsigned next_epoch() {
     }
     return e;
 }
-
-}  // namespace
 
 int validate(const FaFwdParams* p) {
     if (p == nullptr) {
@@ -149,7 +149,7 @@ int launch_one(const FaFwdParams* p, cudaStream_t stream, int num_splits, void* 
         return cuda_fail(err, "cudaGetDevice");
     }
     fa_sm100::DeviceStatus* status = nullptr;
-    err = status_ptr_for(device, &status);
+    err = device_status_ptr(device, &status);
     if (err != cudaSuccess) {
         return cuda_fail(err, "cudaGetSymbolAddress");
     }
@@ -258,7 +258,7 @@ int fa_device_status(int32_t device, int32_t clear, uint32_t* status_out) {
     }
     fa_sm100::DeviceStatus* ptr = nullptr;
     fa_sm100::DeviceStatus host{};
-    err = fa_capi::status_ptr_for(device, &ptr);
+    err = fa_capi::device_status_ptr(device, &ptr);
     if (err == cudaSuccess) {
         err = cudaDeviceSynchronize();
     }

@@ -24,6 +24,10 @@ const char* last_error();
 
 bool aligned16(const void* p);
 
+// The watchdog record of `device` (which must be current), and a launch epoch (never 0).
+cudaError_t device_status_ptr(int device, fa_sm100::DeviceStatus** out);
+unsigned next_epoch();
+
 // The reference's fa::flash_fwd checks (csrc/kernels/flash_fwd.cu:625-652), same messages.
 int validate(const FaFwdParams* p);
 

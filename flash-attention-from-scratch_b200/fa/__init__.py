@@ -9,16 +9,20 @@
 Same public surface as the reference package (fa/__init__.py:14-38): ``forward``,
 ``forward_variant`` and ``attention_reference``; plus ``forward_splitkv``, ``forward_host`` (CPU
 tensors in and out, transfers overlapped with the kernels) and the multi-GPU ``forward_sharded`` /
-``plan_shards``. The kernel is tcgen05 / TMEM / TMA code for sm_100a in
+``plan_shards``. Streaming attention (an extension): ``forward_window`` / ``backward_window`` /
+``window_attention`` over a sliding window with sinks, and ``PagedKVCache`` with ``append_kv`` and
+``forward_cached``. The kernel is tcgen05 / TMEM / TMA code for sm_100a in
 libfa_b200.so; there is no CPU or fallback path.
 """
 
 import torch
 
 from fa import _C
+from fa.cache import PagedKVCache, append_kv, forward_cached
 from fa.host import forward_host
 from fa.reference import attention_reference
 from fa.shard import forward_sharded, plan_shards
+from fa.window import backward_window, forward_window, window_attention
 
 
 def forward(
@@ -93,4 +97,5 @@ def forward_splitkv(
 
 
 __all__ = ["forward", "forward_variant", "forward_splitkv", "forward_fp8", "quantize_fp8", "forward_host",
-           "attention_reference", "forward_sharded", "plan_shards"]
+           "attention_reference", "forward_sharded", "plan_shards", "forward_window", "backward_window",
+           "window_attention", "PagedKVCache", "append_kv", "forward_cached"]

@@ -1,0 +1,198 @@
+"""A paged key/value cache: appending to it (with the rotation by position) and attention over it.
+
+    cache = fa.PagedKVCache.empty(num_pages, page_size, kv_heads, head_dim)      # e4m3 with scales
+    lengths += new                                                              # tokens, the new ones included
+    q = fa.append_kv(cache, k, v, table, lengths, cos=cos, sin=sin, q=q)         # store k, v; rotate q
+    o = fa.forward_cached(q, cache, table, lengths, window=4096, sinks=4)
+
+Position j of sequence b is in slot j % page_size of page table[b, j // page_size]. Not in the
+reference, which has no cache (its q, k and v have one length).
+
+lengths, counts and the table stay on the device and are not read by the host, so a call can be
+captured in a CUDA graph and replayed as they change. Positions outside the table and pages outside
+the pool are skipped by the kernels and set bit 5 (32) of fa._C.device_status.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+import struct
+
+import torch
+
+from fa import _C
+from fa.window import _tensor_strides
+
+# FaCache, then FaAppendParams' and FaCachedParams' own fields (include/fa_b200.h).
+_CACHE = "7P5q7iB3x"
+_APPEND = struct.Struct("@" + _CACHE + "6P9q3iBB2x")
+_CACHED = struct.Struct("@" + _CACHE + "2P3q3ifB3x4x")
+
+
+class PagedKVCache:
+    """The pool of pages: k, v [num_pages, kv_heads, page_size, head_dim] (the last two dims
+    contiguous), float8_e4m3fn with k_scale, v_scale [num_pages, kv_heads] float32 (a value is its
+    code times its page's and head's scale), or float16 / bfloat16 without scales."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
+                 v_scale: torch.Tensor | None = None) -> None:
+        for t in (k, v):
+            if not t.is_cuda:
+                raise RuntimeError("the cache's k and v must be CUDA tensors")
+            if t.dtype not in _C.DTYPES and t.dtype != torch.float8_e4m3fn:
+                raise RuntimeError("the cache's k and v must be float8_e4m3fn, float16 or bfloat16")
+            if t.dim() != 4:
+                raise RuntimeError("the cache's k and v must have shape [pages, kv_heads, page_size, head_dim]")
+            if t.numel() > 0 and (t.stride(3) != 1 or t.stride(2) != t.shape[3]):
+                raise RuntimeError("a page's tokens must be contiguous for every head")
+        if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+            raise RuntimeError("the cache's k and v must have the same shape, dtype and device")
+        e4m3 = k.dtype == torch.float8_e4m3fn
+        for s in (k_scale, v_scale):
+            if (s is not None) != e4m3:
+                raise RuntimeError("a float8_e4m3fn cache needs k_scale and v_scale, a 16-bit one has none")
+            if s is not None and (s.shape != k.shape[:2] or s.dtype != torch.float32 or s.device != k.device
+                                  or not s.is_contiguous()):
+                raise RuntimeError("k_scale and v_scale must be contiguous float32 [pages, kv_heads] on k's device")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+
+    @classmethod
+    def empty(cls, num_pages: int, page_size: int, kv_heads: int, head_dim: int,
+              dtype: torch.dtype = torch.float8_e4m3fn, device: torch.device | str = "cuda") -> PagedKVCache:
+        """A pool of zeroed pages."""
+        shape = (num_pages, kv_heads, page_size, head_dim)
+        k, v = (torch.zeros(shape, dtype=torch.uint8 if dtype == torch.float8_e4m3fn else dtype, device=device).view(dtype)
+                for _ in "kv")
+        scales = (None, None)
+        if dtype == torch.float8_e4m3fn:
+            scales = tuple(torch.ones(shape[:2], dtype=torch.float32, device=device) for _ in "kv")
+        return cls(k, v, *scales)
+
+    def _fields(self, table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor | None, batch: int, tokens: int):
+        """FaCache's fields for these sequences, checked."""
+        k, v = self.k, self.v
+        device = k.device
+        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != batch or table.device != device or (
+                table.stride(1) != 1 and table.shape[1] > 1):
+            raise RuntimeError("page_table must be an int32 [B, pages] tensor with contiguous rows on the cache's device")
+        for t in (lengths,) if counts is None else (lengths, counts):
+            if t.dtype != torch.int32 or t.shape != (batch,) or t.device != device or not t.is_contiguous():
+                raise RuntimeError("lengths and counts must be contiguous int32 [B] tensors on the cache's device")
+        ks, vs = self.k_scale, self.v_scale
+        (k0, k1, _, _), (v0, v1, _, _) = k.stride(), v.stride()
+        pages, heads = self.num_pages, self.kv_heads
+        return (k.data_ptr(), v.data_ptr(), 0 if ks is None else ks.data_ptr(), 0 if vs is None else vs.data_ptr(),
+                table.data_ptr(), lengths.data_ptr(), 0 if counts is None else counts.data_ptr(),
+                k0 if pages > 1 else 0, k1 if heads > 1 else 0, v0 if pages > 1 else 0, v1 if heads > 1 else 0,
+                table.stride(0) if batch > 1 else table.shape[1], pages, self.page_size, table.shape[1], heads,
+                self.head_dim, batch, tokens, _C.DTYPES.get(k.dtype, _C.FA_DTYPE_FLOAT8_E4M3))
+
+
+def _check_tokens(cache: PagedKVCache, *tensors: torch.Tensor) -> None:
+    first = tensors[0]
+    for t in tensors:
+        if not t.is_cuda:
+            raise RuntimeError("q, k, v must be CUDA tensors")
+        if t.dtype not in _C.DTYPES:
+            raise RuntimeError("q, k, v must be float16 (or bfloat16)")
+        if t.dtype != first.dtype or (cache.k.dtype != torch.float8_e4m3fn and t.dtype != cache.k.dtype):
+            raise RuntimeError("q, k, v must have the same dtype, that of a 16-bit cache")
+        if t.dim() != 4:
+            raise RuntimeError("q, k, v must have shape [B, H, T, D]")
+        if t.device != cache.k.device:
+            raise RuntimeError("q, k, v must be on the cache's device")
+        if t.shape[0] != first.shape[0] or t.shape[2] != first.shape[2] or t.shape[3] != cache.head_dim:
+            raise RuntimeError("q, k, v must have the same batch and tokens, and the cache's head dim")
+
+
+def append_kv(
+    cache: PagedKVCache,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    page_table: torch.Tensor,
+    lengths: torch.Tensor,
+    counts: torch.Tensor | None = None,
+    cos: torch.Tensor | None = None,
+    sin: torch.Tensor | None = None,
+    q: torch.Tensor | None = None,
+    interleaved: bool = False,
+) -> torch.Tensor | None:
+    """Stores k, v [B, Hkv, T, D] into the cache and returns q [B, H, T, D] rotated (None without q).
+
+    lengths [B] int32 counts every sequence's tokens with the new ones; of the T new ones the first
+    counts[b] (all without counts) are real, at positions lengths[b] - counts[b] onwards, and the
+    rest is padding: not stored, zeros in the returned q. cos, sin [rows, R / 2] float32 turn the
+    first R dims (a multiple of 16) of q and k in pairs (i, i + R / 2), or (2 i, 2 i + 1) when
+    interleaved; without them nothing is turned. The rotation is in float32 and rounded once.
+
+    An e4m3 page's scale is the smallest power of two (2^-60 or more) that brings its values within
+    448. It grows while the page fills (older tokens are rescaled, exactly but for subnormal codes)
+    and starts anew with the page's first slot. No two sequences may append to one page."""
+    tensors = (k, v) if q is None else (k, v, q)
+    _check_tokens(cache, *tensors)
+    if k.shape != v.shape or k.shape[1] != cache.kv_heads:
+        raise RuntimeError("k and v must have shape [B, kv_heads, T, D]")
+    batch, _, tokens, dim = k.shape
+    rows = half = 0
+    if (cos is None) != (sin is None):
+        raise RuntimeError("cos and sin go together")
+    if cos is not None:
+        for t in (cos, sin):
+            if t.dtype != torch.float32 or t.dim() != 2 or t.device != k.device or not t.is_contiguous():
+                raise RuntimeError("cos and sin must be contiguous float32 [rows, R / 2] tensors on k's device")
+        if cos.shape != sin.shape:
+            raise RuntimeError("cos and sin must have the same shape")
+        rows, half = cos.shape
+    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    fields = cache._fields(page_table, lengths, counts, batch, tokens)
+    if batch == 0 or tokens == 0:
+        return out
+    params = _APPEND.pack(
+        *fields, k.data_ptr(), v.data_ptr(), 0 if q is None else q.data_ptr(), 0 if q is None else out.data_ptr(),
+        0 if cos is None else cos.data_ptr(), 0 if cos is None else sin.data_ptr(), *_tensor_strides(k), *_tensor_strides(v),
+        *((0, 0, 0) if q is None else _tensor_strides(q)), 0 if q is None else q.shape[1], rows, 2 * half, interleaved,
+        _C.DTYPES[k.dtype])
+    with torch.cuda.device(k.device):
+        rc = _C.lib.fa_append_kv(params, torch.cuda.current_stream(k.device).cuda_stream)
+    if rc != _C.FA_OK:
+        _C._raise(rc)
+    return out
+
+
+def forward_cached(
+    q: torch.Tensor,
+    cache: PagedKVCache,
+    page_table: torch.Tensor,
+    lengths: torch.Tensor,
+    counts: torch.Tensor | None = None,
+    window: int = 0,
+    sinks: int = 0,
+    softmax_scale: float | None = None,
+) -> torch.Tensor:
+    """O [B, H, T, D] of the newest tokens' queries q [B, H, T, D] over the cache.
+
+    lengths and counts as in append_kv: query t of sequence b is at position p = lengths[b] -
+    counts[b] + t and sees position j when 0 <= j <= p and (window == 0, or p - j < window, or
+    j < sinks); a row that sees nothing, padding among them, is zeros. H is a multiple of the
+    cache's heads, grouped as in forward_window. Scores, softmax and sums are in float32."""
+    _check_tokens(cache, q)
+    batch, heads, tokens, dim = q.shape
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    fields = cache._fields(page_table, lengths, counts, batch, tokens)
+    if q.numel() == 0:
+        return o
+    scale = 1.0 / math.sqrt(dim) if softmax_scale is None else float(softmax_scale)
+    params = _CACHED.pack(*fields, q.data_ptr(), o.data_ptr(), *_tensor_strides(q), heads, window, sinks, scale,
+                          _C.DTYPES[q.dtype])
+    with torch.cuda.device(q.device):
+        nbytes = ctypes.c_uint64(0)
+        rc = _C.lib.fa_cached_workspace_size(params, ctypes.byref(nbytes))
+        if rc == _C.FA_OK:
+            ws = torch.empty(nbytes.value, dtype=torch.uint8, device=q.device)
+            rc = _C.lib.fa_cached_attention(params, ws.data_ptr(), nbytes.value,
+                                            torch.cuda.current_stream(q.device).cuda_stream)
+    if rc != _C.FA_OK:
+        _C._raise(rc)
+    return o

@@ -198,6 +198,152 @@ FA_API int fa_flash_fwd_fp8(const FaFwdParams* params, float q_descale, float k_
 FA_API int fa_flash_fwd_splitkv_static(const FaFwdParams* params, int32_t num_splits,
                                        fa_stream_t stream);
 
+/* ---- Streaming attention (no counterpart in the reference, whose one kernel attends over dense
+ *      tensors of equal lengths and heads): a sliding window with sinks, forward and backward, a
+ *      paged key/value cache, and attention over it.
+ *
+ *      In all of them key position j is visible to a query at position p when 0 <= j <= p and
+ *      (window == 0, or p - j < window, or j < sinks). A query that sees nothing gives O = 0,
+ *      LSE = -infinity and no gradient. heads must be a multiple of kv_heads: query head h reads
+ *      key/value head h / (heads / kv_heads). Strides count elements; the head dim is
+ *      contiguous, every other stride a multiple of 8 elements (16 in a FA_DTYPE_FLOAT8_E4M3
+ *      cache), and every tensor 16-byte aligned. */
+
+/* Window attention over dense tensors: q, o, d_o, dq [batch, heads, q_len, head_dim], k, v, dk,
+ * dv [batch, kv_heads, k_len, head_dim]; query i is at position k_len - q_len + i. Strides are
+ * {batch, head, row}, positive for a dim of more than one element (no broadcast dims). dtype is FA_DTYPE_FLOAT16 or FA_DTYPE_BFLOAT16, for all of them. */
+typedef struct FaWindowParams {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* o;          /* written by the forward, read by the backward */
+    float* lse;       /* [batch, heads, q_len] contiguous, natural log of the row's sum of
+                         exp(scale * score); forward: written, may be NULL; backward: read */
+    const void* d_o;  /* backward only, as are dq, dk and dv */
+    void* dq;
+    void* dk;
+    void* dv;
+    int64_t q_stride[3];
+    int64_t k_stride[3];
+    int64_t v_stride[3];
+    int64_t o_stride[3];
+    int64_t do_stride[3];
+    int64_t dq_stride[3];
+    int64_t dk_stride[3];
+    int64_t dv_stride[3];
+    int32_t batch;
+    int32_t heads;
+    int32_t kv_heads;
+    int32_t q_len;
+    int32_t k_len;
+    int32_t head_dim; /* 64 or 128 */
+    int32_t window;   /* 0: none */
+    int32_t sinks;
+    float softmax_scale;
+    uint8_t dtype;
+    uint8_t reserved[3];
+} FaWindowParams;
+
+/* Enqueues O (and LSE) on `stream`. */
+FA_API int fa_window_fwd(const FaWindowParams* params, fa_stream_t stream);
+
+/* Bytes of device workspace fa_window_bwd needs on the current device (148 SMs assumed without
+ * one). */
+FA_API int fa_window_bwd_workspace_size(const FaWindowParams* params, uint64_t* bytes_out);
+
+/* Enqueues dQ, dK and dV on `stream`, from the forward's o and lse. `workspace`: device memory
+ * of at least that many bytes, 16-byte aligned; it needs no initialisation and may be reused
+ * once the call's work has completed. The gradients are bitwise deterministic. */
+FA_API int fa_window_bwd(const FaWindowParams* params, void* workspace, uint64_t workspace_bytes,
+                         fa_stream_t stream);
+
+/* A paged cache and the sequences in it. k, v: [num_pages, kv_heads, page_size, head_dim], the
+ * last two dims contiguous. FA_DTYPE_FLOAT8_E4M3 holds value / scale with one positive scale for
+ * every page and head, [num_pages, kv_heads] contiguous; the 16-bit types have no scales (NULL).
+ * Position j of sequence b is in slot j % page_size of page page_table[b][j / page_size].
+ * lengths[b]: tokens of sequence b, the call's `tokens` newest ones included. counts[b] (or NULL:
+ * all) of the call's tokens are real: token t of sequence b is at position lengths[b] -
+ * counts[b] + t, and tokens from counts[b] on are padding. The three are read on the device;
+ * positions outside the table and pages outside the pool are skipped, and set bit 5 (32) of
+ * fa_device_status. */
+typedef struct FaCache {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    const int32_t* page_table; /* [batch, max_pages], rows table_stride apart */
+    const int32_t* lengths;    /* [batch] */
+    const int32_t* counts;     /* [batch] or NULL */
+    int64_t k_stride[2];       /* {page, head} */
+    int64_t v_stride[2];
+    int64_t table_stride;
+    int32_t num_pages;
+    int32_t page_size;         /* a power of two, 8 .. 256 */
+    int32_t max_pages;         /* max_pages * page_size < 2^31 */
+    int32_t kv_heads;
+    int32_t head_dim;          /* 64 or 128 */
+    int32_t batch;
+    int32_t tokens;
+    uint8_t dtype;             /* FA_DTYPE_* */
+    uint8_t reserved[3];
+} FaCache;
+
+/* Rotates new queries and keys by their positions and stores keys and values into the cache.
+ * k_new, v_new [batch, kv_heads, tokens, head_dim], q and q_out [batch, heads, tokens, head_dim]
+ * (q NULL: no queries; q_out contiguous; zeros for padding tokens), strides {batch, head, token},
+ * of type `dtype`; a 16-bit cache has the same type. cos, sin: [table_rows, rotary_dim / 2]
+ * floats, contiguous (NULL: no rotation): the first rotary_dim (a multiple of 16) dims turn in
+ * pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with `interleaved`; a position beyond
+ * table_rows is skipped like one outside the page table.
+ *
+ * e4m3: a page's scale is the smallest power of two (2^-60 or more) that brings its largest finite
+ * value within 448. It only grows while a page fills (older tokens are rescaled) and starts anew
+ * when the page's first slot is written. Infinities saturate, NaN stays NaN. */
+typedef struct FaAppendParams {
+    FaCache cache;
+    const void* k_new;
+    const void* v_new;
+    const void* q;
+    void* q_out;
+    const float* cos;
+    const float* sin;
+    int64_t k_new_stride[3];
+    int64_t v_new_stride[3];
+    int64_t q_stride[3];
+    int32_t heads;
+    int32_t table_rows;
+    int32_t rotary_dim;
+    uint8_t interleaved;
+    uint8_t dtype; /* FA_DTYPE_FLOAT16 or FA_DTYPE_BFLOAT16 */
+    uint8_t reserved[2];
+} FaAppendParams;
+
+FA_API int fa_append_kv(const FaAppendParams* params, fa_stream_t stream);
+
+/* O = softmax(scale * q K^T | visible) V over the cache: q [batch, heads, tokens, head_dim] with
+ * strides {batch, head, token}, o contiguous (zeros for padding tokens), both of type `dtype`;
+ * a 16-bit cache has the same type. */
+typedef struct FaCachedParams {
+    FaCache cache;
+    const void* q;
+    void* o;
+    int64_t q_stride[3];
+    int32_t heads;
+    int32_t window; /* 0: none */
+    int32_t sinks;
+    float softmax_scale;
+    uint8_t dtype; /* FA_DTYPE_FLOAT16 or FA_DTYPE_BFLOAT16 */
+    uint8_t reserved[3];
+} FaCachedParams;
+
+/* Bytes of device workspace fa_cached_attention needs on the current device (148 SMs assumed
+ * without one). */
+FA_API int fa_cached_workspace_size(const FaCachedParams* params, uint64_t* bytes_out);
+
+/* Enqueues O on `stream`; `workspace` as in fa_window_bwd. Bitwise deterministic. */
+FA_API int fa_cached_attention(const FaCachedParams* params, void* workspace, uint64_t workspace_bytes,
+                               fa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
