@@ -1,11 +1,40 @@
-// Attention of the newest tokens of every sequence over the paged cache.
+// Attention of the newest tokens of every sequence over the paged cache (flash decoding).
 //
-// One warp per query row, the head dim over the lanes, keys one after the other with a running
-// maximum and sum: O = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m).
+//   O = sum_j e^(s_j) v_j / sum_j e^(s_j),   s_j = scale q.k_j over the visible positions j
+//
+// Every cache element is read once for a tile of 16 query rows (the query heads that share a kv
+// head, times the tokens), so the kernel is bound by DRAM bytes; what it needs is many loads in
+// flight, equal work for every SM whatever the lengths, and few instructions a byte.
+//
+// Split. The work is a list of (sequence, kv head, row tile) items of as many key tiles as the
+// sequence shows, laid end to end in units of key tiles and cut into equal ranges, one for each
+// CTA of a grid that fills the GPU. Lengths are on the device, so every CTA adds them up itself. A
+// CTA walks its range; an item that lies within it is written at once, one that was cut
+// leaves its unnormalised rows with (max, sum) in the workspace, at most two records a CTA, and a
+// second kernel (started early, by programmatic launch) joins them in order: no atomics.
+//
+// Within a CTA each of 4 warps takes every fourth key tile through a ring of its own, filled with
+// 16-byte cp.async copies: no CTA barrier until the item's end, where the warps' rows are joined in
+// shared memory. A key tile is 4 KB of K and 4 KB of V: 32 tokens of 128 e4m3 values, 16 of 128
+// 16-bit ones. 2 CTAs of 96 KB an SM keep up to 128 KB in flight; 6.5 TB/s at about 1 us needs 44.
+//
+// Products are mma.sync m16n8k16: with 16 rows of queries and two operations a byte of K
+// or V an M = 128 tcgen05 tile would be seven eighths padding, and dequantised operands would have to
+// go back to shared memory for it. e4m3 widens exactly to float16; bfloat16 queries are brought
+// into float16's range by a power of two per row, which is exact but for values 2^-38 below
+// the row's largest. Both products permute their contraction (head dim, keys) and output columns so
+// that a lane's fragments are whole 16-byte words of the cache's own rows.
+//
+// e4m3's value scales. With w_j = e^(s_j) vs_j (vs_j: the scale of j's page) O = sum w_j c_j / sum
+// (w_j / vs_j) over the codes c_j. The running maximum is taken over log2 w_j = s_j log2 e + log2
+// vs_j, so P <= 1 keeps its 11 bits where the output comes from, whatever the scales of other
+// pages; the sum takes P / vs_j in fp32. Scales below 2^-60 (0 among them) enter as 2^-60 with P
+// scaled down.
 
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -16,127 +45,782 @@ namespace fa_sm100 {
 
 namespace {
 
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kRows = 16;          // query rows of an item: the M of the matrix instruction
+constexpr int kStages = 3;         // key tiles of a warp's ring
+constexpr int kTileBytes = 4096;   // K (or V) of a key tile
+constexpr int kAuxFloats = 16;     // of a stage: 8 K scales, 8 V scales
+constexpr int kCtasPerSm = 2;
+constexpr int kMinTiles = kWarps;  // least key tiles of a CTA: one for each warp
+constexpr float kMinScale = 8.673617379884035e-19f;  // 2^-60
+constexpr int kSmem = kWarps * kStages * (2 * kTileBytes + kAuxFloats * 4);
+
+template <int D_, bool BF16_, bool E4M3_>
+struct Cfg {
+    static constexpr int D = D_;
+    static constexpr bool BF16 = BF16_;  // queries and output
+    static constexpr bool E4M3 = E4M3_;
+    static constexpr bool kMmaBf16 = BF16 && !E4M3;
+    static constexpr int kElem = E4M3 ? 1 : 2;
+    static constexpr int kRowBytes = D * kElem;
+    static constexpr int kKeys = kTileBytes / kRowBytes;  // 16, 32 or 64
+    static constexpr int kChunks = kRowBytes / 16;
+    static constexpr int kSteps = D / 16;   // k steps of Q K^T
+    static constexpr int kNTiles = kKeys / 8;
+    static constexpr int kOTiles = D / 8;
+    static constexpr bool kNarrow = kRowBytes == 64;  // two rows in a 128-byte line
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 template <bool BF16>
-__device__ __forceinline__ float widen(uint16_t x) {
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (BF16) {
-        return __uint_as_float(static_cast<uint32_t>(x) << 16);
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     } else {
-        return __half2float(__ushort_as_half(x));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
 }
 
-template <int D, bool BF16, bool E4M3>
-__global__ void __launch_bounds__(128) cached_rows_kernel(const __grid_constant__ FaCachedParams p,
-                                                          DeviceStatus* status) {
-    constexpr int PER = D / 32;
-    const FaCache& c = p.cache;
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ float lds_f(uint32_t at) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ void sts_f(uint32_t at, float v) {
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+
+// Byte offsets of chunk `c` (16 bytes) of token `r` in a K and in a V tile. The swizzles make the
+// fragment reads below free of bank conflicts: a K read takes chunks t, t + 4, .. of tokens g
+// (lane = 4 g + t), a V read chunk g of tokens 2 t, 2 t + 1.
+template <class C>
+__device__ __forceinline__ uint32_t k_offset(int r, int c) {
+    return static_cast<uint32_t>(r * C::kRowBytes + (C::kNarrow ? c : c ^ ((r & 1) << 2)) * 16);
+}
+template <class C>
+__device__ __forceinline__ uint32_t v_offset(int r, int c) {
+    if constexpr (C::kNarrow) {
+        const int row = (r & ~3) | ((r & 1) << 1) | ((r >> 1) & 1);
+        return static_cast<uint32_t>(row * 64 + (c ^ ((r >> 1) & 2)) * 16);
+    } else {
+        return static_cast<uint32_t>(r * C::kRowBytes + (c ^ (r & 7)) * 16);
+    }
+}
+
+// What a sequence shows its queries: positions [0, sinks) and [first, last], as a list of key tiles.
+struct Sequence {
+    int pos0;    // position of its first query (may be negative)
+    int count;   // queries
+    int last;    // last position any query sees, -1 if none
+    int first;   // first position of the earliest window
+    int sink_tiles, first_tile, tiles;
+};
+
+template <class C>
+__device__ __forceinline__ Sequence sequence(const FaCachedParams& p, int b) {
+    Sequence s;
+    const int len = p.cache.lengths[b];
+    s.count = p.cache.counts != nullptr ? min(max(p.cache.counts[b], 0), p.cache.tokens) : p.cache.tokens;
+    s.pos0 = len - s.count;
+    s.last = s.count > 0 ? max(len - 1, -1) : -1;
+    s.first = window_first(max(s.pos0, 0), p.window);
+    s.first_tile = s.first / C::kKeys;
+    s.sink_tiles = min((min(p.sinks, s.first) + C::kKeys - 1) / C::kKeys, s.first_tile);
+    // A sequence that shows nothing keeps one (hidden) tile, so that its rows are written.
+    s.tiles = s.last < 0 ? 1 : s.sink_tiles + s.last / C::kKeys - s.first_tile + 1;
+    return s;
+}
+
+struct Range {
+    long long total, per;   // key tiles of all items, of a CTA
+    long long found_base;   // start of the sequence found
+    int found;
+};
+
+// The work list's length, and the sequence that holds unit `at(per)` of it. All threads call.
+template <class C, class At>
+__device__ __forceinline__ Range locate(const FaCachedParams& p, int grid, At at) {
+    __shared__ long long warp_sum[kWarps];
+    __shared__ long long found_base;
+    __shared__ int found;
+    const int heads_rows = p.cache.kv_heads * ((p.heads / p.cache.kv_heads * p.cache.tokens + kRows - 1) / kRows);
     const int lane = static_cast<int>(threadIdx.x) % 32;
-    const long long row = static_cast<long long>(blockIdx.x) * 4 + threadIdx.x / 32;
-    if (row >= static_cast<long long>(c.batch) * p.heads * c.tokens) {
+    const int warp = static_cast<int>(threadIdx.x) / 32;
+    const int share = (p.cache.batch + kThreads - 1) / kThreads;
+    const int b0 = min(static_cast<int>(threadIdx.x) * share, p.cache.batch);
+    const int b1 = min(b0 + share, p.cache.batch);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) {
+        mine += sequence<C>(p, b).tiles;
+    }
+    mine *= heads_rows;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+        incl += lane >= o ? up : 0;
+    }
+    if (lane == 31) {
+        warp_sum[warp] = incl;
+    }
+    if (threadIdx.x == 0) {
+        found = -1;
+    }
+    __syncthreads();
+    Range r;
+    r.total = 0;
+    long long before = incl - mine;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        before += w < warp ? warp_sum[w] : 0;
+        r.total += warp_sum[w];
+    }
+    r.per = max((r.total + grid - 1) / grid, static_cast<long long>(kMinTiles));
+    const long long target = at(r.per);
+    if (target >= before && target < before + mine) {
+        long long base = before;
+        for (int b = b0; b < b1; ++b) {
+            const long long n = static_cast<long long>(sequence<C>(p, b).tiles) * heads_rows;
+            if (target < base + n) {
+                found = b;
+                found_base = base;
+                break;
+            }
+            base += n;
+        }
+    }
+    __syncthreads();
+    r.found = found;
+    r.found_base = found_base;
+    return r;
+}
+
+struct Record {  // of a cut item's rows in the workspace
+    float* o;    // [record][16][D]
+    float2* ml;  // [record][16]
+};
+
+// One range of key tiles [v0, v1) of an item; `tiles` of the item in all.
+template <class C>
+__device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* status, uint8_t* smem, const Sequence& s,
+                                       int b, int kvh, int row0, int v0, int v1, Record rec, long long record) {
+    constexpr int D = C::D;
+    const FaCache& c = p.cache;
+    const int warp = static_cast<int>(threadIdx.x) / 32;
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    const int g = lane / 4;
+    const int t = lane % 4;
+    const int group = p.heads / c.kv_heads;
+    const int rows = group * c.tokens;
+    const uint32_t ring = smem_u32(smem) + warp * kStages * 2 * kTileBytes;
+    const uint32_t aux = smem_u32(smem) + kWarps * kStages * 2 * kTileBytes + warp * kStages * kAuxFloats * 4;
+
+    // Pages of a key tile: `span` tokens each, at most 8 of them.
+    const int log2_page = 31 - __clz(c.page_size);
+    const int log2_span = min(log2_page, 31 - __clz(C::kKeys));
+    const int spans = C::kKeys >> log2_span;
+
+    auto tile_key = [&](int v) { return (v < s.sink_tiles ? v : v - s.sink_tiles + s.first_tile) * C::kKeys; };
+    auto shown = [&](int key) { return key <= s.last && (key >= s.first || key < p.sinks); };
+    // Lane i < spans: the page of the tile's i-th span (-1: outside the pool, or hidden).
+    auto fetch = [&](int v) {
+        int id = -1;
+        if (v < v1 && lane < spans) {
+            const int key = tile_key(v) + (lane << log2_span);
+            const int end = key + (1 << log2_span) - 1;
+            if (key <= s.last && (end >= s.first || key < p.sinks)) {
+                const int page = key >> log2_page;
+                id = page < c.max_pages ? __ldg(c.page_table + b * c.table_stride + page) : -1;
+                if (id < 0 || id >= c.num_pages) {
+                    id = -1;
+                    atomicOr(&status->code, kStatusBadPage);
+                }
+            }
+        }
+        return id;
+    };
+    const int chunk = lane % C::kChunks;
+    const uint8_t* kbase = static_cast<const uint8_t*>(c.k) + kvh * c.k_stride[1] * C::kElem + chunk * 16;
+    const uint8_t* vbase = static_cast<const uint8_t*>(c.v) + kvh * c.v_stride[1] * C::kElem + chunk * 16;
+    const int64_t kpage = c.k_stride[0] * C::kElem;
+    const int64_t vpage = c.v_stride[0] * C::kElem;
+    auto issue = [&](int v, int stage, int ids) {
+        if (v < v1) {
+            const int key0 = tile_key(v);
+            const uint32_t ks = ring + stage * 2 * kTileBytes;
+            const uint32_t vs = ks + kTileBytes;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * (32 / C::kChunks) + lane / C::kChunks;
+                const int id = __shfl_sync(0xffffffffu, ids, r >> log2_span);
+                const int key = key0 + r;
+                const bool real = id >= 0 && shown(key);
+                const int64_t slot = static_cast<int64_t>(key & (c.page_size - 1)) * C::kRowBytes;
+                cp_async16(ks + k_offset<C>(r, chunk), real ? kbase + id * kpage + slot : kbase, real);
+                cp_async16(vs + v_offset<C>(r, chunk), real ? vbase + id * vpage + slot : vbase, real);
+            }
+            if (lane < spans) {
+                const uint32_t at = aux + stage * kAuxFloats * 4 + lane * 4;
+                if (C::E4M3 && ids >= 0) {
+                    const int64_t n = static_cast<int64_t>(ids) * c.kv_heads + kvh;
+                    cp_async4(at, c.k_scale + n);
+                    cp_async4(at + 32, c.v_scale + n);
+                } else {
+                    sts_f(at, ids >= 0 ? 1.0f : -1.0f);  // below 0: the span is hidden
+                    sts_f(at + 32, 1.0f);
+                }
+            }
+        }
+        cp_commit();
+    };
+
+    // The warp's first tiles are on their way while the queries are read.
+    int next = v0 + warp;
+    int ids = fetch(next);
+    for (int i = 0; i < kStages - 1; ++i) {
+        const int ahead = fetch(next + kWarps);
+        issue(next, i, ids);
+        ids = ahead;
+        next += kWarps;
+    }
+
+    // Query fragments: rows g and g + 8; a k step takes 4 dims of every lane t.
+    uint32_t q[C::kSteps][4];
+    float factor[2];  // scale * log2 e, and the row's power of two taken back
+    int pos[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int r = row0 + g + 8 * half;
+        const int head = r / c.tokens;
+        const int token = r - head * c.tokens;
+        const bool real = r < rows && token < s.count;
+        pos[half] = real ? s.pos0 + token : -1;
+        const uint16_t* src = static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] +
+                              static_cast<int64_t>(kvh * group + head) * p.q_stride[1] + token * p.q_stride[2];
+        float amax = 0.0f;
+#pragma unroll
+        for (int k = 0; k < C::kSteps; ++k) {
+            const int d = C::E4M3 ? 16 * (t + 4 * (k / 4)) + 4 * (k % 4) : 8 * (t + 4 * (k / 2)) + 4 * (k % 2);
+            const uint2 w = real ? __ldg(reinterpret_cast<const uint2*>(src + d)) : make_uint2(0u, 0u);
+            q[k][half] = w.x;
+            q[k][2 + half] = w.y;
+            if constexpr (C::E4M3 && C::BF16) {
+                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(__uint_as_float(w.x << 16)), fabsf(__uint_as_float(w.x & 0xFFFF0000u))),
+                                         fmaxf(fabsf(__uint_as_float(w.y << 16)), fabsf(__uint_as_float(w.y & 0xFFFF0000u)))));
+            }
+        }
+        factor[half] = p.softmax_scale * 1.4426950408889634f;
+        if constexpr (C::E4M3 && C::BF16) {
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            // 2^(13 - exponent of amax), both it and its inverse normal; 1 for zeros, inf and NaN.
+            const int e = static_cast<int>(__float_as_uint(amax) >> 23);
+            const int shift = (e == 0 || e == 255) ? 0 : min(max(140 - e, -100), 100);
+            const float up = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+            factor[half] *= __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
+#pragma unroll
+            for (int k = 0; k < C::kSteps; ++k) {
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const uint32_t x = q[k][2 * w + half];
+                    q[k][2 * w + half] = pack_half2(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xFFFF0000u) * up);
+                }
+            }
+        }
+    }
+
+    float o[C::kOTiles][4];
+#pragma unroll
+    for (int i = 0; i < C::kOTiles; ++i) {
+        o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    }
+    float m[2] = {-INFINITY, -INFINITY};
+    float l[2] = {0.0f, 0.0f};
+
+    int stage = 0;
+    for (int v = v0 + warp; v < v1; v += kWarps) {
+        cp_wait<kStages - 2>();
+        __syncwarp();  // the tile is there, and every lane has left the stage that is refilled next
+        {
+            const int ahead = fetch(next + kWarps);
+            issue(next, stage == 0 ? kStages - 1 : stage - 1, ids);
+            ids = ahead;
+            next += kWarps;
+        }
+        const uint32_t ks = ring + stage * 2 * kTileBytes;
+        const uint32_t vs = ks + kTileBytes;
+        const uint32_t sc = aux + stage * kAuxFloats * 4;
+        const int key0 = tile_key(v);
+
+        // Scores: keys 8 n + g of the tile, lane t's dims.
+        float x[C::kNTiles][4];
+#pragma unroll
+        for (int n = 0; n < C::kNTiles; ++n) {
+            x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
+#pragma unroll
+            for (int cc = 0; cc < C::kChunks / 4; ++cc) {
+                const uint4 w4 = lds128(ks + k_offset<C>(8 * n + g, t + 4 * cc));
+                const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                if constexpr (C::E4M3) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        mma16816<false>(x[n], q[4 * cc + i], e4m3x2_to_half2(w[i]), e4m3x2_to_half2(w[i] >> 16));
+                    }
+                } else {
+                    mma16816<C::kMmaBf16>(x[n], q[2 * cc], w[0], w[1]);
+                    mma16816<C::kMmaBf16>(x[n], q[2 * cc + 1], w[2], w[3]);
+                }
+            }
+        }
+
+        // log2 of the weights, and what is hidden.
+        const bool whole = key0 + C::kKeys - 1 <= s.pos0 &&
+                           (p.window == 0 || s.last - key0 < p.window || key0 + C::kKeys <= p.sinks);
+        float inv_vs[C::kNTiles];
+        float shrink = 1.0f;  // of P, for scales below 2^-60
+        float tile_shrink[C::kNTiles];
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < C::kNTiles; ++n) {
+            const int span = (8 * n) >> log2_span;
+            const float kscale = lds_f(sc + span * 4);
+            float lv = kscale < 0.0f ? -INFINITY : 0.0f;
+            inv_vs[n] = 1.0f;
+            tile_shrink[n] = 1.0f;
+            if constexpr (C::E4M3) {
+                const float vscale = lds_f(sc + 32 + span * 4);
+                const float used = fmaxf(vscale, kMinScale);
+                inv_vs[n] = __frcp_rn(used);
+                lv += __log2f(used);
+                tile_shrink[n] = vscale >= kMinScale ? 1.0f : vscale * inv_vs[n];
+                shrink = fminf(shrink, tile_shrink[n]);
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const float f = factor[half] * (C::E4M3 ? fabsf(kscale) : 1.0f);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float y = fmaf(x[n][2 * half + e], f, lv);
+                    if (!whole) {
+                        const int key = key0 + 8 * n + 2 * t + e;
+                        const int gap = pos[half] - key;
+                        const bool seen = gap >= 0 && (p.window == 0 || gap < p.window || key < p.sinks);
+                        y = seen ? y : -INFINITY;
+                    }
+                    x[n][2 * half + e] = y;
+                    top[half] = fmaxf(top[half], y);
+                }
+            }
+        }
+        float used[2];
+        bool grew = false;
+        float alpha[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
+            top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
+            const float now = fmaxf(m[half], top[half]);
+            used[half] = now == -INFINITY ? 0.0f : now;
+            alpha[half] = ex2_approx(m[half] - used[half]);
+            grew = grew || now > m[half];
+            m[half] = now;
+        }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                l[half] *= alpha[half];
+#pragma unroll
+                for (int i = 0; i < C::kOTiles; ++i) {
+                    o[i][2 * half] *= alpha[half];
+                    o[i][2 * half + 1] *= alpha[half];
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < C::kNTiles; ++n) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const float p0 = ex2_approx(x[n][2 * half] - used[half]);
+                const float p1 = ex2_approx(x[n][2 * half + 1] - used[half]);
+                l[half] = C::E4M3 ? fmaf(p0 + p1, inv_vs[n], l[half]) : l[half] + (p0 + p1);
+                x[n][2 * half] = p0;
+                x[n][2 * half + 1] = p1;
+            }
+        }
+        if (C::E4M3 && shrink != 1.0f) {
+#pragma unroll
+            for (int n = 0; n < C::kNTiles; ++n) {
+                x[n][0] *= tile_shrink[n];
+                x[n][1] *= tile_shrink[n];
+                x[n][2] *= tile_shrink[n];
+                x[n][3] *= tile_shrink[n];
+            }
+        }
+
+        // O += P V, 16 keys a step: lane (g, t) brings keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 and
+        // the dims of its chunk g, byte i of it for output tile i.
+#pragma unroll
+        for (int k = 0; k < C::kKeys / 16; ++k) {
+            uint32_t a[4];
+            a[0] = pack2<C::kMmaBf16>(x[2 * k][0], x[2 * k][1]);
+            a[1] = pack2<C::kMmaBf16>(x[2 * k][2], x[2 * k][3]);
+            a[2] = pack2<C::kMmaBf16>(x[2 * k + 1][0], x[2 * k + 1][1]);
+            a[3] = pack2<C::kMmaBf16>(x[2 * k + 1][2], x[2 * k + 1][3]);
+            const int r = 16 * k + 2 * t;
+            if constexpr (C::E4M3) {
+                constexpr int W = C::kNarrow ? 2 : 4;  // words of a lane's dims
+                uint32_t w[4][W];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = r + (i & 1) + 8 * (i >> 1);
+                    if constexpr (C::kNarrow) {
+                        const uint2 y = lds64(vs + v_offset<C>(key, g >> 1) + (g & 1) * 8);
+                        w[i][0] = y.x;
+                        w[i][1] = y.y;
+                    } else {
+                        const uint4 y = lds128(vs + v_offset<C>(key, g));
+                        w[i][0] = y.x;
+                        w[i][1] = y.y;
+                        w[i][2] = y.z;
+                        w[i][3] = y.w;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    const uint32_t lo0 = __byte_perm(w[0][j], w[1][j], 0x5140);
+                    const uint32_t hi0 = __byte_perm(w[0][j], w[1][j], 0x7362);
+                    const uint32_t lo1 = __byte_perm(w[2][j], w[3][j], 0x5140);
+                    const uint32_t hi1 = __byte_perm(w[2][j], w[3][j], 0x7362);
+                    mma16816<false>(o[4 * j], a, e4m3x2_to_half2(lo0), e4m3x2_to_half2(lo1));
+                    mma16816<false>(o[4 * j + 1], a, e4m3x2_to_half2(lo0 >> 16), e4m3x2_to_half2(lo1 >> 16));
+                    mma16816<false>(o[4 * j + 2], a, e4m3x2_to_half2(hi0), e4m3x2_to_half2(hi1));
+                    mma16816<false>(o[4 * j + 3], a, e4m3x2_to_half2(hi0 >> 16), e4m3x2_to_half2(hi1 >> 16));
+                }
+            } else {
+#pragma unroll
+                for (int cc = 0; cc < C::kChunks / 8; ++cc) {
+                    uint4 y[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        y[i] = lds128(vs + v_offset<C>(r + (i & 1) + 8 * (i >> 1), g + 8 * cc));
+                    }
+                    const uint32_t w[4][4] = {{y[0].x, y[0].y, y[0].z, y[0].w},
+                                              {y[1].x, y[1].y, y[1].z, y[1].w},
+                                              {y[2].x, y[2].y, y[2].z, y[2].w},
+                                              {y[3].x, y[3].y, y[3].z, y[3].w}};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        mma16816<C::kMmaBf16>(o[8 * cc + 2 * j], a, __byte_perm(w[0][j], w[1][j], 0x5410),
+                                              __byte_perm(w[2][j], w[3][j], 0x5410));
+                        mma16816<C::kMmaBf16>(o[8 * cc + 2 * j + 1], a, __byte_perm(w[0][j], w[1][j], 0x7632),
+                                              __byte_perm(w[2][j], w[3][j], 0x7632));
+                    }
+                }
+            }
+        }
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+    cp_wait<0>();
+    __syncthreads();
+
+    // Join the warps' rows: [warp][16][D] floats over the rings, then [warp][16] (max, sum). Groups
+    // of 4 dims are swizzled by their row and 32-dim block against bank conflicts.
+    float4* all_o = reinterpret_cast<float4*>(smem);
+    float2* all_ml = reinterpret_cast<float2*>(smem + kWarps * kRows * D * 4);
+    static_assert(kWarps * kRows * (D * 4 + 8) <= kSmem, "the joined rows fit over the rings");
+    auto place = [](int row, int four) { return row * (D / 4) + (four ^ (((four >> 3) & 3) | ((row & 1) << 2))); };
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+        const int row = g + 8 * half;
+        if (t == 0) {
+            all_ml[warp * kRows + row] = make_float2(m[half], l[half]);
+        }
+        // Column c of output tile i is dim W c + i of its block of 8 W dims (W output tiles).
+        constexpr int W = C::E4M3 ? C::kOTiles : 8;
+#pragma unroll
+        for (int i = 0; i < C::kOTiles; i += 4) {
+            const int block = i / W * 8 * W;
+            const int d0 = block + W * (2 * t) + i % W;
+            const int d1 = d0 + W;
+            all_o[warp * (kRows * D / 4) + place(row, d0 / 4)] =
+                make_float4(o[i][2 * half], o[i + 1][2 * half], o[i + 2][2 * half], o[i + 3][2 * half]);
+            all_o[warp * (kRows * D / 4) + place(row, d1 / 4)] =
+                make_float4(o[i][2 * half + 1], o[i + 1][2 * half + 1], o[i + 2][2 * half + 1], o[i + 3][2 * half + 1]);
+        }
+    }
+    __syncthreads();
+    constexpr int kLanes = kThreads / kRows;  // 8 threads a row, D / 8 dims each
+    const int row = static_cast<int>(threadIdx.x) / kLanes;
+    const int part = static_cast<int>(threadIdx.x) % kLanes;
+    const int r = row0 + row;
+    if (r < rows) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            top = fmaxf(top, all_ml[w * kRows + row].x);
+        }
+        const float used = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f;
+        float weight[kWarps];
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            weight[w] = ex2_approx(all_ml[w * kRows + row].x - used);
+            sum = fmaf(all_ml[w * kRows + row].y, weight[w], sum);
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int head = r / c.tokens;
+        const int token = r - head * c.tokens;
+        const bool real = token < s.count;  // else padding: zeros (its row saw unmasked tiles, too)
+        const long long out_row =
+            (static_cast<long long>(b) * p.heads + kvh * group + head) * c.tokens + token;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const int four = part * (D / 32) + i;
+            float4 sum4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float4 y = all_o[w * (kRows * D / 4) + place(row, four)];
+                sum4.x = fmaf(y.x, weight[w], sum4.x);
+                sum4.y = fmaf(y.y, weight[w], sum4.y);
+                sum4.z = fmaf(y.z, weight[w], sum4.z);
+                sum4.w = fmaf(y.w, weight[w], sum4.w);
+            }
+            if (record < 0) {
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.o) + out_row * D + four * 4) =
+                    real ? make_uint2(pack2<C::BF16>(sum4.x * inv, sum4.y * inv), pack2<C::BF16>(sum4.z * inv, sum4.w * inv))
+                         : make_uint2(0u, 0u);
+            } else {
+                reinterpret_cast<float4*>(rec.o)[(record * kRows + row) * (D / 4) + four] =
+                    real ? sum4 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+        }
+        if (record >= 0 && part == 0) {
+            rec.ml[record * kRows + row] = real ? make_float2(top, sum) : make_float2(-INFINITY, 0.0f);
+        }
+    }
+    __syncthreads();  // the rings are free for the next item
+}
+
+template <class C>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) cached_kernel(const __grid_constant__ FaCachedParams p,
+                                                                      DeviceStatus* status, Record rec) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int grid = static_cast<int>(gridDim.x);
+    const long long cta = blockIdx.x;
+    const Range range = locate<C>(p, grid, [&](long long per) { return cta * per; });
+    if (range.found < 0) {
+        return;  // past the end of the list
+    }
+    const int row_tiles = (p.heads / p.cache.kv_heads * p.cache.tokens + kRows - 1) / kRows;
+    const int items = p.cache.kv_heads * row_tiles;
+    long long at = cta * range.per;
+    const long long end = min(at + range.per, range.total);
+    int b = range.found;
+    Sequence s = sequence<C>(p, b);
+    long long in_seq = at - range.found_base;
+    int item = static_cast<int>(in_seq / s.tiles);
+    int v = static_cast<int>(in_seq - static_cast<long long>(item) * s.tiles);
+    bool first = true;
+    while (at < end) {
+        const int take = static_cast<int>(min(static_cast<long long>(s.tiles - v), end - at));
+        const bool whole = v == 0 && take == s.tiles;
+        attend<C>(p, status, smem, s, b, item / row_tiles, (item % row_tiles) * kRows, v, v + take, rec,
+                  whole ? -1 : 2 * cta + (first ? 0 : 1));
+        first = false;
+        at += take;
+        v = 0;
+        if (at < end && ++item == items) {
+            item = 0;
+            s = sequence<C>(p, ++b);
+        }
+    }
+}
+
+// Joins the records of the item that was cut at unit k per, k = blockIdx.x + 1, if that is its
+// first cut; row blockIdx.y of it. Warps take the records in turn, then join in order.
+template <class C>
+__global__ void __launch_bounds__(kThreads) cached_join_kernel(const __grid_constant__ FaCachedParams p, Record rec,
+                                                               int grid) {
+    constexpr int D = C::D;
+    __shared__ float2 all_ml[kWarps];
+    __shared__ float all_o[kWarps][D];
+    const long long k = blockIdx.x + 1;
+    const Range range = locate<C>(p, grid, [&](long long per) { return k * per; });
+    if (range.found < 0) {
         return;
     }
-    const int bh = static_cast<int>(row / c.tokens);
-    const int t = static_cast<int>(row - static_cast<long long>(bh) * c.tokens);
-    const int b = bh / p.heads;
-    const int h = bh - b * p.heads;
-    const int kvh = h / (p.heads / c.kv_heads);
-    const int len = c.lengths[b];
-    const int count = c.counts != nullptr ? min(max(c.counts[b], 0), c.tokens) : c.tokens;
-    const int pos = t < count ? len - count + t : -1;
-    float q[PER], acc[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        q[i] = widen<BF16>(static_cast<const uint16_t*>(p.q)[b * p.q_stride[0] + h * p.q_stride[1] +
-                                                             t * p.q_stride[2] + lane * PER + i]);
-        acc[i] = 0.0f;
+    const int group = p.heads / p.cache.kv_heads;
+    const int rows = group * p.cache.tokens;
+    const int row_tiles = (rows + kRows - 1) / kRows;
+    const Sequence s = sequence<C>(p, range.found);
+    const long long item = (k * range.per - range.found_base) / s.tiles;
+    const long long start = range.found_base + item * s.tiles;
+    const int row0 = static_cast<int>(item % row_tiles) * kRows;
+    const int row = static_cast<int>(blockIdx.y);
+    if (start == k * range.per || start / range.per != k - 1 || row0 + row >= rows) {
+        return;
     }
+    const long long c0 = start / range.per;
+    const long long c1 = (start + s.tiles - 1) / range.per;
+    const int warp = static_cast<int>(threadIdx.x) / 32;
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    constexpr int PER = D / 32;
+    cudaGridDependencySynchronize();  // the records are there
     float m = -INFINITY, l = 0.0f;
-    const int first = window_first(pos, p.window);
-    int j = p.sinks > 0 ? 0 : first;
-    for (; j <= pos; ++j) {
-        if (j == p.sinks && j < first) {
-            j = first;
-        }
-        const int page = j / c.page_size;
-        const int id = page < c.max_pages ? c.page_table[b * c.table_stride + page] : -1;
-        if (id < 0 || id >= c.num_pages) {
-            if (lane == 0) {
-                atomicOr(&status->code, kStatusBadPage);
-            }
-            continue;
-        }
-        const int64_t slot = static_cast<int64_t>(j % c.page_size) * D + lane * PER;
-        const int64_t ka = id * c.k_stride[0] + kvh * c.k_stride[1] + slot;
-        const int64_t va = id * c.v_stride[0] + kvh * c.v_stride[1] + slot;
-        float kx[PER], vx[PER];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            if constexpr (E4M3) {
-                const int64_t s = static_cast<int64_t>(id) * c.kv_heads + kvh;
-                kx[i] = unpack_half2(e4m3x2_to_half2(static_cast<const uint8_t*>(c.k)[ka + i])).x * c.k_scale[s];
-                vx[i] = unpack_half2(e4m3x2_to_half2(static_cast<const uint8_t*>(c.v)[va + i])).x * c.v_scale[s];
-            } else {
-                kx[i] = widen<BF16>(static_cast<const uint16_t*>(c.k)[ka + i]);
-                vx[i] = widen<BF16>(static_cast<const uint16_t*>(c.v)[va + i]);
-            }
-        }
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            s = fmaf(q[i], kx[i], s);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            s += __shfl_xor_sync(0xffffffffu, s, o);
-        }
-        s *= p.softmax_scale;
-        const float top = fmaxf(m, s);
-        const float used = top == -INFINITY ? 0.0f : top;
-        const float a = __expf(m - used);
-        const float w = __expf(s - used);
-        m = top;
-        l = fmaf(l, a, w);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            acc[i] = fmaf(acc[i], a, w * vx[i]);
-        }
-    }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    float o[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        static_cast<uint16_t*>(p.o)[row * D + lane * PER + i] =
-            static_cast<uint16_t>(pack2<BF16>(acc[i] * inv, 0.0f) & 0xFFFFu);
+        o[i] = 0.0f;
     }
+#pragma unroll 4
+    for (long long c = c0 + warp; c <= c1; c += kWarps) {
+        // A CTA's first stretch is its record 0; the item starts in c0, as its second unless there.
+        const long long record = (2 * c + (c * range.per >= start ? 0 : 1)) * kRows + row;
+        const float2 ml = rec.ml[record];
+        float y[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            y[i] = rec.o[record * D + i * 32 + lane];
+        }
+        const float now = fmaxf(m, ml.x);
+        const float used = now == -INFINITY ? 0.0f : now;
+        const float a = ex2_approx(m - used);
+        const float w = ex2_approx(ml.x - used);
+        m = now;
+        l = fmaf(ml.y, w, l * a);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            o[i] = fmaf(y[i], w, o[i] * a);
+        }
+    }
+    if (lane == 0) {
+        all_ml[warp] = make_float2(m, l);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        all_o[warp][i * 32 + lane] = o[i];
+    }
+    __syncthreads();
+    const int d = static_cast<int>(threadIdx.x);
+    if (d < D / 2) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            top = fmaxf(top, all_ml[w].x);
+        }
+        const float used = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f, a = 0.0f, b = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float f = ex2_approx(all_ml[w].x - used);
+            sum = fmaf(all_ml[w].y, f, sum);
+            a = fmaf(all_o[w][2 * d], f, a);
+            b = fmaf(all_o[w][2 * d + 1], f, b);
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int kvh = static_cast<int>(item / row_tiles);
+        const int head = (row0 + row) / p.cache.tokens;
+        const int token = row0 + row - head * p.cache.tokens;
+        const long long out_row =
+            (static_cast<long long>(range.found) * p.heads + kvh * group + head) * p.cache.tokens + token;
+        reinterpret_cast<uint32_t*>(p.o)[out_row * (D / 2) + d] = pack2<C::BF16>(a * inv, b * inv);
+    }
+}
+
+// CTAs of a call: what fills the GPU, or fewer where the table's whole capacity is less work.
+int grid_for(const FaCachedParams& p, int sm_count) {
+    const FaCache& c = p.cache;
+    const int row_bytes = c.head_dim * (c.dtype == FA_DTYPE_FLOAT8_E4M3 ? 1 : 2);
+    const int keys = kTileBytes / row_bytes;
+    const long long rows = static_cast<long long>(p.heads / c.kv_heads) * c.tokens;
+    const long long items = static_cast<long long>(c.batch) * c.kv_heads * ((rows + kRows - 1) / kRows);
+    long long shown = static_cast<long long>(c.max_pages) * c.page_size;
+    if (p.window > 0) {
+        shown = std::min<long long>(shown, static_cast<long long>(p.window) + p.sinks + c.tokens + 2 * keys);
+    }
+    const long long tiles = items * (shown / keys + 1);
+    return static_cast<int>(std::max<long long>(1, std::min<long long>(kCtasPerSm * sm_count, (tiles + kMinTiles - 1) / kMinTiles)));
+}
+
+template <class C>
+cudaError_t launch(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
+    cudaError_t err = ensure_smem_limit<cached_kernel<C>>(kSmem);
+    if (err != cudaSuccess) {
+        return err;
+    }
+    const int grid = grid_for(p, sm_count);
+    Record rec;
+    rec.o = static_cast<float*>(workspace);
+    rec.ml = reinterpret_cast<float2*>(rec.o + static_cast<size_t>(grid) * 2 * kRows * C::D);
+    cached_kernel<C><<<grid, kThreads, kSmem, stream>>>(p, status, rec);
+    err = cudaGetLastError();
+    if (err != cudaSuccess || grid == 1) {
+        return err;
+    }
+    const int rows = std::min(kRows, p.heads / p.cache.kv_heads * p.cache.tokens);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(grid - 1), static_cast<unsigned>(rows));
+    config.blockDim = dim3(kThreads);
+    config.stream = stream;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, cached_join_kernel<C>, p, rec, grid);
 }
 
 template <int D>
-cudaError_t launch_dim(const FaCachedParams& p, DeviceStatus* status, cudaStream_t stream) {
-    const long long rows = static_cast<long long>(p.cache.batch) * p.heads * p.cache.tokens;
-    if ((rows + 3) / 4 > 0x7fffffffLL) {
-        return cudaErrorInvalidConfiguration;
-    }
-    const unsigned grid = static_cast<unsigned>((rows + 3) / 4);
+cudaError_t launch_dim(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
     const bool bf16 = p.dtype == FA_DTYPE_BFLOAT16;
     if (p.cache.dtype == FA_DTYPE_FLOAT8_E4M3) {
-        if (bf16) {
-            cached_rows_kernel<D, true, true><<<grid, 128, 0, stream>>>(p, status);
-        } else {
-            cached_rows_kernel<D, false, true><<<grid, 128, 0, stream>>>(p, status);
-        }
-    } else if (bf16) {
-        cached_rows_kernel<D, true, false><<<grid, 128, 0, stream>>>(p, status);
-    } else {
-        cached_rows_kernel<D, false, false><<<grid, 128, 0, stream>>>(p, status);
+        return bf16 ? launch<Cfg<D, true, true>>(p, status, workspace, sm_count, stream)
+                    : launch<Cfg<D, false, true>>(p, status, workspace, sm_count, stream);
     }
-    return cudaGetLastError();
+    return bf16 ? launch<Cfg<D, true, false>>(p, status, workspace, sm_count, stream)
+                : launch<Cfg<D, false, false>>(p, status, workspace, sm_count, stream);
 }
 
 }  // namespace
 
-unsigned long long cached_workspace_bytes(const FaCachedParams&, int) { return 0; }
+unsigned long long cached_workspace_bytes(const FaCachedParams& p, int sm_count) {
+    return static_cast<unsigned long long>(grid_for(p, sm_count)) * 2 * kRows * (p.cache.head_dim + 2) * 4;
+}
 
-cudaError_t launch_cached(const FaCachedParams& p, DeviceStatus* status, void*, int, cudaStream_t stream) {
-    return p.cache.head_dim == 64 ? launch_dim<64>(p, status, stream) : launch_dim<128>(p, status, stream);
+cudaError_t launch_cached(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count,
+                          cudaStream_t stream) {
+    return p.cache.head_dim == 64 ? launch_dim<64>(p, status, workspace, sm_count, stream)
+                                  : launch_dim<128>(p, status, workspace, sm_count, stream);
 }
 
 }  // namespace fa_sm100
