@@ -48,16 +48,17 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;          // query rows of an item: the M of the matrix instruction
-constexpr int kStages = 3;         // key tiles of a warp's ring
+constexpr int kStages = 2;         // key tiles of a warp's ring
 constexpr int kTileBytes = 4096;   // K (or V) of a key tile
 constexpr int kAuxFloats = 16;     // of a stage: 8 K scales, 8 V scales
-constexpr int kCtasPerSm = 2;
+constexpr int kCtasPerSm = 3;
 constexpr int kMinTiles = kWarps;  // least key tiles of a CTA: one for each warp
 constexpr float kMinScale = 8.673617379884035e-19f;  // 2^-60
 constexpr int kSmem = kWarps * kStages * (2 * kTileBytes + kAuxFloats * 4);
 
-template <int D_, bool BF16_, bool E4M3_>
+template <int D_, bool BF16_, bool E4M3_, bool ONE_PAGE_>
 struct Cfg {
+    static constexpr bool ONE_PAGE = ONE_PAGE_;  // a key tile lies within one page
     static constexpr int D = D_;
     static constexpr bool BF16 = BF16_;  // queries and output
     static constexpr bool E4M3 = E4M3_;
@@ -99,23 +100,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
     }
 }
 
-__device__ __forceinline__ uint4 lds128(uint32_t at) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-    return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t at) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
-    return v;
-}
-__device__ __forceinline__ float lds_f(uint32_t at) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
-    return v;
-}
-__device__ __forceinline__ void sts_f(uint32_t at, float v) {
-    asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+// Two e4m3 pairs of a word, widened exactly.
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
 }
 
 // Byte offsets of chunk `c` (16 bytes) of token `r` in a K and in a V tile. The swizzles make the
@@ -240,25 +230,27 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
     const int t = lane % 4;
     const int group = p.heads / c.kv_heads;
     const int rows = group * c.tokens;
-    const uint32_t ring = smem_u32(smem) + warp * kStages * 2 * kTileBytes;
-    const uint32_t aux = smem_u32(smem) + kWarps * kStages * 2 * kTileBytes + warp * kStages * kAuxFloats * 4;
+    uint8_t* ring = smem + warp * kStages * 2 * kTileBytes;
+    float* aux = reinterpret_cast<float*>(smem + kWarps * kStages * 2 * kTileBytes) + warp * kStages * kAuxFloats;
 
-    // Pages of a key tile: `span` tokens each, at most 8 of them.
+    // Pages of a key tile: `spans` of them (at most 8), 2^log2_span tokens each.
     const int log2_page = 31 - __clz(c.page_size);
-    const int log2_span = min(log2_page, 31 - __clz(C::kKeys));
+    const int log2_span = C::ONE_PAGE ? 31 - __clz(C::kKeys) : log2_page;
     const int spans = C::kKeys >> log2_span;
 
     auto tile_key = [&](int v) { return (v < s.sink_tiles ? v : v - s.sink_tiles + s.first_tile) * C::kKeys; };
     auto shown = [&](int key) { return key <= s.last && (key >= s.first || key < p.sinks); };
-    // Lane i < spans: the page of the tile's i-th span (-1: outside the pool, or hidden).
+    // The page of the tile (ONE_PAGE: in every lane) or of its span number `lane`; -1 for one that is
+    // outside the pool or hidden.
+    const int32_t* table = c.page_table + b * c.table_stride;
     auto fetch = [&](int v) {
         int id = -1;
-        if (v < v1 && lane < spans) {
-            const int key = tile_key(v) + (lane << log2_span);
+        if (v < v1 && (C::ONE_PAGE || lane < spans)) {
+            const int key = tile_key(v) + (C::ONE_PAGE ? 0 : lane << log2_span);
             const int end = key + (1 << log2_span) - 1;
             if (key <= s.last && (end >= s.first || key < p.sinks)) {
                 const int page = key >> log2_page;
-                id = page < c.max_pages ? __ldg(c.page_table + b * c.table_stride + page) : -1;
+                id = page < c.max_pages ? __ldg(table + page) : -1;
                 if (id < 0 || id >= c.num_pages) {
                     id = -1;
                     atomicOr(&status->code, kStatusBadPage);
@@ -268,34 +260,58 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
         return id;
     };
     const int chunk = lane % C::kChunks;
+    constexpr int kStep = 32 / C::kChunks;  // tokens of one copy of the warp
+    const int r0 = lane / C::kChunks;
     const uint8_t* kbase = static_cast<const uint8_t*>(c.k) + kvh * c.k_stride[1] * C::kElem + chunk * 16;
     const uint8_t* vbase = static_cast<const uint8_t*>(c.v) + kvh * c.v_stride[1] * C::kElem + chunk * 16;
     const int64_t kpage = c.k_stride[0] * C::kElem;
     const int64_t vpage = c.v_stride[0] * C::kElem;
+    float next_ks = -1.0f, next_vs = 1.0f;  // ONE_PAGE: scales of the tile last asked for (K: below 0, hidden)
     auto issue = [&](int v, int stage, int ids) {
         if (v < v1) {
             const int key0 = tile_key(v);
-            const uint32_t ks = ring + stage * 2 * kTileBytes;
+            const uint32_t ks = smem_u32(ring) + stage * 2 * kTileBytes;
             const uint32_t vs = ks + kTileBytes;
+            const int last = key0 + C::kKeys - 1;
+            if (C::ONE_PAGE && ids >= 0 && last <= s.last && (key0 >= s.first || last < p.sinks)) {
+                // The usual tile: all of it shown, contiguous in its page.
+                const int64_t slot = static_cast<int64_t>((key0 & (c.page_size - 1)) + r0) * C::kRowBytes;
+                const uint8_t* ksrc = kbase + ids * kpage + slot;
+                const uint8_t* vsrc = vbase + ids * vpage + slot;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = i * (32 / C::kChunks) + lane / C::kChunks;
-                const int id = __shfl_sync(0xffffffffu, ids, r >> log2_span);
-                const int key = key0 + r;
-                const bool real = id >= 0 && shown(key);
-                const int64_t slot = static_cast<int64_t>(key & (c.page_size - 1)) * C::kRowBytes;
-                cp_async16(ks + k_offset<C>(r, chunk), real ? kbase + id * kpage + slot : kbase, real);
-                cp_async16(vs + v_offset<C>(r, chunk), real ? vbase + id * vpage + slot : vbase, real);
+                for (int i = 0; i < 8; ++i) {
+                    cp_async16(ks + k_offset<C>(i * kStep + r0, chunk), ksrc + i * kStep * C::kRowBytes, true);
+                    cp_async16(vs + v_offset<C>(i * kStep + r0, chunk), vsrc + i * kStep * C::kRowBytes, true);
+                }
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < 8; ++i) {
+                    const int r = i * kStep + r0;
+                    const int id = C::ONE_PAGE ? ids : __shfl_sync(0xffffffffu, ids, r >> log2_span);
+                    const int key = key0 + r;
+                    const bool real = id >= 0 && shown(key);
+                    const int64_t slot = static_cast<int64_t>(key & (c.page_size - 1)) * C::kRowBytes;
+                    cp_async16(ks + k_offset<C>(r, chunk), real ? kbase + id * kpage + slot : kbase, real);
+                    cp_async16(vs + v_offset<C>(r, chunk), real ? vbase + id * vpage + slot : vbase, real);
+                }
             }
-            if (lane < spans) {
-                const uint32_t at = aux + stage * kAuxFloats * 4 + lane * 4;
+            if constexpr (C::ONE_PAGE) {
+                next_ks = ids >= 0 ? 1.0f : -1.0f;
+                next_vs = 1.0f;
                 if (C::E4M3 && ids >= 0) {
                     const int64_t n = static_cast<int64_t>(ids) * c.kv_heads + kvh;
-                    cp_async4(at, c.k_scale + n);
-                    cp_async4(at + 32, c.v_scale + n);
+                    next_ks = __ldg(c.k_scale + n);
+                    next_vs = __ldg(c.v_scale + n);
+                }
+            } else if (lane < spans) {
+                float* at = aux + stage * kAuxFloats + lane;
+                if (C::E4M3 && ids >= 0) {
+                    const int64_t n = static_cast<int64_t>(ids) * c.kv_heads + kvh;
+                    cp_async4(smem_u32(at), c.k_scale + n);
+                    cp_async4(smem_u32(at + 8), c.v_scale + n);
                 } else {
-                    sts_f(at, ids >= 0 ? 1.0f : -1.0f);  // below 0: the span is hidden
-                    sts_f(at + 32, 1.0f);
+                    at[0] = ids >= 0 ? 1.0f : -1.0f;
+                    at[8] = 1.0f;
                 }
             }
         }
@@ -305,9 +321,10 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
     // The warp's first tiles are on their way while the queries are read.
     int next = v0 + warp;
     int ids = fetch(next);
-    for (int i = 0; i < kStages - 1; ++i) {
+    static_assert(kStages == 2, "the scales of one tile ahead are kept");
+    {
         const int ahead = fetch(next + kWarps);
-        issue(next, i, ids);
+        issue(next, 0, ids);
         ids = ahead;
         next += kWarps;
     }
@@ -369,15 +386,17 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
     for (int v = v0 + warp; v < v1; v += kWarps) {
         cp_wait<kStages - 2>();
         __syncwarp();  // the tile is there, and every lane has left the stage that is refilled next
+        const float page_ks = next_ks;
+        const float page_vs = next_vs;
         {
             const int ahead = fetch(next + kWarps);
-            issue(next, stage == 0 ? kStages - 1 : stage - 1, ids);
+            issue(next, stage ^ 1, ids);
             ids = ahead;
             next += kWarps;
         }
-        const uint32_t ks = ring + stage * 2 * kTileBytes;
-        const uint32_t vs = ks + kTileBytes;
-        const uint32_t sc = aux + stage * kAuxFloats * 4;
+        const uint8_t* ks = ring + stage * 2 * kTileBytes;
+        const uint8_t* vs = ks + kTileBytes;
+        const float* sc = aux + stage * kAuxFloats;
         const int key0 = tile_key(v);
 
         // Scores: keys 8 n + g of the tile, lane t's dims.
@@ -387,12 +406,14 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
             x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
 #pragma unroll
             for (int cc = 0; cc < C::kChunks / 4; ++cc) {
-                const uint4 w4 = lds128(ks + k_offset<C>(8 * n + g, t + 4 * cc));
+                const uint4 w4 = *reinterpret_cast<const uint4*>(ks + k_offset<C>(8 * n + g, t + 4 * cc));
                 const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
                 if constexpr (C::E4M3) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        mma16816<false>(x[n], q[4 * cc + i], e4m3x2_to_half2(w[i]), e4m3x2_to_half2(w[i] >> 16));
+                        uint32_t lo, hi;
+                        widen4(w[i], lo, hi);
+                        mma16816<false>(x[n], q[4 * cc + i], lo, hi);
                     }
                 } else {
                     mma16816<C::kMmaBf16>(x[n], q[2 * cc], w[0], w[1]);
@@ -411,14 +432,14 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
 #pragma unroll
         for (int n = 0; n < C::kNTiles; ++n) {
             const int span = (8 * n) >> log2_span;
-            const float kscale = lds_f(sc + span * 4);
+            const float kscale = C::ONE_PAGE ? page_ks : sc[span];
             float lv = kscale < 0.0f ? -INFINITY : 0.0f;
             inv_vs[n] = 1.0f;
             tile_shrink[n] = 1.0f;
             if constexpr (C::E4M3) {
-                const float vscale = lds_f(sc + 32 + span * 4);
+                const float vscale = C::ONE_PAGE ? page_vs : sc[8 + span];
                 const float used = fmaxf(vscale, kMinScale);
-                inv_vs[n] = __frcp_rn(used);
+                inv_vs[n] = __fdividef(1.0f, used);
                 lv += __log2f(used);
                 tile_shrink[n] = vscale >= kMinScale ? 1.0f : vscale * inv_vs[n];
                 shrink = fminf(shrink, tile_shrink[n]);
@@ -502,11 +523,11 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
                 for (int i = 0; i < 4; ++i) {
                     const int key = r + (i & 1) + 8 * (i >> 1);
                     if constexpr (C::kNarrow) {
-                        const uint2 y = lds64(vs + v_offset<C>(key, g >> 1) + (g & 1) * 8);
+                        const uint2 y = *reinterpret_cast<const uint2*>(vs + v_offset<C>(key, g >> 1) + (g & 1) * 8);
                         w[i][0] = y.x;
                         w[i][1] = y.y;
                     } else {
-                        const uint4 y = lds128(vs + v_offset<C>(key, g));
+                        const uint4 y = *reinterpret_cast<const uint4*>(vs + v_offset<C>(key, g));
                         w[i][0] = y.x;
                         w[i][1] = y.y;
                         w[i][2] = y.z;
@@ -519,10 +540,15 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
                     const uint32_t hi0 = __byte_perm(w[0][j], w[1][j], 0x7362);
                     const uint32_t lo1 = __byte_perm(w[2][j], w[3][j], 0x5140);
                     const uint32_t hi1 = __byte_perm(w[2][j], w[3][j], 0x7362);
-                    mma16816<false>(o[4 * j], a, e4m3x2_to_half2(lo0), e4m3x2_to_half2(lo1));
-                    mma16816<false>(o[4 * j + 1], a, e4m3x2_to_half2(lo0 >> 16), e4m3x2_to_half2(lo1 >> 16));
-                    mma16816<false>(o[4 * j + 2], a, e4m3x2_to_half2(hi0), e4m3x2_to_half2(hi1));
-                    mma16816<false>(o[4 * j + 3], a, e4m3x2_to_half2(hi0 >> 16), e4m3x2_to_half2(hi1 >> 16));
+                    uint32_t b0[4], b1[4];
+                    widen4(lo0, b0[0], b0[1]);
+                    widen4(hi0, b0[2], b0[3]);
+                    widen4(lo1, b1[0], b1[1]);
+                    widen4(hi1, b1[2], b1[3]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        mma16816<false>(o[4 * j + i], a, b0[i], b1[i]);
+                    }
                 }
             } else {
 #pragma unroll
@@ -530,7 +556,7 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
                     uint4 y[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        y[i] = lds128(vs + v_offset<C>(r + (i & 1) + 8 * (i >> 1), g + 8 * cc));
+                        y[i] = *reinterpret_cast<const uint4*>(vs + v_offset<C>(r + (i & 1) + 8 * (i >> 1), g + 8 * cc));
                     }
                     const uint32_t w[4][4] = {{y[0].x, y[0].y, y[0].z, y[0].w},
                                               {y[1].x, y[1].y, y[1].z, y[1].w},
@@ -546,7 +572,7 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
                 }
             }
         }
-        stage = stage + 1 == kStages ? 0 : stage + 1;
+        stage ^= 1;
     }
     cp_wait<0>();
     __syncthreads();
@@ -757,11 +783,12 @@ __global__ void __launch_bounds__(kThreads) cached_join_kernel(const __grid_cons
     }
 }
 
+int tile_keys(const FaCache& c) { return kTileBytes / (c.head_dim * (c.dtype == FA_DTYPE_FLOAT8_E4M3 ? 1 : 2)); }
+
 // CTAs of a call: what fills the GPU, or fewer where the table's whole capacity is less work.
 int grid_for(const FaCachedParams& p, int sm_count) {
     const FaCache& c = p.cache;
-    const int row_bytes = c.head_dim * (c.dtype == FA_DTYPE_FLOAT8_E4M3 ? 1 : 2);
-    const int keys = kTileBytes / row_bytes;
+    const int keys = tile_keys(c);
     const long long rows = static_cast<long long>(p.heads / c.kv_heads) * c.tokens;
     const long long items = static_cast<long long>(c.batch) * c.kv_heads * ((rows + kRows - 1) / kRows);
     long long shown = static_cast<long long>(c.max_pages) * c.page_size;
@@ -800,15 +827,23 @@ cudaError_t launch(const FaCachedParams& p, DeviceStatus* status, void* workspac
     return cudaLaunchKernelEx(&config, cached_join_kernel<C>, p, rec, grid);
 }
 
-template <int D>
-cudaError_t launch_dim(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
+template <int D, bool ONE_PAGE>
+cudaError_t launch_pages(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count,
+                         cudaStream_t stream) {
     const bool bf16 = p.dtype == FA_DTYPE_BFLOAT16;
     if (p.cache.dtype == FA_DTYPE_FLOAT8_E4M3) {
-        return bf16 ? launch<Cfg<D, true, true>>(p, status, workspace, sm_count, stream)
-                    : launch<Cfg<D, false, true>>(p, status, workspace, sm_count, stream);
+        return bf16 ? launch<Cfg<D, true, true, ONE_PAGE>>(p, status, workspace, sm_count, stream)
+                    : launch<Cfg<D, false, true, ONE_PAGE>>(p, status, workspace, sm_count, stream);
     }
-    return bf16 ? launch<Cfg<D, true, false>>(p, status, workspace, sm_count, stream)
-                : launch<Cfg<D, false, false>>(p, status, workspace, sm_count, stream);
+    return bf16 ? launch<Cfg<D, true, false, ONE_PAGE>>(p, status, workspace, sm_count, stream)
+                : launch<Cfg<D, false, false, ONE_PAGE>>(p, status, workspace, sm_count, stream);
+}
+
+template <int D>
+cudaError_t launch_dim(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count,
+                       cudaStream_t stream) {
+    return p.cache.page_size >= tile_keys(p.cache) ? launch_pages<D, true>(p, status, workspace, sm_count, stream)
+                                                   : launch_pages<D, false>(p, status, workspace, sm_count, stream);
 }
 
 }  // namespace
