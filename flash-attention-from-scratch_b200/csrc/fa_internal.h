@@ -44,6 +44,17 @@ struct FastDiv {
     }
 };
 
+// Window build of the kernel (FwdCfg::WIN): query row i is at key position i + shift and sees
+// position j <= i + shift with i + shift - j < window or j < sinks.
+struct WindowArgs {
+    int shift;          // k_len - q_len
+    int window;         // 2^30 and more: none
+    int sinks;
+    FastDiv div_heads;  // query heads
+    FastDiv div_group;  // query heads per key/value head
+    float* lse;         // [batch * heads][q_len], or NULL
+};
+
 struct FwdArgs {
     int seqlen;           // N (queries == keys)
     int num_bh;           // B * H
@@ -74,6 +85,7 @@ struct FwdArgs {
     int num_items;        // work items, set by the launcher
     void* o;              // output [num_bh][seqlen][D] fp16 / bf16, set by the launcher
     float out_scale;      // fp8: O is multiplied by V's descale in the epilogue (else unused)
+    WindowArgs win;       // window build only
 };
 
 // Split-KV workspace bytes for a problem (16-byte aligned sections).

@@ -60,6 +60,7 @@
 #include "fa_internal.h"
 #include "sm100_ptx.cuh"
 #include "softmax_common.cuh"
+#include "stream_internal.h"
 #include "tma_host.h"
 
 // Software-exp2 share (how many of every 8 column pairs of a 128-key tile take exp2_poly2
@@ -124,8 +125,13 @@ constexpr int kBoxBytes = 128 * 128; // one TMA box: 128 rows x 128 B (64 fp16 o
 constexpr int kPersistentMaxN = 2048; // persistent grid (one CTA per SM walks the items) up to this N
 constexpr int kPersistentMaxNFull = 8192;  // ... and up to this N without the causal mask
 
-template <int D_, bool CAUSAL_, int VARIANT_, bool BF16_ = false, bool FP8_ = false>
+template <int D_, bool CAUSAL_, int VARIANT_, bool BF16_ = false, bool FP8_ = false, bool WIN_ = false>
 struct FwdCfg {
+    // Causal sliding window with sinks, grouped heads, q_len != k_len, strided tensors (4-D tensor
+    // maps) and the row's log-sum-exp: an item's key tiles are the sinks' and the union of its
+    // query tiles' windows, and a query tile skips those it does not see.
+    static constexpr bool WIN = WIN_;
+    static_assert(!WIN_ || (CAUSAL_ && VARIANT_ == kVariantOpt && !FP8_), "the window build is causal, 16-bit, opt");
     static constexpr int D = D_;
     static constexpr bool CAUSAL = CAUSAL_;
     static constexpr int VARIANT = VARIANT_;
@@ -332,6 +338,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
     };
     struct Item {
         int bh;
+        int z[2], w[2];  // WIN: head and batch coordinates of q (and o), of k and v
+        int sink_tiles, first_tile;  // WIN: the key tiles [0, sink_tiles), [first_tile, ..] make the list
+        int tile_lo[NQ], tile_hi[NQ];  // WIN: key tiles of query tile t's windows
         int q_row0;
         int kv0;       // first key tile of the item's key range
         int n_kv[NQ];  // key tiles query tile t processes, from kv0
@@ -355,6 +364,34 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             nsplit = args.num_splits;
         }
         int m_block;
+        if constexpr (Cfg::WIN) {
+            // Items cost about the same: heads in order, row blocks in order.
+            it.bh = args.div_nb.div(lin);
+            m_block = lin - it.bh * nb;
+            it.q_row0 = m_block * NQ * kBM;
+            it.w[0] = it.w[1] = args.win.div_heads.div(it.bh);
+            it.z[0] = it.bh - it.w[0] * static_cast<int>(args.win.div_heads.d);
+            it.z[1] = args.win.div_group.div(it.z[0]);
+            it.kv0 = 0;
+            it.split = false;
+            it.rec0 = 0;
+            int hi = 0;
+#pragma unroll
+            for (int t = 0; t < NQ; ++t) {
+                // A tile whose rows see nothing still takes key tile 0, all masked: O = 0 is stored.
+                const int q0 = it.q_row0 + t * kBM;
+                const int lo_pos = max(q0 + args.win.shift, 0);
+                const int hi_pos = max(min(q0 + kBM, n) - 1 + args.win.shift, 0);
+                it.tile_lo[t] = max(lo_pos - args.win.window + 1, 0) / kBN;
+                it.tile_hi[t] = hi_pos / kBN;
+                it.n_kv[t] = q0 < n ? 1 : 0;  // present
+                hi = q0 < n ? it.tile_hi[t] : hi;
+            }
+            it.first_tile = it.tile_lo[0];
+            it.sink_tiles = min((args.win.sinks + kBN - 1) / kBN, it.first_tile);
+            it.n_max = it.sink_tiles + hi - it.first_tile + 1;
+            return;
+        }
         if constexpr (Cfg::CAUSAL) {
             // A causal row block covers more key tiles the later its rows are. Items run in
             // index order, so the index is mapped to (row block, head) longest first across a
@@ -400,6 +437,18 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                           ? (static_cast<long long>(z) * args.tail_blocks + p) * (NQ * kBM)
                           : (static_cast<long long>(z) * args.num_bh + it.bh) * args.rows_pad + it.q_row0;
         }
+    };
+
+    // WIN: the key tile at place j of an item's list, whether query tile t takes it, and t's last place.
+    auto list_tile = [&](const Item& it, int j) { return j < it.sink_tiles ? j : j - it.sink_tiles + it.first_tile; };
+    auto takes = [&](const Item& it, int t, int j) {
+        const int lo = t == 0 ? it.tile_lo[0] : it.tile_lo[NQ - 1];
+        const int hi = t == 0 ? it.tile_hi[0] : it.tile_hi[NQ - 1];
+        const int k = list_tile(it, j);
+        return (t == 0 ? it.n_kv[0] : it.n_kv[NQ - 1]) > 0 && k <= hi && (k >= lo || k * kBN < args.win.sinks);
+    };
+    auto last_place = [&](const Item& it, int t) {
+        return (t == 0 ? it.tile_hi[0] : it.tile_hi[NQ - 1]) - it.first_tile + it.sink_tiles;
     };
 
     const WaitCtx wctx{&sb.abort, &args.status->code, &args.status->epoch_aborted, args.epoch};
@@ -514,12 +563,21 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             // Only what the key-tile loop needs stays live through it; the epilogue decodes the
             // item again for its head and key range.
             int q0, nt, kv0;
+            int places = 0, sink_tiles = 0, first_tile = 0, tile_lo = 0, tile_hi = 0;  // WIN
             {
                 Item it;
                 decode(idx, it);
                 q0 = it.q_row0 + t * kBM;
                 nt = (t == 0) ? it.n_kv[0] : it.n_kv[NQ - 1];  // a select keeps `it` in registers
                 kv0 = it.kv0;
+                if constexpr (Cfg::WIN) {
+                    places = nt > 0 ? it.n_max : 0;
+                    sink_tiles = it.sink_tiles;
+                    first_tile = it.first_tile;
+                    tile_lo = t == 0 ? it.tile_lo[0] : it.tile_lo[NQ - 1];
+                    tile_hi = t == 0 ? it.tile_hi[0] : it.tile_hi[NQ - 1];
+                    nt = 0;  // counted below
+                }
             }
             const int grow = q0 + row;  // global query row
             // Last key index this row may see: keys > lim are masked (ragged N, causal).
@@ -529,7 +587,16 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             float row_sum = 0.0f;       // running sum of this thread's fp16-rounded probabilities
             float alpha_prev = 1.0f;    // two S buffers: the rescale of the fold still pending
 
-            for (int j = 0; j < nt; ++j) {
+            for (int place = 0; place < (Cfg::WIN ? places : nt); ++place) {
+                int j = place;
+                int key_tile = kv0 + j;
+                if constexpr (Cfg::WIN) {
+                    key_tile = place < sink_tiles ? place : place - sink_tiles + first_tile;
+                    if (key_tile > tile_hi || (key_tile < tile_lo && key_tile * kBN >= args.win.sinks)) {
+                        continue;
+                    }
+                    j = nt++;
+                }
                 const int gj = g0 + j;  // running index of S_t(j), P_t(j) and P.V_t(j)
                 // Two S buffers (kSBufs): S(j) in buffer gj & 1, whose barrier completes every
                 // other S.
@@ -566,14 +633,29 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                     }
                 }
 
-                const int kbase = (kv0 + j) * kBN;
+                const int kbase = key_tile * kBN;
                 // Only the last key tile can hold keys >= N, and for causal rows only the
                 // diagonal tile (key tile q0 / 128) holds keys after the row: every other tile
                 // is unmasked.
-                const bool masked = (kbase + kBN > n) || (Cfg::CAUSAL && kbase == q0);
+                // WIN: a tile that reaches past the first row's position or before the last row's window.
+                const bool masked = Cfg::WIN ? (kbase + kBN - 1 > q0 + args.win.shift ||
+                                                (q0 + kBM - 1 + args.win.shift - kbase >= args.win.window &&
+                                                 kbase + kBN > args.win.sinks))
+                                             : ((kbase + kBN > n) || (Cfg::CAUSAL && kbase == q0));
                 float tile_max;
                 float mul;
-                if (masked) {
+                if (Cfg::WIN && masked) {
+                    // Columns [from, to] of this row's window, and those before `sink`.
+                    const int to = grow + args.win.shift - kbase;
+                    const int from = to - args.win.window + 1;
+                    const int sink = min(args.win.sinks - kbase, to + 1);
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        sr[c] = f2u(((c >= from && c <= to) || c < sink) ? u2f(sr[c]) * scale_log2 : -INFINITY);
+                    }
+                    tile_max = row_extreme<true, NC>(sr);
+                    mul = 1.0f;
+                } else if (masked) {
                     // Scale first, then mask, so masked scores are -inf whatever the scale's sign.
                     const int cmax = lim - kbase;
 #pragma unroll
@@ -763,6 +845,14 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             }
             Item it;
             decode(idx, it);
+            if constexpr (Cfg::WIN) {
+                // A row that sees nothing keeps row_max = -inf (the software 2^x may leave a
+                // vanishing row_sum there).
+                if (args.win.lse != nullptr && ok && grow < n) {
+                    args.win.lse[static_cast<long long>(it.bh) * n + grow] =
+                        row_max == -INFINITY ? -INFINITY : (row_max + __log2f(row_sum)) * 0.6931471805599453f;
+                }
+            }
             if (it.split) {
                 // Split-KV: the row's unnormalised O over this item's key range and its (m, l) go
                 // to the workspace; a range with no keys for this tile records l = 0, which the
@@ -794,6 +884,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 }
             } else if (tma_store_o && ok && nt > 0) {
                 float inv_sum = (row_sum > 0.0f) ? (1.0f / row_sum) : 0.0f;
+                if constexpr (Cfg::WIN) {
+                    inv_sum = row_max == -INFINITY ? 0.0f : inv_sum;
+                }
                 if constexpr (Cfg::FP8) {
                     inv_sum *= args.out_scale;  // V's descale
                 }
@@ -830,7 +923,11 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                     if (mbar_wait(smem_u32(&sb.epi[t]), 0, wctx, kStatusTimeoutEpilogue)) {
 #pragma unroll
                         for (int b = 0; b < Cfg::kOutBoxes; ++b) {
-                            tma_store_3d(&tm_o, smem_u32(out) + b * kBoxBytes, b * 64, q0, it.bh);
+                            if constexpr (Cfg::WIN) {
+                                tma_store_4d(&tm_o, smem_u32(out) + b * kBoxBytes, b * 64, q0, it.z[0], it.w[0]);
+                            } else {
+                                tma_store_3d(&tm_o, smem_u32(out) + b * kBoxBytes, b * 64, q0, it.bh);
+                            }
                         }
                         tma_store_commit();
                         tma_store_wait_read();
@@ -851,6 +948,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 uint8_t* out = smem + Cfg::kSmemStage;
                 if (turn && nt > 0) {
                     float inv_sum = (row_sum > 0.0f) ? (1.0f / row_sum) : 0.0f;
+                    if constexpr (Cfg::WIN) {
+                        inv_sum = row_max == -INFINITY ? 0.0f : inv_sum;
+                    }
                     if constexpr (Cfg::FP8) {
                         inv_sum *= args.out_scale;
                     }
@@ -887,7 +987,11 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                         nt > 0) {
 #pragma unroll
                         for (int b = 0; b < Cfg::kOutBoxes; ++b) {
-                            tma_store_3d(&tm_o, smem_u32(out) + b * kBoxBytes, b * 64, q0, it.bh);
+                            if constexpr (Cfg::WIN) {
+                                tma_store_4d(&tm_o, smem_u32(out) + b * kBoxBytes, b * 64, q0, it.z[0], it.w[0]);
+                            } else {
+                                tma_store_3d(&tm_o, smem_u32(out) + b * kBoxBytes, b * 64, q0, it.bh);
+                            }
                         }
                         tma_store_commit();
                         tma_store_wait_read();
@@ -936,8 +1040,13 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                             mbar_arrive_expect_tx(bar, Cfg::kTileBytes);
 #pragma unroll
                             for (int b = 0; b < Cfg::kBoxes; ++b) {
-                                tma_load_3d(smem_base + Cfg::kSmemQ + t * Cfg::kQTileBytes + b * kBoxBytes,
-                                            &tm_q, bar, b * Cfg::kBoxElems, it.q_row0 + t * kBM, it.bh);
+                                const uint32_t dst = smem_base + Cfg::kSmemQ + t * Cfg::kQTileBytes + b * kBoxBytes;
+                                if constexpr (Cfg::WIN) {
+                                    tma_load_4d(dst, &tm_q, bar, b * Cfg::kBoxElems, it.q_row0 + t * kBM, it.z[0],
+                                                it.w[0]);
+                                } else {
+                                    tma_load_3d(dst, &tm_q, bar, b * Cfg::kBoxElems, it.q_row0 + t * kBM, it.bh);
+                                }
                             }
                             ++q_loads[t];
                         }
@@ -963,8 +1072,13 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                         } else {
 #pragma unroll
                             for (int b = 0; b < Cfg::kBoxes; ++b) {
-                                tma_load_3d(smem_base + Cfg::kSmemKV + stage * Cfg::kTileBytes + b * kBoxBytes,
-                                            map, bar, b * Cfg::kBoxElems, (it.kv0 + j) * kBN, it.bh);
+                                const uint32_t dst = smem_base + Cfg::kSmemKV + stage * Cfg::kTileBytes + b * kBoxBytes;
+                                if constexpr (Cfg::WIN) {
+                                    tma_load_4d(dst, map, bar, b * Cfg::kBoxElems, list_tile(it, j) * kBN, it.z[1],
+                                                it.w[1]);
+                                } else {
+                                    tma_load_3d(dst, map, bar, b * Cfg::kBoxElems, (it.kv0 + j) * kBN, it.bh);
+                                }
                             }
                         }
                         loaded[stage] = true;
@@ -1022,6 +1136,10 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 decode(idx, it);
                 const int n_t = (t == 0) ? it.n_kv[0] : it.n_kv[NQ - 1];
                 const int n_max = it.n_max;
+                // Whether tile t takes place j of the item's key tiles, and its last place.
+                auto has = [&](int j) { return Cfg::WIN ? takes(it, t, j) : j < n_t; };
+                const int last_j = Cfg::WIN ? last_place(it, t) : n_t - 1;
+                bool pv_first = true;
                 if (n_t > 0) {
                     ok = mbar_wait(smem_u32(&sb.q_full[t]), q_uses & 1, wctx, kStatusTimeoutMma);
                     ++q_uses;
@@ -1030,7 +1148,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                     const int k_slot = ring++;
                     ok = mbar_wait(smem_u32(&sb.kv_full[k_slot % STAGES]), (k_slot / STAGES) & 1, wctx,
                                    kStatusTimeoutMma);
-                    if (ok && n_t > 0) {
+                    if (ok && has(0)) {
                         if constexpr (Cfg::SEP_P) {
                             // The softmax has the previous item's last S_t in registers.
                             if (s_cnt > 0) {
@@ -1042,7 +1160,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                             tc_fence_after();
                             issue_s_mma<Cfg>(s_addr, qd, kd0 + stage_off(k_slot % STAGES));
                             umma_commit(smem_u32(&sb.s_full[t]));
-                            if (n_t == 1) {
+                            if (last_j == 0) {
                                 umma_commit(smem_u32(&sb.q_empty[t]));  // Q_t read for the last time
                             }
                             ++s_cnt;
@@ -1058,14 +1176,15 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                     const bool has_next = (j + 1 < n_max);
                     const int k_slot = has_next ? ring++ : 0;
                     const int ks = k_slot % STAGES;
-                    const bool active = (j < n_t);
-                    const bool next_s = (j + 1 < n_t);
+                    const bool active = has(j);
+                    const bool next_s = has_next && has(j + 1);
                     bool k_ready = false;
-                    if (active) {
+                    if (active || (Cfg::WIN && next_s)) {
                         if constexpr (Cfg::SEP_P) {
                             // S_t(j+1) as soon as the softmax has S_t(j) in registers.
                             if (next_s) {
-                                ok = mbar_wait(smem_u32(&sb.s_free[t]), (s_cnt - 1) & 1, wctx, kStatusTimeoutMma);
+                                ok = s_cnt == 0 ||
+                                     mbar_wait(smem_u32(&sb.s_free[t]), (s_cnt - 1) & 1, wctx, kStatusTimeoutMma);
                                 ok = ok && mbar_wait(smem_u32(&sb.kv_full[ks]), (k_slot / STAGES) & 1, wctx,
                                                      kStatusTimeoutMma);
                                 if (!ok) {
@@ -1075,26 +1194,31 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                                 tc_fence_after();
                                 issue_s_mma<Cfg>(s_addr, qd, kd0 + stage_off(ks));
                                 umma_commit(smem_u32(&sb.s_full[t]));
-                                if (j + 2 == n_t) {
+                                if (j + 1 == last_j) {
                                     umma_commit(smem_u32(&sb.q_empty[t]));
                                 }
                                 ++s_cnt;
                             }
                         }
-                        ok = mbar_wait(smem_u32(&sb.p_full[t]), pv_cnt & 1, wctx, kStatusTimeoutMma);
+                        if (active) {
+                            ok = mbar_wait(smem_u32(&sb.p_full[t]), pv_cnt & 1, wctx, kStatusTimeoutMma);
+                        }
                         ok = ok && mbar_wait(smem_u32(&sb.kv_full[vs]), (v_slot / STAGES) & 1, wctx,
                                              kStatusTimeoutMma);
                         if (!ok) {
                             break;
                         }
                         tc_fence_after();
-                        if constexpr (Cfg::ACC16) {
-                            issue_pv_mma_f16<Cfg>(tmem + Cfg::tmem_t(t), p_addr, vd0 + stage_off(vs));
-                        } else {
-                            issue_pv_mma_f32<Cfg>(o_addr, p_addr, vd0 + stage_off(vs), j == 0);
+                        if (active) {
+                            if constexpr (Cfg::ACC16) {
+                                issue_pv_mma_f16<Cfg>(tmem + Cfg::tmem_t(t), p_addr, vd0 + stage_off(vs));
+                            } else {
+                                issue_pv_mma_f32<Cfg>(o_addr, p_addr, vd0 + stage_off(vs), pv_first);
+                            }
+                            umma_commit(smem_u32(&sb.o_done[t]));
+                            ++pv_cnt;
+                            pv_first = false;
                         }
-                        umma_commit(smem_u32(&sb.o_done[t]));
-                        ++pv_cnt;
                         if constexpr (!Cfg::SEP_P) {
                             // S_t(j+1) reuses the columns P_t(j) was read from by the MMAs above
                             // (tcgen05.mma operations of one thread execute in issue order).
@@ -1108,7 +1232,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                                 tc_fence_after();
                                 issue_s_mma<Cfg>(s_addr, qd, kd0 + stage_off(ks));
                                 umma_commit(smem_u32(&sb.s_full[t]));
-                                if (j + 2 == n_t) {
+                                if (j + 1 == last_j) {
                                     umma_commit(smem_u32(&sb.q_empty[t]));
                                 }
                                 ++s_cnt;
@@ -1268,8 +1392,13 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 Item it;
                 decode(idx, it);
                 const int n_max = it.n_max;
+                // Whether tile t takes place j of the item's key tiles, and its last place.
+                auto has = [&](int t, int j) { return Cfg::WIN ? takes(it, t, j) : j < it.n_kv[t]; };
+                auto last_j = [&](int t) { return Cfg::WIN ? last_place(it, t) : it.n_kv[t] - 1; };
+                bool pv_first[NQ];
 #pragma unroll
                 for (int t = 0; t < NQ; ++t) {
+                    pv_first[t] = true;
                     if (ok && it.n_kv[t] > 0) {
                         ok = mbar_wait(smem_u32(&sb.q_full[t]), q_uses[t] & 1, wctx, kStatusTimeoutMma);
                         ++q_uses[t];
@@ -1283,8 +1412,8 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                                    kStatusTimeoutMma);
 #pragma unroll
                     for (int t = 0; t < NQ; ++t) {
-                        if (ok && it.n_kv[t] > 0) {
-                            ok = issue_s(t, k_slot % STAGES, it.n_kv[t] == 1);
+                        if (ok && has(t, 0)) {
+                            ok = issue_s(t, k_slot % STAGES, last_j(t) == 0);
                         }
                     }
                     if (ok) {
@@ -1301,10 +1430,11 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                     bool v_ready = false;
 #pragma unroll
                     for (int t = 0; t < NQ; ++t) {
-                        if (!ok || j >= it.n_kv[t]) {
+                        const bool active = has(t, j);
+                        const bool next_s = has_next && has(t, j + 1);
+                        if (!ok || !(active || (Cfg::WIN && next_s))) {
                             continue;
                         }
-                        const bool next_s = (j + 1 < it.n_kv[t]);
                         const uint32_t s_addr = tmem + Cfg::kTmemS + t * kBN;
                         if constexpr (Cfg::SEP_P) {
                             // S_t(j+1) as soon as the softmax has S_t(j) in registers.
@@ -1314,13 +1444,15 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                                                    wctx, kStatusTimeoutMma);
                                     k_ready = true;
                                 }
-                                ok = ok && issue_s(t, ks, j + 2 == it.n_kv[t]);
+                                ok = ok && issue_s(t, ks, j + 1 == last_j(t));
                                 if (!ok) {
                                     break;
                                 }
                             }
                         }
-                        ok = mbar_wait(smem_u32(&sb.p_full[t]), pv_cnt[t] & 1, wctx, kStatusTimeoutMma);
+                        if (active) {
+                            ok = mbar_wait(smem_u32(&sb.p_full[t]), pv_cnt[t] & 1, wctx, kStatusTimeoutMma);
+                        }
                         if (ok && !v_ready) {
                             ok = mbar_wait(smem_u32(&sb.kv_full[vs]), (v_slot / STAGES) & 1, wctx,
                                            kStatusTimeoutMma);
@@ -1330,17 +1462,20 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                             break;
                         }
                         tc_fence_after();
-                        const uint64_t vd = vd0 + stage_off(vs);
-                        if constexpr (Cfg::ACC16) {
-                            issue_pv_mma_f16<Cfg>(tmem + Cfg::tmem_t(t), s_addr, vd);
-                        } else if constexpr (Cfg::SEP_P) {
-                            issue_pv_mma_f32<Cfg>(tmem + Cfg::kTmemO + t * Cfg::D,
-                                                  tmem + Cfg::kTmemExtra + t * 64, vd, j == 0);
-                        } else {
-                            issue_pv_mma_f32<Cfg>(tmem + Cfg::kTmemO + t * Cfg::D, s_addr, vd, j == 0);
+                        if (active) {
+                            const uint64_t vd = vd0 + stage_off(vs);
+                            if constexpr (Cfg::ACC16) {
+                                issue_pv_mma_f16<Cfg>(tmem + Cfg::tmem_t(t), s_addr, vd);
+                            } else if constexpr (Cfg::SEP_P) {
+                                issue_pv_mma_f32<Cfg>(tmem + Cfg::kTmemO + t * Cfg::D,
+                                                      tmem + Cfg::kTmemExtra + t * 64, vd, pv_first[t]);
+                            } else {
+                                issue_pv_mma_f32<Cfg>(tmem + Cfg::kTmemO + t * Cfg::D, s_addr, vd, pv_first[t]);
+                            }
+                            umma_commit(smem_u32(&sb.o_done[t]));
+                            ++pv_cnt[t];
+                            pv_first[t] = false;
                         }
-                        umma_commit(smem_u32(&sb.o_done[t]));
-                        ++pv_cnt[t];
                         if constexpr (!Cfg::SEP_P) {
                             // S_t(j+1) reuses the columns P_t(j) was read from by the MMAs above.
                             if (next_s) {
@@ -1349,7 +1484,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                                                    wctx, kStatusTimeoutMma);
                                     k_ready = true;
                                 }
-                                ok = ok && issue_s(t, ks, j + 2 == it.n_kv[t]);
+                                ok = ok && issue_s(t, ks, j + 1 == last_j(t));
                                 if (!ok) {
                                     break;
                                 }
@@ -1746,6 +1881,62 @@ cudaError_t launch_forward(const FwdProblem& prob, const FwdArgs& args, const Pl
                    : launch_variant<128, false>(variant, bf16, maps[0], maps[1], maps[2], maps[3], a, plan, stream);
     }
     return cudaErrorInvalidValue;
+}
+
+// Window attention: the window build on a persistent grid (its items are short: a few key tiles
+// each), or one CTA per item when they do not fill the GPU.
+template <int D, bool BF16>
+static cudaError_t launch_window_cfg(const FaWindowParams& p, FwdArgs& args, int sm_count, cudaStream_t stream) {
+    using Cfg = FwdCfg<D, true, kVariantOpt, BF16, false, true>;
+    const long long nb = (p.q_len + Cfg::NQ * kBM - 1) / (Cfg::NQ * kBM);
+    const long long items = nb * args.num_bh;
+    if (items > 0x7fffffffLL) {
+        return cudaErrorInvalidConfiguration;
+    }
+    CUtensorMap q, k, v, o;
+    if (encode_strided_map(&q, p.q, p.q_stride, p.batch, p.heads, p.q_len, D, kBM, BF16) != CUDA_SUCCESS ||
+        encode_strided_map(&k, p.k, p.k_stride, p.batch, p.kv_heads, p.k_len, D, kBN, BF16) != CUDA_SUCCESS ||
+        encode_strided_map(&v, p.v, p.v_stride, p.batch, p.kv_heads, p.k_len, D, kBN, BF16) != CUDA_SUCCESS ||
+        encode_strided_map(&o, p.o, p.o_stride, p.batch, p.heads, p.q_len, D, kBM, BF16) != CUDA_SUCCESS) {
+        return cudaErrorInvalidValue;
+    }
+    args.num_items = static_cast<int>(items);
+    args.num_splits = args.tail_splits = 1;
+    args.tail_from = args.num_items;
+    args.div_nb = FastDiv(static_cast<int>(nb));
+    args.div_per_split = FastDiv(args.num_items);
+    const cudaError_t err = ensure_smem_limit<fa_fwd_sm100_kernel<Cfg>>(Cfg::kSmemAlloc);
+    if (err != cudaSuccess) {
+        return err;
+    }
+    const int grid = std::min(args.num_items, sm_count);
+    fa_fwd_sm100_kernel<Cfg><<<grid, Cfg::kThreads, Cfg::kSmemAlloc, stream>>>(q, k, v, o, args);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_window_fwd(const FaWindowParams& p, DeviceStatus* status, unsigned epoch, int sm_count,
+                              cudaStream_t stream) {
+    FwdArgs args{};
+    args.seqlen = p.q_len;
+    args.num_bh = p.batch * p.heads;
+    args.scale_log2 = static_cast<float>(static_cast<double>(p.softmax_scale) * M_LOG2E);
+    args.epoch = epoch;
+    args.status = status;
+    args.o = p.o;
+    args.out_scale = 1.0f;
+    args.win.shift = p.k_len - p.q_len;
+    args.win.window = p.window == 0 ? kNoWindow : std::min(p.window, kNoWindow);
+    args.win.sinks = std::min(p.sinks, p.k_len);
+    args.win.div_heads = FastDiv(p.heads);
+    args.win.div_group = FastDiv(p.heads / p.kv_heads);
+    args.win.lse = p.lse;
+    const bool bf16 = p.dtype == FA_DTYPE_BFLOAT16;
+    if (p.head_dim == 64) {
+        return bf16 ? launch_window_cfg<64, true>(p, args, sm_count, stream)
+                    : launch_window_cfg<64, false>(p, args, sm_count, stream);
+    }
+    return bf16 ? launch_window_cfg<128, true>(p, args, sm_count, stream)
+                : launch_window_cfg<128, false>(p, args, sm_count, stream);
 }
 
 template <int D>

@@ -16,6 +16,9 @@ namespace fa_sm100 {
 // skipped (the kernels' own bounds check on data the host does not see).
 constexpr unsigned kStatusBadPage = 1u << 5;
 
+// A window that hides nothing (lengths are at most 2^30).
+constexpr int kNoWindow = 1 << 30;
+
 // The last key position a row at `pos` sees is pos; the first one of its window is this.
 __host__ __device__ __forceinline__ int window_first(int pos, int window) {
     return (window > 0 && pos >= window) ? pos - window + 1 : 0;

@@ -164,19 +164,6 @@ unsigned blocks(long long rows) { return static_cast<unsigned>((rows + 3) / 4); 
 
 }  // namespace
 
-cudaError_t launch_window_fwd(const FaWindowParams& p, DeviceStatus*, unsigned, int, cudaStream_t stream) {
-    const unsigned grid = blocks(static_cast<long long>(p.batch) * p.heads * p.q_len);
-    const bool bf16 = p.dtype == FA_DTYPE_BFLOAT16;
-    if (p.head_dim == 64) {
-        bf16 ? query_rows_kernel<64, true, false><<<grid, 128, 0, stream>>>(p, nullptr)
-             : query_rows_kernel<64, false, false><<<grid, 128, 0, stream>>>(p, nullptr);
-    } else {
-        bf16 ? query_rows_kernel<128, true, false><<<grid, 128, 0, stream>>>(p, nullptr)
-             : query_rows_kernel<128, false, false><<<grid, 128, 0, stream>>>(p, nullptr);
-    }
-    return cudaGetLastError();
-}
-
 unsigned long long window_bwd_workspace_bytes(const FaWindowParams& p, int) {
     return 4ull * p.batch * p.heads * p.q_len;
 }
