@@ -45,7 +45,7 @@ LIBS = {
         "flash_fwd_sm100.cu",
         "cache_append_sm100.cu",
         "cache_attn_sm100.cu",
-        "window_sm100.cu",
+        "window_bwd_sm100.cu",
         "capi.cu",
         "capi_static.cu",
         "capi_stream.cu",

@@ -1,0 +1,977 @@
+// Backward of window attention with sinks for B200 (sm_100a): tcgen05.mma into tensor memory, TMA
+// rings, softmax warpgroups with one row a thread.
+//
+//   S = scale Q K^T (masked), P = e^(S - LSE), delta = rowsum(dO o O), dP = dO V^T,
+//   dS = P o (dP - delta),  dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K
+//
+// Three passes: delta by rows (bound by DRAM bytes); dK and dV by key tiles; dQ by query tiles. The last
+// two recompute P, seven products a tile pair where one pass over both would take five, but every
+// sum then has one owner: no atomics, no float32 dQ in memory, the same bits every time. They are
+// one kernel, written for a resident pair of tiles (R0, R1) and streamed pairs (X, Y):
+//
+//                 R0  R1  X  Y    S            dP            products
+//   DKV           K   V   Q  dO   K Q^T = S^T  V dO^T = dP^T  dV += P^T Y,  dK += dS^T X
+//   dQ            Q   dO  K  V    Q K^T        dO V^T                       dQ += dS X
+//
+// Tensor memory (columns): S 0..127, dP 128..255, the products' accumulators from 256. P and dS are
+// 16-bit matrix operands read from tensor memory: each lies over the float32 values it was made
+// of, in the half of the columns its own warpgroup has read.
+// The tensor pipe is kept busy by the order of issue: P(i) in hand -> dV(i), S(i+1); dS(i) in hand ->
+// dK(i), dP(i+1). The exponentials of a tile run under the products of dS of the one before.
+//
+// Warps: two warpgroups share a tile's 128 x 128 scores, 64 columns each (thread = row); a third
+// has the TMA producer, the MMA issuer and (DKV) the loader of LSE and delta of the streamed rows. The grid is persistent,
+// one CTA an SM; every role walks the same items with running barrier phases, so that the next item's
+// loads and first products run under an item's last tile and its stores.
+//
+// DKV items. A key tile takes the query tiles of its window, of every head of its group; those
+// with sinks take all later ones. Lists longer than `chunk` tiles are cut; a cut list's parts leave float32 sums in
+// the workspace and a last kernel adds them up in order.
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "sm100_ptx.cuh"
+#include "softmax_common.cuh"
+#include "stream_internal.h"
+#include "tma_host.h"
+
+namespace fa_sm100 {
+
+namespace {
+
+constexpr int kTile = 128;             // rows of every tile
+constexpr int kBox = kTile * 128;      // one TMA box: 128 rows x 128 bytes
+constexpr int kXStages = 3;
+constexpr int kYStages = 2;
+constexpr int kBwdThreads = 384;
+constexpr int kSoftmaxWarps = 8;
+constexpr int kProducerWarp = 8;
+constexpr int kMmaWarp = 9;
+constexpr int kLoaderWarp = 10;
+// Registers: 8 softmax warps take 208 and the other four leave 88, the launch's 384 x 168 in all.
+constexpr int kRegsSoftmax = 208;
+constexpr int kRegsOther = 88;
+static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kBwdThreads * 168, "register split");
+constexpr int kEmuPer8 = 2;  // column pairs of 8 whose 2^x runs on the FMA pipe
+
+struct BwdArgs {
+    int batch, heads, kv_heads, group;
+    int q_len, k_len, shift, window, sinks;
+    int q_tiles, k_tiles;
+    int sink_tiles;         // DKV: key tiles that hold sinks, first in the item order
+    int sink_chunk, tile_chunk;    // DKV: most query tiles of an item of a key tile with sinks, of another
+    int sink_chunks, tile_chunks;  // DKV: items of such a key tile
+    int items;
+    float scale, scale_log2;
+    const float* lse;       // [batch * heads][q_len]
+    const float* delta;
+    float* parts;           // DKV: cut lists' sums, [part][dV, dK][D / 4][128 keys][4]
+    void* out0;             // DKV: dV
+    void* out1;             // dK or dQ
+    int64_t out0_stride[3], out1_stride[3];
+    FastDiv div_qtiles, div_ktiles_rest, div_heads, div_kv_heads, div_group, div_sink_tiles, div_sink_chunks,
+        div_tile_chunks;
+    unsigned epoch;
+    DeviceStatus* status;
+};
+
+template <int D_, bool BF16_, bool DKV_>
+struct BwdCfg {
+    static constexpr int D = D_;
+    static constexpr bool BF16 = BF16_;
+    static constexpr bool DKV = DKV_;
+    static constexpr int kBoxes = D / 64;
+    static constexpr int kTileBytes = kTile * D * 2;
+    static constexpr int kSmemR0 = 0;
+    static constexpr int kSmemR1 = kTileBytes;
+    static constexpr int kSmemX = 2 * kTileBytes;
+    static constexpr int kSmemY = kSmemX + kXStages * kTileBytes;
+    static constexpr int kSmemShared = kSmemY + kYStages * kTileBytes;
+    static constexpr int kTmemS = 0;
+    static constexpr int kTmemDP = 128;
+    static constexpr int kTmemAcc0 = 256;              // DKV: dV
+    static constexpr int kTmemAcc1 = DKV ? 256 + D : 256;  // dK or dQ
+    // d = 128: P over S and dS over dP, each half in its warpgroup's columns (products of one shape run
+    // in issue order). d = 64: columns of their own, since the two kinds of product differ in shape there.
+    static constexpr int kTmemP = D == 128 ? kTmemS : 384;
+    static constexpr int kTmemDS = D == 128 ? kTmemDP : 448;
+    static constexpr int kTmemHalf = D == 128 ? 64 : 32;  // columns between the halves
+    static constexpr int kTmemCols = 512;
+};
+
+struct BwdShared {
+    uint64_t r0_full, r0_empty, r1_full, r1_empty;
+    uint64_t x_full[kXStages], x_empty[kXStages];
+    uint64_t y_full[kYStages], y_empty[kYStages];
+    uint64_t s_full, p_full, dp_full, ds_full, acc_done, acc_free, mma_idle;
+    uint32_t tmem_base;
+    int abort;
+    alignas(16) float lse2[2][kTile];   // DKV: of the streamed rows, log2 units; +inf: P = 0
+    alignas(16) float delta[2][kTile];
+};
+
+// No static shared memory: the tiles start the dynamic window, 1024-byte aligned, and with d = 128 leave
+// 3 KB of the 227 for the rest.
+template <class Cfg>
+constexpr int bwd_smem() {
+    static_assert(Cfg::kSmemShared + sizeof(BwdShared) <= 227 * 1024, "shared memory budget");
+    return Cfg::kSmemShared + static_cast<int>(sizeof(BwdShared));
+}
+
+struct BwdItem {
+    int b, kvh, head;   // head: dQ
+    int row0;           // of the resident tiles
+    int n;              // streamed tiles
+    // DKV: tiles first .. first + n - 1 of the list (head of the group, query tile q0 .. q0 + per - 1)
+    int first, q0, per;
+    long long part;     // -1: the sums are whole
+    bool skip;          // DKV: a part that its list does not have
+    // dQ: key tiles [0, sink_tiles), [first_tile, ..]
+    int sink_tiles, first_tile;
+};
+
+// The query tiles that see key tile kt: [q0, q0 + per).
+__host__ __device__ inline void query_tiles(const BwdArgs& a, int kt, int& q0, int& per) {
+    const long long k0 = static_cast<long long>(kt) * kTile;
+    const long long lo = k0 - a.shift > 0 ? k0 - a.shift : 0;
+    const long long k_last = (k0 + kTile < a.k_len ? k0 + kTile : a.k_len) - 1;
+    long long hi = k0 < a.sinks ? a.q_len - 1 : k_last + a.window - 1 - a.shift;
+    hi = hi < a.q_len - 1 ? hi : a.q_len - 1;
+    q0 = static_cast<int>(lo / kTile);
+    per = hi >= lo ? static_cast<int>(hi / kTile) - q0 + 1 : 0;
+}
+
+template <class Cfg>
+__device__ __forceinline__ BwdItem decode_item(const BwdArgs& a, int idx) {
+    BwdItem it{};
+    it.part = -1;
+    if constexpr (Cfg::DKV) {
+        // Key tiles with sinks first (the longest lists), then the others.
+        const int sink_items = a.batch * a.kv_heads * a.sink_tiles * a.sink_chunks;
+        int kt, bk, c, chunk;
+        if (idx < sink_items) {
+            const int u = a.div_sink_chunks.div(idx);
+            c = idx - u * a.sink_chunks;
+            bk = a.div_sink_tiles.div(u);
+            kt = u - bk * a.sink_tiles;
+            chunk = a.sink_chunk;
+            it.part = idx;
+        } else {
+            const int r = idx - sink_items;
+            const int u = a.div_tile_chunks.div(r);
+            c = r - u * a.tile_chunks;
+            bk = a.div_ktiles_rest.div(u);
+            kt = u - bk * (a.k_tiles - a.sink_tiles) + a.sink_tiles;
+            chunk = a.tile_chunk;
+            it.part = (a.sink_chunks > 1 ? sink_items : 0) + static_cast<long long>(r);
+        }
+        it.b = a.div_kv_heads.div(bk);
+        it.kvh = bk - it.b * a.kv_heads;
+        it.row0 = kt * kTile;
+        query_tiles(a, kt, it.q0, it.per);
+        const int total = it.per * a.group;
+        it.first = c * chunk;
+        it.n = max(0, min(chunk, total - it.first));
+        it.skip = c > 0 && it.n == 0;
+        if (total <= chunk) {
+            it.part = -1;
+        }
+    } else {
+        const int bh = a.div_qtiles.div(idx);
+        it.row0 = (idx - bh * a.q_tiles) * kTile;
+        it.b = a.div_heads.div(bh);
+        it.head = bh - it.b * a.heads;
+        it.kvh = a.div_group.div(it.head);
+        const int lo_pos = max(it.row0 + a.shift, 0);
+        const int hi_pos = max(min(it.row0 + kTile, a.q_len) - 1 + a.shift, 0);
+        it.first_tile = max(lo_pos - a.window + 1, 0) / kTile;
+        it.sink_tiles = min((a.sinks + kTile - 1) / kTile, it.first_tile);
+        it.n = it.sink_tiles + hi_pos / kTile - it.first_tile + 1;
+    }
+    return it;
+}
+
+// Streamed tile i of an item: its first row, and (DKV) its head.
+template <class Cfg>
+__device__ __forceinline__ void stream_tile(const BwdArgs& a, const BwdItem& it, int i, int& row, int& head) {
+    if constexpr (Cfg::DKV) {
+        const int at = it.first + i;
+        const int g = at / it.per;
+        row = (it.q0 + at - g * it.per) * kTile;
+        head = it.kvh * a.group + g;
+    } else {
+        row = (i < it.sink_tiles ? i : i - it.sink_tiles + it.first_tile) * kTile;
+        head = it.kvh;
+    }
+}
+
+// D (128 x 128) = A B^T, both operands 128 rows of the head dim in shared memory.
+template <class Cfg>
+__device__ __forceinline__ void issue_scores(uint32_t d, uint64_t a, uint64_t b) {
+    constexpr uint32_t idesc = make_idesc_f16(kTile, kTile, true, false, Cfg::BF16);
+#pragma unroll
+    for (int k = 0; k < Cfg::D / 16; ++k) {
+        const uint64_t off = static_cast<uint64_t>(((k / 4) * kBox + (k % 4) * 32) >> 4);
+        umma_ss(d, a + off, b + off, idesc, k > 0 ? 1u : 0u);
+    }
+}
+
+// acc (128 x D) += W T: W (128 x 128, 16-bit) in tensor memory, its columns 0..63 from `w`, 64..127 from
+// w + kTmemHalf; T the 128 rows of a streamed tile.
+template <class Cfg>
+__device__ __forceinline__ void issue_product(uint32_t acc, uint32_t w, uint64_t t, bool first) {
+    constexpr uint32_t idesc = make_idesc_f16(kTile, Cfg::D, true, true, Cfg::BF16);
+#pragma unroll
+    for (int k = 0; k < kTile / 16; ++k) {
+        umma_ts(acc, w + (k / 4) * Cfg::kTmemHalf + (k % 4) * 8, t + static_cast<uint64_t>(k * (2048 >> 4)), idesc,
+                (first && k == 0) ? 0u : 1u);
+    }
+}
+
+template <class Cfg>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    window_bwd_kernel(const __grid_constant__ CUtensorMap tm_r0, const __grid_constant__ CUtensorMap tm_r1,
+                      const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_y,
+                      const __grid_constant__ BwdArgs args) {
+    constexpr int D = Cfg::D;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    BwdShared& sh = *reinterpret_cast<BwdShared*>(smem_raw + Cfg::kSmemShared);
+    const int warp = static_cast<int>(threadIdx.x) / 32;
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    const uint32_t smem = smem_u32(smem_raw);
+    if ((smem & 1023u) != 0) {  // the swizzled layouts need it; the driver places the window so
+        atomicOr(&args.status->code, kStatusTimeoutTeardown);
+        return;
+    }
+    const int grid = static_cast<int>(gridDim.x);
+    const int cta = static_cast<int>(blockIdx.x);
+    const WaitCtx wctx{&sh.abort, &args.status->code, &args.status->epoch_aborted, args.epoch};
+
+    if (threadIdx.x == 0) {
+        sh.abort = 0;
+        mbar_init(smem_u32(&sh.r0_full), 1);
+        mbar_init(smem_u32(&sh.r0_empty), 1);
+        mbar_init(smem_u32(&sh.r1_full), 1);
+        mbar_init(smem_u32(&sh.r1_empty), 1);
+        for (int s = 0; s < kXStages; ++s) {
+            mbar_init(smem_u32(&sh.x_full[s]), Cfg::DKV ? 2 : 1);  // the copy, and the rows' statistics
+            mbar_init(smem_u32(&sh.x_empty[s]), 1);
+        }
+        for (int s = 0; s < kYStages; ++s) {
+            mbar_init(smem_u32(&sh.y_full[s]), 1);
+            mbar_init(smem_u32(&sh.y_empty[s]), 1);
+        }
+        mbar_init(smem_u32(&sh.s_full), 1);
+        mbar_init(smem_u32(&sh.p_full), kSoftmaxWarps);
+        mbar_init(smem_u32(&sh.dp_full), 1);
+        mbar_init(smem_u32(&sh.ds_full), kSoftmaxWarps);
+        mbar_init(smem_u32(&sh.acc_done), 1);
+        mbar_init(smem_u32(&sh.acc_free), kSoftmaxWarps);
+        mbar_init(smem_u32(&sh.mma_idle), 1);
+        mbar_fence_init();
+    }
+    if (warp == kMmaWarp) {
+        tmem_alloc(smem_u32(&sh.tmem_base), Cfg::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem_base;
+    // The kernel before this one in the stream wrote delta.
+    cudaGridDependencySynchronize();
+
+    if (warp < kSoftmaxWarps) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    }
+
+    if (warp < kSoftmaxWarps) {
+        // ================================== softmax ====================================
+        const int wg = warp / 4;
+        const int row = (warp % 4) * 32 + lane;
+        const int col0 = wg * 64;
+        const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
+        const uint32_t t_s = tmem + lanes + Cfg::kTmemS + col0;
+        const uint32_t t_dp = tmem + lanes + Cfg::kTmemDP + col0;
+        const uint32_t t_p = tmem + lanes + Cfg::kTmemP + wg * Cfg::kTmemHalf;
+        const uint32_t t_ds = tmem + lanes + Cfg::kTmemDS + wg * Cfg::kTmemHalf;
+        const float scale_log2 = args.scale_log2;
+        int g = 0;      // streamed tiles so far
+        int done = 0;   // accumulations read out so far
+        bool ok = true;
+        auto statistics = [&](int idx, float& lse2, float& delta) {  // dQ: of this thread's row
+            lse2 = INFINITY;
+            delta = 0.0f;
+            if (!Cfg::DKV && idx < args.items) {
+                const BwdItem it = decode_item<Cfg>(args, idx);
+                if (it.row0 + row < args.q_len) {
+                    const long long at =
+                        (static_cast<long long>(it.b) * args.heads + it.head) * args.q_len + it.row0 + row;
+                    const float lse = __ldg(args.lse + at);
+                    lse2 = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
+                    delta = __ldg(args.delta + at);
+                }
+            }
+        };
+        float next_lse2, next_delta;
+        statistics(cta, next_lse2, next_delta);
+        for (int idx = cta; idx < args.items; idx += grid) {
+            const BwdItem it = decode_item<Cfg>(args, idx);
+            if (it.skip) {
+                continue;
+            }
+            const float row_lse2 = next_lse2;
+            const float row_delta = next_delta;
+            statistics(idx + grid, next_lse2, next_delta);
+            for (int i = 0; i < it.n; ++i, ++g) {
+                int tile_row, head;
+                stream_tile<Cfg>(args, it, i, tile_row, head);
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.s_full), g & 1, wctx, kStatusTimeoutSoftmax));
+                if (!ok) {
+                    continue;
+                }
+                tc_fence_after();
+                uint32_t p[64];
+                tmem_ld64(t_s, p);
+                tmem_wait_ld();
+                if constexpr (!Cfg::DKV) {
+                    // S is in registers: the next scores may take its columns.
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(smem_u32(&sh.p_full));
+                    }
+                }
+                const int slot = g % 2;
+                // Masks: query position minus key position in [0, window), or the key a sink.
+                const int q_row = Cfg::DKV ? tile_row : it.row0;
+                const int k_row = Cfg::DKV ? it.row0 : tile_row;
+                const int gap = q_row + args.shift - k_row;  // of the tiles' first rows
+                const bool masked = gap < kTile - 1 || (gap + kTile - 1 >= args.window && k_row + kTile > args.sinks);
+                float2 neg[4];
+#pragma unroll
+                for (int c4 = 0; c4 < 16; ++c4) {
+                    if constexpr (Cfg::DKV) {
+                        const float4 l4 = *reinterpret_cast<const float4*>(&sh.lse2[slot][col0 + 4 * c4]);
+                        neg[0] = make_float2(-l4.x, -l4.y);
+                        neg[1] = make_float2(-l4.z, -l4.w);
+                    } else {
+                        neg[0] = neg[1] = make_float2(-row_lse2, -row_lse2);
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int c = 4 * c4 + 2 * h;
+                        const float2 x = __ffma2_rn(make_float2(u2f(p[c]), u2f(p[c + 1])),
+                                                    make_float2(scale_log2, scale_log2), neg[h]);
+                        p[c] = f2u(x.x);
+                        p[c + 1] = f2u(x.y);
+                    }
+                }
+                if (masked) {
+                    if constexpr (Cfg::DKV) {
+                        // Row = key: it is seen by the columns [from, to].
+                        const int from = row - gap - col0;
+                        const int to = k_row + row < args.sinks ? kNoWindow : from + args.window - 1;
+#pragma unroll
+                        for (int c = 0; c < 64; ++c) {
+                            p[c] = (c >= from && c <= to) ? p[c] : 0xff800000u;
+                        }
+                    } else {
+                        // Row = query: it sees the columns [from, to], and those before `sink`.
+                        const int to = gap + row - col0;
+                        const int from = to - args.window + 1;
+                        const int sink = min(args.sinks - k_row - col0, to + 1);
+#pragma unroll
+                        for (int c = 0; c < 64; ++c) {
+                            p[c] = ((c >= from && c <= to) || c < sink) ? p[c] : 0xff800000u;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 64; c += 2) {
+                    const float2 x = make_float2(u2f(p[c]), u2f(p[c + 1]));
+                    const float2 e = ((c / 2) % 8) < kEmuPer8 ? exp2_poly2_deg3(x)
+                                                              : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                    p[c] = f2u(e.x);
+                    p[c + 1] = f2u(e.y);
+                }
+                if constexpr (Cfg::DKV) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        w[c] = pack2<Cfg::BF16>(u2f(p[2 * c]), u2f(p[2 * c + 1]));
+                    }
+                    tmem_st32(t_p, w);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(smem_u32(&sh.p_full));
+                    }
+                }
+                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.dp_full), g & 1, wctx, kStatusTimeoutSoftmax));
+                if (!ok) {
+                    continue;
+                }
+                tc_fence_after();
+                uint32_t w[32];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t dp[32];
+                    tmem_ld32(t_dp + half * 32, dp);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int c4 = 0; c4 < 8; ++c4) {
+                        float2 d01, d23;
+                        if constexpr (Cfg::DKV) {
+                            const float4 d4 = *reinterpret_cast<const float4*>(&sh.delta[slot][col0 + half * 32 + 4 * c4]);
+                            d01 = make_float2(-d4.x, -d4.y);
+                            d23 = make_float2(-d4.z, -d4.w);
+                        } else {
+                            d01 = d23 = make_float2(-row_delta, -row_delta);
+                        }
+                        const int c = half * 32 + 4 * c4;
+                        const float2 a = __fmul2_rn(make_float2(u2f(p[c]), u2f(p[c + 1])),
+                                                    __fadd2_rn(make_float2(u2f(dp[4 * c4]), u2f(dp[4 * c4 + 1])), d01));
+                        const float2 b = __fmul2_rn(make_float2(u2f(p[c + 2]), u2f(p[c + 3])),
+                                                    __fadd2_rn(make_float2(u2f(dp[4 * c4 + 2]), u2f(dp[4 * c4 + 3])), d23));
+                        w[half * 16 + 2 * c4] = pack2<Cfg::BF16>(a.x, a.y);
+                        w[half * 16 + 2 * c4 + 1] = pack2<Cfg::BF16>(b.x, b.y);
+                    }
+                }
+                tmem_st32(t_ds, w);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(smem_u32(&sh.ds_full));
+                }
+            }
+
+            // The item's sums: DKV: warpgroup 0 stores dV, 1 dK; dQ: a half of the columns each.
+            if (it.n > 0) {
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.acc_done), done & 1, wctx, kStatusTimeoutSoftmax));
+                ++done;
+                if (!ok) {
+                    continue;
+                }
+                tc_fence_after();
+            }
+            if (!ok) {
+                continue;
+            }
+            constexpr int kCols = Cfg::DKV ? D : D / 2;
+            const int out_col = Cfg::DKV ? 0 : wg * kCols;
+            const uint32_t t_acc = tmem + lanes + ((Cfg::DKV && wg == 0) ? Cfg::kTmemAcc0 : Cfg::kTmemAcc1) + out_col;
+            const float factor = (Cfg::DKV && wg == 0) ? 1.0f : args.scale;
+            const int rows = Cfg::DKV ? args.k_len : args.q_len;
+            const bool first_out = Cfg::DKV && wg == 0;
+            const int64_t* st = first_out ? args.out0_stride : args.out1_stride;
+            uint16_t* dst = static_cast<uint16_t*>(first_out ? args.out0 : args.out1) + it.b * st[0] +
+                            (Cfg::DKV ? it.kvh : it.head) * st[1] + static_cast<int64_t>(it.row0 + row) * st[2] + out_col;
+            float4* part = reinterpret_cast<float4*>(args.parts) + (it.part * 2 + wg) * (D / 4) * kTile + row;
+#pragma unroll
+            for (int c = 0; c < kCols / 32; ++c) {
+                uint32_t x[32];
+                if (it.n > 0) {
+                    tmem_ld32(t_acc + c * 32, x);
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        x[e] = 0u;
+                    }
+                }
+                if (c == kCols / 32 - 1 && it.n > 0) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(smem_u32(&sh.acc_free));
+                    }
+                }
+                if (Cfg::DKV && it.part >= 0) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        part[(c * 8 + e) * kTile] = make_float4(u2f(x[4 * e]) * factor, u2f(x[4 * e + 1]) * factor,
+                                                                u2f(x[4 * e + 2]) * factor, u2f(x[4 * e + 3]) * factor);
+                    }
+                } else if (it.row0 + row < rows) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t h[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            h[k] = pack2<Cfg::BF16>(u2f(x[8 * e + 2 * k]) * factor, u2f(x[8 * e + 2 * k + 1]) * factor);
+                        }
+                        *reinterpret_cast<uint4*>(dst + c * 32 + e * 8) = make_uint4(h[0], h[1], h[2], h[3]);
+                    }
+                }
+            }
+        }
+    } else if (warp == kProducerWarp) {
+        // ================================ TMA producer =================================
+        if (lane == 0) {
+            bool ok = true;
+            int g = 0;      // streamed tiles so far
+            int items = 0;  // resident pairs so far
+            for (int idx = cta; ok && idx < args.items; idx += grid) {
+                const BwdItem it = decode_item<Cfg>(args, idx);
+                if (it.n == 0) {
+                    continue;
+                }
+                const int r_head = Cfg::DKV ? it.kvh : it.head;
+                auto load = [&](uint32_t dst, const CUtensorMap* map, uint64_t* bar, int row, int head) {
+                    mbar_arrive_expect_tx(smem_u32(bar), Cfg::kTileBytes);
+#pragma unroll
+                    for (int b = 0; b < Cfg::kBoxes; ++b) {
+                        tma_load_4d(dst + b * kBox, map, smem_u32(bar), b * 64, row, head, it.b);
+                    }
+                };
+                for (int i = 0; ok && i < it.n; ++i, ++g) {
+                    int row, head;
+                    stream_tile<Cfg>(args, it, i, row, head);
+                    const int xs = g % kXStages;
+                    const int ys = g % kYStages;
+                    if (i == 0) {
+                        // R0 is free after the item's last scores, R1 after its last dP.
+                        ok = items == 0 ||
+                             mbar_wait(smem_u32(&sh.r0_empty), (items - 1) & 1, wctx, kStatusTimeoutProducer);
+                        if (ok) {
+                            load(smem + Cfg::kSmemR0, &tm_r0, &sh.r0_full, it.row0, r_head);
+                        }
+                    }
+                    ok = ok && mbar_wait(smem_u32(&sh.x_empty[xs]), ((g / kXStages) & 1) ^ 1, wctx, kStatusTimeoutProducer);
+                    if (ok) {
+                        load(smem + Cfg::kSmemX + xs * Cfg::kTileBytes, &tm_x, &sh.x_full[xs], row, head);
+                    }
+                    if (i == 0) {
+                        ok = ok && (items == 0 ||
+                                    mbar_wait(smem_u32(&sh.r1_empty), (items - 1) & 1, wctx, kStatusTimeoutProducer));
+                        if (ok) {
+                            load(smem + Cfg::kSmemR1, &tm_r1, &sh.r1_full, it.row0, r_head);
+                            ++items;
+                        }
+                    }
+                    ok = ok && mbar_wait(smem_u32(&sh.y_empty[ys]), ((g / kYStages) & 1) ^ 1, wctx, kStatusTimeoutProducer);
+                    if (ok) {
+                        load(smem + Cfg::kSmemY + ys * Cfg::kTileBytes, &tm_y, &sh.y_full[ys], row, head);
+                    }
+                }
+            }
+            if (!ok) {
+                // Copies in flight end by themselves within microseconds; give them that long before
+                // the CTA's shared memory is released.
+                const unsigned long long t0 = globaltimer_ns();
+                while (globaltimer_ns() - t0 < 1000000ull) {
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == kMmaWarp) {
+        // ================================= MMA issuer ==================================
+        if (lane == 0) {
+            bool ok = true;
+            int g = 0;
+            int items = 0;
+            const uint64_t r0 = make_desc_kmajor_sw128(smem + Cfg::kSmemR0);
+            const uint64_t r1 = make_desc_kmajor_sw128(smem + Cfg::kSmemR1);
+            const uint64_t xk = make_desc_kmajor_sw128(smem + Cfg::kSmemX);
+            const uint64_t xn = make_desc_mnmajor_sw128(smem + Cfg::kSmemX, kBox);
+            const uint64_t yk = make_desc_kmajor_sw128(smem + Cfg::kSmemY);
+            const uint64_t yn = make_desc_mnmajor_sw128(smem + Cfg::kSmemY, kBox);
+            auto off = [](int stage) { return static_cast<uint64_t>(stage * (Cfg::kTileBytes >> 4)); };
+            auto wait = [&](uint64_t* bar, int parity) {
+                return mbar_wait(smem_u32(bar), parity & 1, wctx, kStatusTimeoutMma);
+            };
+            auto scores = [&](int at, bool last) {  // S of streamed tile `at`
+                if (!wait(&sh.x_full[at % kXStages], at / kXStages)) {
+                    return false;
+                }
+                tc_fence_after();
+                issue_scores<Cfg>(tmem + Cfg::kTmemS, r0, xk + off(at % kXStages));
+                umma_commit(smem_u32(&sh.s_full));
+                if (last) {
+                    umma_commit(smem_u32(&sh.r0_empty));
+                }
+                return true;
+            };
+            auto dscores = [&](int at, bool last) {  // dP
+                if (!wait(&sh.y_full[at % kYStages], at / kYStages)) {
+                    return false;
+                }
+                tc_fence_after();
+                issue_scores<Cfg>(tmem + Cfg::kTmemDP, r1, yk + off(at % kYStages));
+                umma_commit(smem_u32(&sh.dp_full));
+                if (!Cfg::DKV) {
+                    umma_commit(smem_u32(&sh.y_empty[at % kYStages]));
+                }
+                if (last) {
+                    umma_commit(smem_u32(&sh.r1_empty));
+                }
+                return true;
+            };
+            for (int idx = cta; ok && idx < args.items; idx += grid) {
+                const BwdItem it = decode_item<Cfg>(args, idx);
+                if (it.n == 0) {
+                    continue;
+                }
+                ok = wait(&sh.r0_full, items) && scores(g, it.n == 1) && wait(&sh.r1_full, items) &&
+                     dscores(g, it.n == 1);
+                for (int i = 0; ok && i < it.n; ++i, ++g) {
+                    const bool more = i + 1 < it.n;
+                    const bool last = i + 2 == it.n;
+                    ok = wait(&sh.p_full, g);
+                    if (!ok) {
+                        break;
+                    }
+                    if (i == 0 && items > 0) {
+                        // The item before this one has left the accumulators.
+                        ok = wait(&sh.acc_free, items - 1);
+                        if (!ok) {
+                            break;
+                        }
+                    }
+                    tc_fence_after();
+                    if constexpr (Cfg::DKV) {
+                        issue_product<Cfg>(tmem + Cfg::kTmemAcc0, tmem + Cfg::kTmemP, yn + off(g % kYStages), i == 0);
+                        umma_commit(smem_u32(&sh.y_empty[g % kYStages]));
+                    }
+                    ok = (!more || scores(g + 1, last)) && wait(&sh.ds_full, g);
+                    if (!ok) {
+                        break;
+                    }
+                    tc_fence_after();
+                    issue_product<Cfg>(tmem + Cfg::kTmemAcc1, tmem + Cfg::kTmemDS, xn + off(g % kXStages), i == 0);
+                    umma_commit(smem_u32(&sh.x_empty[g % kXStages]));
+                    if (!more) {
+                        umma_commit(smem_u32(&sh.acc_done));
+                    }
+                    ok = !more || dscores(g + 1, last);
+                }
+                ++items;
+            }
+            // Every MMA issued above must be complete before tensor memory is released.
+            umma_commit(smem_u32(&sh.mma_idle));
+            mbar_wait_drain(smem_u32(&sh.mma_idle), 0, wctx, kStatusTimeoutTeardown);
+        }
+        __syncwarp();
+    } else if (Cfg::DKV && warp == kLoaderWarp) {
+        // ====================== LSE and delta of the streamed query rows ======================
+        bool ok = true;
+        int g = 0;
+        for (int idx = cta; ok && idx < args.items; idx += grid) {
+            const BwdItem it = decode_item<Cfg>(args, idx);
+            for (int i = 0; ok && i < it.n; ++i, ++g) {
+                int row, head;
+                stream_tile<Cfg>(args, it, i, row, head);
+                const long long base = (static_cast<long long>(it.b) * args.heads + head) * args.q_len;
+                float lse[4], delta[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int r = row + k * 32 + lane;
+                    lse[k] = r < args.q_len ? __ldg(args.lse + base + r) : -INFINITY;
+                    delta[k] = r < args.q_len ? __ldg(args.delta + base + r) : 0.0f;
+                }
+                // Two slots: that of tile g is free once the products of tile g - 2 are done.
+                const int slot = g % 2;
+                if (g >= 2) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.x_empty[(g - 2) % kXStages]),
+                                                           ((g - 2) / kXStages) & 1, wctx, kStatusTimeoutProducer));
+                }
+                if (!ok) {
+                    break;
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    sh.lse2[slot][k * 32 + lane] = lse[k] == -INFINITY ? INFINITY : lse[k] * 1.4426950408889634f;
+                    sh.delta[slot][k * 32 + lane] = delta[k];
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(smem_u32(&sh.x_full[g % kXStages]));
+                }
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc(tmem, Cfg::kTmemCols);
+    }
+}
+
+// delta[row] = dO.O, a row by D / 8 lanes.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ FaWindowParams p, float* delta) {
+    constexpr int C = D / 8;
+    const long long row = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / C;
+    const int chunk = static_cast<int>(threadIdx.x) % C;
+    float sum = 0.0f;
+    const long long rows = static_cast<long long>(p.batch) * p.heads * p.q_len;
+    if (row < rows) {
+        const int bh = static_cast<int>(row / p.q_len);
+        const int64_t i = row - static_cast<long long>(bh) * p.q_len;
+        const int b = bh / p.heads;
+        const int h = bh - b * p.heads;
+        const uint4 o = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.o) + b * p.o_stride[0] +
+                                                             h * p.o_stride[1] + i * p.o_stride[2] + chunk * 8));
+        const uint4 d = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.d_o) + b * p.do_stride[0] +
+                                                             h * p.do_stride[1] + i * p.do_stride[2] + chunk * 8));
+        const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
+        const uint32_t dw[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if constexpr (BF16) {
+                sum = fmaf(u2f(ow[k] << 16), u2f(dw[k] << 16), sum);
+                sum = fmaf(u2f(ow[k] & 0xFFFF0000u), u2f(dw[k] & 0xFFFF0000u), sum);
+            } else {
+                const float2 x = unpack_half2(ow[k]);
+                const float2 y = unpack_half2(dw[k]);
+                sum = fmaf(x.x, y.x, sum);
+                sum = fmaf(x.y, y.y, sum);
+            }
+        }
+    }
+#pragma unroll
+    for (int o = C / 2; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    if (row < rows && chunk == 0) {
+        delta[row] = sum;
+    }
+}
+
+// Adds up a cut list's parts, in order. A CTA a key tile of (batch, kv head); lanes take 8 keys x 4
+// groups of 4 dims, so that reads are 128-byte and writes 32-byte pieces.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) window_bwd_join_kernel(const __grid_constant__ BwdArgs a) {
+    const int kt = static_cast<int>(blockIdx.x);
+    const int bk = static_cast<int>(blockIdx.y);
+    const int which = static_cast<int>(blockIdx.z);
+    int q0, per;
+    query_tiles(a, kt, q0, per);
+    const int total = per * a.group;
+    cudaGridDependencySynchronize();
+    const bool sink = kt < a.sink_tiles;
+    const int chunk = sink ? a.sink_chunk : a.tile_chunk;
+    if (total <= chunk) {
+        return;  // stored whole
+    }
+    const int parts = (total + chunk - 1) / chunk;
+    const long long sink_items = static_cast<long long>(a.batch) * a.kv_heads * a.sink_tiles * a.sink_chunks;
+    const long long first =
+        sink ? (static_cast<long long>(bk) * a.sink_tiles + kt) * a.sink_chunks
+             : (a.sink_chunks > 1 ? sink_items : 0) +
+                   (static_cast<long long>(bk) * (a.k_tiles - a.sink_tiles) + kt - a.sink_tiles) * a.tile_chunks;
+    const int b = bk / a.kv_heads;
+    const int h = bk - b * a.kv_heads;
+    const int64_t* st = which == 0 ? a.out0_stride : a.out1_stride;
+    uint16_t* dst = static_cast<uint16_t*>(which == 0 ? a.out0 : a.out1) + b * st[0] + h * st[1];
+    const float4* src = reinterpret_cast<const float4*>(a.parts) + (first * 2 + which) * (D / 4) * kTile;
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    for (int u = static_cast<int>(threadIdx.x) / 32; u < (D / 16) * (kTile / 8); u += 8) {
+        const int key = u / (D / 16) * 8 + lane % 8;
+        const int four = u % (D / 16) * 4 + lane / 8;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int c = 0; c < parts; ++c) {
+            const float4 x = src[(static_cast<long long>(c) * 2 * (D / 4) + four) * kTile + key];
+            sum.x += x.x;
+            sum.y += x.y;
+            sum.z += x.z;
+            sum.w += x.w;
+        }
+        if (kt * kTile + key < a.k_len) {
+            *reinterpret_cast<uint2*>(dst + static_cast<int64_t>(kt * kTile + key) * st[2] + four * 4) =
+                make_uint2(pack2<BF16>(sum.x, sum.y), pack2<BF16>(sum.z, sum.w));
+        }
+    }
+}
+
+// The sizes both passes share, and DKV's cut: the one that ends soonest when the items go over the SMs in
+// turn, an item costing its streamed tiles and about 2 more.
+BwdArgs bwd_args(const FaWindowParams& p, int sm_count) {
+    BwdArgs a{};
+    a.batch = p.batch;
+    a.heads = p.heads;
+    a.kv_heads = p.kv_heads;
+    a.group = p.heads / p.kv_heads;
+    a.q_len = p.q_len;
+    a.k_len = p.k_len;
+    a.shift = p.k_len - p.q_len;
+    a.window = p.window == 0 ? kNoWindow : std::min(p.window, kNoWindow);
+    a.sinks = std::min(p.sinks, p.k_len);
+    a.q_tiles = (p.q_len + kTile - 1) / kTile;
+    a.k_tiles = (p.k_len + kTile - 1) / kTile;
+    a.sink_tiles = (a.sinks + kTile - 1) / kTile;
+    // Streamed tiles of a key tile with sinks (the first has most) and of another (in the middle).
+    int q0 = 0, sink_per = 0;
+    if (a.sink_tiles > 0) {
+        query_tiles(a, 0, q0, sink_per);
+    }
+    const long long sink_total = std::max(1LL, static_cast<long long>(sink_per) * a.group);
+    const int lo = ((-a.shift) % kTile + kTile) % kTile;  // first query row of a key tile within its query tile
+    const long long tile_per = std::min<long long>(a.q_tiles, (static_cast<long long>(lo) + kTile + a.window - 2) / kTile + 1);
+    const long long tile_total = std::max(1LL, tile_per * a.group);
+    const long long heads = static_cast<long long>(p.batch) * p.kv_heads;
+    const long long tiles = heads * (a.k_tiles - a.sink_tiles);
+    const long long sinks = heads * a.sink_tiles;
+    double best = 1e300;
+    for (int cut = 1; cut <= 32; ++cut) {
+        const long long chunk = ((tiles > 0 ? tile_total : sink_total) + cut - 1) / cut;
+        // No more parts of lists with sinks than 8 an SM: they are memory, too.
+        const long long most = std::max(1LL, 8LL * sm_count / std::max(1LL, sinks));
+        const long long sink_chunk = std::max(chunk, (sink_total + most - 1) / most);
+        const long long tile_chunks = (tile_total + chunk - 1) / chunk;
+        const long long sink_chunks = (sink_total + sink_chunk - 1) / sink_chunk;
+        const long long work = tiles * (tile_total + 2 * tile_chunks) + sinks * (sink_total + 2 * sink_chunks);
+        const long long items = tiles * tile_chunks + sinks * sink_chunks;
+        const long long item = std::min(std::max(chunk, sink_chunk), std::max(tile_total, sink_total)) + 2;
+        const double turns = static_cast<double>((items + sm_count - 1) / sm_count) * static_cast<double>(item);
+        const double even = static_cast<double>(work) / sm_count + static_cast<double>(item);
+        const double cost = std::min(turns, even) + (cut > 1 ? 1.0 : 0.0);
+        if (cost < 0.97 * best) {
+            best = cost;
+            a.tile_chunk = static_cast<int>(chunk);
+            a.sink_chunk = static_cast<int>(sink_chunk);
+            a.tile_chunks = static_cast<int>(tile_chunks);
+            a.sink_chunks = static_cast<int>(sink_chunks);
+        }
+        if (chunk <= 2) {
+            break;
+        }
+    }
+    a.scale = p.softmax_scale;
+    a.scale_log2 = static_cast<float>(static_cast<double>(p.softmax_scale) * M_LOG2E);
+    a.div_qtiles = FastDiv(a.q_tiles);
+    a.div_ktiles_rest = FastDiv(std::max(1, a.k_tiles - a.sink_tiles));
+    a.div_heads = FastDiv(a.heads);
+    a.div_kv_heads = FastDiv(a.kv_heads);
+    a.div_group = FastDiv(a.group);
+    a.div_sink_tiles = FastDiv(std::max(1, a.sink_tiles));
+    a.div_sink_chunks = FastDiv(a.sink_chunks);
+    a.div_tile_chunks = FastDiv(a.tile_chunks);
+    return a;
+}
+
+long long dkv_items(const BwdArgs& a) {
+    return static_cast<long long>(a.batch) * a.kv_heads *
+           (static_cast<long long>(a.sink_tiles) * a.sink_chunks +
+            static_cast<long long>(a.k_tiles - a.sink_tiles) * a.tile_chunks);
+}
+
+unsigned long long parts_of(const BwdArgs& a) {
+    const unsigned long long heads = static_cast<unsigned long long>(a.batch) * a.kv_heads;
+    return heads * ((a.sink_chunks > 1 ? static_cast<unsigned long long>(a.sink_tiles) * a.sink_chunks : 0) +
+                    (a.tile_chunks > 1 ? static_cast<unsigned long long>(a.k_tiles - a.sink_tiles) * a.tile_chunks : 0));
+}
+
+unsigned long long delta_bytes(const FaWindowParams& p) {
+    return (4ull * p.batch * p.heads * p.q_len + 255) / 256 * 256;
+}
+
+// Launches after the kernel before it has started to end: it waits for its results itself.
+template <class Kernel, class... Args>
+cudaError_t launch_early(Kernel kernel, dim3 grid, int threads, int smem, cudaStream_t stream, const Args&... args) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(static_cast<unsigned>(threads));
+    config.dynamicSmemBytes = static_cast<size_t>(smem);
+    config.stream = stream;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
+template <int D, bool BF16>
+cudaError_t bwd(const FaWindowParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count,
+                cudaStream_t stream) {
+    BwdArgs a = bwd_args(p, sm_count);
+    a.epoch = epoch;
+    a.status = status;
+    float* delta = static_cast<float*>(workspace);
+    a.lse = p.lse;
+    a.delta = delta;
+    a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + delta_bytes(p));
+    const long long q_items = static_cast<long long>(p.batch) * p.heads * a.q_tiles;
+    const long long k_items = dkv_items(a);
+    const long long rows = static_cast<long long>(p.batch) * p.heads * p.q_len;
+    const long long delta_grid = (rows * (D / 8) + 255) / 256;
+    if (q_items > 0x7fffffffLL || k_items > 0x7fffffffLL || delta_grid > 0x7fffffffLL) {
+        return cudaErrorInvalidConfiguration;
+    }
+    CUtensorMap q, k, v, d_o;
+    if (encode_strided_map(&q, p.q, p.q_stride, p.batch, p.heads, p.q_len, D, kTile, BF16) != CUDA_SUCCESS ||
+        encode_strided_map(&k, p.k, p.k_stride, p.batch, p.kv_heads, p.k_len, D, kTile, BF16) != CUDA_SUCCESS ||
+        encode_strided_map(&v, p.v, p.v_stride, p.batch, p.kv_heads, p.k_len, D, kTile, BF16) != CUDA_SUCCESS ||
+        encode_strided_map(&d_o, p.d_o, p.do_stride, p.batch, p.heads, p.q_len, D, kTile, BF16) != CUDA_SUCCESS) {
+        return cudaErrorInvalidValue;
+    }
+    using Dkv = BwdCfg<D, BF16, true>;
+    using Dq = BwdCfg<D, BF16, false>;
+    cudaError_t err = ensure_smem_limit<window_bwd_kernel<Dkv>>(bwd_smem<Dkv>());
+    if (err == cudaSuccess) {
+        err = ensure_smem_limit<window_bwd_kernel<Dq>>(bwd_smem<Dq>());
+    }
+    if (err != cudaSuccess) {
+        return err;
+    }
+    delta_kernel<D, BF16><<<static_cast<unsigned>(delta_grid), 256, 0, stream>>>(p, delta);
+    err = cudaGetLastError();
+    if (err != cudaSuccess) {
+        return err;
+    }
+    auto strides = [](int64_t(&to)[3], const int64_t(&from)[3]) { std::copy(from, from + 3, to); };
+    a.items = static_cast<int>(k_items);
+    a.out0 = p.dv;
+    a.out1 = p.dk;
+    strides(a.out0_stride, p.dv_stride);
+    strides(a.out1_stride, p.dk_stride);
+    err = launch_early(window_bwd_kernel<Dkv>, dim3(static_cast<unsigned>(std::min<long long>(k_items, sm_count))),
+                       kBwdThreads, bwd_smem<Dkv>(), stream, k, v, q, d_o, a);
+    if (err == cudaSuccess && parts_of(a) > 0) {
+        err = launch_early(window_bwd_join_kernel<D, BF16>,
+                           dim3(static_cast<unsigned>(a.k_tiles), static_cast<unsigned>(p.batch * p.kv_heads), 2), 256, 0,
+                           stream, a);
+    }
+    if (err != cudaSuccess) {
+        return err;
+    }
+    a.items = static_cast<int>(q_items);
+    a.out0 = nullptr;
+    a.out1 = p.dq;
+    strides(a.out1_stride, p.dq_stride);
+    return launch_early(window_bwd_kernel<Dq>, dim3(static_cast<unsigned>(std::min<long long>(q_items, sm_count))),
+                        kBwdThreads, bwd_smem<Dq>(), stream, q, d_o, k, v, a);
+}
+
+}  // namespace
+
+unsigned long long window_bwd_workspace_bytes(const FaWindowParams& p, int sm_count) {
+    return delta_bytes(p) + parts_of(bwd_args(p, sm_count)) * 2 * kTile * p.head_dim * 4;
+}
+
+cudaError_t launch_window_bwd(const FaWindowParams& p, DeviceStatus* status, unsigned epoch, void* workspace,
+                              int sm_count, cudaStream_t stream) {
+    const bool bf16 = p.dtype == FA_DTYPE_BFLOAT16;
+    if (p.head_dim == 64) {
+        return bf16 ? bwd<64, true>(p, status, epoch, workspace, sm_count, stream)
+                    : bwd<64, false>(p, status, epoch, workspace, sm_count, stream);
+    }
+    return bf16 ? bwd<128, true>(p, status, epoch, workspace, sm_count, stream)
+                : bwd<128, false>(p, status, epoch, workspace, sm_count, stream);
+}
+
+}  // namespace fa_sm100
