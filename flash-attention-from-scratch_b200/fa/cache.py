@@ -22,7 +22,7 @@ import struct
 import torch
 
 from fa import _C
-from fa.window import _tensor_strides
+from fa.window import _NO_STRIDES, _on_device, _tensor_strides
 
 # FaCache, then FaAppendParams' and FaCachedParams' own fields (include/fa_b200.h).
 _CACHE = "7P5q7iB3x"
@@ -57,6 +57,14 @@ class PagedKVCache:
                 raise RuntimeError("k_scale and v_scale must be contiguous float32 [pages, kv_heads] on k's device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        # The parts of FaCache that stay as they are: the pool's pointers, its strides, its sizes.
+        (k0, k1, _, _), (v0, v1, _, _) = k.stride(), v.stride()
+        many, heads = self.num_pages > 1, self.kv_heads > 1
+        self._pointers = tuple(0 if t is None else t.data_ptr() for t in (k, v, k_scale, v_scale))
+        self._strides = (k0 * many, k1 * heads, v0 * many, v1 * heads)
+        self._sizes = (self.kv_heads, self.head_dim)
+        self._dtype = _C.DTYPES.get(k.dtype, _C.FA_DTYPE_FLOAT8_E4M3)
+        self.device, self._index = k.device, k.get_device()
 
     @classmethod
     def empty(cls, num_pages: int, page_size: int, kv_heads: int, head_dim: int,
@@ -72,39 +80,38 @@ class PagedKVCache:
 
     def _fields(self, table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor | None, batch: int, tokens: int):
         """FaCache's fields for these sequences, checked."""
-        k, v = self.k, self.v
-        device = k.device
-        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != batch or table.device != device or (
-                table.stride(1) != 1 and table.shape[1] > 1):
-            raise RuntimeError("page_table must be an int32 [B, pages] tensor with contiguous rows on the cache's device")
+        device = self.device
+        if table.dtype != torch.int32 or table.dim() != 2 or table.device != device:
+            raise RuntimeError("page_table must be an int32 [B, pages] tensor on the cache's device")
+        (rows, width), (stride, unit) = table.shape, table.stride()
+        if rows != batch or (unit != 1 and width > 1):
+            raise RuntimeError("page_table must be an int32 [B, pages] tensor with contiguous rows")
         for t in (lengths,) if counts is None else (lengths, counts):
             if t.dtype != torch.int32 or t.shape != (batch,) or t.device != device or not t.is_contiguous():
                 raise RuntimeError("lengths and counts must be contiguous int32 [B] tensors on the cache's device")
-        ks, vs = self.k_scale, self.v_scale
-        (k0, k1, _, _), (v0, v1, _, _) = k.stride(), v.stride()
-        pages, heads = self.num_pages, self.kv_heads
-        return (k.data_ptr(), v.data_ptr(), 0 if ks is None else ks.data_ptr(), 0 if vs is None else vs.data_ptr(),
-                table.data_ptr(), lengths.data_ptr(), 0 if counts is None else counts.data_ptr(),
-                k0 if pages > 1 else 0, k1 if heads > 1 else 0, v0 if pages > 1 else 0, v1 if heads > 1 else 0,
-                table.stride(0) if batch > 1 else table.shape[1], pages, self.page_size, table.shape[1], heads,
-                self.head_dim, batch, tokens, _C.DTYPES.get(k.dtype, _C.FA_DTYPE_FLOAT8_E4M3))
+        return (*self._pointers, table.data_ptr(), lengths.data_ptr(), 0 if counts is None else counts.data_ptr(),
+                *self._strides, stride if batch > 1 else width, self.num_pages, self.page_size, width, *self._sizes,
+                batch, tokens, self._dtype)
 
 
 def _check_tokens(cache: PagedKVCache, *tensors: torch.Tensor) -> None:
     first = tensors[0]
+    dtype, want = first.dtype, None
     for t in tensors:
         if not t.is_cuda:
             raise RuntimeError("q, k, v must be CUDA tensors")
         if t.dtype not in _C.DTYPES:
             raise RuntimeError("q, k, v must be float16 (or bfloat16)")
-        if t.dtype != first.dtype or (cache.k.dtype != torch.float8_e4m3fn and t.dtype != cache.k.dtype):
+        if t.dtype != dtype or (cache.k_scale is None and t.dtype != cache.k.dtype):
             raise RuntimeError("q, k, v must have the same dtype, that of a 16-bit cache")
         if t.dim() != 4:
             raise RuntimeError("q, k, v must have shape [B, H, T, D]")
-        if t.device != cache.k.device:
+        if t.device != cache.device:
             raise RuntimeError("q, k, v must be on the cache's device")
-        if t.shape[0] != first.shape[0] or t.shape[2] != first.shape[2] or t.shape[3] != cache.head_dim:
+        b, _, n, d = t.shape
+        if (b, n) != (want or (b, n)) or d != cache.head_dim:
             raise RuntimeError("q, k, v must have the same batch and tokens, and the cache's head dim")
+        want = (b, n)
 
 
 def append_kv(
@@ -145,20 +152,28 @@ def append_kv(
         if cos.shape != sin.shape:
             raise RuntimeError("cos and sin must have the same shape")
         rows, half = cos.shape
-    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = None if q is None else torch.empty_like(q, memory_format=torch.contiguous_format)
     fields = cache._fields(page_table, lengths, counts, batch, tokens)
     if batch == 0 or tokens == 0:
         return out
+    tables = (0, 0) if cos is None else (cos.data_ptr(), sin.data_ptr())
+    query = (0, 0) if q is None else (q.data_ptr(), out.data_ptr())
     params = _APPEND.pack(
-        *fields, k.data_ptr(), v.data_ptr(), 0 if q is None else q.data_ptr(), 0 if q is None else out.data_ptr(),
-        0 if cos is None else cos.data_ptr(), 0 if cos is None else sin.data_ptr(), *_tensor_strides(k), *_tensor_strides(v),
-        *((0, 0, 0) if q is None else _tensor_strides(q)), 0 if q is None else q.shape[1], rows, 2 * half, interleaved,
-        _C.DTYPES[k.dtype])
-    with torch.cuda.device(k.device):
-        rc = _C.lib.fa_append_kv(params, torch.cuda.current_stream(k.device).cuda_stream)
-    if rc != _C.FA_OK:
-        _C._raise(rc)
+        *fields, k.data_ptr(), v.data_ptr(), *query, *tables, *_tensor_strides(k), *_tensor_strides(v),
+        *(_NO_STRIDES if q is None else _tensor_strides(q)), 0 if q is None else q.shape[1], rows, 2 * half,
+        interleaved, _C.DTYPES[k.dtype])
+    _on_device(cache._index, _C.lib.fa_append_kv, params)
     return out
+
+
+def _run_cached(params: bytes, device: torch.device, stream: int) -> int:
+    """fa_cached_attention with a workspace from torch."""
+    nbytes = ctypes.c_uint64(0)
+    rc = _C.lib.fa_cached_workspace_size(params, ctypes.byref(nbytes))
+    if rc == _C.FA_OK:
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+        rc = _C.lib.fa_cached_attention(params, ws.data_ptr(), nbytes.value, stream)
+    return rc
 
 
 def forward_cached(
@@ -179,20 +194,12 @@ def forward_cached(
     cache's heads, grouped as in forward_window. Scores, softmax and sums are in float32."""
     _check_tokens(cache, q)
     batch, heads, tokens, dim = q.shape
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     fields = cache._fields(page_table, lengths, counts, batch, tokens)
     if q.numel() == 0:
         return o
     scale = 1.0 / math.sqrt(dim) if softmax_scale is None else float(softmax_scale)
     params = _CACHED.pack(*fields, q.data_ptr(), o.data_ptr(), *_tensor_strides(q), heads, window, sinks, scale,
                           _C.DTYPES[q.dtype])
-    with torch.cuda.device(q.device):
-        nbytes = ctypes.c_uint64(0)
-        rc = _C.lib.fa_cached_workspace_size(params, ctypes.byref(nbytes))
-        if rc == _C.FA_OK:
-            ws = torch.empty(nbytes.value, dtype=torch.uint8, device=q.device)
-            rc = _C.lib.fa_cached_attention(params, ws.data_ptr(), nbytes.value,
-                                            torch.cuda.current_stream(q.device).cuda_stream)
-    if rc != _C.FA_OK:
-        _C._raise(rc)
+    _on_device(cache._index, _run_cached, params, cache.device)
     return o

@@ -16,17 +16,24 @@ import struct
 
 import torch
 
+from torch._C import _cuda_getCurrentRawStream as _raw_stream
+
 from fa import _C
 
 # FaWindowParams (include/fa_b200.h): 9 pointers, 8 x 3 strides, 8 ints, the scale, the dtype.
 _PARAMS = struct.Struct("@9P24q8ifB3x")
 
 
+_NO_GRADS = (0,) * 4
+_NO_STRIDES = (0,) * 3
+
+
 def _tensor_strides(t: torch.Tensor) -> tuple[int, int, int]:
     """{batch, head, row} strides; 0 for a dim of one element, whose stride means nothing."""
-    (s0, s1, s2, s3), (n0, n1, n2, n3) = t.stride(), t.shape
-    if s3 != 1 and n3 > 1:
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1:
         raise RuntimeError("tensors must have a contiguous last dimension")
+    n0, n1, n2, _ = t.shape
     return (s0 if n0 > 1 else 0, s1 if n1 > 1 else 0, s2 if n2 > 1 else 0)
 
 
@@ -47,34 +54,35 @@ def _check(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
         raise RuntimeError("q must have shape [B, H, Nq, D], k and v [B, Hkv, Nk, D]")
 
 
-def _run(entry, size_entry, q, k, v, o, lse, do, dq, dk, dv, window, sinks, scale) -> None:
-    """Packs FaWindowParams and calls `entry` on the current stream of q's device, with a
-    workspace from torch of the size that `size_entry` (or None) names."""
-    device = q.device
-    zero = (0, 0, 0)
-    grads = (do, dq, dk, dv)
-    params = _PARAMS.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(),
-        *(0 if t is None else t.data_ptr() for t in grads),
-        *_tensor_strides(q), *_tensor_strides(k), *_tensor_strides(v), *_tensor_strides(o),
-        *(s for t in grads for s in (zero if t is None else _tensor_strides(t))),
-        q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], window, sinks, scale, _C.DTYPES[q.dtype])
-    with torch.cuda.device(device):
-        stream = torch.cuda.current_stream(device).cuda_stream
-        if size_entry is None:
-            rc = entry(params, stream)
-        else:
-            nbytes = ctypes.c_uint64(0)
-            rc = size_entry(params, ctypes.byref(nbytes))
-            if rc == _C.FA_OK:
-                ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
-                rc = entry(params, ws.data_ptr(), nbytes.value, stream)
+def _pack(q, k, v, o, lse, grads, grad_strides, window, sinks, softmax_scale) -> bytes:
+    (b, h, nq, d), (_, hk, nk, _) = q.shape, k.shape
+    scale = 1.0 / math.sqrt(d) if softmax_scale is None else float(softmax_scale)
+    return _PARAMS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(), *grads,
+        *_tensor_strides(q), *_tensor_strides(k), *_tensor_strides(v), *_tensor_strides(o), *grad_strides,
+        b, h, hk, nq, nk, d, window, sinks, scale, _C.DTYPES[q.dtype])
+
+
+def _on_device(index: int, call, *args) -> None:
+    """call(*args, stream) with device `index` and its current stream; raises the library's error."""
+    stream = _raw_stream(index)
+    if torch.cuda.current_device() == index:
+        rc = call(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = call(*args, stream)
     if rc != _C.FA_OK:
         _C._raise(rc)
 
 
-def _scale(softmax_scale: float | None, q: torch.Tensor) -> float:
-    return 1.0 / math.sqrt(q.shape[3]) if softmax_scale is None else float(softmax_scale)
+def _run_bwd(params: bytes, device: torch.device, stream: int) -> int:
+    """fa_window_bwd with a workspace from torch."""
+    nbytes = ctypes.c_uint64(0)
+    rc = _C.lib.fa_window_bwd_workspace_size(params, ctypes.byref(nbytes))
+    if rc == _C.FA_OK:
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+        rc = _C.lib.fa_window_bwd(params, ws.data_ptr(), nbytes.value, stream)
+    return rc
 
 
 def forward_window(
@@ -91,10 +99,11 @@ def forward_window(
     of each row's sum of exp(scale * score), -inf for a row that sees nothing. The result carries
     no gradient: window_attention does."""
     _check(q, k, v)
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
-    if q.numel() > 0 and k.shape[2] > 0:
-        _run(_C.lib.fa_window_fwd, None, q, k, v, o, lse, None, None, None, None, window, sinks, _scale(softmax_scale, q))
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = o.new_empty(q.shape[:3], dtype=torch.float32) if return_lse else None
+    if q.numel() > 0 and k.numel() > 0:
+        params = _pack(q, k, v, o, lse, _NO_GRADS, _NO_STRIDES * 4, window, sinks, softmax_scale)
+        _on_device(q.get_device(), _C.lib.fa_window_fwd, params)
     else:
         o.zero_()
         if lse is not None:
@@ -122,10 +131,12 @@ def backward_window(
             raise RuntimeError("do and o must be tensors like q")
     if lse.shape != q.shape[:3] or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
         raise RuntimeError("lse must be a contiguous float32 [B, H, Nq] tensor on q's device")
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     if q.numel() > 0 and k.numel() > 0:
-        _run(_C.lib.fa_window_bwd, _C.lib.fa_window_bwd_workspace_size, q, k, v, o, lse, do, dq, dk, dv, window, sinks,
-             _scale(softmax_scale, q))
+        strides = (*_tensor_strides(do), *_tensor_strides(dq), *_tensor_strides(dk), *_tensor_strides(dv))
+        grads = (do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
+        params = _pack(q, k, v, o, lse, grads, strides, window, sinks, softmax_scale)
+        _on_device(q.get_device(), _run_bwd, params, q.device)
     else:
         for t in (dq, dk, dv):
             t.zero_()
@@ -149,8 +160,9 @@ class _WindowAttention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, do):
+        if torch.is_grad_enabled():
+            raise RuntimeError("window_attention can be differentiated once (no create_graph)")
         return (*backward_window(_loadable(do), *ctx.saved_tensors, *ctx.how), None, None, None)
 
 
