@@ -56,51 +56,71 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
                       pack2<BF16>(x[6], x[7]));
 }
 
-// Rotates the 8 dims of `chunk` (dims 8 chunk ...) of a row at `pos`. The lanes of a row are
-// consecutive; with halves a lane's partner dims are in the lane rotary / 16 chunks away. Called
-// by whole warps; `live` lanes have a valid position.
-__device__ __forceinline__ void rotate8(float (&x)[8], int chunk, int pos, bool live, const FaAppendParams& p) {
+// cos and sin of the 8 dims of `chunk` (dims 8 chunk ...) at a position: one value a dim with
+// halves, one a pair (4 of the 8) when interleaved.
+struct Angles {
+    float c[8], s[8];
+};
+
+__device__ __forceinline__ void load_angles(Angles& a, int chunk, int pos, bool live, const FaAppendParams& p) {
     const int half = p.rotary_dim / 2;
+    const int hc = half / 8;  // chunks of a half
+    const bool turns = live && chunk < 2 * hc;
+    const long long at = static_cast<long long>(pos) * half +
+                         (p.interleaved ? chunk * 4 : (chunk < hc ? chunk : chunk - hc) * 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        a.c[i] = 1.0f;
+        a.s[i] = 0.0f;
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        if (turns && (q == 0 || !p.interleaved)) {
+            const float4 c = __ldg(reinterpret_cast<const float4*>(p.cos + at + 4 * q));
+            const float4 s = __ldg(reinterpret_cast<const float4*>(p.sin + at + 4 * q));
+            a.c[4 * q] = c.x;
+            a.c[4 * q + 1] = c.y;
+            a.c[4 * q + 2] = c.z;
+            a.c[4 * q + 3] = c.w;
+            a.s[4 * q] = s.x;
+            a.s[4 * q + 1] = s.y;
+            a.s[4 * q + 2] = s.z;
+            a.s[4 * q + 3] = s.w;
+        }
+    }
+}
+
+// Rotates the 8 dims of `chunk` of a row. The lanes of a row are consecutive; with halves a lane's
+// partner dims are in the lane rotary / 16 chunks away, so whole warps call.
+__device__ __forceinline__ void rotate8(float (&x)[8], const Angles& a, int chunk, const FaAppendParams& p) {
+    const int hc = p.rotary_dim / 16;
+    const bool turns = chunk < 2 * hc;
     if (p.interleaved) {
-        if (live && chunk * 8 < p.rotary_dim) {
-            const long long at = static_cast<long long>(pos) * half + chunk * 4;
-            const float4 c = *reinterpret_cast<const float4*>(p.cos + at);
-            const float4 s = *reinterpret_cast<const float4*>(p.sin + at);
-            const float cc[4] = {c.x, c.y, c.z, c.w};
-            const float ss[4] = {s.x, s.y, s.z, s.w};
+        if (turns) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float a = x[2 * i];
-                const float b = x[2 * i + 1];
-                x[2 * i] = __fsub_rn(__fmul_rn(a, cc[i]), __fmul_rn(b, ss[i]));
-                x[2 * i + 1] = __fadd_rn(__fmul_rn(b, cc[i]), __fmul_rn(a, ss[i]));
+                const float u = x[2 * i];
+                const float v = x[2 * i + 1];
+                x[2 * i] = __fsub_rn(__fmul_rn(u, a.c[i]), __fmul_rn(v, a.s[i]));
+                x[2 * i + 1] = __fadd_rn(__fmul_rn(v, a.c[i]), __fmul_rn(u, a.s[i]));
             }
         }
         return;
     }
     const int lane = static_cast<int>(threadIdx.x) & 31;
-    const int hc = half / 8;  // chunks of a half
     const bool first = chunk < hc;
-    const int src = first ? lane + hc : lane - hc;
+    const int src = (first ? lane + hc : lane - hc) & 31;
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        y[i] = __shfl_sync(0xffffffffu, x[i], src & 31);
+        y[i] = __shfl_sync(0xffffffffu, x[i], src);
     }
-    if (live && chunk < 2 * hc) {
-        const long long at = static_cast<long long>(pos) * half + (first ? chunk : chunk - hc) * 8;
+    if (turns) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const float4 c = *reinterpret_cast<const float4*>(p.cos + at + 4 * q);
-            const float4 s = *reinterpret_cast<const float4*>(p.sin + at + 4 * q);
-            const float cc[4] = {c.x, c.y, c.z, c.w};
-            const float ss[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float a = __fmul_rn(x[4 * q + i], cc[i]);
-                const float b = __fmul_rn(y[4 * q + i], ss[i]);
-                x[4 * q + i] = first ? __fsub_rn(a, b) : __fadd_rn(a, b);
-            }
+        for (int i = 0; i < 8; ++i) {
+            const float u = __fmul_rn(x[i], a.c[i]);
+            const float v = __fmul_rn(y[i], a.s[i]);
+            x[i] = first ? __fsub_rn(u, v) : __fadd_rn(u, v);
         }
     }
 }
@@ -174,7 +194,9 @@ __device__ __forceinline__ void store_page(const FaAppendParams& p, DeviceStatus
             }
             unpack8<BF16>(raw, x[i]);
             if (turn) {
-                rotate8(x[i], chunk, lo + r, live, p);
+                Angles a;
+                load_angles(a, chunk, lo + r, live, p);
+                rotate8(x[i], a, chunk, p);
             }
             if constexpr (E4M3) {
 #pragma unroll
@@ -252,50 +274,64 @@ __device__ __forceinline__ void store_page(const FaAppendParams& p, DeviceStatus
     }
 }
 
+// How the rows of q go over the threads: a CTA has `tokens` tokens (a power of two) of as many
+// heads at a time as its rows allow, and takes `heads` of them in turn, so that a thread stays
+// with one token and reads its angles once.
+struct QuerySplit {
+    int log2_tokens, heads, token_blocks, head_blocks;
+};
+
 template <int D, bool BF16>
-__device__ __forceinline__ void rotate_queries(const FaAppendParams& p, DeviceStatus* status, int block) {
+__device__ __forceinline__ void rotate_queries(const FaAppendParams& p, DeviceStatus* status, int block,
+                                               const QuerySplit& split) {
     constexpr int C = D / 8;
+    constexpr int kAtOnce = 4;  // loads in flight of a thread
     const FaCache& c = p.cache;
     const int chunk = static_cast<int>(threadIdx.x) % C;
-    const int groups = static_cast<int>(blockDim.x) / C;
-    const long long total = static_cast<long long>(c.batch) * p.heads * c.tokens;
-    const long long row0 = static_cast<long long>(block) * groups * kRowsPerThread + threadIdx.x / C;
-#pragma unroll 2
-    for (int i = 0; i < kRowsPerThread; ++i) {
-        const long long row = row0 + static_cast<long long>(i) * groups;
-        bool live = row < total;
-        int t = 0, h = 0, b = 0, pos = 0;
-        if (live) {
-            const int bh = static_cast<int>(row / c.tokens);
-            t = static_cast<int>(row - static_cast<long long>(bh) * c.tokens);
-            b = bh / p.heads;
-            h = bh - b * p.heads;
-        }
-        const bool mine = live;
-        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-        if (live) {
-            const int count = c.counts != nullptr ? min(max(c.counts[b], 0), c.tokens) : c.tokens;
-            pos = c.lengths[b] - count + t;
-            live = t < count;
-            if (live && (pos < 0 || (p.cos != nullptr && pos >= p.table_rows))) {
-                live = false;
-                if (chunk == 0 && h == 0) {
-                    atomicOr(&status->code, kStatusBadPage);
-                }
+    const int row = static_cast<int>(threadIdx.x) / C;
+    const int head_step = (static_cast<int>(blockDim.x) / C) >> split.log2_tokens;
+    const int hb = block % split.head_blocks;
+    const int tb = block / split.head_blocks % split.token_blocks;
+    const int b = block / split.head_blocks / split.token_blocks;
+    const int t = (tb << split.log2_tokens) + (row & ((1 << split.log2_tokens) - 1));
+    const int h_end = min((hb + 1) * split.heads, p.heads);
+    const int h0 = hb * split.heads + (row >> split.log2_tokens);
+    const int count = c.counts != nullptr ? min(max(c.counts[b], 0), c.tokens) : c.tokens;
+    const int pos = c.lengths[b] - count + t;
+    const bool mine = t < c.tokens;
+    bool live = t < count;
+    if (live && (pos < 0 || (p.cos != nullptr && pos >= p.table_rows))) {
+        live = false;
+        atomicOr(&status->code, kStatusBadPage);
+    }
+    const uint16_t* src = static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] + t * p.q_stride[2] + chunk * 8;
+    uint16_t* dst = static_cast<uint16_t*>(p.q_out) + (static_cast<int64_t>(b) * p.heads * c.tokens + t) * D + chunk * 8;
+    Angles a;
+    if (p.cos != nullptr) {
+        load_angles(a, chunk, pos, live, p);
+    }
+    for (int h = h0; __any_sync(0xffffffffu, h < h_end); h += kAtOnce * head_step) {
+        uint4 raw[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int hi = h + i * head_step;
+            raw[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (live && hi < h_end) {
+                raw[i] = __ldg(reinterpret_cast<const uint4*>(src + hi * p.q_stride[1]));
             }
         }
-        if (live) {
-            raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] +
-                                                       h * p.q_stride[1] + t * p.q_stride[2] + chunk * 8));
-        }
-        if (p.cos != nullptr) {
-            float x[8];
-            unpack8<BF16>(raw, x);
-            rotate8(x, chunk, pos, live, p);
-            raw = live ? pack8<BF16>(x) : make_uint4(0u, 0u, 0u, 0u);
-        }
-        if (mine) {
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.q_out) + row * D + chunk * 8) = raw;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int hi = h + i * head_step;
+            if (p.cos != nullptr) {
+                float x[8];
+                unpack8<BF16>(raw[i], x);
+                rotate8(x, a, chunk, p);
+                raw[i] = live ? pack8<BF16>(x) : make_uint4(0u, 0u, 0u, 0u);
+            }
+            if (mine && hi < h_end) {
+                *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(hi) * c.tokens * D) = raw[i];
+            }
         }
     }
 }
@@ -303,11 +339,11 @@ __device__ __forceinline__ void rotate_queries(const FaAppendParams& p, DeviceSt
 template <int D, bool BF16, bool E4M3>
 __global__ void __launch_bounds__(kMaxThreads) append_kernel(const __grid_constant__ FaAppendParams p,
                                                              DeviceStatus* status, int page_blocks, int spans,
-                                                             int log2_page) {
+                                                             int log2_page, QuerySplit split) {
     if (static_cast<int>(blockIdx.x) < page_blocks) {
         store_page<D, BF16, E4M3>(p, status, static_cast<int>(blockIdx.x), spans, log2_page);
     } else {
-        rotate_queries<D, BF16>(p, status, static_cast<int>(blockIdx.x) - page_blocks);
+        rotate_queries<D, BF16>(p, status, static_cast<int>(blockIdx.x) - page_blocks, split);
     }
 }
 
@@ -319,10 +355,21 @@ cudaError_t launch(const FaAppendParams& p, DeviceStatus* status, cudaStream_t s
     const long long pages = static_cast<long long>(c.batch) * spans * c.kv_heads * 2;
     // A page is at most kRowsPerThread rows a thread.
     const int threads = std::min(kMaxThreads, std::max(32, c.page_size * (D / 8) / kRowsPerThread));
-    const long long rows = p.q != nullptr ? static_cast<long long>(c.batch) * p.heads * c.tokens : 0;
-    const int rows_per_block = threads / (D / 8) * kRowsPerThread;
-    const long long blocks = pages + (rows + rows_per_block - 1) / rows_per_block;
-    if (blocks > 0x7fffffffLL || rows / c.tokens > 0x7fffffffLL) {
+    QuerySplit split{};
+    long long query_blocks = 0;
+    if (p.q != nullptr) {
+        const int rows = threads / (D / 8);
+        while ((1 << split.log2_tokens) < std::min(rows, c.tokens)) {
+            ++split.log2_tokens;
+        }
+        // Heads of a CTA: 4 loads in flight a thread, twice (with few tokens once: more CTAs).
+        split.heads = (rows >> split.log2_tokens) * (split.log2_tokens > 0 ? 8 : 4);
+        split.token_blocks = (c.tokens + (1 << split.log2_tokens) - 1) >> split.log2_tokens;
+        split.head_blocks = (p.heads + split.heads - 1) / split.heads;
+        query_blocks = static_cast<long long>(c.batch) * split.token_blocks * split.head_blocks;
+    }
+    const long long blocks = pages + query_blocks;
+    if (blocks > 0x7fffffffLL) {
         return cudaErrorInvalidConfiguration;
     }
     int log2_page = 0;
@@ -330,7 +377,7 @@ cudaError_t launch(const FaAppendParams& p, DeviceStatus* status, cudaStream_t s
         ++log2_page;
     }
     append_kernel<D, BF16, E4M3><<<static_cast<unsigned>(blocks), threads, 0, stream>>>(
-        p, status, static_cast<int>(pages), spans, log2_page);
+        p, status, static_cast<int>(pages), spans, log2_page, split);
     return cudaGetLastError();
 }
 
