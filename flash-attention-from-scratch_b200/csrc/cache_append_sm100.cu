@@ -31,8 +31,8 @@ namespace fa_sm100 {
 
 namespace {
 
-constexpr int kRowsPerThread = 8;
-constexpr int kMaxThreads = 512;
+constexpr int kRowsPerThread = 4;
+constexpr int kMaxThreads = 1024;  // a page of 256 tokens x 128 dims; leaves 64 registers a thread
 
 template <bool BF16>
 __device__ __forceinline__ void unpack8(const uint4& raw, float (&x)[8]) {
@@ -57,7 +57,7 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
 }
 
 // cos and sin of the 8 dims of `chunk` (dims 8 chunk ...) at a position: one value a dim with
-// halves, one a pair (4 of the 8) when interleaved.
+// halves (sin negated in the first), one a pair (4 of the 8) when interleaved.
 struct Angles {
     float c[8], s[8];
 };
@@ -82,17 +82,21 @@ __device__ __forceinline__ void load_angles(Angles& a, int chunk, int pos, bool 
             a.c[4 * q + 1] = c.y;
             a.c[4 * q + 2] = c.z;
             a.c[4 * q + 3] = c.w;
-            a.s[4 * q] = s.x;
-            a.s[4 * q + 1] = s.y;
-            a.s[4 * q + 2] = s.z;
-            a.s[4 * q + 3] = s.w;
+            const bool negate = !p.interleaved && chunk < hc;
+            a.s[4 * q] = negate ? -s.x : s.x;
+            a.s[4 * q + 1] = negate ? -s.y : s.y;
+            a.s[4 * q + 2] = negate ? -s.z : s.z;
+            a.s[4 * q + 3] = negate ? -s.w : s.w;
         }
     }
 }
 
-// Rotates the 8 dims of `chunk` of a row. The lanes of a row are consecutive; with halves a lane's
-// partner dims are in the lane rotary / 16 chunks away, so whole warps call.
-__device__ __forceinline__ void rotate8(float (&x)[8], const Angles& a, int chunk, const FaAppendParams& p) {
+// Rotates the 8 dims of `chunk` of a row (16-bit in `raw`, widened to x). The lanes of a row are
+// consecutive; with halves a lane's partner dims are in the lane rotary / 16 chunks away, so whole
+// warps call.
+template <bool BF16>
+__device__ __forceinline__ void rotate8(float (&x)[8], const uint4& raw, const Angles& a, int chunk,
+                                        const FaAppendParams& p) {
     const int hc = p.rotary_dim / 16;
     const bool turns = chunk < 2 * hc;
     if (p.interleaved) {
@@ -108,19 +112,20 @@ __device__ __forceinline__ void rotate8(float (&x)[8], const Angles& a, int chun
         return;
     }
     const int lane = static_cast<int>(threadIdx.x) & 31;
-    const bool first = chunk < hc;
-    const int src = (first ? lane + hc : lane - hc) & 31;
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        y[i] = __shfl_sync(0xffffffffu, x[i], src);
-    }
+    const int src = (chunk < hc ? lane + hc : lane - hc) & 31;
+    uint4 other;
+    other.x = __shfl_sync(0xffffffffu, raw.x, src);
+    other.y = __shfl_sync(0xffffffffu, raw.y, src);
+    other.z = __shfl_sync(0xffffffffu, raw.z, src);
+    other.w = __shfl_sync(0xffffffffu, raw.w, src);
     if (turns) {
+        float y[8];
+        unpack8<BF16>(other, y);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float u = __fmul_rn(x[i], a.c[i]);
-            const float v = __fmul_rn(y[i], a.s[i]);
-            x[i] = first ? __fsub_rn(u, v) : __fadd_rn(u, v);
+            // The first half's sines are negated: x1 c + x2 (-s) is x1 c - x2 s, to the bit. (The paired
+            // forms of these two are contracted to one rounding, so they stay scalar.)
+            x[i] = __fadd_rn(__fmul_rn(x[i], a.c[i]), __fmul_rn(y[i], a.s[i]));
         }
     }
 }
@@ -181,29 +186,41 @@ __device__ __forceinline__ void store_page(const FaAppendParams& p, DeviceStatus
     const bool turn = !is_v && p.cos != nullptr;
     const int rows = hi - lo;
 
+    uint4 raw[kRowsPerThread];
+#pragma unroll
+    for (int i = 0; i < kRowsPerThread; ++i) {
+        const int r = i * groups + group;
+        raw[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows) {
+            raw[i] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<int64_t>(lo + r - start) * st[2]));
+        }
+    }
     float x[kRowsPerThread][8];
     float amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < kRowsPerThread; ++i) {
         if (i * groups < rows) {
             const int r = i * groups + group;
-            const bool live = r < rows;
-            uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-            if (live) {
-                raw = __ldg(reinterpret_cast<const uint4*>(src + static_cast<int64_t>(lo + r - start) * st[2]));
-            }
-            unpack8<BF16>(raw, x[i]);
+            unpack8<BF16>(raw[i], x[i]);
             if (turn) {
                 Angles a;
-                load_angles(a, chunk, lo + r, live, p);
-                rotate8(x[i], a, chunk, p);
+                load_angles(a, chunk, lo + r, r < rows, p);
+                rotate8<BF16>(x[i], raw[i], a, chunk, p);
             }
             if constexpr (E4M3) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float a = fabsf(x[i][e]);
-                    amax = fmaxf(amax, a <= FLT_MAX ? a : 0.0f);
+                    amax = fmaxf(amax, fabsf(x[i][e]));  // NaN passes by
                 }
+            }
+        }
+    }
+    if (E4M3 && amax > FLT_MAX) {  // infinities do not count either
+        amax = 0.0f;
+        for (int i = 0; i < kRowsPerThread && i * groups < rows; ++i) {
+            for (int e = 0; e < 8; ++e) {
+                const float v = fabsf(x[i][e]);
+                amax = fmaxf(amax, v <= FLT_MAX ? v : 0.0f);
             }
         }
     }
@@ -241,7 +258,11 @@ __device__ __forceinline__ void store_page(const FaAppendParams& p, DeviceStatus
         // s is a power of two unless a caller brought other scales: then the quotient is divided.
         const bool pow2 = (__float_as_uint(s) & 0x7FFFFFu) == 0;
         const float inv = 1.0f / s;
-        auto code = [&](float v) { return pow2 ? v * inv : __fdiv_rn(v, s); };
+        auto codes = [&](float u, float v) {
+            const float2 w = pow2 ? __fmul2_rn(make_float2(u, v), make_float2(inv, inv))
+                                  : make_float2(__fdiv_rn(u, s), __fdiv_rn(v, s));
+            return pack_e4m3x2(w.x, w.y);
+        };
         uint8_t* dst = static_cast<uint8_t*>(is_v ? c.v : c.k) + slot0;
         if (in_page > 0 && s > before) {
             const float ratio = before / s;
@@ -265,8 +286,7 @@ __device__ __forceinline__ void store_page(const FaAppendParams& p, DeviceStatus
                 uint32_t w[2];
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    w[q] = pack_e4m3x2(code(x[i][4 * q]), code(x[i][4 * q + 1])) |
-                           (pack_e4m3x2(code(x[i][4 * q + 2]), code(x[i][4 * q + 3])) << 16);
+                    w[q] = codes(x[i][4 * q], x[i][4 * q + 1]) | (codes(x[i][4 * q + 2], x[i][4 * q + 3]) << 16);
                 }
                 *reinterpret_cast<uint2*>(dst + static_cast<int64_t>(in_page + r) * D) = make_uint2(w[0], w[1]);
             }
@@ -326,7 +346,7 @@ __device__ __forceinline__ void rotate_queries(const FaAppendParams& p, DeviceSt
             if (p.cos != nullptr) {
                 float x[8];
                 unpack8<BF16>(raw[i], x);
-                rotate8(x, a, chunk, p);
+                rotate8<BF16>(x, raw[i], a, chunk, p);
                 raw[i] = live ? pack8<BF16>(x) : make_uint4(0u, 0u, 0u, 0u);
             }
             if (mine && hi < h_end) {
