@@ -56,76 +56,73 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
                       pack2<BF16>(x[6], x[7]));
 }
 
+// How pairs are turned.
+enum : int { kNoTurn = 0, kHalves = 1, kInterleaved = 2 };
+
 // cos and sin of the 8 dims of `chunk` (dims 8 chunk ...) at a position: one value a dim with
 // halves (sin negated in the first), one a pair (4 of the 8) when interleaved.
 struct Angles {
     float c[8], s[8];
 };
 
+template <int TURN>
 __device__ __forceinline__ void load_angles(Angles& a, int chunk, int pos, bool live, const FaAppendParams& p) {
     const int half = p.rotary_dim / 2;
     const int hc = half / 8;  // chunks of a half
-    const bool turns = live && chunk < 2 * hc;
+    const bool first = TURN == kInterleaved || chunk < hc;
     const long long at = static_cast<long long>(pos) * half +
-                         (p.interleaved ? chunk * 4 : (chunk < hc ? chunk : chunk - hc) * 8);
+                         (TURN == kInterleaved ? chunk * 4 : (first ? chunk : chunk - hc) * 8);
+    const uint32_t sign = TURN == kHalves && first ? 0x80000000u : 0u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        a.c[i] = 1.0f;
-        a.s[i] = 0.0f;
-    }
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        if (turns && (q == 0 || !p.interleaved)) {
-            const float4 c = __ldg(reinterpret_cast<const float4*>(p.cos + at + 4 * q));
-            const float4 s = __ldg(reinterpret_cast<const float4*>(p.sin + at + 4 * q));
-            a.c[4 * q] = c.x;
-            a.c[4 * q + 1] = c.y;
-            a.c[4 * q + 2] = c.z;
-            a.c[4 * q + 3] = c.w;
-            const bool negate = !p.interleaved && chunk < hc;
-            a.s[4 * q] = negate ? -s.x : s.x;
-            a.s[4 * q + 1] = negate ? -s.y : s.y;
-            a.s[4 * q + 2] = negate ? -s.z : s.z;
-            a.s[4 * q + 3] = negate ? -s.w : s.w;
+    for (int q = 0; q < (TURN == kInterleaved ? 1 : 2); ++q) {
+        float4 c = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (live && chunk < 2 * hc) {
+            c = __ldg(reinterpret_cast<const float4*>(p.cos + at + 4 * q));
+            s = __ldg(reinterpret_cast<const float4*>(p.sin + at + 4 * q));
         }
+        a.c[4 * q] = c.x;
+        a.c[4 * q + 1] = c.y;
+        a.c[4 * q + 2] = c.z;
+        a.c[4 * q + 3] = c.w;
+        a.s[4 * q] = __uint_as_float(__float_as_uint(s.x) ^ sign);
+        a.s[4 * q + 1] = __uint_as_float(__float_as_uint(s.y) ^ sign);
+        a.s[4 * q + 2] = __uint_as_float(__float_as_uint(s.z) ^ sign);
+        a.s[4 * q + 3] = __uint_as_float(__float_as_uint(s.w) ^ sign);
     }
 }
 
 // Rotates the 8 dims of `chunk` of a row (16-bit in `raw`, widened to x). The lanes of a row are
 // consecutive; with halves a lane's partner dims are in the lane rotary / 16 chunks away, so whole
-// warps call.
-template <bool BF16>
-__device__ __forceinline__ void rotate8(float (&x)[8], const uint4& raw, const Angles& a, int chunk,
-                                        const FaAppendParams& p) {
-    const int hc = p.rotary_dim / 16;
+// warps call. Dims beyond rotary_dim stay as they are.
+template <int TURN, bool BF16>
+__device__ __forceinline__ void rotate8(float (&x)[8], const uint4& raw, const Angles& a, int chunk, int hc) {
     const bool turns = chunk < 2 * hc;
-    if (p.interleaved) {
-        if (turns) {
+    if constexpr (TURN == kInterleaved) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float u = x[2 * i];
-                const float v = x[2 * i + 1];
-                x[2 * i] = __fsub_rn(__fmul_rn(u, a.c[i]), __fmul_rn(v, a.s[i]));
-                x[2 * i + 1] = __fadd_rn(__fmul_rn(v, a.c[i]), __fmul_rn(u, a.s[i]));
-            }
+        for (int i = 0; i < 4; ++i) {
+            const float u = x[2 * i];
+            const float v = x[2 * i + 1];
+            x[2 * i] = turns ? __fsub_rn(__fmul_rn(u, a.c[i]), __fmul_rn(v, a.s[i])) : u;
+            x[2 * i + 1] = turns ? __fadd_rn(__fmul_rn(v, a.c[i]), __fmul_rn(u, a.s[i])) : v;
         }
-        return;
-    }
-    const int lane = static_cast<int>(threadIdx.x) & 31;
-    const int src = (chunk < hc ? lane + hc : lane - hc) & 31;
-    uint4 other;
-    other.x = __shfl_sync(0xffffffffu, raw.x, src);
-    other.y = __shfl_sync(0xffffffffu, raw.y, src);
-    other.z = __shfl_sync(0xffffffffu, raw.z, src);
-    other.w = __shfl_sync(0xffffffffu, raw.w, src);
-    if (turns) {
+    } else {
+        const int lane = static_cast<int>(threadIdx.x) & 31;
+        const int src = (chunk < hc ? lane + hc : lane - hc) & 31;
+        uint4 other;
+        other.x = __shfl_sync(0xffffffffu, raw.x, src);
+        other.y = __shfl_sync(0xffffffffu, raw.y, src);
+        other.z = __shfl_sync(0xffffffffu, raw.z, src);
+        other.w = __shfl_sync(0xffffffffu, raw.w, src);
         float y[8];
         unpack8<BF16>(other, y);
+        if (turns) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            // The first half's sines are negated: x1 c + x2 (-s) is x1 c - x2 s, to the bit. (The paired
-            // forms of these two are contracted to one rounding, so they stay scalar.)
-            x[i] = __fadd_rn(__fmul_rn(x[i], a.c[i]), __fmul_rn(y[i], a.s[i]));
+            for (int i = 0; i < 8; ++i) {
+                // The first half's sines are negated: x1 c + x2 (-s) is x1 c - x2 s, to the bit. (The
+                // paired forms of these two are contracted to one rounding, so they stay scalar.)
+                x[i] = __fadd_rn(__fmul_rn(x[i], a.c[i]), __fmul_rn(y[i], a.s[i]));
+            }
         }
     }
 }
@@ -138,13 +135,11 @@ __device__ __forceinline__ float block_scale(float amax) {
     return __uint_as_float(static_cast<uint32_t>(k + 127) << 23);
 }
 
-template <int D, bool BF16, bool E4M3>
-__device__ __forceinline__ void store_page(const FaAppendParams& p, DeviceStatus* status, int unit, int spans,
-                                           int log2_page) {
+template <int D, bool BF16, bool E4M3, int TURN>
+__device__ __forceinline__ void store_page(const FaAppendParams& p, DeviceStatus* status, int unit, bool is_v,
+                                           int spans, int log2_page) {
     constexpr int C = D / 8;  // lanes of a row
     const FaCache& c = p.cache;
-    const bool is_v = (unit & 1) != 0;
-    unit >>= 1;
     const int h = unit % c.kv_heads;
     unit /= c.kv_heads;
     const int span = unit % spans;
@@ -183,7 +178,7 @@ __device__ __forceinline__ void store_page(const FaAppendParams& p, DeviceStatus
     const int groups = static_cast<int>(blockDim.x) / C;
     const int64_t* st = is_v ? p.v_new_stride : p.k_new_stride;
     const uint16_t* src = static_cast<const uint16_t*>(is_v ? p.v_new : p.k_new) + b * st[0] + h * st[1] + chunk * 8;
-    const bool turn = !is_v && p.cos != nullptr;
+    const int hc = p.rotary_dim / 16;
     const int rows = hi - lo;
 
     uint4 raw[kRowsPerThread];
@@ -202,10 +197,10 @@ __device__ __forceinline__ void store_page(const FaAppendParams& p, DeviceStatus
         if (i * groups < rows) {
             const int r = i * groups + group;
             unpack8<BF16>(raw[i], x[i]);
-            if (turn) {
+            if constexpr (TURN != kNoTurn) {
                 Angles a;
-                load_angles(a, chunk, lo + r, r < rows, p);
-                rotate8<BF16>(x[i], raw[i], a, chunk, p);
+                load_angles<TURN>(a, chunk, lo + r, r < rows, p);
+                rotate8<TURN, BF16>(x[i], raw[i], a, chunk, hc);
             }
             if constexpr (E4M3) {
 #pragma unroll
@@ -258,11 +253,6 @@ __device__ __forceinline__ void store_page(const FaAppendParams& p, DeviceStatus
         // s is a power of two unless a caller brought other scales: then the quotient is divided.
         const bool pow2 = (__float_as_uint(s) & 0x7FFFFFu) == 0;
         const float inv = 1.0f / s;
-        auto codes = [&](float u, float v) {
-            const float2 w = pow2 ? __fmul2_rn(make_float2(u, v), make_float2(inv, inv))
-                                  : make_float2(__fdiv_rn(u, s), __fdiv_rn(v, s));
-            return pack_e4m3x2(w.x, w.y);
-        };
         uint8_t* dst = static_cast<uint8_t*>(is_v ? c.v : c.k) + slot0;
         if (in_page > 0 && s > before) {
             const float ratio = before / s;
@@ -279,17 +269,25 @@ __device__ __forceinline__ void store_page(const FaAppendParams& p, DeviceStatus
                 *at = make_uint2(v[0], v[1]);
             }
         }
+        auto store = [&](auto quotient) {
 #pragma unroll
-        for (int i = 0; i < kRowsPerThread; ++i) {
-            const int r = i * groups + group;
-            if (r < rows) {
-                uint32_t w[2];
+            for (int i = 0; i < kRowsPerThread; ++i) {
+                const int r = i * groups + group;
+                if (r < rows) {
+                    uint32_t w[2];
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    w[q] = codes(x[i][4 * q], x[i][4 * q + 1]) | (codes(x[i][4 * q + 2], x[i][4 * q + 3]) << 16);
+                    for (int q = 0; q < 2; ++q) {
+                        w[q] = pack_e4m3x2(quotient(x[i][4 * q]), quotient(x[i][4 * q + 1])) |
+                               (pack_e4m3x2(quotient(x[i][4 * q + 2]), quotient(x[i][4 * q + 3])) << 16);
+                    }
+                    *reinterpret_cast<uint2*>(dst + static_cast<int64_t>(in_page + r) * D) = make_uint2(w[0], w[1]);
                 }
-                *reinterpret_cast<uint2*>(dst + static_cast<int64_t>(in_page + r) * D) = make_uint2(w[0], w[1]);
             }
+        };
+        if (pow2) {
+            store([&](float v) { return v * inv; });
+        } else {
+            store([&](float v) { return __fdiv_rn(v, s); });
         }
     }
 }
@@ -301,7 +299,7 @@ struct QuerySplit {
     int log2_tokens, heads, token_blocks, head_blocks;
 };
 
-template <int D, bool BF16>
+template <int D, bool BF16, int TURN>
 __device__ __forceinline__ void rotate_queries(const FaAppendParams& p, DeviceStatus* status, int block,
                                                const QuerySplit& split) {
     constexpr int C = D / 8;
@@ -326,48 +324,61 @@ __device__ __forceinline__ void rotate_queries(const FaAppendParams& p, DeviceSt
     }
     const uint16_t* src = static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] + t * p.q_stride[2] + chunk * 8;
     uint16_t* dst = static_cast<uint16_t*>(p.q_out) + (static_cast<int64_t>(b) * p.heads * c.tokens + t) * D + chunk * 8;
+    const int64_t src_step = p.q_stride[1] * head_step;
+    const int64_t dst_step = static_cast<int64_t>(head_step) * c.tokens * D;
+    const int hc = p.rotary_dim / 16;
+    src += h0 * p.q_stride[1];
+    dst += static_cast<int64_t>(h0) * c.tokens * D;
     Angles a;
-    if (p.cos != nullptr) {
-        load_angles(a, chunk, pos, live, p);
+    if constexpr (TURN != kNoTurn) {
+        load_angles<TURN>(a, chunk, pos, live, p);
     }
+    const bool any_live = __any_sync(0xffffffffu, live);
     for (int h = h0; __any_sync(0xffffffffu, h < h_end); h += kAtOnce * head_step) {
         uint4 raw[kAtOnce];
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i) {
-            const int hi = h + i * head_step;
             raw[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (live && hi < h_end) {
-                raw[i] = __ldg(reinterpret_cast<const uint4*>(src + hi * p.q_stride[1]));
+            if (live && h + i * head_step < h_end) {
+                raw[i] = __ldg(reinterpret_cast<const uint4*>(src + i * src_step));
+            }
+        }
+        if (TURN != kNoTurn && any_live) {
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                // Padding beside a real token: zeros, which turn into zeros.
+                float x[8];
+                unpack8<BF16>(raw[i], x);
+                rotate8<TURN, BF16>(x, raw[i], a, chunk, hc);
+                raw[i] = pack8<BF16>(x);
             }
         }
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i) {
-            const int hi = h + i * head_step;
-            if (p.cos != nullptr) {
-                float x[8];
-                unpack8<BF16>(raw[i], x);
-                rotate8<BF16>(x, raw[i], a, chunk, p);
-                raw[i] = live ? pack8<BF16>(x) : make_uint4(0u, 0u, 0u, 0u);
-            }
-            if (mine && hi < h_end) {
-                *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(hi) * c.tokens * D) = raw[i];
+            if (mine && h + i * head_step < h_end) {
+                *reinterpret_cast<uint4*>(dst + i * dst_step) = raw[i];
             }
         }
+        src += kAtOnce * src_step;
+        dst += kAtOnce * dst_step;
     }
 }
 
-template <int D, bool BF16, bool E4M3>
+template <int D, bool BF16, bool E4M3, int TURN>
 __global__ void __launch_bounds__(kMaxThreads) append_kernel(const __grid_constant__ FaAppendParams p,
                                                              DeviceStatus* status, int page_blocks, int spans,
                                                              int log2_page, QuerySplit split) {
-    if (static_cast<int>(blockIdx.x) < page_blocks) {
-        store_page<D, BF16, E4M3>(p, status, static_cast<int>(blockIdx.x), spans, log2_page);
+    const int block = static_cast<int>(blockIdx.x);
+    if (block >= page_blocks) {
+        rotate_queries<D, BF16, TURN>(p, status, block - page_blocks, split);
+    } else if ((block & 1) == 0) {
+        store_page<D, BF16, E4M3, TURN>(p, status, block >> 1, false, spans, log2_page);
     } else {
-        rotate_queries<D, BF16>(p, status, static_cast<int>(blockIdx.x) - page_blocks, split);
+        store_page<D, BF16, E4M3, kNoTurn>(p, status, block >> 1, true, spans, log2_page);
     }
 }
 
-template <int D, bool BF16, bool E4M3>
+template <int D, bool BF16, bool E4M3, int TURN>
 cudaError_t launch(const FaAppendParams& p, DeviceStatus* status, cudaStream_t stream) {
     const FaCache& c = p.cache;
     // Every page a sequence's tokens can touch, from any place in the first one.
@@ -396,18 +407,27 @@ cudaError_t launch(const FaAppendParams& p, DeviceStatus* status, cudaStream_t s
     while ((1 << log2_page) < c.page_size) {
         ++log2_page;
     }
-    append_kernel<D, BF16, E4M3><<<static_cast<unsigned>(blocks), threads, 0, stream>>>(
+    append_kernel<D, BF16, E4M3, TURN><<<static_cast<unsigned>(blocks), threads, 0, stream>>>(
         p, status, static_cast<int>(pages), spans, log2_page, split);
     return cudaGetLastError();
 }
 
-template <int D>
-cudaError_t launch_dim(const FaAppendParams& p, DeviceStatus* status, cudaStream_t stream) {
+template <int D, int TURN>
+cudaError_t launch_types(const FaAppendParams& p, DeviceStatus* status, cudaStream_t stream) {
     const bool bf16 = p.dtype == FA_DTYPE_BFLOAT16;
     if (p.cache.dtype == FA_DTYPE_FLOAT8_E4M3) {
-        return bf16 ? launch<D, true, true>(p, status, stream) : launch<D, false, true>(p, status, stream);
+        return bf16 ? launch<D, true, true, TURN>(p, status, stream) : launch<D, false, true, TURN>(p, status, stream);
     }
-    return bf16 ? launch<D, true, false>(p, status, stream) : launch<D, false, false>(p, status, stream);
+    return bf16 ? launch<D, true, false, TURN>(p, status, stream) : launch<D, false, false, TURN>(p, status, stream);
+}
+
+template <int D>
+cudaError_t launch_dim(const FaAppendParams& p, DeviceStatus* status, cudaStream_t stream) {
+    if (p.cos == nullptr) {
+        return launch_types<D, kNoTurn>(p, status, stream);
+    }
+    return p.interleaved ? launch_types<D, kInterleaved>(p, status, stream)
+                         : launch_types<D, kHalves>(p, status, stream);
 }
 
 }  // namespace
