@@ -439,16 +439,23 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         }
     };
 
-    // WIN: the key tile at place j of an item's list, whether query tile t takes it, and t's last place.
+    // WIN: the key tile at place j of an item's list, and the places query tile t takes: up to `last`
+    // but for the hole [hole0, hole1), window tiles of an earlier query tile of the item (kept as three
+    // numbers, since the MMA issuer asks between one product and the next).
     auto list_tile = [&](const Item& it, int j) { return j < it.sink_tiles ? j : j - it.sink_tiles + it.first_tile; };
-    auto takes = [&](const Item& it, int t, int j) {
+    struct Places {
+        int last, hole0, hole1;
+        __device__ __forceinline__ bool has(int j) const { return j <= last && (j < hole0 || j >= hole1); }
+    };
+    auto places_of = [&](const Item& it, int t) {
         const int lo = t == 0 ? it.tile_lo[0] : it.tile_lo[NQ - 1];
         const int hi = t == 0 ? it.tile_hi[0] : it.tile_hi[NQ - 1];
-        const int k = list_tile(it, j);
-        return (t == 0 ? it.n_kv[0] : it.n_kv[NQ - 1]) > 0 && k <= hi && (k >= lo || k * kBN < args.win.sinks);
-    };
-    auto last_place = [&](const Item& it, int t) {
-        return (t == 0 ? it.tile_hi[0] : it.tile_hi[NQ - 1]) - it.first_tile + it.sink_tiles;
+        const int to_place = it.sink_tiles - it.first_tile;
+        Places p;
+        p.last = (t == 0 ? it.n_kv[0] : it.n_kv[NQ - 1]) > 0 ? hi + to_place : -1;
+        p.hole0 = max(it.first_tile, (args.win.sinks + kBN - 1) / kBN) + to_place;
+        p.hole1 = lo + to_place;
+        return p;
     };
 
     const WaitCtx wctx{&sb.abort, &args.status->code, &args.status->epoch_aborted, args.epoch};
@@ -563,7 +570,8 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             // Only what the key-tile loop needs stays live through it; the epilogue decodes the
             // item again for its head and key range.
             int q0, nt, kv0;
-            int places = 0, sink_tiles = 0, first_tile = 0, tile_lo = 0, tile_hi = 0;  // WIN
+            int places = 0, sink_tiles = 0, first_tile = 0;  // WIN
+            Places mine{-1, 0, 0};
             {
                 Item it;
                 decode(idx, it);
@@ -571,11 +579,10 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 nt = (t == 0) ? it.n_kv[0] : it.n_kv[NQ - 1];  // a select keeps `it` in registers
                 kv0 = it.kv0;
                 if constexpr (Cfg::WIN) {
-                    places = nt > 0 ? it.n_max : 0;
+                    mine = places_of(it, t);
+                    places = mine.last + 1;
                     sink_tiles = it.sink_tiles;
                     first_tile = it.first_tile;
-                    tile_lo = t == 0 ? it.tile_lo[0] : it.tile_lo[NQ - 1];
-                    tile_hi = t == 0 ? it.tile_hi[0] : it.tile_hi[NQ - 1];
                     nt = 0;  // counted below
                 }
             }
@@ -591,10 +598,10 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 int j = place;
                 int key_tile = kv0 + j;
                 if constexpr (Cfg::WIN) {
-                    key_tile = place < sink_tiles ? place : place - sink_tiles + first_tile;
-                    if (key_tile > tile_hi || (key_tile < tile_lo && key_tile * kBN >= args.win.sinks)) {
+                    if (!mine.has(place)) {
                         continue;
                     }
+                    key_tile = place < sink_tiles ? place : place - sink_tiles + first_tile;
                     j = nt++;
                 }
                 const int gj = g0 + j;  // running index of S_t(j), P_t(j) and P.V_t(j)
@@ -1137,8 +1144,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 const int n_t = (t == 0) ? it.n_kv[0] : it.n_kv[NQ - 1];
                 const int n_max = it.n_max;
                 // Whether tile t takes place j of the item's key tiles, and its last place.
-                auto has = [&](int j) { return Cfg::WIN ? takes(it, t, j) : j < n_t; };
-                const int last_j = Cfg::WIN ? last_place(it, t) : n_t - 1;
+                const Places mine = places_of(it, t);
+                auto has = [&](int j) { return Cfg::WIN ? mine.has(j) : j < n_t; };
+                const int last_j = Cfg::WIN ? mine.last : n_t - 1;
                 bool pv_first = true;
                 if (n_t > 0) {
                     ok = mbar_wait(smem_u32(&sb.q_full[t]), q_uses & 1, wctx, kStatusTimeoutMma);
@@ -1393,12 +1401,14 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 decode(idx, it);
                 const int n_max = it.n_max;
                 // Whether tile t takes place j of the item's key tiles, and its last place.
-                auto has = [&](int t, int j) { return Cfg::WIN ? takes(it, t, j) : j < it.n_kv[t]; };
-                auto last_j = [&](int t) { return Cfg::WIN ? last_place(it, t) : it.n_kv[t] - 1; };
+                Places mine[NQ];
+                auto has = [&](int t, int j) { return Cfg::WIN ? mine[t].has(j) : j < it.n_kv[t]; };
+                auto last_j = [&](int t) { return Cfg::WIN ? mine[t].last : it.n_kv[t] - 1; };
                 bool pv_first[NQ];
 #pragma unroll
                 for (int t = 0; t < NQ; ++t) {
                     pv_first[t] = true;
+                    mine[t] = places_of(it, t);
                     if (ok && it.n_kv[t] > 0) {
                         ok = mbar_wait(smem_u32(&sb.q_full[t]), q_uses[t] & 1, wctx, kStatusTimeoutMma);
                         ++q_uses[t];
