@@ -651,17 +651,15 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                                              : ((kbase + kBN > n) || (Cfg::CAUSAL && kbase == q0));
                 float tile_max;
                 float mul;
-                if (Cfg::WIN && masked) {
-                    // Columns [from, to] of this row's window, and those before `sink`.
-                    const int to = grow + args.win.shift - kbase;
-                    const int from = to - args.win.window + 1;
-                    const int sink = min(args.win.sinks - kbase, to + 1);
-#pragma unroll
-                    for (int c = 0; c < NC; ++c) {
-                        sr[c] = f2u(((c >= from && c <= to) || c < sink) ? u2f(sr[c]) * scale_log2 : -INFINITY);
+                if constexpr (Cfg::WIN) {
+                    // Hidden scores become what the scale (never 0 here) takes to -inf.
+                    if (masked) {
+                        hide_columns<NC>(sr, grow + args.win.shift - kbase, args.win.window, args.win.sinks - kbase,
+                                         f2u(scale_log2 > 0.0f ? -INFINITY : INFINITY));
                     }
-                    tile_max = row_extreme<true, NC>(sr);
-                    mul = 1.0f;
+                    tile_max = (scale_log2 >= 0.0f ? row_extreme<true, NC>(sr) : row_extreme<false, NC>(sr)) *
+                               scale_log2;
+                    mul = scale_log2;
                 } else if (masked) {
                     // Scale first, then mask, so masked scores are -inf whatever the scale's sign.
                     const int cmax = lim - kbase;
@@ -1930,6 +1928,9 @@ cudaError_t launch_window_fwd(const FaWindowParams& p, DeviceStatus* status, uns
     args.seqlen = p.q_len;
     args.num_bh = p.batch * p.heads;
     args.scale_log2 = static_cast<float>(static_cast<double>(p.softmax_scale) * M_LOG2E);
+    if (args.scale_log2 == 0.0f) {
+        args.scale_log2 = 1e-37f;  // all scores equal, as with 0, but infinities stay what they are
+    }
     args.epoch = epoch;
     args.status = status;
     args.o = p.o;

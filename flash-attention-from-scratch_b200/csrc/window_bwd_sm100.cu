@@ -233,6 +233,18 @@ __device__ __forceinline__ void issue_product(uint32_t acc, uint32_t w, uint64_t
     }
 }
 
+// hide_columns with rows = keys: kept are the columns [from, from + span).
+__device__ __forceinline__ void hide_key_columns(uint32_t (&x)[64], int from, int span) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        const uint32_t keep = bits_up_to(from + span - 1 - 32 * g) & ~bits_up_to(from - 1 - 32 * g);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+            x[32 * g + c] = (keep >> c) & 1u ? x[32 * g + c] : 0xff800000u;
+        }
+    }
+}
+
 template <class Cfg>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     window_bwd_kernel(const __grid_constant__ CUtensorMap tm_r0, const __grid_constant__ CUtensorMap tm_r1,
@@ -376,22 +388,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                 }
                 if (masked) {
                     if constexpr (Cfg::DKV) {
-                        // Row = key: it is seen by the columns [from, to].
-                        const int from = row - gap - col0;
-                        const int to = k_row + row < args.sinks ? kNoWindow : from + args.window - 1;
-#pragma unroll
-                        for (int c = 0; c < 64; ++c) {
-                            p[c] = (c >= from && c <= to) ? p[c] : 0xff800000u;
-                        }
+                        // Row = key: it is seen by the columns [from, from + window), a sink by all from
+                        // `from` on.
+                        hide_key_columns(p, row - gap - col0, k_row + row < args.sinks ? kNoWindow : args.window);
                     } else {
-                        // Row = query: it sees the columns [from, to], and those before `sink`.
-                        const int to = gap + row - col0;
-                        const int from = to - args.window + 1;
-                        const int sink = min(args.sinks - k_row - col0, to + 1);
-#pragma unroll
-                        for (int c = 0; c < 64; ++c) {
-                            p[c] = ((c >= from && c <= to) || c < sink) ? p[c] : 0xff800000u;
-                        }
+                        // Row = query: it sees the columns (to - window, to], and the sinks.
+                        hide_columns<64>(p, gap + row - col0, args.window, args.sinks - k_row - col0, 0xff800000u);
                     }
                 }
 #pragma unroll
