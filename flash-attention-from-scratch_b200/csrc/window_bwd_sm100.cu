@@ -20,13 +20,15 @@
 // dK(i), dP(i+1). The exponentials of a tile run under the products of dS of the one before.
 //
 // Warps: two warpgroups share a tile's 128 x 128 scores, 64 columns each (thread = row); a third
-// has the TMA producer, the MMA issuer and (DKV) the loader of LSE and delta of the streamed rows. The grid is persistent,
-// one CTA an SM; every role walks the same items with running barrier phases, so that the next item's
-// loads and first products run under an item's last tile and its stores.
+// has the TMA producer, the MMA issuer and (DKV) the loader of LSE and delta of the streamed rows. Every
+// role walks the same items with running barrier phases, so that the next item's loads and first
+// products run under an item's last tile and its stores.
 //
-// DKV items. A key tile takes the query tiles of its window, of every head of its group; those
-// with sinks take all later ones. Lists longer than `chunk` tiles are cut; a cut list's parts leave float32 sums in
-// the workspace and a last kernel adds them up in order.
+// Split. A resident tile's list of streamed tiles (DKV: the query tiles of its window, of every head
+// of its group; keys with sinks take all later ones) makes an item; the items laid end to end are cut
+// into equal ranges of streamed tiles, one a CTA, one CTA an SM. Whole lists in turn left up to a
+// quarter of the SMs idle (254 lists of 132 tiles on 148 SMs). A cut list's parts leave float32
+// sums in the workspace, at most two a CTA, and a last kernel adds them up in order.
 
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -62,20 +64,19 @@ constexpr int kEmuPer8 = 2;  // column pairs of 8 whose 2^x runs on the FMA pipe
 struct BwdArgs {
     int batch, heads, kv_heads, group;
     int q_len, k_len, shift, window, sinks;
-    int q_tiles, k_tiles;
-    int sink_tiles;         // DKV: key tiles that hold sinks, first in the item order
-    int sink_chunk, tile_chunk;    // DKV: most query tiles of an item of a key tile with sinks, of another
-    int sink_chunks, tile_chunks;  // DKV: items of such a key tile
-    int items;
+    int tiles;              // resident tiles of a head (DKV: key tiles of a kv head)
+    int grid;               // CTAs
+    long long head_steps;   // streamed tiles of a head's lists
+    long long steps;        // of all heads'
+    long long per;          // of a CTA
     float scale, scale_log2;
     const float* lse;       // [batch * heads][q_len]
     const float* delta;
-    float* parts;           // DKV: cut lists' sums, [part][dV, dK][D / 4][128 keys][4]
+    float* parts;           // cut lists' sums, [part][outputs][D / 4][128 rows][4]
     void* out0;             // DKV: dV
     void* out1;             // dK or dQ
     int64_t out0_stride[3], out1_stride[3];
-    FastDiv div_qtiles, div_ktiles_rest, div_heads, div_kv_heads, div_group, div_sink_tiles, div_sink_chunks,
-        div_tile_chunks;
+    FastDiv div_heads, div_group;  // heads of the lists (DKV: kv heads)
     unsigned epoch;
     DeviceStatus* status;
 };
@@ -111,6 +112,8 @@ struct BwdShared {
     uint64_t s_full, p_full, dp_full, ds_full, acc_done, acc_free, mma_idle;
     uint32_t tmem_base;
     int abort;
+    int tile, offset;  // where the CTA's range starts
+    long long warp_sum[kBwdThreads / 32];
     alignas(16) float lse2[2][kTile];   // DKV: of the streamed rows, log2 units; +inf: P = 0
     alignas(16) float delta[2][kTile];
 };
@@ -126,86 +129,126 @@ constexpr int bwd_smem() {
 struct BwdItem {
     int b, kvh, head;   // head: dQ
     int row0;           // of the resident tiles
-    int n;              // streamed tiles
-    // DKV: tiles first .. first + n - 1 of the list (head of the group, query tile q0 .. q0 + per - 1)
-    int first, q0, per;
-    long long part;     // -1: the sums are whole
-    bool skip;          // DKV: a part that its list does not have
-    // dQ: key tiles [0, sink_tiles), [first_tile, ..]
-    int sink_tiles, first_tile;
+    int total;          // streamed tiles of the list
+    int first, n;       // this CTA's part of it
+    long long part;     // record of the part's sums, -1: it is the whole list
+    int q0, per;        // DKV: the list is query tiles [q0, q0 + per) of every head of the group
+    int sink_tiles, first_tile;  // dQ: the list is key tiles [0, sink_tiles), [first_tile, ..]
 };
 
-// The query tiles that see key tile kt: [q0, q0 + per).
-__host__ __device__ inline void query_tiles(const BwdArgs& a, int kt, int& q0, int& per) {
-    const long long k0 = static_cast<long long>(kt) * kTile;
-    const long long lo = k0 - a.shift > 0 ? k0 - a.shift : 0;
-    const long long k_last = (k0 + kTile < a.k_len ? k0 + kTile : a.k_len) - 1;
-    long long hi = k0 < a.sinks ? a.q_len - 1 : k_last + a.window - 1 - a.shift;
-    hi = hi < a.q_len - 1 ? hi : a.q_len - 1;
-    q0 = static_cast<int>(lo / kTile);
-    per = hi >= lo ? static_cast<int>(hi / kTile) - q0 + 1 : 0;
+// The list of resident tile `tile`: its length, and what it is made of. A tile with nothing to see
+// keeps one streamed tile, all hidden, so that its zeros are written.
+template <bool DKV>
+__host__ __device__ inline void tile_list(const BwdArgs& a, int tile, BwdItem& it) {
+    it.row0 = tile * kTile;
+    if (DKV) {
+        const long long k0 = it.row0;
+        const long long lo = k0 - a.shift > 0 ? k0 - a.shift : 0;
+        const long long k_last = (k0 + kTile < a.k_len ? k0 + kTile : a.k_len) - 1;
+        long long hi = k0 < a.sinks ? a.q_len - 1 : k_last + a.window - 1 - a.shift;
+        hi = hi < a.q_len - 1 ? hi : a.q_len - 1;
+        it.q0 = static_cast<int>(lo / kTile);
+        it.per = hi >= lo ? static_cast<int>(hi / kTile) - it.q0 + 1 : 0;
+        it.total = it.per > 0 ? it.per * a.group : 1;
+        it.per = it.per > 0 ? it.per : 1;
+    } else {
+        const int lo_pos = it.row0 + a.shift > 0 ? it.row0 + a.shift : 0;
+        const int end = it.row0 + kTile < a.q_len ? it.row0 + kTile : a.q_len;
+        const int hi_pos = end - 1 + a.shift > 0 ? end - 1 + a.shift : 0;
+        it.first_tile = lo_pos - a.window + 1 > 0 ? (lo_pos - a.window + 1) / kTile : 0;
+        const int sinks = (a.sinks + kTile - 1) / kTile;
+        it.sink_tiles = sinks < it.first_tile ? sinks : it.first_tile;
+        it.total = it.sink_tiles + hi_pos / kTile - it.first_tile + 1;
+    }
 }
 
-template <class Cfg>
-__device__ __forceinline__ BwdItem decode_item(const BwdArgs& a, int idx) {
-    BwdItem it{};
-    it.part = -1;
-    if constexpr (Cfg::DKV) {
-        // Key tiles with sinks first (the longest lists), then the others.
-        const int sink_items = a.batch * a.kv_heads * a.sink_tiles * a.sink_chunks;
-        int kt, bk, c, chunk;
-        if (idx < sink_items) {
-            const int u = a.div_sink_chunks.div(idx);
-            c = idx - u * a.sink_chunks;
-            bk = a.div_sink_tiles.div(u);
-            kt = u - bk * a.sink_tiles;
-            chunk = a.sink_chunk;
-            it.part = idx;
-        } else {
-            const int r = idx - sink_items;
-            const int u = a.div_tile_chunks.div(r);
-            c = r - u * a.tile_chunks;
-            bk = a.div_ktiles_rest.div(u);
-            kt = u - bk * (a.k_tiles - a.sink_tiles) + a.sink_tiles;
-            chunk = a.tile_chunk;
-            it.part = (a.sink_chunks > 1 ? sink_items : 0) + static_cast<long long>(r);
-        }
-        it.b = a.div_kv_heads.div(bk);
-        it.kvh = bk - it.b * a.kv_heads;
-        it.row0 = kt * kTile;
-        query_tiles(a, kt, it.q0, it.per);
-        const int total = it.per * a.group;
-        it.first = c * chunk;
-        it.n = max(0, min(chunk, total - it.first));
-        it.skip = c > 0 && it.n == 0;
-        if (total <= chunk) {
-            it.part = -1;
-        }
-    } else {
-        const int bh = a.div_qtiles.div(idx);
-        it.row0 = (idx - bh * a.q_tiles) * kTile;
-        it.b = a.div_heads.div(bh);
-        it.head = bh - it.b * a.heads;
-        it.kvh = a.div_group.div(it.head);
-        const int lo_pos = max(it.row0 + a.shift, 0);
-        const int hi_pos = max(min(it.row0 + kTile, a.q_len) - 1 + a.shift, 0);
-        it.first_tile = max(lo_pos - a.window + 1, 0) / kTile;
-        it.sink_tiles = min((a.sinks + kTile - 1) / kTile, it.first_tile);
-        it.n = it.sink_tiles + hi_pos / kTile - it.first_tile + 1;
+template <bool DKV>
+__device__ __forceinline__ int list_length(const BwdArgs& a, int tile) {
+    BwdItem it;
+    tile_list<DKV>(a, tile, it);
+    return it.total;
+}
+
+// The resident tile whose list holds streamed tile `at` of a head's lists, and its place in the list.
+// All THREADS of a block call; the result is in *tile, *offset after the next barrier.
+template <bool DKV, int THREADS>
+__device__ __forceinline__ void locate_tile(const BwdArgs& a, long long at, long long* warp_sum, int* tile, int* offset) {
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    const int warp = static_cast<int>(threadIdx.x) / 32;
+    const int share = (a.tiles + THREADS - 1) / THREADS;
+    const int t0 = min(static_cast<int>(threadIdx.x) * share, a.tiles);
+    const int t1 = min(t0 + share, a.tiles);
+    long long mine = 0;
+    for (int t = t0; t < t1; ++t) {
+        mine += list_length<DKV>(a, t);
     }
-    return it;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+        incl += lane >= o ? up : 0;
+    }
+    if (lane == 31) {
+        warp_sum[warp] = incl;
+    }
+    __syncthreads();
+    long long before = incl - mine;
+    for (int w = 0; w < warp; ++w) {
+        before += warp_sum[w];
+    }
+    if (at >= before && at < before + mine) {
+        for (int t = t0; t < t1; ++t) {
+            const int n = list_length<DKV>(a, t);
+            if (at < before + n) {
+                *tile = t;
+                *offset = static_cast<int>(at - before);
+                break;
+            }
+            before += n;
+        }
+    }
+}
+
+// Walks a CTA's range, list by list.
+struct Cursor {
+    int bx, tile, offset;  // head of the lists, resident tile, place in its list
+    long long left;
+    long long record;      // of the next part
+};
+
+template <bool DKV>
+__device__ __forceinline__ bool next_item(const BwdArgs& a, Cursor& c, BwdItem& it) {
+    if (c.left <= 0) {
+        return false;
+    }
+    tile_list<DKV>(a, c.tile, it);
+    it.b = a.div_heads.div(c.bx);
+    const int h = c.bx - it.b * static_cast<int>(a.div_heads.d);
+    it.head = h;
+    it.kvh = DKV ? h : a.div_group.div(h);
+    it.first = c.offset;
+    it.n = static_cast<int>(min(static_cast<long long>(it.total - c.offset), c.left));
+    it.part = it.n == it.total ? -1 : c.record;
+    c.record |= 1;  // a CTA's range has at most two parts: its first list's and its last's
+    c.left -= it.n;
+    c.offset = 0;
+    if (++c.tile == a.tiles) {
+        c.tile = 0;
+        ++c.bx;
+    }
+    return true;
 }
 
 // Streamed tile i of an item: its first row, and (DKV) its head.
 template <class Cfg>
 __device__ __forceinline__ void stream_tile(const BwdArgs& a, const BwdItem& it, int i, int& row, int& head) {
+    const int at = it.first + i;
     if constexpr (Cfg::DKV) {
-        const int at = it.first + i;
         const int g = at / it.per;
         row = (it.q0 + at - g * it.per) * kTile;
         head = it.kvh * a.group + g;
     } else {
-        row = (i < it.sink_tiles ? i : i - it.sink_tiles + it.first_tile) * kTile;
+        row = (at < it.sink_tiles ? at : at - it.sink_tiles + it.first_tile) * kTile;
         head = it.kvh;
     }
 }
@@ -260,8 +303,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         atomicOr(&args.status->code, kStatusTimeoutTeardown);
         return;
     }
-    const int grid = static_cast<int>(gridDim.x);
-    const int cta = static_cast<int>(blockIdx.x);
+    const long long start = static_cast<long long>(blockIdx.x) * args.per;
+    const int first_head = static_cast<int>(start / args.head_steps);
     const WaitCtx wctx{&sh.abort, &args.status->code, &args.status->epoch_aborted, args.epoch};
 
     if (threadIdx.x == 0) {
@@ -291,10 +334,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tmem_alloc(smem_u32(&sh.tmem_base), Cfg::kTmemCols);
         tmem_relinquish();
     }
+    locate_tile<Cfg::DKV, kBwdThreads>(args, start - first_head * args.head_steps, sh.warp_sum, &sh.tile, &sh.offset);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem_base;
+    Cursor cursor;
+    cursor.bx = first_head;
+    cursor.tile = sh.tile;
+    cursor.offset = sh.offset;
+    cursor.left = min(args.per, args.steps - start);
+    cursor.record = 2 * static_cast<long long>(blockIdx.x);
     // The kernel before this one in the stream wrote delta.
     cudaGridDependencySynchronize();
 
@@ -318,30 +368,27 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         int g = 0;      // streamed tiles so far
         int done = 0;   // accumulations read out so far
         bool ok = true;
-        auto statistics = [&](int idx, float& lse2, float& delta) {  // dQ: of this thread's row
-            lse2 = INFINITY;
-            delta = 0.0f;
-            if (!Cfg::DKV && idx < args.items) {
-                const BwdItem it = decode_item<Cfg>(args, idx);
-                if (it.row0 + row < args.q_len) {
-                    const long long at =
-                        (static_cast<long long>(it.b) * args.heads + it.head) * args.q_len + it.row0 + row;
-                    const float lse = __ldg(args.lse + at);
-                    lse2 = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
-                    delta = __ldg(args.delta + at);
-                }
+        BwdItem it, next;
+        bool more = next_item<Cfg::DKV>(args, cursor, next);
+        float next_lse2, next_delta;
+        auto statistics = [&]() {  // dQ: of this thread's row of the next item
+            next_lse2 = INFINITY;
+            next_delta = 0.0f;
+            if (!Cfg::DKV && more && next.row0 + row < args.q_len) {
+                const long long at =
+                    (static_cast<long long>(next.b) * args.heads + next.head) * args.q_len + next.row0 + row;
+                const float lse = __ldg(args.lse + at);
+                next_lse2 = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
+                next_delta = __ldg(args.delta + at);
             }
         };
-        float next_lse2, next_delta;
-        statistics(cta, next_lse2, next_delta);
-        for (int idx = cta; idx < args.items; idx += grid) {
-            const BwdItem it = decode_item<Cfg>(args, idx);
-            if (it.skip) {
-                continue;
-            }
+        statistics();
+        while (more) {
+            it = next;
             const float row_lse2 = next_lse2;
             const float row_delta = next_delta;
-            statistics(idx + grid, next_lse2, next_delta);
+            more = next_item<Cfg::DKV>(args, cursor, next);
+            statistics();
             for (int i = 0; i < it.n; ++i, ++g) {
                 int tile_row, head;
                 stream_tile<Cfg>(args, it, i, tile_row, head);
@@ -458,17 +505,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             }
 
             // The item's sums: DKV: warpgroup 0 stores dV, 1 dK; dQ: a half of the columns each.
-            if (it.n > 0) {
-                ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.acc_done), done & 1, wctx, kStatusTimeoutSoftmax));
-                ++done;
-                if (!ok) {
-                    continue;
-                }
-                tc_fence_after();
-            }
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.acc_done), done & 1, wctx, kStatusTimeoutSoftmax));
+            ++done;
             if (!ok) {
                 continue;
             }
+            tc_fence_after();
             constexpr int kCols = Cfg::DKV ? D : D / 2;
             const int out_col = Cfg::DKV ? 0 : wg * kCols;
             const uint32_t t_acc = tmem + lanes + ((Cfg::DKV && wg == 0) ? Cfg::kTmemAcc0 : Cfg::kTmemAcc1) + out_col;
@@ -478,27 +520,21 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             const int64_t* st = first_out ? args.out0_stride : args.out1_stride;
             uint16_t* dst = static_cast<uint16_t*>(first_out ? args.out0 : args.out1) + it.b * st[0] +
                             (Cfg::DKV ? it.kvh : it.head) * st[1] + static_cast<int64_t>(it.row0 + row) * st[2] + out_col;
-            float4* part = reinterpret_cast<float4*>(args.parts) + (it.part * 2 + wg) * (D / 4) * kTile + row;
+            float4* part = reinterpret_cast<float4*>(args.parts) +
+                           (Cfg::DKV ? (it.part * 2 + wg) * (D / 4) : it.part * (D / 4) + out_col / 4) * kTile + row;
 #pragma unroll
             for (int c = 0; c < kCols / 32; ++c) {
                 uint32_t x[32];
-                if (it.n > 0) {
-                    tmem_ld32(t_acc + c * 32, x);
-                    tmem_wait_ld();
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        x[e] = 0u;
-                    }
-                }
-                if (c == kCols / 32 - 1 && it.n > 0) {
+                tmem_ld32(t_acc + c * 32, x);
+                tmem_wait_ld();
+                if (c == kCols / 32 - 1) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
                         mbar_arrive(smem_u32(&sh.acc_free));
                     }
                 }
-                if (Cfg::DKV && it.part >= 0) {
+                if (it.part >= 0) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         part[(c * 8 + e) * kTile] = make_float4(u2f(x[4 * e]) * factor, u2f(x[4 * e + 1]) * factor,
@@ -523,11 +559,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             bool ok = true;
             int g = 0;      // streamed tiles so far
             int items = 0;  // resident pairs so far
-            for (int idx = cta; ok && idx < args.items; idx += grid) {
-                const BwdItem it = decode_item<Cfg>(args, idx);
-                if (it.n == 0) {
-                    continue;
-                }
+            BwdItem it;
+            while (ok && next_item<Cfg::DKV>(args, cursor, it)) {
                 const int r_head = Cfg::DKV ? it.kvh : it.head;
                 auto load = [&](uint32_t dst, const CUtensorMap* map, uint64_t* bar, int row, int head) {
                     mbar_arrive_expect_tx(smem_u32(bar), Cfg::kTileBytes);
@@ -619,11 +652,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                 }
                 return true;
             };
-            for (int idx = cta; ok && idx < args.items; idx += grid) {
-                const BwdItem it = decode_item<Cfg>(args, idx);
-                if (it.n == 0) {
-                    continue;
-                }
+            BwdItem it;
+            while (ok && next_item<Cfg::DKV>(args, cursor, it)) {
                 ok = wait(&sh.r0_full, items) && scores(g, it.n == 1) && wait(&sh.r1_full, items) &&
                      dscores(g, it.n == 1);
                 for (int i = 0; ok && i < it.n; ++i, ++g) {
@@ -668,8 +698,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         // ====================== LSE and delta of the streamed query rows ======================
         bool ok = true;
         int g = 0;
-        for (int idx = cta; ok && idx < args.items; idx += grid) {
-            const BwdItem it = decode_item<Cfg>(args, idx);
+        BwdItem it;
+        while (ok && next_item<Cfg::DKV>(args, cursor, it)) {
             for (int i = 0; ok && i < it.n; ++i, ++g) {
                 int row, head;
                 stream_tile<Cfg>(args, it, i, row, head);
@@ -752,55 +782,77 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ FaWi
     }
 }
 
-// Adds up a cut list's parts, in order. A CTA a key tile of (batch, kv head); lanes take 8 keys x 4
-// groups of 4 dims, so that reads are 128-byte and writes 32-byte pieces.
-template <int D, bool BF16>
-__global__ void __launch_bounds__(256) window_bwd_join_kernel(const __grid_constant__ BwdArgs a) {
-    const int kt = static_cast<int>(blockIdx.x);
-    const int bk = static_cast<int>(blockIdx.y);
-    const int which = static_cast<int>(blockIdx.z);
-    int q0, per;
-    query_tiles(a, kt, q0, per);
-    const int total = per * a.group;
-    cudaGridDependencySynchronize();
-    const bool sink = kt < a.sink_tiles;
-    const int chunk = sink ? a.sink_chunk : a.tile_chunk;
-    if (total <= chunk) {
-        return;  // stored whole
+// Adds up the parts of the list that is cut at the end of CTA blockIdx.x's range (of the dK, dV pass, then
+// of the dQ pass), if that is its first cut; a quarter of the dims by blockIdx.y % 4, dV and dK by
+// blockIdx.y / 4. Lanes take 8 rows x 4 groups of 4 dims: 128-byte reads, 32-byte writes.
+constexpr int kJoinThreads = 256;
+
+template <int D, bool BF16, bool DKV>
+__device__ __forceinline__ void join(const BwdArgs& a, int boundary) {
+    __shared__ long long warp_sum[kJoinThreads / 32];
+    __shared__ int tile, offset;
+    const int which = static_cast<int>(blockIdx.y) / 4;
+    if (which >= (DKV ? 2 : 1)) {
+        return;
     }
-    const int parts = (total + chunk - 1) / chunk;
-    const long long sink_items = static_cast<long long>(a.batch) * a.kv_heads * a.sink_tiles * a.sink_chunks;
-    const long long first =
-        sink ? (static_cast<long long>(bk) * a.sink_tiles + kt) * a.sink_chunks
-             : (a.sink_chunks > 1 ? sink_items : 0) +
-                   (static_cast<long long>(bk) * (a.k_tiles - a.sink_tiles) + kt - a.sink_tiles) * a.tile_chunks;
-    const int b = bk / a.kv_heads;
-    const int h = bk - b * a.kv_heads;
-    const int64_t* st = which == 0 ? a.out0_stride : a.out1_stride;
-    uint16_t* dst = static_cast<uint16_t*>(which == 0 ? a.out0 : a.out1) + b * st[0] + h * st[1];
-    const float4* src = reinterpret_cast<const float4*>(a.parts) + (first * 2 + which) * (D / 4) * kTile;
+    const long long cut = (boundary + 1) * a.per;
+    const int bx = static_cast<int>(cut / a.head_steps);
+    locate_tile<DKV, kJoinThreads>(a, cut - bx * a.head_steps, warp_sum, &tile, &offset);
+    __syncthreads();
+    const long long begin = cut - offset;
+    if (offset == 0 || begin / a.per != boundary) {
+        return;
+    }
+    BwdItem it;
+    tile_list<DKV>(a, tile, it);
+    const long long last = (begin + it.total - 1) / a.per;
+    const int b = a.div_heads.div(bx);
+    const int h = bx - b * static_cast<int>(a.div_heads.d);
+    const bool first_out = DKV && which == 0;
+    const int64_t* st = first_out ? a.out0_stride : a.out1_stride;
+    uint16_t* dst = static_cast<uint16_t*>(first_out ? a.out0 : a.out1) + b * st[0] + h * st[1];
+    const int rows = DKV ? a.k_len : a.q_len;
     const int lane = static_cast<int>(threadIdx.x) % 32;
-    for (int u = static_cast<int>(threadIdx.x) / 32; u < (D / 16) * (kTile / 8); u += 8) {
-        const int key = u / (D / 16) * 8 + lane % 8;
-        const int four = u % (D / 16) * 4 + lane / 8;
+    const int quarter = static_cast<int>(blockIdx.y) % 4;
+    constexpr int kOutputs = DKV ? 2 : 1;
+    for (int u = static_cast<int>(threadIdx.x) / 32; u < (D / 64) * (kTile / 8); u += kJoinThreads / 32) {
+        const int row = u / (D / 64) * 8 + lane % 8;
+        const int four = quarter * (D / 16) + u % (D / 64) * 4 + lane / 8;
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-        for (int c = 0; c < parts; ++c) {
-            const float4 x = src[(static_cast<long long>(c) * 2 * (D / 4) + four) * kTile + key];
+        for (long long c = boundary; c <= last; ++c) {
+            // The list is its first CTA's last part unless it starts that CTA's range; else a first part.
+            const long long record = 2 * c + (c * a.per >= begin ? 0 : 1);
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(a.parts) +
+                                    ((record * kOutputs + which) * (D / 4) + four) * kTile + row);
             sum.x += x.x;
             sum.y += x.y;
             sum.z += x.z;
             sum.w += x.w;
         }
-        if (kt * kTile + key < a.k_len) {
-            *reinterpret_cast<uint2*>(dst + static_cast<int64_t>(kt * kTile + key) * st[2] + four * 4) =
+        if (it.row0 + row < rows) {
+            *reinterpret_cast<uint2*>(dst + static_cast<int64_t>(it.row0 + row) * st[2] + four * 4) =
                 make_uint2(pack2<BF16>(sum.x, sum.y), pack2<BF16>(sum.z, sum.w));
         }
     }
 }
 
-// The sizes both passes share, and DKV's cut: the one that ends soonest when the items go over the SMs in
-// turn, an item costing its streamed tiles and about 2 more.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kJoinThreads) window_bwd_join_kernel(const __grid_constant__ BwdArgs dkv,
+                                                                       const __grid_constant__ BwdArgs dq) {
+    cudaGridDependencySynchronize();
+    const int block = static_cast<int>(blockIdx.x);
+    if (block < dkv.grid - 1) {
+        join<D, BF16, true>(dkv, block);
+    } else {
+        join<D, BF16, false>(dq, block - (dkv.grid - 1));
+    }
+}
+
+constexpr int kMinSteps = 4;  // least streamed tiles of a CTA's range
+
+// The sizes of a pass, and its cut into ranges.
+template <bool DKV>
 BwdArgs bwd_args(const FaWindowParams& p, int sm_count) {
     BwdArgs a{};
     a.batch = p.batch;
@@ -812,69 +864,25 @@ BwdArgs bwd_args(const FaWindowParams& p, int sm_count) {
     a.shift = p.k_len - p.q_len;
     a.window = p.window == 0 ? kNoWindow : std::min(p.window, kNoWindow);
     a.sinks = std::min(p.sinks, p.k_len);
-    a.q_tiles = (p.q_len + kTile - 1) / kTile;
-    a.k_tiles = (p.k_len + kTile - 1) / kTile;
-    a.sink_tiles = (a.sinks + kTile - 1) / kTile;
-    // Streamed tiles of a key tile with sinks (the first has most) and of another (in the middle).
-    int q0 = 0, sink_per = 0;
-    if (a.sink_tiles > 0) {
-        query_tiles(a, 0, q0, sink_per);
+    a.tiles = ((DKV ? p.k_len : p.q_len) + kTile - 1) / kTile;
+    for (int t = 0; t < a.tiles; ++t) {
+        BwdItem it;
+        tile_list<DKV>(a, t, it);
+        a.head_steps += it.total;
     }
-    const long long sink_total = std::max(1LL, static_cast<long long>(sink_per) * a.group);
-    const int lo = ((-a.shift) % kTile + kTile) % kTile;  // first query row of a key tile within its query tile
-    const long long tile_per = std::min<long long>(a.q_tiles, (static_cast<long long>(lo) + kTile + a.window - 2) / kTile + 1);
-    const long long tile_total = std::max(1LL, tile_per * a.group);
-    const long long heads = static_cast<long long>(p.batch) * p.kv_heads;
-    const long long tiles = heads * (a.k_tiles - a.sink_tiles);
-    const long long sinks = heads * a.sink_tiles;
-    double best = 1e300;
-    for (int cut = 1; cut <= 32; ++cut) {
-        const long long chunk = ((tiles > 0 ? tile_total : sink_total) + cut - 1) / cut;
-        // No more parts of lists with sinks than 8 an SM: they are memory, too.
-        const long long most = std::max(1LL, 8LL * sm_count / std::max(1LL, sinks));
-        const long long sink_chunk = std::max(chunk, (sink_total + most - 1) / most);
-        const long long tile_chunks = (tile_total + chunk - 1) / chunk;
-        const long long sink_chunks = (sink_total + sink_chunk - 1) / sink_chunk;
-        const long long work = tiles * (tile_total + 2 * tile_chunks) + sinks * (sink_total + 2 * sink_chunks);
-        const long long items = tiles * tile_chunks + sinks * sink_chunks;
-        const long long item = std::min(std::max(chunk, sink_chunk), std::max(tile_total, sink_total)) + 2;
-        const double turns = static_cast<double>((items + sm_count - 1) / sm_count) * static_cast<double>(item);
-        const double even = static_cast<double>(work) / sm_count + static_cast<double>(item);
-        const double cost = std::min(turns, even) + (cut > 1 ? 1.0 : 0.0);
-        if (cost < 0.97 * best) {
-            best = cost;
-            a.tile_chunk = static_cast<int>(chunk);
-            a.sink_chunk = static_cast<int>(sink_chunk);
-            a.tile_chunks = static_cast<int>(tile_chunks);
-            a.sink_chunks = static_cast<int>(sink_chunks);
-        }
-        if (chunk <= 2) {
-            break;
-        }
-    }
+    a.steps = a.head_steps * p.batch * (DKV ? p.kv_heads : p.heads);
+    a.per = std::max<long long>(kMinSteps, (a.steps + sm_count - 1) / sm_count);
+    a.grid = static_cast<int>((a.steps + a.per - 1) / a.per);
     a.scale = p.softmax_scale;
     a.scale_log2 = static_cast<float>(static_cast<double>(p.softmax_scale) * M_LOG2E);
-    a.div_qtiles = FastDiv(a.q_tiles);
-    a.div_ktiles_rest = FastDiv(std::max(1, a.k_tiles - a.sink_tiles));
-    a.div_heads = FastDiv(a.heads);
-    a.div_kv_heads = FastDiv(a.kv_heads);
+    a.div_heads = FastDiv(DKV ? p.kv_heads : p.heads);
     a.div_group = FastDiv(a.group);
-    a.div_sink_tiles = FastDiv(std::max(1, a.sink_tiles));
-    a.div_sink_chunks = FastDiv(a.sink_chunks);
-    a.div_tile_chunks = FastDiv(a.tile_chunks);
     return a;
 }
 
-long long dkv_items(const BwdArgs& a) {
-    return static_cast<long long>(a.batch) * a.kv_heads *
-           (static_cast<long long>(a.sink_tiles) * a.sink_chunks +
-            static_cast<long long>(a.k_tiles - a.sink_tiles) * a.tile_chunks);
-}
-
-unsigned long long parts_of(const BwdArgs& a) {
-    const unsigned long long heads = static_cast<unsigned long long>(a.batch) * a.kv_heads;
-    return heads * ((a.sink_chunks > 1 ? static_cast<unsigned long long>(a.sink_tiles) * a.sink_chunks : 0) +
-                    (a.tile_chunks > 1 ? static_cast<unsigned long long>(a.k_tiles - a.sink_tiles) * a.tile_chunks : 0));
+template <bool DKV>
+unsigned long long part_bytes(const BwdArgs& a, int head_dim) {
+    return a.grid > 1 ? 2ull * a.grid * (DKV ? 2 : 1) * kTile * head_dim * 4 : 0;
 }
 
 unsigned long long delta_bytes(const FaWindowParams& p) {
@@ -900,18 +908,26 @@ cudaError_t launch_early(Kernel kernel, dim3 grid, int threads, int smem, cudaSt
 template <int D, bool BF16>
 cudaError_t bwd(const FaWindowParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count,
                 cudaStream_t stream) {
-    BwdArgs a = bwd_args(p, sm_count);
-    a.epoch = epoch;
-    a.status = status;
+    BwdArgs dkv = bwd_args<true>(p, sm_count);
+    BwdArgs dq = bwd_args<false>(p, sm_count);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
     float* delta = static_cast<float*>(workspace);
-    a.lse = p.lse;
-    a.delta = delta;
-    a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + delta_bytes(p));
-    const long long q_items = static_cast<long long>(p.batch) * p.heads * a.q_tiles;
-    const long long k_items = dkv_items(a);
+    dkv.epoch = dq.epoch = epoch;
+    dkv.status = dq.status = status;
+    dkv.lse = dq.lse = p.lse;
+    dkv.delta = dq.delta = delta;
+    dkv.parts = reinterpret_cast<float*>(ws + delta_bytes(p));
+    dq.parts = reinterpret_cast<float*>(ws + delta_bytes(p) + part_bytes<true>(dkv, D));
+    dkv.out0 = p.dv;
+    dkv.out1 = p.dk;
+    dq.out1 = p.dq;
+    auto strides = [](int64_t(&to)[3], const int64_t(&from)[3]) { std::copy(from, from + 3, to); };
+    strides(dkv.out0_stride, p.dv_stride);
+    strides(dkv.out1_stride, p.dk_stride);
+    strides(dq.out1_stride, p.dq_stride);
     const long long rows = static_cast<long long>(p.batch) * p.heads * p.q_len;
     const long long delta_grid = (rows * (D / 8) + 255) / 256;
-    if (q_items > 0x7fffffffLL || k_items > 0x7fffffffLL || delta_grid > 0x7fffffffLL) {
+    if (delta_grid > 0x7fffffffLL) {
         return cudaErrorInvalidConfiguration;
     }
     CUtensorMap q, k, v, d_o;
@@ -935,34 +951,25 @@ cudaError_t bwd(const FaWindowParams& p, DeviceStatus* status, unsigned epoch, v
     if (err != cudaSuccess) {
         return err;
     }
-    auto strides = [](int64_t(&to)[3], const int64_t(&from)[3]) { std::copy(from, from + 3, to); };
-    a.items = static_cast<int>(k_items);
-    a.out0 = p.dv;
-    a.out1 = p.dk;
-    strides(a.out0_stride, p.dv_stride);
-    strides(a.out1_stride, p.dk_stride);
-    err = launch_early(window_bwd_kernel<Dkv>, dim3(static_cast<unsigned>(std::min<long long>(k_items, sm_count))),
-                       kBwdThreads, bwd_smem<Dkv>(), stream, k, v, q, d_o, a);
-    if (err == cudaSuccess && parts_of(a) > 0) {
-        err = launch_early(window_bwd_join_kernel<D, BF16>,
-                           dim3(static_cast<unsigned>(a.k_tiles), static_cast<unsigned>(p.batch * p.kv_heads), 2), 256, 0,
-                           stream, a);
+    err = launch_early(window_bwd_kernel<Dkv>, dim3(static_cast<unsigned>(dkv.grid)), kBwdThreads, bwd_smem<Dkv>(),
+                       stream, k, v, q, d_o, dkv);
+    if (err == cudaSuccess) {
+        err = launch_early(window_bwd_kernel<Dq>, dim3(static_cast<unsigned>(dq.grid)), kBwdThreads, bwd_smem<Dq>(),
+                           stream, q, d_o, k, v, dq);
     }
-    if (err != cudaSuccess) {
-        return err;
+    const int cuts = dkv.grid + dq.grid - 2;
+    if (err == cudaSuccess && cuts > 0) {
+        err = launch_early(window_bwd_join_kernel<D, BF16>, dim3(static_cast<unsigned>(cuts), 8), kJoinThreads, 0, stream,
+                           dkv, dq);
     }
-    a.items = static_cast<int>(q_items);
-    a.out0 = nullptr;
-    a.out1 = p.dq;
-    strides(a.out1_stride, p.dq_stride);
-    return launch_early(window_bwd_kernel<Dq>, dim3(static_cast<unsigned>(std::min<long long>(q_items, sm_count))),
-                        kBwdThreads, bwd_smem<Dq>(), stream, q, d_o, k, v, a);
+    return err;
 }
 
 }  // namespace
 
 unsigned long long window_bwd_workspace_bytes(const FaWindowParams& p, int sm_count) {
-    return delta_bytes(p) + parts_of(bwd_args(p, sm_count)) * 2 * kTile * p.head_dim * 4;
+    return delta_bytes(p) + part_bytes<true>(bwd_args<true>(p, sm_count), p.head_dim) +
+           part_bytes<false>(bwd_args<false>(p, sm_count), p.head_dim);
 }
 
 cudaError_t launch_window_bwd(const FaWindowParams& p, DeviceStatus* status, unsigned epoch, void* workspace,
