@@ -272,7 +272,7 @@ __device__ __forceinline__ void issue_product(uint32_t acc, uint32_t w, uint64_t
 #pragma unroll
     for (int k = 0; k < kTile / 16; ++k) {
         umma_ts(acc, w + (k / 4) * Cfg::kTmemHalf + (k % 4) * 8, t + static_cast<uint64_t>(k * (2048 >> 4)), idesc,
-                (first && k == 0) ? 0u : 1u);
+                     (first && k == 0) ? 0u : 1u);
     }
 }
 
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     constexpr int D = Cfg::D;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     BwdShared& sh = *reinterpret_cast<BwdShared*>(smem_raw + Cfg::kSmemShared);
-    const int warp = static_cast<int>(threadIdx.x) / 32;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) / 32, 0);
     const int lane = static_cast<int>(threadIdx.x) % 32;
     const uint32_t smem = smem_u32(smem_raw);
     if ((smem & 1023u) != 0) {  // the swizzled layouts need it; the driver places the window so
@@ -338,11 +338,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sh.tmem_base;
+    // Owning all 512 columns means owning them from 0: a constant, like the shared-memory addresses.
+    constexpr uint32_t tmem = 0;
+    if (sh.tmem_base != tmem) {
+        if (threadIdx.x == 0) {
+            atomicOr(&args.status->code, kStatusTimeoutTeardown);
+        }
+        __syncthreads();
+        if (warp == kMmaWarp) {
+            tmem_dealloc(sh.tmem_base, Cfg::kTmemCols);
+        }
+        return;
+    }
     Cursor cursor;
     cursor.bx = first_head;
-    cursor.tile = sh.tile;
-    cursor.offset = sh.offset;
+    cursor.tile = __shfl_sync(0xffffffffu, sh.tile, 0);  // the same in all lanes, known to be
+    cursor.offset = __shfl_sync(0xffffffffu, sh.offset, 0);
     cursor.left = min(args.per, args.steps - start);
     cursor.record = 2 * static_cast<long long>(blockIdx.x);
     // The kernel before this one in the stream wrote delta.
@@ -611,7 +622,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         __syncwarp();
     } else if (warp == kMmaWarp) {
         // ================================= MMA issuer ==================================
-        if (lane == 0) {
+        // The whole warp walks in step, one elected lane issues.
+        {
             bool ok = true;
             int g = 0;
             int items = 0;
@@ -623,18 +635,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             const uint64_t yn = make_desc_mnmajor_sw128(smem + Cfg::kSmemY, kBox);
             auto off = [](int stage) { return static_cast<uint64_t>(stage * (Cfg::kTileBytes >> 4)); };
             auto wait = [&](uint64_t* bar, int parity) {
-                return mbar_wait(smem_u32(bar), parity & 1, wctx, kStatusTimeoutMma);
+                return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity & 1, wctx, kStatusTimeoutMma)) != 0;
             };
             auto scores = [&](int at, bool last) {  // S of streamed tile `at`
                 if (!wait(&sh.x_full[at % kXStages], at / kXStages)) {
                     return false;
                 }
                 tc_fence_after();
-                issue_scores<Cfg>(tmem + Cfg::kTmemS, r0, xk + off(at % kXStages));
-                umma_commit(smem_u32(&sh.s_full));
-                if (last) {
-                    umma_commit(smem_u32(&sh.r0_empty));
+                const uint64_t x = xk + off(at % kXStages);
+                if (elect_one()) {
+                    issue_scores<Cfg>(tmem + Cfg::kTmemS, r0, x);
+                    umma_commit(smem_u32(&sh.s_full));
+                    if (last) {
+                        umma_commit(smem_u32(&sh.r0_empty));
+                    }
                 }
+                __syncwarp();
                 return true;
             };
             auto dscores = [&](int at, bool last) {  // dP
@@ -642,14 +658,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                     return false;
                 }
                 tc_fence_after();
-                issue_scores<Cfg>(tmem + Cfg::kTmemDP, r1, yk + off(at % kYStages));
-                umma_commit(smem_u32(&sh.dp_full));
-                if (!Cfg::DKV) {
-                    umma_commit(smem_u32(&sh.y_empty[at % kYStages]));
+                const uint64_t y = yk + off(at % kYStages);
+                if (elect_one()) {
+                    issue_scores<Cfg>(tmem + Cfg::kTmemDP, r1, y);
+                    umma_commit(smem_u32(&sh.dp_full));
+                    if (!Cfg::DKV) {
+                        umma_commit(smem_u32(&sh.y_empty[at % kYStages]));
+                    }
+                    if (last) {
+                        umma_commit(smem_u32(&sh.r1_empty));
+                    }
                 }
-                if (last) {
-                    umma_commit(smem_u32(&sh.r1_empty));
-                }
+                __syncwarp();
                 return true;
             };
             BwdItem it;
@@ -672,25 +692,36 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                     }
                     tc_fence_after();
                     if constexpr (Cfg::DKV) {
-                        issue_product<Cfg>(tmem + Cfg::kTmemAcc0, tmem + Cfg::kTmemP, yn + off(g % kYStages), i == 0);
-                        umma_commit(smem_u32(&sh.y_empty[g % kYStages]));
+                        const uint64_t y = yn + off(g % kYStages);
+                        if (elect_one()) {
+                            issue_product<Cfg>(tmem + Cfg::kTmemAcc0, tmem + Cfg::kTmemP, y, i == 0);
+                            umma_commit(smem_u32(&sh.y_empty[g % kYStages]));
+                        }
+                        __syncwarp();
                     }
                     ok = (!more || scores(g + 1, last)) && wait(&sh.ds_full, g);
                     if (!ok) {
                         break;
                     }
                     tc_fence_after();
-                    issue_product<Cfg>(tmem + Cfg::kTmemAcc1, tmem + Cfg::kTmemDS, xn + off(g % kXStages), i == 0);
-                    umma_commit(smem_u32(&sh.x_empty[g % kXStages]));
-                    if (!more) {
-                        umma_commit(smem_u32(&sh.acc_done));
+                    const uint64_t x = xn + off(g % kXStages);
+                    if (elect_one()) {
+                        issue_product<Cfg>(tmem + Cfg::kTmemAcc1, tmem + Cfg::kTmemDS, x, i == 0);
+                        umma_commit(smem_u32(&sh.x_empty[g % kXStages]));
+                        if (!more) {
+                            umma_commit(smem_u32(&sh.acc_done));
+                        }
                     }
+                    __syncwarp();
                     ok = !more || dscores(g + 1, last);
                 }
                 ++items;
             }
             // Every MMA issued above must be complete before tensor memory is released.
-            umma_commit(smem_u32(&sh.mma_idle));
+            if (elect_one()) {
+                umma_commit(smem_u32(&sh.mma_idle));
+            }
+            __syncwarp();
             mbar_wait_drain(smem_u32(&sh.mma_idle), 0, wctx, kStatusTimeoutTeardown);
         }
         __syncwarp();
