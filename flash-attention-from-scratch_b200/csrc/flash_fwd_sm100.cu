@@ -317,7 +317,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     __shared__ SharedBarriers sb;
 
-    const int warp = static_cast<int>(threadIdx.x) / 32;
+    // WIN: known to be the same in all lanes of a warp.
+    const int warp = Cfg::WIN ? __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) / 32, 0)
+                              : static_cast<int>(threadIdx.x) / 32;
     const int lane = static_cast<int>(threadIdx.x) % 32;
 
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -503,7 +505,33 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sb.tmem_base;
+    // WIN: owning all 512 columns means owning them from 0, a constant for the products' operands.
+    const uint32_t tmem = Cfg::WIN ? 0u : sb.tmem_base;
+    if (Cfg::WIN && sb.tmem_base != 0) {
+        if (threadIdx.x == 0) {
+            atomicOr(&args.status->code, kStatusTimeoutTeardown);
+        }
+        __syncthreads();
+        if (warp == Cfg::kMmaWarp) {
+            tmem_dealloc(sb.tmem_base, Cfg::kTmemCols);
+        }
+        return;
+    }
+    // The MMA issuers. WIN: a whole warp walks in step and one elected lane issues; else one thread does all.
+    auto issuer_wait = [&](uint32_t bar, uint32_t parity) -> bool {
+        const bool there = mbar_wait(bar, parity, wctx, kStatusTimeoutMma);
+        return Cfg::WIN ? __all_sync(0xffffffffu, there) != 0 : there;
+    };
+    auto issue = [&](auto products) {
+        if constexpr (Cfg::WIN) {
+            if (elect_one()) {
+                products();
+            }
+            __syncwarp();
+        } else {
+            products();
+        }
+    };
 
     if constexpr (NQ == 2 && Cfg::kRegsSoftmax != 0) {
         if (warp < Cfg::kSoftmaxWarps) {
@@ -1115,7 +1143,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         // issuer) and issues only tile t's MMAs. It waits for every slot to land before it
         // releases it, even one its tile does not read, so it can never release a later use
         // of a slot before the producer has filled the current one.
-        if (lane == 0) {
+        if (Cfg::WIN || lane == 0) {
             const int t = (warp == Cfg::kMmaWarp) ? 0 : 1;
             bool ok = true;
             const uint32_t kv_addr0 = smem_base + Cfg::kSmemKV;
@@ -1147,33 +1175,34 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 const int last_j = Cfg::WIN ? mine.last : n_t - 1;
                 bool pv_first = true;
                 if (n_t > 0) {
-                    ok = mbar_wait(smem_u32(&sb.q_full[t]), q_uses & 1, wctx, kStatusTimeoutMma);
+                    ok = issuer_wait(smem_u32(&sb.q_full[t]), q_uses & 1);
                     ++q_uses;
                 }
                 if (ok && n_max > 0) {
                     const int k_slot = ring++;
-                    ok = mbar_wait(smem_u32(&sb.kv_full[k_slot % STAGES]), (k_slot / STAGES) & 1, wctx,
-                                   kStatusTimeoutMma);
+                    ok = issuer_wait(smem_u32(&sb.kv_full[k_slot % STAGES]), (k_slot / STAGES) & 1);
                     if (ok && has(0)) {
                         if constexpr (Cfg::SEP_P) {
                             // The softmax has the previous item's last S_t in registers.
                             if (s_cnt > 0) {
-                                ok = mbar_wait(smem_u32(&sb.s_free[t]), (s_cnt - 1) & 1, wctx,
-                                               kStatusTimeoutMma);
+                                ok = issuer_wait(smem_u32(&sb.s_free[t]), (s_cnt - 1) & 1);
                             }
                         }
                         if (ok) {
                             tc_fence_after();
-                            issue_s_mma<Cfg>(s_addr, qd, kd0 + stage_off(k_slot % STAGES));
-                            umma_commit(smem_u32(&sb.s_full[t]));
-                            if (last_j == 0) {
-                                umma_commit(smem_u32(&sb.q_empty[t]));  // Q_t read for the last time
-                            }
+                            const uint64_t kd = kd0 + stage_off(k_slot % STAGES);
+                            issue([&] {
+                                issue_s_mma<Cfg>(s_addr, qd, kd);
+                                umma_commit(smem_u32(&sb.s_full[t]));
+                                if (last_j == 0) {
+                                    umma_commit(smem_u32(&sb.q_empty[t]));  // Q_t read for the last time
+                                }
+                            });
                             ++s_cnt;
                         }
                     }
                     if (ok) {
-                        umma_commit(smem_u32(&sb.kv_empty[k_slot % STAGES]));
+                        issue([&] { umma_commit(smem_u32(&sb.kv_empty[k_slot % STAGES])); });
                     }
                 }
                 for (int j = 0; ok && j < n_max; ++j) {
@@ -1190,38 +1219,42 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                             // S_t(j+1) as soon as the softmax has S_t(j) in registers.
                             if (next_s) {
                                 ok = s_cnt == 0 ||
-                                     mbar_wait(smem_u32(&sb.s_free[t]), (s_cnt - 1) & 1, wctx, kStatusTimeoutMma);
-                                ok = ok && mbar_wait(smem_u32(&sb.kv_full[ks]), (k_slot / STAGES) & 1, wctx,
-                                                     kStatusTimeoutMma);
+                                     issuer_wait(smem_u32(&sb.s_free[t]), (s_cnt - 1) & 1);
+                                ok = ok && issuer_wait(smem_u32(&sb.kv_full[ks]), (k_slot / STAGES) & 1);
                                 if (!ok) {
                                     break;
                                 }
                                 k_ready = true;
                                 tc_fence_after();
-                                issue_s_mma<Cfg>(s_addr, qd, kd0 + stage_off(ks));
-                                umma_commit(smem_u32(&sb.s_full[t]));
-                                if (j + 1 == last_j) {
-                                    umma_commit(smem_u32(&sb.q_empty[t]));
-                                }
+                                const uint64_t kd = kd0 + stage_off(ks);
+                                issue([&] {
+                                    issue_s_mma<Cfg>(s_addr, qd, kd);
+                                    umma_commit(smem_u32(&sb.s_full[t]));
+                                    if (j + 1 == last_j) {
+                                        umma_commit(smem_u32(&sb.q_empty[t]));
+                                    }
+                                });
                                 ++s_cnt;
                             }
                         }
                         if (active) {
-                            ok = mbar_wait(smem_u32(&sb.p_full[t]), pv_cnt & 1, wctx, kStatusTimeoutMma);
+                            ok = issuer_wait(smem_u32(&sb.p_full[t]), pv_cnt & 1);
                         }
-                        ok = ok && mbar_wait(smem_u32(&sb.kv_full[vs]), (v_slot / STAGES) & 1, wctx,
-                                             kStatusTimeoutMma);
+                        ok = ok && issuer_wait(smem_u32(&sb.kv_full[vs]), (v_slot / STAGES) & 1);
                         if (!ok) {
                             break;
                         }
                         tc_fence_after();
                         if (active) {
-                            if constexpr (Cfg::ACC16) {
-                                issue_pv_mma_f16<Cfg>(tmem + Cfg::tmem_t(t), p_addr, vd0 + stage_off(vs));
-                            } else {
-                                issue_pv_mma_f32<Cfg>(o_addr, p_addr, vd0 + stage_off(vs), pv_first);
-                            }
-                            umma_commit(smem_u32(&sb.o_done[t]));
+                            const uint64_t vd = vd0 + stage_off(vs);
+                            issue([&] {
+                                if constexpr (Cfg::ACC16) {
+                                    issue_pv_mma_f16<Cfg>(tmem + Cfg::tmem_t(t), p_addr, vd);
+                                } else {
+                                    issue_pv_mma_f32<Cfg>(o_addr, p_addr, vd, pv_first);
+                                }
+                                umma_commit(smem_u32(&sb.o_done[t]));
+                            });
                             ++pv_cnt;
                             pv_first = false;
                         }
@@ -1229,40 +1262,42 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                             // S_t(j+1) reuses the columns P_t(j) was read from by the MMAs above
                             // (tcgen05.mma operations of one thread execute in issue order).
                             if (next_s) {
-                                ok = mbar_wait(smem_u32(&sb.kv_full[ks]), (k_slot / STAGES) & 1, wctx,
-                                                     kStatusTimeoutMma);
+                                ok = issuer_wait(smem_u32(&sb.kv_full[ks]), (k_slot / STAGES) & 1);
                                 if (!ok) {
                                     break;
                                 }
                                 k_ready = true;
                                 tc_fence_after();
-                                issue_s_mma<Cfg>(s_addr, qd, kd0 + stage_off(ks));
-                                umma_commit(smem_u32(&sb.s_full[t]));
-                                if (j + 1 == last_j) {
-                                    umma_commit(smem_u32(&sb.q_empty[t]));
-                                }
+                                const uint64_t kd = kd0 + stage_off(ks);
+                                issue([&] {
+                                    issue_s_mma<Cfg>(s_addr, qd, kd);
+                                    umma_commit(smem_u32(&sb.s_full[t]));
+                                    if (j + 1 == last_j) {
+                                        umma_commit(smem_u32(&sb.q_empty[t]));
+                                    }
+                                });
                                 ++s_cnt;
                             }
                         }
                     } else {
-                        ok = mbar_wait(smem_u32(&sb.kv_full[vs]), (v_slot / STAGES) & 1, wctx,
-                                       kStatusTimeoutMma);
+                        ok = issuer_wait(smem_u32(&sb.kv_full[vs]), (v_slot / STAGES) & 1);
                     }
                     if (ok && has_next && !k_ready) {
-                        ok = mbar_wait(smem_u32(&sb.kv_full[ks]), (k_slot / STAGES) & 1, wctx,
-                                       kStatusTimeoutMma);
+                        ok = issuer_wait(smem_u32(&sb.kv_full[ks]), (k_slot / STAGES) & 1);
                     }
                     if (!ok) {
                         break;
                     }
-                    umma_commit(smem_u32(&sb.kv_empty[vs]));
-                    if (has_next) {
-                        umma_commit(smem_u32(&sb.kv_empty[ks]));
-                    }
+                    issue([&] {
+                        umma_commit(smem_u32(&sb.kv_empty[vs]));
+                        if (has_next) {
+                            umma_commit(smem_u32(&sb.kv_empty[ks]));
+                        }
+                    });
                 }
             }
             // Every MMA issued above must be complete before tensor memory is released.
-            umma_commit(smem_u32(&sb.mma_idle));
+            issue([&] { umma_commit(smem_u32(&sb.mma_idle)); });
             mbar_wait_drain(smem_u32(&sb.mma_idle), 0, wctx, kStatusTimeoutTeardown);
         }
         __syncwarp();
@@ -1350,7 +1385,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         __syncwarp();
     } else if (Cfg::kIssuers == 1 && Cfg::kSBufs == 1 && warp == Cfg::kMmaWarp) {
         // ================================== MMA issuer ====================================
-        if (lane == 0) {
+        if (Cfg::WIN || lane == 0) {
             bool ok = true;
             const uint32_t q_addr0 = smem_base + Cfg::kSmemQ;
             const uint32_t kv_addr0 = smem_base + Cfg::kSmemKV;
@@ -1377,16 +1412,20 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             auto issue_s = [&](int t, int ks, bool last_of_item) -> bool {
                 if constexpr (Cfg::SEP_P) {
                     if (s_cnt[t] > 0 &&
-                        !mbar_wait(smem_u32(&sb.s_free[t]), (s_cnt[t] - 1) & 1, wctx, kStatusTimeoutMma)) {
+                        !issuer_wait(smem_u32(&sb.s_free[t]), (s_cnt[t] - 1) & 1)) {
                         return false;
                     }
                 }
                 tc_fence_after();
-                issue_s_mma<Cfg>(tmem + Cfg::kTmemS + t * kBN, q_desc(t), kd0 + stage_off(ks));
-                umma_commit(smem_u32(&sb.s_full[t]));
-                if (last_of_item) {
-                    umma_commit(smem_u32(&sb.q_empty[t]));  // Q_t read for the last time
-                }
+                const uint64_t qd = q_desc(t);
+                const uint64_t kd = kd0 + stage_off(ks);
+                issue([&] {
+                    issue_s_mma<Cfg>(tmem + Cfg::kTmemS + t * kBN, qd, kd);
+                    umma_commit(smem_u32(&sb.s_full[t]));
+                    if (last_of_item) {
+                        umma_commit(smem_u32(&sb.q_empty[t]));  // Q_t read for the last time
+                    }
+                });
                 ++s_cnt[t];
                 return true;
             };
@@ -1408,7 +1447,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                     pv_first[t] = true;
                     mine[t] = places_of(it, t);
                     if (ok && it.n_kv[t] > 0) {
-                        ok = mbar_wait(smem_u32(&sb.q_full[t]), q_uses[t] & 1, wctx, kStatusTimeoutMma);
+                        ok = issuer_wait(smem_u32(&sb.q_full[t]), q_uses[t] & 1);
                         ++q_uses[t];
                     }
                 }
@@ -1416,8 +1455,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                     // S_t(0) of every tile of the item: each follows the previous item's last
                     // P.V_t in issue order (P_t of that tile lay in S_t's columns).
                     const int k_slot = ring++;
-                    ok = mbar_wait(smem_u32(&sb.kv_full[k_slot % STAGES]), (k_slot / STAGES) & 1, wctx,
-                                   kStatusTimeoutMma);
+                    ok = issuer_wait(smem_u32(&sb.kv_full[k_slot % STAGES]), (k_slot / STAGES) & 1);
 #pragma unroll
                     for (int t = 0; t < NQ; ++t) {
                         if (ok && has(t, 0)) {
@@ -1425,7 +1463,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                         }
                     }
                     if (ok) {
-                        umma_commit(smem_u32(&sb.kv_empty[k_slot % STAGES]));
+                        issue([&] { umma_commit(smem_u32(&sb.kv_empty[k_slot % STAGES])); });
                     }
                 }
                 for (int j = 0; ok && j < n_max; ++j) {
@@ -1448,8 +1486,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                             // S_t(j+1) as soon as the softmax has S_t(j) in registers.
                             if (next_s) {
                                 if (!k_ready) {
-                                    ok = mbar_wait(smem_u32(&sb.kv_full[ks]), (k_slot / STAGES) & 1,
-                                                   wctx, kStatusTimeoutMma);
+                                    ok = issuer_wait(smem_u32(&sb.kv_full[ks]), (k_slot / STAGES) & 1);
                                     k_ready = true;
                                 }
                                 ok = ok && issue_s(t, ks, j + 1 == last_j(t));
@@ -1459,11 +1496,10 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                             }
                         }
                         if (active) {
-                            ok = mbar_wait(smem_u32(&sb.p_full[t]), pv_cnt[t] & 1, wctx, kStatusTimeoutMma);
+                            ok = issuer_wait(smem_u32(&sb.p_full[t]), pv_cnt[t] & 1);
                         }
                         if (ok && !v_ready) {
-                            ok = mbar_wait(smem_u32(&sb.kv_full[vs]), (v_slot / STAGES) & 1, wctx,
-                                           kStatusTimeoutMma);
+                            ok = issuer_wait(smem_u32(&sb.kv_full[vs]), (v_slot / STAGES) & 1);
                             v_ready = true;
                         }
                         if (!ok) {
@@ -1472,15 +1508,17 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                         tc_fence_after();
                         if (active) {
                             const uint64_t vd = vd0 + stage_off(vs);
-                            if constexpr (Cfg::ACC16) {
-                                issue_pv_mma_f16<Cfg>(tmem + Cfg::tmem_t(t), s_addr, vd);
-                            } else if constexpr (Cfg::SEP_P) {
-                                issue_pv_mma_f32<Cfg>(tmem + Cfg::kTmemO + t * Cfg::D,
-                                                      tmem + Cfg::kTmemExtra + t * 64, vd, pv_first[t]);
-                            } else {
-                                issue_pv_mma_f32<Cfg>(tmem + Cfg::kTmemO + t * Cfg::D, s_addr, vd, pv_first[t]);
-                            }
-                            umma_commit(smem_u32(&sb.o_done[t]));
+                            issue([&] {
+                                if constexpr (Cfg::ACC16) {
+                                    issue_pv_mma_f16<Cfg>(tmem + Cfg::tmem_t(t), s_addr, vd);
+                                } else if constexpr (Cfg::SEP_P) {
+                                    issue_pv_mma_f32<Cfg>(tmem + Cfg::kTmemO + t * Cfg::D,
+                                                          tmem + Cfg::kTmemExtra + t * 64, vd, pv_first[t]);
+                                } else {
+                                    issue_pv_mma_f32<Cfg>(tmem + Cfg::kTmemO + t * Cfg::D, s_addr, vd, pv_first[t]);
+                                }
+                                umma_commit(smem_u32(&sb.o_done[t]));
+                            });
                             ++pv_cnt[t];
                             pv_first[t] = false;
                         }
@@ -1488,8 +1526,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                             // S_t(j+1) reuses the columns P_t(j) was read from by the MMAs above.
                             if (next_s) {
                                 if (!k_ready) {
-                                    ok = mbar_wait(smem_u32(&sb.kv_full[ks]), (k_slot / STAGES) & 1,
-                                                   wctx, kStatusTimeoutMma);
+                                    ok = issuer_wait(smem_u32(&sb.kv_full[ks]), (k_slot / STAGES) & 1);
                                     k_ready = true;
                                 }
                                 ok = ok && issue_s(t, ks, j + 1 == last_j(t));
@@ -1502,14 +1539,16 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                     if (!ok) {
                         break;
                     }
-                    umma_commit(smem_u32(&sb.kv_empty[vs]));
-                    if (has_next) {
-                        umma_commit(smem_u32(&sb.kv_empty[ks]));
-                    }
+                    issue([&] {
+                        umma_commit(smem_u32(&sb.kv_empty[vs]));
+                        if (has_next) {
+                            umma_commit(smem_u32(&sb.kv_empty[ks]));
+                        }
+                    });
                 }
             }
             // Every MMA issued above must be complete before tensor memory is released.
-            umma_commit(smem_u32(&sb.mma_idle));
+            issue([&] { umma_commit(smem_u32(&sb.mma_idle)); });
             mbar_wait_drain(smem_u32(&sb.mma_idle), 0, wctx, kStatusTimeoutTeardown);
         }
         __syncwarp();
