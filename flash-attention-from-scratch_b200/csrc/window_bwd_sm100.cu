@@ -14,10 +14,12 @@
 //   dQ            Q   dO  K  V    Q K^T        dO V^T                       dQ += dS X
 //
 // Tensor memory (columns): S 0..127, dP 128..255, the products' accumulators from 256. P and dS are
-// 16-bit matrix operands read from tensor memory: each lies over the float32 values it was made
-// of, in the half of the columns its own warpgroup has read.
-// The tensor pipe is kept busy by the order of issue: P(i) in hand -> dV(i), S(i+1); dS(i) in hand ->
-// dK(i), dP(i+1). The exponentials of a tile run under the products of dS of the one before.
+// 16-bit matrix operands read from tensor memory. dQ has room for two dS of its own. DKV with d =
+// 128 has none left: P(i) lies in the first half of dP's columns until dV(i) has read it, then dP(i) takes
+// them all, and once every warp has read dP(i), dS(i) goes to the second half and P(i + 1) to the first.
+// The tensor pipe is kept busy by the order of issue. DKV: S(i + 1) as soon as S(i) is in registers; with
+// P(i) and dS(i - 1) in hand dV(i), dK(i - 1), dP(i), under which the exponentials of tile i + 1 run. dQ: S(i + 1) as
+// early, and with dS(i) in hand dP(i + 1), dQ(i).
 //
 // Warps: two warpgroups share a tile's 128 x 128 scores, 64 columns each (thread = row); a third
 // has the TMA producer, the MMA issuer and (DKV) the loader of LSE and delta of the streamed rows. Every
@@ -59,7 +61,7 @@ constexpr int kLoaderWarp = 10;
 constexpr int kRegsSoftmax = 208;
 constexpr int kRegsOther = 88;
 static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kBwdThreads * 168, "register split");
-constexpr int kEmuPer8 = 2;  // column pairs of 8 whose 2^x runs on the FMA pipe
+constexpr int kEmuPer8 = 3;  // column pairs of 8 whose 2^x runs on the FMA pipe (1: 2% slower, 4: the same)
 
 struct BwdArgs {
     int batch, heads, kv_heads, group;
@@ -97,11 +99,11 @@ struct BwdCfg {
     static constexpr int kTmemDP = 128;
     static constexpr int kTmemAcc0 = 256;              // DKV: dV
     static constexpr int kTmemAcc1 = DKV ? 256 + D : 256;  // dK or dQ
-    // d = 128: P over S and dS over dP, each half in its warpgroup's columns (products of one shape run
-    // in issue order). d = 64: columns of their own, since the two kinds of product differ in shape there.
-    static constexpr int kTmemP = D == 128 ? kTmemS : 384;
-    static constexpr int kTmemDS = D == 128 ? kTmemDP : 448;
-    static constexpr int kTmemHalf = D == 128 ? 64 : 32;  // columns between the halves
+    // Columns of the 16-bit operands (64 each): DKV with d = 128 over dP's (see above).
+    static constexpr bool kOverDP = DKV && D == 128;
+    static constexpr int kTmemP = kOverDP ? kTmemDP : 384;
+    static constexpr int kTmemDS = kOverDP ? kTmemDP + 64 : (DKV ? 448 : 384);
+    static constexpr int kTmemDS2 = DKV ? kTmemDS : 448;  // of odd tiles
     static constexpr int kTmemCols = 512;
 };
 
@@ -109,13 +111,15 @@ struct BwdShared {
     uint64_t r0_full, r0_empty, r1_full, r1_empty;
     uint64_t x_full[kXStages], x_empty[kXStages];
     uint64_t y_full[kYStages], y_empty[kYStages];
-    uint64_t s_full, p_full, dp_full, ds_full, acc_done, acc_free, mma_idle;
+    uint64_t lse_free[2];
+    uint64_t s_full, s_read, dp_full, ds_full, acc_done, acc_free, mma_idle;
     uint32_t tmem_base;
     int abort;
     int tile, offset;  // where the CTA's range starts
     long long warp_sum[kBwdThreads / 32];
-    alignas(16) float lse2[2][kTile];   // DKV: of the streamed rows, log2 units; +inf: P = 0
-    alignas(16) float delta[2][kTile];
+    // DKV: of the streamed rows: minus LSE in log2 units (-inf: P = 0), minus delta.
+    alignas(16) float lse2[2][kTile];
+    alignas(16) float delta[kXStages][kTile];
 };
 
 // No static shared memory: the tiles start the dynamic window, 1024-byte aligned, and with d = 128 leave
@@ -264,14 +268,14 @@ __device__ __forceinline__ void issue_scores(uint32_t d, uint64_t a, uint64_t b)
     }
 }
 
-// acc (128 x D) += W T: W (128 x 128, 16-bit) in tensor memory, its columns 0..63 from `w`, 64..127 from
-// w + kTmemHalf; T the 128 rows of a streamed tile.
+// acc (128 x D) += W T: W (128 x 128, 16-bit) in tensor memory, 64 columns from `w`; T the 128 rows of a
+// streamed tile.
 template <class Cfg>
 __device__ __forceinline__ void issue_product(uint32_t acc, uint32_t w, uint64_t t, bool first) {
     constexpr uint32_t idesc = make_idesc_f16(kTile, Cfg::D, true, true, Cfg::BF16);
 #pragma unroll
     for (int k = 0; k < kTile / 16; ++k) {
-        umma_ts(acc, w + (k / 4) * Cfg::kTmemHalf + (k % 4) * 8, t + static_cast<uint64_t>(k * (2048 >> 4)), idesc,
+        umma_ts(acc, w + k * 8, t + static_cast<uint64_t>(k * (2048 >> 4)), idesc,
                      (first && k == 0) ? 0u : 1u);
     }
 }
@@ -321,8 +325,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             mbar_init(smem_u32(&sh.y_full[s]), 1);
             mbar_init(smem_u32(&sh.y_empty[s]), 1);
         }
+        mbar_init(smem_u32(&sh.lse_free[0]), kSoftmaxWarps);
+        mbar_init(smem_u32(&sh.lse_free[1]), kSoftmaxWarps);
         mbar_init(smem_u32(&sh.s_full), 1);
-        mbar_init(smem_u32(&sh.p_full), kSoftmaxWarps);
+        mbar_init(smem_u32(&sh.s_read), kSoftmaxWarps);
         mbar_init(smem_u32(&sh.dp_full), 1);
         mbar_init(smem_u32(&sh.ds_full), kSoftmaxWarps);
         mbar_init(smem_u32(&sh.acc_done), 1);
@@ -356,8 +362,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     cursor.offset = __shfl_sync(0xffffffffu, sh.offset, 0);
     cursor.left = min(args.per, args.steps - start);
     cursor.record = 2 * static_cast<long long>(blockIdx.x);
-    // The kernel before this one in the stream wrote delta.
-    cudaGridDependencySynchronize();
+    if constexpr (Cfg::DKV) {
+        cudaGridDependencySynchronize();  // delta is there
+        cudaTriggerProgrammaticLaunchCompletion();  // the dQ pass may take SMs as they get free
+    }
 
     if (warp < kSoftmaxWarps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
@@ -373,24 +381,32 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
         const uint32_t t_s = tmem + lanes + Cfg::kTmemS + col0;
         const uint32_t t_dp = tmem + lanes + Cfg::kTmemDP + col0;
-        const uint32_t t_p = tmem + lanes + Cfg::kTmemP + wg * Cfg::kTmemHalf;
-        const uint32_t t_ds = tmem + lanes + Cfg::kTmemDS + wg * Cfg::kTmemHalf;
+        const uint32_t t_p = tmem + lanes + Cfg::kTmemP + wg * 32;
+        const uint32_t t_ds = tmem + lanes + Cfg::kTmemDS + wg * 32;
         const float scale_log2 = args.scale_log2;
-        int g = 0;      // streamed tiles so far
+        int g = 0;      // streamed tiles whose S was read so far
+        int gd = 0;     // ... whose dP was
         int done = 0;   // accumulations read out so far
         bool ok = true;
+        auto arrive = [&](uint64_t* bar) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(smem_u32(bar));
+            }
+        };
         BwdItem it, next;
         bool more = next_item<Cfg::DKV>(args, cursor, next);
         float next_lse2, next_delta;
-        auto statistics = [&]() {  // dQ: of this thread's row of the next item
-            next_lse2 = INFINITY;
+        auto statistics = [&]() {  // dQ: of this thread's row of the next item, negated
+            next_lse2 = -INFINITY;
             next_delta = 0.0f;
             if (!Cfg::DKV && more && next.row0 + row < args.q_len) {
                 const long long at =
                     (static_cast<long long>(next.b) * args.heads + next.head) * args.q_len + next.row0 + row;
                 const float lse = __ldg(args.lse + at);
-                next_lse2 = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
-                next_delta = __ldg(args.delta + at);
+                next_lse2 = lse == -INFINITY ? -INFINITY : lse * -1.4426950408889634f;
+                next_delta = -__ldg(args.delta + at);
             }
         };
         statistics();
@@ -400,40 +416,29 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             const float row_delta = next_delta;
             more = next_item<Cfg::DKV>(args, cursor, next);
             statistics();
-            for (int i = 0; i < it.n; ++i, ++g) {
+            // P of tile i (DKV: packed; dQ: fp32 bits) from S.
+            auto probabilities = [&](int i, uint32_t (&p)[64]) {
                 int tile_row, head;
                 stream_tile<Cfg>(args, it, i, tile_row, head);
                 ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.s_full), g & 1, wctx, kStatusTimeoutSoftmax));
                 if (!ok) {
-                    continue;
+                    return;
                 }
                 tc_fence_after();
-                uint32_t p[64];
                 tmem_ld64(t_s, p);
                 tmem_wait_ld();
-                if constexpr (!Cfg::DKV) {
-                    // S is in registers: the next scores may take its columns.
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(smem_u32(&sh.p_full));
-                    }
-                }
-                const int slot = g % 2;
-                // Masks: query position minus key position in [0, window), or the key a sink.
-                const int q_row = Cfg::DKV ? tile_row : it.row0;
-                const int k_row = Cfg::DKV ? it.row0 : tile_row;
-                const int gap = q_row + args.shift - k_row;  // of the tiles' first rows
-                const bool masked = gap < kTile - 1 || (gap + kTile - 1 >= args.window && k_row + kTile > args.sinks);
-                float2 neg[4];
+                // S is in registers: the next scores may take its columns.
+                arrive(&sh.s_read);
+                [[maybe_unused]] const float* lse2 = sh.lse2[g % 2] + col0;
 #pragma unroll
                 for (int c4 = 0; c4 < 16; ++c4) {
+                    float2 neg[2];
                     if constexpr (Cfg::DKV) {
-                        const float4 l4 = *reinterpret_cast<const float4*>(&sh.lse2[slot][col0 + 4 * c4]);
-                        neg[0] = make_float2(-l4.x, -l4.y);
-                        neg[1] = make_float2(-l4.z, -l4.w);
+                        const float4 l4 = *reinterpret_cast<const float4*>(lse2 + 4 * c4);
+                        neg[0] = make_float2(l4.x, l4.y);
+                        neg[1] = make_float2(l4.z, l4.w);
                     } else {
-                        neg[0] = neg[1] = make_float2(-row_lse2, -row_lse2);
+                        neg[0] = neg[1] = make_float2(row_lse2, row_lse2);
                     }
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -444,7 +449,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                         p[c + 1] = f2u(x.y);
                     }
                 }
-                if (masked) {
+                if constexpr (Cfg::DKV) {
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(smem_u32(&sh.lse_free[g % 2]));
+                    }
+                }
+                // Masks: query position minus key position in [0, window), or the key a sink.
+                const int q_row = Cfg::DKV ? tile_row : it.row0;
+                const int k_row = Cfg::DKV ? it.row0 : tile_row;
+                const int gap = q_row + args.shift - k_row;  // of the tiles' first rows
+                if (gap < kTile - 1 || (gap + kTile - 1 >= args.window && k_row + kTile > args.sinks)) {
                     if constexpr (Cfg::DKV) {
                         // Row = key: it is seen by the columns [from, from + window), a sink by all from
                         // `from` on.
@@ -459,59 +474,94 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                     const float2 x = make_float2(u2f(p[c]), u2f(p[c + 1]));
                     const float2 e = ((c / 2) % 8) < kEmuPer8 ? exp2_poly2_deg3(x)
                                                               : make_float2(ex2_approx(x.x), ex2_approx(x.y));
-                    p[c] = f2u(e.x);
-                    p[c + 1] = f2u(e.y);
-                }
-                if constexpr (Cfg::DKV) {
-                    uint32_t w[32];
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        w[c] = pack2<Cfg::BF16>(u2f(p[2 * c]), u2f(p[2 * c + 1]));
-                    }
-                    tmem_st32(t_p, w);
-                    tmem_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(smem_u32(&sh.p_full));
+                    if constexpr (Cfg::DKV) {
+                        p[c / 2] = pack2<Cfg::BF16>(e.x, e.y);
+                    } else {
+                        p[c] = f2u(e.x);
+                        p[c + 1] = f2u(e.y);
                     }
                 }
-                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.dp_full), g & 1, wctx, kStatusTimeoutSoftmax));
+            };
+            // dS of the tile whose dP is next, from its P.
+            auto gradients = [&](const auto& p, uint32_t (&w)[32]) {
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.dp_full), gd & 1, wctx, kStatusTimeoutSoftmax));
                 if (!ok) {
-                    continue;
+                    return;
                 }
                 tc_fence_after();
-                uint32_t w[32];
+                [[maybe_unused]] const float* delta = sh.delta[gd % kXStages] + col0;
+                uint32_t dp[64];
+                tmem_ld64(t_dp, dp);
+                tmem_wait_ld();
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t dp[32];
-                    tmem_ld32(t_dp + half * 32, dp);
-                    tmem_wait_ld();
+                for (int c4 = 0; c4 < 16; ++c4) {
+                    float2 d[2];
+                    if constexpr (Cfg::DKV) {
+                        const float4 d4 = *reinterpret_cast<const float4*>(delta + 4 * c4);
+                        d[0] = make_float2(d4.x, d4.y);
+                        d[1] = make_float2(d4.z, d4.w);
+                    } else {
+                        d[0] = d[1] = make_float2(row_delta, row_delta);
+                    }
 #pragma unroll
-                    for (int c4 = 0; c4 < 8; ++c4) {
-                        float2 d01, d23;
+                    for (int h = 0; h < 2; ++h) {
+                        const int c = 4 * c4 + 2 * h;
+                        float2 x;
                         if constexpr (Cfg::DKV) {
-                            const float4 d4 = *reinterpret_cast<const float4*>(&sh.delta[slot][col0 + half * 32 + 4 * c4]);
-                            d01 = make_float2(-d4.x, -d4.y);
-                            d23 = make_float2(-d4.z, -d4.w);
+                            x = unpack2<Cfg::BF16>(p[c / 2]);
                         } else {
-                            d01 = d23 = make_float2(-row_delta, -row_delta);
+                            x = make_float2(u2f(p[c]), u2f(p[c + 1]));
                         }
-                        const int c = half * 32 + 4 * c4;
-                        const float2 a = __fmul2_rn(make_float2(u2f(p[c]), u2f(p[c + 1])),
-                                                    __fadd2_rn(make_float2(u2f(dp[4 * c4]), u2f(dp[4 * c4 + 1])), d01));
-                        const float2 b = __fmul2_rn(make_float2(u2f(p[c + 2]), u2f(p[c + 3])),
-                                                    __fadd2_rn(make_float2(u2f(dp[4 * c4 + 2]), u2f(dp[4 * c4 + 3])), d23));
-                        w[half * 16 + 2 * c4] = pack2<Cfg::BF16>(a.x, a.y);
-                        w[half * 16 + 2 * c4 + 1] = pack2<Cfg::BF16>(b.x, b.y);
+                        const float2 y = __fmul2_rn(x, __fadd2_rn(make_float2(u2f(dp[c]), u2f(dp[c + 1])), d[h]));
+                        w[c / 2] = pack2<Cfg::BF16>(y.x, y.y);
                     }
                 }
-                tmem_st32(t_ds, w);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(smem_u32(&sh.ds_full));
+            };
+            if constexpr (Cfg::DKV) {
+                // Step i: P of tile i, dS of tile i - 1.
+                uint32_t p_last[32];
+                for (int i = 0; i <= it.n; ++i) {
+                    uint32_t p[64], w[32];
+                    if (i < it.n) {
+                        probabilities(i, p);
+                        ++g;
+                    }
+                    if (i > 0) {
+                        gradients(p_last, w);
+                        ++gd;
+                        if constexpr (Cfg::kOverDP) {
+                            // Every warp has dP in registers; its columns take dS and the next P. (Warps that
+                            // gave up come here, too.)
+                            asm volatile("bar.sync 1, 256;" ::: "memory");
+                        }
+                        if (ok) {
+                            tmem_st32(t_ds, w);
+                        }
+                    }
+                    if (i < it.n) {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) {
+                            p_last[c] = p[c];
+                        }
+                        if (ok) {
+                            tmem_st32(t_p, p_last);
+                        }
+                    }
+                    if (ok) {
+                        tmem_wait_st();
+                        arrive(&sh.ds_full);
+                    }
+                }
+            } else {
+                for (int i = 0; i < it.n; ++i, ++g, ++gd) {
+                    uint32_t p[64], w[32];
+                    probabilities(i, p);
+                    gradients(p, w);
+                    if (ok) {
+                        tmem_st32(t_ds + (g % 2) * (Cfg::kTmemDS2 - Cfg::kTmemDS), w);
+                        tmem_wait_st();
+                        arrive(&sh.ds_full);
+                    }
                 }
             }
 
@@ -653,68 +703,84 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                 __syncwarp();
                 return true;
             };
-            auto dscores = [&](int at, bool last) {  // dP
-                if (!wait(&sh.y_full[at % kYStages], at / kYStages)) {
-                    return false;
-                }
-                tc_fence_after();
+            auto dscores = [&](int at, bool last) {  // dP, the last use of Y
                 const uint64_t y = yk + off(at % kYStages);
                 if (elect_one()) {
                     issue_scores<Cfg>(tmem + Cfg::kTmemDP, r1, y);
                     umma_commit(smem_u32(&sh.dp_full));
-                    if (!Cfg::DKV) {
-                        umma_commit(smem_u32(&sh.y_empty[at % kYStages]));
-                    }
+                    umma_commit(smem_u32(&sh.y_empty[at % kYStages]));
                     if (last) {
                         umma_commit(smem_u32(&sh.r1_empty));
                     }
                 }
                 __syncwarp();
-                return true;
             };
+            auto dproduct = [&](int at, bool first, bool last) {  // dK or dQ, the last use of X
+                const uint64_t x = xn + off(at % kXStages);
+                const uint32_t ds = tmem + ((at & 1) ? Cfg::kTmemDS2 : Cfg::kTmemDS);
+                if (elect_one()) {
+                    issue_product<Cfg>(tmem + Cfg::kTmemAcc1, ds, x, first);
+                    umma_commit(smem_u32(&sh.x_empty[at % kXStages]));
+                    if (last) {
+                        umma_commit(smem_u32(&sh.acc_done));
+                    }
+                }
+                __syncwarp();
+            };
+            int steps = 0;  // completions of ds_full so far
             BwdItem it;
             while (ok && next_item<Cfg::DKV>(args, cursor, it)) {
-                ok = wait(&sh.r0_full, items) && scores(g, it.n == 1) && wait(&sh.r1_full, items) &&
-                     dscores(g, it.n == 1);
-                for (int i = 0; ok && i < it.n; ++i, ++g) {
-                    const bool more = i + 1 < it.n;
-                    const bool last = i + 2 == it.n;
-                    ok = wait(&sh.p_full, g);
+                const int n = it.n;
+                ok = wait(&sh.r0_full, items) && scores(g, n == 1) && wait(&sh.r1_full, items);
+                if (!Cfg::DKV) {
+                    ok = ok && wait(&sh.y_full[g % kYStages], g / kYStages);
+                    if (ok) {
+                        tc_fence_after();
+                        dscores(g, n == 1);
+                    }
+                }
+                for (int i = 0; ok && i < (Cfg::DKV ? n + 1 : n); ++i) {
+                    const int at = g + i;
+                    if (i < n) {
+                        ok = wait(&sh.s_read, at);
+                        if (ok && i + 1 < n) {
+                            ok = scores(at + 1, i + 2 == n);
+                        }
+                    }
+                    ok = ok && wait(&sh.ds_full, steps++);
+                    if (ok && i == 0 && items > 0) {
+                        ok = wait(&sh.acc_free, items - 1);  // the item before has left the accumulators
+                    }
+                    const int y_next = Cfg::DKV ? i : i + 1;  // the tile whose dP comes now
+                    if (ok && y_next < n) {
+                        ok = wait(&sh.y_full[(g + y_next) % kYStages], (g + y_next) / kYStages);
+                    }
                     if (!ok) {
                         break;
-                    }
-                    if (i == 0 && items > 0) {
-                        // The item before this one has left the accumulators.
-                        ok = wait(&sh.acc_free, items - 1);
-                        if (!ok) {
-                            break;
-                        }
                     }
                     tc_fence_after();
                     if constexpr (Cfg::DKV) {
-                        const uint64_t y = yn + off(g % kYStages);
-                        if (elect_one()) {
-                            issue_product<Cfg>(tmem + Cfg::kTmemAcc0, tmem + Cfg::kTmemP, y, i == 0);
-                            umma_commit(smem_u32(&sh.y_empty[g % kYStages]));
+                        if (i < n) {
+                            const uint64_t y = yn + off(at % kYStages);
+                            if (elect_one()) {
+                                issue_product<Cfg>(tmem + Cfg::kTmemAcc0, tmem + Cfg::kTmemP, y, i == 0);
+                            }
+                            __syncwarp();
                         }
-                        __syncwarp();
-                    }
-                    ok = (!more || scores(g + 1, last)) && wait(&sh.ds_full, g);
-                    if (!ok) {
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint64_t x = xn + off(g % kXStages);
-                    if (elect_one()) {
-                        issue_product<Cfg>(tmem + Cfg::kTmemAcc1, tmem + Cfg::kTmemDS, x, i == 0);
-                        umma_commit(smem_u32(&sh.x_empty[g % kXStages]));
-                        if (!more) {
-                            umma_commit(smem_u32(&sh.acc_done));
+                        if (i > 0) {
+                            dproduct(at - 1, i == 1, i == n);
                         }
+                        if (i < n) {
+                            dscores(at, i + 1 == n);
+                        }
+                    } else {
+                        if (i + 1 < n) {
+                            dscores(at + 1, i + 2 == n);
+                        }
+                        dproduct(at, i == 0, i + 1 == n);
                     }
-                    __syncwarp();
-                    ok = !more || dscores(g + 1, last);
                 }
+                g += n;
                 ++items;
             }
             // Every MMA issued above must be complete before tensor memory is released.
@@ -742,19 +808,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                     lse[k] = r < args.q_len ? __ldg(args.lse + base + r) : -INFINITY;
                     delta[k] = r < args.q_len ? __ldg(args.delta + base + r) : 0.0f;
                 }
-                // Two slots: that of tile g is free once the products of tile g - 2 are done.
-                const int slot = g % 2;
+                // LSE has two slots, free after the exponentials of tile g - 2; delta three, like X.
+                ok = mbar_wait(smem_u32(&sh.x_empty[g % kXStages]), ((g / kXStages) & 1) ^ 1, wctx, kStatusTimeoutProducer);
                 if (g >= 2) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.x_empty[(g - 2) % kXStages]),
-                                                           ((g - 2) / kXStages) & 1, wctx, kStatusTimeoutProducer));
+                    ok = ok && mbar_wait(smem_u32(&sh.lse_free[g % 2]), ((g - 2) / 2) & 1, wctx, kStatusTimeoutProducer);
                 }
+                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) {
                     break;
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    sh.lse2[slot][k * 32 + lane] = lse[k] == -INFINITY ? INFINITY : lse[k] * 1.4426950408889634f;
-                    sh.delta[slot][k * 32 + lane] = delta[k];
+                    sh.lse2[g % 2][k * 32 + lane] = lse[k] == -INFINITY ? -INFINITY : lse[k] * -1.4426950408889634f;
+                    sh.delta[g % kXStages][k * 32 + lane] = -delta[k];
                 }
                 __syncwarp();
                 if (lane == 0) {
@@ -769,6 +835,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     if (warp == kMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, Cfg::kTmemCols);
+    }
+    if constexpr (!Cfg::DKV) {
+        // The dQ pass needs delta, which was complete before any of its CTAs could start, and nothing of the
+        // dK, dV pass beside it; but its own end stands for both.
+        cudaGridDependencySynchronize();
     }
 }
 
