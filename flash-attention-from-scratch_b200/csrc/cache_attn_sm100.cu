@@ -663,6 +663,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cached_kernel(const __gr
     extern __shared__ __align__(128) uint8_t smem[];
     const int grid = static_cast<int>(gridDim.x);
     const long long cta = blockIdx.x;
+    cudaTriggerProgrammaticLaunchCompletion();  // the join's CTAs may take SMs as they get free
     const Range range = locate<C>(p, grid, [&](long long per) { return cta * per; });
     if (range.found < 0) {
         return;  // past the end of the list
