@@ -384,8 +384,13 @@ cudaError_t launch(const FaAppendParams& p, DeviceStatus* status, cudaStream_t s
     // Every page a sequence's tokens can touch, from any place in the first one.
     const int spans = (c.tokens + c.page_size - 2) / c.page_size + 1;
     const long long pages = static_cast<long long>(c.batch) * spans * c.kv_heads * 2;
-    // A page is at most kRowsPerThread rows a thread.
-    const int threads = std::min(kMaxThreads, std::max(32, c.page_size * (D / 8) / kRowsPerThread));
+    // A page's new rows are at most kRowsPerThread a thread. A decode step has one: with a warp a CTA all
+    // of them run at once (128 sequences x 8 heads: 10.3 us with the threads of a whole page, 3.9 us with a warp).
+    int rows_most = 1;
+    while (rows_most < std::min(c.page_size, c.tokens)) {
+        rows_most *= 2;
+    }
+    const int threads = std::min(kMaxThreads, std::max(32, rows_most * (D / 8) / kRowsPerThread));
     QuerySplit split{};
     long long query_blocks = 0;
     if (p.q != nullptr) {

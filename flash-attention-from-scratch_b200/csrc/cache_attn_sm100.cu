@@ -53,6 +53,7 @@ constexpr int kTileBytes = 4096;   // K (or V) of a key tile
 constexpr int kAuxFloats = 16;     // of a stage: 8 K scales, 8 V scales
 constexpr int kCtasPerSm = 3;
 constexpr int kMinTiles = kWarps;  // least key tiles of a CTA: one for each warp
+constexpr int kWholeTiles = 8;     // up to this many key tiles in the table's capacity items are not cut
 constexpr float kMinScale = 8.673617379884035e-19f;  // 2^-60
 constexpr int kSmem = kWarps * kStages * (2 * kTileBytes + kAuxFloats * 4);
 
@@ -273,7 +274,19 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
             const uint32_t ks = smem_u32(ring) + stage * 2 * kTileBytes;
             const uint32_t vs = ks + kTileBytes;
             const int last = key0 + C::kKeys - 1;
-            if (C::ONE_PAGE && ids >= 0 && last <= s.last && (key0 >= s.first || last < p.sinks)) {
+            const bool shows_all = last <= s.last && (key0 >= s.first || last < p.sinks);
+            if (!C::ONE_PAGE && shows_all && __all_sync(0xffffffffu, ids >= 0 || lane >= spans)) {
+                // All of the tile is shown, in several pages.
+                const int in_page = c.page_size - 1;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int r = i * kStep + r0;
+                    const int id = __shfl_sync(0xffffffffu, ids, r >> log2_span);
+                    const int slot = ((key0 + r) & in_page) * C::kRowBytes;
+                    cp_async16(ks + k_offset<C>(r, chunk), kbase + (id * kpage + slot), true);
+                    cp_async16(vs + v_offset<C>(r, chunk), vbase + (id * vpage + slot), true);
+                }
+            } else if (C::ONE_PAGE && shows_all && ids >= 0) {
                 // The usual tile: all of it shown, contiguous in its page.
                 const int64_t slot = static_cast<int64_t>((key0 & (c.page_size - 1)) + r0) * C::kRowBytes;
                 const uint8_t* ksrc = kbase + ids * kpage + slot;
@@ -657,6 +670,19 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
     __syncthreads();  // the rings are free for the next item
 }
 
+// Items that are never cut, one a CTA.
+template <class C>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) cached_whole_kernel(const __grid_constant__ FaCachedParams p,
+                                                                            DeviceStatus* status) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int row_tiles = (p.heads / p.cache.kv_heads * p.cache.tokens + kRows - 1) / kRows;
+    const int items = p.cache.kv_heads * row_tiles;
+    const int b = static_cast<int>(blockIdx.x) / items;
+    const int item = static_cast<int>(blockIdx.x) - b * items;
+    const Sequence s = sequence<C>(p, b);
+    attend<C>(p, status, smem, s, b, item / row_tiles, (item % row_tiles) * kRows, 0, s.tiles, Record{}, -1);
+}
+
 template <class C>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) cached_kernel(const __grid_constant__ FaCachedParams p,
                                                                       DeviceStatus* status, Record rec) {
@@ -786,8 +812,16 @@ __global__ void __launch_bounds__(kThreads) cached_join_kernel(const __grid_cons
 
 int tile_keys(const FaCache& c) { return kTileBytes / (c.head_dim * (c.dtype == FA_DTYPE_FLOAT8_E4M3 ? 1 : 2)); }
 
-// CTAs of a call: what fills the GPU, or fewer where the table's whole capacity is less work.
-int grid_for(const FaCachedParams& p, int sm_count) {
+// How a call is cut. Short contexts (by the table's capacity, since lengths are on the device): an item is
+// one CTA's, two key tiles a warp, in one launch. Longer ones: the CTAs that fill the GPU, or
+// fewer where the capacity is less work, and a second launch to join (one token over 777 in 25
+// tiles of 16 heads: 10.3 us so, 14.0 us with a CTA a head and 7 tiles a warp).
+struct Split {
+    bool whole;
+    long long grid;
+};
+
+Split split_for(const FaCachedParams& p, int sm_count) {
     const FaCache& c = p.cache;
     const int keys = tile_keys(c);
     const long long rows = static_cast<long long>(p.heads / c.kv_heads) * c.tokens;
@@ -796,17 +830,29 @@ int grid_for(const FaCachedParams& p, int sm_count) {
     if (p.window > 0) {
         shown = std::min<long long>(shown, static_cast<long long>(p.window) + p.sinks + c.tokens + 2 * keys);
     }
-    const long long tiles = items * (shown / keys + 1);
-    return static_cast<int>(std::max<long long>(1, std::min<long long>(kCtasPerSm * sm_count, (tiles + kMinTiles - 1) / kMinTiles)));
+    const long long tiles = shown / keys + 1;
+    if (tiles <= kWholeTiles) {
+        return {true, items};
+    }
+    return {false, std::min<long long>(kCtasPerSm * sm_count, (items * tiles + kMinTiles - 1) / kMinTiles)};
 }
 
 template <class C>
 cudaError_t launch(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
-    cudaError_t err = ensure_smem_limit<cached_kernel<C>>(kSmem);
+    const Split split = split_for(p, sm_count);
+    if (split.grid > 0x7fffffffLL) {
+        return cudaErrorInvalidConfiguration;
+    }
+    const int grid = static_cast<int>(split.grid);
+    cudaError_t err = split.whole ? ensure_smem_limit<cached_whole_kernel<C>>(kSmem)
+                                  : ensure_smem_limit<cached_kernel<C>>(kSmem);
     if (err != cudaSuccess) {
         return err;
     }
-    const int grid = grid_for(p, sm_count);
+    if (split.whole) {
+        cached_whole_kernel<C><<<grid, kThreads, kSmem, stream>>>(p, status);
+        return cudaGetLastError();
+    }
     Record rec;
     rec.o = static_cast<float*>(workspace);
     rec.ml = reinterpret_cast<float2*>(rec.o + static_cast<size_t>(grid) * 2 * kRows * C::D);
@@ -850,7 +896,8 @@ cudaError_t launch_dim(const FaCachedParams& p, DeviceStatus* status, void* work
 }  // namespace
 
 unsigned long long cached_workspace_bytes(const FaCachedParams& p, int sm_count) {
-    return static_cast<unsigned long long>(grid_for(p, sm_count)) * 2 * kRows * (p.cache.head_dim + 2) * 4;
+    const Split split = split_for(p, sm_count);
+    return split.whole ? 0 : static_cast<unsigned long long>(split.grid) * 2 * kRows * (p.cache.head_dim + 2) * 4;
 }
 
 cudaError_t launch_cached(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count,

@@ -171,8 +171,9 @@ def _run_cached(params: bytes, device: torch.device, stream: int) -> int:
     nbytes = ctypes.c_uint64(0)
     rc = _C.lib.fa_cached_workspace_size(params, ctypes.byref(nbytes))
     if rc == _C.FA_OK:
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
-        rc = _C.lib.fa_cached_attention(params, ws.data_ptr(), nbytes.value, stream)
+        need = nbytes.value
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        rc = _C.lib.fa_cached_attention(params, ws.data_ptr() if need else 0, need, stream)
     return rc
 
 
