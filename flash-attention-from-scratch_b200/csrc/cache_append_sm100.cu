@@ -366,15 +366,19 @@ __device__ __forceinline__ void rotate_queries(const FaAppendParams& p, DeviceSt
 
 template <int D, bool BF16, bool E4M3, int TURN>
 __global__ void __launch_bounds__(kMaxThreads) append_kernel(const __grid_constant__ FaAppendParams p,
-                                                             DeviceStatus* status, int page_blocks, int spans,
+                                                             DeviceStatus* status, unsigned long long page_share, int spans,
                                                              int log2_page, QuerySplit split) {
-    const int block = static_cast<int>(blockIdx.x);
-    if (block >= page_blocks) {
-        rotate_queries<D, BF16, TURN>(p, status, block - page_blocks, split);
-    } else if ((block & 1) == 0) {
-        store_page<D, BF16, E4M3, TURN>(p, status, block >> 1, false, spans, log2_page);
+    // Pages and rows of q alternate in proportion, so that one's stores run beside the other's waits: page
+    // blocks before block b are floor(b pages / blocks), kept as a 32-bit fraction rounded up.
+    const unsigned long long b = blockIdx.x;
+    const int before = static_cast<int>((b * page_share) >> 32);
+    const bool is_page = static_cast<int>(((b + 1) * page_share) >> 32) > before;
+    if (!is_page) {
+        rotate_queries<D, BF16, TURN>(p, status, static_cast<int>(b) - before, split);
+    } else if ((before & 1) == 0) {
+        store_page<D, BF16, E4M3, TURN>(p, status, before >> 1, false, spans, log2_page);
     } else {
-        store_page<D, BF16, E4M3, kNoTurn>(p, status, block >> 1, true, spans, log2_page);
+        store_page<D, BF16, E4M3, kNoTurn>(p, status, before >> 1, true, spans, log2_page);
     }
 }
 
@@ -408,12 +412,13 @@ cudaError_t launch(const FaAppendParams& p, DeviceStatus* status, cudaStream_t s
     if (blocks > 0x7fffffffLL) {
         return cudaErrorInvalidConfiguration;
     }
+    const unsigned long long page_share = ((static_cast<unsigned long long>(pages) << 32) + blocks - 1) / blocks;
     int log2_page = 0;
     while ((1 << log2_page) < c.page_size) {
         ++log2_page;
     }
     append_kernel<D, BF16, E4M3, TURN><<<static_cast<unsigned>(blocks), threads, 0, stream>>>(
-        p, status, static_cast<int>(pages), spans, log2_page, split);
+        p, status, page_share, spans, log2_page, split);
     return cudaGetLastError();
 }
 

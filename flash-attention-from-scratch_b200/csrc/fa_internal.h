@@ -53,6 +53,7 @@ struct WindowArgs {
     FastDiv div_heads;  // query heads
     FastDiv div_group;  // query heads per key/value head
     float* lse;         // [batch * heads][q_len], or NULL
+    int halves_from;    // items from here on are single query tiles of row block halves_from + (i - halves_from) / 2
 };
 
 struct FwdArgs {

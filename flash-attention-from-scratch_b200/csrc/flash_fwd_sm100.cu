@@ -367,10 +367,14 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         }
         int m_block;
         if constexpr (Cfg::WIN) {
-            // Items cost about the same: heads in order, row blocks in order.
+            // Items cost about the same: heads in order, row blocks in order. Those of the last, partial
+            // wave are single query tiles.
+            const int over = idx - args.win.halves_from;
+            const int half = over >= 0 ? over & 1 : 0;
+            lin = over >= 0 ? args.win.halves_from + (over >> 1) : idx;
             it.bh = args.div_nb.div(lin);
             m_block = lin - it.bh * nb;
-            it.q_row0 = m_block * NQ * kBM;
+            it.q_row0 = (m_block * NQ + half) * kBM;
             it.w[0] = it.w[1] = args.win.div_heads.div(it.bh);
             it.z[0] = it.bh - it.w[0] * static_cast<int>(args.win.div_heads.d);
             it.z[1] = args.win.div_group.div(it.z[0]);
@@ -382,12 +386,13 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             for (int t = 0; t < NQ; ++t) {
                 // A tile whose rows see nothing still takes key tile 0, all masked: O = 0 is stored.
                 const int q0 = it.q_row0 + t * kBM;
+                const bool present = q0 < n && (t == 0 || over < 0);
                 const int lo_pos = max(q0 + args.win.shift, 0);
                 const int hi_pos = max(min(q0 + kBM, n) - 1 + args.win.shift, 0);
                 it.tile_lo[t] = max(lo_pos - args.win.window + 1, 0) / kBN;
                 it.tile_hi[t] = hi_pos / kBN;
-                it.n_kv[t] = q0 < n ? 1 : 0;  // present
-                hi = q0 < n ? it.tile_hi[t] : hi;
+                it.n_kv[t] = present ? 1 : 0;
+                hi = present ? it.tile_hi[t] : hi;
             }
             it.first_tile = it.tile_lo[0];
             it.sink_tiles = min((args.win.sinks + kBN - 1) / kBN, it.first_tile);
@@ -1936,10 +1941,16 @@ template <int D, bool BF16>
 static cudaError_t launch_window_cfg(const FaWindowParams& p, FwdArgs& args, int sm_count, cudaStream_t stream) {
     using Cfg = FwdCfg<D, true, kVariantOpt, BF16, false, true>;
     const long long nb = (p.q_len + Cfg::NQ * kBM - 1) / (Cfg::NQ * kBM);
-    const long long items = nb * args.num_bh;
-    if (items > 0x7fffffffLL) {
+    // Row blocks of two query tiles; where the last wave of them would fill less than half the SMs, its
+    // tiles go one to a CTA (512 blocks on 148 SMs, 16 x 8191, window 1024: 98 us with whole blocks, 95 so).
+    const long long blocks = nb * args.num_bh;
+    if (2 * blocks > 0x7fffffffLL) {
         return cudaErrorInvalidConfiguration;
     }
+    const long long last_wave = blocks % sm_count;
+    const long long halved = 2 * last_wave <= sm_count ? last_wave : 0;
+    const long long items = blocks + halved;
+    args.win.halves_from = static_cast<int>(blocks - halved);
     CUtensorMap q, k, v, o;
     if (encode_strided_map(&q, p.q, p.q_stride, p.batch, p.heads, p.q_len, D, kBM, BF16) != CUDA_SUCCESS ||
         encode_strided_map(&k, p.k, p.k_stride, p.batch, p.kv_heads, p.k_len, D, kBN, BF16) != CUDA_SUCCESS ||
