@@ -396,7 +396,8 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             }
             it.first_tile = it.tile_lo[0];
             it.sink_tiles = min((args.win.sinks + kBN - 1) / kBN, it.first_tile);
-            it.n_max = it.sink_tiles + hi - it.first_tile + 1;
+            // The second half of a block may lie past the last row: nothing to load.
+            it.n_max = it.n_kv[0] > 0 ? it.sink_tiles + hi - it.first_tile + 1 : 0;
             return;
         }
         if constexpr (Cfg::CAUSAL) {
