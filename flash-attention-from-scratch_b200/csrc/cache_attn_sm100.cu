@@ -719,14 +719,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cached_kernel(const __gr
     }
 }
 
-// Joins the records of the item that was cut at unit k per, k = blockIdx.x + 1, if that is its
-// first cut; row blockIdx.y of it. Warps take the records in turn, then join in order.
-template <class C>
+// Joins the records of the item that was cut at unit k per, k = blockIdx.x + 1, if that is its first
+// cut, always in the same order. SPREAD: a row a CTA, its 4 warps taking the records in turn and joining in
+// order, where all those CTAs are resident at once or an item has many records (few, long sequences). Else a
+// warp a row, 4 rows a CTA (64 sequences x 4 tokens: 122 us a call with SPREAD, 110 without; one token
+// over 777: 10.3 us with, 12.7 without).
+template <class C, bool SPREAD>
 __global__ void __launch_bounds__(kThreads) cached_join_kernel(const __grid_constant__ FaCachedParams p, Record rec,
                                                                int grid) {
     constexpr int D = C::D;
-    __shared__ float2 all_ml[kWarps];
-    __shared__ float all_o[kWarps][D];
+    constexpr int PER = D / 32;
     const long long k = blockIdx.x + 1;
     const Range range = locate<C>(p, grid, [&](long long per) { return k * per; });
     if (range.found < 0) {
@@ -739,15 +741,15 @@ __global__ void __launch_bounds__(kThreads) cached_join_kernel(const __grid_cons
     const long long item = (k * range.per - range.found_base) / s.tiles;
     const long long start = range.found_base + item * s.tiles;
     const int row0 = static_cast<int>(item % row_tiles) * kRows;
-    const int row = static_cast<int>(blockIdx.y);
-    if (start == k * range.per || start / range.per != k - 1 || row0 + row >= rows) {
+    const int warp = static_cast<int>(threadIdx.x) / 32;
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    const int row = SPREAD ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * kWarps + warp;
+    const int row_first = SPREAD ? row : static_cast<int>(blockIdx.y) * kWarps;
+    if (start == k * range.per || start / range.per != k - 1 || row0 + row_first >= rows) {
         return;
     }
     const long long c0 = start / range.per;
     const long long c1 = (start + s.tiles - 1) / range.per;
-    const int warp = static_cast<int>(threadIdx.x) / 32;
-    const int lane = static_cast<int>(threadIdx.x) % 32;
-    constexpr int PER = D / 32;
     cudaGridDependencySynchronize();  // the records are there
     float m = -INFINITY, l = 0.0f;
     float o[PER];
@@ -755,58 +757,77 @@ __global__ void __launch_bounds__(kThreads) cached_join_kernel(const __grid_cons
     for (int i = 0; i < PER; ++i) {
         o[i] = 0.0f;
     }
+    if (row < kRows) {
 #pragma unroll 4
-    for (long long c = c0 + warp; c <= c1; c += kWarps) {
-        // A CTA's first stretch is its record 0; the item starts in c0, as its second unless there.
-        const long long record = (2 * c + (c * range.per >= start ? 0 : 1)) * kRows + row;
-        const float2 ml = rec.ml[record];
-        float y[PER];
+        for (long long c = c0 + (SPREAD ? warp : 0); c <= c1; c += SPREAD ? kWarps : 1) {
+            // A CTA's first stretch is its record 0; the item starts in c0, as its second unless there.
+            const long long record = (2 * c + (c * range.per >= start ? 0 : 1)) * kRows + row;
+            const float2 ml = rec.ml[record];
+            float y[PER];
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                y[i] = rec.o[record * D + lane * PER + i];
+            }
+            const float now = fmaxf(m, ml.x);
+            const float used = now == -INFINITY ? 0.0f : now;
+            const float a = ex2_approx(m - used);
+            const float w = ex2_approx(ml.x - used);
+            m = now;
+            l = fmaf(ml.y, w, l * a);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                o[i] = fmaf(y[i], w, o[i] * a);
+            }
+        }
+    }
+    if constexpr (SPREAD) {
+        __shared__ float2 all_ml[kWarps];
+        __shared__ float all_o[kWarps][D];
+        if (lane == 0) {
+            all_ml[warp] = make_float2(m, l);
+        }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            y[i] = rec.o[record * D + i * 32 + lane];
+            all_o[warp][lane * PER + i] = o[i];
         }
-        const float now = fmaxf(m, ml.x);
-        const float used = now == -INFINITY ? 0.0f : now;
-        const float a = ex2_approx(m - used);
-        const float w = ex2_approx(ml.x - used);
-        m = now;
-        l = fmaf(ml.y, w, l * a);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            o[i] = fmaf(y[i], w, o[i] * a);
+        __syncthreads();
+        if (warp > 0) {
+            return;
         }
-    }
-    if (lane == 0) {
-        all_ml[warp] = make_float2(m, l);
-    }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        all_o[warp][i * 32 + lane] = o[i];
-    }
-    __syncthreads();
-    const int d = static_cast<int>(threadIdx.x);
-    if (d < D / 2) {
-        float top = -INFINITY;
+        m = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            top = fmaxf(top, all_ml[w].x);
+            m = fmaxf(m, all_ml[w].x);
         }
-        const float used = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f, a = 0.0f, b = 0.0f;
+        const float used = m == -INFINITY ? 0.0f : m;
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            o[i] = 0.0f;
+        }
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float f = ex2_approx(all_ml[w].x - used);
-            sum = fmaf(all_ml[w].y, f, sum);
-            a = fmaf(all_o[w][2 * d], f, a);
-            b = fmaf(all_o[w][2 * d + 1], f, b);
+            l = fmaf(all_ml[w].y, f, l);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                o[i] = fmaf(all_o[w][lane * PER + i], f, o[i]);
+            }
         }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int kvh = static_cast<int>(item / row_tiles);
-        const int head = (row0 + row) / p.cache.tokens;
-        const int token = row0 + row - head * p.cache.tokens;
-        const long long out_row =
-            (static_cast<long long>(range.found) * p.heads + kvh * group + head) * p.cache.tokens + token;
-        reinterpret_cast<uint32_t*>(p.o)[out_row * (D / 2) + d] = pack2<C::BF16>(a * inv, b * inv);
+    }
+    if (row >= kRows || row0 + row >= rows) {
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int kvh = static_cast<int>(item / row_tiles);
+    const int head = (row0 + row) / p.cache.tokens;
+    const int token = row0 + row - head * p.cache.tokens;
+    const long long out_row =
+        (static_cast<long long>(range.found) * p.heads + kvh * group + head) * p.cache.tokens + token;
+#pragma unroll
+    for (int i = 0; i < PER; i += 2) {
+        reinterpret_cast<uint32_t*>(p.o)[(out_row * D + lane * PER + i) / 2] =
+            pack2<C::BF16>(o[i] * inv, o[i + 1] * inv);
     }
 }
 
@@ -819,6 +840,7 @@ int tile_keys(const FaCache& c) { return kTileBytes / (c.head_dim * (c.dtype == 
 struct Split {
     bool whole;
     long long grid;
+    long long items;
 };
 
 Split split_for(const FaCachedParams& p, int sm_count) {
@@ -832,9 +854,9 @@ Split split_for(const FaCachedParams& p, int sm_count) {
     }
     const long long tiles = shown / keys + 1;
     if (tiles <= kWholeTiles) {
-        return {true, items};
+        return {true, items, items};
     }
-    return {false, std::min<long long>(kCtasPerSm * sm_count, (items * tiles + kMinTiles - 1) / kMinTiles)};
+    return {false, std::min<long long>(kCtasPerSm * sm_count, (items * tiles + kMinTiles - 1) / kMinTiles), items};
 }
 
 template <class C>
@@ -863,7 +885,9 @@ cudaError_t launch(const FaCachedParams& p, DeviceStatus* status, void* workspac
     }
     const int rows = std::min(kRows, p.heads / p.cache.kv_heads * p.cache.tokens);
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(static_cast<unsigned>(grid - 1), static_cast<unsigned>(rows));
+    constexpr int kResident = 16;  // CTAs of the join on an SM
+    const bool spread = static_cast<long long>(grid - 1) * rows <= kResident * sm_count || grid > 8 * split.items;
+    config.gridDim = dim3(static_cast<unsigned>(grid - 1), static_cast<unsigned>(spread ? rows : (rows + kWarps - 1) / kWarps));
     config.blockDim = dim3(kThreads);
     config.stream = stream;
     cudaLaunchAttribute early{};
@@ -871,7 +895,8 @@ cudaError_t launch(const FaCachedParams& p, DeviceStatus* status, void* workspac
     early.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &early;
     config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, cached_join_kernel<C>, p, rec, grid);
+    return spread ? cudaLaunchKernelEx(&config, cached_join_kernel<C, true>, p, rec, grid)
+                  : cudaLaunchKernelEx(&config, cached_join_kernel<C, false>, p, rec, grid);
 }
 
 template <int D, bool ONE_PAGE>
