@@ -127,6 +127,7 @@ struct BwdShared {
 template <class Cfg>
 constexpr int bwd_smem() {
     static_assert(Cfg::kSmemShared + sizeof(BwdShared) <= 227 * 1024, "shared memory budget");
+    static_assert(Cfg::kSmemShared + sizeof(BwdShared) > 114 * 1024, "one CTA an SM: it owns all of tensor memory");
     return Cfg::kSmemShared + static_cast<int>(sizeof(BwdShared));
 }
 
@@ -426,17 +427,23 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                 }
                 tc_fence_after();
                 tmem_ld64(t_s, p);
+                // The columns' LSE comes meanwhile: shared memory is busy with the products' operands.
+                [[maybe_unused]] float4 lse2[16];
+                if constexpr (Cfg::DKV) {
+#pragma unroll
+                    for (int c4 = 0; c4 < 16; ++c4) {
+                        lse2[c4] = *reinterpret_cast<const float4*>(&sh.lse2[g % 2][col0 + 4 * c4]);
+                    }
+                }
                 tmem_wait_ld();
                 // S is in registers: the next scores may take its columns.
                 arrive(&sh.s_read);
-                [[maybe_unused]] const float* lse2 = sh.lse2[g % 2] + col0;
 #pragma unroll
                 for (int c4 = 0; c4 < 16; ++c4) {
                     float2 neg[2];
                     if constexpr (Cfg::DKV) {
-                        const float4 l4 = *reinterpret_cast<const float4*>(lse2 + 4 * c4);
-                        neg[0] = make_float2(l4.x, l4.y);
-                        neg[1] = make_float2(l4.z, l4.w);
+                        neg[0] = make_float2(lse2[c4].x, lse2[c4].y);
+                        neg[1] = make_float2(lse2[c4].z, lse2[c4].w);
                     } else {
                         neg[0] = neg[1] = make_float2(row_lse2, row_lse2);
                     }
@@ -492,12 +499,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                 [[maybe_unused]] const float* delta = sh.delta[gd % kXStages] + col0;
                 uint32_t dp[64];
                 tmem_ld64(t_dp, dp);
+                [[maybe_unused]] float4 delta_half[8];
+                if constexpr (Cfg::DKV) {
+#pragma unroll
+                    for (int c4 = 0; c4 < 8; ++c4) {
+                        delta_half[c4] = *reinterpret_cast<const float4*>(delta + 4 * c4);
+                    }
+                }
                 tmem_wait_ld();
 #pragma unroll
                 for (int c4 = 0; c4 < 16; ++c4) {
                     float2 d[2];
                     if constexpr (Cfg::DKV) {
-                        const float4 d4 = *reinterpret_cast<const float4*>(delta + 4 * c4);
+                        const float4 d4 = c4 < 8 ? delta_half[c4 % 8] : *reinterpret_cast<const float4*>(delta + 4 * c4);
                         d[0] = make_float2(d4.x, d4.y);
                         d[1] = make_float2(d4.z, d4.w);
                     } else {
