@@ -57,6 +57,7 @@ constexpr int kSoftmaxWarps = 8;
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
 constexpr int kLoaderWarp = 10;
+constexpr int kScoreWarp = 11;  // issues S; kMmaWarp the other products
 // Registers: 8 softmax warps take 208 and the other four leave 88, the launch's 384 x 168 in all.
 constexpr int kRegsSoftmax = 208;
 constexpr int kRegsOther = 88;
@@ -111,8 +112,8 @@ struct BwdShared {
     uint64_t r0_full, r0_empty, r1_full, r1_empty;
     uint64_t x_full[kXStages], x_empty[kXStages];
     uint64_t y_full[kYStages], y_empty[kYStages];
-    uint64_t lse_free[2];
-    uint64_t s_full, s_read, dp_full, ds_full, acc_done, acc_free, mma_idle;
+    uint64_t s_read[2];  // of alternate tiles
+    uint64_t s_full, dp_full, ds_full, acc_done, acc_free, mma_idle;
     uint32_t tmem_base;
     int abort;
     int tile, offset;  // where the CTA's range starts
@@ -326,15 +327,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             mbar_init(smem_u32(&sh.y_full[s]), 1);
             mbar_init(smem_u32(&sh.y_empty[s]), 1);
         }
-        mbar_init(smem_u32(&sh.lse_free[0]), kSoftmaxWarps);
-        mbar_init(smem_u32(&sh.lse_free[1]), kSoftmaxWarps);
+        mbar_init(smem_u32(&sh.s_read[0]), kSoftmaxWarps);
+        mbar_init(smem_u32(&sh.s_read[1]), kSoftmaxWarps);
         mbar_init(smem_u32(&sh.s_full), 1);
-        mbar_init(smem_u32(&sh.s_read), kSoftmaxWarps);
         mbar_init(smem_u32(&sh.dp_full), 1);
         mbar_init(smem_u32(&sh.ds_full), kSoftmaxWarps);
         mbar_init(smem_u32(&sh.acc_done), 1);
         mbar_init(smem_u32(&sh.acc_free), kSoftmaxWarps);
-        mbar_init(smem_u32(&sh.mma_idle), 1);
+        mbar_init(smem_u32(&sh.mma_idle), 2);
         mbar_fence_init();
     }
     if (warp == kMmaWarp) {
@@ -436,8 +436,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                     }
                 }
                 tmem_wait_ld();
-                // S is in registers: the next scores may take its columns.
-                arrive(&sh.s_read);
+                // S and LSE are in registers: the next scores may take S's columns, the LSE of tile i + 2 its slot.
+                arrive(&sh.s_read[g % 2]);
 #pragma unroll
                 for (int c4 = 0; c4 < 16; ++c4) {
                     float2 neg[2];
@@ -454,12 +454,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                                                     make_float2(scale_log2, scale_log2), neg[h]);
                         p[c] = f2u(x.x);
                         p[c + 1] = f2u(x.y);
-                    }
-                }
-                if constexpr (Cfg::DKV) {
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(smem_u32(&sh.lse_free[g % 2]));
                     }
                 }
                 // Masks: query position minus key position in [0, window), or the key a sink.
@@ -685,28 +679,123 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         __syncwarp();
     } else if (warp == kMmaWarp) {
-        // ================================= MMA issuer ==================================
-        // The whole warp walks in step, one elected lane issues.
-        {
-            bool ok = true;
-            int g = 0;
-            int items = 0;
-            const uint64_t r0 = make_desc_kmajor_sw128(smem + Cfg::kSmemR0);
-            const uint64_t r1 = make_desc_kmajor_sw128(smem + Cfg::kSmemR1);
-            const uint64_t xk = make_desc_kmajor_sw128(smem + Cfg::kSmemX);
-            const uint64_t xn = make_desc_mnmajor_sw128(smem + Cfg::kSmemX, kBox);
-            const uint64_t yk = make_desc_kmajor_sw128(smem + Cfg::kSmemY);
-            const uint64_t yn = make_desc_mnmajor_sw128(smem + Cfg::kSmemY, kBox);
-            auto off = [](int stage) { return static_cast<uint64_t>(stage * (Cfg::kTileBytes >> 4)); };
-            auto wait = [&](uint64_t* bar, int parity) {
-                return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity & 1, wctx, kStatusTimeoutMma)) != 0;
-            };
-            auto scores = [&](int at, bool last) {  // S of streamed tile `at`
-                if (!wait(&sh.x_full[at % kXStages], at / kXStages)) {
-                    return false;
+        // =============================== MMA issuers ===================================
+        // The whole warp walks in step, one elected lane issues. This one: dP and the sums.
+        bool ok = true;
+        int g = 0;
+        int items = 0;
+        const uint64_t r1 = make_desc_kmajor_sw128(smem + Cfg::kSmemR1);
+        const uint64_t xn = make_desc_mnmajor_sw128(smem + Cfg::kSmemX, kBox);
+        const uint64_t yk = make_desc_kmajor_sw128(smem + Cfg::kSmemY);
+        const uint64_t yn = make_desc_mnmajor_sw128(smem + Cfg::kSmemY, kBox);
+        auto off = [](int stage) { return static_cast<uint64_t>(stage * (Cfg::kTileBytes >> 4)); };
+        auto wait = [&](uint64_t* bar, int parity) {
+            return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity & 1, wctx, kStatusTimeoutMma)) != 0;
+        };
+        auto dscores = [&](int at, bool last) {  // dP, the last use of Y
+            const uint64_t y = yk + off(at % kYStages);
+            if (elect_one()) {
+                issue_scores<Cfg>(tmem + Cfg::kTmemDP, r1, y);
+                umma_commit(smem_u32(&sh.dp_full));
+                umma_commit(smem_u32(&sh.y_empty[at % kYStages]));
+                if (last) {
+                    umma_commit(smem_u32(&sh.r1_empty));
+                }
+            }
+            __syncwarp();
+        };
+        auto dproduct = [&](int at, bool first, bool last) {  // dK or dQ, the last use of X
+            const uint64_t x = xn + off(at % kXStages);
+            const uint32_t ds = tmem + ((at & 1) ? Cfg::kTmemDS2 : Cfg::kTmemDS);
+            if (elect_one()) {
+                issue_product<Cfg>(tmem + Cfg::kTmemAcc1, ds, x, first);
+                umma_commit(smem_u32(&sh.x_empty[at % kXStages]));
+                if (last) {
+                    umma_commit(smem_u32(&sh.acc_done));
+                }
+            }
+            __syncwarp();
+        };
+        int steps = 0;  // completions of ds_full so far
+        BwdItem it;
+        while (ok && next_item<Cfg::DKV>(args, cursor, it)) {
+            const int n = it.n;
+            ok = wait(&sh.r1_full, items);
+            if (!Cfg::DKV) {
+                ok = ok && wait(&sh.y_full[g % kYStages], g / kYStages);
+                if (ok) {
+                    tc_fence_after();
+                    dscores(g, n == 1);
+                }
+            }
+            for (int i = 0; ok && i < (Cfg::DKV ? n + 1 : n); ++i) {
+                const int at = g + i;
+                const int y_next = Cfg::DKV ? i : i + 1;  // the tile whose dP comes now
+                if (y_next < n) {
+                    ok = wait(&sh.y_full[(g + y_next) % kYStages], (g + y_next) / kYStages);
+                }
+                if (ok && i == 0 && items > 0) {
+                    ok = wait(&sh.acc_free, items - 1);  // the item before has left the accumulators
+                }
+                ok = ok && wait(&sh.ds_full, steps++);
+                if (!ok) {
+                    break;
                 }
                 tc_fence_after();
-                const uint64_t x = xk + off(at % kXStages);
+                if constexpr (Cfg::DKV) {
+                    if (i < n) {
+                        const uint64_t y = yn + off(at % kYStages);
+                        if (elect_one()) {
+                            issue_product<Cfg>(tmem + Cfg::kTmemAcc0, tmem + Cfg::kTmemP, y, i == 0);
+                        }
+                        __syncwarp();
+                    }
+                    if (i > 0) {
+                        dproduct(at - 1, i == 1, i == n);
+                    }
+                    if (i < n) {
+                        dscores(at, i + 1 == n);
+                    }
+                } else {
+                    if (i + 1 < n) {
+                        dscores(at + 1, i + 2 == n);
+                    }
+                    dproduct(at, i == 0, i + 1 == n);
+                }
+            }
+            g += n;
+            ++items;
+        }
+        // Every MMA issued must be complete before tensor memory is released.
+        if (elect_one()) {
+            umma_commit(smem_u32(&sh.mma_idle));
+        }
+        __syncwarp();
+        mbar_wait_drain(smem_u32(&sh.mma_idle), 0, wctx, kStatusTimeoutTeardown);
+        __syncwarp();
+    } else if (warp == kScoreWarp) {
+        // S of every streamed tile, as soon as the one before is in registers. In a warp of its own, since issuing
+        // holds a warp until the tensor pipe takes its products.
+        bool ok = true;
+        int g = 0;
+        int items = 0;
+        const uint64_t r0 = make_desc_kmajor_sw128(smem + Cfg::kSmemR0);
+        const uint64_t xk = make_desc_kmajor_sw128(smem + Cfg::kSmemX);
+        auto wait = [&](uint64_t* bar, int parity) {
+            return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity & 1, wctx, kStatusTimeoutMma)) != 0;
+        };
+        BwdItem it;
+        while (ok && next_item<Cfg::DKV>(args, cursor, it)) {
+            ok = wait(&sh.r0_full, items);
+            for (int i = 0; ok && i < it.n; ++i, ++g) {
+                ok = wait(&sh.x_full[g % kXStages], g / kXStages) &&
+                     (g == 0 || wait(&sh.s_read[(g - 1) % 2], (g - 1) / 2));
+                if (!ok) {
+                    break;
+                }
+                tc_fence_after();
+                const uint64_t x = xk + static_cast<uint64_t>((g % kXStages) * (Cfg::kTileBytes >> 4));
+                const bool last = i + 1 == it.n;
                 if (elect_one()) {
                     issue_scores<Cfg>(tmem + Cfg::kTmemS, r0, x);
                     umma_commit(smem_u32(&sh.s_full));
@@ -715,95 +804,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                     }
                 }
                 __syncwarp();
-                return true;
-            };
-            auto dscores = [&](int at, bool last) {  // dP, the last use of Y
-                const uint64_t y = yk + off(at % kYStages);
-                if (elect_one()) {
-                    issue_scores<Cfg>(tmem + Cfg::kTmemDP, r1, y);
-                    umma_commit(smem_u32(&sh.dp_full));
-                    umma_commit(smem_u32(&sh.y_empty[at % kYStages]));
-                    if (last) {
-                        umma_commit(smem_u32(&sh.r1_empty));
-                    }
-                }
-                __syncwarp();
-            };
-            auto dproduct = [&](int at, bool first, bool last) {  // dK or dQ, the last use of X
-                const uint64_t x = xn + off(at % kXStages);
-                const uint32_t ds = tmem + ((at & 1) ? Cfg::kTmemDS2 : Cfg::kTmemDS);
-                if (elect_one()) {
-                    issue_product<Cfg>(tmem + Cfg::kTmemAcc1, ds, x, first);
-                    umma_commit(smem_u32(&sh.x_empty[at % kXStages]));
-                    if (last) {
-                        umma_commit(smem_u32(&sh.acc_done));
-                    }
-                }
-                __syncwarp();
-            };
-            int steps = 0;  // completions of ds_full so far
-            BwdItem it;
-            while (ok && next_item<Cfg::DKV>(args, cursor, it)) {
-                const int n = it.n;
-                ok = wait(&sh.r0_full, items) && scores(g, n == 1) && wait(&sh.r1_full, items);
-                if (!Cfg::DKV) {
-                    ok = ok && wait(&sh.y_full[g % kYStages], g / kYStages);
-                    if (ok) {
-                        tc_fence_after();
-                        dscores(g, n == 1);
-                    }
-                }
-                for (int i = 0; ok && i < (Cfg::DKV ? n + 1 : n); ++i) {
-                    const int at = g + i;
-                    if (i < n) {
-                        ok = wait(&sh.s_read, at);
-                        if (ok && i + 1 < n) {
-                            ok = scores(at + 1, i + 2 == n);
-                        }
-                    }
-                    ok = ok && wait(&sh.ds_full, steps++);
-                    if (ok && i == 0 && items > 0) {
-                        ok = wait(&sh.acc_free, items - 1);  // the item before has left the accumulators
-                    }
-                    const int y_next = Cfg::DKV ? i : i + 1;  // the tile whose dP comes now
-                    if (ok && y_next < n) {
-                        ok = wait(&sh.y_full[(g + y_next) % kYStages], (g + y_next) / kYStages);
-                    }
-                    if (!ok) {
-                        break;
-                    }
-                    tc_fence_after();
-                    if constexpr (Cfg::DKV) {
-                        if (i < n) {
-                            const uint64_t y = yn + off(at % kYStages);
-                            if (elect_one()) {
-                                issue_product<Cfg>(tmem + Cfg::kTmemAcc0, tmem + Cfg::kTmemP, y, i == 0);
-                            }
-                            __syncwarp();
-                        }
-                        if (i > 0) {
-                            dproduct(at - 1, i == 1, i == n);
-                        }
-                        if (i < n) {
-                            dscores(at, i + 1 == n);
-                        }
-                    } else {
-                        if (i + 1 < n) {
-                            dscores(at + 1, i + 2 == n);
-                        }
-                        dproduct(at, i == 0, i + 1 == n);
-                    }
-                }
-                g += n;
-                ++items;
             }
-            // Every MMA issued above must be complete before tensor memory is released.
-            if (elect_one()) {
-                umma_commit(smem_u32(&sh.mma_idle));
-            }
-            __syncwarp();
-            mbar_wait_drain(smem_u32(&sh.mma_idle), 0, wctx, kStatusTimeoutTeardown);
+            ++items;
         }
+        if (elect_one()) {
+            umma_commit(smem_u32(&sh.mma_idle));
+        }
+        __syncwarp();
+        mbar_wait_drain(smem_u32(&sh.mma_idle), 0, wctx, kStatusTimeoutTeardown);
         __syncwarp();
     } else if (Cfg::DKV && warp == kLoaderWarp) {
         // ====================== LSE and delta of the streamed query rows ======================
@@ -822,10 +830,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                     lse[k] = r < args.q_len ? __ldg(args.lse + base + r) : -INFINITY;
                     delta[k] = r < args.q_len ? __ldg(args.delta + base + r) : 0.0f;
                 }
-                // LSE has two slots, free after the exponentials of tile g - 2; delta three, like X.
+                // LSE has two slots, free when tile g - 2 has been read; delta three, like X.
                 ok = mbar_wait(smem_u32(&sh.x_empty[g % kXStages]), ((g / kXStages) & 1) ^ 1, wctx, kStatusTimeoutProducer);
                 if (g >= 2) {
-                    ok = ok && mbar_wait(smem_u32(&sh.lse_free[g % 2]), ((g - 2) / 2) & 1, wctx, kStatusTimeoutProducer);
+                    ok = ok && mbar_wait(smem_u32(&sh.s_read[g % 2]), ((g - 2) / 2) & 1, wctx, kStatusTimeoutProducer);
                 }
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) {
