@@ -886,8 +886,8 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             decode(idx, it);
             if constexpr (Cfg::WIN) {
                 // A row that sees nothing keeps row_max = -inf (the software 2^x may leave a
-                // vanishing row_sum there).
-                if (args.win.lse != nullptr && ok && grow < n) {
+                // vanishing row_sum there). The rows of a query tile that the item lacks (nt = 0) are another's.
+                if (args.win.lse != nullptr && ok && nt > 0 && grow < n) {
                     args.win.lse[static_cast<long long>(it.bh) * n + grow] =
                         row_max == -INFINITY ? -INFINITY : (row_max + __log2f(row_sum)) * 0.6931471805599453f;
                 }

@@ -91,6 +91,27 @@ def test_long_rows_small_window_and_far_sinks(d):
     _check_backward(do, q, k, v, 200, 5)
 
 
+@pytest.mark.parametrize("b,h,hk,n,d,window,sinks", [(1, 16, 4, 8191, 128, 1024, 4), (1, 6, 2, 9000, 64, 3000, 130)])
+def test_last_wave_of_single_query_tiles(b, h, hk, n, d, window, sinks):
+    """More row blocks than SMs and a short last wave, whose query tiles go one to a CTA: every row's O and
+    LSE are its own, and so are the gradients made of them."""
+    q, k, v, do = _inputs(b, h, hk, n, n, d, BF, seed=n)
+    o, lse = fa.forward_window(q, k, v, window, sinks, return_lse=True)
+    got = fa.backward_window(do, q, k, v, o, lse, window, sinks)
+    u, g = oracle.unit(BF), h // hk
+    for j in range(hk):
+        one = lambda t: t[:, j : j + 1]  # noqa: E731
+        own = lambda t: t[:, j * g : (j + 1) * g]  # noqa: E731
+        args = (own(q), one(k), one(v), window, sinks)
+        want, want_lse, _ = oracle.window_forward(*args)
+        oracle.check(own(o), want, oracle.forward_bound(want, v.double().abs().max(), u, u), "O")
+        assert (own(lse).double() - want_lse).abs().max().item() <= 2 * (u + oracle.POLY)
+        grads = oracle.window_backward(own(do), *args)[:3]
+        for name, x, w, e in zip(("dQ", "dK", "dV"), (own(got[0]), one(got[1]), one(got[2])), grads,
+                                 oracle.backward_bounds(own(do), *args)):
+            oracle.check(x, w, e, name)
+
+
 def test_many_heads_walk_a_persistent_grid():
     q, k, v, do = _inputs(3, 32, 8, 300, 300, 64, HALF, seed=6)
     _check_forward(q, k, v, 70, 2)
