@@ -16,7 +16,13 @@
 // Within a CTA each of 4 warps takes every fourth key tile through a ring of its own, filled with
 // 16-byte cp.async copies: no CTA barrier until the item's end, where the warps' rows are joined in
 // shared memory. A key tile is 4 KB of K and 4 KB of V: 32 tokens of 128 e4m3 values, 16 of 128
-// 16-bit ones. 2 CTAs of 96 KB an SM keep up to 128 KB in flight; 6.5 TB/s at about 1 us needs 44.
+// 16-bit ones. Rings of 2 tiles and 3 CTAs an SM (168 registers a thread) keep 96 KB in flight; 6.5 TB/s
+// at about 1 us needs 44. (3 tiles and 2 CTAs: 136 us where this takes 87, for want of warps.)
+//
+// Measured, 32 query heads on 8, D 128, e4m3, pages of 64: 32 sequences of 4000 to 8000 tokens 77 us (5.2 TB/s),
+// 4 of 120000 to 131000 167 us (6.1 TB/s), 64 x 4 drafted tokens over a window of 4096 and 4 sinks 110 us
+// (4.9 TB/s). What is left: the instructions of a tile (about 730, half of the issue slots), and for short
+// ranges the start of an item, its join in shared memory and the second launch.
 //
 // Products are mma.sync m16n8k16: with 16 rows of queries and two operations a byte of K
 // or V an M = 128 tcgen05 tile would be seven eighths padding, and dequantised operands would have to

@@ -169,6 +169,25 @@ def test_same_bits_every_time_and_on_another_stream():
     assert torch.equal(o, o2) and all(torch.equal(a, b) for a, b in zip(first, again))
 
 
+def test_step_in_a_graph_follows_its_inputs():
+    """Forward and backward captured once and replayed on other values."""
+    q, k, v, do = _inputs(1, 8, 2, 1500, 1500, 64, BF, seed=21)
+    def step():
+        o, lse = fa.forward_window(q, k, v, 300, 4, return_lse=True)
+        return (o, lse, *fa.backward_window(do, q, k, v, o, lse, 300, 4))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (22, 23):
+        for t, x in zip((q, k, v, do), _inputs(1, 8, 2, 1500, 1500, 64, BF, seed=seed)):
+            t.copy_(x)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
 def test_matches_plain_causal_forward_without_a_window():
     q, k, v, _ = _inputs(1, 4, 4, 900, 900, 128, BF, seed=12)
     u = oracle.unit(BF)
