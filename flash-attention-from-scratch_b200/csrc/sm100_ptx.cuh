@@ -541,13 +541,4 @@ __device__ __forceinline__ float2 unpack_half2(uint32_t r) {
     return __half22float2(*reinterpret_cast<const __half2*>(&r));
 }
 
-template <bool BF16>
-__device__ __forceinline__ float2 unpack2(uint32_t r) {
-    if constexpr (BF16) {
-        return make_float2(__uint_as_float(r << 16), __uint_as_float(r & 0xFFFF0000u));
-    } else {
-        return unpack_half2(r);
-    }
-}
-
 }  // namespace fa_sm100

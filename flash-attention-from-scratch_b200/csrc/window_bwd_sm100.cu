@@ -33,8 +33,8 @@
 // quarter of the SMs idle (254 lists of 132 tiles on 148 SMs). A cut list's parts leave float32
 // sums in the workspace, at most two a CTA, and a last kernel adds them up in order.
 
-// Measured, bf16, D 128 (of 1689 TFLOP/s): 16 x 8191 on 4 kv heads, window 1024 + 4 sinks 283 us, 8 x 16384 on 2,
-// window 4096 710 us (850 TFLOP/s of the 5 products of visible pairs, 1190 of the 7 computed). A DKV step is
+// Measured, bf16, D 128 (of 1689 TFLOP/s): 16 x 8191 on 4 kv heads, window 1024 + 4 sinks 289 us, 8 x 16384 on 2,
+// window 4096 720 us (836 TFLOP/s of the 5 products of visible pairs, 1170 of the 7 computed). A DKV step is
 // 2048 cycles of products and 2400 of shared memory (192 KB of operands, 64 KB arriving, the columns' LSE and delta),
 // a dQ step 1536 and 1800, which is what bounds them: without the exponentials they take as long. Tiles
 // shared by two SMs (cta_group::2) would halve the streamed operands.
@@ -65,9 +65,10 @@ constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
 constexpr int kLoaderWarp = 10;
 constexpr int kScoreWarp = 11;  // issues S; kMmaWarp the other products
-// Registers: 8 softmax warps take 208 and the other four leave 88, the launch's 384 x 168 in all.
-constexpr int kRegsSoftmax = 208;
-constexpr int kRegsOther = 88;
+// Registers: 8 softmax warps take 224 and the other four keep 56, the launch's 384 x 168 in all (P of two tiles
+// in float32: 208 and 88 spill more and take 2% longer).
+constexpr int kRegsSoftmax = 224;
+constexpr int kRegsOther = 56;
 static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kBwdThreads * 168, "register split");
 constexpr int kEmuPer8 = 3;  // column pairs of 8 whose 2^x runs on the FMA pipe (1: 2% slower, 4: the same)
 
@@ -424,7 +425,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             const float row_delta = next_delta;
             more = next_item<Cfg::DKV>(args, cursor, next);
             statistics();
-            // P of tile i (DKV: packed; dQ: fp32 bits) from S.
+            // P of tile i in float32 from S. It is rounded to 16 bits for dV's product alone; dS is made of P and dP
+            // in float32 and rounded once, for its own products. (With the rounded P in dS dK was off by twice
+            // what rounding dK itself costs; this takes 3% longer.)
             auto probabilities = [&](int i, uint32_t (&p)[64]) {
                 int tile_row, head;
                 stream_tile<Cfg>(args, it, i, tile_row, head);
@@ -434,23 +437,26 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                 }
                 tc_fence_after();
                 tmem_ld64(t_s, p);
-                // The columns' LSE comes meanwhile: shared memory is busy with the products' operands.
-                [[maybe_unused]] float4 lse2[16];
+                // Half of the columns' LSE comes meanwhile: shared memory is busy with the products' operands.
+                [[maybe_unused]] float4 early[8];
                 if constexpr (Cfg::DKV) {
 #pragma unroll
-                    for (int c4 = 0; c4 < 16; ++c4) {
-                        lse2[c4] = *reinterpret_cast<const float4*>(&sh.lse2[g % 2][col0 + 4 * c4]);
+                    for (int c4 = 0; c4 < 8; ++c4) {
+                        early[c4] = *reinterpret_cast<const float4*>(&sh.lse2[g % 2][col0 + 4 * c4]);
                     }
                 }
                 tmem_wait_ld();
-                // S and LSE are in registers: the next scores may take S's columns, the LSE of tile i + 2 its slot.
-                arrive(&sh.s_read[g % 2]);
+                if constexpr (!Cfg::DKV) {
+                    arrive(&sh.s_read[g % 2]);  // S is in registers: the next scores may take its columns
+                }
 #pragma unroll
                 for (int c4 = 0; c4 < 16; ++c4) {
                     float2 neg[2];
                     if constexpr (Cfg::DKV) {
-                        neg[0] = make_float2(lse2[c4].x, lse2[c4].y);
-                        neg[1] = make_float2(lse2[c4].z, lse2[c4].w);
+                        const float4 l4 =
+                            c4 < 8 ? early[c4 % 8] : *reinterpret_cast<const float4*>(&sh.lse2[g % 2][col0 + 4 * c4]);
+                        neg[0] = make_float2(l4.x, l4.y);
+                        neg[1] = make_float2(l4.z, l4.w);
                     } else {
                         neg[0] = neg[1] = make_float2(row_lse2, row_lse2);
                     }
@@ -462,6 +468,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                         p[c] = f2u(x.x);
                         p[c + 1] = f2u(x.y);
                     }
+                }
+                if constexpr (Cfg::DKV) {
+                    arrive(&sh.s_read[g % 2]);  // ... and the LSE of tile i + 2 its slot
                 }
                 // Masks: query position minus key position in [0, window), or the key a sink.
                 const int q_row = Cfg::DKV ? tile_row : it.row0;
@@ -480,14 +489,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
                 for (int c = 0; c < 64; c += 2) {
                     const float2 x = make_float2(u2f(p[c]), u2f(p[c + 1]));
-                    const float2 e = ((c / 2) % 8) < kEmuPer8 ? exp2_poly2_deg3(x)
+                    const float2 e = ((c / 2) % 8) < kEmuPer8 ? exp2_poly2(x)
                                                               : make_float2(ex2_approx(x.x), ex2_approx(x.y));
-                    if constexpr (Cfg::DKV) {
-                        p[c / 2] = pack2<Cfg::BF16>(e.x, e.y);
-                    } else {
-                        p[c] = f2u(e.x);
-                        p[c + 1] = f2u(e.y);
-                    }
+                    p[c] = f2u(e.x);
+                    p[c + 1] = f2u(e.y);
                 }
             };
             // dS of the tile whose dP is next, from its P.
@@ -497,22 +502,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                     return;
                 }
                 tc_fence_after();
+                uint32_t dp[32];
                 [[maybe_unused]] const float* delta = sh.delta[gd % kXStages] + col0;
-                uint32_t dp[64];
-                tmem_ld64(t_dp, dp);
-                [[maybe_unused]] float4 delta_half[8];
-                if constexpr (Cfg::DKV) {
-#pragma unroll
-                    for (int c4 = 0; c4 < 8; ++c4) {
-                        delta_half[c4] = *reinterpret_cast<const float4*>(delta + 4 * c4);
-                    }
-                }
-                tmem_wait_ld();
 #pragma unroll
                 for (int c4 = 0; c4 < 16; ++c4) {
+                    if (c4 % 8 == 0) {
+                        tmem_ld32(t_dp + 4 * c4, dp);
+                        tmem_wait_ld();
+                    }
                     float2 d[2];
                     if constexpr (Cfg::DKV) {
-                        const float4 d4 = c4 < 8 ? delta_half[c4 % 8] : *reinterpret_cast<const float4*>(delta + 4 * c4);
+                        const float4 d4 = *reinterpret_cast<const float4*>(delta + 4 * c4);
                         d[0] = make_float2(d4.x, d4.y);
                         d[1] = make_float2(d4.z, d4.w);
                     } else {
@@ -521,20 +521,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int c = 4 * c4 + 2 * h;
-                        float2 x;
-                        if constexpr (Cfg::DKV) {
-                            x = unpack2<Cfg::BF16>(p[c / 2]);
-                        } else {
-                            x = make_float2(u2f(p[c]), u2f(p[c + 1]));
-                        }
-                        const float2 y = __fmul2_rn(x, __fadd2_rn(make_float2(u2f(dp[c]), u2f(dp[c + 1])), d[h]));
+                        const float2 y = __fmul2_rn(make_float2(u2f(p[c]), u2f(p[c + 1])), __fadd2_rn(make_float2(u2f(dp[c % 32]), u2f(dp[c % 32 + 1])), d[h]));
                         w[c / 2] = pack2<Cfg::BF16>(y.x, y.y);
                     }
                 }
             };
             if constexpr (Cfg::DKV) {
                 // Step i: P of tile i, dS of tile i - 1.
-                uint32_t p_last[32];
+                uint32_t p_last[64];
                 for (int i = 0; i <= it.n; ++i) {
                     uint32_t p[64], w[32];
                     if (i < it.n) {
@@ -556,10 +550,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                     if (i < it.n) {
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {
-                            p_last[c] = p[c];
+                            w[c] = pack2<Cfg::BF16>(u2f(p[2 * c]), u2f(p[2 * c + 1]));
                         }
                         if (ok) {
-                            tmem_st32(t_p, p_last);
+                            tmem_st32(t_p, w);
+                        }
+#pragma unroll
+                        for (int c = 0; c < 64; ++c) {
+                            p_last[c] = p[c];
                         }
                     }
                     if (ok) {
