@@ -870,25 +870,35 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
 }
 
-// delta[row] = dO.O, a row by D / 8 lanes.
+// delta[row] = dO.O, a row by D / 8 lanes, kDeltaRows rows a thread of head blockIdx.y. Bound by DRAM bytes.
+constexpr int kDeltaRows = 4;
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ FaWindowParams p, float* delta) {
     constexpr int C = D / 8;
-    const long long row = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / C;
+    constexpr int kGroups = 256 / C;
     const int chunk = static_cast<int>(threadIdx.x) % C;
-    float sum = 0.0f;
-    const long long rows = static_cast<long long>(p.batch) * p.heads * p.q_len;
-    if (row < rows) {
-        const int bh = static_cast<int>(row / p.q_len);
-        const int64_t i = row - static_cast<long long>(bh) * p.q_len;
-        const int b = bh / p.heads;
-        const int h = bh - b * p.heads;
-        const uint4 o = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.o) + b * p.o_stride[0] +
-                                                             h * p.o_stride[1] + i * p.o_stride[2] + chunk * 8));
-        const uint4 d = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.d_o) + b * p.do_stride[0] +
-                                                             h * p.do_stride[1] + i * p.do_stride[2] + chunk * 8));
-        const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
-        const uint32_t dw[4] = {d.x, d.y, d.z, d.w};
+    const int bh = static_cast<int>(blockIdx.y);
+    const int b = bh / p.heads;
+    const int h = bh - b * p.heads;
+    const uint16_t* o_head = static_cast<const uint16_t*>(p.o) + b * p.o_stride[0] + h * p.o_stride[1] + chunk * 8;
+    const uint16_t* d_head = static_cast<const uint16_t*>(p.d_o) + b * p.do_stride[0] + h * p.do_stride[1] + chunk * 8;
+    const int row0 = static_cast<int>(blockIdx.x) * (kGroups * kDeltaRows) + static_cast<int>(threadIdx.x) / C;
+    uint4 o[kDeltaRows], d[kDeltaRows];
+#pragma unroll
+    for (int i = 0; i < kDeltaRows; ++i) {
+        const int64_t row = row0 + i * kGroups;
+        o[i] = d[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < p.q_len) {
+            o[i] = __ldg(reinterpret_cast<const uint4*>(o_head + row * p.o_stride[2]));
+            d[i] = __ldg(reinterpret_cast<const uint4*>(d_head + row * p.do_stride[2]));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kDeltaRows; ++i) {
+        const uint32_t ow[4] = {o[i].x, o[i].y, o[i].z, o[i].w};
+        const uint32_t dw[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
+        float sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             if constexpr (BF16) {
@@ -901,29 +911,25 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ FaWi
                 sum = fmaf(x.y, y.y, sum);
             }
         }
-    }
 #pragma unroll
-    for (int o = C / 2; o > 0; o >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    }
-    if (row < rows && chunk == 0) {
-        delta[row] = sum;
+        for (int k = C / 2; k > 0; k >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, k);
+        }
+        const int row = row0 + i * kGroups;
+        if (row < p.q_len && chunk == 0) {
+            delta[static_cast<long long>(bh) * p.q_len + row] = sum;
+        }
     }
 }
 
-// Adds up the parts of the list that is cut at the end of CTA blockIdx.x's range (of the dK, dV pass, then
-// of the dQ pass), if that is its first cut; a quarter of the dims by blockIdx.y % 4, dV and dK by
-// blockIdx.y / 4. Lanes take 8 rows x 4 groups of 4 dims: 128-byte reads, 32-byte writes.
+// Adds up the parts of the list that is cut at the end of CTA `boundary`'s range (of the dK, dV pass, then
+// of the dQ pass), if that is its first cut; a quarter of the dims of dV (which 0), dK or dQ (1). Lanes take 8 rows x 4 groups of 4 dims: 128-byte reads, 32-byte writes.
 constexpr int kJoinThreads = 256;
 
 template <int D, bool BF16, bool DKV>
-__device__ __forceinline__ void join(const BwdArgs& a, int boundary) {
+__device__ __forceinline__ void join(const BwdArgs& a, int boundary, int which, int quarter) {
     __shared__ long long warp_sum[kJoinThreads / 32];
     __shared__ int tile, offset;
-    const int which = static_cast<int>(blockIdx.y) / 4;
-    if (which >= (DKV ? 2 : 1)) {
-        return;
-    }
     const long long cut = (boundary + 1) * a.per;
     const int bx = static_cast<int>(cut / a.head_steps);
     locate_tile<DKV, kJoinThreads>(a, cut - bx * a.head_steps, warp_sum, &tile, &offset);
@@ -942,26 +948,38 @@ __device__ __forceinline__ void join(const BwdArgs& a, int boundary) {
     uint16_t* dst = static_cast<uint16_t*>(first_out ? a.out0 : a.out1) + b * st[0] + h * st[1];
     const int rows = DKV ? a.k_len : a.q_len;
     const int lane = static_cast<int>(threadIdx.x) % 32;
-    const int quarter = static_cast<int>(blockIdx.y) % 4;
     constexpr int kOutputs = DKV ? 2 : 1;
-    for (int u = static_cast<int>(threadIdx.x) / 32; u < (D / 64) * (kTile / 8); u += kJoinThreads / 32) {
+    // All of a thread's pieces of a part are on their way at once.
+    constexpr int kPieces = (D / 64) * (kTile / 8) / (kJoinThreads / 32);
+    float4 sum[kPieces];
+    int at[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const int u = static_cast<int>(threadIdx.x) / 32 + i * (kJoinThreads / 32);
         const int row = u / (D / 64) * 8 + lane % 8;
         const int four = quarter * (D / 16) + u % (D / 64) * 4 + lane / 8;
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (long long c = boundary; c <= last; ++c) {
-            // The list is its first CTA's last part unless it starts that CTA's range; else a first part.
-            const long long record = 2 * c + (c * a.per >= begin ? 0 : 1);
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(a.parts) +
-                                    ((record * kOutputs + which) * (D / 4) + four) * kTile + row);
-            sum.x += x.x;
-            sum.y += x.y;
-            sum.z += x.z;
-            sum.w += x.w;
+        at[i] = four * kTile + row;
+        sum[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    for (long long c = boundary; c <= last; ++c) {
+        // The list is its first CTA's last part unless it starts that CTA's range; else a first part.
+        const long long record = 2 * c + (c * a.per >= begin ? 0 : 1);
+        const float4* src = reinterpret_cast<const float4*>(a.parts) + (record * kOutputs + (DKV ? which : 0)) * (D / 4) * kTile;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const float4 x = __ldcg(src + at[i]);
+            sum[i].x += x.x;
+            sum[i].y += x.y;
+            sum[i].z += x.z;
+            sum[i].w += x.w;
         }
+    }
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const int row = at[i] % kTile;
         if (it.row0 + row < rows) {
-            *reinterpret_cast<uint2*>(dst + static_cast<int64_t>(it.row0 + row) * st[2] + four * 4) =
-                make_uint2(pack2<BF16>(sum.x, sum.y), pack2<BF16>(sum.z, sum.w));
+            *reinterpret_cast<uint2*>(dst + static_cast<int64_t>(it.row0 + row) * st[2] + at[i] / kTile * 4) =
+                make_uint2(pack2<BF16>(sum[i].x, sum[i].y), pack2<BF16>(sum[i].z, sum[i].w));
         }
     }
 }
@@ -970,11 +988,13 @@ template <int D, bool BF16>
 __global__ void __launch_bounds__(kJoinThreads) window_bwd_join_kernel(const __grid_constant__ BwdArgs dkv,
                                                                        const __grid_constant__ BwdArgs dq) {
     cudaGridDependencySynchronize();
-    const int block = static_cast<int>(blockIdx.x);
-    if (block < dkv.grid - 1) {
-        join<D, BF16, true>(dkv, block);
+    const int quarter = static_cast<int>(blockIdx.x) % 4;
+    const int unit = static_cast<int>(blockIdx.x) / 4;
+    const int dkv_units = 2 * (dkv.grid - 1);
+    if (unit < dkv_units) {
+        join<D, BF16, true>(dkv, unit / 2, unit % 2, quarter);
     } else {
-        join<D, BF16, false>(dq, block - (dkv.grid - 1));
+        join<D, BF16, false>(dq, unit - dkv_units, 1, quarter);
     }
 }
 
@@ -1054,11 +1074,9 @@ cudaError_t bwd(const FaWindowParams& p, DeviceStatus* status, unsigned epoch, v
     strides(dkv.out0_stride, p.dv_stride);
     strides(dkv.out1_stride, p.dk_stride);
     strides(dq.out1_stride, p.dq_stride);
-    const long long rows = static_cast<long long>(p.batch) * p.heads * p.q_len;
-    const long long delta_grid = (rows * (D / 8) + 255) / 256;
-    if (delta_grid > 0x7fffffffLL) {
-        return cudaErrorInvalidConfiguration;
-    }
+    const int delta_rows = 256 / (D / 8) * kDeltaRows;
+    const dim3 delta_grid(static_cast<unsigned>((p.q_len + delta_rows - 1) / delta_rows),
+                          static_cast<unsigned>(p.batch * p.heads));
     CUtensorMap q, k, v, d_o;
     if (encode_strided_map(&q, p.q, p.q_stride, p.batch, p.heads, p.q_len, D, kTile, BF16) != CUDA_SUCCESS ||
         encode_strided_map(&k, p.k, p.k_stride, p.batch, p.kv_heads, p.k_len, D, kTile, BF16) != CUDA_SUCCESS ||
@@ -1075,7 +1093,7 @@ cudaError_t bwd(const FaWindowParams& p, DeviceStatus* status, unsigned epoch, v
     if (err != cudaSuccess) {
         return err;
     }
-    delta_kernel<D, BF16><<<static_cast<unsigned>(delta_grid), 256, 0, stream>>>(p, delta);
+    delta_kernel<D, BF16><<<delta_grid, 256, 0, stream>>>(p, delta);
     err = cudaGetLastError();
     if (err != cudaSuccess) {
         return err;
@@ -1086,9 +1104,9 @@ cudaError_t bwd(const FaWindowParams& p, DeviceStatus* status, unsigned epoch, v
         err = launch_early(window_bwd_kernel<Dq>, dim3(static_cast<unsigned>(dq.grid)), kBwdThreads, bwd_smem<Dq>(),
                            stream, q, d_o, k, v, dq);
     }
-    const int cuts = dkv.grid + dq.grid - 2;
-    if (err == cudaSuccess && cuts > 0) {
-        err = launch_early(window_bwd_join_kernel<D, BF16>, dim3(static_cast<unsigned>(cuts), 8), kJoinThreads, 0, stream,
+    const int units = 2 * (dkv.grid - 1) + dq.grid - 1;  // outputs of lists that may be cut
+    if (err == cudaSuccess && units > 0) {
+        err = launch_early(window_bwd_join_kernel<D, BF16>, dim3(static_cast<unsigned>(4 * units)), kJoinThreads, 0, stream,
                            dkv, dq);
     }
     return err;
