@@ -737,8 +737,11 @@ __global__ void __launch_bounds__(kThreads) cached_join_kernel(const __grid_cons
     constexpr int PER = D / 32;
     const long long k = blockIdx.x + 1;
     const Range range = locate<C>(p, grid, [&](long long per) { return k * per; });
-    if (range.found < 0) {
+    // One CTA waits whatever it finds to do, so that this kernel's end stands for the end of the one before.
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
         cudaGridDependencySynchronize();
+    }
+    if (range.found < 0) {
         return;
     }
     const int group = p.heads / p.cache.kv_heads;
@@ -752,13 +755,12 @@ __global__ void __launch_bounds__(kThreads) cached_join_kernel(const __grid_cons
     const int lane = static_cast<int>(threadIdx.x) % 32;
     const int row = SPREAD ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * kWarps + warp;
     const int row_first = SPREAD ? row : static_cast<int>(blockIdx.y) * kWarps;
-    // Every CTA waits, with nothing to do as well: this kernel's end stands for the end of the one before.
-    cudaGridDependencySynchronize();
     if (start == k * range.per || start / range.per != k - 1 || row0 + row_first >= rows) {
         return;
     }
     const long long c0 = start / range.per;
     const long long c1 = (start + s.tiles - 1) / range.per;
+    cudaGridDependencySynchronize();  // the records are there
     float m = -INFINITY, l = 0.0f;
     float o[PER];
 #pragma unroll
