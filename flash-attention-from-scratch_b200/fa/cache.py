@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 import struct
 
 import torch
@@ -30,13 +31,43 @@ _APPEND = struct.Struct("@" + _CACHE + "6P9q3iBB2x")
 _CACHED = struct.Struct("@" + _CACHE + "2P3q3ifB3x4x")
 
 
+def _tensor(name: str) -> property:
+    """One of a cache's tensors. Another one in its place is looked at by the next call."""
+
+    def put(self, t):
+        setattr(self, name, t)
+        self._pointers = None
+
+    return property(operator.attrgetter(name), put)
+
+
 class PagedKVCache:
     """The pool of pages: k, v [num_pages, kv_heads, page_size, head_dim] (the last two dims
     contiguous), float8_e4m3fn with k_scale, v_scale [num_pages, kv_heads] float32 (a value is its
-    code times its page's and head's scale), or float16 / bfloat16 without scales."""
+    code times its page's and head's scale), or float16 / bfloat16 without scales.
+
+    The four may be replaced (a pool grows by cache.k = torch.cat([cache.k, more]), and so on for the
+    others): the next call checks them and uses them. A captured graph keeps those it was captured with."""
+
+    k, v, k_scale, v_scale = (_tensor(name) for name in ("_k", "_v", "_k_scale", "_v_scale"))
+    num_pages = property(lambda self: self._k.shape[0])
+    kv_heads = property(lambda self: self._k.shape[1])
+    page_size = property(lambda self: self._k.shape[2])
+    head_dim = property(lambda self: self._k.shape[3])
+    device = property(lambda self: self._k.device)
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None) -> None:
+        self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
+        self._lay_out()
+
+    def _addresses(self) -> tuple[int, int, int, int]:
+        ks, vs = self._k_scale, self._v_scale
+        return (self._k.data_ptr(), self._v.data_ptr(), 0 if ks is None else ks.data_ptr(), 0 if vs is None else vs.data_ptr())
+
+    def _lay_out(self) -> None:
+        """Checks the tensors and takes down the parts of FaCache that stay as they are with them."""
+        k, v, k_scale, v_scale = self._k, self._v, self._k_scale, self._v_scale
         for t in (k, v):
             if not t.is_cuda:
                 raise RuntimeError("the cache's k and v must be CUDA tensors")
@@ -55,16 +86,19 @@ class PagedKVCache:
             if s is not None and (s.shape != k.shape[:2] or s.dtype != torch.float32 or s.device != k.device
                                   or not s.is_contiguous()):
                 raise RuntimeError("k_scale and v_scale must be contiguous float32 [pages, kv_heads] on k's device")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
-        # The parts of FaCache that stay as they are: the pool's pointers, its strides, its sizes.
-        (k0, k1, _, _), (v0, v1, _, _) = k.stride(), v.stride()
-        many, heads = self.num_pages > 1, self.kv_heads > 1
-        self._pointers = tuple(0 if t is None else t.data_ptr() for t in (k, v, k_scale, v_scale))
-        self._strides = (k0 * many, k1 * heads, v0 * many, v1 * heads)
-        self._sizes = (self.kv_heads, self.head_dim)
+        (pages, heads, page_size, head_dim), (k0, k1, _, _), (v0, v1, _, _) = k.shape, k.stride(), v.stride()
+        self._strides = (k0 * (pages > 1), k1 * (heads > 1), v0 * (pages > 1), v1 * (heads > 1))
+        self._pool = (pages, page_size)
+        self._heads = (heads, head_dim)
         self._dtype = _C.DTYPES.get(k.dtype, _C.FA_DTYPE_FLOAT8_E4M3)
-        self.device, self._index = k.device, k.get_device()
+        self._tokens_as = None if e4m3 else k.dtype
+        self._device, self._index = k.device, k.get_device()
+        self._pointers = self._addresses()
+
+    def _look(self) -> None:
+        """Memory that was replaced, or moved under a tensor that was not, is never reached by its old address."""
+        if self._addresses() != self._pointers:
+            self._lay_out()
 
     @classmethod
     def empty(cls, num_pages: int, page_size: int, kv_heads: int, head_dim: int,
@@ -80,7 +114,7 @@ class PagedKVCache:
 
     def _fields(self, table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor | None, batch: int, tokens: int):
         """FaCache's fields for these sequences, checked."""
-        device = self.device
+        device = self._device
         if table.dtype != torch.int32 or table.dim() != 2 or table.device != device:
             raise RuntimeError("page_table must be an int32 [B, pages] tensor on the cache's device")
         (rows, width), (stride, unit) = table.shape, table.stride()
@@ -90,26 +124,26 @@ class PagedKVCache:
             if t.dtype != torch.int32 or t.shape != (batch,) or t.device != device or not t.is_contiguous():
                 raise RuntimeError("lengths and counts must be contiguous int32 [B] tensors on the cache's device")
         return (*self._pointers, table.data_ptr(), lengths.data_ptr(), 0 if counts is None else counts.data_ptr(),
-                *self._strides, stride if batch > 1 else width, self.num_pages, self.page_size, width, *self._sizes,
-                batch, tokens, self._dtype)
+                *self._strides, stride if batch > 1 else width, *self._pool, width, *self._heads, batch, tokens, self._dtype)
 
 
 def _check_tokens(cache: PagedKVCache, *tensors: torch.Tensor) -> None:
-    first = tensors[0]
-    dtype, want = first.dtype, None
+    cache._look()
+    only, device, dim = cache._tokens_as, cache._device, cache._heads[1]
+    dtype, want = tensors[0].dtype, None
     for t in tensors:
         if not t.is_cuda:
             raise RuntimeError("q, k, v must be CUDA tensors")
         if t.dtype not in _C.DTYPES:
             raise RuntimeError("q, k, v must be float16 (or bfloat16)")
-        if t.dtype != dtype or (cache.k_scale is None and t.dtype != cache.k.dtype):
+        if t.dtype != dtype or (only is not None and dtype != only):
             raise RuntimeError("q, k, v must have the same dtype, that of a 16-bit cache")
         if t.dim() != 4:
             raise RuntimeError("q, k, v must have shape [B, H, T, D]")
-        if t.device != cache.device:
+        if t.device != device:
             raise RuntimeError("q, k, v must be on the cache's device")
         b, _, n, d = t.shape
-        if (b, n) != (want or (b, n)) or d != cache.head_dim:
+        if (b, n) != (want or (b, n)) or d != dim:
             raise RuntimeError("q, k, v must have the same batch and tokens, and the cache's head dim")
         want = (b, n)
 
@@ -139,7 +173,7 @@ def append_kv(
     and starts anew with the page's first slot. No two sequences may append to one page."""
     tensors = (k, v) if q is None else (k, v, q)
     _check_tokens(cache, *tensors)
-    if k.shape != v.shape or k.shape[1] != cache.kv_heads:
+    if k.shape != v.shape or k.shape[1] != cache._heads[0]:
         raise RuntimeError("k and v must have shape [B, kv_heads, T, D]")
     batch, _, tokens, dim = k.shape
     rows = half = 0
@@ -202,5 +236,5 @@ def forward_cached(
     scale = 1.0 / math.sqrt(dim) if softmax_scale is None else float(softmax_scale)
     params = _CACHED.pack(*fields, q.data_ptr(), o.data_ptr(), *_tensor_strides(q), heads, window, sinks, scale,
                           _C.DTYPES[q.dtype])
-    _on_device(cache._index, _run_cached, params, cache.device)
+    _on_device(cache._index, _run_cached, params, cache._device)
     return o

@@ -1,0 +1,72 @@
+"""The streaming operators at the edges of their contracts: a cache whose tensors are replaced, and
+what else a caller may do or bring that the ordinary cases do not show."""
+
+import math
+
+import pytest
+import torch
+
+import fa
+import stream_oracle as oracle
+from fa import _C
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+HALF, BF, E4M3 = torch.float16, torch.bfloat16, torch.float8_e4m3fn
+
+
+def _ints(*x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _rand(gen, shape, dtype, scale=1.0):
+    return (torch.randn(shape, generator=gen, device=DEV) * scale).to(dtype)
+
+
+def _bytes(t):
+    return t.view(torch.uint8)
+
+
+# ------------------------------------------------------------------------------------ the cache
+
+
+def _grown(t, more):
+    """t with `more` pages of zeros after its own."""
+    new = torch.cat([_bytes(t), torch.zeros((more, *_bytes(t).shape[1:]), dtype=torch.uint8, device=DEV)])
+    return new.view(t.dtype)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, HALF])
+def test_cache_follows_tensors_that_are_replaced(dtype):
+    """A pool that grows, one that is moved to other memory under the same tensor: what was there is
+    neither read nor written any more. (The old tensors stay alive here.)"""
+    gen = torch.Generator(DEV).manual_seed(1)
+    cache = fa.PagedKVCache.empty(2, 16, 2, 64, dtype=dtype, device=DEV)
+    k, v, q = (_rand(gen, (1, h, 40, 64), HALF) for h in (2, 2, 4))
+    fa.append_kv(cache, k[:, :, :32], v[:, :, :32], _ints(1, 0).view(1, 2), _ints(32))
+    old = [t for t in (cache.k, cache.v, cache.k_scale, cache.v_scale) if t is not None]
+    was = [_bytes(t).clone() for t in old]
+
+    cache.k = _grown(cache.k, 1)
+    assert cache.num_pages == 3
+    with pytest.raises(RuntimeError, match="same shape"):  # v has not followed yet
+        fa.append_kv(cache, k[:, :, 32:], v[:, :, 32:], _ints(1, 0, 2).view(1, 3), _ints(40))
+    cache.v = _grown(cache.v, 1)
+    if dtype == E4M3:
+        cache.k_scale, cache.v_scale = (torch.cat([s, torch.ones(1, 2, device=DEV)]) for s in (cache.k_scale, cache.v_scale))
+    table = _ints(1, 0, 2).view(1, 3)
+    fa.append_kv(cache, k[:, :, 32:], v[:, :, 32:], table, _ints(40))
+    whole = fa.PagedKVCache.empty(3, 16, 2, 64, dtype=dtype, device=DEV)
+    fa.append_kv(whole, k, v, table, _ints(40))
+    assert torch.equal(_bytes(cache.k), _bytes(whole.k)) and torch.equal(_bytes(cache.v), _bytes(whole.v))
+    assert torch.equal(fa.forward_cached(q[:, :, -1:], cache, table, _ints(40)), fa.forward_cached(q[:, :, -1:], whole, table, _ints(40)))
+    assert all(torch.equal(_bytes(t), w) for t, w in zip(old, was))
+
+    moved = cache.k.data
+    was = _bytes(moved).clone()
+    cache.k.data = _bytes(cache.k).clone().view(dtype)
+    fa.append_kv(cache, -k[:, :, :8], v[:, :, :8], table, _ints(8))
+    fa.append_kv(whole, -k[:, :, :8], v[:, :, :8], table, _ints(8))
+    assert torch.equal(_bytes(moved), was) and torch.equal(_bytes(cache.k), _bytes(whole.k))
+    assert _C.device_status(0) == 0
