@@ -132,27 +132,31 @@ __device__ __forceinline__ uint32_t v_offset(int r, int c) {
     }
 }
 
-// What a sequence shows its queries: positions [0, sinks) and [first, last], as a list of key tiles.
+// Positions that the page tables have a place for (below 2^31).
+__device__ __forceinline__ int held(const FaCache& c) { return c.max_pages * c.page_size; }
+
+// What a sequence shows its queries: positions [0, sinks) and [first, last], as a list of key tiles. The list
+// ends with the page table, whatever length the device holds, so that a call's work is bounded by its arguments.
 struct Sequence {
     int pos0;    // position of its first query (may be negative)
     int count;   // queries
-    int last;    // last position any query sees, -1 if none
-    int first;   // first position of the earliest window
+    int last;    // last position any query sees and the table has, -1 if none
+    int first;   // first position of the earliest window, at most the table's end
     int sink_tiles, first_tile, tiles;
 };
 
 template <class C>
 __device__ __forceinline__ Sequence sequence(const FaCachedParams& p, int b) {
     Sequence s;
-    const int len = p.cache.lengths[b];
+    const int len = max(p.cache.lengths[b], 0);
     s.count = p.cache.counts != nullptr ? min(max(p.cache.counts[b], 0), p.cache.tokens) : p.cache.tokens;
     s.pos0 = len - s.count;
-    s.last = s.count > 0 ? max(len - 1, -1) : -1;
-    s.first = window_first(max(s.pos0, 0), p.window);
+    s.last = s.count > 0 ? min(len, held(p.cache)) - 1 : -1;
+    s.first = min(window_first(max(s.pos0, 0), p.window), held(p.cache));
     s.first_tile = s.first / C::kKeys;
     s.sink_tiles = min((min(p.sinks, s.first) + C::kKeys - 1) / C::kKeys, s.first_tile);
     // A sequence that shows nothing keeps one (hidden) tile, so that its rows are written.
-    s.tiles = s.last < 0 ? 1 : s.sink_tiles + s.last / C::kKeys - s.first_tile + 1;
+    s.tiles = s.last < 0 ? 1 : max(s.sink_tiles + s.last / C::kKeys - s.first_tile + 1, 1);
     return s;
 }
 
@@ -240,6 +244,10 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
     uint8_t* ring = smem + warp * kStages * 2 * kTileBytes;
     float* aux = reinterpret_cast<float*>(smem + kWarps * kStages * 2 * kTileBytes) + warp * kStages * kAuxFloats;
 
+    if (threadIdx.x == 0 && s.count > 0 && s.pos0 + s.count > held(c)) {
+        atomicOr(&status->code, kStatusBadPage);  // positions that the table has no place for are left out
+    }
+
     // Pages of a key tile: `spans` of them (at most 8), 2^log2_span tokens each.
     const int log2_page = 31 - __clz(c.page_size);
     const int log2_span = C::ONE_PAGE ? 31 - __clz(C::kKeys) : log2_page;
@@ -256,8 +264,7 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
             const int key = tile_key(v) + (C::ONE_PAGE ? 0 : lane << log2_span);
             const int end = key + (1 << log2_span) - 1;
             if (key <= s.last && (end >= s.first || key < p.sinks)) {
-                const int page = key >> log2_page;
-                id = page < c.max_pages ? __ldg(table + page) : -1;
+                id = __ldg(table + (key >> log2_page));
                 if (id < 0 || id >= c.num_pages) {
                     id = -1;
                     atomicOr(&status->code, kStatusBadPage);
@@ -443,7 +450,7 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
 
         // log2 of the weights, and what is hidden.
         const bool whole = key0 + C::kKeys - 1 <= s.pos0 &&
-                           (p.window == 0 || s.last - key0 < p.window || key0 + C::kKeys <= p.sinks);
+                           (p.window == 0 || s.pos0 + s.count - 1 - key0 < p.window || key0 + C::kKeys <= p.sinks);
         float inv_vs[C::kNTiles];
         float shrink = 1.0f;  // of P, for scales below 2^-60
         float tile_shrink[C::kNTiles];

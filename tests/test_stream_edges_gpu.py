@@ -70,3 +70,29 @@ def test_cache_follows_tensors_that_are_replaced(dtype):
     fa.append_kv(whole, -k[:, :, :8], v[:, :, :8], table, _ints(8))
     assert torch.equal(_bytes(moved), was) and torch.equal(_bytes(cache.k), _bytes(whole.k))
     assert _C.device_status(0) == 0
+
+
+def _filled(gen, batch, pages, page, heads, d, dtype):
+    """A cache of values near 1 and a table of all its pages, in random order."""
+    table = torch.randperm(batch * pages, generator=gen, device=DEV).to(torch.int32).view(batch, pages)
+    k, v = (_rand(gen, (batch * pages, heads, page, d), HALF).to(dtype) for _ in "kv")
+    scales = (torch.ones(batch * pages, heads, device=DEV) for _ in "kv") if dtype == E4M3 else (None, None)
+    return fa.PagedKVCache(k, v, *scales), table
+
+
+@pytest.mark.parametrize("dtype", [E4M3, HALF])
+@pytest.mark.parametrize("page,pages", [(8, 3), (16, 4), (64, 20)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (30, 0), (30, 5), (5000, 40)])
+def test_lengths_beyond_the_table_end_with_it(page, pages, window, sinks, dtype):
+    """A length that the table has no place for costs no more than the table's own, and what the table has of
+    its view is attended to; the other sequences are as they would be."""
+    gen = torch.Generator(DEV).manual_seed(2)
+    cache, table = _filled(gen, 6, pages, page, 2, 64, dtype)
+    most = page * pages
+    q = _rand(gen, (6, 4, 2, 64), HALF)
+    lengths = _ints(most, most + 1, most + 20, 2**31 - 1, -(2**31), 7)
+    got = fa.forward_cached(q, cache, table, lengths, window=window, sinks=sinks)
+    assert _C.device_status(0, clear=True) == 32
+    lengths = lengths.clamp(min=0)
+    want, vmax = oracle.cached(q, cache, table, lengths, None, window, sinks)
+    oracle.check(got, want, oracle.forward_bound(want, vmax, oracle.unit(HALF), oracle.unit(HALF)), "O")
