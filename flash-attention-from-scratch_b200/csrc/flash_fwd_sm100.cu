@@ -892,11 +892,11 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
             Item it;
             decode(idx, it);
             if constexpr (Cfg::WIN) {
-                // A row that sees nothing keeps row_max = -inf (the software 2^x may leave a
-                // vanishing row_sum there). The rows of a query tile that the item lacks (nt = 0) are another's.
+                // A row that sees nothing has row_max = -inf and row_sum = 0, so -inf. The rows of a query tile that the
+                // item lacks (nt = 0) are another's.
                 if (args.win.lse != nullptr && ok && nt > 0 && grow < n) {
                     args.win.lse[static_cast<long long>(it.bh) * n + grow] =
-                        row_max == -INFINITY ? -INFINITY : (row_max + __log2f(row_sum)) * 0.6931471805599453f;
+                        (row_max + __log2f(row_sum)) * 0.6931471805599453f;
                 }
             }
             if (it.split) {
@@ -930,9 +930,6 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 }
             } else if (tma_store_o && ok && nt > 0) {
                 float inv_sum = (row_sum > 0.0f) ? (1.0f / row_sum) : 0.0f;
-                if constexpr (Cfg::WIN) {
-                    inv_sum = row_max == -INFINITY ? 0.0f : inv_sum;
-                }
                 if constexpr (Cfg::FP8) {
                     inv_sum *= args.out_scale;  // V's descale
                 }
@@ -994,9 +991,6 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 uint8_t* out = smem + Cfg::kSmemStage;
                 if (turn && nt > 0) {
                     float inv_sum = (row_sum > 0.0f) ? (1.0f / row_sum) : 0.0f;
-                    if constexpr (Cfg::WIN) {
-                        inv_sum = row_max == -INFINITY ? 0.0f : inv_sum;
-                    }
                     if constexpr (Cfg::FP8) {
                         inv_sum *= args.out_scale;
                     }

@@ -427,11 +427,13 @@ __device__ __forceinline__ float ex2_approx(float x) {
 // f = x - j in [-1/2, 1/2]; 2^f by a degree-4 polynomial fitted for minimax relative error
 // with Lawson's algorithm (csrc/fit_exp2_poly.py: max relative error 2.9e-6 in float32, far
 // below the 4.9e-4 of the fp16 rounding that follows); 2^j is added into the exponent field.
-// Inputs below -126 are clamped (their 2^x rounds to 0 in fp16 anyway); -inf gives 2^-126.
+// Inputs below -127 are clamped to it, where p is 1 and its exponent field comes down to 0: what is hidden
+// (-inf) gives 0 exactly, in bfloat16 too, whose range reaches 2^-126. Between -127 and -126 the result is
+// some value below 2^-126.
 __device__ __forceinline__ float2 exp2_poly2(float2 x) {
     constexpr float kRound = 12582912.0f;  // 1.5 * 2^23
-    x.x = fmaxf(x.x, -126.0f);
-    x.y = fmaxf(x.y, -126.0f);
+    x.x = fmaxf(x.x, -127.0f);
+    x.y = fmaxf(x.y, -127.0f);
     const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
     const float2 r = __fadd2_rn(t, make_float2(-kRound, -kRound));
     const float2 f = __ffma2_rn(r, make_float2(-1.0f, -1.0f), x);
@@ -450,8 +452,8 @@ __device__ __forceinline__ float2 exp2_poly2(float2 x) {
 // 1.0e-4 in float32, below the 2.4e-4 worst relative rounding of the fp16 value it feeds).
 __device__ __forceinline__ float2 exp2_poly2_deg3(float2 x) {
     constexpr float kRound = 12582912.0f;  // 1.5 * 2^23
-    x.x = fmaxf(x.x, -126.0f);
-    x.y = fmaxf(x.y, -126.0f);
+    x.x = fmaxf(x.x, -127.0f);
+    x.y = fmaxf(x.y, -127.0f);
     const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
     const float2 r = __fadd2_rn(t, make_float2(-kRound, -kRound));
     const float2 f = __ffma2_rn(r, make_float2(-1.0f, -1.0f), x);
@@ -487,6 +489,18 @@ __device__ __forceinline__ void add_f16x2_to_f32(float& lo_acc, float& hi_acc, u
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Larger of each pair of halves, NaN if either is.
+template <bool BF16>
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if constexpr (BF16) {
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    } else {
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    }
+    return d;
 }
 
 // bfloat16 counterparts: lo_acc += low half of b, hi_acc += high half (bf16 -> fp32 exactly,

@@ -96,3 +96,59 @@ def test_lengths_beyond_the_table_end_with_it(page, pages, window, sinks, dtype)
     lengths = lengths.clamp(min=0)
     want, vmax = oracle.cached(q, cache, table, lengths, None, window, sinks)
     oracle.check(got, want, oracle.forward_bound(want, vmax, oracle.unit(HALF), oracle.unit(HALF)), "O")
+
+
+# ------------------------------------------------------------------------------ window attention
+
+
+def _dense(b, h, hk, nq, nk, d, dtype, seed):
+    gen = torch.Generator(DEV).manual_seed(seed)
+    return tuple(_rand(gen, s, dtype) for s in ((b, h, nq, d), (b, hk, nk, d), (b, hk, nk, d), (b, h, nq, d)))
+
+
+def _step(q, k, v, do, window, sinks):
+    o, lse = fa.forward_window(q, k, v, window, sinks, return_lse=True)
+    return (o, lse, *fa.backward_window(do, q, k, v, o, lse, window, sinks))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("big", [3e38, -3e38])
+def test_bf16_hidden_values_weigh_nothing(d, big):
+    """Later keys, and keys before the window, that share a tile with visible ones: values at the end of
+    bfloat16's range do not move a row that does not see them by a bit."""
+    q, k, v, _ = _dense(1, 2, 2, 400, 400, d, BF, seed=3)
+    for window, sinks in ((40, 0), (40, 3), (0, 0)):
+        o, lse = fa.forward_window(q, k, v, window, sinks, return_lse=True)
+        later, k2 = v.clone(), k.clone()
+        later[:, :, 200:], k2[:, :, 200:] = big, 1e30
+        o2, lse2 = fa.forward_window(q, k2, later, window, sinks, return_lse=True)
+        assert torch.equal(o[:, :, :200], o2[:, :, :200]) and torch.equal(lse[:, :, :200], lse2[:, :, :200])
+        if window:
+            before = v.clone()
+            before[:, :, sinks:200] = big
+            assert torch.equal(o[:, :, 239:], fa.forward_window(q, k, before, window, sinks)[:, :, 239:])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_bf16_gradients_of_hidden_pairs_are_zero(d):
+    """Hidden values of 1e36 (their products with dO stay finite) leave the gradients of rows and keys that have no
+    part in them as they are; keys that no query sees, and rows that see nothing, have gradients of 0."""
+    q, k, v, do = _dense(1, 2, 1, 400, 400, d, BF, seed=4)
+    plain = _step(q, k, v, do, 40, 0)
+    v2 = v.clone()
+    v2[:, :, 200:] = 1e36
+    other = _step(q, k, v2, do, 40, 0)
+    assert torch.equal(plain[2][:, :, :200], other[2][:, :, :200])  # dQ
+    assert torch.equal(plain[3][:, :, :161], other[3][:, :, :161])  # dK: key 160 is seen up to row 199
+    assert torch.equal(plain[4][:, :, :161], other[4][:, :, :161])  # dV
+
+    q, k, v, do = _dense(1, 2, 1, 100, 700, d, BF, seed=5)
+    _, _, _, dk, dv = _step(q, k, v, do, 64, 4)
+    assert not dk[:, :, 4:537].any() and not dv[:, :, 4:537].any() and dk[:, :, 537:].any()
+
+    q, k, v, do = _dense(1, 2, 1, 500, 100, d, BF, seed=6)  # rows up to 399 see nothing
+    o, lse, dq, dk, dv = _step(q, k, v, do, 50, 0)
+    assert not o[:, :, :400].any() and (lse[:, :, :400] == -math.inf).all() and not dq[:, :, :400].any()
+    do[:, :, :400] = 1e36
+    again = fa.backward_window(do, q, k, v, o, lse, 50, 0)
+    assert torch.equal(again[1], dk) and torch.equal(again[2], dv) and not again[0][:, :, :400].any()
