@@ -160,7 +160,9 @@ struct FwdCfg {
     // at d = 64 and 64 at d = 128), so the partial overflows fp16 for no input the reference
     // accepts. O_t and the row sum carry the same power-of-two factor, which O / l cancels.
     static constexpr bool ACC16 = (VARIANT_ == kVariantFp16Acc);
-    static constexpr int kAccShift = ACC16 ? (D == 64 ? 2 : 1) : 0;
+    // The window build's bfloat16 P are shifted by the lazy threshold, to p <= 1: the unnormalised O of values
+    // near the end of bfloat16's range, which is float32's, then overflows 2^8 times later.
+    static constexpr int kAccShift = ACC16 ? (D == 64 ? 2 : 1) : (WIN_ && BF16_ ? 8 : 0);
     // Lazy rescale (reference LAZY, flash_fwd.cu:365-376): keep a stale row max until the
     // tile max exceeds it by more than 2^8. Threshold 0 = exact running max.
     // fp8: P is stored as p * 2^(8 - threshold) so that, with p <= 2^threshold under the lazy
@@ -738,7 +740,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
 
                 // Probabilities, packed fp16 pairs, into P_t.
                 const float2 mul2 = make_float2(mul, mul);
-                // fp16acc stores p * 2^-kAccShift, fp8 p * 2^kPLog2Scale: the shift joins the max
+                // fp16acc (and the bf16 window build) stores p * 2^-kAccShift, fp8 p * 2^kPLog2Scale: the shift joins the max
                 // in the exponent.
                 const float neg = Cfg::FP8 ? Cfg::kPLog2Scale - max_used
                                            : ((Cfg::kAccShift != 0) ? -max_used - static_cast<float>(Cfg::kAccShift)
@@ -896,7 +898,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 // item lacks (nt = 0) are another's.
                 if (args.win.lse != nullptr && ok && nt > 0 && grow < n) {
                     args.win.lse[static_cast<long long>(it.bh) * n + grow] =
-                        (row_max + __log2f(row_sum)) * 0.6931471805599453f;
+                        (row_max + static_cast<float>(Cfg::kAccShift) + __log2f(row_sum)) * 0.6931471805599453f;
                 }
             }
             if (it.split) {

@@ -491,18 +491,6 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Larger of each pair of halves, NaN if either is.
-template <bool BF16>
-__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
-    uint32_t d;
-    if constexpr (BF16) {
-        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    } else {
-        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    }
-    return d;
-}
-
 // bfloat16 counterparts: lo_acc += low half of b, hi_acc += high half (bf16 -> fp32 exactly,
 // then an fp32 add), and two floats rounded to nearest-even bfloat16, lo in the low half.
 __device__ __forceinline__ void add_bf16x2_to_f32(float& lo_acc, float& hi_acc, uint32_t b) {

@@ -428,13 +428,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             // P of tile i in float32 from S. It is rounded to 16 bits for dV's product alone; dS is made of P and dP
             // in float32 and rounded once, for its own products. (With the rounded P in dS dK was off by twice
             // what rounding dK itself costs; this takes 3% longer.)
-            // True if the tile has hidden pairs.
             auto probabilities = [&](int i, uint32_t (&p)[64]) {
                 int tile_row, head;
                 stream_tile<Cfg>(args, it, i, tile_row, head);
                 ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.s_full), g & 1, wctx, kStatusTimeoutSoftmax));
                 if (!ok) {
-                    return false;
+                    return;
                 }
                 tc_fence_after();
                 tmem_ld64(t_s, p);
@@ -477,8 +476,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                 const int q_row = Cfg::DKV ? tile_row : it.row0;
                 const int k_row = Cfg::DKV ? it.row0 : tile_row;
                 const int gap = q_row + args.shift - k_row;  // of the tiles' first rows
-                const bool masked = gap < kTile - 1 || (gap + kTile - 1 >= args.window && k_row + kTile > args.sinks);
-                if (masked) {
+                if (gap < kTile - 1 || (gap + kTile - 1 >= args.window && k_row + kTile > args.sinks)) {
                     if constexpr (Cfg::DKV) {
                         // Row = key: it is seen by the columns [from, from + window), a sink by all from
                         // `from` on.
@@ -496,10 +494,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                     p[c] = f2u(e.x);
                     p[c + 1] = f2u(e.y);
                 }
-                return masked;
             };
             // dS of the tile whose dP is next, from its P.
-            auto gradients = [&](const auto& p, bool masked, uint32_t (&w)[32]) {
+            auto gradients = [&](const auto& p, uint32_t (&w)[32]) {
                 ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.dp_full), gd & 1, wctx, kStatusTimeoutSoftmax));
                 if (!ok) {
                     return;
@@ -528,37 +525,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                         w[c / 2] = pack2<Cfg::BF16>(y.x, y.y);
                     }
                 }
-                if (masked) {
-                    // P of a hidden pair is 0 exactly, but its dP and delta may be infinite or NaN (another row's
-                    // O that overflowed, say), and 0 times that is NaN: then hidden pairs are set to 0. (Setting
-                    // them in every masked tile took 4% of the whole at a window of 1024.)
-                    uint32_t nan = w[0];
-#pragma unroll
-                    for (int c = 1; c < 32; ++c) {
-                        nan = max2_nan<Cfg::BF16>(nan, w[c]);
-                    }
-                    constexpr uint32_t kInf = Cfg::BF16 ? 0x7f80u : 0x7c00u;
-                    if (__any_sync(0xffffffffu, (nan & 0x7fffu) > kInf || ((nan >> 16) & 0x7fffu) > kInf)) {
-#pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            w[c] &= (p[2 * c] != 0u ? 0xffffu : 0u) | (p[2 * c + 1] != 0u ? 0xffff0000u : 0u);
-                        }
-                    }
-                }
             };
             if constexpr (Cfg::DKV) {
                 // Step i: P of tile i, dS of tile i - 1.
                 uint32_t p_last[64];
-                bool masked_last = false;
                 for (int i = 0; i <= it.n; ++i) {
                     uint32_t p[64], w[32];
-                    bool masked = false;
                     if (i < it.n) {
-                        masked = probabilities(i, p);
+                        probabilities(i, p);
                         ++g;
                     }
                     if (i > 0) {
-                        gradients(p_last, masked_last, w);
+                        gradients(p_last, w);
                         ++gd;
                         if constexpr (Cfg::kOverDP) {
                             // Every warp has dP in registers; its columns take dS and the next P. (Warps that
@@ -581,7 +559,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                         for (int c = 0; c < 64; ++c) {
                             p_last[c] = p[c];
                         }
-                        masked_last = masked;
                     }
                     if (ok) {
                         tmem_wait_st();
@@ -591,8 +568,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             } else {
                 for (int i = 0; i < it.n; ++i, ++g, ++gd) {
                     uint32_t p[64], w[32];
-                    const bool masked = probabilities(i, p);
-                    gradients(p, masked, w);
+                    probabilities(i, p);
+                    gradients(p, w);
                     if (ok) {
                         tmem_st32(t_ds + (g % 2) * (Cfg::kTmemDS2 - Cfg::kTmemDS), w);
                         tmem_wait_st();
