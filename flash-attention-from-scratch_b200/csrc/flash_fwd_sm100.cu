@@ -719,8 +719,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                                scale_log2;
                     mul = scale_log2;
                 }
-                // Running max update (lazy for "opt": keep the old max unless it grew by > 2^8).
-                const float new_max = (tile_max > row_max + Cfg::kRescaleThreshold) ? tile_max : row_max;
+                // Running max update (lazy for "opt": keep the old max unless it grew by > 2^8). Written so that a NaN
+                // is taken: it makes this tile's P, the sum and, by the rescale, O NaN.
+                const float new_max = (tile_max <= row_max + Cfg::kRescaleThreshold) ? row_max : tile_max;
                 const float max_used = (new_max == -INFINITY) ? 0.0f : new_max;
                 const bool grew = (new_max != row_max);
                 const float alpha = grew ? ex2_approx(row_max - max_used) : 1.0f;  // 0 on tile 0
@@ -1573,7 +1574,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
 
 // Split-KV combine (reference: none; Flash-Decoding's merge of per-range softmax partials).
 // One warp per output row, lanes over the head dim, ranges merged in index order (so the result
-// is deterministic): M = max m_s over the ranges with l_s > 0, then
+// is deterministic): M = max m_s over the ranges with l_s != 0 (a NaN range is not left out), then
 // O = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, rounded to fp16 (BF16: bfloat16).
 // Rows: with split-KV (tail_blocks == 0) every row of every head, row r of head bh at record
 // bh * rows_pad + r; with a tail split the rows of the tail blocks, row r of tail block p at
@@ -1621,7 +1622,7 @@ __global__ void __launch_bounds__(256) splitkv_combine_kernel(const CombineArgs 
     float m_max = -INFINITY;
     for (int sp = 0; sp < a.num_splits; ++sp) {
         const float2 ml = a.ws_ml[rec0 + sp * a.split_stride];
-        if (ml.y > 0.0f) {
+        if (ml.y != 0.0f) {
             m_max = fmaxf(m_max, ml.x);
         }
     }
@@ -1634,7 +1635,7 @@ __global__ void __launch_bounds__(256) splitkv_combine_kernel(const CombineArgs 
     for (int sp = 0; sp < a.num_splits; ++sp) {
         const long long rec = rec0 + sp * a.split_stride;
         const float2 ml = a.ws_ml[rec];
-        if (!(ml.y > 0.0f)) {
+        if (ml.y == 0.0f) {
             continue;
         }
         const float w = exp2f(ml.x - m_max);

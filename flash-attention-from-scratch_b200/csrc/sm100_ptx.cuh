@@ -429,7 +429,9 @@ __device__ __forceinline__ float ex2_approx(float x) {
 // below the 4.9e-4 of the fp16 rounding that follows); 2^j is added into the exponent field.
 // Inputs below -127 are clamped to it, where p is 1 and its exponent field comes down to 0: what is hidden
 // (-inf) gives 0 exactly, in bfloat16 too, whose range reaches 2^-126. Between -127 and -126 the result is
-// some value below 2^-126.
+// some value below 2^-126. NaN gives 0, too, and +inf NaN: a caller that may have NaN puts +inf in its place, or
+// has the NaN from elsewhere. (Keeping it by a clamp that does and a multiplication by 2^j cost the window
+// backward, where three columns of eight come this way, 8%.)
 __device__ __forceinline__ float2 exp2_poly2(float2 x) {
     constexpr float kRound = 12582912.0f;  // 1.5 * 2^23
     x.x = fmaxf(x.x, -127.0f);
@@ -450,6 +452,7 @@ __device__ __forceinline__ float2 exp2_poly2(float2 x) {
 
 // Cheaper variant of exp2_poly2: degree-3 polynomial (fit_exp2_poly.py 3: max relative error
 // 1.0e-4 in float32, below the 2.4e-4 worst relative rounding of the fp16 value it feeds).
+// The forward, which uses it, has a row's NaN from the row's maximum.
 __device__ __forceinline__ float2 exp2_poly2_deg3(float2 x) {
     constexpr float kRound = 12582912.0f;  // 1.5 * 2^23
     x.x = fmaxf(x.x, -127.0f);
@@ -465,16 +468,28 @@ __device__ __forceinline__ float2 exp2_poly2_deg3(float2 x) {
                        __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 
-// Row-max helper: three-input max.
+// Row-max helpers: max and min of two and of three, NaN if one of them is.
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+__device__ __forceinline__ float fmin_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 
 __device__ __forceinline__ float fmin3(float a, float b, float c) {
     float d;
-    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 

@@ -34,7 +34,8 @@ __device__ __forceinline__ void hide_columns(uint32_t (&x)[N], int to, int span,
 }
 
 // Row max (or min, for a negative scale) of N scores (N = 64 or 128): eight independent
-// three-input chains over columns 8 .. N-9, then the last eight columns.
+// three-input chains over columns 8 .. N-9, then the last eight columns. A NaN among them is the result: the
+// software 2^x that some columns take would lose it, while a NaN maximum makes the whole row NaN.
 template <bool MAX, int N>
 __device__ __forceinline__ float row_extreme(const uint32_t (&sr)[N]) {
     static_assert(N % 16 == 0 && N >= 32, "row_extreme covers N = 16 k columns");
@@ -53,10 +54,10 @@ __device__ __forceinline__ float row_extreme(const uint32_t (&sr)[N]) {
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        m[i] = MAX ? fmaxf(m[i], u2f(sr[N - 8 + i])) : fminf(m[i], u2f(sr[N - 8 + i]));
+        m[i] = MAX ? fmax_nan(m[i], u2f(sr[N - 8 + i])) : fmin_nan(m[i], u2f(sr[N - 8 + i]));
     }
-    return MAX ? fmax3(fmax3(m[0], m[1], m[2]), fmax3(m[3], m[4], m[5]), fmaxf(m[6], m[7]))
-               : fmin3(fmin3(m[0], m[1], m[2]), fmin3(m[3], m[4], m[5]), fminf(m[6], m[7]));
+    return MAX ? fmax3(fmax3(m[0], m[1], m[2]), fmax3(m[3], m[4], m[5]), fmax_nan(m[6], m[7]))
+               : fmin3(fmin3(m[0], m[1], m[2]), fmin3(m[3], m[4], m[5]), fmin_nan(m[6], m[7]));
 }
 
 }  // namespace fa_sm100

@@ -128,6 +128,7 @@ struct BwdShared {
     long long warp_sum[kBwdThreads / 32];
     // DKV: of the streamed rows: minus LSE in log2 units (-inf: P = 0), minus delta.
     alignas(16) float lse2[2][kTile];
+    int lse_nan[2];  // whether there is a NaN among them
     alignas(16) float delta[kXStages][kTile];
 };
 
@@ -439,7 +440,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                 tmem_ld64(t_s, p);
                 // Half of the columns' LSE comes meanwhile: shared memory is busy with the products' operands.
                 [[maybe_unused]] float4 early[8];
+                [[maybe_unused]] int lse_nan = 0;
                 if constexpr (Cfg::DKV) {
+                    lse_nan = sh.lse_nan[g % 2];
 #pragma unroll
                     for (int c4 = 0; c4 < 8; ++c4) {
                         early[c4] = *reinterpret_cast<const float4*>(&sh.lse2[g % 2][col0 + 4 * c4]);
@@ -484,6 +487,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                     } else {
                         // Row = query: it sees the columns (to - window, to], and the sinks.
                         hide_columns<64>(p, gap + row - col0, args.window, args.sinks - k_row - col0, 0xff800000u);
+                    }
+                }
+                if constexpr (Cfg::DKV) {
+                    // A row whose LSE is NaN (a NaN score) is NaN in dV, too: the software 2^x makes it of +inf. (dQ
+                    // has the whole row NaN, and other columns that keep it.)
+                    if (lse_nan != 0) {
+#pragma unroll
+                        for (int c = 0; c < 64; ++c) {
+                            if (((c / 2) % 8) < kEmuPer8 && u2f(p[c]) != u2f(p[c])) {
+                                p[c] = 0x7f800000u;
+                            }
+                        }
                     }
                 }
 #pragma unroll
@@ -843,6 +858,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) {
                     break;
+                }
+                const bool nan = __any_sync(0xffffffffu, lse[0] != lse[0] || lse[1] != lse[1] || lse[2] != lse[2] || lse[3] != lse[3]);
+                if (lane == 0) {
+                    sh.lse_nan[g % 2] = nan ? 1 : 0;
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {

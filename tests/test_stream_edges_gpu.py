@@ -152,3 +152,41 @@ def test_bf16_gradients_of_hidden_pairs_are_zero(d):
     do[:, :, :400] = 1e36
     again = fa.backward_window(do, q, k, v, o, lse, 50, 0)
     assert torch.equal(again[1], dk) and torch.equal(again[2], dv) and not again[0][:, :, :400].any()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [HALF, BF])
+def test_nan_in_a_key_reaches_every_row_that_sees_it(d, dtype):
+    """Whatever column of a tile the key is in: 2^x is computed in two ways, by columns."""
+    q, k, v, do = _dense(1, 2, 1, 300, 300, d, dtype, seed=7)
+    window = 100
+    plain = _step(q, k, v, do, window, 0)
+    for key in range(130, 146):
+        bad = k.clone()
+        bad[0, 0, key, 5] = math.nan
+        o, lse, dq, dk, dv = _step(q, bad, v, do, window, 0)
+        sees = slice(key, key + window)
+        assert o[:, :, sees].isnan().all() and lse[:, :, sees].isnan().all(), key
+        for x, y in ((o, plain[0]), (lse, plain[1])):
+            assert torch.equal(x[:, :, :key], y[:, :, :key]) and torch.equal(x[:, :, key + window :], y[:, :, key + window :])
+        assert dq[:, :, sees].isnan().all(), key
+        # Their keys: those rows' P is NaN.
+        keys = slice(key - window + 1, key + window)
+        assert dk[:, :, keys].isnan().all() and dv[:, :, keys].isnan().all(), key
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [HALF, BF])
+def test_nan_in_a_key_of_the_dense_forward(d, dtype):
+    q, k, v, _ = _dense(1, 2, 2, 600, 600, d, dtype, seed=8)
+    plain = fa.forward(q, k, v, causal=True)
+    for key in (*range(260, 276), 599):
+        bad = k.clone()
+        bad[0, :, key, 3] = math.nan
+        o = fa.forward(q, bad, v, causal=True)
+        assert o[:, :, key:].isnan().all() and torch.equal(o[:, :, :key], plain[:, :, :key]), key
+        assert fa.forward(q, bad, v).isnan().all(), key
+        assert fa.forward_splitkv(q, bad, v, num_splits=3).isnan().all(), key
+        if dtype == HALF:
+            for variant in ("baseline", "fp16acc"):
+                assert fa.forward_variant(q, bad, v, variant=variant).isnan().all(), (variant, key)
