@@ -71,6 +71,7 @@ constexpr int kRegsSoftmax = 224;
 constexpr int kRegsOther = 56;
 static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kBwdThreads * 168, "register split");
 constexpr int kEmuPer8 = 3;  // column pairs of 8 whose 2^x runs on the FMA pipe (1: 2% slower, 4: the same)
+__host__ __device__ constexpr bool emulated(int column) { return (column / 2) % 8 < kEmuPer8; }
 
 struct BwdArgs {
     int batch, heads, kv_heads, group;
@@ -128,7 +129,6 @@ struct BwdShared {
     long long warp_sum[kBwdThreads / 32];
     // DKV: of the streamed rows: minus LSE in log2 units (-inf: P = 0), minus delta.
     alignas(16) float lse2[2][kTile];
-    int lse_nan[2];  // whether there is a NaN among them
     alignas(16) float delta[kXStages][kTile];
 };
 
@@ -440,9 +440,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                 tmem_ld64(t_s, p);
                 // Half of the columns' LSE comes meanwhile: shared memory is busy with the products' operands.
                 [[maybe_unused]] float4 early[8];
-                [[maybe_unused]] int lse_nan = 0;
                 if constexpr (Cfg::DKV) {
-                    lse_nan = sh.lse_nan[g % 2];
 #pragma unroll
                     for (int c4 = 0; c4 < 8; ++c4) {
                         early[c4] = *reinterpret_cast<const float4*>(&sh.lse2[g % 2][col0 + 4 * c4]);
@@ -489,23 +487,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                         hide_columns<64>(p, gap + row - col0, args.window, args.sinks - k_row - col0, 0xff800000u);
                     }
                 }
-                if constexpr (Cfg::DKV) {
-                    // A row whose LSE is NaN (a NaN score) is NaN in dV, too: the software 2^x makes it of +inf. (dQ
-                    // has the whole row NaN, and other columns that keep it.)
-                    if (lse_nan != 0) {
-#pragma unroll
-                        for (int c = 0; c < 64; ++c) {
-                            if (((c / 2) % 8) < kEmuPer8 && u2f(p[c]) != u2f(p[c])) {
-                                p[c] = 0x7f800000u;
-                            }
-                        }
-                    }
-                }
 #pragma unroll
                 for (int c = 0; c < 64; c += 2) {
                     const float2 x = make_float2(u2f(p[c]), u2f(p[c + 1]));
-                    const float2 e = ((c / 2) % 8) < kEmuPer8 ? exp2_poly2(x)
-                                                              : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                    const float2 e = emulated(c) ? exp2_poly2(x)
+                                                 : make_float2(ex2_approx(x.x), ex2_approx(x.y));
                     p[c] = f2u(e.x);
                     p[c + 1] = f2u(e.y);
                 }
@@ -859,13 +845,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                 if (!ok) {
                     break;
                 }
-                const bool nan = __any_sync(0xffffffffu, lse[0] != lse[0] || lse[1] != lse[1] || lse[2] != lse[2] || lse[3] != lse[3]);
-                if (lane == 0) {
-                    sh.lse_nan[g % 2] = nan ? 1 : 0;
-                }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    sh.lse2[g % 2][k * 32 + lane] = lse[k] == -INFINITY ? -INFINITY : lse[k] * -1.4426950408889634f;
+                    // A row whose LSE is NaN (a NaN score) makes P NaN: in the columns of the software 2^x, +inf does.
+                    const float x = lse[k] * -1.4426950408889634f;
+                    const float nan = emulated(lane) ? INFINITY : x;
+                    sh.lse2[g % 2][k * 32 + lane] = lse[k] == -INFINITY ? -INFINITY : (x != x ? nan : x);
                     sh.delta[g % kXStages][k * 32 + lane] = -delta[k];
                 }
                 __syncwarp();
