@@ -4,6 +4,9 @@
 //   S = scale Q K^T (masked), P = e^(S - LSE), delta = rowsum(dO o O), dP = dO V^T,
 //   dS = P o (dP - delta),  dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K
 //
+// P and dS are rounded to 16 bits for their products; in float16, whose range is short, times a power of two
+// (head_power).
+//
 // Three passes: delta by rows (bound by DRAM bytes); dK and dV by key tiles; dQ by query tiles. The last
 // two recompute P, seven products a tile pair where one pass over both would take five, but every
 // sum then has one owner: no atomics, no float32 dQ in memory, the same bits every time. They are
@@ -59,6 +62,10 @@ constexpr int kTile = 128;             // rows of every tile
 constexpr int kBox = kTile * 128;      // one TMA box: 128 rows x 128 bytes
 constexpr int kXStages = 3;
 constexpr int kYStages = 2;
+// Items whose powers are kept (float16). The loader is at most three streamed tiles ahead of the products, and an
+// item's products wait for the sums of the one before to be read, so that four are never overwritten too early.
+constexpr int kPowers = 4;
+static_assert(kPowers > kXStages, "an item's power stays until its sums are read");
 constexpr int kBwdThreads = 384;
 constexpr int kSoftmaxWarps = 8;
 constexpr int kProducerWarp = 8;
@@ -84,6 +91,9 @@ struct BwdArgs {
     float scale, scale_log2;
     const float* lse;       // [batch * heads][q_len]
     const float* delta;
+    const float* do_size;   // float16: largest |dO|_2 of kSlotRows query rows, [batch * heads][q_slots]
+    const float* v_size;    // ... |V|_2 of key rows, [batch * kv_heads][k_slots]
+    int q_slots, k_slots;   // of a head
     float* parts;           // cut lists' sums, [part][outputs][D / 4][128 rows][4]
     void* out0;             // DKV: dV
     void* out1;             // dK or dQ
@@ -98,6 +108,7 @@ struct BwdCfg {
     static constexpr int D = D_;
     static constexpr bool BF16 = BF16_;
     static constexpr bool DKV = DKV_;
+    static constexpr bool kLoads = DKV_ || !BF16_;  // there is work for the loader warp
     static constexpr int kBoxes = D / 64;
     static constexpr int kTileBytes = kTile * D * 2;
     static constexpr int kSmemR0 = 0;
@@ -130,6 +141,7 @@ struct BwdShared {
     // DKV: of the streamed rows: minus LSE in log2 units (-inf: P = 0), minus delta.
     alignas(16) float lse2[2][kTile];
     alignas(16) float delta[kXStages][kTile];
+    float power[kPowers];  // float16: head_power
 };
 
 // No static shared memory: the tiles start the dynamic window, 1024-byte aligned, and with d = 128 leave
@@ -150,6 +162,28 @@ struct BwdItem {
     int q0, per;        // DKV: the list is query tiles [q0, q0 + per) of every head of the group
     int sink_tiles, first_tile;  // dQ: the list is key tiles [0, sink_tiles), [first_tile, ..]
 };
+
+// Rows of a delta block, and of a slot of do_size and v_size.
+constexpr int kDeltaThreads = 256;
+constexpr int kDeltaRows = 4;  // of a thread
+template <int D>
+constexpr int kSlotRows = kDeltaThreads / (D / 8) * kDeltaRows;
+
+// The power of two, 2^15 at most, that brings `bound` below 2^16; 1 where it is 0 or not finite.
+__device__ __forceinline__ float power_for(float bound) {
+    const int e = static_cast<int>(__float_as_uint(bound) >> 23);  // bound < 2^(e - 126)
+    return __uint_as_float(static_cast<uint32_t>((e == 0 || e >= 255) ? 127 : 127 + max(min(142 - e, 15), -100)) << 23);
+}
+__device__ __forceinline__ float inverse_power(float p) { return __uint_as_float((254u << 23) - __float_as_uint(p)); }
+__device__ __forceinline__ float exponent(float p) { return static_cast<float>(static_cast<int>(__float_as_uint(p) >> 23) - 127); }
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    }
+    return x;
+}
 
 // The list of resident tile `tile`: its length, and what it is made of. A tile with nothing to see
 // keeps one streamed tile, all hidden, so that its zeros are written.
@@ -268,6 +302,31 @@ __device__ __forceinline__ void stream_tile(const BwdArgs& a, const BwdItem& it,
     }
 }
 
+// float16: the power of two that P and dS carry, by the exponent of P, and the sums give back; one for a kv head and its
+// group. With delta = sum_k P_k dP_k, |dS_j| = P_j |dP_j - delta| <= P_j (1 - P_j) 2 max|dP| <= max|dO|_2 max|V|_2 / 2, so that
+// neither P nor dS overflows with it (a tenth is left for what P, O and the norms round). Without, dS of ordinary
+// small dO (P is about 1 / window) fell among float16's subnormals: with a window of 1024 and dO of 1e-3 the gradients
+// were off by 0.13%, of 1e-4 by 1.3%; and large ones overflowed. A power below 1 costs small P of dV bits instead;
+// rows whose dO is 10^4 below the largest still have normal dS. (A factor on dS alone, in the streamed delta and an FMA,
+// took 17% of the dK, dV pass at d = 64; a power for each item, from its own list, 7 to 18%. This, with the norms,
+// takes 1 to 3% of the whole.) bfloat16 has float32's range and needs none. The whole loader warp calls.
+__device__ __forceinline__ float head_power(const BwdArgs& a, int b, int kvh) {
+    const float* d_o = a.do_size + (static_cast<long long>(b) * a.heads + kvh * a.group) * a.q_slots;
+    const float* v = a.v_size + (static_cast<long long>(b) * a.kv_heads + kvh) * a.k_slots;
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    float most = 0.0f, value = 0.0f;
+    const long long n = static_cast<long long>(a.group) * a.q_slots;
+#pragma unroll 8
+    for (long long i = lane; i < n; i += 32) {
+        most = fmaxf(most, __ldg(d_o + i));
+    }
+#pragma unroll 4
+    for (int i = lane; i < a.k_slots; i += 32) {
+        value = fmaxf(value, __ldg(v + i));
+    }
+    return power_for(0.55f * warp_max(most) * warp_max(value));
+}
+
 // D (128 x 128) = A B^T, both operands 128 rows of the head dim in shared memory.
 template <class Cfg>
 __device__ __forceinline__ void issue_scores(uint32_t d, uint64_t a, uint64_t b) {
@@ -329,7 +388,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         mbar_init(smem_u32(&sh.r1_full), 1);
         mbar_init(smem_u32(&sh.r1_empty), 1);
         for (int s = 0; s < kXStages; ++s) {
-            mbar_init(smem_u32(&sh.x_full[s]), Cfg::DKV ? 2 : 1);  // the copy, and the rows' statistics
+            mbar_init(smem_u32(&sh.x_full[s]), Cfg::kLoads ? 2 : 1);  // the copy, and the loader's
             mbar_init(smem_u32(&sh.x_empty[s]), 1);
         }
         for (int s = 0; s < kYStages; ++s) {
@@ -422,7 +481,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         statistics();
         while (more) {
             it = next;
-            const float row_lse2 = next_lse2;
+            float row_lse2 = next_lse2;
             const float row_delta = next_delta;
             more = next_item<Cfg::DKV>(args, cursor, next);
             statistics();
@@ -437,6 +496,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                     return;
                 }
                 tc_fence_after();
+                if constexpr (!Cfg::DKV && !Cfg::BF16) {
+                    if (i == 0) {
+                        row_lse2 += exponent(sh.power[done % kPowers]);
+                    }
+                }
                 tmem_ld64(t_s, p);
                 // Half of the columns' LSE comes meanwhile: shared memory is busy with the products' operands.
                 [[maybe_unused]] float4 early[8];
@@ -589,7 +653,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             constexpr int kCols = Cfg::DKV ? D : D / 2;
             const int out_col = Cfg::DKV ? 0 : wg * kCols;
             const uint32_t t_acc = tmem + lanes + ((Cfg::DKV && wg == 0) ? Cfg::kTmemAcc0 : Cfg::kTmemAcc1) + out_col;
-            const float factor = (Cfg::DKV && wg == 0) ? 1.0f : args.scale;
+            float factor = (Cfg::DKV && wg == 0) ? 1.0f : args.scale;
+            if constexpr (!Cfg::BF16) {
+                factor *= inverse_power(sh.power[(done - 1) % kPowers]);
+            }
             const int rows = Cfg::DKV ? args.k_len : args.q_len;
             const bool first_out = Cfg::DKV && wg == 0;
             const int64_t* st = first_out ? args.out0_stride : args.out1_stride;
@@ -819,45 +886,60 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         __syncwarp();
         mbar_wait_drain(smem_u32(&sh.mma_idle), 0, wctx, kStatusTimeoutTeardown);
         __syncwarp();
-    } else if (Cfg::DKV && warp == kLoaderWarp) {
-        // ====================== LSE and delta of the streamed query rows ======================
+    } else if (Cfg::kLoads && warp == kLoaderWarp) {
+        // ========== LSE and delta of the streamed query rows (DKV), the items' powers (float16) ==========
         bool ok = true;
         int g = 0;
+        int items = 0;
+        [[maybe_unused]] float power = 1.0f;  // of kv head `power_of`
+        [[maybe_unused]] int power_of = -1;
         BwdItem it;
         while (ok && next_item<Cfg::DKV>(args, cursor, it)) {
+            if (!Cfg::BF16 && it.b * args.kv_heads + it.kvh != power_of) {
+                power_of = it.b * args.kv_heads + it.kvh;
+                power = head_power(args, it.b, it.kvh);
+            }
             for (int i = 0; ok && i < it.n; ++i, ++g) {
-                int row, head;
-                stream_tile<Cfg>(args, it, i, row, head);
-                const long long base = (static_cast<long long>(it.b) * args.heads + head) * args.q_len;
-                float lse[4], delta[4];
+                [[maybe_unused]] float lse[4], delta[4];
+                if constexpr (Cfg::DKV) {
+                    int row, head;
+                    stream_tile<Cfg>(args, it, i, row, head);
+                    const long long base = (static_cast<long long>(it.b) * args.heads + head) * args.q_len;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int r = row + k * 32 + lane;
-                    lse[k] = r < args.q_len ? __ldg(args.lse + base + r) : -INFINITY;
-                    delta[k] = r < args.q_len ? __ldg(args.delta + base + r) : 0.0f;
+                    for (int k = 0; k < 4; ++k) {
+                        const int r = row + k * 32 + lane;
+                        lse[k] = r < args.q_len ? __ldg(args.lse + base + r) : -INFINITY;
+                        delta[k] = r < args.q_len ? __ldg(args.delta + base + r) : 0.0f;
+                    }
                 }
                 // LSE has two slots, free when tile g - 2 has been read; delta three, like X.
                 ok = mbar_wait(smem_u32(&sh.x_empty[g % kXStages]), ((g / kXStages) & 1) ^ 1, wctx, kStatusTimeoutProducer);
-                if (g >= 2) {
+                if (Cfg::DKV && g >= 2) {
                     ok = ok && mbar_wait(smem_u32(&sh.s_read[g % 2]), ((g - 2) / 2) & 1, wctx, kStatusTimeoutProducer);
                 }
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) {
                     break;
                 }
+                if constexpr (Cfg::DKV) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    // A row whose LSE is NaN (a NaN score) makes P NaN: in the columns of the software 2^x, +inf does.
-                    const float x = lse[k] * -1.4426950408889634f;
-                    const float nan = emulated(lane) ? INFINITY : x;
-                    sh.lse2[g % 2][k * 32 + lane] = lse[k] == -INFINITY ? -INFINITY : (x != x ? nan : x);
-                    sh.delta[g % kXStages][k * 32 + lane] = -delta[k];
+                    for (int k = 0; k < 4; ++k) {
+                        // A row whose LSE is NaN (a NaN score) makes P NaN: in the columns of the software 2^x, +inf does.
+                        const float x = lse[k] * -1.4426950408889634f + (Cfg::BF16 ? 0.0f : exponent(power));
+                        const float nan = emulated(lane) ? INFINITY : x;
+                        sh.lse2[g % 2][k * 32 + lane] = lse[k] == -INFINITY ? -INFINITY : (x != x ? nan : x);
+                        sh.delta[g % kXStages][k * 32 + lane] = -delta[k];
+                    }
+                }
+                if (!Cfg::BF16 && i == 0 && lane == 0) {
+                    sh.power[items % kPowers] = power;
                 }
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(smem_u32(&sh.x_full[g % kXStages]));
                 }
             }
+            ++items;
         }
     }
 
@@ -874,35 +956,46 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
 }
 
-// delta[row] = dO.O, a row by D / 8 lanes, kDeltaRows rows a thread of head blockIdx.y. Bound by DRAM bytes.
-constexpr int kDeltaRows = 4;
-
+// delta[row] = dO.O, a row by D / 8 lanes, kDeltaRows rows a thread of head blockIdx.y. Bound by DRAM bytes. float16:
+// also what bounds dS, the largest |dO| of the block's rows, and |V| (blockIdx.z = 1).
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ FaWindowParams p, float* delta) {
+__global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const __grid_constant__ FaWindowParams p, float* delta, float* do_size,
+                                                              float* v_size, int q_slots, int k_slots) {
     constexpr int C = D / 8;
-    constexpr int kGroups = 256 / C;
+    constexpr int kGroups = kDeltaThreads / C;
+    const bool values = !BF16 && blockIdx.z != 0;
+    const int heads = values ? p.kv_heads : p.heads;
+    const int len = values ? p.k_len : p.q_len;
     const int chunk = static_cast<int>(threadIdx.x) % C;
     const int bh = static_cast<int>(blockIdx.y);
-    const int b = bh / p.heads;
-    const int h = bh - b * p.heads;
+    const int b = bh / heads;
+    const int h = bh - b * heads;
+    if (!BF16 && (b >= p.batch || static_cast<int>(blockIdx.x) >= (values ? k_slots : q_slots))) {
+        return;
+    }
+    const int64_t* d_st = values ? p.v_stride : p.do_stride;
     const uint16_t* o_head = static_cast<const uint16_t*>(p.o) + b * p.o_stride[0] + h * p.o_stride[1] + chunk * 8;
-    const uint16_t* d_head = static_cast<const uint16_t*>(p.d_o) + b * p.do_stride[0] + h * p.do_stride[1] + chunk * 8;
-    const int row0 = static_cast<int>(blockIdx.x) * (kGroups * kDeltaRows) + static_cast<int>(threadIdx.x) / C;
+    const uint16_t* d_head = static_cast<const uint16_t*>(values ? p.v : p.d_o) + b * d_st[0] + h * d_st[1] + chunk * 8;
+    const int row0 = static_cast<int>(blockIdx.x) * kSlotRows<D> + static_cast<int>(threadIdx.x) / C;
     uint4 o[kDeltaRows], d[kDeltaRows];
 #pragma unroll
     for (int i = 0; i < kDeltaRows; ++i) {
         const int64_t row = row0 + i * kGroups;
         o[i] = d[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (row < p.q_len) {
-            o[i] = __ldg(reinterpret_cast<const uint4*>(o_head + row * p.o_stride[2]));
-            d[i] = __ldg(reinterpret_cast<const uint4*>(d_head + row * p.do_stride[2]));
+        if (row < len) {
+            if (!values) {
+                o[i] = __ldg(reinterpret_cast<const uint4*>(o_head + row * p.o_stride[2]));
+            }
+            d[i] = __ldg(reinterpret_cast<const uint4*>(d_head + row * d_st[2]));
         }
     }
+    [[maybe_unused]] float most = 0.0f;
 #pragma unroll
     for (int i = 0; i < kDeltaRows; ++i) {
         const uint32_t ow[4] = {o[i].x, o[i].y, o[i].z, o[i].w};
         const uint32_t dw[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
         float sum = 0.0f;
+        [[maybe_unused]] float square = 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             if constexpr (BF16) {
@@ -913,15 +1006,37 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ FaWi
                 const float2 y = unpack_half2(dw[k]);
                 sum = fmaf(x.x, y.x, sum);
                 sum = fmaf(x.y, y.y, sum);
+                square = fmaf(y.x, y.x, square);
+                square = fmaf(y.y, y.y, square);
             }
         }
 #pragma unroll
         for (int k = C / 2; k > 0; k >>= 1) {
             sum += __shfl_xor_sync(0xffffffffu, sum, k);
+            if constexpr (!BF16) {
+                square += __shfl_xor_sync(0xffffffffu, square, k);
+            }
         }
         const int row = row0 + i * kGroups;
-        if (row < p.q_len && chunk == 0) {
-            delta[static_cast<long long>(bh) * p.q_len + row] = sum;
+        if (!values && row < len && chunk == 0) {
+            delta[static_cast<long long>(bh) * len + row] = sum;
+        }
+        if constexpr (!BF16) {
+            most = fmaxf(most, square);
+        }
+    }
+    if constexpr (!BF16) {
+        __shared__ float all[kDeltaThreads / 32];
+        most = warp_max(most);
+        if (threadIdx.x % 32 == 0) {
+            all[threadIdx.x / 32] = most;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < kDeltaThreads / 32; ++w) {
+                most = fmaxf(most, all[w]);
+            }
+            (values ? v_size + static_cast<long long>(bh) * k_slots : do_size + static_cast<long long>(bh) * q_slots)[blockIdx.x] = sqrtf(most);
         }
     }
 }
@@ -1038,8 +1153,25 @@ unsigned long long part_bytes(const BwdArgs& a, int head_dim) {
     return a.grid > 1 ? 2ull * a.grid * (DKV ? 2 : 1) * kTile * head_dim * 4 : 0;
 }
 
-unsigned long long delta_bytes(const FaWindowParams& p) {
-    return (4ull * p.batch * p.heads * p.q_len + 255) / 256 * 256;
+// Where the row statistics lie in the workspace.
+struct Statistics {
+    int q_slots, k_slots;
+    unsigned long long do_size, v_size, bytes;  // delta is first
+};
+
+Statistics statistics_of(const FaWindowParams& p) {
+    const auto up = [](unsigned long long n) { return (n + 255) / 256 * 256; };
+    const int slot_rows = p.head_dim == 64 ? kSlotRows<64> : kSlotRows<128>;
+    Statistics s{};
+    s.bytes = up(4ull * p.batch * p.heads * p.q_len);
+    if (p.dtype == FA_DTYPE_FLOAT16) {
+        s.q_slots = (p.q_len + slot_rows - 1) / slot_rows;
+        s.k_slots = (p.k_len + slot_rows - 1) / slot_rows;
+        s.do_size = s.bytes;
+        s.v_size = s.do_size + up(4ull * p.batch * p.heads * s.q_slots);
+        s.bytes = s.v_size + up(4ull * p.batch * p.kv_heads * s.k_slots);
+    }
+    return s;
 }
 
 // Launches after the kernel before it has started to end: it waits for its results itself.
@@ -1069,8 +1201,15 @@ cudaError_t bwd(const FaWindowParams& p, DeviceStatus* status, unsigned epoch, v
     dkv.status = dq.status = status;
     dkv.lse = dq.lse = p.lse;
     dkv.delta = dq.delta = delta;
-    dkv.parts = reinterpret_cast<float*>(ws + delta_bytes(p));
-    dq.parts = reinterpret_cast<float*>(ws + delta_bytes(p) + part_bytes<true>(dkv, D));
+    const Statistics st = statistics_of(p);
+    float* do_size = reinterpret_cast<float*>(ws + st.do_size);
+    float* v_size = reinterpret_cast<float*>(ws + st.v_size);
+    dkv.do_size = dq.do_size = do_size;
+    dkv.v_size = dq.v_size = v_size;
+    dkv.q_slots = dq.q_slots = st.q_slots;
+    dkv.k_slots = dq.k_slots = st.k_slots;
+    dkv.parts = reinterpret_cast<float*>(ws + st.bytes);
+    dq.parts = reinterpret_cast<float*>(ws + st.bytes + part_bytes<true>(dkv, D));
     dkv.out0 = p.dv;
     dkv.out1 = p.dk;
     dq.out1 = p.dq;
@@ -1078,9 +1217,8 @@ cudaError_t bwd(const FaWindowParams& p, DeviceStatus* status, unsigned epoch, v
     strides(dkv.out0_stride, p.dv_stride);
     strides(dkv.out1_stride, p.dk_stride);
     strides(dq.out1_stride, p.dq_stride);
-    const int delta_rows = 256 / (D / 8) * kDeltaRows;
-    const dim3 delta_grid(static_cast<unsigned>((p.q_len + delta_rows - 1) / delta_rows),
-                          static_cast<unsigned>(p.batch * p.heads));
+    const int delta_blocks = BF16 ? (p.q_len + kSlotRows<D> - 1) / kSlotRows<D> : std::max(st.q_slots, st.k_slots);
+    const dim3 delta_grid(static_cast<unsigned>(delta_blocks), static_cast<unsigned>(p.batch * p.heads), BF16 ? 1 : 2);
     CUtensorMap q, k, v, d_o;
     if (encode_strided_map(&q, p.q, p.q_stride, p.batch, p.heads, p.q_len, D, kTile, BF16) != CUDA_SUCCESS ||
         encode_strided_map(&k, p.k, p.k_stride, p.batch, p.kv_heads, p.k_len, D, kTile, BF16) != CUDA_SUCCESS ||
@@ -1097,7 +1235,7 @@ cudaError_t bwd(const FaWindowParams& p, DeviceStatus* status, unsigned epoch, v
     if (err != cudaSuccess) {
         return err;
     }
-    delta_kernel<D, BF16><<<delta_grid, 256, 0, stream>>>(p, delta);
+    delta_kernel<D, BF16><<<delta_grid, kDeltaThreads, 0, stream>>>(p, delta, do_size, v_size, st.q_slots, st.k_slots);
     err = cudaGetLastError();
     if (err != cudaSuccess) {
         return err;
@@ -1119,7 +1257,7 @@ cudaError_t bwd(const FaWindowParams& p, DeviceStatus* status, unsigned epoch, v
 }  // namespace
 
 unsigned long long window_bwd_workspace_bytes(const FaWindowParams& p, int sm_count) {
-    return delta_bytes(p) + part_bytes<true>(bwd_args<true>(p, sm_count), p.head_dim) +
+    return statistics_of(p).bytes + part_bytes<true>(bwd_args<true>(p, sm_count), p.head_dim) +
            part_bytes<false>(bwd_args<false>(p, sm_count), p.head_dim);
 }
 

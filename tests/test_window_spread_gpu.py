@@ -58,3 +58,33 @@ def test_gradients_of_long_rows_by_norms(b, h, hk, n, d, window, sinks, dtype):
 def test_gradients_of_other_scales_by_norms(scale, dtype):
     q, k, v, do = _inputs(1, 4, 2, 300, 300, 64, dtype, seed=107)
     _check(q, k, v, do, 100, 3, scale)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [1e-3, 1e-4, 1e-5])
+def test_float16_gradients_of_small_do(d, size):
+    """dS of dO like a mean loss's: P / window of it is far below float16's normal range."""
+    q, k, v, do = _inputs(1, 4, 2, 3000, 3000, d, HALF, seed=200)
+    _check(q, k, v, (do.float() * size).to(HALF), 1500, 4)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_float16_gradients_of_large_do(d):
+    """dP beyond float16's range, with gradients within it."""
+    q, k, v, do = _inputs(1, 2, 2, 500, 500, d, HALF, seed=201)
+    _check(q * 0.25, k * 0.25, v * 30, do * 1000, 0, 0)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("h,hk", [(4, 2), (4, 4)])
+def test_float16_gradients_of_uneven_do(d, h, hk):
+    """Rows, heads and sequences whose dO are up to 10^4 apart, rows of zeros and a head of zeros among them; keys
+    seen from one end of a row alone."""
+    q, k, v, do = _inputs(3, h, hk, 700, 700, d, HALF, seed=202)
+    size = 10.0 ** (torch.arange(700, device=DEV) % 5 - 4.0)[:, None]
+    size[::7] = 0
+    do = (do.float() * size).to(HALF)
+    do[1] *= 1e-3
+    do[2, 1] = 0
+    v[2] *= 100
+    _check(q, k, v, do, 200, 3)
