@@ -8,6 +8,8 @@
 Position j of sequence b is in slot j % page_size of page table[b, j // page_size]. Not in the
 reference, which has no cache (its q, k and v have one length).
 
+Serving only: neither call carries a gradient (to k, v or q, or into the cache).
+
 lengths, counts and the table stay on the device and are not read by the host, so a call can be
 captured in a CUDA graph and replayed as they change. Positions outside the table and pages outside
 the pool are skipped by the kernels and set bit 5 (32) of fa._C.device_status.
@@ -170,7 +172,8 @@ def append_kv(
 
     An e4m3 page's scale is the smallest power of two (2^-60 or more) that brings its values within
     448. It grows while the page fills (older tokens are rescaled, exactly but for subnormal codes)
-    and starts anew with the page's first slot. No two sequences may append to one page."""
+    and starts anew with the page's first slot. No two sequences may append to one page. The returned q
+    carries no gradient."""
     tensors = (k, v) if q is None else (k, v, q)
     _check_tokens(cache, *tensors)
     if k.shape != v.shape or k.shape[1] != cache._heads[0]:
@@ -226,7 +229,8 @@ def forward_cached(
     lengths and counts as in append_kv: query t of sequence b is at position p = lengths[b] -
     counts[b] + t and sees position j when 0 <= j <= p and (window == 0, or p - j < window, or
     j < sinks); a row that sees nothing, padding among them, is zeros. H is a multiple of the
-    cache's heads, grouped as in forward_window. Scores, softmax and sums are in float32."""
+    cache's heads, grouped as in forward_window. Scores, softmax and sums are in float32. The result
+    carries no gradient."""
     _check_tokens(cache, q)
     batch, heads, tokens, dim = q.shape
     o = torch.empty_like(q, memory_format=torch.contiguous_format)

@@ -151,6 +151,18 @@ def _loadable(t: torch.Tensor) -> torch.Tensor:
     return t if ok else t.contiguous()
 
 
+class _Once(torch.autograd.Function):
+    """Gradients as they are, whose own gradient is an error (and not, silently, nothing)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, *grads):
+        return tuple(g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("window_attention can be differentiated once")
+
+
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, softmax_scale):
@@ -161,9 +173,12 @@ class _WindowAttention(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, do):
-        if torch.is_grad_enabled():
-            raise RuntimeError("window_attention can be differentiated once (no create_graph)")
-        return (*backward_window(_loadable(do), *ctx.saved_tensors, *ctx.how), None, None, None)
+        q, k, v, o, lse = ctx.saved_tensors
+        with torch.no_grad():
+            grads = backward_window(_loadable(do), q, k, v, o, lse, *ctx.how)
+        if torch.is_grad_enabled():  # create_graph, for whatever part of the model
+            grads = _Once.apply(q, k, v, *grads)
+        return (*grads, None, None, None)
 
 
 def window_attention(

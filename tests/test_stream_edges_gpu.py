@@ -190,3 +190,20 @@ def test_nan_in_a_key_of_the_dense_forward(d, dtype):
         if dtype == HALF:
             for variant in ("baseline", "fp16acc"):
                 assert fa.forward_variant(q, bad, v, variant=variant).isnan().all(), (variant, key)
+
+
+def test_a_graph_of_the_gradients_may_be_asked_for():
+    """create_graph for another part's sake: the gradients are the same, and only differentiating them again
+    through the attention is refused."""
+    q, k, v, do = _dense(1, 2, 1, 64, 64, 64, HALF, seed=9)
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    o = fa.window_attention(q, k, v, 20)
+    plain = torch.autograd.grad(o, (q, k, v), do, retain_graph=True)
+    again = torch.autograd.grad(o, (q, k, v), do, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, again))
+    other = torch.ones(3, device=DEV, requires_grad=True)  # a penalty on another part's gradient
+    slope = torch.autograd.grad((o.float().sum() * 0 + (other**3).sum()), (q, other), create_graph=True)[1]
+    assert torch.equal(torch.autograd.grad(slope.sum(), other)[0], 6 * other.detach())
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        again[0].sum().backward()
