@@ -63,6 +63,23 @@ constexpr int kWholeTiles = 8;     // up to this many key tiles in the table's c
 constexpr float kMinScale = 8.673617379884035e-19f;  // 2^-60
 constexpr int kSmem = kWarps * kStages * (2 * kTileBytes + kAuxFloats * 4);
 
+// Values that are not finite, of keys that some of an item's rows see and some do not, in bits of (row, dim): NaN,
+// +inf and -inf. See attend().
+struct Apart {
+    uint32_t bits[3][kRows][128 / 32];
+};
+
+__device__ __forceinline__ float not_finite_sum(const Apart& a, int row, int dim) {
+    const uint32_t bit = 1u << (dim % 32);
+    float sum = 0.0f;
+    sum += (a.bits[0][row][dim / 32] & bit) != 0 ? NAN : 0.0f;
+    sum += (a.bits[1][row][dim / 32] & bit) != 0 ? INFINITY : 0.0f;
+    sum += (a.bits[2][row][dim / 32] & bit) != 0 ? -INFINITY : 0.0f;
+    return sum;
+}
+
+constexpr int kSmemCareful = kSmem + static_cast<int>(sizeof(Apart));
+
 template <int D_, bool BF16_, bool E4M3_, bool ONE_PAGE_>
 struct Cfg {
     static constexpr bool ONE_PAGE = ONE_PAGE_;  // a key tile lies within one page
@@ -113,6 +130,18 @@ __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
         "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
         : "=r"(lo), "=r"(hi)
         : "r"(w));
+}
+
+// Nonzero if a word of cache elements holds one that is not finite.
+template <class C>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    if constexpr (C::E4M3) {
+        return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // e4m3 has NaN (all ones) and no infinity
+    } else if constexpr (C::BF16) {
+        return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+    } else {
+        return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+    }
 }
 
 // Byte offsets of chunk `c` (16 bytes) of token `r` in a K and in a V tile. The swizzles make the
@@ -224,13 +253,53 @@ __device__ __forceinline__ Range locate(const FaCachedParams& p, int grid, At at
     return r;
 }
 
+// Takes what is not finite out of 16 bytes `at` of a V tile (chunk `chunk` of the token at position `key`) and notes it for
+// the rows of the item that see it.
+template <class C>
+__device__ __forceinline__ void set_apart(const FaCachedParams& p, const Sequence& s, Apart& apart, uint8_t* at, int row0, int key,
+                                       int chunk) {
+    const int rows = p.heads / p.cache.kv_heads * p.cache.tokens;
+    for (int e = 0; e < 16 / C::kElem; ++e) {
+        int kind = 0;
+        if constexpr (C::E4M3) {
+            if ((at[e] & 0x7f) != 0x7f) {
+                continue;
+            }
+            at[e] = 0;
+        } else {
+            uint16_t* x = reinterpret_cast<uint16_t*>(at) + e;
+            constexpr uint32_t kInf = C::BF16 ? 0x7f80u : 0x7c00u;
+            if ((*x & 0x7fffu) < kInf) {
+                continue;
+            }
+            kind = (*x & 0x7fffu) > kInf ? 0 : (*x >> 15) + 1;
+            *x = 0;
+        }
+        const int dim = chunk * (16 / C::kElem) + e;
+        for (int row = 0; row < kRows && row0 + row < rows; ++row) {
+            const int token = (row0 + row) % p.cache.tokens;
+            const int gap = s.pos0 + token - key;
+            if (token < s.count && gap >= 0 && (p.window == 0 || gap < p.window || key < p.sinks)) {
+                atomicOr(&apart.bits[kind][row][dim / 32], 1u << (dim % 32));
+            }
+        }
+    }
+}
+
 struct Record {  // of a cut item's rows in the workspace
     float* o;    // [record][16][D]
     float2* ml;  // [record][16]
+    int* odd;    // [CTA], several tokens: whether a result of its range is not finite
 };
 
-// One range of key tiles [v0, v1) of an item; `tiles` of the item in all.
-template <class C>
+// One range of key tiles [v0, v1) of an item.
+//
+// Several tokens: where not all rows see all of a tile, 0 times an infinite or NaN value is NaN in rows that it is hidden from
+// (a drafted token's, in the rows of the tokens before it). A CTA with a result that is not finite says so, and a second
+// kernel takes its range again, CAREFUL: such values are taken out of those tiles, and added to the rows that see
+// them when the rows are joined. (In this loop, which has no registers left, looking for them in every such tile, or
+// keeping rows apart in the product, cost drafted tokens 3 to 50%.)
+template <class C, bool CAREFUL>
 __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* status, uint8_t* smem, const Sequence& s,
                                        int b, int kvh, int row0, int v0, int v1, Record rec, long long record) {
     constexpr int D = C::D;
@@ -243,6 +312,14 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
     const int rows = group * c.tokens;
     uint8_t* ring = smem + warp * kStages * 2 * kTileBytes;
     float* aux = reinterpret_cast<float*>(smem + kWarps * kStages * 2 * kTileBytes) + warp * kStages * kAuxFloats;
+    [[maybe_unused]] Apart& apart = *reinterpret_cast<Apart*>(smem + kSmem);
+    if constexpr (CAREFUL) {
+        uint32_t* words = &apart.bits[0][0][0];
+        for (int i = static_cast<int>(threadIdx.x); i < static_cast<int>(sizeof(Apart) / 4); i += kThreads) {
+            words[i] = 0;
+        }
+        __syncthreads();
+    }
 
     if (threadIdx.x == 0 && s.count > 0 && s.pos0 + s.count > held(c)) {
         atomicOr(&status->code, kStatusBadPage);  // positions that the table has no place for are left out
@@ -532,6 +609,18 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
             }
         }
 
+        if (CAREFUL && !whole) {
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * kStep + r0;
+                uint8_t* at = ring + stage * 2 * kTileBytes + kTileBytes + v_offset<C>(r, chunk);
+                const uint4 y = *reinterpret_cast<const uint4*>(at);
+                if ((not_finite<C>(y.x) | not_finite<C>(y.y) | not_finite<C>(y.z) | not_finite<C>(y.w)) != 0) {
+                    set_apart<C>(p, s, apart, at, row0, key0 + r, chunk);
+                }
+            }
+            __syncwarp();
+        }
+
         // O += P V, 16 keys a step: lane (g, t) brings keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 and
         // the dims of its chunk g, byte i of it for output tile i.
 #pragma unroll
@@ -635,6 +724,7 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
     const int row = static_cast<int>(threadIdx.x) / kLanes;
     const int part = static_cast<int>(threadIdx.x) % kLanes;
     const int r = row0 + row;
+    bool odd = false;
     if (r < rows) {
         float top = -INFINITY;
 #pragma unroll
@@ -667,6 +757,14 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
                 sum4.z = fmaf(y.z, weight[w], sum4.z);
                 sum4.w = fmaf(y.w, weight[w], sum4.w);
             }
+            if constexpr (CAREFUL) {
+                sum4.x += not_finite_sum(apart, row, four * 4);
+                sum4.y += not_finite_sum(apart, row, four * 4 + 1);
+                sum4.z += not_finite_sum(apart, row, four * 4 + 2);
+                sum4.w += not_finite_sum(apart, row, four * 4 + 3);
+            } else {
+                odd = odd || !(fabsf(sum4.x) + fabsf(sum4.y) + fabsf(sum4.z) + fabsf(sum4.w) < INFINITY);
+            }
             if (record < 0) {
                 *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.o) + out_row * D + four * 4) =
                     real ? make_uint2(pack2<C::BF16>(sum4.x * inv, sum4.y * inv), pack2<C::BF16>(sum4.z * inv, sum4.w * inv))
@@ -680,56 +778,86 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
             rec.ml[record * kRows + row] = real ? make_float2(top, sum) : make_float2(-INFINITY, 0.0f);
         }
     }
-    __syncthreads();  // the rings are free for the next item
+    const bool any_odd = __syncthreads_or(odd) != 0;  // ... and the rings are free for the next item
+    if (!CAREFUL && any_odd && s.count > 1 && threadIdx.x == 0) {
+        rec.odd[blockIdx.x] = 1;
+    }
+}
+
+// Calls take(i) for the ranges (or whole items) of this CTA: its own in the first kernel, one for each CTA; in the second
+// (CAREFUL), whose few CTAs look at all answers of the first, those of results that were not finite.
+template <bool CAREFUL, class Take>
+__device__ __forceinline__ void take_ranges(const FaCachedParams& p, const Record& rec, int ranges, Take take) {
+    cudaTriggerProgrammaticLaunchCompletion();  // the next kernel's CTAs may take SMs as they get free
+    if constexpr (CAREFUL) {
+        cudaGridDependencySynchronize();  // the answers are there
+        bool any = false;
+        for (long long i = blockIdx.x + static_cast<long long>(threadIdx.x) * gridDim.x; i < ranges; i += static_cast<long long>(kThreads) * gridDim.x) {
+            any = any || rec.odd[i] != 0;
+        }
+        if (__syncthreads_or(any) != 0) {
+            for (long long i = blockIdx.x; i < ranges; i += gridDim.x) {
+                if (rec.odd[i] != 0) {
+                    take(static_cast<int>(i));
+                }
+            }
+        }
+    } else {
+        if (p.cache.tokens > 1 && threadIdx.x == 0) {
+            rec.odd[blockIdx.x] = 0;
+        }
+        take(static_cast<int>(blockIdx.x));
+    }
 }
 
 // Items that are never cut, one a CTA.
-template <class C>
+template <class C, bool CAREFUL>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) cached_whole_kernel(const __grid_constant__ FaCachedParams p,
-                                                                            DeviceStatus* status) {
+                                                                            DeviceStatus* status, Record rec, int ranges) {
     extern __shared__ __align__(128) uint8_t smem[];
     const int row_tiles = (p.heads / p.cache.kv_heads * p.cache.tokens + kRows - 1) / kRows;
     const int items = p.cache.kv_heads * row_tiles;
-    const int b = static_cast<int>(blockIdx.x) / items;
-    const int item = static_cast<int>(blockIdx.x) - b * items;
-    const Sequence s = sequence<C>(p, b);
-    attend<C>(p, status, smem, s, b, item / row_tiles, (item % row_tiles) * kRows, 0, s.tiles, Record{}, -1);
+    take_ranges<CAREFUL>(p, rec, ranges, [&](int range) {
+        const int b = range / items;
+        const int item = range - b * items;
+        const Sequence s = sequence<C>(p, b);
+        attend<C, CAREFUL>(p, status, smem, s, b, item / row_tiles, (item % row_tiles) * kRows, 0, s.tiles, rec, -1);
+    });
 }
 
-template <class C>
+template <class C, bool CAREFUL>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) cached_kernel(const __grid_constant__ FaCachedParams p,
-                                                                      DeviceStatus* status, Record rec) {
+                                                                      DeviceStatus* status, Record rec, int ranges) {
     extern __shared__ __align__(128) uint8_t smem[];
-    const int grid = static_cast<int>(gridDim.x);
-    const long long cta = blockIdx.x;
-    cudaTriggerProgrammaticLaunchCompletion();  // the join's CTAs may take SMs as they get free
-    const Range range = locate<C>(p, grid, [&](long long per) { return cta * per; });
-    if (range.found < 0) {
-        return;  // past the end of the list
-    }
-    const int row_tiles = (p.heads / p.cache.kv_heads * p.cache.tokens + kRows - 1) / kRows;
-    const int items = p.cache.kv_heads * row_tiles;
-    long long at = cta * range.per;
-    const long long end = min(at + range.per, range.total);
-    int b = range.found;
-    Sequence s = sequence<C>(p, b);
-    long long in_seq = at - range.found_base;
-    int item = static_cast<int>(in_seq / s.tiles);
-    int v = static_cast<int>(in_seq - static_cast<long long>(item) * s.tiles);
-    bool first = true;
-    while (at < end) {
-        const int take = static_cast<int>(min(static_cast<long long>(s.tiles - v), end - at));
-        const bool whole = v == 0 && take == s.tiles;
-        attend<C>(p, status, smem, s, b, item / row_tiles, (item % row_tiles) * kRows, v, v + take, rec,
-                  whole ? -1 : 2 * cta + (first ? 0 : 1));
-        first = false;
-        at += take;
-        v = 0;
-        if (at < end && ++item == items) {
-            item = 0;
-            s = sequence<C>(p, ++b);
+    take_ranges<CAREFUL>(p, rec, ranges, [&](int cta) {
+        const Range range = locate<C>(p, ranges, [&](long long per) { return cta * per; });
+        if (range.found < 0) {
+            return;  // past the end of the list
         }
-    }
+        const int row_tiles = (p.heads / p.cache.kv_heads * p.cache.tokens + kRows - 1) / kRows;
+        const int items = p.cache.kv_heads * row_tiles;
+        long long at = cta * range.per;
+        const long long end = min(at + range.per, range.total);
+        int b = range.found;
+        Sequence s = sequence<C>(p, b);
+        long long in_seq = at - range.found_base;
+        int item = static_cast<int>(in_seq / s.tiles);
+        int v = static_cast<int>(in_seq - static_cast<long long>(item) * s.tiles);
+        bool first = true;
+        while (at < end) {
+            const int take = static_cast<int>(min(static_cast<long long>(s.tiles - v), end - at));
+            const bool whole = v == 0 && take == s.tiles;
+            attend<C, CAREFUL>(p, status, smem, s, b, item / row_tiles, (item % row_tiles) * kRows, v, v + take, rec,
+                               whole ? -1 : 2ll * cta + (first ? 0 : 1));
+            first = false;
+            at += take;
+            v = 0;
+            if (at < end && ++item == items) {
+                item = 0;
+                s = sequence<C>(p, ++b);
+            }
+        }
+    });
 }
 
 // Joins the records of the item that was cut at unit k per, k = blockIdx.x + 1, if that is its first
@@ -876,44 +1004,77 @@ Split split_for(const FaCachedParams& p, int sm_count) {
     return {false, std::min<long long>(kCtasPerSm * sm_count, (items * tiles + kMinTiles - 1) / kMinTiles), items};
 }
 
-template <class C>
-cudaError_t launch(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
-    const Split split = split_for(p, sm_count);
-    if (split.grid > 0x7fffffffLL) {
-        return cudaErrorInvalidConfiguration;
-    }
-    const int grid = static_cast<int>(split.grid);
-    cudaError_t err = split.whole ? ensure_smem_limit<cached_whole_kernel<C>>(kSmem)
-                                  : ensure_smem_limit<cached_kernel<C>>(kSmem);
-    if (err != cudaSuccess) {
-        return err;
-    }
-    if (split.whole) {
-        cached_whole_kernel<C><<<grid, kThreads, kSmem, stream>>>(p, status);
-        return cudaGetLastError();
-    }
-    Record rec;
-    rec.o = static_cast<float*>(workspace);
-    rec.ml = reinterpret_cast<float2*>(rec.o + static_cast<size_t>(grid) * 2 * kRows * C::D);
-    cached_kernel<C><<<grid, kThreads, kSmem, stream>>>(p, status, rec);
-    err = cudaGetLastError();
-    if (err != cudaSuccess || grid == 1) {
-        return err;
-    }
-    const int rows = std::min(kRows, p.heads / p.cache.kv_heads * p.cache.tokens);
+// Launches after the kernel before it has started to end: it waits for its results itself.
+template <class... Params, class... Args>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int smem, cudaStream_t stream, const Args&... args) {
     cudaLaunchConfig_t config{};
-    constexpr int kResident = 16;  // CTAs of the join on an SM
-    const bool spread = static_cast<long long>(grid - 1) * rows <= kResident * sm_count || grid > 8 * split.items;
-    config.gridDim = dim3(static_cast<unsigned>(grid - 1), static_cast<unsigned>(spread ? rows : (rows + kWarps - 1) / kWarps));
+    config.gridDim = grid;
     config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = static_cast<size_t>(smem);
     config.stream = stream;
     cudaLaunchAttribute early{};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &early;
     config.numAttrs = 1;
-    return spread ? cudaLaunchKernelEx(&config, cached_join_kernel<C, true>, p, rec, grid)
-                  : cudaLaunchKernelEx(&config, cached_join_kernel<C, false>, p, rec, grid);
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
+template <class C>
+cudaError_t launch_join(const FaCachedParams& p, const Record& rec, const Split& split, int sm_count, cudaStream_t stream) {
+    const int grid = static_cast<int>(split.grid);
+    const int rows = std::min(kRows, p.heads / p.cache.kv_heads * p.cache.tokens);
+    constexpr int kResident = 16;  // CTAs of the join on an SM
+    const bool spread = static_cast<long long>(grid - 1) * rows <= kResident * sm_count || grid > 8 * split.items;
+    const dim3 join_grid(static_cast<unsigned>(grid - 1), static_cast<unsigned>(spread ? rows : (rows + kWarps - 1) / kWarps));
+    return spread ? launch_early(cached_join_kernel<C, true>, join_grid, 0, stream, p, rec, grid)
+                  : launch_early(cached_join_kernel<C, false>, join_grid, 0, stream, p, rec, grid);
+}
+
+// All items or ranges; with several tokens, those that have to be taken carefully; the join of what was cut.
+template <class C, bool WHOLE>
+cudaError_t launch_kernels(const FaCachedParams& p, DeviceStatus* status, const Record& rec, const Split& split, int sm_count,
+                           cudaStream_t stream) {
+    constexpr auto kernel = WHOLE ? cached_whole_kernel<C, false> : cached_kernel<C, false>;
+    constexpr auto careful = WHOLE ? cached_whole_kernel<C, true> : cached_kernel<C, true>;
+    const int ranges = static_cast<int>(split.grid);
+    cudaError_t err = ensure_smem_limit<kernel>(kSmem);
+    if (err == cudaSuccess && p.cache.tokens > 1) {
+        err = ensure_smem_limit<careful>(kSmemCareful);
+    }
+    if (err != cudaSuccess) {
+        return err;
+    }
+    kernel<<<ranges, kThreads, kSmem, stream>>>(p, status, rec, ranges);
+    err = cudaGetLastError();
+    if (err == cudaSuccess && p.cache.tokens > 1) {
+        // Half as many CTAs as SMs: they find room while the first kernel's last ranges run, and the join's CTAs after
+        // them (64 sequences x 4 tokens: 112.5 us, with a CTA for each range 115, without this kernel 110).
+        err = launch_early(careful, dim3(static_cast<unsigned>(std::min(ranges, std::max(sm_count / 2, 1)))), kSmemCareful, stream,
+                           p, status, rec, ranges);
+    }
+    if (err == cudaSuccess && !WHOLE && ranges > 1) {
+        err = launch_join<C>(p, rec, split, sm_count, stream);
+    }
+    return err;
+}
+
+template <class C>
+cudaError_t launch(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
+    const Split split = split_for(p, sm_count);
+    if (split.grid > 0x7fffffffLL) {
+        return cudaErrorInvalidConfiguration;
+    }
+    Record rec{};
+    if (split.whole) {
+        rec.odd = static_cast<int*>(workspace);
+        return launch_kernels<C, true>(p, status, rec, split, sm_count, stream);
+    }
+    const size_t rows = static_cast<size_t>(split.grid) * 2 * kRows;
+    rec.o = static_cast<float*>(workspace);
+    rec.ml = reinterpret_cast<float2*>(rec.o + rows * C::D);
+    rec.odd = reinterpret_cast<int*>(rec.ml + rows);
+    return launch_kernels<C, false>(p, status, rec, split, sm_count, stream);
 }
 
 template <int D, bool ONE_PAGE>
@@ -939,7 +1100,8 @@ cudaError_t launch_dim(const FaCachedParams& p, DeviceStatus* status, void* work
 
 unsigned long long cached_workspace_bytes(const FaCachedParams& p, int sm_count) {
     const Split split = split_for(p, sm_count);
-    return split.whole ? 0 : static_cast<unsigned long long>(split.grid) * 2 * kRows * (p.cache.head_dim + 2) * 4;
+    const unsigned long long records = split.whole ? 0 : static_cast<unsigned long long>(split.grid) * 2 * kRows * (p.cache.head_dim + 2) * 4;
+    return records + (p.cache.tokens > 1 ? 4ull * split.grid : 0);
 }
 
 cudaError_t launch_cached(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count,

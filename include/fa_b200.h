@@ -322,7 +322,8 @@ FA_API int fa_append_kv(const FaAppendParams* params, fa_stream_t stream);
 
 /* O = softmax(scale * q K^T | visible) V over the cache: q [batch, heads, tokens, head_dim] with
  * strides {batch, head, token}, o contiguous (zeros for padding tokens), both of type `dtype`;
- * a 16-bit cache has the same type. */
+ * a 16-bit cache has the same type. What a query does not see has no part in its output, whatever
+ * it holds, infinities and NaN among it (a later token's included). */
 typedef struct FaCachedParams {
     FaCache cache;
     const void* q;

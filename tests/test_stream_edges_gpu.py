@@ -207,3 +207,56 @@ def test_a_graph_of_the_gradients_may_be_asked_for():
     assert torch.equal(torch.autograd.grad(slope.sum(), other)[0], 6 * other.detach())
     with pytest.raises(RuntimeError, match="differentiated once"):
         again[0].sum().backward()
+
+
+# ------------------------------------------------------------------------- several tokens at once
+
+
+@pytest.mark.parametrize("dtype,cache_dtype", [(BF, E4M3), (HALF, E4M3), (BF, BF), (HALF, HALF)])
+@pytest.mark.parametrize("h,hk,t,page", [(4, 4, 4, 64), (16, 2, 4, 16), (8, 2, 3, 8), (2, 1, 20, 32), (3, 1, 37, 64)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(dtype, cache_dtype, h, hk, t, page, d):
+    """Of a later drafted token, and of a key that only the first tokens' windows still hold: an infinite or
+    NaN value makes its own column infinite or NaN in the rows that see it, and changes nothing else."""
+    gen = torch.Generator(DEV).manual_seed(10 + t)
+    pages = -(-150 // page)
+    cache, table = _filled(gen, 2, pages, page, hk, d, cache_dtype)
+    q = _rand(gen, (2, h, t, d), dtype)
+    lengths = _ints(150, 90 + t)
+    first = (lengths - t).tolist()
+    raw = cache.v.view(torch.uint8 if cache_dtype == E4M3 else torch.int16)
+    codes = {E4M3: (0x7F, 0xFF), HALF: (0x7E00, 0x7C00), BF: (0x7FC0, 0x7F80)}[cache_dtype]
+    for window, sinks in ((0, 0), (40, 3)):
+        plain = fa.forward_cached(q, cache, table, lengths, window=window, sinks=sinks)
+        assert torch.isfinite(plain).all()
+        for which, offset in enumerate((t - 1, 1, 1 - window) if window else (t - 1, 1)):
+            keys = [f + offset for f in first]
+            where = [(int(table[b, k // page]), k % page) for b, k in enumerate(keys)]
+            column = 5 + 16 * which
+            was = [raw[at, :, slot, column].clone() for at, slot in where]
+            for (at, slot) in where:
+                raw[at, :, slot, column] = codes[which % 2]
+            got = fa.forward_cached(q, cache, table, lengths, window=window, sinks=sinks)
+            want = plain.clone()
+            for b, k in enumerate(keys):
+                pos = first[b] + torch.arange(t, device=DEV)
+                sees = (k <= pos) & ((pos - k < window) if window else torch.ones_like(pos, dtype=torch.bool))
+                assert sees.any() and not sees.all()
+                bad = ~torch.isfinite(got[b, :, sees, column])
+                assert bad.all()
+                want[b, :, sees, column] = got[b, :, sees, column]
+            same = (got == want) | (got.isnan() & want.isnan())
+            assert same.all(), (window, which)
+            for (at, slot), x in zip(where, was):
+                raw[at, :, slot, column] = x
+    assert _C.device_status(0) == 0
+
+
+def test_scores_of_a_later_token_that_are_nan_stay_with_it():
+    gen = torch.Generator(DEV).manual_seed(11)
+    cache, table = _filled(gen, 1, 3, 64, 2, 128, E4M3)
+    q = _rand(gen, (1, 8, 4, 128), BF)
+    plain = fa.forward_cached(q, cache, table, _ints(130))
+    cache.k.view(torch.uint8)[int(table[0, 2]), :, 1, 9] = 0x7F  # position 129, the last token's
+    got = fa.forward_cached(q, cache, table, _ints(130))
+    assert torch.equal(got[:, :, :3], plain[:, :, :3]) and got[:, :, 3].isnan().all()
