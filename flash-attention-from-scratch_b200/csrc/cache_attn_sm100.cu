@@ -27,8 +27,8 @@
 // Products are mma.sync m16n8k16: with 16 rows of queries and two operations a byte of K
 // or V an M = 128 tcgen05 tile would be seven eighths padding, and dequantised operands would have to
 // go back to shared memory for it. e4m3 widens exactly to float16; bfloat16 queries are brought
-// into float16's range by a power of two per row, which is exact but for values 2^-38 below
-// the row's largest. Both products permute their contraction (head dim, keys) and output columns so
+// into float16's range by a power of two per row: the largest in [2^13, 2^14), steps of 2^-24, so that values
+// down to 2^-30 of the row's largest are exact; smaller ones round to those steps and vanish from 2^-38 on. Both products permute their contraction (head dim, keys) and output columns so
 // that a lane's fragments are whole 16-byte words of the cache's own rows.
 //
 // e4m3's value scales. With w_j = e^(s_j) vs_j (vs_j: the scale of j's page) O = sum w_j c_j / sum

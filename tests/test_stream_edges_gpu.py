@@ -260,3 +260,28 @@ def test_scores_of_a_later_token_that_are_nan_stay_with_it():
     cache.k.view(torch.uint8)[int(table[0, 2]), :, 1, 9] = 0x7F  # position 129, the last token's
     got = fa.forward_cached(q, cache, table, _ints(130))
     assert torch.equal(got[:, :, :3], plain[:, :, :3]) and got[:, :, 3].isnan().all()
+
+
+# ------------------------------------------------------------------------- bfloat16 queries, e4m3 keys
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_bf16_queries_of_mixed_size_over_e4m3(d):
+    """A row whose values are up to 2^30 apart, the small ones meeting large keys: they are in the scores in full.
+    From 2^-38 on they are not there, and nothing else happens."""
+    gen = torch.Generator(DEV).manual_seed(12)
+    k = (torch.randn(2, 1, 64, d, generator=gen, device=DEV) * 64).to(E4M3)
+    k[..., 0] = 0
+    v = _rand(gen, (2, 1, 64, d), HALF).to(E4M3)
+    table, lengths = _ints(0, 1).view(1, 2), _ints(100)
+    for power, exact in ((-20, True), (-29, True), (-30, True), (-40, False)):
+        # the small queries' scores are of the order of 1 whatever their size
+        scale = torch.full((2, 1), 2.0 ** (-power - 6), device=DEV)
+        cache = fa.PagedKVCache(k, v, scale, torch.ones(2, 1, device=DEV))
+        q = torch.zeros(1, 2, 1, d, dtype=BF, device=DEV)
+        q[..., 0] = 1.0
+        q[:, 0, :, 1:9] = 1.9921875 * 2.0**power
+        q[:, 1, :, 1:9] = -1.0078125 * 2.0**power
+        got = fa.forward_cached(q, cache, table, lengths)
+        want, vmax = oracle.cached(q if exact else torch.zeros_like(q), cache, table, lengths)
+        oracle.check(got, want, oracle.forward_bound(want, vmax, oracle.unit(HALF), oracle.unit(BF)), f"O at 2^{power}")
