@@ -25,7 +25,7 @@ import struct
 import torch
 
 from fa import _C
-from fa.window import _NO_STRIDES, _on_device, _tensor_strides
+from fa.window import _NO_STRIDES, _on_device, _packed, _tensor_strides
 
 # FaCache, then FaAppendParams' and FaCachedParams' own fields (include/fa_b200.h).
 _CACHE = "7P5q7iB3x"
@@ -238,7 +238,8 @@ def forward_cached(
     if q.numel() == 0:
         return o
     scale = 1.0 / math.sqrt(dim) if softmax_scale is None else float(softmax_scale)
-    params = _CACHED.pack(*fields, q.data_ptr(), o.data_ptr(), *_tensor_strides(q), heads, window, sinks, scale,
-                          _C.DTYPES[q.dtype])
+    params = _packed(
+        _CACHED, *fields, q.data_ptr(), o.data_ptr(), *_tensor_strides(q), heads, window, sinks, scale,
+        _C.DTYPES[q.dtype])
     _on_device(cache._index, _run_cached, params, cache._device)
     return o

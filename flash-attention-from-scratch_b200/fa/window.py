@@ -28,6 +28,15 @@ _NO_GRADS = (0,) * 4
 _NO_STRIDES = (0,) * 3
 
 
+def _packed(block: struct.Struct, *values) -> bytes:
+    """A parameter block. What its types do not hold is the caller's window or sinks: sizes of tensors that exist fit
+    or are refused by the library, as is a softmax_scale that becomes infinite."""
+    try:
+        return block.pack(*values)
+    except struct.error as e:
+        raise ValueError(f"window and sinks must be 32-bit integers: {e}") from None
+
+
 def _tensor_strides(t: torch.Tensor) -> tuple[int, int, int]:
     """{batch, head, row} strides; 0 for a dim of one element, whose stride means nothing."""
     s0, s1, s2, s3 = t.stride()
@@ -57,8 +66,8 @@ def _check(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
 def _pack(q, k, v, o, lse, grads, grad_strides, window, sinks, softmax_scale) -> bytes:
     (b, h, nq, d), (_, hk, nk, _) = q.shape, k.shape
     scale = 1.0 / math.sqrt(d) if softmax_scale is None else float(softmax_scale)
-    return _PARAMS.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(), *grads,
+    return _packed(
+        _PARAMS, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(), *grads,
         *_tensor_strides(q), *_tensor_strides(k), *_tensor_strides(v), *_tensor_strides(o), *grad_strides,
         b, h, hk, nq, nk, d, window, sinks, scale, _C.DTYPES[q.dtype])
 

@@ -285,3 +285,19 @@ def test_bf16_queries_of_mixed_size_over_e4m3(d):
         got = fa.forward_cached(q, cache, table, lengths)
         want, vmax = oracle.cached(q if exact else torch.zeros_like(q), cache, table, lengths)
         oracle.check(got, want, oracle.forward_bound(want, vmax, oracle.unit(HALF), oracle.unit(BF)), f"O at 2^{power}")
+
+
+# ------------------------------------------------------------------------------------ arguments
+
+
+@pytest.mark.parametrize("change", [{"window": 1 << 31}, {"sinks": 1 << 40}, {"window": 2.5}])
+def test_arguments_beyond_their_types_are_refused(change):
+    """In the library's manner: an error that says what is wrong with which argument."""
+    q, k, v, do = _dense(1, 2, 1, 16, 16, 64, HALF, seed=13)
+    cache = fa.PagedKVCache.empty(1, 16, 1, 64, device=DEV)
+    args = {"window": 4, "sinks": 1} | change
+    o, lse = fa.forward_window(q, k, v, 4, return_lse=True)
+    for call in (lambda: fa.forward_window(q, k, v, **args), lambda: fa.backward_window(do, q, k, v, o, lse, **args),
+                 lambda: fa.forward_cached(q[:, :, :1], cache, _ints(0).view(1, 1), _ints(5), **args)):
+        with pytest.raises(ValueError, match="32-bit"):
+            call()
