@@ -19,17 +19,22 @@
 // 16-bit ones. Rings of 2 tiles and 3 CTAs an SM (168 registers a thread) keep 96 KB in flight; 6.5 TB/s
 // at about 1 us needs 44. (3 tiles and 2 CTAs: 136 us where this takes 87, for want of warps.)
 //
-// Measured, 32 query heads on 8, D 128, e4m3, pages of 64: 32 sequences of 4000 to 8000 tokens 77 us (5.2 TB/s),
-// 4 of 120000 to 131000 167 us (6.1 TB/s), 64 x 4 drafted tokens over a window of 4096 and 4 sinks 110 us
-// (4.9 TB/s). What is left: the instructions of a tile (about 730, half of the issue slots), and for short
-// ranges the start of an item, its join in shared memory and the second launch.
+// Measured, 32 query heads on 8, D 128, e4m3, pages of 64, one state replayed in bursts: 32 sequences of 4000 to 8000
+// tokens 78 us (5.1 TB/s), 4 of 120000 to 131000 168 us (6.0 TB/s), 64 x 4 drafted tokens over a window of 4096 and 4
+// sinks 112 us (4.8 TB/s); calls in turn under load that lasts, at the power cap, 80, 182 and 116 us. With 16-bit
+// values 126, 305 and 178 us, at the copy's rate. What is left: the instructions of a tile (about 730, half of the
+// issue slots), and for short ranges the start of an item, its join in shared memory and the second launch. A long
+// chunk of tokens is slow: a sequence has one list of key tiles, from its first query's window to its last
+// query, for all its row tiles, and from 16 tokens on a row tile is one head's, so that a group's heads read
+// the tiles each for itself (4000 tokens on nothing before them 1.6 ms, where the dense window forward takes 0.18).
 //
 // Products are mma.sync m16n8k16: with 16 rows of queries and two operations a byte of K
 // or V an M = 128 tcgen05 tile would be seven eighths padding, and dequantised operands would have to
 // go back to shared memory for it. e4m3 widens exactly to float16; bfloat16 queries are brought
 // into float16's range by a power of two per row: the largest in [2^13, 2^14), steps of 2^-24, so that values
-// down to 2^-30 of the row's largest are exact; smaller ones round to those steps and vanish from 2^-38 on. Both products permute their contraction (head dim, keys) and output columns so
-// that a lane's fragments are whole 16-byte words of the cache's own rows.
+// down to 2^-30 of the row's largest are exact; smaller ones round to those steps and vanish from 2^-38 on. Both
+// products permute their contraction (head dim, keys) and output columns so that a lane's fragments are whole
+// 16-byte words of the cache's own rows.
 //
 // e4m3's value scales. With w_j = e^(s_j) vs_j (vs_j: the scale of j's page) O = sum w_j c_j / sum
 // (w_j / vs_j) over the codes c_j. The running maximum is taken over log2 w_j = s_j log2 e + log2

@@ -17,10 +17,11 @@
 //
 // The window build (FwdCfg's WIN flag; window attention of an extension): the same pipeline over a list of
 // key tiles, those of the sinks and of the item's windows, with grouped heads, q_len != k_len, 4-D tensor
-// maps for strides and the row's log-sum-exp. Measured, bf16, window 1024 + 4 sinks: 4 x 16 x 4096 x 128
-// 159 us (760 TFLOP/s of visible pairs), 16 x 8191 x 128 on 4 kv heads 94 us; window 4096, 8 x 16384:
-// 259 us (930). A tile of two query tiles takes about 1.9 us, an item about 5 us beside its tiles (fill, drain, epilogue,
-// masked tiles), which bounds short windows.
+// maps for strides and the row's log-sum-exp. Measured, bf16, window 1024 + 4 sinks, in bursts (SM clock 1.9 GHz):
+// 4 x 16 x 4096 x 128 161 us (750 TFLOP/s of visible pairs), 16 x 8191 x 128 on 4 kv heads 98 us; window 4096,
+// 8 x 16384: 264 us (910). Under load that lasts, at the power cap (1.8 GHz), the first takes 176 us. A tile of
+// two query tiles takes about 1.9 us, an item about 5 us beside its tiles (fill, drain, epilogue, masked tiles),
+// which bounds short windows.
 //
 // Work item = one (b,h) head x NQ consecutive 128-row query tiles (NQ = 2; 1 for fp16acc, d = 128)
 // x one key range (split-KV). Each CTA runs one item, or, for short rows (N <= 2048), a

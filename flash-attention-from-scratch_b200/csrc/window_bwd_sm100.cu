@@ -36,11 +36,13 @@
 // quarter of the SMs idle (254 lists of 132 tiles on 148 SMs). A cut list's parts leave float32
 // sums in the workspace, at most two a CTA, and a last kernel adds them up in order.
 
-// Measured, bf16, D 128 (of 1689 TFLOP/s): 16 x 8191 on 4 kv heads, window 1024 + 4 sinks 279 us, 8 x 16384 on 2,
-// window 4096 725 us (830 TFLOP/s of the 5 products of visible pairs, 1160 of the 7 computed). A DKV step is
-// 2048 cycles of products and 2400 of shared memory (192 KB of operands, 64 KB arriving, the columns' LSE and delta),
-// a dQ step 1536 and 1800, which is what bounds them: without the exponentials they take as long. Tiles
-// shared by two SMs (cta_group::2) would halve the streamed operands.
+// Measured, bf16, D 128 (of 1689 TFLOP/s), in bursts: 16 x 8191 on 4 kv heads, window 1024 + 4 sinks 280 us, 8 x 16384 on
+// 2, window 4096 780 us (770 TFLOP/s of the 5 products of visible pairs, 1080 of the 7 computed); float16 290 and 810 us. A
+// DKV step is 2048 cycles of products and 2400 of shared memory (192 KB of operands, 64 KB arriving, the columns' LSE and
+// delta), a dQ step 1536 and 1800, which is what bounds them: without the exponentials they take as long. Tiles
+// shared by two SMs (cta_group::2) would halve the streamed operands. At d = 64 the softmax bounds them (2 x 16 x 8192 on 4
+// kv heads, window 1024: 420 us), and its loop is about as long as the SM fetches in time: a few dozen instructions more
+// took up to 18% of the dK, dV pass, with the stalls for want of an instruction up from 0.25 to 0.44 an issue.
 
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -2,7 +2,8 @@
 
 Query i of q [B, H, Nq, D] is at position p = Nk - Nq + i of the keys k, v [B, Hkv, Nk, D] and
 sees key j when 0 <= j <= p and (window == 0, or p - j < window, or j < sinks). H is a multiple of
-Hkv: query head h reads key/value head h // (H // Hkv). A query that sees nothing gives O = 0.
+Hkv: query head h reads key/value head h // (H // Hkv). A query that sees nothing gives O = 0. What is hidden
+weighs 0 exactly, but infinities and NaN of v (in the gradients: of any input) reach rows of the same tile of 128.
 float16 or bfloat16, D in {64, 128}; the last dim is contiguous, the other strides are multiples
 of 8 elements (a [B, N, H, D] tensor's transpose(1, 2) is fine). Not in the reference, whose
 attention is over all keys or all keys up to the query's own, and forward only.

@@ -211,7 +211,12 @@ FA_API int fa_flash_fwd_splitkv_static(const FaFwdParams* params, int32_t num_sp
 
 /* Window attention over dense tensors: q, o, d_o, dq [batch, heads, q_len, head_dim], k, v, dk,
  * dv [batch, kv_heads, k_len, head_dim]; query i is at position k_len - q_len + i. Strides are
- * {batch, head, row}, positive for a dim of more than one element (no broadcast dims). dtype is FA_DTYPE_FLOAT16 or FA_DTYPE_BFLOAT16, for all of them. */
+ * {batch, head, row}, positive for a dim of more than one element (no broadcast dims). dtype is FA_DTYPE_FLOAT16
+ * or FA_DTYPE_BFLOAT16, for all of them.
+ *
+ * Hidden pairs weigh 0 exactly, in O and in the gradients. Tiles of 128 queries and 128 keys are multiplied whole,
+ * though, so an infinite or NaN value of v (in the gradients: of q, k, v, o or d_o) makes NaN of rows that share a tile with
+ * it without seeing it. A NaN score makes its row's O, LSE and gradients NaN. */
 typedef struct FaWindowParams {
     const void* q;
     const void* k;
