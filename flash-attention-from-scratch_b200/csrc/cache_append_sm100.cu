@@ -146,13 +146,13 @@ __device__ __forceinline__ void store_page(const FaAppendParams& p, DeviceStatus
     unit /= c.kv_heads;
     const int span = unit % spans;
     const int b = unit / spans;
-    const int len = c.lengths[b];
+    const int len = max(c.lengths[b], 0);
     const int count = c.counts != nullptr ? min(max(c.counts[b], 0), c.tokens) : c.tokens;
     const int start = len - count;
     const int page = (max(start, 0) >> log2_page) + span;
-    const int base = page << log2_page;
+    const int base = static_cast<int>(static_cast<unsigned>(page) << log2_page);  // negative: a page beyond 2^31 tokens
     const int lo = max(start, base);
-    int hi = min(len, base + c.page_size);
+    int hi = base < 0 ? 0 : (len - base > c.page_size ? base + c.page_size : len);
     const bool leader = threadIdx.x == 0 && h == 0 && !is_v;
     if (leader && span == 0 && start < 0 && count > 0) {
         atomicOr(&status->code, kStatusBadPage);
@@ -317,7 +317,7 @@ __device__ __forceinline__ void rotate_queries(const FaAppendParams& p, DeviceSt
     const int h_end = min((hb + 1) * split.heads, p.heads);
     const int h0 = hb * split.heads + (row >> split.log2_tokens);
     const int count = c.counts != nullptr ? min(max(c.counts[b], 0), c.tokens) : c.tokens;
-    const int pos = c.lengths[b] - count + t;
+    const int pos = max(c.lengths[b], 0) - count + t;
     const bool mine = t < c.tokens;
     bool live = t < count;
     if (live && (pos < 0 || (p.cos != nullptr && pos >= p.table_rows))) {

@@ -98,6 +98,21 @@ def test_lengths_beyond_the_table_end_with_it(page, pages, window, sinks, dtype)
     oracle.check(got, want, oracle.forward_bound(want, vmax, oracle.unit(HALF), oracle.unit(HALF)), "O")
 
 
+@pytest.mark.parametrize("length", [2**31 - 1, 2**31 - 17, -(2**31), -1])
+@pytest.mark.parametrize("page", [8, 64])
+def test_append_at_the_ends_of_the_integers_is_skipped_and_reported(length, page):
+    """Lengths that no table has a place for, at the ends of their type: nothing is stored for them, the bit is set,
+    and the other sequence is as it would be."""
+    gen = torch.Generator(DEV).manual_seed(3)
+    cache = fa.PagedKVCache(*(torch.zeros(6, 1, page, 64, dtype=HALF, device=DEV) for _ in "kv"))
+    k = _rand(gen, (2, 1, 20, 64), HALF)
+    table = _ints(0, 1, 2, 3, 4, 5).view(2, 3)
+    fa.append_kv(cache, k, k, table, _ints(length, 20))
+    assert _C.device_status(0, clear=True) == 32
+    for pool in (cache.k, cache.v):
+        assert not pool[:3].any() and torch.equal(oracle.dense(pool, None, table)[1, :, :20], k[1].double())
+
+
 # ------------------------------------------------------------------------------ window attention
 
 
