@@ -45,6 +45,9 @@ LIBS = {
         "flash_fwd_sm100.cu",
         "cache_append_sm100.cu",
         "cache_attn_sm100.cu",
+        "tree_attn_sm100.cu",
+        "rotary_sm100.cu",
+        "pages_sm100.cu",
         "window_bwd_sm100.cu",
         "capi.cu",
         "capi_static.cu",

@@ -1,6 +1,6 @@
 #pragma once
 // Host/device shared definitions of the streaming-attention kernels: the paged cache
-// (cache_append_sm100.cu, cache_attn_sm100.cu) and window attention (window_bwd_sm100.cu and the
+// (cache_append_sm100.cu, cache_attn_sm100.cu, tree_attn_sm100.cu, pages_sm100.cu), rotation (rotary_sm100.cu) and window attention (window_bwd_sm100.cu and the
 // window build of flash_fwd_sm100.cu).
 
 #include <cuda_runtime.h>
@@ -29,6 +29,18 @@ cudaError_t launch_append(const FaAppendParams& p, DeviceStatus* status, cudaStr
 unsigned long long cached_workspace_bytes(const FaCachedParams& p, int sm_count);
 cudaError_t launch_cached(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count,
                           cudaStream_t stream);
+
+unsigned long long tree_workspace_bytes(const FaTreeParams& p, int sm_count);
+cudaError_t launch_tree(const FaTreeParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream);
+
+cudaError_t launch_rotary(const FaRotaryParams& p, DeviceStatus* status, int sm_count, cudaStream_t stream);
+
+cudaError_t launch_keep_tokens(const FaKeepParams& p, DeviceStatus* status, cudaStream_t stream);
+cudaError_t launch_copy_pages(const FaCopyParams& p, DeviceStatus* status, cudaStream_t stream);
+cudaError_t launch_fork_pages(const FaPages& p, DeviceStatus* status, cudaStream_t stream);
+cudaError_t launch_free_pages(const FaPages& p, DeviceStatus* status, cudaStream_t stream);
+unsigned long long reserve_workspace_bytes(const FaPages& p);
+cudaError_t launch_reserve_pages(const FaPages& p, DeviceStatus* status, void* workspace, cudaStream_t stream);
 
 cudaError_t launch_window_fwd(const FaWindowParams& p, DeviceStatus* status, unsigned epoch, int sm_count,
                               cudaStream_t stream);

@@ -116,14 +116,19 @@ def _load() -> ctypes.CDLL:
     lib.fa_flash_fwd_fp8.argtypes = [ctypes.POINTER(FaFwdParams), ctypes.c_float, ctypes.c_float, ctypes.c_float,
                                      ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]
     lib.fa_flash_fwd_fp8.restype = ctypes.c_int
-    # The streaming operators take their parameter blocks as packed bytes (fa/window.py, fa/cache.py).
-    for name, extra in (("fa_window_fwd", ()), ("fa_append_kv", ()),
+    # The streaming operators take their parameter blocks as packed bytes (fa/window.py, fa/cache.py,
+    # fa/rotation.py, fa/draft.py, fa/pages.py).
+    for name, extra in (("fa_window_fwd", ()), ("fa_append_kv", ()), ("fa_rotary", ()), ("fa_keep_tokens", ()),
+                        ("fa_copy_pages", ()), ("fa_fork_pages", ()), ("fa_free_pages", ()),
+                        ("fa_tree_attention", (ctypes.c_void_p, ctypes.c_uint64)),
+                        ("fa_reserve_pages", (ctypes.c_void_p, ctypes.c_uint64)),
                         ("fa_window_bwd", (ctypes.c_void_p, ctypes.c_uint64)),
                         ("fa_cached_attention", (ctypes.c_void_p, ctypes.c_uint64))):
         fn = getattr(lib, name)
         fn.argtypes = [ctypes.c_char_p, *extra, ctypes.c_void_p]
         fn.restype = ctypes.c_int
-    for name in ("fa_window_bwd_workspace_size", "fa_cached_workspace_size"):
+    for name in ("fa_window_bwd_workspace_size", "fa_cached_workspace_size", "fa_tree_workspace_size",
+                 "fa_reserve_workspace_size"):
         fn = getattr(lib, name)
         fn.argtypes = [ctypes.c_char_p, ctypes.POINTER(ctypes.c_uint64)]
         fn.restype = ctypes.c_int

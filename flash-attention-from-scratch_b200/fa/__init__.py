@@ -11,7 +11,9 @@ Same public surface as the reference package (fa/__init__.py:14-38): ``forward``
 tensors in and out, transfers overlapped with the kernels) and the multi-GPU ``forward_sharded`` /
 ``plan_shards``. Streaming attention (an extension): ``forward_window`` / ``backward_window`` /
 ``window_attention`` over a sliding window with sinks, and ``PagedKVCache`` with ``append_kv`` and
-``forward_cached``. The kernel is tcgen05 / TMEM / TMA code for sm_100a in
+``forward_cached``. Drafted tokens (an extension): ``rotary`` by positions on several axes,
+``forward_tree`` and ``keep_tokens`` over the cache, ``reserve_pages`` / ``fork_pages`` /
+``free_pages`` / ``copy_pages`` for its pages. The kernel is tcgen05 / TMEM / TMA code for sm_100a in
 libfa_b200.so; there is no CPU or fallback path.
 """
 
@@ -19,8 +21,11 @@ import torch
 
 from fa import _C
 from fa.cache import PagedKVCache, append_kv, forward_cached
+from fa.draft import forward_tree, keep_tokens
 from fa.host import forward_host
+from fa.pages import copy_pages, fork_pages, free_pages, reserve_pages
 from fa.reference import attention_reference
+from fa.rotation import backward_rotary, forward_rotary, rotary
 from fa.shard import forward_sharded, plan_shards
 from fa.window import backward_window, forward_window, window_attention
 
@@ -98,4 +103,5 @@ def forward_splitkv(
 
 __all__ = ["forward", "forward_variant", "forward_splitkv", "forward_fp8", "quantize_fp8", "forward_host",
            "attention_reference", "forward_sharded", "plan_shards", "forward_window", "backward_window",
-           "window_attention", "PagedKVCache", "append_kv", "forward_cached"]
+           "window_attention", "PagedKVCache", "append_kv", "forward_cached", "forward_rotary", "backward_rotary", "rotary",
+           "forward_tree", "keep_tokens", "reserve_pages", "fork_pages", "free_pages", "copy_pages"]

@@ -350,6 +350,158 @@ FA_API int fa_cached_workspace_size(const FaCachedParams* params, uint64_t* byte
 FA_API int fa_cached_attention(const FaCachedParams* params, void* workspace, uint64_t workspace_bytes,
                                fa_stream_t stream);
 
+/* ---- Drafting and keeping tokens (no counterpart in the reference): rotation by positions on
+ *      several axes, attention of a tree of drafted tokens over the cache, the accepted path moved
+ *      together, and the pages' bookkeeping. Buffers, streams, errors and status bits as above. */
+
+/* Rotates rows of queries and keys: q, q_out [batch, heads, tokens, head_dim], k, k_out [batch,
+ * kv_heads, tokens, head_dim] (k NULL: none), strides {batch, head, token}, the outputs contiguous
+ * and apart from the inputs. Pair i, the dims (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with
+ * `interleaved`, turns by cos and sin [table_rows, rotary_dim / 2] (floats, contiguous) at row
+ * positions[axis_of_pair[i]][batch][token], column i; dims from rotary_dim on are copied. inverse
+ * turns back, which is the gradient's way through it. The products and their sum are rounded to
+ * float32 each, the result once more to `dtype`, as in fa_append_kv. A token with a negative position
+ * on any axis is padding: zeros. One with a position of table_rows or more is zeros, too, and sets
+ * bit 5 (32) of fa_device_status. */
+typedef struct FaRotaryParams {
+    const void* q;
+    const void* k;
+    void* q_out;
+    void* k_out;
+    const int32_t* positions; /* {axis, batch, token} strides below, which may be 0 */
+    const float* cos;
+    const float* sin;
+    int64_t q_stride[3];
+    int64_t k_stride[3];
+    int64_t position_stride[3];
+    int32_t batch;
+    int32_t heads;
+    int32_t kv_heads; /* 0 without k */
+    int32_t tokens;
+    int32_t head_dim;   /* 64 or 128 */
+    int32_t rotary_dim; /* a multiple of 16 up to head_dim */
+    int32_t table_rows;
+    int32_t axes; /* 1 .. 4 */
+    uint8_t axis_of_pair[64];
+    uint8_t interleaved;
+    uint8_t inverse;
+    uint8_t dtype; /* FA_DTYPE_FLOAT16 or FA_DTYPE_BFLOAT16 */
+    uint8_t reserved[5];
+} FaRotaryParams;
+
+FA_API int fa_rotary(const FaRotaryParams* params, fa_stream_t stream);
+
+/* Attention of a tree of drafted tokens: like fa_cached_attention, but the `tokens` (at most 256)
+ * newest tokens are nodes of a tree, stored in the cache behind the context one after another.
+ * parents [batch, tokens]: the index of each node's parent, below its own, or -1 for a node that
+ * hangs on the context. Anything else counts as -1 and sets bit 5 (32) of fa_device_status. Node t is
+ * at position p = context + (number of its ancestors), context = lengths[b] - counts[b]. It sees
+ * position j of the context when window == 0, or p - j < window, or j < sinks, and of the nodes its
+ * ancestors and itself. window is 0 or at least `tokens`. */
+typedef struct FaTreeParams {
+    FaCache cache;
+    const void* q;
+    void* o;
+    const int32_t* parents;
+    int64_t q_stride[3];
+    int64_t parent_stride; /* from row to row; may be 0 */
+    int32_t heads;
+    int32_t window; /* 0: none */
+    int32_t sinks;
+    float softmax_scale;
+    uint8_t dtype; /* FA_DTYPE_FLOAT16 or FA_DTYPE_BFLOAT16 */
+    uint8_t reserved[7];
+} FaTreeParams;
+
+/* Bytes of device workspace fa_tree_attention needs on the current device (148 SMs assumed without
+ * one). */
+FA_API int fa_tree_workspace_size(const FaTreeParams* params, uint64_t* bytes_out);
+
+/* Enqueues O on `stream`; `workspace` as in fa_window_bwd. Bitwise deterministic. */
+FA_API int fa_tree_attention(const FaTreeParams* params, void* workspace, uint64_t workspace_bytes,
+                             fa_stream_t stream);
+
+/* Moves kept tokens together: of the cache.counts[b] (or all cache.tokens, at most 256) newest tokens
+ * of sequence b, token kept[b][j] goes to where token j was, for every j before the first -1. kept
+ * [batch, most] ascends in every row; an entry that does not, or is no token's, ends the row and sets
+ * bit 5 (32) of fa_device_status. new_lengths[b] = lengths[b] - counts[b] + (number kept).
+ *
+ * e4m3: the scale of a page that tokens come to becomes the largest of its own and theirs; where it grows the
+ * page's other tokens (below lengths[b]) are rescaled. No page of the kept tokens may belong to two
+ * sequences. Positions outside the table and pages outside the pool are skipped as in fa_append_kv. */
+typedef struct FaKeepParams {
+    FaCache cache;
+    const int32_t* kept;
+    int32_t* new_lengths;
+    int64_t kept_stride;
+    int32_t most; /* up to cache.tokens */
+    int32_t reserved;
+} FaKeepParams;
+
+FA_API int fa_keep_tokens(const FaKeepParams* params, fa_stream_t stream);
+
+/* Copies pages src[i] to dst[i] (all heads of k and v, and the scales), i < count. A pair with a
+ * negative page is skipped, one with a page outside the pool too, and sets bit 5 (32) of
+ * fa_device_status. No page may be the target of two pairs, nor the target of one and the source of
+ * another. Of `cache` the pool's fields are used: k to v_scale, k_stride, v_stride, num_pages,
+ * page_size, kv_heads, head_dim, dtype. */
+typedef struct FaCopyParams {
+    FaCache cache;
+    const int32_t* src;
+    const int32_t* dst;
+    int32_t count;
+    int32_t reserved;
+} FaCopyParams;
+
+FA_API int fa_copy_pages(const FaCopyParams* params, fa_stream_t stream);
+
+/* The bookkeeping of a pool's pages: refs [num_pages] counts the page-table entries that hold each
+ * page (0: free), and an entry of -1 holds none. Entries outside the pool count as -1 and set bit 5
+ * (32) of fa_device_status. One FaPages serves three calls, which read and write on the device only:
+ *
+ * fa_fork_pages: row i of `table` becomes a copy of row rows[i] of `from` [from_batch, width], whose pages
+ * count one reference more. A rows[i] of -1 gives a row without pages; another one outside `from` too, and
+ * sets bit 5.
+ *
+ * fa_free_pages: entries from keep[b] on (all, without keep) of row b of `table` become -1 and their pages count
+ * one reference less. A page that has none left to give sets bit 5 and stays at 0.
+ *
+ * fa_reserve_pages: makes room for the counts[b] (or `tokens`) newest of lengths[b] tokens of row b, pages of its
+ * own for the positions from lengths[b] - counts[b] on: where the entry is missing, or its page has
+ * other references, a free page takes its place, lowest number first, rows in order, entries in order, and the shared page
+ * counts one reference less. What is free and shared is as the call finds it. If the first of these pages was
+ * shared and holds older tokens, src[b], dst[b] are the pages to copy (fa_copy_pages), else -1. A row is
+ * granted when it needs no page, or the rows up to it need no more than there are; granted[b] is then 1, else
+ * 0 and the row stays as it was. A row whose positions do not fit the table, or are negative, is not granted and sets bit 5.
+ * No row of `table` may occur twice. */
+typedef struct FaPages {
+    int32_t* refs;
+    int32_t* table; /* [batch, width], rows table_stride apart */
+    const int32_t* from;
+    const int32_t* rows;
+    const int32_t* keep;
+    const int32_t* lengths;
+    const int32_t* counts;
+    uint8_t* granted;
+    int32_t* src;
+    int32_t* dst;
+    int64_t table_stride;
+    int64_t from_stride;
+    int32_t num_pages;
+    int32_t batch;
+    int32_t width; /* width * page_size < 2^31 */
+    int32_t from_batch;
+    int32_t tokens;
+    int32_t page_size; /* a power of two, 8 .. 256 */
+} FaPages;
+
+FA_API int fa_fork_pages(const FaPages* params, fa_stream_t stream);
+FA_API int fa_free_pages(const FaPages* params, fa_stream_t stream);
+
+/* Bytes of device workspace fa_reserve_pages needs; `workspace` as in fa_window_bwd. */
+FA_API int fa_reserve_workspace_size(const FaPages* params, uint64_t* bytes_out);
+FA_API int fa_reserve_pages(const FaPages* params, void* workspace, uint64_t workspace_bytes, fa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
