@@ -10,6 +10,7 @@
 #include <cmath>
 #include <cstdint>
 
+#include "softmax_common.cuh"
 #include "sm100_ptx.cuh"
 #include "stream_internal.h"
 
@@ -18,8 +19,87 @@ namespace fa_sm100 {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100: smaller scales of values enter as this, with P scaled down
+constexpr float kLeastFactor = 1e-37f;               // of a score: what is hidden (-inf) stays so
+constexpr float kLazy = 8.0f;                        // P is at most 2^this before O and the sum are rescaled
 constexpr int kMostNodes = 256;
 constexpr int kMaskWords = kMostNodes / 32;
+
+constexpr int kTile = 128;  // query rows, and keys, of a product
+constexpr int kBox = 128 * 128;  // bytes of 128 rows of 64 16-bit values, 128-byte swizzle
+
+constexpr int kSoftmaxWarps = 8;
+constexpr int kLoadWarps = 8;  // half of them K, half V
+constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
+constexpr int kWarps = kMmaWarp + 4;  // whole warpgroups: registers are handed over between those
+constexpr int kThreads = kWarps * 32;
+// Registers: launched with 96 a thread (65536 / 640, in steps of 8), 480 for a lane of the five warpgroups.
+constexpr int kRegsSoftmax = 112;
+constexpr int kRegsLoad = 96;
+constexpr int kRegsMma = 64;
+static_assert(2 * kRegsSoftmax + 2 * kRegsLoad + kRegsMma <= 5 * 96, "no more than the launch has");
+
+constexpr int kListWarp = kMmaWarp + 1;  // and the two after it: the list of key tiles
+constexpr int kListWarps = 3;
+constexpr int kVStages = 2;
+constexpr int kListed = 8;  // key tiles listed ahead
+constexpr int kGroups = kTile / 8;  // keys that surely share a page
+
+template <int D_, bool BF16_, bool E4M3_, int NR_>
+struct Cfg {
+    static constexpr int D = D_;
+    static constexpr bool BF16 = BF16_;  // queries and output
+    static constexpr bool E4M3 = E4M3_;
+    static constexpr int NR = NR_;  // row tiles of an item: 1 (key tiles alternate between the softmax warpgroups) or 2
+    static constexpr bool kMmaBf16 = BF16 && !E4M3;
+    static constexpr int kElem = E4M3 ? 1 : 2;
+    static constexpr int kTileBytes = kBox * (D / 64);
+    static constexpr int kSmemQ = 0;
+    static constexpr int kSmemK = NR * kTileBytes;
+    static constexpr int kKStages = NR == 1 ? 3 : 2;
+    static constexpr int kSmemV = kSmemK + kKStages * kTileBytes;
+    static constexpr int kSmemShared = kSmemV + kVStages * kTileBytes;
+    static constexpr int kRows = NR * kTile;
+    // Tensor memory: two scores, P over each's first half, two sums.
+    static constexpr uint32_t kTmemS = 0;
+    static constexpr uint32_t kTmemO = 2 * kTile;
+    // A loader warpgroup's copies: 16 bytes a thread and pass.
+    static constexpr int kChunks = D * kElem / 16;
+    static constexpr int kPassRows = 128 / kChunks;
+    static constexpr int kPasses = kTile / kPassRows;
+    static constexpr int kHold = kPasses < 8 ? kPasses : 8;  // words of a thread's part of a tile: all or half
+    static constexpr int kParts = kPasses / kHold;
+};
+
+struct Listed {             // a key tile
+    float4 group[kGroups];  // e4m3: K's scale, log2 of V's, 1 / V's, what P shrinks by
+    int id[kGroups];        // pages; -1: missing, outside the pool, or not shown
+    int key0;               // first position; -1: the list's end
+    int kvh;
+    int first, last;        // what is shown: [first, last] and what is before the sinks
+    uint32_t gone;          // bits of groups that are shown and have no page
+    uint32_t shrinks;       // of groups whose P shrinks
+    int mixed;              // rows may differ in what they see
+};
+
+struct Shared {
+    Listed list[kListed];
+    uint64_t list_full[kListed], list_empty[kListed];
+    uint64_t k_full[3], k_empty[3], v_full[kVStages], v_empty[kVStages];
+    uint64_t s_full[2], p_full[2];
+    uint64_t q_full, q_empty, done, o_free, ml_full, mma_idle;
+    long long warp_sum[kWarps];
+    long long found_base;
+    int found;
+    uint32_t tmem_base;
+    int abort;
+    int odd;
+};
+
+template <class C>
+constexpr int smem_bytes() {
+    return C::kSmemShared + static_cast<int>(sizeof(Shared)) + 1024;  // the tiles begin on 1024 bytes
+}
 
 template <bool BF16>
 __device__ __forceinline__ float widen16(uint16_t x) {
@@ -46,7 +126,7 @@ __device__ __forceinline__ Drafted drafted(const FaCache& c, int b) {
 }
 
 // One row on its own: warps take its visible keys in turn, lanes the dims. What it does not see is not looked at.
-constexpr int kRowWarps = 4;
+constexpr int kRowWarps = 8;
 
 template <int D, bool BF16, bool E4M3>
 __device__ __forceinline__ void attend_row(const FaTreeParams& p, DeviceStatus* status, int b, int h, int t) {
@@ -185,42 +265,1155 @@ __device__ __forceinline__ void attend_row(const FaTreeParams& p, DeviceStatus* 
     }
 }
 
-template <int D, bool BF16, bool E4M3>
-__global__ void __launch_bounds__(kRowWarps * 32) tree_row_kernel(const __grid_constant__ FaTreeParams p, DeviceStatus* status) {
-    const long long row = blockIdx.x;
-    const int t = static_cast<int>(row % p.cache.tokens);
-    const long long head = row / p.cache.tokens;
-    attend_row<D, BF16, E4M3>(p, status, static_cast<int>(head / p.heads), static_cast<int>(head % p.heads), t);
+// What a sequence shows its nodes, as a list of key tiles: those of the sinks, then from the earliest window (that of a
+// node on the context) to the last token that the table has.
+struct Sequence : Drafted {
+    int first, last;  // positions; last is -1 if there is none
+    int sink_tiles, first_tile, tiles;
+};
+
+__device__ __forceinline__ Sequence sequence(const FaTreeParams& p, int b) {
+    Sequence s;
+    static_cast<Drafted&>(s) = drafted(p.cache, b);
+    const int limit = held(p.cache);
+    s.first = min(window_first(max(s.context, 0), p.window), limit);
+    s.last = s.count > 0 ? min(s.context + s.count, limit) - 1 : -1;
+    s.first_tile = s.first / kTile;
+    s.sink_tiles = min((min(p.sinks, s.first) + kTile - 1) / kTile, s.first_tile);
+    // A sequence that shows nothing keeps one (hidden) tile, so that its rows are written.
+    s.tiles = s.last < 0 ? 1 : max(s.sink_tiles + s.last / kTile - s.first_tile + 1, 1);
+    return s;
+}
+
+__device__ __forceinline__ int tile_key(const Sequence& s, int v) { return (v < s.sink_tiles ? v : v - s.sink_tiles + s.first_tile) * kTile; }
+
+// How a call is cut: items are (sequence, kv head, block of rows), each a list of key tiles. `whole`: an item a CTA. Else
+// the lists are laid end to end and cut into equal ranges, one a CTA; parts of cut items go to records, which a second
+// kernel joins.
+struct Split {
+    int whole;
+    int grid;
+    int row_blocks;
+    int items;  // of a sequence
+};
+
+struct Record {
+    float* o;    // [2 grid][rows of an item][D]
+    float2* ml;  // [2 grid][rows of an item]
+    int* odd;    // [grid]: values that are not finite where some rows do not see them
+};
+
+struct Range {
+    long long total, per;  // key tiles of all items, of a CTA
+    long long found_base;  // start of the sequence found
+    int found;             // -1: beyond the end
+};
+
+// The work list's length, and the sequence that holds unit `at(per)` of it. All threads of a CTA of WARPS warps call.
+template <int WARPS, class At>
+__device__ __forceinline__ Range locate(const FaTreeParams& p, const Split& split, long long* warp_sum, long long* found_base,
+                                        int* found, At at) {
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    const int warp = static_cast<int>(threadIdx.x) / 32;
+    const int share = (p.cache.batch + WARPS * 32 - 1) / (WARPS * 32);
+    const int b0 = min(static_cast<int>(threadIdx.x) * share, p.cache.batch);
+    const int b1 = min(b0 + share, p.cache.batch);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) {
+        mine += sequence(p, b).tiles;
+    }
+    mine *= split.items;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+        incl += lane >= o ? up : 0;
+    }
+    if (lane == 31) {
+        warp_sum[warp] = incl;
+    }
+    if (threadIdx.x == 0) {
+        *found = -1;
+    }
+    __syncthreads();
+    Range r;
+    r.total = 0;
+    long long before = incl - mine;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        before += w < warp ? warp_sum[w] : 0;
+        r.total += warp_sum[w];
+    }
+    r.per = (r.total + split.grid - 1) / split.grid;
+    const long long target = at(r.per);
+    if (target >= before && target < before + mine) {
+        long long base = before;
+        for (int b = b0; b < b1; ++b) {
+            const long long n = static_cast<long long>(sequence(p, b).tiles) * split.items;
+            if (target < base + n) {
+                *found = b;
+                *found_base = base;
+                break;
+            }
+            base += n;
+        }
+    }
+    __syncthreads();
+    r.found = *found;
+    r.found_base = *found_base;
+    return r;
+}
+
+// A CTA's range as pieces of items, in order. Every role walks it on its own.
+struct Walk {
+    Sequence s;
+    int b, item, v;
+    long long left;    // units from here on
+    int record;        // of the next cut piece
+};
+
+struct Piece {
+    int b, kvh, block, v0, v1;
+    int record;  // -1: a whole item
+};
+
+__device__ __forceinline__ Walk start_walk(const FaTreeParams& p, const Split& split, const Range& range, int cta) {
+    Walk w;
+    if (split.whole) {
+        w.b = cta / split.items;
+        w.item = cta - w.b * split.items;
+        w.v = 0;
+        w.s = sequence(p, w.b);
+        w.left = w.s.tiles;
+    } else if (range.found < 0) {
+        w.b = w.item = w.v = 0;
+        w.left = 0;
+        w.s = Sequence{};
+    } else {
+        const long long at = cta * range.per;
+        w.b = range.found;
+        w.s = sequence(p, w.b);
+        const long long in_seq = at - range.found_base;
+        w.item = static_cast<int>(in_seq / w.s.tiles);
+        w.v = static_cast<int>(in_seq - static_cast<long long>(w.item) * w.s.tiles);
+        w.left = min(range.per, range.total - at);
+    }
+    w.record = 2 * cta;
+    return w;
+}
+
+// The piece at hand; `s` is its sequence. False at the end.
+__device__ __forceinline__ bool next_piece(const FaTreeParams& p, const Split& split, Walk& w, Piece& piece, Sequence& s) {
+    if (w.left <= 0) {
+        return false;
+    }
+    s = w.s;
+    piece.b = w.b;
+    piece.kvh = w.item / split.row_blocks;
+    piece.block = w.item - piece.kvh * split.row_blocks;
+    piece.v0 = w.v;
+    const int take = static_cast<int>(min(static_cast<long long>(s.tiles - w.v), w.left));
+    piece.v1 = w.v + take;
+    piece.record = w.v == 0 && take == s.tiles ? -1 : w.record;
+    w.record = 2 * static_cast<int>(blockIdx.x) + 1;  // a range has a cut piece at its start and at its end
+    w.left -= take;
+    w.v = 0;
+    if (w.left > 0 && ++w.item == split.items) {
+        w.item = 0;
+        w.s = sequence(p, ++w.b);
+    }
+    return true;
+}
+
+// Nonzero if a word of cache elements holds one that is not finite.
+template <class C>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    if constexpr (C::E4M3) {
+        return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // e4m3 has NaN (all ones) and no infinity
+    } else if constexpr (C::BF16) {
+        return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+    } else {
+        return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+    }
+}
+
+// Two e4m3 pairs of a word, widened exactly.
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+}
+
+// Byte offset of 16-byte chunk `c` (8 dims) of row `r` in a tile of 64-dim boxes with the 128-byte swizzle.
+__device__ __forceinline__ uint32_t tile_offset(int r, int c) {
+    return static_cast<uint32_t>((c >> 3) * kBox + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+__device__ __forceinline__ void store_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// The range's key tiles, listed for the loaders and the softmax: every third by this warp, so that the loads of pages and
+// scales of three tiles wait for each other's time alone.
+template <class C>
+__device__ __forceinline__ void list_tiles(const FaTreeParams& p, const Split& split, DeviceStatus* status, Walk walk, Shared& sh,
+                                           int which, const WaitCtx& wctx) {
+    const FaCache& c = p.cache;
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    const int log2_page = 31 - __clz(c.page_size);
+    Piece piece;
+    Sequence s;
+    bool more = next_piece(p, split, walk, piece, s);
+    int v = more ? piece.v0 : 0;
+    int skip = which;
+    for (int n = which;; n += kListWarps) {
+        for (; skip > 0 && more; --skip) {
+            if (++v == piece.v1) {
+                more = next_piece(p, split, walk, piece, s);
+                v = more ? piece.v0 : 0;
+            }
+        }
+        if (skip > 0) {
+            return;  // the end is another warp's
+        }
+        skip = kListWarps;
+        Listed& to = sh.list[n % kListed];
+        const bool ok = mbar_wait(smem_u32(&sh.list_empty[n % kListed]), ((n / kListed) & 1) ^ 1, wctx, kStatusTimeoutProducer);
+        if (__all_sync(0xffffffffu, ok) == 0) {
+            return;
+        }
+        int id = -1;
+        if (more) {
+            const int key0 = tile_key(s, v);
+            const int key = key0 + 8 * (lane % kGroups);
+            const bool shown = key >= 0 && key <= s.last && (key + 7 >= s.first || key < p.sinks);
+            if (shown) {
+                id = __ldg(c.page_table + piece.b * c.table_stride + (key >> log2_page));
+                if (id < 0 || id >= c.num_pages) {
+                    id = -1;
+                    atomicOr(&status->code, kStatusBadPage);
+                }
+            }
+            bool shrinks = false;
+            if constexpr (C::E4M3) {
+                float ks = 1.0f, vs = 1.0f;
+                if (id >= 0) {
+                    const int64_t at = static_cast<int64_t>(id) * c.kv_heads + piece.kvh;
+                    ks = __ldg(c.k_scale + at);
+                    vs = __ldg(c.v_scale + at);
+                }
+                const float used = fmaxf(vs, kMinScale);
+                const float inv = __fdividef(1.0f, used);
+                shrinks = vs < kMinScale;
+                if (lane < kGroups) {
+                    to.group[lane] = make_float4(ks, __log2f(used), inv, shrinks ? vs * inv : 1.0f);
+                }
+            }
+            const uint32_t gone = __ballot_sync(0xffffffffu, shown && id < 0 && lane < kGroups);
+            const uint32_t shrink = __ballot_sync(0xffffffffu, shrinks && lane < kGroups);
+            if (lane < kGroups) {
+                to.id[lane] = id;
+            }
+            if (lane == 0) {
+                to.key0 = key0;
+                to.kvh = piece.kvh;
+                to.first = s.first;
+                to.last = s.last;
+                to.gone = gone;
+                to.shrinks = shrink;
+                to.mixed = c.tokens > 1 && (key0 + kTile > s.context || (p.window > 0 && key0 < window_first(max(s.context, 0) + s.count, p.window)));
+            }
+        } else if (lane == 0) {
+            to.key0 = -1;
+        }
+        __syncwarp();
+        if (lane == 0) {
+            mbar_arrive(smem_u32(&sh.list_full[n % kListed]));
+        }
+        if (!more) {
+            return;
+        }
+    }
+}
+
+// One warpgroup brings K or V, tile after tile: 16-byte words of the cache's rows, two parts of words per thread in
+// flight while it widens (e4m3) and stores what has come.
+template <class C, bool IS_V>
+__device__ __forceinline__ void load_tiles(const FaTreeParams& p, Shared& sh, uint32_t ring, const WaitCtx& wctx) {
+    constexpr int kStages = IS_V ? kVStages : C::kKStages;
+    const FaCache& c = p.cache;
+    const int lt = static_cast<int>(threadIdx.x) % 128;
+    const int lane = lt % 32;
+    const int chunk = lt % C::kChunks;
+    const int r0 = lt / C::kChunks;
+    const uint8_t* base = static_cast<const uint8_t*>(IS_V ? c.v : c.k) + chunk * 16;
+    const int64_t page_bytes = (IS_V ? c.v_stride[0] : c.k_stride[0]) * C::kElem;
+    const int64_t head_bytes = (IS_V ? c.v_stride[1] : c.k_stride[1]) * C::kElem;
+    uint64_t* full = IS_V ? sh.v_full : sh.k_full;
+    uint64_t* empty = IS_V ? sh.v_empty : sh.k_empty;
+    const int in_page = c.page_size - 1;
+    bool odd = false;
+
+    // Part `u` of the list is asked for; 0: there is none, 1: it comes, 3: and rows may differ in what they see of it.
+    auto ask = [&](int u, uint4 (&word)[C::kHold]) {
+        const int n = u / C::kParts;
+        const bool ok = mbar_wait(smem_u32(&sh.list_full[n % kListed]), (n / kListed) & 1, wctx, kStatusTimeoutProducer);
+        if (__all_sync(0xffffffffu, ok) == 0) {
+            return 0;
+        }
+        const Listed& t = sh.list[n % kListed];
+        const int key0 = t.key0;
+        if (key0 < 0) {
+            return 0;
+        }
+        const uint8_t* head = base + t.kvh * head_bytes;
+        const int first = t.first;
+        const int last = t.last;
+#pragma unroll
+        for (int i = 0; i < C::kHold; ++i) {
+            const int r = ((u % C::kParts) * C::kHold + i) * C::kPassRows + r0;
+            const int id = t.id[r >> 3];
+            const int key = key0 + r;
+            // Zeros for what no row of the call sees.
+            const bool shown = id >= 0 && key <= last && (key >= first || key < p.sinks);
+            word[i] = shown ? __ldg(reinterpret_cast<const uint4*>(head + id * page_bytes + (key & in_page) * (C::D * C::kElem)))
+                            : make_uint4(0u, 0u, 0u, 0u);
+        }
+        const int mixed = t.mixed;
+        if (u % C::kParts == C::kParts - 1) {
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(smem_u32(&sh.list_empty[n % kListed]));
+            }
+        }
+        return mixed != 0 ? 3 : 1;
+    };
+    auto bring = [&](int u, const uint4 (&word)[C::kHold], int kind) {
+        const int n = u / C::kParts;
+        const int slot = n % kStages;
+        const bool ok = u % C::kParts > 0 || mbar_wait(smem_u32(&empty[slot]), ((n / kStages) & 1) ^ 1, wctx, kStatusTimeoutProducer);
+        if (__all_sync(0xffffffffu, ok) == 0) {
+            return false;
+        }
+        const uint32_t tile = ring + slot * C::kTileBytes;
+#pragma unroll
+        for (int i = 0; i < C::kHold; ++i) {
+            const int r = ((u % C::kParts) * C::kHold + i) * C::kPassRows + r0;
+            const uint4 w = word[i];
+            if (IS_V && kind == 3) {
+                odd = odd || (not_finite<C>(w.x) | not_finite<C>(w.y) | not_finite<C>(w.z) | not_finite<C>(w.w)) != 0;
+            }
+            if constexpr (C::E4M3) {
+                uint32_t h[8];
+                widen4(w.x, h[0], h[1]);
+                widen4(w.y, h[2], h[3]);
+                widen4(w.z, h[4], h[5]);
+                widen4(w.w, h[6], h[7]);
+                // Lanes of the second box go the other way round, against bank conflicts.
+                const bool swap = (chunk & 4) != 0;
+                store_shared16(tile + tile_offset(r, 2 * chunk + (swap ? 1 : 0)), swap ? h[4] : h[0], swap ? h[5] : h[1],
+                               swap ? h[6] : h[2], swap ? h[7] : h[3]);
+                store_shared16(tile + tile_offset(r, 2 * chunk + (swap ? 0 : 1)), swap ? h[0] : h[4], swap ? h[1] : h[5],
+                               swap ? h[2] : h[6], swap ? h[3] : h[7]);
+            } else {
+                store_shared16(tile + tile_offset(r, chunk), w.x, w.y, w.z, w.w);
+            }
+        }
+        if (u % C::kParts == C::kParts - 1) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(smem_u32(&full[slot]));
+            }
+        }
+        return true;
+    };
+
+    uint4 a[C::kHold], b[C::kHold];
+    int kind_a = ask(0, a);
+    int kind_b = kind_a != 0 ? ask(1, b) : 0;
+    for (int u = 0; kind_a != 0; u += 2) {
+        if (!bring(u, a, kind_a)) {
+            break;
+        }
+        kind_a = kind_b != 0 ? ask(u + 2, a) : 0;
+        if (kind_b == 0 || !bring(u + 1, b, kind_b)) {
+            break;
+        }
+        kind_b = kind_a != 0 ? ask(u + 3, b) : 0;
+    }
+    if (IS_V && odd) {
+        sh.odd = 1;
+    }
+}
+
+template <class C>
+__device__ __forceinline__ void issue_scores(uint32_t d, uint64_t a, uint64_t b) {
+    constexpr uint32_t idesc = make_idesc_f16(kTile, kTile, true, false, C::kMmaBf16);
+#pragma unroll
+    for (int k = 0; k < C::D / 16; ++k) {
+        const uint64_t off = static_cast<uint64_t>(((k / 4) * kBox + (k % 4) * 32) >> 4);
+        umma_ss(d, a + off, b + off, idesc, k > 0 ? 1u : 0u);
+    }
+}
+
+template <class C>
+__device__ __forceinline__ void issue_product(uint32_t acc, uint32_t w, uint64_t t, bool first) {
+    constexpr uint32_t idesc = make_idesc_f16(kTile, C::D, true, true, C::kMmaBf16);
+#pragma unroll
+    for (int k = 0; k < kTile / 16; ++k) {
+        umma_ts(acc, w + k * 8, t + static_cast<uint64_t>(k * (2048 >> 4)), idesc, (first && k == 0) ? 0u : 1u);
+    }
+}
+
+// Products, in the order in which scores and P take each other's place: S(s + 2) after P(s) V. Step s is key tile s (NR 1)
+// or row tile s % 2 of key tile s / 2 (NR 2).
+template <class C>
+__device__ __forceinline__ void issue_products(const FaTreeParams& p, const Split& split, Walk walk, Shared& sh, uint32_t smem,
+                                               const WaitCtx& wctx) {
+    constexpr int NR = C::NR;
+    const uint64_t q = make_desc_kmajor_sw128(smem + C::kSmemQ);
+    const uint64_t k = make_desc_kmajor_sw128(smem + C::kSmemK);
+    const uint64_t v = make_desc_mnmajor_sw128(smem + C::kSmemV, kBox);
+    auto off = [](int tile) { return static_cast<uint64_t>(tile * (C::kTileBytes >> 4)); };
+    auto wait = [&](uint64_t* bar, int parity) {
+        const bool there = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity & 1, wctx, kStatusTimeoutMma)) != 0;
+        tc_fence_after();
+        return there;
+    };
+    bool ok = true;
+    int tiles = 0;  // key tiles of the pieces before
+    int taken[2] = {0, 0};
+    Piece piece;
+    Sequence s;
+    for (int items = 0; ok && next_piece(p, split, walk, piece, s); ++items) {
+        const int n = piece.v1 - piece.v0;
+        const int steps = n * NR;
+        auto scores = [&](int step) {
+            const int tile = tiles + (NR == 1 ? step : step >> 1);
+            const int w = step & 1;
+            if (NR == 1 || w == 0) {
+                ok = wait(&sh.k_full[tile % C::kKStages], tile / C::kKStages);
+            }
+            if (ok) {
+                if (elect_one()) {
+                    issue_scores<C>(C::kTmemS + w * kTile, q + off(NR == 1 ? 0 : w), k + off(tile % C::kKStages));
+                    umma_commit(smem_u32(&sh.s_full[w]));
+                    if (NR == 1 || w == 1) {
+                        umma_commit(smem_u32(&sh.k_empty[tile % C::kKStages]));
+                    }
+                    if (step == steps - 1) {
+                        umma_commit(smem_u32(&sh.q_empty));
+                    }
+                }
+                __syncwarp();
+            }
+        };
+        ok = wait(&sh.q_full, items);
+        if (ok) {
+            scores(0);
+        }
+        if (ok && steps > 1) {
+            scores(1);
+        }
+        if (ok && items > 0) {
+            ok = wait(&sh.o_free, items - 1);
+        }
+        for (int step = 0; ok && step < steps; ++step) {
+            const int tile = tiles + (NR == 1 ? step : step >> 1);
+            const int w = step & 1;
+            if (NR == 1 || w == 0) {
+                ok = wait(&sh.v_full[tile % kVStages], tile / kVStages);
+            }
+            ok = ok && wait(&sh.p_full[w], taken[w]++);
+            if (!ok) {
+                break;
+            }
+            if (elect_one()) {
+                issue_product<C>(C::kTmemO + w * C::D, C::kTmemS + w * kTile, v + off(tile % kVStages), step < 2);
+                if (NR == 1 || w == 1) {
+                    umma_commit(smem_u32(&sh.v_empty[tile % kVStages]));
+                }
+                if (step == steps - 1) {
+                    umma_commit(smem_u32(&sh.done));
+                }
+            }
+            __syncwarp();
+            if (step + 2 < steps) {
+                scores(step + 2);
+            }
+        }
+        tiles += n;
+    }
+    // Every product issued must be complete before tensor memory is released.
+    if (elect_one()) {
+        umma_commit(smem_u32(&sh.mma_idle));
+    }
+    __syncwarp();
+    mbar_wait_drain(smem_u32(&sh.mma_idle), 0, wctx, kStatusTimeoutTeardown);
+    __syncwarp();
+}
+
+// A thread's query row.
+struct Row {
+    bool real;          // a node's (else padding, or beyond the rows)
+    int head, token;    // head of the group
+    uint32_t mask[kMaskWords];  // the node and its ancestors
+    int first;          // first position of its window
+    float factor;       // of a score, in log2 units
+};
+
+// The words of one row that are its own to bring (WORDS 16-byte words from word `from`), into Q's tile; and what
+// bfloat16 queries over an e4m3 cache are scaled down by. See the cached kernel: the largest of a row goes to [2^13, 2^14).
+template <class C>
+__device__ __forceinline__ void bring_query(const FaTreeParams& p, Row& row, int b, int head, uint32_t tile, int r, int from, int words) {
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] +
+                                                      head * p.q_stride[1] + row.token * p.q_stride[2]);
+    const uint32_t sign = p.softmax_scale < 0.0f ? 0x80008000u : 0u;  // the factor stays positive
+    row.factor = fmaxf(fabsf(p.softmax_scale) * kLog2e, kLeastFactor);
+    float up = 1.0f;
+    if constexpr (C::E4M3 && C::BF16) {
+        uint32_t top = 0;  // of the values' bits without sign: their order is that of the sizes
+        if (row.real) {
+#pragma unroll 4
+            for (int i = 0; i < C::D / 8; ++i) {
+                const uint4 w = __ldg(src + i);
+                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    top = max(top, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
+                }
+            }
+        }
+        // 2^(13 - exponent of the largest), both it and its inverse normal; 1 for zeros, inf and NaN.
+        const int e = static_cast<int>(top >> 7);
+        const int shift = (e == 0 || e == 255) ? 0 : min(max(140 - e, -100), 100);
+        up = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+        row.factor = fmaxf(row.factor * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23), kLeastFactor);
+    }
+#pragma unroll 4
+    for (int i = from; i < from + words; ++i) {
+        const uint4 w = row.real ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+        uint32_t x[4] = {w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign};
+        if constexpr (C::E4M3 && C::BF16) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = pack_half2(__uint_as_float(x[e] << 16) * up, __uint_as_float(x[e] & 0xFFFF0000u) * up);
+            }
+        }
+        store_shared16(tile + tile_offset(r, i), x[0], x[1], x[2], x[3]);
+    }
+}
+
+// 32 columns of scores, keys from kb on: those that the row does not see become -inf.
+template <class C>
+__device__ __forceinline__ uint32_t kept_columns(const FaTreeParams& p, const Sequence& s, const Row& row, int kb, uint32_t gone) {
+    if (!row.real) {
+        return 0;
+    }
+    uint32_t keep = bits_up_to(min(s.context - 1, s.last) - kb);
+    if (p.window > 0) {
+        keep &= ~bits_up_to(row.first - 1 - kb) | bits_up_to(p.sinks - 1 - kb);
+    }
+    const int node = kb - s.context;  // of the first column
+    if (node > -32 && node < kMostNodes) {
+        const int word = node >> 5;
+        uint32_t lo = 0, hi = 0;
+#pragma unroll
+        for (int i = 0; i < kMaskWords; ++i) {
+            lo = i == word ? row.mask[i] : lo;
+            hi = i == word + 1 ? row.mask[i] : hi;
+        }
+        keep |= __funnelshift_r(lo, hi, node & 31) & bits_up_to(s.last - kb);
+    }
+    // 4 groups of 8 keys.
+    const uint32_t pages = ~gone;
+    keep &= ((pages & 1u) * 0xffu) | (((pages >> 1) & 1u) * 0xff00u) | (((pages >> 2) & 1u) * 0xff0000u) | (((pages >> 3) & 1u) * 0xff000000u);
+    return keep;
+}
+
+template <class C>
+__device__ __forceinline__ void softmax(const FaTreeParams& p, const Split& split, DeviceStatus* status, Walk walk, Shared& sh,
+                                        uint32_t smem, const Record& rec, const WaitCtx& wctx) {
+    constexpr int D = C::D;
+    constexpr int NR = C::NR;
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    const int warp = static_cast<int>(threadIdx.x) / 32;
+    const int w = warp / 4;                  // warpgroup
+    const int r = (warp % 4) * 32 + lane;    // row of its tile
+    const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
+    const uint32_t tmem_s = lanes + C::kTmemS + w * kTile;
+    const uint32_t tmem_o = lanes + C::kTmemO + w * D;
+    const int group = p.heads / p.cache.kv_heads;
+    const int rows = group * p.cache.tokens;
+    auto wait = [&](uint64_t* bar, int parity) {
+        const bool there = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity & 1, wctx, kStatusTimeoutSoftmax)) != 0;
+        tc_fence_after();
+        return there;
+    };
+    auto arrive = [&](uint64_t* bar) {
+        __syncwarp();
+        if (lane == 0) {
+            mbar_arrive(smem_u32(bar));
+        }
+    };
+    int tiles = 0;   // key tiles of the pieces before
+    int steps = 0;   // scores taken
+    Piece piece;
+    Sequence s;
+    for (int items = 0; next_piece(p, split, walk, piece, s); ++items) {
+        const int n = piece.v1 - piece.v0;
+        const int row_index = piece.block * C::kRows + (NR == 2 ? w * kTile : 0) + r;
+        Row row;
+        row.head = row_index / p.cache.tokens;
+        row.token = row_index - row.head * p.cache.tokens;
+        row.real = row_index < rows && row.token < s.count;
+        const int head = piece.kvh * group + row.head;
+        if (items > 0 && !wait(&sh.q_empty, items - 1)) {
+            return;
+        }
+        constexpr int kWords = D / 8 / (NR == 1 ? 2 : 1);
+        bring_query<C>(p, row, piece.b, head, smem + C::kSmemQ + (NR == 2 ? w * C::kTileBytes : 0), r, NR == 1 ? w * kWords : 0, kWords);
+        fence_proxy_async_smem();
+        arrive(&sh.q_full);
+        // The way up from the row's node.
+        int depth = 0;
+#pragma unroll
+        for (int i = 0; i < kMaskWords; ++i) {
+            row.mask[i] = 0;
+        }
+        if (row.real) {
+            const int32_t* parents = p.parents + piece.b * p.parent_stride;
+            int at = row.token;
+            bool bad = false;
+#pragma unroll
+            for (int i = kMaskWords - 1; i >= 0; --i) {
+                while (at >= 32 * i) {
+                    row.mask[i] |= 1u << (at & 31);
+                    ++depth;
+                    const int up = __ldg(parents + at);
+                    bad = bad || up < -1 || up >= at;
+                    at = up < -1 || up >= at ? -1 : up;
+                }
+            }
+            if (bad || s.context < 0 || s.context > held(p.cache) - s.count) {
+                atomicOr(&status->code, kStatusBadPage);
+            }
+        }
+        row.first = window_first(max(s.context + depth - 1, 0), p.window);
+
+        float m = -INFINITY, l = 0.0f;
+        int mine = 0;  // scores of this piece taken
+        for (int t = NR == 1 ? w : 0; t < n; t += NR == 1 ? 2 : 1, ++mine) {
+            const int key0 = tile_key(s, piece.v0 + t);
+            const int slot = (tiles + t) % kListed;
+            if (!wait(&sh.list_full[slot], (tiles + t) / kListed) || !wait(&sh.s_full[w], steps)) {
+                return;
+            }
+            ++steps;
+            const Listed& aux = sh.list[slot];
+            const uint32_t gone = aux.gone;
+            // Whether all rows see all of the tile.
+            const bool full = gone == 0 && key0 + kTile <= min(s.context, s.last + 1) &&
+                              (p.window == 0 || key0 >= window_first(max(s.context, 0) + s.count, p.window) || key0 + kTile <= p.sinks);
+            float top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t x[32];
+                tmem_ld32(tmem_s + 32 * c, x);
+                tmem_wait_ld();
+                if (!full) {
+                    const uint32_t keep = kept_columns<C>(p, s, row, key0 + 32 * c, gone >> (4 * c));
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        x[i] = (keep >> i) & 1u ? x[i] : 0xff800000u;
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    float most = fmax_nan(u2f(x[8 * g]), u2f(x[8 * g + 1]));
+                    most = fmax3(most, u2f(x[8 * g + 2]), u2f(x[8 * g + 3]));
+                    most = fmax3(most, u2f(x[8 * g + 4]), u2f(x[8 * g + 5]));
+                    most = fmax3(most, u2f(x[8 * g + 6]), u2f(x[8 * g + 7]));
+                    if constexpr (C::E4M3) {
+                        const float4 a = aux.group[4 * c + g];
+                        most = fmaf(most, fmaxf(row.factor * a.x, kLeastFactor), a.y);
+                    }
+                    top = fmax_nan(top, most);
+                }
+            }
+            if constexpr (!C::E4M3) {
+                top *= row.factor;
+            }
+            float alpha = 1.0f;
+            if (!(top <= m + kLazy)) {  // NaN among it
+                alpha = ex2_approx(m - top);
+                m = top;
+            }
+            if (mine > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+                l *= alpha;
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t x[32];
+                    tmem_ld32(tmem_o + 32 * c, x);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        x[i] = f2u(u2f(x[i]) * alpha);
+                    }
+                    tmem_st32(tmem_o + 32 * c, x);
+                }
+                tmem_wait_st();
+            }
+            const float used = m == -INFINITY ? 0.0f : m;
+            const bool shrinks = C::E4M3 && aux.shrinks != 0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t x[32];
+                tmem_ld32(tmem_s + 32 * c, x);
+                tmem_wait_ld();
+                if (!full) {
+                    const uint32_t keep = kept_columns<C>(p, s, row, key0 + 32 * c, gone >> (4 * c));
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        x[i] = (keep >> i) & 1u ? x[i] : 0xff800000u;
+                    }
+                }
+                uint32_t packed[16];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    float f = row.factor, add = -used, inv = 1.0f, shrink = 1.0f;
+                    if constexpr (C::E4M3) {
+                        const float4 a = aux.group[4 * c + g];
+                        f = fmaxf(f * a.x, kLeastFactor);
+                        add = a.y - used;
+                        inv = a.z;
+                        shrink = a.w;
+                    }
+                    float y[8];
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        y[i] = ex2_approx(fmaf(u2f(x[8 * g + i]), f, add));
+                        sum += y[i];
+                    }
+                    l = fmaf(sum, inv, l);
+                    if (shrinks) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            y[i] *= shrink;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        packed[4 * g + i] = pack2<C::kMmaBf16>(y[2 * i], y[2 * i + 1]);
+                    }
+                }
+                tmem_st16(tmem_s + 16 * c, packed);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            arrive(&sh.p_full[w]);
+            arrive(&sh.list_empty[slot]);
+        }
+        tiles += n;
+
+        // The end of the piece: rows of both warpgroups joined (NR 1), normalised or left in a record.
+        if (!wait(&sh.done, items)) {
+            return;
+        }
+        float weight[2] = {1.0f, 0.0f};
+        float other_m = -INFINITY, other_l = 0.0f;
+        if constexpr (NR == 1) {
+            // Each tells the other its maximum and sum through its scores' columns, which are free.
+            uint32_t mine2[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                mine2[i] = 0;
+            }
+            mine2[0] = f2u(m);
+            mine2[1] = f2u(l);
+            tmem_st16(tmem_s, mine2);
+            tmem_wait_st();
+            tc_fence_before();
+            arrive(&sh.ml_full);
+            if (!wait(&sh.ml_full, items)) {
+                return;
+            }
+            uint32_t theirs[16];
+            tmem_ld16(lanes + C::kTmemS + (1 - w) * kTile, theirs);
+            tmem_wait_ld();
+            other_m = u2f(theirs[0]);
+            other_l = u2f(theirs[1]);
+            const float all = fmax_nan(m, other_m);
+            const float base = all == -INFINITY ? 0.0f : all;
+            weight[0] = ex2_approx(m - base);
+            weight[1] = ex2_approx(other_m - base);
+            l = l * weight[0] + other_l * weight[1];
+            m = all;
+        }
+        constexpr int kColumns = NR == 1 ? D / 2 : D;  // of this thread
+        const int column0 = NR == 1 ? w * kColumns : 0;
+        const uint32_t own = tmem_o + column0;
+        const uint32_t theirs = lanes + C::kTmemO + (1 - w) * D + column0;
+        const bool both = NR == 1 && n > 1;           // the other sum exists
+        const bool self = NR == 2 || w == 0 || n > 1;  // this one does
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const bool in_rows = row_index < rows;
+        const int64_t out_row = (static_cast<int64_t>(piece.b) * p.heads + head) * p.cache.tokens + row.token;
+        const int64_t record_row = static_cast<int64_t>(piece.record) * C::kRows + (NR == 2 ? w * kTile : 0) + r;
+#pragma unroll 1
+        for (int c = 0; c < kColumns / 16; ++c) {
+            uint32_t x[16], y[16];
+            if (self) {
+                tmem_ld16(own + 16 * c, x);
+            }
+            if (NR == 1 && (both || !self)) {
+                tmem_ld16(theirs + 16 * c, y);
+            }
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float z = self ? u2f(x[i]) * weight[0] : 0.0f;
+                if (NR == 1 && (both || !self)) {
+                    z = fmaf(u2f(y[i]), weight[1], z);
+                }
+                x[i] = row.real ? f2u(z) : 0u;
+            }
+            if (!in_rows) {
+                continue;
+            }
+            if (piece.record < 0) {
+                uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + out_row * D + column0 + 16 * c);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    to[i] = make_uint4(pack2<C::BF16>(u2f(x[8 * i]) * inv, u2f(x[8 * i + 1]) * inv),
+                                       pack2<C::BF16>(u2f(x[8 * i + 2]) * inv, u2f(x[8 * i + 3]) * inv),
+                                       pack2<C::BF16>(u2f(x[8 * i + 4]) * inv, u2f(x[8 * i + 5]) * inv),
+                                       pack2<C::BF16>(u2f(x[8 * i + 6]) * inv, u2f(x[8 * i + 7]) * inv));
+                }
+            } else {
+                uint4* to = reinterpret_cast<uint4*>(rec.o + record_row * D + column0 + 16 * c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    to[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                }
+            }
+        }
+        if (piece.record >= 0 && in_rows && (NR == 2 || w == 0)) {
+            rec.ml[record_row] = row.real ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
+        }
+        tc_fence_before();
+        arrive(&sh.o_free);
+    }
+}
+
+template <class C>
+__global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ FaTreeParams p, DeviceStatus* status, unsigned epoch,
+                                                           Split split, Record rec) {
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    Shared& sh = *reinterpret_cast<Shared*>(smem + C::kSmemShared);
+    const int warp = static_cast<int>(threadIdx.x) / 32;
+    const WaitCtx wctx{&sh.abort, &status->code, &status->epoch_aborted, epoch};
+    cudaTriggerProgrammaticLaunchCompletion();  // the second kernel's CTAs may take SMs as they get free
+    if (threadIdx.x == 0) {
+        sh.abort = 0;
+        sh.odd = 0;
+        for (int i = 0; i < C::kKStages; ++i) {
+            mbar_init(smem_u32(&sh.k_full[i]), kLoadWarps / 2);
+            mbar_init(smem_u32(&sh.k_empty[i]), 1);
+        }
+        for (int i = 0; i < kVStages; ++i) {
+            mbar_init(smem_u32(&sh.v_full[i]), kLoadWarps / 2);
+            mbar_init(smem_u32(&sh.v_empty[i]), 1);
+        }
+        for (int i = 0; i < kListed; ++i) {
+            mbar_init(smem_u32(&sh.list_full[i]), 1);
+            mbar_init(smem_u32(&sh.list_empty[i]), kLoadWarps + C::NR * kSoftmaxWarps / 2);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&sh.s_full[i]), 1);
+            mbar_init(smem_u32(&sh.p_full[i]), kSoftmaxWarps / 2);
+        }
+        mbar_init(smem_u32(&sh.q_full), kSoftmaxWarps);
+        mbar_init(smem_u32(&sh.q_empty), 1);
+        mbar_init(smem_u32(&sh.done), 1);
+        mbar_init(smem_u32(&sh.o_free), kSoftmaxWarps);
+        mbar_init(smem_u32(&sh.ml_full), kSoftmaxWarps);
+        mbar_init(smem_u32(&sh.mma_idle), 1);
+        mbar_fence_init();
+    }
+    if (warp == kMmaWarp) {
+        tmem_alloc(smem_u32(&sh.tmem_base), 512);
+        tmem_relinquish();
+    }
+    Range range{};
+    if (!split.whole) {
+        range = locate<kWarps>(p, split, sh.warp_sum, &sh.found_base, &sh.found, [&](long long per) { return blockIdx.x * per; });
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    // Owning all 512 columns means owning them from 0, a constant for the products' operands.
+    if (sh.tmem_base != 0) {
+        if (threadIdx.x == 0) {
+            atomicOr(&status->code, kStatusTimeoutTeardown);
+        }
+    } else {
+        const Walk walk = start_walk(p, split, range, static_cast<int>(blockIdx.x));
+        if (warp < kSoftmaxWarps) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+            softmax<C>(p, split, status, walk, sh, smem_u32(smem), rec, wctx);
+        } else if (warp < kSoftmaxWarps + kLoadWarps / 2) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
+            load_tiles<C, false>(p, sh, smem_u32(smem) + C::kSmemK, wctx);
+        } else if (warp < kMmaWarp) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
+            load_tiles<C, true>(p, sh, smem_u32(smem) + C::kSmemV, wctx);
+        } else {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
+            if (warp == kMmaWarp) {
+                issue_products<C>(p, split, walk, sh, smem_u32(smem), wctx);
+            } else {
+                list_tiles<C>(p, split, status, walk, sh, warp - kListWarp, wctx);
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc(sh.tmem_base, 512);
+    }
+    if (rec.odd != nullptr && threadIdx.x == 0) {
+        rec.odd[blockIdx.x] = sh.odd;
+    }
+}
+
+// The second kernel. Its first CTAs join the records of cut items: CTA k those of the item that was cut at unit (k + 1) per, if
+// that is its first cut, always in the same order; a warp takes a row. The others, `fixers` of them, compute rows anew,
+// one by one, of items in whose tiles infinities or NaN are hidden from some rows (0 times them would be NaN there).
+template <class C>
+__global__ void __launch_bounds__(kRowWarps * 32) tree_finish_kernel(const __grid_constant__ FaTreeParams p, DeviceStatus* status,
+                                                                     Split split, Record rec, int joins, int fixers) {
+    constexpr int D = C::D;
+    constexpr int kPer = D / 32;
+    __shared__ long long warp_sum[kRowWarps];
+    __shared__ long long found_base;
+    __shared__ int found;
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    const int warp = static_cast<int>(threadIdx.x) / 32;
+    const int group = p.heads / p.cache.kv_heads;
+    const int rows = group * p.cache.tokens;
+    // One CTA waits whatever it finds to do, so that this kernel's end stands for the end of the one before.
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+        cudaGridDependencySynchronize();
+    }
+    if (static_cast<int>(blockIdx.x) < joins) {
+        const long long k = blockIdx.x + 1;
+        const Range range = locate<kRowWarps>(p, split, warp_sum, &found_base, &found, [&](long long per) { return k * per; });
+        if (range.found < 0) {
+            return;
+        }
+        const Sequence s = sequence(p, range.found);
+        const long long item = (k * range.per - range.found_base) / s.tiles;
+        const long long start = range.found_base + item * s.tiles;
+        if (start == k * range.per || start / range.per != k - 1) {
+            return;
+        }
+        const int kvh = static_cast<int>(item / split.row_blocks);
+        const int block = static_cast<int>(item - static_cast<long long>(kvh) * split.row_blocks);
+        const int r = static_cast<int>(blockIdx.y) * kRowWarps + warp;
+        const int row_index = block * C::kRows + r;
+        if (row_index - warp >= rows) {
+            return;
+        }
+        const long long c0 = start / range.per;
+        const long long c1 = (start + s.tiles - 1) / range.per;
+        cudaGridDependencySynchronize();  // the records are there
+        if (row_index >= rows) {
+            return;
+        }
+        float m = -INFINITY, l = 0.0f;
+        float o[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            o[i] = 0.0f;
+        }
+        bool odd = false;
+#pragma unroll 4
+        for (long long c = c0; c <= c1; ++c) {
+            // A CTA's first cut piece is its record 0; the item starts in c0, as its second unless there.
+            const long long record = (2 * c + (c * range.per >= start ? 0 : 1)) * C::kRows + r;
+            odd = odd || (rec.odd != nullptr && rec.odd[c] != 0);
+            const float2 ml = rec.ml[record];
+            float y[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                y[i] = rec.o[record * D + lane * kPer + i];
+            }
+            const float now = fmax_nan(m, ml.x);
+            const float used = now == -INFINITY ? 0.0f : now;
+            const float a = ex2_approx(m - used);
+            const float f = ex2_approx(ml.x - used);
+            m = now;
+            l = fmaf(ml.y, f, l * a);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                o[i] = fmaf(y[i], f, o[i] * a);
+            }
+        }
+        if (odd) {
+            return;  // its rows are computed anew
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int head = row_index / p.cache.tokens;
+        const int token = row_index - head * p.cache.tokens;
+        const int64_t out_row = (static_cast<int64_t>(range.found) * p.heads + kvh * group + head) * p.cache.tokens + token;
+#pragma unroll
+        for (int i = 0; i < kPer; i += 2) {
+            reinterpret_cast<uint32_t*>(p.o)[(out_row * D + lane * kPer + i) / 2] = pack2<C::BF16>(o[i] * inv, o[i + 1] * inv);
+        }
+        return;
+    }
+    if (blockIdx.y > 0) {
+        return;
+    }
+    cudaGridDependencySynchronize();
+    const int fixer = static_cast<int>(blockIdx.x) - joins;
+    bool any = false;
+    for (int i = static_cast<int>(threadIdx.x); i < split.grid; i += kRowWarps * 32) {
+        any = any || rec.odd[i] != 0;
+    }
+    if (__syncthreads_or(any) == 0) {
+        return;
+    }
+    for (int cta = 0; cta < split.grid; ++cta) {
+        if (rec.odd[cta] == 0) {
+            continue;
+        }
+        Range range{};
+        if (!split.whole) {
+            range = locate<kRowWarps>(p, split, warp_sum, &found_base, &found, [&](long long per) { return cta * per; });
+        }
+        Walk walk = start_walk(p, split, range, cta);
+        Piece piece;
+        Sequence s;
+        while (next_piece(p, split, walk, piece, s)) {
+            for (int r = fixer; r < C::kRows; r += fixers) {
+                const int row_index = piece.block * C::kRows + r;
+                if (row_index < rows) {
+                    const int head = row_index / p.cache.tokens;
+                    __syncthreads();  // the shared memory of the row before is free
+                    attend_row<D, C::BF16, C::E4M3>(p, status, piece.b, piece.kvh * group + head, row_index - head * p.cache.tokens);
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Launches after the kernel before it has started to end: it waits for its results itself.
+template <class... Params, class... Args>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, const Args&... args) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(static_cast<unsigned>(threads));
+    config.stream = stream;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
+constexpr int kWholeTiles = 8;  // up to this many key tiles in the table's capacity items are not cut
+constexpr int kFixers = 64;
+
+int row_tiles(const FaTreeParams& p) { return p.heads / p.cache.kv_heads * p.cache.tokens > kTile ? 2 : 1; }
+
+// `grid` is 0 for what no grid holds.
+Split split_for(const FaTreeParams& p, int sm_count) {
+    const FaCache& c = p.cache;
+    const long long rows = static_cast<long long>(p.heads / c.kv_heads) * c.tokens;
+    const long long block = static_cast<long long>(row_tiles(p)) * kTile;
+    const long long row_blocks = (rows + block - 1) / block;
+    const long long items = static_cast<long long>(c.kv_heads) * row_blocks;
+    long long shown = static_cast<long long>(c.max_pages) * c.page_size;
+    if (p.window > 0) {
+        shown = std::min<long long>(shown, static_cast<long long>(p.window) + p.sinks + c.tokens + 3 * kTile);
+    }
+    const long long tiles = (shown + kTile - 1) / kTile;
+    Split s;
+    s.row_blocks = static_cast<int>(row_blocks);
+    s.items = static_cast<int>(items);
+    s.whole = tiles <= kWholeTiles && items * c.batch <= sm_count;
+    s.grid = static_cast<int>(s.whole ? items * c.batch : std::min<long long>(sm_count, items * c.batch * tiles));
+    return s;
+}
+
+template <class C>
+cudaError_t launch(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count, cudaStream_t stream) {
+    const Split split = split_for(p, sm_count);
+    constexpr auto kernel = tree_kernel<C>;
+    cudaError_t err = ensure_smem_limit<kernel>(smem_bytes<C>());
+    if (err != cudaSuccess) {
+        return err;
+    }
+    Record rec{};
+    int* odd = static_cast<int*>(workspace);
+    if (!split.whole) {
+        const size_t rows = static_cast<size_t>(split.grid) * 2 * C::kRows;
+        rec.o = static_cast<float*>(workspace);
+        rec.ml = reinterpret_cast<float2*>(rec.o + rows * C::D);
+        odd = reinterpret_cast<int*>(rec.ml + rows);
+    }
+    rec.odd = p.cache.tokens > 1 ? odd : nullptr;
+    kernel<<<static_cast<unsigned>(split.grid), kThreads, smem_bytes<C>(), stream>>>(p, status, epoch, split, rec);
+    err = cudaGetLastError();
+    const int joins = split.whole ? 0 : split.grid - 1;
+    const int fixers = rec.odd != nullptr ? kFixers : 0;
+    if (err == cudaSuccess && joins + fixers > 0) {
+        const int rows = std::min(C::kRows, p.heads / p.cache.kv_heads * p.cache.tokens);
+        const dim3 grid(static_cast<unsigned>(joins + fixers), static_cast<unsigned>(joins > 0 ? (rows + kRowWarps - 1) / kRowWarps : 1));
+        err = launch_early(tree_finish_kernel<C>, grid, kRowWarps * 32, stream, p, status, split, rec, joins, fixers);
+    }
+    return err;
 }
 
 template <int D, bool BF16, bool E4M3>
-cudaError_t launch(const FaTreeParams& p, DeviceStatus* status, void*, int, cudaStream_t stream) {
-    const long long grid = static_cast<long long>(p.cache.batch) * p.heads * p.cache.tokens;
-    if (grid > 0x7fffffffLL) {
-        return cudaErrorInvalidConfiguration;
-    }
-    tree_row_kernel<D, BF16, E4M3><<<static_cast<unsigned>(grid), kRowWarps * 32, 0, stream>>>(p, status);
-    return cudaGetLastError();
+cudaError_t launch_rows(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count, cudaStream_t stream) {
+    return row_tiles(p) == 1 ? launch<Cfg<D, BF16, E4M3, 1>>(p, status, epoch, workspace, sm_count, stream)
+                             : launch<Cfg<D, BF16, E4M3, 2>>(p, status, epoch, workspace, sm_count, stream);
 }
 
 template <int D>
-cudaError_t launch_types(const FaTreeParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
+cudaError_t launch_types(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count, cudaStream_t stream) {
     const bool bf16 = p.dtype == FA_DTYPE_BFLOAT16;
     if (p.cache.dtype == FA_DTYPE_FLOAT8_E4M3) {
-        return bf16 ? launch<D, true, true>(p, status, workspace, sm_count, stream)
-                    : launch<D, false, true>(p, status, workspace, sm_count, stream);
+        return bf16 ? launch_rows<D, true, true>(p, status, epoch, workspace, sm_count, stream)
+                    : launch_rows<D, false, true>(p, status, epoch, workspace, sm_count, stream);
     }
-    return bf16 ? launch<D, true, false>(p, status, workspace, sm_count, stream)
-                : launch<D, false, false>(p, status, workspace, sm_count, stream);
+    return bf16 ? launch_rows<D, true, false>(p, status, epoch, workspace, sm_count, stream)
+                : launch_rows<D, false, false>(p, status, epoch, workspace, sm_count, stream);
 }
 
 }  // namespace
 
-unsigned long long tree_workspace_bytes(const FaTreeParams&, int) { return 0; }
+unsigned long long tree_workspace_bytes(const FaTreeParams& p, int sm_count) {
+    const Split split = split_for(p, sm_count);
+    const unsigned long long records =
+        split.whole ? 0 : static_cast<unsigned long long>(split.grid) * 2 * row_tiles(p) * kTile * (p.cache.head_dim + 2) * 4;
+    return records + (p.cache.tokens > 1 ? 4ull * split.grid : 0);
+}
 
-cudaError_t launch_tree(const FaTreeParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
-    return p.cache.head_dim == 64 ? launch_types<64>(p, status, workspace, sm_count, stream)
-                                  : launch_types<128>(p, status, workspace, sm_count, stream);
+cudaError_t launch_tree(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count, cudaStream_t stream) {
+    return p.cache.head_dim == 64 ? launch_types<64>(p, status, epoch, workspace, sm_count, stream)
+                                  : launch_types<128>(p, status, epoch, workspace, sm_count, stream);
 }
 
 }  // namespace fa_sm100
