@@ -73,10 +73,9 @@ struct Cfg {
 
 struct Listed {             // a key tile
     float4 group[kGroups];  // e4m3: K's scale, log2 of V's, 1 / V's, what P shrinks by
-    int id[kGroups];        // pages; -1: missing, outside the pool, or not shown
+    int64_t at[2][kGroups]; // byte offsets of a group's first row in K and in V
+    uint4 shown;            // bits of the rows that some row of the call sees and that have a page
     int key0;               // first position; -1: the list's end
-    int kvh;
-    int first, last;        // what is shown: [first, last] and what is before the sinks
     uint32_t gone;          // bits of groups that are shown and have no page
     uint32_t shrinks;       // of groups whose P shrinks
     int mixed;              // rows may differ in what they see
@@ -464,31 +463,34 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const Split& s
     const int log2_page = 31 - __clz(c.page_size);
     Piece piece;
     Sequence s;
-    bool more = next_piece(p, split, walk, piece, s);
-    int v = more ? piece.v0 : 0;
-    int skip = which;
-    for (int n = which;; n += kListWarps) {
-        for (; skip > 0 && more; --skip) {
-            if (++v == piece.v1) {
-                more = next_piece(p, split, walk, piece, s);
-                v = more ? piece.v0 : 0;
+    piece.v1 = 0;
+    int n = -1;  // the tile at hand
+    int v = -1;
+    int turn = which;  // the tile that is this warp's
+    while (true) {
+        bool more = true;
+        if (++v >= piece.v1) {
+            more = next_piece(p, split, walk, piece, s);
+            v = piece.v0;
+        }
+        if (++n != turn) {
+            if (!more) {
+                return;  // the end is another warp's
             }
+            continue;
         }
-        if (skip > 0) {
-            return;  // the end is another warp's
-        }
-        skip = kListWarps;
+        turn += kListWarps;
         Listed& to = sh.list[n % kListed];
         const bool ok = mbar_wait(smem_u32(&sh.list_empty[n % kListed]), ((n / kListed) & 1) ^ 1, wctx, kStatusTimeoutProducer);
         if (__all_sync(0xffffffffu, ok) == 0) {
             return;
         }
-        int id = -1;
         if (more) {
             const int key0 = tile_key(s, v);
             const int key = key0 + 8 * (lane % kGroups);
-            const bool shown = key >= 0 && key <= s.last && (key + 7 >= s.first || key < p.sinks);
-            if (shown) {
+            const bool wanted = key >= 0 && key <= s.last && (key + 7 >= s.first || key < p.sinks);
+            int id = -1;
+            if (wanted) {
                 id = __ldg(c.page_table + piece.b * c.table_stride + (key >> log2_page));
                 if (id < 0 || id >= c.num_pages) {
                     id = -1;
@@ -510,16 +512,24 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const Split& s
                     to.group[lane] = make_float4(ks, __log2f(used), inv, shrinks ? vs * inv : 1.0f);
                 }
             }
-            const uint32_t gone = __ballot_sync(0xffffffffu, shown && id < 0 && lane < kGroups);
-            const uint32_t shrink = __ballot_sync(0xffffffffu, shrinks && lane < kGroups);
-            if (lane < kGroups) {
-                to.id[lane] = id;
+            const uint32_t paged = __ballot_sync(0xffffffffu, id >= 0) & 0xffffu;
+            const uint32_t gone = __ballot_sync(0xffffffffu, wanted && id < 0) & 0xffffu;
+            const uint32_t shrink = __ballot_sync(0xffffffffu, shrinks) & 0xffffu;
+            const int slot = (key & (c.page_size - 1)) * (C::D * C::kElem);
+            const bool is_v = lane >= kGroups;  // half of the lanes take K, half V
+            to.at[is_v][lane % kGroups] = max(id, 0) * (is_v ? c.v_stride[0] : c.k_stride[0]) * C::kElem +
+                                          piece.kvh * (is_v ? c.v_stride[1] : c.k_stride[1]) * C::kElem + slot;
+            if (lane < 4) {
+                const int kb = key0 + 32 * lane;
+                uint32_t bits = bits_up_to(s.last - kb) & (~bits_up_to(s.first - 1 - kb) | bits_up_to(p.sinks - 1 - kb));
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    bits &= (paged >> (4 * lane + g)) & 1u ? 0xffffffffu : ~(0xffu << (8 * g));
+                }
+                reinterpret_cast<uint32_t*>(&to.shown)[lane] = bits;
             }
             if (lane == 0) {
                 to.key0 = key0;
-                to.kvh = piece.kvh;
-                to.first = s.first;
-                to.last = s.last;
                 to.gone = gone;
                 to.shrinks = shrink;
                 to.mixed = c.tokens > 1 && (key0 + kTile > s.context || (p.window > 0 && key0 < window_first(max(s.context, 0) + s.count, p.window)));
@@ -537,22 +547,27 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const Split& s
     }
 }
 
-// One warpgroup brings K or V, tile after tile: 16-byte words of the cache's rows, two parts of words per thread in
-// flight while it widens (e4m3) and stores what has come.
-template <class C, bool IS_V>
-__device__ __forceinline__ void load_tiles(const FaTreeParams& p, Shared& sh, uint32_t ring, const WaitCtx& wctx) {
-    constexpr int kStages = IS_V ? kVStages : C::kKStages;
+// One warpgroup brings K, one V, tile after tile: 16-byte words of the cache's rows, two parts of words per thread in
+// flight while it widens (e4m3) and stores what has come. The code is the same for both: what the warps of an SM run
+// side by side has to fit its instruction cache.
+template <class C>
+__device__ __forceinline__ void load_tiles(const FaTreeParams& p, Shared& sh, uint32_t smem, bool is_v, const WaitCtx& wctx) {
+    const int stages = is_v ? kVStages : C::kKStages;
     const FaCache& c = p.cache;
     const int lt = static_cast<int>(threadIdx.x) % 128;
     const int lane = lt % 32;
-    const int chunk = lt % C::kChunks;
-    const int r0 = lt / C::kChunks;
-    const uint8_t* base = static_cast<const uint8_t*>(IS_V ? c.v : c.k) + chunk * 16;
-    const int64_t page_bytes = (IS_V ? c.v_stride[0] : c.k_stride[0]) * C::kElem;
-    const int64_t head_bytes = (IS_V ? c.v_stride[1] : c.k_stride[1]) * C::kElem;
-    uint64_t* full = IS_V ? sh.v_full : sh.k_full;
-    uint64_t* empty = IS_V ? sh.v_empty : sh.k_empty;
-    const int in_page = c.page_size - 1;
+    // Lanes of a warp over its rows' words. e4m3, D = 128: 8 lanes that store together take 4 words of two rows, whose
+    // swizzles differ, against bank conflicts; the other cases have none as they come.
+    constexpr bool kPaired = C::E4M3 && C::D == 128;
+    const int chunk = kPaired ? (lane & 3) + ((lane >> 1) & 4) : lt % C::kChunks;
+    const int r0 = kPaired ? (lt / 32) * 4 + ((lane >> 4) & 1) * 2 + ((lane >> 2) & 1) : lt / C::kChunks;
+    const uint8_t* base = static_cast<const uint8_t*>(is_v ? c.v : c.k) + (r0 & 7) * (C::D * C::kElem) + chunk * 16;
+    const uint32_t ring = smem + (is_v ? C::kSmemV : C::kSmemK);
+    const uint32_t full = smem_u32(is_v ? sh.v_full : sh.k_full);
+    const uint32_t empty = smem_u32(is_v ? sh.v_empty : sh.k_empty);
+    // Where the thread's words go: rows are a multiple of 8 apart, so that the swizzle is the same for all.
+    const uint32_t to0 = tile_offset(r0, C::E4M3 ? 2 * chunk : chunk);
+    const uint32_t to1 = tile_offset(r0, C::E4M3 ? 2 * chunk + 1 : chunk);
     bool odd = false;
 
     // Part `u` of the list is asked for; 0: there is none, 1: it comes, 3: and rows may differ in what they see of it.
@@ -563,22 +578,26 @@ __device__ __forceinline__ void load_tiles(const FaTreeParams& p, Shared& sh, ui
             return 0;
         }
         const Listed& t = sh.list[n % kListed];
-        const int key0 = t.key0;
-        if (key0 < 0) {
+        if (t.key0 < 0) {
             return 0;
         }
-        const uint8_t* head = base + t.kvh * head_bytes;
-        const int first = t.first;
-        const int last = t.last;
+        const uint4 shown = t.shown;
+        const int from = (u % C::kParts) * C::kHold * C::kPassRows + r0;
+        const int64_t* at = &t.at[is_v][from >> 3];
+        if ((shown.x & shown.y & shown.z & shown.w) == 0xffffffffu) {
 #pragma unroll
-        for (int i = 0; i < C::kHold; ++i) {
-            const int r = ((u % C::kParts) * C::kHold + i) * C::kPassRows + r0;
-            const int id = t.id[r >> 3];
-            const int key = key0 + r;
+            for (int i = 0; i < C::kHold; ++i) {
+                word[i] = __ldg(reinterpret_cast<const uint4*>(base + at[i * (C::kPassRows / 8)]));
+            }
+        } else {
             // Zeros for what no row of the call sees.
-            const bool shown = id >= 0 && key <= last && (key >= first || key < p.sinks);
-            word[i] = shown ? __ldg(reinterpret_cast<const uint4*>(head + id * page_bytes + (key & in_page) * (C::D * C::kElem)))
-                            : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int i = 0; i < C::kHold; ++i) {
+                const int r = from + i * C::kPassRows;
+                const uint32_t bits = reinterpret_cast<const uint32_t*>(&t.shown)[r >> 5];
+                word[i] = (bits >> (r & 31)) & 1u ? __ldg(reinterpret_cast<const uint4*>(base + at[i * (C::kPassRows / 8)]))
+                                                  : make_uint4(0u, 0u, 0u, 0u);
+            }
         }
         const int mixed = t.mixed;
         if (u % C::kParts == C::kParts - 1) {
@@ -589,42 +608,47 @@ __device__ __forceinline__ void load_tiles(const FaTreeParams& p, Shared& sh, ui
         }
         return mixed != 0 ? 3 : 1;
     };
+    int slot = 0;
+    uint32_t parity = 1;
     auto bring = [&](int u, const uint4 (&word)[C::kHold], int kind) {
-        const int n = u / C::kParts;
-        const int slot = n % kStages;
-        const bool ok = u % C::kParts > 0 || mbar_wait(smem_u32(&empty[slot]), ((n / kStages) & 1) ^ 1, wctx, kStatusTimeoutProducer);
+        const bool ok = u % C::kParts > 0 || mbar_wait(empty + 8 * slot, parity, wctx, kStatusTimeoutProducer);
         if (__all_sync(0xffffffffu, ok) == 0) {
             return false;
         }
-        const uint32_t tile = ring + slot * C::kTileBytes;
+        const uint32_t tile = ring + slot * C::kTileBytes + (u % C::kParts) * C::kHold * C::kPassRows * 128;
+        if (is_v && kind == 3) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int i = 0; i < C::kHold; ++i) {
+                any |= not_finite<C>(word[i].x) | not_finite<C>(word[i].y) | not_finite<C>(word[i].z) | not_finite<C>(word[i].w);
+            }
+            odd = odd || any != 0;
+        }
 #pragma unroll
         for (int i = 0; i < C::kHold; ++i) {
-            const int r = ((u % C::kParts) * C::kHold + i) * C::kPassRows + r0;
             const uint4 w = word[i];
-            if (IS_V && kind == 3) {
-                odd = odd || (not_finite<C>(w.x) | not_finite<C>(w.y) | not_finite<C>(w.z) | not_finite<C>(w.w)) != 0;
-            }
+            const uint32_t row = i * C::kPassRows * 128;
             if constexpr (C::E4M3) {
                 uint32_t h[8];
                 widen4(w.x, h[0], h[1]);
                 widen4(w.y, h[2], h[3]);
                 widen4(w.z, h[4], h[5]);
                 widen4(w.w, h[6], h[7]);
-                // Lanes of the second box go the other way round, against bank conflicts.
-                const bool swap = (chunk & 4) != 0;
-                store_shared16(tile + tile_offset(r, 2 * chunk + (swap ? 1 : 0)), swap ? h[4] : h[0], swap ? h[5] : h[1],
-                               swap ? h[6] : h[2], swap ? h[7] : h[3]);
-                store_shared16(tile + tile_offset(r, 2 * chunk + (swap ? 0 : 1)), swap ? h[0] : h[4], swap ? h[1] : h[5],
-                               swap ? h[2] : h[6], swap ? h[3] : h[7]);
+                store_shared16(tile + to0 + row, h[0], h[1], h[2], h[3]);
+                store_shared16(tile + to1 + row, h[4], h[5], h[6], h[7]);
             } else {
-                store_shared16(tile + tile_offset(r, chunk), w.x, w.y, w.z, w.w);
+                store_shared16(tile + to0 + row, w.x, w.y, w.z, w.w);
             }
         }
         if (u % C::kParts == C::kParts - 1) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(smem_u32(&full[slot]));
+                mbar_arrive(full + 8 * slot);
+            }
+            if (++slot == stages) {
+                slot = 0;
+                parity ^= 1;
             }
         }
         return true;
@@ -632,18 +656,18 @@ __device__ __forceinline__ void load_tiles(const FaTreeParams& p, Shared& sh, ui
 
     uint4 a[C::kHold], b[C::kHold];
     int kind_a = ask(0, a);
-    int kind_b = kind_a != 0 ? ask(1, b) : 0;
+    int kind_b = 0;
     for (int u = 0; kind_a != 0; u += 2) {
-        if (!bring(u, a, kind_a)) {
+        kind_b = ask(u + 1, b);
+        if (!bring(u, a, kind_a) || kind_b == 0) {
             break;
         }
-        kind_a = kind_b != 0 ? ask(u + 2, a) : 0;
-        if (kind_b == 0 || !bring(u + 1, b, kind_b)) {
+        kind_a = ask(u + 2, a);
+        if (!bring(u + 1, b, kind_b)) {
             break;
         }
-        kind_b = kind_a != 0 ? ask(u + 3, b) : 0;
     }
-    if (IS_V && odd) {
+    if (is_v && odd) {
         sh.odd = 1;
     }
 }
@@ -684,7 +708,7 @@ __device__ __forceinline__ void issue_products(const FaTreeParams& p, const Spli
     };
     bool ok = true;
     int tiles = 0;  // key tiles of the pieces before
-    int taken[2] = {0, 0};
+    int taken0 = 0, taken1 = 0;  // P of either warpgroup
     Piece piece;
     Sequence s;
     for (int items = 0; ok && next_piece(p, split, walk, piece, s); ++items) {
@@ -711,35 +735,32 @@ __device__ __forceinline__ void issue_products(const FaTreeParams& p, const Spli
             }
         };
         ok = wait(&sh.q_full, items);
-        if (ok) {
-            scores(0);
-        }
-        if (ok && steps > 1) {
-            scores(1);
-        }
-        if (ok && items > 0) {
-            ok = wait(&sh.o_free, items - 1);
-        }
-        for (int step = 0; ok && step < steps; ++step) {
-            const int tile = tiles + (NR == 1 ? step : step >> 1);
-            const int w = step & 1;
-            if (NR == 1 || w == 0) {
-                ok = wait(&sh.v_full[tile % kVStages], tile / kVStages);
-            }
-            ok = ok && wait(&sh.p_full[w], taken[w]++);
-            if (!ok) {
-                break;
-            }
-            if (elect_one()) {
-                issue_product<C>(C::kTmemO + w * C::D, C::kTmemS + w * kTile, v + off(tile % kVStages), step < 2);
-                if (NR == 1 || w == 1) {
-                    umma_commit(smem_u32(&sh.v_empty[tile % kVStages]));
+#pragma unroll 1
+        for (int step = -2; ok && step < steps; ++step) {
+            if (step >= 0) {
+                const int tile = tiles + (NR == 1 ? step : step >> 1);
+                const int w = step & 1;
+                if (step == 0 && items > 0) {
+                    ok = wait(&sh.o_free, items - 1);
                 }
-                if (step == steps - 1) {
-                    umma_commit(smem_u32(&sh.done));
+                if (NR == 1 || w == 0) {
+                    ok = ok && wait(&sh.v_full[tile % kVStages], tile / kVStages);
                 }
+                ok = ok && wait(&sh.p_full[w], w == 0 ? taken0++ : taken1++);
+                if (!ok) {
+                    break;
+                }
+                if (elect_one()) {
+                    issue_product<C>(C::kTmemO + w * C::D, C::kTmemS + w * kTile, v + off(tile % kVStages), step < 2);
+                    if (NR == 1 || w == 1) {
+                        umma_commit(smem_u32(&sh.v_empty[tile % kVStages]));
+                    }
+                    if (step == steps - 1) {
+                        umma_commit(smem_u32(&sh.done));
+                    }
+                }
+                __syncwarp();
             }
-            __syncwarp();
             if (step + 2 < steps) {
                 scores(step + 2);
             }
@@ -918,7 +939,7 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, const Split& spli
             const bool full = gone == 0 && key0 + kTile <= min(s.context, s.last + 1) &&
                               (p.window == 0 || key0 >= window_first(max(s.context, 0) + s.count, p.window) || key0 + kTile <= p.sinks);
             float top = -INFINITY;
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < 4; ++c) {
                 uint32_t x[32];
                 tmem_ld32(tmem_s + 32 * c, x);
@@ -968,7 +989,7 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, const Split& spli
             }
             const float used = m == -INFINITY ? 0.0f : m;
             const bool shrinks = C::E4M3 && aux.shrinks != 0;
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < 4; ++c) {
                 uint32_t x[32];
                 tmem_ld32(tmem_s + 32 * c, x);
@@ -991,23 +1012,24 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, const Split& spli
                         inv = a.z;
                         shrink = a.w;
                     }
-                    float y[8];
-                    float sum = 0.0f;
+                    float2 y[4];
+                    const float2 f2 = make_float2(f, f), add2 = make_float2(add, add);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        y[i] = ex2_approx(fmaf(u2f(x[8 * g + i]), f, add));
-                        sum += y[i];
+                    for (int i = 0; i < 4; ++i) {
+                        y[i] = __ffma2_rn(make_float2(u2f(x[8 * g + 2 * i]), u2f(x[8 * g + 2 * i + 1])), f2, add2);
+                        y[i] = make_float2(ex2_approx(y[i].x), ex2_approx(y[i].y));
                     }
-                    l = fmaf(sum, inv, l);
+                    const float2 sum = __fadd2_rn(__fadd2_rn(y[0], y[1]), __fadd2_rn(y[2], y[3]));
+                    l = fmaf(sum.x + sum.y, inv, l);
                     if (shrinks) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            y[i] *= shrink;
+                        for (int i = 0; i < 4; ++i) {
+                            y[i] = make_float2(y[i].x * shrink, y[i].y * shrink);
                         }
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        packed[4 * g + i] = pack2<C::kMmaBf16>(y[2 * i], y[2 * i + 1]);
+                        packed[4 * g + i] = pack2<C::kMmaBf16>(y[i].x, y[i].y);
                     }
                 }
                 tmem_st16(tmem_s + 16 * c, packed);
@@ -1166,12 +1188,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         if (warp < kSoftmaxWarps) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
             softmax<C>(p, split, status, walk, sh, smem_u32(smem), rec, wctx);
-        } else if (warp < kSoftmaxWarps + kLoadWarps / 2) {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
-            load_tiles<C, false>(p, sh, smem_u32(smem) + C::kSmemK, wctx);
         } else if (warp < kMmaWarp) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
-            load_tiles<C, true>(p, sh, smem_u32(smem) + C::kSmemV, wctx);
+            load_tiles<C>(p, sh, smem_u32(smem), warp >= kSoftmaxWarps + kLoadWarps / 2, wctx);
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
             if (warp == kMmaWarp) {
