@@ -273,6 +273,18 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
         : "memory");
 }
 
+// 32 lanes x 64 consecutive columns into registers FROM .. of 128, for kernels whose launch has fewer than the 146
+// registers a thread that the instruction for 128 columns is compiled with.
+template <int FROM>
+__device__ __forceinline__ void tmem_ld64_of128(uint32_t taddr, uint32_t (&r)[128]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+        : "=r"(r[FROM + 0]), "=r"(r[FROM + 1]), "=r"(r[FROM + 2]), "=r"(r[FROM + 3]), "=r"(r[FROM + 4]), "=r"(r[FROM + 5]), "=r"(r[FROM + 6]), "=r"(r[FROM + 7]), "=r"(r[FROM + 8]), "=r"(r[FROM + 9]), "=r"(r[FROM + 10]), "=r"(r[FROM + 11]), "=r"(r[FROM + 12]), "=r"(r[FROM + 13]), "=r"(r[FROM + 14]), "=r"(r[FROM + 15]), "=r"(r[FROM + 16]), "=r"(r[FROM + 17]), "=r"(r[FROM + 18]), "=r"(r[FROM + 19]), "=r"(r[FROM + 20]), "=r"(r[FROM + 21]), "=r"(r[FROM + 22]), "=r"(r[FROM + 23]), "=r"(r[FROM + 24]), "=r"(r[FROM + 25]), "=r"(r[FROM + 26]), "=r"(r[FROM + 27]), "=r"(r[FROM + 28]), "=r"(r[FROM + 29]), "=r"(r[FROM + 30]), "=r"(r[FROM + 31]), "=r"(r[FROM + 32]), "=r"(r[FROM + 33]), "=r"(r[FROM + 34]), "=r"(r[FROM + 35]), "=r"(r[FROM + 36]), "=r"(r[FROM + 37]), "=r"(r[FROM + 38]), "=r"(r[FROM + 39]), "=r"(r[FROM + 40]), "=r"(r[FROM + 41]), "=r"(r[FROM + 42]), "=r"(r[FROM + 43]), "=r"(r[FROM + 44]), "=r"(r[FROM + 45]), "=r"(r[FROM + 46]), "=r"(r[FROM + 47]), "=r"(r[FROM + 48]), "=r"(r[FROM + 49]), "=r"(r[FROM + 50]), "=r"(r[FROM + 51]), "=r"(r[FROM + 52]), "=r"(r[FROM + 53]), "=r"(r[FROM + 54]), "=r"(r[FROM + 55]), "=r"(r[FROM + 56]), "=r"(r[FROM + 57]), "=r"(r[FROM + 58]), "=r"(r[FROM + 59]), "=r"(r[FROM + 60]), "=r"(r[FROM + 61]), "=r"(r[FROM + 62]), "=r"(r[FROM + 63])
+        : "r"(taddr)
+        : "memory");
+}
+
 // 32 lanes x 128 consecutive 32-bit columns in one instruction (register c = column col + c).
 __device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
     asm volatile(
@@ -398,6 +410,11 @@ __host__ __device__ constexpr uint64_t make_smem_desc(uint32_t saddr, uint32_t l
 // the start address.
 __host__ __device__ constexpr uint64_t make_desc_kmajor_sw128(uint32_t saddr) {
     return make_smem_desc(saddr, 16, 1024);
+}
+
+// The same with rows of 64 bytes and the 64-byte swizzle (layout 4): 8-row atoms of 512 B.
+__host__ __device__ constexpr uint64_t make_desc_kmajor_sw64(uint32_t saddr) {
+    return (make_smem_desc(saddr, 16, 512) & ~(7ull << 61)) | (4ull << 61);
 }
 
 // Operand stored MN-major with 128-byte swizzle (V as the B operand of P.V: N = head dim is

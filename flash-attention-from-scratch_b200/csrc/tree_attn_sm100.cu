@@ -13,6 +13,7 @@
 #include "softmax_common.cuh"
 #include "sm100_ptx.cuh"
 #include "stream_internal.h"
+#include "tma_host.h"
 
 namespace fa_sm100 {
 
@@ -29,21 +30,22 @@ constexpr int kTile = 128;  // query rows, and keys, of a product
 constexpr int kBox = 128 * 128;  // bytes of 128 rows of 64 16-bit values, 128-byte swizzle
 
 constexpr int kSoftmaxWarps = 8;
-constexpr int kLoadWarps = 8;  // half of them K, half V
-constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
+constexpr int kValueWarps = 4;
+constexpr int kMmaWarp = kSoftmaxWarps + kValueWarps;
+constexpr int kListWarp = kMmaWarp + 1;  // and the one after it: the list of key tiles, and their copies
+// Tiles are the list warps' in turn. A warp that waits for a ring's slot has seen the slot `kListWarps` tiles before it
+// consumed; with no more warps than a ring has slots the phase it waits for is then never two behind.
+constexpr int kListWarps = 2;
 constexpr int kWarps = kMmaWarp + 4;  // whole warpgroups: registers are handed over between those
 constexpr int kThreads = kWarps * 32;
-// Registers: launched with 96 a thread (65536 / 640, in steps of 8), 480 for a lane of the five warpgroups.
-constexpr int kRegsSoftmax = 112;
-constexpr int kRegsLoad = 96;
-constexpr int kRegsMma = 64;
-static_assert(2 * kRegsSoftmax + 2 * kRegsLoad + kRegsMma <= 5 * 96, "no more than the launch has");
+// Registers: launched with 128 a thread, 512 for a lane of the four warpgroups.
+constexpr int kRegsSoftmax = 184;
+constexpr int kRegsOther = 72;
+static_assert(2 * kRegsSoftmax + 2 * kRegsOther <= 4 * 128, "no more than the launch has");
 
-constexpr int kListWarp = kMmaWarp + 1;  // and the two after it: the list of key tiles
-constexpr int kListWarps = 3;
-constexpr int kVStages = 2;
-constexpr int kListed = 8;  // key tiles listed ahead
-constexpr int kGroups = kTile / 8;  // keys that surely share a page
+constexpr int kListed = 4;           // key tiles listed ahead
+constexpr int kGroups = kTile / 8;   // keys that surely share a page
+constexpr int kMostStages = 4;
 
 template <int D_, bool BF16_, bool E4M3_, int NR_>
 struct Cfg {
@@ -51,29 +53,31 @@ struct Cfg {
     static constexpr bool BF16 = BF16_;  // queries and output
     static constexpr bool E4M3 = E4M3_;
     static constexpr int NR = NR_;  // row tiles of an item: 1 (key tiles alternate between the softmax warpgroups) or 2
-    static constexpr bool kMmaBf16 = BF16 && !E4M3;
+    static constexpr bool kMmaBf16 = BF16 && !E4M3;  // type of P and V (and of Q and K, over a 16-bit cache)
     static constexpr int kElem = E4M3 ? 1 : 2;
-    static constexpr int kTileBytes = kBox * (D / 64);
+    // e4m3 terms that a query is the sum of: bfloat16 has 8 bits, float16 11, a term 4.
+    static constexpr int kTerms = E4M3 ? (BF16 ? 2 : 3) : 1;
+    static constexpr int kRaw = kTile * D * kElem;      // bytes of a tile as the cache holds it
+    static constexpr int kWide = kTile * D * 2;         // of a tile of 16-bit values
+    static constexpr int kQTile = kTerms * kRaw;
+    // Rings: K as it is; V as it is and, e4m3, widened.
+    static constexpr int kKStages = E4M3 ? (NR == 1 ? 4 : (BF16 ? 3 : 2)) : (NR == 1 ? 3 : 2);
+    static constexpr int kRStages = E4M3 && NR == 1 && BF16 ? 3 : 2;
+    static constexpr int kVStages = 2;
+    static_assert(kKStages >= kListWarps && kRStages >= kListWarps && kVStages >= kListWarps && kListed >= kListWarps, "see kListWarps");
     static constexpr int kSmemQ = 0;
-    static constexpr int kSmemK = NR * kTileBytes;
-    static constexpr int kKStages = NR == 1 ? 3 : 2;
-    static constexpr int kSmemV = kSmemK + kKStages * kTileBytes;
-    static constexpr int kSmemShared = kSmemV + kVStages * kTileBytes;
+    static constexpr int kSmemK = NR * kQTile;
+    static constexpr int kSmemV = kSmemK + kKStages * kRaw;
+    static constexpr int kSmemR = kSmemV + kVStages * kWide;
+    static constexpr int kSmemShared = kSmemR + (E4M3 ? kRStages * kRaw : 0);
     static constexpr int kRows = NR * kTile;
     // Tensor memory: two scores, P over each's first half, two sums.
     static constexpr uint32_t kTmemS = 0;
     static constexpr uint32_t kTmemO = 2 * kTile;
-    // A loader warpgroup's copies: 16 bytes a thread and pass.
-    static constexpr int kChunks = D * kElem / 16;
-    static constexpr int kPassRows = 128 / kChunks;
-    static constexpr int kPasses = kTile / kPassRows;
-    static constexpr int kHold = kPasses < 8 ? kPasses : 8;  // words of a thread's part of a tile: all or half
-    static constexpr int kParts = kPasses / kHold;
 };
 
 struct Listed {             // a key tile
     float4 group[kGroups];  // e4m3: K's scale, log2 of V's, 1 / V's, what P shrinks by
-    int64_t at[2][kGroups]; // byte offsets of a group's first row in K and in V
     uint4 shown;            // bits of the rows that some row of the call sees and that have a page
     int key0;               // first position; -1: the list's end
     uint32_t gone;          // bits of groups that are shown and have no page
@@ -84,7 +88,7 @@ struct Listed {             // a key tile
 struct Shared {
     Listed list[kListed];
     uint64_t list_full[kListed], list_empty[kListed];
-    uint64_t k_full[3], k_empty[3], v_full[kVStages], v_empty[kVStages];
+    uint64_t k_full[kMostStages], k_empty[kMostStages], v_full[2], v_empty[2], r_full[kMostStages], r_empty[kMostStages];
     uint64_t s_full[2], p_full[2];
     uint64_t q_full, q_empty, done, o_free, ml_full, mma_idle;
     long long warp_sum[kWarps];
@@ -449,24 +453,42 @@ __device__ __forceinline__ uint32_t tile_offset(int r, int c) {
     return static_cast<uint32_t>((c >> 3) * kBox + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+// The same in a tile of e4m3 values: rows of 128 bytes with the 128-byte swizzle, or of 64 with the 64-byte one.
+template <int D>
+__device__ __forceinline__ uint32_t code_offset(int r, int c) {
+    return D == 128 ? static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4)) : static_cast<uint32_t>(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+}
+
 __device__ __forceinline__ void store_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// The range's key tiles, listed for the loaders and the softmax: every third by this warp, so that the loads of pages and
-// scales of three tiles wait for each other's time alone.
+__device__ __forceinline__ uint4 load_shared16(uint32_t at) {
+    uint4 w;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at) : "memory");
+    return w;
+}
+
+// The range's key tiles: listed for the others, and copied, K and V, a copy a page. Every second tile is this warp's, so
+// that the loads of pages and scales of two tiles are on their way at once.
 template <class C>
-__device__ __forceinline__ void list_tiles(const FaTreeParams& p, const Split& split, DeviceStatus* status, Walk walk, Shared& sh,
-                                           int which, const WaitCtx& wctx) {
+__device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensorMap* tm_k, const CUtensorMap* tm_v, const Split& split,
+                                           DeviceStatus* status, Walk walk, Shared& sh, uint32_t smem, int which, const WaitCtx& wctx) {
     const FaCache& c = p.cache;
     const int lane = static_cast<int>(threadIdx.x) % 32;
     const int log2_page = 31 - __clz(c.page_size);
+    const int log2_span = min(log2_page, 7);
+    constexpr int kVRing = C::E4M3 ? C::kRStages : C::kVStages;
+    uint64_t* v_free = C::E4M3 ? sh.r_empty : sh.v_empty;
     Piece piece;
     Sequence s;
     piece.v1 = 0;
     int n = -1;  // the tile at hand
     int v = -1;
     int turn = which;  // the tile that is this warp's
+    auto wait = [&](uint64_t* bar, int phase) {
+        return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), (phase & 1) ^ 1, wctx, kStatusTimeoutProducer)) != 0;
+    };
     while (true) {
         bool more = true;
         if (++v >= piece.v1) {
@@ -481,204 +503,226 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const Split& s
         }
         turn += kListWarps;
         Listed& to = sh.list[n % kListed];
-        const bool ok = mbar_wait(smem_u32(&sh.list_empty[n % kListed]), ((n / kListed) & 1) ^ 1, wctx, kStatusTimeoutProducer);
-        if (__all_sync(0xffffffffu, ok) == 0) {
+        if (!more) {
+            if (wait(&sh.list_empty[n % kListed], n / kListed) && lane == 0) {
+                to.key0 = -1;
+                mbar_arrive(smem_u32(&sh.list_full[n % kListed]));
+            }
             return;
         }
-        if (more) {
-            const int key0 = tile_key(s, v);
-            const int key = key0 + 8 * (lane % kGroups);
-            const bool wanted = key >= 0 && key <= s.last && (key + 7 >= s.first || key < p.sinks);
-            int id = -1;
-            if (wanted) {
-                id = __ldg(c.page_table + piece.b * c.table_stride + (key >> log2_page));
-                if (id < 0 || id >= c.num_pages) {
-                    id = -1;
-                    atomicOr(&status->code, kStatusBadPage);
-                }
+        const int key0 = tile_key(s, v);
+        // Lane i's span: what lies in one page.
+        const int span_key = key0 + (lane << log2_span);
+        int id = -1;
+        if (lane < (kTile >> log2_span) && span_key >= 0 && span_key <= s.last &&
+            (span_key + (1 << log2_span) > s.first || span_key < p.sinks)) {
+            id = __ldg(c.page_table + piece.b * c.table_stride + (span_key >> log2_page));
+            if (id < 0 || id >= c.num_pages) {
+                id = -1;
+                atomicOr(&status->code, kStatusBadPage);
             }
-            bool shrinks = false;
-            if constexpr (C::E4M3) {
-                float ks = 1.0f, vs = 1.0f;
-                if (id >= 0) {
-                    const int64_t at = static_cast<int64_t>(id) * c.kv_heads + piece.kvh;
-                    ks = __ldg(c.k_scale + at);
-                    vs = __ldg(c.v_scale + at);
-                }
-                const float used = fmaxf(vs, kMinScale);
-                const float inv = __fdividef(1.0f, used);
-                shrinks = vs < kMinScale;
-                if (lane < kGroups) {
-                    to.group[lane] = make_float4(ks, __log2f(used), inv, shrinks ? vs * inv : 1.0f);
-                }
-            }
-            const uint32_t paged = __ballot_sync(0xffffffffu, id >= 0) & 0xffffu;
-            const uint32_t gone = __ballot_sync(0xffffffffu, wanted && id < 0) & 0xffffu;
-            const uint32_t shrink = __ballot_sync(0xffffffffu, shrinks) & 0xffffu;
-            const int slot = (key & (c.page_size - 1)) * (C::D * C::kElem);
-            const bool is_v = lane >= kGroups;  // half of the lanes take K, half V
-            to.at[is_v][lane % kGroups] = max(id, 0) * (is_v ? c.v_stride[0] : c.k_stride[0]) * C::kElem +
-                                          piece.kvh * (is_v ? c.v_stride[1] : c.k_stride[1]) * C::kElem + slot;
-            if (lane < 4) {
-                const int kb = key0 + 32 * lane;
-                uint32_t bits = bits_up_to(s.last - kb) & (~bits_up_to(s.first - 1 - kb) | bits_up_to(p.sinks - 1 - kb));
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    bits &= (paged >> (4 * lane + g)) & 1u ? 0xffffffffu : ~(0xffu << (8 * g));
-                }
-                reinterpret_cast<uint32_t*>(&to.shown)[lane] = bits;
-            }
+        }
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, id >= 0)) * (static_cast<uint32_t>(C::D * C::kElem) << log2_span);
+        const int y = span_key & (c.page_size - 1);
+        const uint32_t row = static_cast<uint32_t>(lane) << log2_span;
+        auto copy = [&](uint32_t tile, const CUtensorMap* map, uint64_t* full) {
             if (lane == 0) {
-                to.key0 = key0;
-                to.gone = gone;
-                to.shrinks = shrink;
-                to.mixed = c.tokens > 1 && (key0 + kTile > s.context || (p.window > 0 && key0 < window_first(max(s.context, 0) + s.count, p.window)));
+                mbar_arrive_expect_tx(smem_u32(full), bytes);
             }
-        } else if (lane == 0) {
-            to.key0 = -1;
+            __syncwarp();
+            if (id >= 0) {
+                if constexpr (C::E4M3) {
+                    tma_load_4d(tile + row * C::D, map, smem_u32(full), 0, y, piece.kvh, id);
+                } else {
+#pragma unroll
+                    for (int box = 0; box < C::D / 64; ++box) {
+                        tma_load_4d(tile + box * kBox + row * 128, map, smem_u32(full), 64 * box, y, piece.kvh, id);
+                    }
+                }
+            }
+        };
+        if (!wait(&sh.k_empty[n % C::kKStages], n / C::kKStages)) {
+            return;
+        }
+        copy(smem + C::kSmemK + (n % C::kKStages) * C::kRaw, tm_k, &sh.k_full[n % C::kKStages]);
+        // The groups' pages and scales.
+        const int group = lane % kGroups;
+        const int key = key0 + 8 * group;
+        const int page = __shfl_sync(0xffffffffu, id, (8 * group) >> log2_span);
+        const bool wanted = key >= 0 && key <= s.last && (key + 7 >= s.first || key < p.sinks);
+        float ks = 1.0f, vs = 1.0f;
+        if (C::E4M3 && page >= 0) {
+            const int64_t at = static_cast<int64_t>(page) * c.kv_heads + piece.kvh;
+            ks = __ldg(c.k_scale + at);
+            vs = __ldg(c.v_scale + at);
+        }
+        if (!wait(&v_free[n % kVRing], n / kVRing)) {
+            return;
+        }
+        copy(smem + (C::E4M3 ? C::kSmemR : C::kSmemV) + (n % kVRing) * C::kRaw, tm_v, &sh.r_full[n % kVRing]);
+        if (!wait(&sh.list_empty[n % kListed], n / kListed)) {
+            return;
+        }
+        bool shrinks = false;
+        if constexpr (C::E4M3) {
+            const float used = fmaxf(vs, kMinScale);
+            const float inv = __fdividef(1.0f, used);
+            shrinks = vs < kMinScale;
+            if (lane < kGroups) {
+                to.group[lane] = make_float4(ks, __log2f(used), inv, shrinks ? vs * inv : 1.0f);
+            }
+        }
+        const uint32_t paged = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
+        const uint32_t gone = __ballot_sync(0xffffffffu, wanted && page < 0) & 0xffffu;
+        const uint32_t shrink = __ballot_sync(0xffffffffu, shrinks) & 0xffffu;
+        if (lane < 4) {
+            const int kb = key0 + 32 * lane;
+            uint32_t bits = bits_up_to(s.last - kb) & (~bits_up_to(s.first - 1 - kb) | bits_up_to(p.sinks - 1 - kb));
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                bits &= (paged >> (4 * lane + g)) & 1u ? 0xffffffffu : ~(0xffu << (8 * g));
+            }
+            reinterpret_cast<uint32_t*>(&to.shown)[lane] = bits;
+        }
+        if (lane == 0) {
+            to.key0 = key0;
+            to.gone = gone;
+            to.shrinks = shrink;
+            to.mixed = c.tokens > 1 && (key0 + kTile > s.context || (p.window > 0 && key0 < window_first(max(s.context, 0) + s.count, p.window)));
         }
         __syncwarp();
         if (lane == 0) {
             mbar_arrive(smem_u32(&sh.list_full[n % kListed]));
         }
-        if (!more) {
-            return;
-        }
     }
 }
 
-// One warpgroup brings K, one V, tile after tile: 16-byte words of the cache's rows, two parts of words per thread in
-// flight while it widens (e4m3) and stores what has come. The code is the same for both: what the warps of an SM run
-// side by side has to fit its instruction cache.
+// V's tiles made ready: e4m3 values widened to float16 and laid out for the product, rows that no row of the call sees made
+// zeros (0 times what lies there could be NaN), and what is not finite noticed where rows differ in what they see.
 template <class C>
-__device__ __forceinline__ void load_tiles(const FaTreeParams& p, Shared& sh, uint32_t smem, bool is_v, const WaitCtx& wctx) {
-    const int stages = is_v ? kVStages : C::kKStages;
-    const FaCache& c = p.cache;
+__device__ __forceinline__ void ready_values(const FaTreeParams& p, Shared& sh, uint32_t smem, const WaitCtx& wctx) {
+    constexpr int kRing = C::E4M3 ? C::kRStages : C::kVStages;
+    constexpr int kChunks = C::D * C::kElem / 16;  // 16-byte words of a row
     const int lt = static_cast<int>(threadIdx.x) % 128;
     const int lane = lt % 32;
-    // Lanes of a warp over its rows' words. e4m3, D = 128: 8 lanes that store together take 4 words of two rows, whose
-    // swizzles differ, against bank conflicts; the other cases have none as they come.
-    constexpr bool kPaired = C::E4M3 && C::D == 128;
-    const int chunk = kPaired ? (lane & 3) + ((lane >> 1) & 4) : lt % C::kChunks;
-    const int r0 = kPaired ? (lt / 32) * 4 + ((lane >> 4) & 1) * 2 + ((lane >> 2) & 1) : lt / C::kChunks;
-    const uint8_t* base = static_cast<const uint8_t*>(is_v ? c.v : c.k) + (r0 & 7) * (C::D * C::kElem) + chunk * 16;
-    const uint32_t ring = smem + (is_v ? C::kSmemV : C::kSmemK);
-    const uint32_t full = smem_u32(is_v ? sh.v_full : sh.k_full);
-    const uint32_t empty = smem_u32(is_v ? sh.v_empty : sh.k_empty);
-    // Where the thread's words go: rows are a multiple of 8 apart, so that the swizzle is the same for all.
-    const uint32_t to0 = tile_offset(r0, C::E4M3 ? 2 * chunk : chunk);
-    const uint32_t to1 = tile_offset(r0, C::E4M3 ? 2 * chunk + 1 : chunk);
+    const int warp = lt / 32;
+    auto wait = [&](uint64_t* bar, int phase) {
+        return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), phase & 1, wctx, kStatusTimeoutProducer)) != 0;
+    };
     bool odd = false;
-
-    // Part `u` of the list is asked for; 0: there is none, 1: it comes, 3: and rows may differ in what they see of it.
-    auto ask = [&](int u, uint4 (&word)[C::kHold]) {
-        const int n = u / C::kParts;
-        const bool ok = mbar_wait(smem_u32(&sh.list_full[n % kListed]), (n / kListed) & 1, wctx, kStatusTimeoutProducer);
-        if (__all_sync(0xffffffffu, ok) == 0) {
-            return 0;
+    for (int n = 0;; ++n) {
+        if (!wait(&sh.list_full[n % kListed], n / kListed)) {
+            break;
         }
         const Listed& t = sh.list[n % kListed];
         if (t.key0 < 0) {
-            return 0;
+            break;
         }
-        const uint4 shown = t.shown;
-        const int from = (u % C::kParts) * C::kHold * C::kPassRows + r0;
-        const int64_t* at = &t.at[is_v][from >> 3];
-        if ((shown.x & shown.y & shown.z & shown.w) == 0xffffffffu) {
+        const bool mixed = t.mixed != 0;
+        const bool whole = (t.shown.x & t.shown.y & t.shown.z & t.shown.w) == 0xffffffffu;
+        const uint32_t* shown = reinterpret_cast<const uint32_t*>(&t.shown);
+        if (!wait(&sh.r_full[n % kRing], n / kRing)) {
+            break;
+        }
+        const uint32_t wide = smem + C::kSmemV + (n % C::kVStages) * C::kWide;
+        if constexpr (C::E4M3) {
+            const uint32_t raw = smem + C::kSmemR + (n % C::kRStages) * C::kRaw;
+            if (!wait(&sh.v_empty[n % C::kVStages], n / C::kVStages + 1)) {
+                break;
+            }
+            // Words of 8 lanes that load and store together: D = 128, half a row of rows r and r ^ 5, which the swizzles of
+            // 128-byte rows (codes: by r, values: two chunks apart) put into different banks; D = 64, two rows.
+            constexpr int kPasses = kTile * kChunks / 128;
 #pragma unroll
-            for (int i = 0; i < C::kHold; ++i) {
-                word[i] = __ldg(reinterpret_cast<const uint4*>(base + at[i * (C::kPassRows / 8)]));
-            }
-        } else {
-            // Zeros for what no row of the call sees.
+            for (int i0 = 0; i0 < kPasses; i0 += 4) {
+                uint4 w[4];
+                int r[4], chunk;
 #pragma unroll
-            for (int i = 0; i < C::kHold; ++i) {
-                const int r = from + i * C::kPassRows;
-                const uint32_t bits = reinterpret_cast<const uint32_t*>(&t.shown)[r >> 5];
-                word[i] = (bits >> (r & 31)) & 1u ? __ldg(reinterpret_cast<const uint4*>(base + at[i * (C::kPassRows / 8)]))
-                                                  : make_uint4(0u, 0u, 0u, 0u);
-            }
-        }
-        const int mixed = t.mixed;
-        if (u % C::kParts == C::kParts - 1) {
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(smem_u32(&sh.list_empty[n % kListed]));
-            }
-        }
-        return mixed != 0 ? 3 : 1;
-    };
-    int slot = 0;
-    uint32_t parity = 1;
-    auto bring = [&](int u, const uint4 (&word)[C::kHold], int kind) {
-        const bool ok = u % C::kParts > 0 || mbar_wait(empty + 8 * slot, parity, wctx, kStatusTimeoutProducer);
-        if (__all_sync(0xffffffffu, ok) == 0) {
-            return false;
-        }
-        const uint32_t tile = ring + slot * C::kTileBytes + (u % C::kParts) * C::kHold * C::kPassRows * 128;
-        if (is_v && kind == 3) {
-            uint32_t any = 0;
+                for (int i = 0; i < 4; ++i) {
+                    const int pass = i0 + i;
+                    if constexpr (C::D == 128) {
+                        const int a = 2 * (pass & 1) + (lane >> 4);
+                        r[i] = warp * 32 + (pass >> 1) * 8 + ((lane & 4) != 0 ? a ^ 5 : a);
+                        chunk = (lane & 3) + ((lane >> 1) & 4);
+                        w[i] = load_shared16(raw + code_offset<128>(r[i], chunk));
+                    } else {
+                        r[i] = warp * 32 + pass * 8 + (lane >> 2);
+                        chunk = lane & 3;
+                        w[i] = load_shared16(raw + r[i] * 64 + chunk * 16);
+                    }
+                }
+                if (mixed || !whole) {
+                    uint32_t any = 0;
 #pragma unroll
-            for (int i = 0; i < C::kHold; ++i) {
-                any |= not_finite<C>(word[i].x) | not_finite<C>(word[i].y) | not_finite<C>(word[i].z) | not_finite<C>(word[i].w);
-            }
-            odd = odd || any != 0;
-        }
+                    for (int i = 0; i < 4; ++i) {
+                        if (!((shown[r[i] >> 5] >> (r[i] & 31)) & 1u)) {
+                            w[i] = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                        any |= not_finite<C>(w[i].x) | not_finite<C>(w[i].y) | not_finite<C>(w[i].z) | not_finite<C>(w[i].w);
+                    }
+                    odd = odd || (mixed && any != 0);
+                }
 #pragma unroll
-        for (int i = 0; i < C::kHold; ++i) {
-            const uint4 w = word[i];
-            const uint32_t row = i * C::kPassRows * 128;
-            if constexpr (C::E4M3) {
-                uint32_t h[8];
-                widen4(w.x, h[0], h[1]);
-                widen4(w.y, h[2], h[3]);
-                widen4(w.z, h[4], h[5]);
-                widen4(w.w, h[6], h[7]);
-                store_shared16(tile + to0 + row, h[0], h[1], h[2], h[3]);
-                store_shared16(tile + to1 + row, h[4], h[5], h[6], h[7]);
-            } else {
-                store_shared16(tile + to0 + row, w.x, w.y, w.z, w.w);
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t h[8];
+                    widen4(w[i].x, h[0], h[1]);
+                    widen4(w[i].y, h[2], h[3]);
+                    widen4(w[i].z, h[4], h[5]);
+                    widen4(w[i].w, h[6], h[7]);
+                    store_shared16(wide + tile_offset(r[i], 2 * chunk), h[0], h[1], h[2], h[3]);
+                    store_shared16(wide + tile_offset(r[i], 2 * chunk + 1), h[4], h[5], h[6], h[7]);
+                }
             }
-        }
-        if (u % C::kParts == C::kParts - 1) {
             fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(full + 8 * slot);
+        } else if (mixed || !whole) {
+            uint32_t any = 0;
+#pragma unroll 1
+            for (int i = lt; i < kTile * kChunks; i += 128) {
+                const int r = i / kChunks;
+                const uint32_t at = wide + tile_offset(r, i % kChunks);
+                if (!((shown[r >> 5] >> (r & 31)) & 1u)) {
+                    store_shared16(at, 0u, 0u, 0u, 0u);
+                } else {
+                    const uint4 w = load_shared16(at);
+                    any |= not_finite<C>(w.x) | not_finite<C>(w.y) | not_finite<C>(w.z) | not_finite<C>(w.w);
+                }
             }
-            if (++slot == stages) {
-                slot = 0;
-                parity ^= 1;
+            odd = odd || (mixed && any != 0);
+            fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) {
+            mbar_arrive(smem_u32(&sh.v_full[n % C::kVStages]));
+            if constexpr (C::E4M3) {
+                mbar_arrive(smem_u32(&sh.r_empty[n % C::kRStages]));
             }
-        }
-        return true;
-    };
-
-    uint4 a[C::kHold], b[C::kHold];
-    int kind_a = ask(0, a);
-    int kind_b = 0;
-    for (int u = 0; kind_a != 0; u += 2) {
-        kind_b = ask(u + 1, b);
-        if (!bring(u, a, kind_a) || kind_b == 0) {
-            break;
-        }
-        kind_a = ask(u + 2, a);
-        if (!bring(u + 1, b, kind_b)) {
-            break;
+            mbar_arrive(smem_u32(&sh.list_empty[n % kListed]));
         }
     }
-    if (is_v && odd) {
+    if (odd) {
         sh.odd = 1;
     }
 }
 
 template <class C>
 __device__ __forceinline__ void issue_scores(uint32_t d, uint64_t a, uint64_t b) {
+    // kind::f8f6f4 with e4m3 operands has the instruction descriptor of kind::f16 with float16.
     constexpr uint32_t idesc = make_idesc_f16(kTile, kTile, true, false, C::kMmaBf16);
+    if constexpr (C::E4M3) {
 #pragma unroll
-    for (int k = 0; k < C::D / 16; ++k) {
-        const uint64_t off = static_cast<uint64_t>(((k / 4) * kBox + (k % 4) * 32) >> 4);
-        umma_ss(d, a + off, b + off, idesc, k > 0 ? 1u : 0u);
+        for (int term = 0; term < C::kTerms; ++term) {
+#pragma unroll
+            for (int k = 0; k < C::D / 32; ++k) {
+                umma_ss_f8(d, a + static_cast<uint64_t>((term * C::kRaw + 32 * k) >> 4), b + static_cast<uint64_t>((32 * k) >> 4), idesc,
+                           term + k > 0 ? 1u : 0u);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < C::D / 16; ++k) {
+            const uint64_t off = static_cast<uint64_t>(((k / 4) * kBox + (k % 4) * 32) >> 4);
+            umma_ss(d, a + off, b + off, idesc, k > 0 ? 1u : 0u);
+        }
     }
 }
 
@@ -697,10 +741,11 @@ template <class C>
 __device__ __forceinline__ void issue_products(const FaTreeParams& p, const Split& split, Walk walk, Shared& sh, uint32_t smem,
                                                const WaitCtx& wctx) {
     constexpr int NR = C::NR;
-    const uint64_t q = make_desc_kmajor_sw128(smem + C::kSmemQ);
-    const uint64_t k = make_desc_kmajor_sw128(smem + C::kSmemK);
+    auto kmajor = [](uint32_t at) { return C::E4M3 && C::D == 64 ? make_desc_kmajor_sw64(at) : make_desc_kmajor_sw128(at); };
+    const uint64_t q = kmajor(smem + C::kSmemQ);
+    const uint64_t k = kmajor(smem + C::kSmemK);
     const uint64_t v = make_desc_mnmajor_sw128(smem + C::kSmemV, kBox);
-    auto off = [](int tile) { return static_cast<uint64_t>(tile * (C::kTileBytes >> 4)); };
+    auto off = [](int tile, int bytes) { return static_cast<uint64_t>(tile * (bytes >> 4)); };
     auto wait = [&](uint64_t* bar, int parity) {
         const bool there = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity & 1, wctx, kStatusTimeoutMma)) != 0;
         tc_fence_after();
@@ -722,7 +767,7 @@ __device__ __forceinline__ void issue_products(const FaTreeParams& p, const Spli
             }
             if (ok) {
                 if (elect_one()) {
-                    issue_scores<C>(C::kTmemS + w * kTile, q + off(NR == 1 ? 0 : w), k + off(tile % C::kKStages));
+                    issue_scores<C>(C::kTmemS + w * kTile, q + off(NR == 1 ? 0 : w, C::kQTile), k + off(tile % C::kKStages, C::kRaw));
                     umma_commit(smem_u32(&sh.s_full[w]));
                     if (NR == 1 || w == 1) {
                         umma_commit(smem_u32(&sh.k_empty[tile % C::kKStages]));
@@ -744,16 +789,16 @@ __device__ __forceinline__ void issue_products(const FaTreeParams& p, const Spli
                     ok = wait(&sh.o_free, items - 1);
                 }
                 if (NR == 1 || w == 0) {
-                    ok = ok && wait(&sh.v_full[tile % kVStages], tile / kVStages);
+                    ok = ok && wait(&sh.v_full[tile % C::kVStages], tile / C::kVStages);
                 }
                 ok = ok && wait(&sh.p_full[w], w == 0 ? taken0++ : taken1++);
                 if (!ok) {
                     break;
                 }
                 if (elect_one()) {
-                    issue_product<C>(C::kTmemO + w * C::D, C::kTmemS + w * kTile, v + off(tile % kVStages), step < 2);
+                    issue_product<C>(C::kTmemO + w * C::D, C::kTmemS + w * kTile, v + off(tile % C::kVStages, C::kWide), step < 2);
                     if (NR == 1 || w == 1) {
-                        umma_commit(smem_u32(&sh.v_empty[tile % kVStages]));
+                        umma_commit(smem_u32(&sh.v_empty[tile % C::kVStages]));
                     }
                     if (step == steps - 1) {
                         umma_commit(smem_u32(&sh.done));
@@ -785,54 +830,83 @@ struct Row {
     float factor;       // of a score, in log2 units
 };
 
-// The words of one row that are its own to bring (WORDS 16-byte words from word `from`), into Q's tile; and what
-// bfloat16 queries over an e4m3 cache are scaled down by. See the cached kernel: the largest of a row goes to [2^13, 2^14).
+// A row's own part of Q's tile, 16 dims at a time from dim `from` on: as it is, or, over an e4m3 cache, as the sum of e4m3
+// terms (each the nearest to what the ones before leave), brought to [2^8, 448) by a power of two that `factor` takes
+// back. The terms hold bfloat16 and float16 exactly, down to multiples of 2^-10 beside a largest value of 2^8 or more.
 template <class C>
-__device__ __forceinline__ void bring_query(const FaTreeParams& p, Row& row, int b, int head, uint32_t tile, int r, int from, int words) {
+__device__ __forceinline__ void bring_query(const FaTreeParams& p, Row& row, int b, int head, uint32_t tile, int r, int from, int to) {
     const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] +
                                                       head * p.q_stride[1] + row.token * p.q_stride[2]);
     const uint32_t sign = p.softmax_scale < 0.0f ? 0x80008000u : 0u;  // the factor stays positive
     row.factor = fmaxf(fabsf(p.softmax_scale) * kLog2e, kLeastFactor);
-    float up = 1.0f;
-    if constexpr (C::E4M3 && C::BF16) {
-        uint32_t top = 0;  // of the values' bits without sign: their order is that of the sizes
-        if (row.real) {
-#pragma unroll 4
-            for (int i = 0; i < C::D / 8; ++i) {
-                const uint4 w = __ldg(src + i);
-                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    top = max(top, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
-                }
-            }
-        }
-        // 2^(13 - exponent of the largest), both it and its inverse normal; 1 for zeros, inf and NaN.
-        const int e = static_cast<int>(top >> 7);
-        const int shift = (e == 0 || e == 255) ? 0 : min(max(140 - e, -100), 100);
-        up = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
-        row.factor = fmaxf(row.factor * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23), kLeastFactor);
-    }
-#pragma unroll 4
-    for (int i = from; i < from + words; ++i) {
+    auto words = [&](int i, uint32_t (&x)[4]) {
         const uint4 w = row.real ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
-        uint32_t x[4] = {w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign};
-        if constexpr (C::E4M3 && C::BF16) {
+        x[0] = w.x ^ sign;
+        x[1] = w.y ^ sign;
+        x[2] = w.z ^ sign;
+        x[3] = w.w ^ sign;
+    };
+    if constexpr (!C::E4M3) {
+#pragma unroll 4
+        for (int i = from / 8; i < to / 8; ++i) {
+            uint32_t x[4];
+            words(i, x);
+            store_shared16(tile + tile_offset(r, i), x[0], x[1], x[2], x[3]);
+        }
+        return;
+    }
+    uint32_t top = 0;  // of the values' bits without sign: their order is that of the sizes
+#pragma unroll 4
+    for (int i = 0; i < C::D / 8; ++i) {
+        uint32_t x[4];
+        words(i, x);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = pack_half2(__uint_as_float(x[e] << 16) * up, __uint_as_float(x[e] & 0xFFFF0000u) * up);
+        for (int e = 0; e < 4; ++e) {
+            top = max(top, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
+        }
+    }
+    // 2^(8 - exponent of the largest), one less where that would pass 448, both it and its inverse normal; 1 for zeros, inf and NaN.
+    const float most = widen16<C::BF16>(static_cast<uint16_t>(top));
+    const int e = static_cast<int>(__float_as_uint(most) >> 23);
+    const int shift = (e == 0 || e == 255) ? 0 : min(max(135 - e - ((__float_as_uint(most) & 0x7fffffu) > 0x600000u ? 1 : 0), -100), 100);
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+    row.factor = fmaxf(row.factor * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23), kLeastFactor);
+#pragma unroll 1
+    for (int c = from / 16; c < to / 16; ++c) {
+        float f[16];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            uint32_t x[4];
+            words(2 * c + half, x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f[8 * half + 2 * i] = widen16<C::BF16>(static_cast<uint16_t>(x[i] & 0xffffu)) * up;
+                f[8 * half + 2 * i + 1] = widen16<C::BF16>(static_cast<uint16_t>(x[i] >> 16)) * up;
             }
         }
-        store_shared16(tile + tile_offset(r, i), x[0], x[1], x[2], x[3]);
+#pragma unroll
+        for (int term = 0; term < C::kTerms; ++term) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t lo = pack_e4m3x2(f[4 * i], f[4 * i + 1]);
+                const uint32_t hi = pack_e4m3x2(f[4 * i + 2], f[4 * i + 3]);
+                w[i] = lo | (hi << 16);
+                const float2 a = unpack_half2(e4m3x2_to_half2(lo));
+                const float2 b2 = unpack_half2(e4m3x2_to_half2(hi));
+                f[4 * i] -= a.x;
+                f[4 * i + 1] -= a.y;
+                f[4 * i + 2] -= b2.x;
+                f[4 * i + 3] -= b2.y;
+            }
+            store_shared16(tile + term * C::kRaw + code_offset<C::D>(r, c), w[0], w[1], w[2], w[3]);
+        }
     }
 }
 
 // 32 columns of scores, keys from kb on: those that the row does not see become -inf.
 template <class C>
 __device__ __forceinline__ uint32_t kept_columns(const FaTreeParams& p, const Sequence& s, const Row& row, int kb, uint32_t gone) {
-    if (!row.real) {
-        return 0;
-    }
     uint32_t keep = bits_up_to(min(s.context - 1, s.last) - kb);
     if (p.window > 0) {
         keep &= ~bits_up_to(row.first - 1 - kb) | bits_up_to(p.sinks - 1 - kb);
@@ -851,7 +925,97 @@ __device__ __forceinline__ uint32_t kept_columns(const FaTreeParams& p, const Se
     // 4 groups of 8 keys.
     const uint32_t pages = ~gone;
     keep &= ((pages & 1u) * 0xffu) | (((pages >> 1) & 1u) * 0xff00u) | (((pages >> 2) & 1u) * 0xff0000u) | (((pages >> 3) & 1u) * 0xff000000u);
-    return keep;
+    return row.real ? keep : 0u;
+}
+
+// One row's scores turned into P, in place: returns what the sums so far (and l, done here) shrink by. GROUP: keys that share
+// a page, and with it the scales.
+template <class C, int GROUP>
+__device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s, float factor, float& m, float& l) {
+    uint32_t x[128];
+    tmem_ld64_of128<0>(tmem_s, x);
+    tmem_ld64_of128<64>(tmem_s + 64, x);
+    tmem_wait_ld();
+    float top;
+    if constexpr (C::E4M3) {
+        top = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < kTile / GROUP; ++g) {
+            float most[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                most[i] = fmax_nan(u2f(x[GROUP * g + i]), u2f(x[GROUP * g + 4 + i]));
+            }
+#pragma unroll
+            for (int j = 8; j < GROUP; j += 8) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    most[i] = fmax3(most[i], u2f(x[GROUP * g + j + i]), u2f(x[GROUP * g + j + 4 + i]));
+                }
+            }
+            const float2 a = *reinterpret_cast<const float2*>(&aux.group[g * GROUP / 8]);
+            const float all = fmax_nan(fmax3(most[0], most[1], most[2]), most[3]);
+            top = fmax_nan(top, fmaf(all, fmaxf(factor * a.x, kLeastFactor), a.y));
+        }
+    } else {
+        top = row_extreme<true, 128>(x) * factor;
+    }
+    float alpha = 1.0f;
+    if (!(top <= m + kLazy)) {  // NaN among it
+        alpha = ex2_approx(m - top);
+        m = top;
+    }
+    const float used = m == -INFINITY ? 0.0f : m;
+    l *= alpha;
+    __syncwarp();  // tensor memory is accessed by whole warps
+    const bool shrinks = C::E4M3 && aux.shrinks != 0;
+#pragma unroll
+    for (int g = 0; g < kTile / GROUP; ++g) {
+        float f = factor, add = -used, inv = 1.0f, shrink = 1.0f;
+        if constexpr (C::E4M3) {
+            const float4 a = aux.group[g * GROUP / 8];
+            f = fmaxf(f * a.x, kLeastFactor);
+            add = a.y - used;
+            inv = a.z;
+            shrink = a.w;
+        }
+        const float2 f2 = make_float2(f, f), add2 = make_float2(add, add);
+        float2 sum[4];
+#pragma unroll
+        for (int i = 0; i < GROUP / 2; ++i) {
+            uint32_t* at = &x[GROUP * g + 2 * i];
+            float2 y = __ffma2_rn(make_float2(u2f(at[0]), u2f(at[1])), f2, add2);
+            y = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+            sum[i & 3] = i < 4 ? y : __fadd2_rn(sum[i & 3], y);
+            at[0] = f2u(y.x);
+            at[1] = f2u(y.y);
+        }
+        const float2 all = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
+        l = fmaf(all.x + all.y, inv, l);
+        if (shrinks) {
+#pragma unroll
+            for (int i = 0; i < GROUP; ++i) {
+                x[GROUP * g + i] = f2u(u2f(x[GROUP * g + i]) * shrink);
+            }
+        }
+        // P of 32 keys takes 16 columns.
+        if constexpr (GROUP == 32) {
+            uint32_t packed[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                packed[i] = pack2<C::kMmaBf16>(u2f(x[32 * g + 2 * i]), u2f(x[32 * g + 2 * i + 1]));
+            }
+            tmem_st16(tmem_s + 16 * g, packed);
+        } else if (g % 4 == 3) {
+            uint32_t packed[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                packed[i] = pack2<C::kMmaBf16>(u2f(x[8 * (g - 3) + 2 * i]), u2f(x[8 * (g - 3) + 2 * i + 1]));
+            }
+            tmem_st16(tmem_s + 16 * (g / 4), packed);
+        }
+    }
+    return alpha;
 }
 
 template <class C>
@@ -879,6 +1043,7 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, const Split& spli
             mbar_arrive(smem_u32(bar));
         }
     };
+    const bool coarse = p.cache.page_size >= 32;
     int tiles = 0;   // key tiles of the pieces before
     int steps = 0;   // scores taken
     Piece piece;
@@ -894,8 +1059,9 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, const Split& spli
         if (items > 0 && !wait(&sh.q_empty, items - 1)) {
             return;
         }
-        constexpr int kWords = D / 8 / (NR == 1 ? 2 : 1);
-        bring_query<C>(p, row, piece.b, head, smem + C::kSmemQ + (NR == 2 ? w * C::kTileBytes : 0), r, NR == 1 ? w * kWords : 0, kWords);
+        constexpr int kDims = D / (NR == 1 ? 2 : 1);  // NR 1: the warpgroups share the row
+        const int dim0 = NR == 1 ? w * kDims : 0;
+        bring_query<C>(p, row, piece.b, head, smem + C::kSmemQ + (NR == 2 ? w * C::kQTile : 0), r, dim0, dim0 + kDims);
         fence_proxy_async_smem();
         arrive(&sh.q_full);
         // The way up from the row's node.
@@ -938,42 +1104,26 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, const Split& spli
             // Whether all rows see all of the tile.
             const bool full = gone == 0 && key0 + kTile <= min(s.context, s.last + 1) &&
                               (p.window == 0 || key0 >= window_first(max(s.context, 0) + s.count, p.window) || key0 + kTile <= p.sinks);
-            float top = -INFINITY;
+            if (!full) {
+                // What the row does not see becomes -inf.
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-                uint32_t x[32];
-                tmem_ld32(tmem_s + 32 * c, x);
-                tmem_wait_ld();
-                if (!full) {
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t x[32];
+                    tmem_ld32(tmem_s + 32 * c, x);
+                    tmem_wait_ld();
                     const uint32_t keep = kept_columns<C>(p, s, row, key0 + 32 * c, gone >> (4 * c));
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         x[i] = (keep >> i) & 1u ? x[i] : 0xff800000u;
                     }
+                    __syncwarp();
+                    tmem_st32(tmem_s + 32 * c, x);
                 }
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    float most = fmax_nan(u2f(x[8 * g]), u2f(x[8 * g + 1]));
-                    most = fmax3(most, u2f(x[8 * g + 2]), u2f(x[8 * g + 3]));
-                    most = fmax3(most, u2f(x[8 * g + 4]), u2f(x[8 * g + 5]));
-                    most = fmax3(most, u2f(x[8 * g + 6]), u2f(x[8 * g + 7]));
-                    if constexpr (C::E4M3) {
-                        const float4 a = aux.group[4 * c + g];
-                        most = fmaf(most, fmaxf(row.factor * a.x, kLeastFactor), a.y);
-                    }
-                    top = fmax_nan(top, most);
-                }
+                tmem_wait_st();
             }
-            if constexpr (!C::E4M3) {
-                top *= row.factor;
-            }
-            float alpha = 1.0f;
-            if (!(top <= m + kLazy)) {  // NaN among it
-                alpha = ex2_approx(m - top);
-                m = top;
-            }
+            const float alpha = C::E4M3 && !coarse ? exponentials<C, 8>(aux, tmem_s, row.factor, m, l)
+                                                   : exponentials<C, 32>(aux, tmem_s, row.factor, m, l);
             if (mine > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-                l *= alpha;
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                     uint32_t x[32];
@@ -985,54 +1135,6 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, const Split& spli
                     }
                     tmem_st32(tmem_o + 32 * c, x);
                 }
-                tmem_wait_st();
-            }
-            const float used = m == -INFINITY ? 0.0f : m;
-            const bool shrinks = C::E4M3 && aux.shrinks != 0;
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-                uint32_t x[32];
-                tmem_ld32(tmem_s + 32 * c, x);
-                tmem_wait_ld();
-                if (!full) {
-                    const uint32_t keep = kept_columns<C>(p, s, row, key0 + 32 * c, gone >> (4 * c));
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        x[i] = (keep >> i) & 1u ? x[i] : 0xff800000u;
-                    }
-                }
-                uint32_t packed[16];
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    float f = row.factor, add = -used, inv = 1.0f, shrink = 1.0f;
-                    if constexpr (C::E4M3) {
-                        const float4 a = aux.group[4 * c + g];
-                        f = fmaxf(f * a.x, kLeastFactor);
-                        add = a.y - used;
-                        inv = a.z;
-                        shrink = a.w;
-                    }
-                    float2 y[4];
-                    const float2 f2 = make_float2(f, f), add2 = make_float2(add, add);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        y[i] = __ffma2_rn(make_float2(u2f(x[8 * g + 2 * i]), u2f(x[8 * g + 2 * i + 1])), f2, add2);
-                        y[i] = make_float2(ex2_approx(y[i].x), ex2_approx(y[i].y));
-                    }
-                    const float2 sum = __fadd2_rn(__fadd2_rn(y[0], y[1]), __fadd2_rn(y[2], y[3]));
-                    l = fmaf(sum.x + sum.y, inv, l);
-                    if (shrinks) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            y[i] = make_float2(y[i].x * shrink, y[i].y * shrink);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        packed[4 * g + i] = pack2<C::kMmaBf16>(y[i].x, y[i].y);
-                    }
-                }
-                tmem_st16(tmem_s + 16 * c, packed);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -1132,7 +1234,8 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, const Split& spli
 }
 
 template <class C>
-__global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ FaTreeParams p, DeviceStatus* status, unsigned epoch,
+__global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ FaTreeParams p, const __grid_constant__ CUtensorMap tm_k,
+                                                           const __grid_constant__ CUtensorMap tm_v, DeviceStatus* status, unsigned epoch,
                                                            Split split, Record rec) {
     extern __shared__ uint8_t raw[];
     uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
@@ -1143,17 +1246,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     if (threadIdx.x == 0) {
         sh.abort = 0;
         sh.odd = 0;
-        for (int i = 0; i < C::kKStages; ++i) {
-            mbar_init(smem_u32(&sh.k_full[i]), kLoadWarps / 2);
+        for (int i = 0; i < kMostStages; ++i) {
+            mbar_init(smem_u32(&sh.k_full[i]), 1);
             mbar_init(smem_u32(&sh.k_empty[i]), 1);
+            mbar_init(smem_u32(&sh.r_full[i]), 1);
+            mbar_init(smem_u32(&sh.r_empty[i]), kValueWarps);
         }
-        for (int i = 0; i < kVStages; ++i) {
-            mbar_init(smem_u32(&sh.v_full[i]), kLoadWarps / 2);
+        for (int i = 0; i < C::kVStages; ++i) {
+            mbar_init(smem_u32(&sh.v_full[i]), kValueWarps);
             mbar_init(smem_u32(&sh.v_empty[i]), 1);
         }
         for (int i = 0; i < kListed; ++i) {
             mbar_init(smem_u32(&sh.list_full[i]), 1);
-            mbar_init(smem_u32(&sh.list_empty[i]), kLoadWarps + C::NR * kSoftmaxWarps / 2);
+            mbar_init(smem_u32(&sh.list_empty[i]), kValueWarps + C::NR * kSoftmaxWarps / 2);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&sh.s_full[i]), 1);
@@ -1188,15 +1293,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         if (warp < kSoftmaxWarps) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
             softmax<C>(p, split, status, walk, sh, smem_u32(smem), rec, wctx);
-        } else if (warp < kMmaWarp) {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
-            load_tiles<C>(p, sh, smem_u32(smem), warp >= kSoftmaxWarps + kLoadWarps / 2, wctx);
         } else {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
-            if (warp == kMmaWarp) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+            if (warp < kMmaWarp) {
+                ready_values<C>(p, sh, smem_u32(smem), wctx);
+            } else if (warp == kMmaWarp) {
                 issue_products<C>(p, split, walk, sh, smem_u32(smem), wctx);
-            } else {
-                list_tiles<C>(p, split, status, walk, sh, warp - kListWarp, wctx);
+            } else if (warp < kListWarp + kListWarps) {
+                list_tiles<C>(p, &tm_k, &tm_v, split, status, walk, sh, smem_u32(smem), warp - kListWarp, wctx);
+                // Copies in flight end by themselves; after a wait that was given up they get a millisecond.
+                if (sh.abort != 0) {
+                    const unsigned long long t0 = globaltimer_ns();
+                    while (globaltimer_ns() - t0 < 1000000ull) {
+                    }
+                }
             }
         }
     }
@@ -1335,6 +1445,28 @@ __global__ void __launch_bounds__(kRowWarps * 32) tree_finish_kernel(const __gri
     }
 }
 
+// A map of k or v over {head dim, slot, head, page}: boxes of a page's tokens, at most a tile of them.
+CUresult encode_pool_map(CUtensorMap* map, const FaCache& c, void* base, const int64_t (&stride)[2], bool bf16, CUtensorMapSwizzle swizzle) {
+    auto fn = tensor_map_encoder();
+    if (fn == nullptr) {
+        return CUDA_ERROR_NOT_SUPPORTED;
+    }
+    const bool e4m3 = c.dtype == FA_DTYPE_FLOAT8_E4M3;
+    const cuuint64_t elem = e4m3 ? 1 : 2;
+    const cuuint64_t row = c.head_dim * elem;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_size),
+                                static_cast<cuuint64_t>(c.kv_heads), static_cast<cuuint64_t>(c.num_pages)};
+    // The stride of a dim of one element is never used and may be 0.
+    const cuuint64_t strides[3] = {row, c.kv_heads > 1 ? static_cast<cuuint64_t>(stride[1]) * elem : row,
+                                   c.num_pages > 1 ? static_cast<cuuint64_t>(stride[0]) * elem : row};
+    const cuuint32_t box[4] = {e4m3 ? static_cast<cuuint32_t>(c.head_dim) : 64u, static_cast<cuuint32_t>(std::min(c.page_size, kTile)), 1, 1};
+    const cuuint32_t elem_strides[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type = e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                          : (bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
+    return fn(map, type, 4, base, dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
 // Launches after the kernel before it has started to end: it waits for its results itself.
 template <class... Params, class... Args>
 cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, const Args&... args) {
@@ -1392,7 +1524,14 @@ cudaError_t launch(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, 
         odd = reinterpret_cast<int*>(rec.ml + rows);
     }
     rec.odd = p.cache.tokens > 1 ? odd : nullptr;
-    kernel<<<static_cast<unsigned>(split.grid), kThreads, smem_bytes<C>(), stream>>>(p, status, epoch, split, rec);
+    CUtensorMap tm_k, tm_v;
+    const CUtensorMapSwizzle raw_k = C::E4M3 && C::D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+    const CUtensorMapSwizzle raw_v = C::E4M3 && C::D == 64 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
+    if (encode_pool_map(&tm_k, p.cache, p.cache.k, p.cache.k_stride, C::BF16, raw_k) != CUDA_SUCCESS ||
+        encode_pool_map(&tm_v, p.cache, p.cache.v, p.cache.v_stride, C::BF16, raw_v) != CUDA_SUCCESS) {
+        return cudaErrorInvalidValue;
+    }
+    kernel<<<static_cast<unsigned>(split.grid), kThreads, smem_bytes<C>(), stream>>>(p, tm_k, tm_v, status, epoch, split, rec);
     err = cudaGetLastError();
     const int joins = split.whole ? 0 : split.grid - 1;
     const int fixers = rec.odd != nullptr ? kFixers : 0;
