@@ -46,6 +46,7 @@ static_assert(2 * kRegsSoftmax + 2 * kRegsOther <= 4 * 128, "no more than the la
 constexpr int kListed = 4;           // key tiles listed ahead
 constexpr int kGroups = kTile / 8;   // keys that surely share a page
 constexpr int kMostStages = 4;
+constexpr int kParts = 4;  // pieces listed ahead
 
 template <int D_, bool BF16_, bool E4M3_, int NR_>
 struct Cfg {
@@ -83,10 +84,22 @@ struct Listed {             // a key tile
     uint32_t gone;          // bits of groups that are shown and have no page
     uint32_t shrinks;       // of groups whose P shrinks
     int mixed;              // rows may differ in what they see
+    int full;               // all rows see all of it
+};
+
+// A piece of an item, for the softmax and the products: what its walk would keep in their registers.
+struct Part {
+    int n;  // key tiles; 0: the end
+    int b, kvh, block;
+    int record;           // -1: a whole item
+    int context, count;   // of its sequence
+    int last;
 };
 
 struct Shared {
     Listed list[kListed];
+    Part part[kParts];
+    uint64_t part_full[kParts], part_empty[kParts];
     uint64_t list_full[kListed], list_empty[kListed];
     uint64_t k_full[kMostStages], k_empty[kMostStages], v_full[2], v_empty[2], r_full[kMostStages], r_empty[kMostStages];
     uint64_t s_full[2], p_full[2];
@@ -486,6 +499,7 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensor
     int n = -1;  // the tile at hand
     int v = -1;
     int turn = which;  // the tile that is this warp's
+    int parts = 0;
     auto wait = [&](uint64_t* bar, int phase) {
         return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), (phase & 1) ^ 1, wctx, kStatusTimeoutProducer)) != 0;
     };
@@ -494,6 +508,25 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensor
         if (++v >= piece.v1) {
             more = next_piece(p, split, walk, piece, s);
             v = piece.v0;
+            if (which == 0) {
+                Part& to = sh.part[parts % kParts];
+                if (!wait(&sh.part_empty[parts % kParts], parts / kParts)) {
+                    return;
+                }
+                if (lane == 0) {
+                    to.n = more ? piece.v1 - piece.v0 : 0;
+                    to.b = piece.b;
+                    to.kvh = piece.kvh;
+                    to.block = piece.block;
+                    to.record = piece.record;
+                    to.context = s.context;
+                    to.count = s.count;
+                    to.last = s.last;
+                    mbar_arrive(smem_u32(&sh.part_full[parts % kParts]));
+                }
+                __syncwarp();
+                ++parts;
+            }
         }
         if (++n != turn) {
             if (!more) {
@@ -588,7 +621,9 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensor
             to.key0 = key0;
             to.gone = gone;
             to.shrinks = shrink;
-            to.mixed = c.tokens > 1 && (key0 + kTile > s.context || (p.window > 0 && key0 < window_first(max(s.context, 0) + s.count, p.window)));
+            const int near = window_first(max(s.context, 0) + s.count, p.window);
+            to.mixed = c.tokens > 1 && (key0 + kTile > s.context || (p.window > 0 && key0 < near));
+            to.full = gone == 0 && key0 + kTile <= min(s.context, s.last + 1) && (p.window == 0 || key0 >= near || key0 + kTile <= p.sinks);
         }
         __syncwarp();
         if (lane == 0) {
@@ -738,8 +773,7 @@ __device__ __forceinline__ void issue_product(uint32_t acc, uint32_t w, uint64_t
 // Products, in the order in which scores and P take each other's place: S(s + 2) after P(s) V. Step s is key tile s (NR 1)
 // or row tile s % 2 of key tile s / 2 (NR 2).
 template <class C>
-__device__ __forceinline__ void issue_products(const FaTreeParams& p, const Split& split, Walk walk, Shared& sh, uint32_t smem,
-                                               const WaitCtx& wctx) {
+__device__ __forceinline__ void issue_products(Shared& sh, uint32_t smem, const WaitCtx& wctx) {
     constexpr int NR = C::NR;
     auto kmajor = [](uint32_t at) { return C::E4M3 && C::D == 64 ? make_desc_kmajor_sw64(at) : make_desc_kmajor_sw128(at); };
     const uint64_t q = kmajor(smem + C::kSmemQ);
@@ -754,10 +788,17 @@ __device__ __forceinline__ void issue_products(const FaTreeParams& p, const Spli
     bool ok = true;
     int tiles = 0;  // key tiles of the pieces before
     int taken0 = 0, taken1 = 0;  // P of either warpgroup
-    Piece piece;
-    Sequence s;
-    for (int items = 0; ok && next_piece(p, split, walk, piece, s); ++items) {
-        const int n = piece.v1 - piece.v0;
+    for (int items = 0; ok; ++items) {
+        ok = wait(&sh.part_full[items % kParts], items / kParts);
+        const int n = ok ? sh.part[items % kParts].n : 0;
+        if (n == 0) {
+            break;
+        }
+        __syncwarp();
+        if (elect_one()) {
+            mbar_arrive(smem_u32(&sh.part_empty[items % kParts]));
+        }
+        __syncwarp();
         const int steps = n * NR;
         auto scores = [&](int step) {
             const int tile = tiles + (NR == 1 ? step : step >> 1);
@@ -830,83 +871,98 @@ struct Row {
     float factor;       // of a score, in log2 units
 };
 
-// A row's own part of Q's tile, 16 dims at a time from dim `from` on: as it is, or, over an e4m3 cache, as the sum of e4m3
-// terms (each the nearest to what the ones before leave), brought to [2^8, 448) by a power of two that `factor` takes
-// back. The terms hold bfloat16 and float16 exactly, down to multiples of 2^-10 beside a largest value of 2^8 or more.
+// A warp's 32 rows of Q's tile, some rows at a time, 16 dims a lane: as they are, or, over an e4m3 cache, as sums of e4m3
+// terms (each the nearest to what the ones before leave), a row brought to [2^8, 448] by a power of two that its `factor` takes
+// back. The terms hold bfloat16 and float16 exactly, down to multiples of 2^-10 beside that largest value. NR 1: the
+// warpgroups share the rows, each stores half of the dims.
 template <class C>
-__device__ __forceinline__ void bring_query(const FaTreeParams& p, Row& row, int b, int head, uint32_t tile, int r, int from, int to) {
-    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] +
-                                                      head * p.q_stride[1] + row.token * p.q_stride[2]);
+__device__ __forceinline__ void bring_queries(const FaTreeParams& p, Row& row, int b, int head, uint32_t tile, int quarter, int w) {
+    constexpr int kLanes = C::D / 16;      // of a row
+    constexpr int kAtOnce = 32 / kLanes;   // rows
+    constexpr int kPasses = kLanes;
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    const int part = lane % kLanes;
+    const bool mine = C::NR == 2 || part / (kLanes / 2) == w;
+    const uint16_t* from = static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] + head * p.q_stride[1] + row.token * p.q_stride[2];
     const uint32_t sign = p.softmax_scale < 0.0f ? 0x80008000u : 0u;  // the factor stays positive
     row.factor = fmaxf(fabsf(p.softmax_scale) * kLog2e, kLeastFactor);
-    auto words = [&](int i, uint32_t (&x)[4]) {
-        const uint4 w = row.real ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
-        x[0] = w.x ^ sign;
-        x[1] = w.y ^ sign;
-        x[2] = w.z ^ sign;
-        x[3] = w.w ^ sign;
-    };
-    if constexpr (!C::E4M3) {
-#pragma unroll 4
-        for (int i = from / 8; i < to / 8; ++i) {
-            uint32_t x[4];
-            words(i, x);
-            store_shared16(tile + tile_offset(r, i), x[0], x[1], x[2], x[3]);
-        }
-        return;
-    }
-    uint32_t top = 0;  // of the values' bits without sign: their order is that of the sizes
-#pragma unroll 4
-    for (int i = 0; i < C::D / 8; ++i) {
-        uint32_t x[4];
-        words(i, x);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            top = max(top, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
-        }
-    }
-    // 2^(8 - exponent of the largest), one less where that would pass 448, both it and its inverse normal; 1 for zeros, inf and NaN.
-    const float most = widen16<C::BF16>(static_cast<uint16_t>(top));
-    const int e = static_cast<int>(__float_as_uint(most) >> 23);
-    const int shift = (e == 0 || e == 255) ? 0 : min(max(135 - e - ((__float_as_uint(most) & 0x7fffffu) > 0x600000u ? 1 : 0), -100), 100);
-    const float up = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
-    row.factor = fmaxf(row.factor * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23), kLeastFactor);
 #pragma unroll 1
-    for (int c = from / 16; c < to / 16; ++c) {
-        float f[16];
+    for (int pass0 = 0; pass0 < kPasses; pass0 += 4) {
+        uint4 word[4][2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            uint32_t x[4];
-            words(2 * c + half, x);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                f[8 * half + 2 * i] = widen16<C::BF16>(static_cast<uint16_t>(x[i] & 0xffffu)) * up;
-                f[8 * half + 2 * i + 1] = widen16<C::BF16>(static_cast<uint16_t>(x[i] >> 16)) * up;
-            }
+        for (int i = 0; i < 4; ++i) {
+            const int owner = (pass0 + i) * kAtOnce + lane / kLanes;
+            const uint64_t at = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(from), owner);
+            const bool real = __shfl_sync(0xffffffffu, static_cast<int>(row.real), owner) != 0;
+            const uint4* src = reinterpret_cast<const uint4*>(at) + 2 * part;
+            word[i][0] = real ? __ldg(src) : make_uint4(0u, 0u, 0u, 0u);
+            word[i][1] = real ? __ldg(src + 1) : make_uint4(0u, 0u, 0u, 0u);
         }
 #pragma unroll
-        for (int term = 0; term < C::kTerms; ++term) {
-            uint32_t w[4];
+        for (int i = 0; i < 4; ++i) {
+            const int owner = (pass0 + i) * kAtOnce + lane / kLanes;
+            const int r = quarter * 32 + owner;
+            const uint32_t x[8] = {word[i][0].x ^ sign, word[i][0].y ^ sign, word[i][0].z ^ sign, word[i][0].w ^ sign,
+                                   word[i][1].x ^ sign, word[i][1].y ^ sign, word[i][1].z ^ sign, word[i][1].w ^ sign};
+            if constexpr (!C::E4M3) {
+                if (mine) {
+                    store_shared16(tile + tile_offset(r, 2 * part), x[0], x[1], x[2], x[3]);
+                    store_shared16(tile + tile_offset(r, 2 * part + 1), x[4], x[5], x[6], x[7]);
+                }
+            } else {
+                uint32_t top = 0;  // of the values' bits without sign: their order is that of the sizes
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t lo = pack_e4m3x2(f[4 * i], f[4 * i + 1]);
-                const uint32_t hi = pack_e4m3x2(f[4 * i + 2], f[4 * i + 3]);
-                w[i] = lo | (hi << 16);
-                const float2 a = unpack_half2(e4m3x2_to_half2(lo));
-                const float2 b2 = unpack_half2(e4m3x2_to_half2(hi));
-                f[4 * i] -= a.x;
-                f[4 * i + 1] -= a.y;
-                f[4 * i + 2] -= b2.x;
-                f[4 * i + 3] -= b2.y;
+                for (int e = 0; e < 8; ++e) {
+                    top = max(top, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
+                }
+#pragma unroll
+                for (int o = 1; o < kLanes; o <<= 1) {
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                }
+                // 2^(8 - exponent of the largest), one less where that would pass 448, both it and its inverse normal; 1
+                // for zeros, inf and NaN.
+                const uint32_t most = __float_as_uint(widen16<C::BF16>(static_cast<uint16_t>(top)));
+                const int e = static_cast<int>(most >> 23);
+                const int shift = (e == 0 || e == 255) ? 0 : min(max(135 - e - ((most & 0x7fffffu) > 0x600000u ? 1 : 0), -100), 100);
+                const float up = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+                // The row's thread takes it back.
+                const int row_shift = __shfl_sync(0xffffffffu, shift, (lane % kAtOnce) * kLanes);
+                if (lane / kAtOnce == pass0 + i) {
+                    row.factor = fmaxf(row.factor * __uint_as_float(static_cast<uint32_t>(127 - row_shift) << 23), kLeastFactor);
+                }
+                float f[16];
+#pragma unroll
+                for (int e2 = 0; e2 < 8; ++e2) {
+                    f[2 * e2] = widen16<C::BF16>(static_cast<uint16_t>(x[e2] & 0xffffu)) * up;
+                    f[2 * e2 + 1] = widen16<C::BF16>(static_cast<uint16_t>(x[e2] >> 16)) * up;
+                }
+#pragma unroll
+                for (int term = 0; term < C::kTerms; ++term) {
+                    uint32_t code[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t lo = pack_e4m3x2(f[4 * j], f[4 * j + 1]);
+                        const uint32_t hi = pack_e4m3x2(f[4 * j + 2], f[4 * j + 3]);
+                        code[j] = lo | (hi << 16);
+                        const float2 u = unpack_half2(e4m3x2_to_half2(lo));
+                        const float2 v = unpack_half2(e4m3x2_to_half2(hi));
+                        f[4 * j] -= u.x;
+                        f[4 * j + 1] -= u.y;
+                        f[4 * j + 2] -= v.x;
+                        f[4 * j + 3] -= v.y;
+                    }
+                    if (mine) {
+                        store_shared16(tile + term * C::kRaw + code_offset<C::D>(r, part), code[0], code[1], code[2], code[3]);
+                    }
+                }
             }
-            store_shared16(tile + term * C::kRaw + code_offset<C::D>(r, c), w[0], w[1], w[2], w[3]);
         }
     }
 }
 
 // 32 columns of scores, keys from kb on: those that the row does not see become -inf.
 template <class C>
-__device__ __forceinline__ uint32_t kept_columns(const FaTreeParams& p, const Sequence& s, const Row& row, int kb, uint32_t gone) {
+__device__ __forceinline__ uint32_t kept_columns(const FaTreeParams& p, const Part& s, const Row& row, int kb, uint32_t gone) {
     uint32_t keep = bits_up_to(min(s.context - 1, s.last) - kb);
     if (p.window > 0) {
         keep &= ~bits_up_to(row.first - 1 - kb) | bits_up_to(p.sinks - 1 - kb);
@@ -1019,8 +1075,8 @@ __device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s
 }
 
 template <class C>
-__device__ __forceinline__ void softmax(const FaTreeParams& p, const Split& split, DeviceStatus* status, Walk walk, Shared& sh,
-                                        uint32_t smem, const Record& rec, const WaitCtx& wctx) {
+__device__ __forceinline__ void softmax(const FaTreeParams& p, DeviceStatus* status, Shared& sh, uint32_t smem, const Record& rec,
+                                        const WaitCtx& wctx) {
     constexpr int D = C::D;
     constexpr int NR = C::NR;
     const int lane = static_cast<int>(threadIdx.x) % 32;
@@ -1046,22 +1102,24 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, const Split& spli
     const bool coarse = p.cache.page_size >= 32;
     int tiles = 0;   // key tiles of the pieces before
     int steps = 0;   // scores taken
-    Piece piece;
-    Sequence s;
-    for (int items = 0; next_piece(p, split, walk, piece, s); ++items) {
-        const int n = piece.v1 - piece.v0;
-        const int row_index = piece.block * C::kRows + (NR == 2 ? w * kTile : 0) + r;
+    for (int items = 0;; ++items) {
+        if (!wait(&sh.part_full[items % kParts], items / kParts)) {
+            return;
+        }
+        const Part& s = sh.part[items % kParts];  // until the end of the piece
+        const int n = s.n;
+        if (n == 0) {
+            return;
+        }
+        const int row_index = s.block * C::kRows + (NR == 2 ? w * kTile : 0) + r;
         Row row;
         row.head = row_index / p.cache.tokens;
         row.token = row_index - row.head * p.cache.tokens;
         row.real = row_index < rows && row.token < s.count;
-        const int head = piece.kvh * group + row.head;
         if (items > 0 && !wait(&sh.q_empty, items - 1)) {
             return;
         }
-        constexpr int kDims = D / (NR == 1 ? 2 : 1);  // NR 1: the warpgroups share the row
-        const int dim0 = NR == 1 ? w * kDims : 0;
-        bring_query<C>(p, row, piece.b, head, smem + C::kSmemQ + (NR == 2 ? w * C::kQTile : 0), r, dim0, dim0 + kDims);
+        bring_queries<C>(p, row, s.b, s.kvh * group + row.head, smem + C::kSmemQ + (NR == 2 ? w * C::kQTile : 0), warp % 4, w);
         fence_proxy_async_smem();
         arrive(&sh.q_full);
         // The way up from the row's node.
@@ -1071,7 +1129,7 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, const Split& spli
             row.mask[i] = 0;
         }
         if (row.real) {
-            const int32_t* parents = p.parents + piece.b * p.parent_stride;
+            const int32_t* parents = p.parents + s.b * p.parent_stride;
             int at = row.token;
             bool bad = false;
 #pragma unroll
@@ -1093,18 +1151,15 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, const Split& spli
         float m = -INFINITY, l = 0.0f;
         int mine = 0;  // scores of this piece taken
         for (int t = NR == 1 ? w : 0; t < n; t += NR == 1 ? 2 : 1, ++mine) {
-            const int key0 = tile_key(s, piece.v0 + t);
             const int slot = (tiles + t) % kListed;
             if (!wait(&sh.list_full[slot], (tiles + t) / kListed) || !wait(&sh.s_full[w], steps)) {
                 return;
             }
             ++steps;
             const Listed& aux = sh.list[slot];
-            const uint32_t gone = aux.gone;
-            // Whether all rows see all of the tile.
-            const bool full = gone == 0 && key0 + kTile <= min(s.context, s.last + 1) &&
-                              (p.window == 0 || key0 >= window_first(max(s.context, 0) + s.count, p.window) || key0 + kTile <= p.sinks);
-            if (!full) {
+            if (aux.full == 0) {
+                const int key0 = aux.key0;
+                const uint32_t gone = aux.gone;
                 // What the row does not see becomes -inf.
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
@@ -1185,20 +1240,21 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, const Split& spli
         const bool self = NR == 2 || w == 0 || n > 1;  // this one does
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const bool in_rows = row_index < rows;
-        const int64_t out_row = (static_cast<int64_t>(piece.b) * p.heads + head) * p.cache.tokens + row.token;
-        const int64_t record_row = static_cast<int64_t>(piece.record) * C::kRows + (NR == 2 ? w * kTile : 0) + r;
+        const int64_t out_row = (static_cast<int64_t>(s.b) * p.heads + s.kvh * group + row.head) * p.cache.tokens + row.token;
+        const int record = s.record;
+        const int64_t record_row = static_cast<int64_t>(record) * C::kRows + (NR == 2 ? w * kTile : 0) + r;
 #pragma unroll 1
-        for (int c = 0; c < kColumns / 16; ++c) {
-            uint32_t x[16], y[16];
+        for (int c = 0; c < kColumns / 32; ++c) {
+            uint32_t x[32], y[32];
             if (self) {
-                tmem_ld16(own + 16 * c, x);
+                tmem_ld32(own + 32 * c, x);
             }
             if (NR == 1 && (both || !self)) {
-                tmem_ld16(theirs + 16 * c, y);
+                tmem_ld32(theirs + 32 * c, y);
             }
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < 32; ++i) {
                 float z = self ? u2f(x[i]) * weight[0] : 0.0f;
                 if (NR == 1 && (both || !self)) {
                     z = fmaf(u2f(y[i]), weight[1], z);
@@ -1208,28 +1264,29 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, const Split& spli
             if (!in_rows) {
                 continue;
             }
-            if (piece.record < 0) {
-                uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + out_row * D + column0 + 16 * c);
+            if (record < 0) {
+                uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + out_row * D + column0 + 32 * c);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < 4; ++i) {
                     to[i] = make_uint4(pack2<C::BF16>(u2f(x[8 * i]) * inv, u2f(x[8 * i + 1]) * inv),
                                        pack2<C::BF16>(u2f(x[8 * i + 2]) * inv, u2f(x[8 * i + 3]) * inv),
                                        pack2<C::BF16>(u2f(x[8 * i + 4]) * inv, u2f(x[8 * i + 5]) * inv),
                                        pack2<C::BF16>(u2f(x[8 * i + 6]) * inv, u2f(x[8 * i + 7]) * inv));
                 }
             } else {
-                uint4* to = reinterpret_cast<uint4*>(rec.o + record_row * D + column0 + 16 * c);
+                uint4* to = reinterpret_cast<uint4*>(rec.o + record_row * D + column0 + 32 * c);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 8; ++i) {
                     to[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
                 }
             }
         }
-        if (piece.record >= 0 && in_rows && (NR == 2 || w == 0)) {
+        if (record >= 0 && in_rows && (NR == 2 || w == 0)) {
             rec.ml[record_row] = row.real ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
         }
         tc_fence_before();
         arrive(&sh.o_free);
+        arrive(&sh.part_empty[items % kParts]);
     }
 }
 
@@ -1260,6 +1317,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             mbar_init(smem_u32(&sh.list_full[i]), 1);
             mbar_init(smem_u32(&sh.list_empty[i]), kValueWarps + C::NR * kSoftmaxWarps / 2);
         }
+        for (int i = 0; i < kParts; ++i) {
+            mbar_init(smem_u32(&sh.part_full[i]), 1);
+            mbar_init(smem_u32(&sh.part_empty[i]), kSoftmaxWarps + 1);
+        }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&sh.s_full[i]), 1);
             mbar_init(smem_u32(&sh.p_full[i]), kSoftmaxWarps / 2);
@@ -1289,17 +1350,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             atomicOr(&status->code, kStatusTimeoutTeardown);
         }
     } else {
-        const Walk walk = start_walk(p, split, range, static_cast<int>(blockIdx.x));
         if (warp < kSoftmaxWarps) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-            softmax<C>(p, split, status, walk, sh, smem_u32(smem), rec, wctx);
+            softmax<C>(p, status, sh, smem_u32(smem), rec, wctx);
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
             if (warp < kMmaWarp) {
                 ready_values<C>(p, sh, smem_u32(smem), wctx);
             } else if (warp == kMmaWarp) {
-                issue_products<C>(p, split, walk, sh, smem_u32(smem), wctx);
+                issue_products<C>(sh, smem_u32(smem), wctx);
             } else if (warp < kListWarp + kListWarps) {
+                const Walk walk = start_walk(p, split, range, static_cast<int>(blockIdx.x));
                 list_tiles<C>(p, &tm_k, &tm_v, split, status, walk, sh, smem_u32(smem), warp - kListWarp, wctx);
                 // Copies in flight end by themselves; after a wait that was given up they get a millisecond.
                 if (sh.abort != 0) {
