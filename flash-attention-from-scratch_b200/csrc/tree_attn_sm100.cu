@@ -20,7 +20,7 @@ namespace fa_sm100 {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100: smaller scales of values enter as this, with P scaled down
+constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100: values of smaller scales (below 2^-91) count as zeros
 constexpr float kLeastFactor = 1e-37f;               // of a score: what is hidden (-inf) stays so
 constexpr float kLazy = 8.0f;                        // P is at most 2^this before O and the sum are rescaled
 constexpr int kMostNodes = 256;
@@ -36,6 +36,7 @@ constexpr int kListWarp = kMmaWarp + 1;  // and the one after it: the list of ke
 // Tiles are the list warps' in turn. A warp that waits for a ring's slot has seen the slot `kListWarps` tiles before it
 // consumed; with no more warps than a ring has slots the phase it waits for is then never two behind.
 constexpr int kListWarps = 2;
+constexpr int kPartWarp = kListWarp + kListWarps;  // the list of pieces
 constexpr int kWarps = kMmaWarp + 4;  // whole warpgroups: registers are handed over between those
 constexpr int kThreads = kWarps * 32;
 // Registers: launched with 128 a thread, 512 for a lane of the four warpgroups.
@@ -78,11 +79,11 @@ struct Cfg {
 };
 
 struct Listed {             // a key tile
-    float4 group[kGroups];  // e4m3: K's scale, log2 of V's, 1 / V's, what P shrinks by
+    float4 group[kGroups];  // e4m3: K's scale, log2 of V's, 1 / V's
     uint4 shown;            // bits of the rows that some row of the call sees and that have a page
     int key0;               // first position; -1: the list's end
     uint32_t gone;          // bits of groups that are shown and have no page
-    uint32_t shrinks;       // of groups whose P shrinks
+    uint32_t tiny;          // bits of groups whose values count as zeros
     int mixed;              // rows may differ in what they see
     int full;               // all rows see all of it
 };
@@ -94,9 +95,10 @@ struct Part {
     int record;           // -1: a whole item
     int context, count;   // of its sequence
     int last;
+    uint8_t up[kMostNodes];  // nodes' parents, 255 for none
 };
 
-struct Shared {
+struct alignas(16) Shared {
     Listed list[kListed];
     Part part[kParts];
     uint64_t part_full[kParts], part_empty[kParts];
@@ -112,9 +114,17 @@ struct Shared {
     int odd;
 };
 
+// NR 1: what the warpgroups tell each other of the rows they share.
+struct Exchange {
+    float factor[2][kTile];  // of two items in turn
+    float2 ml[2][kTile];
+};
+
 template <class C>
 constexpr int smem_bytes() {
-    return C::kSmemShared + static_cast<int>(sizeof(Shared)) + 1024;  // the tiles begin on 1024 bytes
+    constexpr int bytes = C::kSmemShared + static_cast<int>(sizeof(Shared)) + (C::NR == 1 ? static_cast<int>(sizeof(Exchange)) : 0);
+    static_assert(bytes <= 227 * 1024 && sizeof(Shared) % 16 == 0);
+    return bytes;
 }
 
 template <bool BF16>
@@ -314,7 +324,7 @@ struct Split {
 };
 
 struct Record {
-    float* o;    // [2 grid][rows of an item][D]
+    float* o;    // [2 grid][D / 4][rows of an item][4]
     float2* ml;  // [2 grid][rows of an item]
     int* odd;    // [grid]: values that are not finite where some rows do not see them
 };
@@ -499,7 +509,6 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensor
     int n = -1;  // the tile at hand
     int v = -1;
     int turn = which;  // the tile that is this warp's
-    int parts = 0;
     auto wait = [&](uint64_t* bar, int phase) {
         return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), (phase & 1) ^ 1, wctx, kStatusTimeoutProducer)) != 0;
     };
@@ -508,25 +517,6 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensor
         if (++v >= piece.v1) {
             more = next_piece(p, split, walk, piece, s);
             v = piece.v0;
-            if (which == 0) {
-                Part& to = sh.part[parts % kParts];
-                if (!wait(&sh.part_empty[parts % kParts], parts / kParts)) {
-                    return;
-                }
-                if (lane == 0) {
-                    to.n = more ? piece.v1 - piece.v0 : 0;
-                    to.b = piece.b;
-                    to.kvh = piece.kvh;
-                    to.block = piece.block;
-                    to.record = piece.record;
-                    to.context = s.context;
-                    to.count = s.count;
-                    to.last = s.last;
-                    mbar_arrive(smem_u32(&sh.part_full[parts % kParts]));
-                }
-                __syncwarp();
-                ++parts;
-            }
         }
         if (++n != turn) {
             if (!more) {
@@ -596,18 +586,17 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensor
         if (!wait(&sh.list_empty[n % kListed], n / kListed)) {
             return;
         }
-        bool shrinks = false;
+        bool tiny = false;
         if constexpr (C::E4M3) {
-            const float used = fmaxf(vs, kMinScale);
-            const float inv = __fdividef(1.0f, used);
-            shrinks = vs < kMinScale;
+            tiny = vs < kMinScale;
+            const float used = tiny ? kMinScale : vs;
             if (lane < kGroups) {
-                to.group[lane] = make_float4(ks, __log2f(used), inv, shrinks ? vs * inv : 1.0f);
+                to.group[lane] = make_float4(ks, __log2f(used), __fdividef(1.0f, used), 0.0f);
             }
         }
         const uint32_t paged = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
         const uint32_t gone = __ballot_sync(0xffffffffu, wanted && page < 0) & 0xffffu;
-        const uint32_t shrink = __ballot_sync(0xffffffffu, shrinks) & 0xffffu;
+        const uint32_t tiny_bits = __ballot_sync(0xffffffffu, tiny) & 0xffffu;
         if (lane < 4) {
             const int kb = key0 + 32 * lane;
             uint32_t bits = bits_up_to(s.last - kb) & (~bits_up_to(s.first - 1 - kb) | bits_up_to(p.sinks - 1 - kb));
@@ -620,7 +609,7 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensor
         if (lane == 0) {
             to.key0 = key0;
             to.gone = gone;
-            to.shrinks = shrink;
+            to.tiny = tiny_bits;
             const int near = window_first(max(s.context, 0) + s.count, p.window);
             to.mixed = c.tokens > 1 && (key0 + kTile > s.context || (p.window > 0 && key0 < near));
             to.full = gone == 0 && key0 + kTile <= min(s.context, s.last + 1) && (p.window == 0 || key0 >= near || key0 + kTile <= p.sinks);
@@ -628,6 +617,51 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensor
         __syncwarp();
         if (lane == 0) {
             mbar_arrive(smem_u32(&sh.list_full[n % kListed]));
+        }
+    }
+}
+
+// The range's pieces, listed for the softmax and the products.
+__device__ __forceinline__ void list_parts(const FaTreeParams& p, const Split& split, DeviceStatus* status, Walk walk, Shared& sh,
+                                           const WaitCtx& wctx) {
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    Piece piece;
+    Sequence s;
+    for (int n = 0;; ++n) {
+        const bool more = next_piece(p, split, walk, piece, s);
+        Part& to = sh.part[n % kParts];
+        const bool ok = mbar_wait(smem_u32(&sh.part_empty[n % kParts]), ((n / kParts) & 1) ^ 1, wctx, kStatusTimeoutProducer);
+        if (__all_sync(0xffffffffu, ok) == 0) {
+            return;
+        }
+        if (more) {
+            const int32_t* parents = p.parents + piece.b * p.parent_stride;
+            bool bad = s.count > 0 && (s.context < 0 || s.context > held(p.cache) - s.count);
+            for (int t = lane; t < s.count; t += 32) {
+                const int up = __ldg(parents + t);
+                bad = bad || up < -1 || up >= t;
+                to.up[t] = up < 0 || up >= t ? 255 : static_cast<uint8_t>(up);
+            }
+            if (bad) {
+                atomicOr(&status->code, kStatusBadPage);
+            }
+        }
+        if (lane == 0) {
+            to.n = more ? piece.v1 - piece.v0 : 0;
+            to.b = piece.b;
+            to.kvh = piece.kvh;
+            to.block = piece.block;
+            to.record = piece.record;
+            to.context = s.context;
+            to.count = s.count;
+            to.last = s.last;
+        }
+        __syncwarp();
+        if (lane == 0) {
+            mbar_arrive(smem_u32(&sh.part_full[n % kParts]));
+        }
+        if (!more) {
+            return;
         }
     }
 }
@@ -654,6 +688,7 @@ __device__ __forceinline__ void ready_values(const FaTreeParams& p, Shared& sh, 
             break;
         }
         const bool mixed = t.mixed != 0;
+        [[maybe_unused]] const uint32_t tiny = t.tiny;
         const bool whole = (t.shown.x & t.shown.y & t.shown.z & t.shown.w) == 0xffffffffu;
         const uint32_t* shown = reinterpret_cast<const uint32_t*>(&t.shown);
         if (!wait(&sh.r_full[n % kRing], n / kRing)) {
@@ -686,12 +721,17 @@ __device__ __forceinline__ void ready_values(const FaTreeParams& p, Shared& sh, 
                         w[i] = load_shared16(raw + r[i] * 64 + chunk * 16);
                     }
                 }
-                if (mixed || !whole) {
+                if (mixed || !whole || tiny != 0) {
                     uint32_t any = 0;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if (!((shown[r[i] >> 5] >> (r[i] & 31)) & 1u)) {
                             w[i] = make_uint4(0u, 0u, 0u, 0u);
+                        } else if ((tiny >> (r[i] >> 3)) & 1u) {  // NaN stays
+                            w[i].x &= (not_finite<C>(w[i].x) >> 7) * 255u;
+                            w[i].y &= (not_finite<C>(w[i].y) >> 7) * 255u;
+                            w[i].z &= (not_finite<C>(w[i].z) >> 7) * 255u;
+                            w[i].w &= (not_finite<C>(w[i].w) >> 7) * 255u;
                         }
                         any |= not_finite<C>(w[i].x) | not_finite<C>(w[i].y) | not_finite<C>(w[i].z) | not_finite<C>(w[i].w);
                     }
@@ -865,99 +905,102 @@ __device__ __forceinline__ void issue_products(Shared& sh, uint32_t smem, const 
 // A thread's query row.
 struct Row {
     bool real;          // a node's (else padding, or beyond the rows)
-    int head, token;    // head of the group
+    int token;
     uint32_t mask[kMaskWords];  // the node and its ancestors
     int first;          // first position of its window
     float factor;       // of a score, in log2 units
 };
 
-// A warp's 32 rows of Q's tile, some rows at a time, 16 dims a lane: as they are, or, over an e4m3 cache, as sums of e4m3
-// terms (each the nearest to what the ones before leave), a row brought to [2^8, 448] by a power of two that its `factor` takes
-// back. The terms hold bfloat16 and float16 exactly, down to multiples of 2^-10 beside that largest value. NR 1: the
-// warpgroups share the rows, each stores half of the dims.
-template <class C>
-__device__ __forceinline__ void bring_queries(const FaTreeParams& p, Row& row, int b, int head, uint32_t tile, int quarter, int w) {
-    constexpr int kLanes = C::D / 16;      // of a row
-    constexpr int kAtOnce = 32 / kLanes;   // rows
-    constexpr int kPasses = kLanes;
+// A warp's rows of Q's tile (NR 1: half of its 32, the other warpgroup has the others), 16 dims a lane: as they are, or, over
+// an e4m3 cache, as sums of e4m3 terms (each the nearest to what the ones before leave), a row brought to [2^8, 448] by a
+// power of two that its factor takes back. The terms hold bfloat16 and float16 exactly, down to multiples of 2^-10 beside
+// that largest value. `at`, `real`: the lane's own row; ready() waits until the tile may be written. Returns the factor of the lane's
+// own row (NR 1: in `factors` by row, for both warpgroups).
+template <class C, class Ready>
+__device__ __forceinline__ float bring_queries(const FaTreeParams& p, const uint16_t* at, bool real, uint32_t tile, int quarter, int w,
+                                               float* factors, Ready ready) {
+    constexpr int kLanes = C::D / 16;     // of a row
+    constexpr int kAtOnce = 32 / kLanes;  // rows
+    constexpr int kPasses = kLanes / (C::NR == 1 ? 2 : 1);
     const int lane = static_cast<int>(threadIdx.x) % 32;
     const int part = lane % kLanes;
-    const bool mine = C::NR == 2 || part / (kLanes / 2) == w;
-    const uint16_t* from = static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] + head * p.q_stride[1] + row.token * p.q_stride[2];
+    const int row0 = (C::NR == 1 ? 16 * w : 0) + lane / kLanes;
     const uint32_t sign = p.softmax_scale < 0.0f ? 0x80008000u : 0u;  // the factor stays positive
-    row.factor = fmaxf(fabsf(p.softmax_scale) * kLog2e, kLeastFactor);
-#pragma unroll 1
-    for (int pass0 = 0; pass0 < kPasses; pass0 += 4) {
-        uint4 word[4][2];
+    const float scale = fmaxf(fabsf(p.softmax_scale) * kLog2e, kLeastFactor);
+    float factor = scale;
+    uint4 word[kPasses][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int owner = (pass0 + i) * kAtOnce + lane / kLanes;
-            const uint64_t at = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(from), owner);
-            const bool real = __shfl_sync(0xffffffffu, static_cast<int>(row.real), owner) != 0;
-            const uint4* src = reinterpret_cast<const uint4*>(at) + 2 * part;
-            word[i][0] = real ? __ldg(src) : make_uint4(0u, 0u, 0u, 0u);
-            word[i][1] = real ? __ldg(src + 1) : make_uint4(0u, 0u, 0u, 0u);
-        }
+    for (int i = 0; i < kPasses; ++i) {
+        const uint64_t from = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(at), row0 + i * kAtOnce);
+        const bool there = __shfl_sync(0xffffffffu, static_cast<int>(real), row0 + i * kAtOnce) != 0;
+        const uint4* src = reinterpret_cast<const uint4*>(from) + 2 * part;
+        word[i][0] = there ? __ldg(src) : make_uint4(0u, 0u, 0u, 0u);
+        word[i][1] = there ? __ldg(src + 1) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (!ready()) {
+        return factor;
+    }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int owner = (pass0 + i) * kAtOnce + lane / kLanes;
-            const int r = quarter * 32 + owner;
-            const uint32_t x[8] = {word[i][0].x ^ sign, word[i][0].y ^ sign, word[i][0].z ^ sign, word[i][0].w ^ sign,
-                                   word[i][1].x ^ sign, word[i][1].y ^ sign, word[i][1].z ^ sign, word[i][1].w ^ sign};
-            if constexpr (!C::E4M3) {
-                if (mine) {
-                    store_shared16(tile + tile_offset(r, 2 * part), x[0], x[1], x[2], x[3]);
-                    store_shared16(tile + tile_offset(r, 2 * part + 1), x[4], x[5], x[6], x[7]);
+    for (int i = 0; i < kPasses; ++i) {
+        const int owner = row0 + i * kAtOnce;
+        const int r = quarter * 32 + owner;
+        const uint32_t x[8] = {word[i][0].x ^ sign, word[i][0].y ^ sign, word[i][0].z ^ sign, word[i][0].w ^ sign,
+                               word[i][1].x ^ sign, word[i][1].y ^ sign, word[i][1].z ^ sign, word[i][1].w ^ sign};
+        if constexpr (!C::E4M3) {
+            store_shared16(tile + tile_offset(r, 2 * part), x[0], x[1], x[2], x[3]);
+            store_shared16(tile + tile_offset(r, 2 * part + 1), x[4], x[5], x[6], x[7]);
+        } else {
+            uint32_t top = 0;  // of the values' bits without sign: their order is that of the sizes
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                top = max(top, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
+            }
+#pragma unroll
+            for (int o = 1; o < kLanes; o <<= 1) {
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            }
+            // 2^(8 - exponent of the largest), one less where that would pass 448, both it and its inverse normal; 1 for
+            // zeros, inf and NaN.
+            const uint32_t most = __float_as_uint(widen16<C::BF16>(static_cast<uint16_t>(top)));
+            const int e = static_cast<int>(most >> 23);
+            const int shift = (e == 0 || e == 255) ? 0 : min(max(135 - e - ((most & 0x7fffffu) > 0x600000u ? 1 : 0), -100), 100);
+            const float up = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+            const float back = fmaxf(scale * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23), kLeastFactor);
+            if constexpr (C::NR == 1) {
+                if (part == 0) {
+                    factors[r] = back;
                 }
             } else {
-                uint32_t top = 0;  // of the values' bits without sign: their order is that of the sizes
+                const float rows_own = __shfl_sync(0xffffffffu, back, (lane % kAtOnce) * kLanes);
+                factor = lane / kAtOnce == i ? rows_own : factor;
+            }
+            float f[16];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    top = max(top, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
-                }
+            for (int j = 0; j < 8; ++j) {
+                f[2 * j] = widen16<C::BF16>(static_cast<uint16_t>(x[j] & 0xffffu)) * up;
+                f[2 * j + 1] = widen16<C::BF16>(static_cast<uint16_t>(x[j] >> 16)) * up;
+            }
 #pragma unroll
-                for (int o = 1; o < kLanes; o <<= 1) {
-                    top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                }
-                // 2^(8 - exponent of the largest), one less where that would pass 448, both it and its inverse normal; 1
-                // for zeros, inf and NaN.
-                const uint32_t most = __float_as_uint(widen16<C::BF16>(static_cast<uint16_t>(top)));
-                const int e = static_cast<int>(most >> 23);
-                const int shift = (e == 0 || e == 255) ? 0 : min(max(135 - e - ((most & 0x7fffffu) > 0x600000u ? 1 : 0), -100), 100);
-                const float up = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
-                // The row's thread takes it back.
-                const int row_shift = __shfl_sync(0xffffffffu, shift, (lane % kAtOnce) * kLanes);
-                if (lane / kAtOnce == pass0 + i) {
-                    row.factor = fmaxf(row.factor * __uint_as_float(static_cast<uint32_t>(127 - row_shift) << 23), kLeastFactor);
-                }
-                float f[16];
+            for (int term = 0; term < C::kTerms; ++term) {
+                uint32_t code[4];
 #pragma unroll
-                for (int e2 = 0; e2 < 8; ++e2) {
-                    f[2 * e2] = widen16<C::BF16>(static_cast<uint16_t>(x[e2] & 0xffffu)) * up;
-                    f[2 * e2 + 1] = widen16<C::BF16>(static_cast<uint16_t>(x[e2] >> 16)) * up;
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t lo = pack_e4m3x2(f[4 * j], f[4 * j + 1]);
+                    const uint32_t hi = pack_e4m3x2(f[4 * j + 2], f[4 * j + 3]);
+                    code[j] = lo | (hi << 16);
+                    const float2 u = unpack_half2(e4m3x2_to_half2(lo));
+                    const float2 v = unpack_half2(e4m3x2_to_half2(hi));
+                    f[4 * j] -= u.x;
+                    f[4 * j + 1] -= u.y;
+                    f[4 * j + 2] -= v.x;
+                    f[4 * j + 3] -= v.y;
                 }
-#pragma unroll
-                for (int term = 0; term < C::kTerms; ++term) {
-                    uint32_t code[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t lo = pack_e4m3x2(f[4 * j], f[4 * j + 1]);
-                        const uint32_t hi = pack_e4m3x2(f[4 * j + 2], f[4 * j + 3]);
-                        code[j] = lo | (hi << 16);
-                        const float2 u = unpack_half2(e4m3x2_to_half2(lo));
-                        const float2 v = unpack_half2(e4m3x2_to_half2(hi));
-                        f[4 * j] -= u.x;
-                        f[4 * j + 1] -= u.y;
-                        f[4 * j + 2] -= v.x;
-                        f[4 * j + 3] -= v.y;
-                    }
-                    if (mine) {
-                        store_shared16(tile + term * C::kRaw + code_offset<C::D>(r, part), code[0], code[1], code[2], code[3]);
-                    }
-                }
+                store_shared16(tile + term * C::kRaw + code_offset<C::D>(r, part), code[0], code[1], code[2], code[3]);
             }
         }
     }
+    fence_proxy_async_smem();
+    return factor;
 }
 
 // 32 columns of scores, keys from kb on: those that the row does not see become -inf.
@@ -1024,16 +1067,14 @@ __device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s
     const float used = m == -INFINITY ? 0.0f : m;
     l *= alpha;
     __syncwarp();  // tensor memory is accessed by whole warps
-    const bool shrinks = C::E4M3 && aux.shrinks != 0;
 #pragma unroll
     for (int g = 0; g < kTile / GROUP; ++g) {
-        float f = factor, add = -used, inv = 1.0f, shrink = 1.0f;
+        float f = factor, add = -used, inv = 1.0f;
         if constexpr (C::E4M3) {
             const float4 a = aux.group[g * GROUP / 8];
             f = fmaxf(f * a.x, kLeastFactor);
             add = a.y - used;
             inv = a.z;
-            shrink = a.w;
         }
         const float2 f2 = make_float2(f, f), add2 = make_float2(add, add);
         float2 sum[4];
@@ -1048,12 +1089,6 @@ __device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s
         }
         const float2 all = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
         l = fmaf(all.x + all.y, inv, l);
-        if (shrinks) {
-#pragma unroll
-            for (int i = 0; i < GROUP; ++i) {
-                x[GROUP * g + i] = f2u(u2f(x[GROUP * g + i]) * shrink);
-            }
-        }
         // P of 32 keys takes 16 columns.
         if constexpr (GROUP == 32) {
             uint32_t packed[16];
@@ -1075,7 +1110,7 @@ __device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s
 }
 
 template <class C>
-__device__ __forceinline__ void softmax(const FaTreeParams& p, DeviceStatus* status, Shared& sh, uint32_t smem, const Record& rec,
+__device__ __forceinline__ void softmax(const FaTreeParams& p, Shared& sh, Exchange& ex, uint32_t smem, const Record& rec,
                                         const WaitCtx& wctx) {
     constexpr int D = C::D;
     constexpr int NR = C::NR;
@@ -1102,10 +1137,33 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, DeviceStatus* sta
     const bool coarse = p.cache.page_size >= 32;
     int tiles = 0;   // key tiles of the pieces before
     int steps = 0;   // scores taken
-    for (int items = 0;; ++items) {
+    float next_factor = 0.0f;
+    // The queries of piece `items`, on their way while the piece before ends. False: given up.
+    auto queries = [&](int items) {
         if (!wait(&sh.part_full[items % kParts], items / kParts)) {
-            return;
+            return false;
         }
+        const Part& s = sh.part[items % kParts];
+        if (s.n == 0) {
+            return true;
+        }
+        const int row_index = s.block * C::kRows + (NR == 2 ? w * kTile : 0) + r;
+        const int head = row_index / p.cache.tokens;
+        const int token = row_index - head * p.cache.tokens;
+        bool ok = true;
+        next_factor = bring_queries<C>(
+            p, static_cast<const uint16_t*>(p.q) + s.b * p.q_stride[0] + (s.kvh * group + head) * p.q_stride[1] + token * p.q_stride[2],
+            row_index < rows && token < s.count, smem + C::kSmemQ + (NR == 2 ? w * C::kQTile : 0), warp % 4, w, ex.factor[items & 1],
+            [&] { return ok = items == 0 || wait(&sh.q_empty, items - 1); });
+        if (ok) {
+            arrive(&sh.q_full);
+        }
+        return ok;
+    };
+    if (!queries(0)) {
+        return;
+    }
+    for (int items = 0;; ++items) {
         const Part& s = sh.part[items % kParts];  // until the end of the piece
         const int n = s.n;
         if (n == 0) {
@@ -1113,40 +1171,30 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, DeviceStatus* sta
         }
         const int row_index = s.block * C::kRows + (NR == 2 ? w * kTile : 0) + r;
         Row row;
-        row.head = row_index / p.cache.tokens;
-        row.token = row_index - row.head * p.cache.tokens;
+        row.token = row_index % p.cache.tokens;
         row.real = row_index < rows && row.token < s.count;
-        if (items > 0 && !wait(&sh.q_empty, items - 1)) {
-            return;
+        row.factor = next_factor;
+        if (NR == 1 && C::E4M3) {
+            if (!wait(&sh.q_full, items)) {
+                return;
+            }
+            row.factor = ex.factor[items & 1][r];
         }
-        bring_queries<C>(p, row, s.b, s.kvh * group + row.head, smem + C::kSmemQ + (NR == 2 ? w * C::kQTile : 0), warp % 4, w);
-        fence_proxy_async_smem();
-        arrive(&sh.q_full);
         // The way up from the row's node.
         int depth = 0;
+        int at = row.real ? row.token : -1;
 #pragma unroll
-        for (int i = 0; i < kMaskWords; ++i) {
+        for (int i = kMaskWords - 1; i >= 0; --i) {
             row.mask[i] = 0;
-        }
-        if (row.real) {
-            const int32_t* parents = p.parents + s.b * p.parent_stride;
-            int at = row.token;
-            bool bad = false;
-#pragma unroll
-            for (int i = kMaskWords - 1; i >= 0; --i) {
-                while (at >= 32 * i) {
-                    row.mask[i] |= 1u << (at & 31);
-                    ++depth;
-                    const int up = __ldg(parents + at);
-                    bad = bad || up < -1 || up >= at;
-                    at = up < -1 || up >= at ? -1 : up;
-                }
-            }
-            if (bad || s.context < 0 || s.context > held(p.cache) - s.count) {
-                atomicOr(&status->code, kStatusBadPage);
+            while (at >= 32 * i) {
+                row.mask[i] |= 1u << (at & 31);
+                ++depth;
+                const int up = s.up[at];
+                at = up == 255 ? -1 : up;
             }
         }
         row.first = window_first(max(s.context + depth - 1, 0), p.window);
+        __syncwarp();
 
         float m = -INFINITY, l = 0.0f;
         int mine = 0;  // scores of this piece taken
@@ -1199,90 +1247,81 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, DeviceStatus* sta
         tiles += n;
 
         // The end of the piece: rows of both warpgroups joined (NR 1), normalised or left in a record.
-        if (!wait(&sh.done, items)) {
+        if (!queries(items + 1) || !wait(&sh.done, items)) {
             return;
         }
-        float weight[2] = {1.0f, 0.0f};
-        float other_m = -INFINITY, other_l = 0.0f;
+        float own_weight = 1.0f, other_weight = 0.0f;
         if constexpr (NR == 1) {
-            // Each tells the other its maximum and sum through its scores' columns, which are free.
-            uint32_t mine2[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                mine2[i] = 0;
-            }
-            mine2[0] = f2u(m);
-            mine2[1] = f2u(l);
-            tmem_st16(tmem_s, mine2);
-            tmem_wait_st();
-            tc_fence_before();
+            ex.ml[w][r] = make_float2(m, l);
             arrive(&sh.ml_full);
             if (!wait(&sh.ml_full, items)) {
                 return;
             }
-            uint32_t theirs[16];
-            tmem_ld16(lanes + C::kTmemS + (1 - w) * kTile, theirs);
-            tmem_wait_ld();
-            other_m = u2f(theirs[0]);
-            other_l = u2f(theirs[1]);
-            const float all = fmax_nan(m, other_m);
+            const float2 other = ex.ml[1 - w][r];
+            const float all = fmax_nan(m, other.x);
             const float base = all == -INFINITY ? 0.0f : all;
-            weight[0] = ex2_approx(m - base);
-            weight[1] = ex2_approx(other_m - base);
-            l = l * weight[0] + other_l * weight[1];
+            own_weight = ex2_approx(m - base);
+            other_weight = ex2_approx(other.x - base);
+            l = l * own_weight + other.y * other_weight;
             m = all;
         }
         constexpr int kColumns = NR == 1 ? D / 2 : D;  // of this thread
         const int column0 = NR == 1 ? w * kColumns : 0;
-        const uint32_t own = tmem_o + column0;
-        const uint32_t theirs = lanes + C::kTmemO + (1 - w) * D + column0;
-        const bool both = NR == 1 && n > 1;           // the other sum exists
-        const bool self = NR == 2 || w == 0 || n > 1;  // this one does
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const bool other = NR == 1 && (n > 1 || w == 1);  // the other sum exists
+        const bool self = NR == 2 || w == 0 || n > 1;     // this one does
         const bool in_rows = row_index < rows;
-        const int64_t out_row = (static_cast<int64_t>(s.b) * p.heads + s.kvh * group + row.head) * p.cache.tokens + row.token;
         const int record = s.record;
-        const int64_t record_row = static_cast<int64_t>(record) * C::kRows + (NR == 2 ? w * kTile : 0) + r;
+        const float inv = record >= 0 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+        own_weight = row.real ? own_weight * inv : 0.0f;
+        other_weight = row.real ? other_weight * inv : 0.0f;
+        // Rows of an item lie one after another in the output. In a record four columns of all rows do, so that the
+        // rows' threads write whole lines.
+        uint16_t* out = static_cast<uint16_t*>(p.o) + ((static_cast<int64_t>(s.b) * p.heads + s.kvh * group) * p.cache.tokens + row_index) * D + column0;
+        float4* kept = reinterpret_cast<float4*>(rec.o) +
+                       (static_cast<int64_t>(record) * (D / 4) + column0 / 4) * C::kRows + (NR == 2 ? w * kTile : 0) + r;
 #pragma unroll 1
         for (int c = 0; c < kColumns / 32; ++c) {
-            uint32_t x[32], y[32];
+            uint32_t x[32];
+            __syncwarp();
             if (self) {
-                tmem_ld32(own + 32 * c, x);
-            }
-            if (NR == 1 && (both || !self)) {
-                tmem_ld32(theirs + 32 * c, y);
-            }
-            tmem_wait_ld();
+                tmem_ld32(tmem_o + column0 + 32 * c, x);
+                tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                float z = self ? u2f(x[i]) * weight[0] : 0.0f;
-                if (NR == 1 && (both || !self)) {
-                    z = fmaf(u2f(y[i]), weight[1], z);
-                }
-                x[i] = row.real ? f2u(z) : 0u;
-            }
-            if (!in_rows) {
-                continue;
-            }
-            if (record < 0) {
-                uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + out_row * D + column0 + 32 * c);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    to[i] = make_uint4(pack2<C::BF16>(u2f(x[8 * i]) * inv, u2f(x[8 * i + 1]) * inv),
-                                       pack2<C::BF16>(u2f(x[8 * i + 2]) * inv, u2f(x[8 * i + 3]) * inv),
-                                       pack2<C::BF16>(u2f(x[8 * i + 4]) * inv, u2f(x[8 * i + 5]) * inv),
-                                       pack2<C::BF16>(u2f(x[8 * i + 6]) * inv, u2f(x[8 * i + 7]) * inv));
+                for (int i = 0; i < 32; ++i) {
+                    x[i] = row.real ? f2u(u2f(x[i]) * own_weight) : 0u;
                 }
             } else {
-                uint4* to = reinterpret_cast<uint4*>(rec.o + record_row * D + column0 + 32 * c);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    x[i] = 0u;
+                }
+            }
+            if (other) {
+                uint32_t y[32];
+                tmem_ld32(lanes + C::kTmemO + (1 - w) * D + column0 + 32 * c, y);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    x[i] = row.real ? f2u(fmaf(u2f(y[i]), other_weight, u2f(x[i]))) : 0u;
+                }
+            }
+            if (in_rows && record < 0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    reinterpret_cast<uint4*>(out)[4 * c + i] = make_uint4(
+                        pack2<C::BF16>(u2f(x[8 * i]), u2f(x[8 * i + 1])), pack2<C::BF16>(u2f(x[8 * i + 2]), u2f(x[8 * i + 3])),
+                        pack2<C::BF16>(u2f(x[8 * i + 4]), u2f(x[8 * i + 5])), pack2<C::BF16>(u2f(x[8 * i + 6]), u2f(x[8 * i + 7])));
+                }
+            } else if (in_rows) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    to[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                    kept[static_cast<int64_t>(8 * c + i) * C::kRows] =
+                        make_float4(u2f(x[4 * i]), u2f(x[4 * i + 1]), u2f(x[4 * i + 2]), u2f(x[4 * i + 3]));
                 }
             }
         }
         if (record >= 0 && in_rows && (NR == 2 || w == 0)) {
-            rec.ml[record_row] = row.real ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
+            rec.ml[static_cast<int64_t>(record) * C::kRows + (NR == 2 ? w * kTile : 0) + r] = row.real ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
         }
         tc_fence_before();
         arrive(&sh.o_free);
@@ -1295,7 +1334,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
                                                            const __grid_constant__ CUtensorMap tm_v, DeviceStatus* status, unsigned epoch,
                                                            Split split, Record rec) {
     extern __shared__ uint8_t raw[];
-    uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    uint8_t* smem = raw;  // on 1024 bytes: a kernel without static shared memory has it from there
     Shared& sh = *reinterpret_cast<Shared*>(smem + C::kSmemShared);
     const int warp = static_cast<int>(threadIdx.x) / 32;
     const WaitCtx wctx{&sh.abort, &status->code, &status->epoch_aborted, epoch};
@@ -1345,21 +1384,23 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     __syncthreads();
     tc_fence_after();
     // Owning all 512 columns means owning them from 0, a constant for the products' operands.
-    if (sh.tmem_base != 0) {
+    if (sh.tmem_base != 0 || (smem_u32(smem) & 1023u) != 0) {
         if (threadIdx.x == 0) {
             atomicOr(&status->code, kStatusTimeoutTeardown);
         }
     } else {
         if (warp < kSoftmaxWarps) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-            softmax<C>(p, status, sh, smem_u32(smem), rec, wctx);
+            softmax<C>(p, sh, *reinterpret_cast<Exchange*>(&sh + 1), smem_u32(smem), rec, wctx);
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
             if (warp < kMmaWarp) {
                 ready_values<C>(p, sh, smem_u32(smem), wctx);
             } else if (warp == kMmaWarp) {
                 issue_products<C>(sh, smem_u32(smem), wctx);
-            } else if (warp < kListWarp + kListWarps) {
+            } else if (warp == kPartWarp) {
+                list_parts(p, split, status, start_walk(p, split, range, static_cast<int>(blockIdx.x)), sh, wctx);
+            } else {
                 const Walk walk = start_walk(p, split, range, static_cast<int>(blockIdx.x));
                 list_tiles<C>(p, &tm_k, &tm_v, split, status, walk, sh, smem_u32(smem), warp - kListWarp, wctx);
                 // Copies in flight end by themselves; after a wait that was given up they get a millisecond.
@@ -1390,7 +1431,6 @@ template <class C>
 __global__ void __launch_bounds__(kRowWarps * 32) tree_finish_kernel(const __grid_constant__ FaTreeParams p, DeviceStatus* status,
                                                                      Split split, Record rec, int joins, int fixers) {
     constexpr int D = C::D;
-    constexpr int kPer = D / 32;
     __shared__ long long warp_sum[kRowWarps];
     __shared__ long long found_base;
     __shared__ int found;
@@ -1416,35 +1456,31 @@ __global__ void __launch_bounds__(kRowWarps * 32) tree_finish_kernel(const __gri
         }
         const int kvh = static_cast<int>(item / split.row_blocks);
         const int block = static_cast<int>(item - static_cast<long long>(kvh) * split.row_blocks);
-        const int r = static_cast<int>(blockIdx.y) * kRowWarps + warp;
+        // A warp takes 32 rows and 8 columns, a lane a row.
+        constexpr int kAcross = D / 8;
+        const int unit = static_cast<int>(blockIdx.y) * kRowWarps + warp;
+        const int r = unit / kAcross * 32 + lane;
+        const int eight = unit % kAcross;
         const int row_index = block * C::kRows + r;
-        if (row_index - warp >= rows) {
-            return;
-        }
         const long long c0 = start / range.per;
         const long long c1 = (start + s.tiles - 1) / range.per;
         cudaGridDependencySynchronize();  // the records are there
-        if (row_index >= rows) {
+        if (r >= C::kRows || row_index >= rows) {
             return;
         }
         float m = -INFINITY, l = 0.0f;
-        float o[kPer];
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            o[i] = 0.0f;
-        }
+        float o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         bool odd = false;
 #pragma unroll 4
         for (long long c = c0; c <= c1; ++c) {
             // A CTA's first cut piece is its record 0; the item starts in c0, as its second unless there.
-            const long long record = (2 * c + (c * range.per >= start ? 0 : 1)) * C::kRows + r;
+            const long long record = 2 * c + (c * range.per >= start ? 0 : 1);
             odd = odd || (rec.odd != nullptr && rec.odd[c] != 0);
-            const float2 ml = rec.ml[record];
-            float y[kPer];
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                y[i] = rec.o[record * D + lane * kPer + i];
-            }
+            const float2 ml = rec.ml[record * C::kRows + r];
+            const float4* from = reinterpret_cast<const float4*>(rec.o) + (record * (D / 4) + 2 * eight) * C::kRows + r;
+            const float4 y0 = from[0];
+            const float4 y1 = from[C::kRows];
+            const float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
             const float now = fmax_nan(m, ml.x);
             const float used = now == -INFINITY ? 0.0f : now;
             const float a = ex2_approx(m - used);
@@ -1452,7 +1488,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) tree_finish_kernel(const __gri
             m = now;
             l = fmaf(ml.y, f, l * a);
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
+            for (int i = 0; i < 8; ++i) {
                 o[i] = fmaf(y[i], f, o[i] * a);
             }
         }
@@ -1460,13 +1496,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) tree_finish_kernel(const __gri
             return;  // its rows are computed anew
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const int head = row_index / p.cache.tokens;
-        const int token = row_index - head * p.cache.tokens;
-        const int64_t out_row = (static_cast<int64_t>(range.found) * p.heads + kvh * group + head) * p.cache.tokens + token;
-#pragma unroll
-        for (int i = 0; i < kPer; i += 2) {
-            reinterpret_cast<uint32_t*>(p.o)[(out_row * D + lane * kPer + i) / 2] = pack2<C::BF16>(o[i] * inv, o[i + 1] * inv);
-        }
+        uint16_t* out = static_cast<uint16_t*>(p.o) + ((static_cast<int64_t>(range.found) * p.heads + kvh * group) * p.cache.tokens + row_index) * D;
+        reinterpret_cast<uint4*>(out)[eight] = make_uint4(pack2<C::BF16>(o[0] * inv, o[1] * inv), pack2<C::BF16>(o[2] * inv, o[3] * inv),
+                                                          pack2<C::BF16>(o[4] * inv, o[5] * inv), pack2<C::BF16>(o[6] * inv, o[7] * inv));
         return;
     }
     if (blockIdx.y > 0) {
@@ -1598,7 +1630,7 @@ cudaError_t launch(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, 
     const int fixers = rec.odd != nullptr ? kFixers : 0;
     if (err == cudaSuccess && joins + fixers > 0) {
         const int rows = std::min(C::kRows, p.heads / p.cache.kv_heads * p.cache.tokens);
-        const dim3 grid(static_cast<unsigned>(joins + fixers), static_cast<unsigned>(joins > 0 ? (rows + kRowWarps - 1) / kRowWarps : 1));
+        const dim3 grid(static_cast<unsigned>(joins + fixers), static_cast<unsigned>(joins > 0 ? ((rows + 31) / 32 * (C::D / 8) + kRowWarps - 1) / kRowWarps : 1));
         err = launch_early(tree_finish_kernel<C>, grid, kRowWarps * 32, stream, p, status, split, rec, joins, fixers);
     }
     return err;
