@@ -31,13 +31,13 @@ constexpr int kBox = 128 * 128;  // bytes of 128 rows of 64 16-bit values, 128-b
 
 constexpr int kSoftmaxWarps = 8;
 constexpr int kValueWarps = 4;
-constexpr int kMmaWarp = kSoftmaxWarps + kValueWarps;
+constexpr int kScoreWarp = kSoftmaxWarps + kValueWarps;  // issues Q K^T
+constexpr int kMmaWarp = kScoreWarp + 1;                 // issues P V, owns tensor memory
 constexpr int kListWarp = kMmaWarp + 1;  // and the one after it: the list of key tiles, and their copies
 // Tiles are the list warps' in turn. A warp that waits for a ring's slot has seen the slot `kListWarps` tiles before it
 // consumed; with no more warps than a ring has slots the phase it waits for is then never two behind.
 constexpr int kListWarps = 2;
-constexpr int kPartWarp = kListWarp + kListWarps;  // the list of pieces
-constexpr int kWarps = kMmaWarp + 4;  // whole warpgroups: registers are handed over between those
+constexpr int kWarps = kScoreWarp + 4;  // whole warpgroups: registers are handed over between those
 constexpr int kThreads = kWarps * 32;
 // Registers: launched with 128 a thread, 512 for a lane of the four warpgroups.
 constexpr int kRegsSoftmax = 184;
@@ -47,7 +47,7 @@ static_assert(2 * kRegsSoftmax + 2 * kRegsOther <= 4 * 128, "no more than the la
 constexpr int kListed = 4;           // key tiles listed ahead
 constexpr int kGroups = kTile / 8;   // keys that surely share a page
 constexpr int kMostStages = 4;
-constexpr int kParts = 4;  // pieces listed ahead
+constexpr int kParts = 2;  // pieces listed, the one at hand and the next
 
 template <int D_, bool BF16_, bool E4M3_, int NR_>
 struct Cfg {
@@ -73,8 +73,10 @@ struct Cfg {
     static constexpr int kSmemR = kSmemV + kVStages * kWide;
     static constexpr int kSmemShared = kSmemR + (E4M3 ? kRStages * kRaw : 0);
     static constexpr int kRows = NR * kTile;
-    // Tensor memory: two scores, P over each's first half, two sums.
+    // Tensor memory: one tile's scores, which a warpgroup takes into registers at once, so that the next tile's follow while it
+    // computes; P and the sums of either warpgroup.
     static constexpr uint32_t kTmemS = 0;
+    static constexpr uint32_t kTmemP = kTile;
     static constexpr uint32_t kTmemO = 2 * kTile;
 };
 
@@ -95,7 +97,9 @@ struct Part {
     int record;           // -1: a whole item
     int context, count;   // of its sequence
     int last;
-    uint8_t up[kMostNodes];  // nodes' parents, 255 for none
+    // A node's way up in runs: `low` the first node of the run of nodes, each the parent of the next, that ends with the
+    // node; `up` the parent of that first one, 255 for none.
+    uint8_t low[kMostNodes], up[kMostNodes];
 };
 
 struct alignas(16) Shared {
@@ -104,7 +108,7 @@ struct alignas(16) Shared {
     uint64_t part_full[kParts], part_empty[kParts];
     uint64_t list_full[kListed], list_empty[kListed];
     uint64_t k_full[kMostStages], k_empty[kMostStages], v_full[2], v_empty[2], r_full[kMostStages], r_empty[kMostStages];
-    uint64_t s_full[2], p_full[2];
+    uint64_t s_full[2], s_free[2], p_full[2], p_free[2];  // by warpgroup
     uint64_t q_full, q_empty, done, o_free, ml_full, mma_idle;
     long long warp_sum[kWarps];
     long long found_base;
@@ -314,8 +318,10 @@ __device__ __forceinline__ Sequence sequence(const FaTreeParams& p, int b) {
 __device__ __forceinline__ int tile_key(const Sequence& s, int v) { return (v < s.sink_tiles ? v : v - s.sink_tiles + s.first_tile) * kTile; }
 
 // How a call is cut: items are (sequence, kv head, block of rows), each a list of key tiles. `whole`: an item a CTA. Else
-// the lists are laid end to end and cut into equal ranges, one a CTA; parts of cut items go to records, which a second
-// kernel joins.
+// the lists are laid end to end, each behind the few units that an item costs beside its tiles, and cut into equal ranges,
+// one a CTA; parts of cut items go to records, which a second kernel joins.
+constexpr int kItemHead = 4;
+
 struct Split {
     int whole;
     int grid;
@@ -346,7 +352,7 @@ __device__ __forceinline__ Range locate(const FaTreeParams& p, const Split& spli
     const int b1 = min(b0 + share, p.cache.batch);
     long long mine = 0;
     for (int b = b0; b < b1; ++b) {
-        mine += sequence(p, b).tiles;
+        mine += sequence(p, b).tiles + kItemHead;
     }
     mine *= split.items;
     long long incl = mine;
@@ -375,7 +381,7 @@ __device__ __forceinline__ Range locate(const FaTreeParams& p, const Split& spli
     if (target >= before && target < before + mine) {
         long long base = before;
         for (int b = b0; b < b1; ++b) {
-            const long long n = static_cast<long long>(sequence(p, b).tiles) * split.items;
+            const long long n = static_cast<long long>(sequence(p, b).tiles + kItemHead) * split.items;
             if (target < base + n) {
                 *found = b;
                 *found_base = base;
@@ -420,9 +426,12 @@ __device__ __forceinline__ Walk start_walk(const FaTreeParams& p, const Split& s
         w.b = range.found;
         w.s = sequence(p, w.b);
         const long long in_seq = at - range.found_base;
-        w.item = static_cast<int>(in_seq / w.s.tiles);
-        w.v = static_cast<int>(in_seq - static_cast<long long>(w.item) * w.s.tiles);
+        w.item = static_cast<int>(in_seq / (w.s.tiles + kItemHead));
+        w.v = static_cast<int>(in_seq - static_cast<long long>(w.item) * (w.s.tiles + kItemHead)) - kItemHead;
         w.left = min(range.per, range.total - at);
+        if (w.v < 0 && w.left <= -w.v) {
+            w.left = 0;
+        }
     }
     w.record = 2 * cta;
     return w;
@@ -432,6 +441,10 @@ __device__ __forceinline__ Walk start_walk(const FaTreeParams& p, const Split& s
 __device__ __forceinline__ bool next_piece(const FaTreeParams& p, const Split& split, Walk& w, Piece& piece, Sequence& s) {
     if (w.left <= 0) {
         return false;
+    }
+    if (w.v < 0) {  // what an item costs beside its tiles
+        w.left += w.v;
+        w.v = 0;
     }
     s = w.s;
     piece.b = w.b;
@@ -443,10 +456,13 @@ __device__ __forceinline__ bool next_piece(const FaTreeParams& p, const Split& s
     piece.record = w.v == 0 && take == s.tiles ? -1 : w.record;
     w.record = 2 * static_cast<int>(blockIdx.x) + 1;  // a range has a cut piece at its start and at its end
     w.left -= take;
-    w.v = 0;
+    w.v = -kItemHead;
     if (w.left > 0 && ++w.item == split.items) {
         w.item = 0;
         w.s = sequence(p, ++w.b);
+    }
+    if (w.left <= kItemHead) {
+        w.left = 0;  // the range ends before the item's first tile
     }
     return true;
 }
@@ -492,6 +508,63 @@ __device__ __forceinline__ uint4 load_shared16(uint32_t at) {
     return w;
 }
 
+// A piece listed for the softmax and the products; n = 0: the end.
+__device__ __forceinline__ bool list_part(const FaTreeParams& p, DeviceStatus* status, Shared& sh, int part, const Piece& piece, const Sequence& s,
+                                          int n, const WaitCtx& wctx) {
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    Part& to = sh.part[part % kParts];
+    const bool ok = mbar_wait(smem_u32(&sh.part_empty[part % kParts]), ((part / kParts) & 1) ^ 1, wctx, kStatusTimeoutProducer);
+    if (__all_sync(0xffffffffu, ok) == 0) {
+        return false;
+    }
+    if (n > 0) {
+        const int32_t* parents = p.parents + piece.b * p.parent_stride;
+        bool bad = s.count > 0 && (s.context < 0 || s.context > held(p.cache) - s.count);
+        int start = 0;  // of the run at the end of the nodes before
+        for (int t0 = 0; t0 < s.count; t0 += 32) {
+            const int t = t0 + lane;
+            int up = t < s.count ? __ldg(parents + t) : -1;
+            if (up < -1 || up >= t) {
+                bad = true;
+                up = -1;
+            }
+            int low = t > 0 && up == t - 1 ? -1 : t;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int before = __shfl_up_sync(0xffffffffu, low, o);
+                low = lane >= o ? max(low, before) : low;
+            }
+            low = max(low, start);
+            start = __shfl_sync(0xffffffffu, low, 31);
+            if (t < s.count) {
+                to.low[t] = static_cast<uint8_t>(low);
+                // The first node's parent: the entry of the run's first node, which is its own.
+                if (low == t) {
+                    to.up[t] = up < 0 ? 255 : static_cast<uint8_t>(up);
+                }
+            }
+        }
+        if (bad) {
+            atomicOr(&status->code, kStatusBadPage);
+        }
+    }
+    if (lane == 0) {
+        to.n = n;
+        to.b = piece.b;
+        to.kvh = piece.kvh;
+        to.block = piece.block;
+        to.record = piece.record;
+        to.context = s.context;
+        to.count = s.count;
+        to.last = s.last;
+    }
+    __syncwarp();
+    if (lane == 0) {
+        mbar_arrive(smem_u32(&sh.part_full[part % kParts]));
+    }
+    return true;
+}
+
 // The range's key tiles: listed for the others, and copied, K and V, a copy a page. Every second tile is this warp's, so
 // that the loads of pages and scales of two tiles are on their way at once.
 template <class C>
@@ -509,6 +582,7 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensor
     int n = -1;  // the tile at hand
     int v = -1;
     int turn = which;  // the tile that is this warp's
+    int parts = 0;
     auto wait = [&](uint64_t* bar, int phase) {
         return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), (phase & 1) ^ 1, wctx, kStatusTimeoutProducer)) != 0;
     };
@@ -517,6 +591,9 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensor
         if (++v >= piece.v1) {
             more = next_piece(p, split, walk, piece, s);
             v = piece.v0;
+            if (which == 0 && !list_part(p, status, sh, parts++, piece, s, more ? piece.v1 - piece.v0 : 0, wctx)) {
+                return;
+            }
         }
         if (++n != turn) {
             if (!more) {
@@ -617,51 +694,6 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensor
         __syncwarp();
         if (lane == 0) {
             mbar_arrive(smem_u32(&sh.list_full[n % kListed]));
-        }
-    }
-}
-
-// The range's pieces, listed for the softmax and the products.
-__device__ __forceinline__ void list_parts(const FaTreeParams& p, const Split& split, DeviceStatus* status, Walk walk, Shared& sh,
-                                           const WaitCtx& wctx) {
-    const int lane = static_cast<int>(threadIdx.x) % 32;
-    Piece piece;
-    Sequence s;
-    for (int n = 0;; ++n) {
-        const bool more = next_piece(p, split, walk, piece, s);
-        Part& to = sh.part[n % kParts];
-        const bool ok = mbar_wait(smem_u32(&sh.part_empty[n % kParts]), ((n / kParts) & 1) ^ 1, wctx, kStatusTimeoutProducer);
-        if (__all_sync(0xffffffffu, ok) == 0) {
-            return;
-        }
-        if (more) {
-            const int32_t* parents = p.parents + piece.b * p.parent_stride;
-            bool bad = s.count > 0 && (s.context < 0 || s.context > held(p.cache) - s.count);
-            for (int t = lane; t < s.count; t += 32) {
-                const int up = __ldg(parents + t);
-                bad = bad || up < -1 || up >= t;
-                to.up[t] = up < 0 || up >= t ? 255 : static_cast<uint8_t>(up);
-            }
-            if (bad) {
-                atomicOr(&status->code, kStatusBadPage);
-            }
-        }
-        if (lane == 0) {
-            to.n = more ? piece.v1 - piece.v0 : 0;
-            to.b = piece.b;
-            to.kvh = piece.kvh;
-            to.block = piece.block;
-            to.record = piece.record;
-            to.context = s.context;
-            to.count = s.count;
-            to.last = s.last;
-        }
-        __syncwarp();
-        if (lane == 0) {
-            mbar_arrive(smem_u32(&sh.part_full[n % kParts]));
-        }
-        if (!more) {
-            return;
         }
     }
 }
@@ -810,90 +842,118 @@ __device__ __forceinline__ void issue_product(uint32_t acc, uint32_t w, uint64_t
     }
 }
 
-// Products, in the order in which scores and P take each other's place: S(s + 2) after P(s) V. Step s is key tile s (NR 1)
-// or row tile s % 2 of key tile s / 2 (NR 2).
-template <class C>
-__device__ __forceinline__ void issue_products(Shared& sh, uint32_t smem, const WaitCtx& wctx) {
-    constexpr int NR = C::NR;
-    auto kmajor = [](uint32_t at) { return C::E4M3 && C::D == 64 ? make_desc_kmajor_sw64(at) : make_desc_kmajor_sw128(at); };
-    const uint64_t q = kmajor(smem + C::kSmemQ);
-    const uint64_t k = kmajor(smem + C::kSmemK);
-    const uint64_t v = make_desc_mnmajor_sw128(smem + C::kSmemV, kBox);
-    auto off = [](int tile, int bytes) { return static_cast<uint64_t>(tile * (bytes >> 4)); };
-    auto wait = [&](uint64_t* bar, int parity) {
-        const bool there = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity & 1, wctx, kStatusTimeoutMma)) != 0;
-        tc_fence_after();
-        return there;
-    };
-    bool ok = true;
-    int tiles = 0;  // key tiles of the pieces before
-    int taken0 = 0, taken1 = 0;  // P of either warpgroup
-    for (int items = 0; ok; ++items) {
-        ok = wait(&sh.part_full[items % kParts], items / kParts);
-        const int n = ok ? sh.part[items % kParts].n : 0;
+// Products, scores and P V by a warp each: a warp's waits on barriers, which queue behind the products' own traffic in shared
+// memory, come to about 300 cycles even for what is there, so that one warp for both is what the kernel would wait for. Step
+// s is key tile s (NR 1) or row tile s % 2 of key tile s / 2 (NR 2), warpgroup s % 2's.
+template <class C, class Scores>
+__device__ __forceinline__ bool walk_parts(Shared& sh, const WaitCtx& wctx, Scores take) {
+    for (int items = 0, tiles = 0;; ++items) {
+        if (__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.part_full[items % kParts]), (items / kParts) & 1, wctx, kStatusTimeoutMma)) == 0) {
+            return false;
+        }
+        const int n = sh.part[items % kParts].n;
         if (n == 0) {
-            break;
+            return true;
         }
         __syncwarp();
         if (elect_one()) {
             mbar_arrive(smem_u32(&sh.part_empty[items % kParts]));
         }
         __syncwarp();
-        const int steps = n * NR;
-        auto scores = [&](int step) {
-            const int tile = tiles + (NR == 1 ? step : step >> 1);
-            const int w = step & 1;
-            if (NR == 1 || w == 0) {
-                ok = wait(&sh.k_full[tile % C::kKStages], tile / C::kKStages);
-            }
-            if (ok) {
-                if (elect_one()) {
-                    issue_scores<C>(C::kTmemS + w * kTile, q + off(NR == 1 ? 0 : w, C::kQTile), k + off(tile % C::kKStages, C::kRaw));
-                    umma_commit(smem_u32(&sh.s_full[w]));
-                    if (NR == 1 || w == 1) {
-                        umma_commit(smem_u32(&sh.k_empty[tile % C::kKStages]));
-                    }
-                    if (step == steps - 1) {
-                        umma_commit(smem_u32(&sh.q_empty));
-                    }
-                }
-                __syncwarp();
-            }
-        };
-        ok = wait(&sh.q_full, items);
-#pragma unroll 1
-        for (int step = -2; ok && step < steps; ++step) {
-            if (step >= 0) {
-                const int tile = tiles + (NR == 1 ? step : step >> 1);
-                const int w = step & 1;
-                if (step == 0 && items > 0) {
-                    ok = wait(&sh.o_free, items - 1);
-                }
-                if (NR == 1 || w == 0) {
-                    ok = ok && wait(&sh.v_full[tile % C::kVStages], tile / C::kVStages);
-                }
-                ok = ok && wait(&sh.p_full[w], w == 0 ? taken0++ : taken1++);
-                if (!ok) {
-                    break;
-                }
-                if (elect_one()) {
-                    issue_product<C>(C::kTmemO + w * C::D, C::kTmemS + w * kTile, v + off(tile % C::kVStages, C::kWide), step < 2);
-                    if (NR == 1 || w == 1) {
-                        umma_commit(smem_u32(&sh.v_empty[tile % C::kVStages]));
-                    }
-                    if (step == steps - 1) {
-                        umma_commit(smem_u32(&sh.done));
-                    }
-                }
-                __syncwarp();
-            }
-            if (step + 2 < steps) {
-                scores(step + 2);
-            }
+        if (!take(items, tiles, n * C::NR)) {
+            return false;
         }
         tiles += n;
     }
+}
+
+__device__ __forceinline__ bool mma_wait(uint64_t* bar, int parity, const WaitCtx& wctx) {
+    const bool there = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity & 1, wctx, kStatusTimeoutMma)) != 0;
+    tc_fence_after();
+    return there;
+}
+
+template <class C>
+__device__ __forceinline__ void score_warp(Shared& sh, uint32_t smem, const WaitCtx& wctx) {
+    constexpr int NR = C::NR;
+    auto kmajor = [](uint32_t at) { return C::E4M3 && C::D == 64 ? make_desc_kmajor_sw64(at) : make_desc_kmajor_sw128(at); };
+    const uint64_t q = kmajor(smem + C::kSmemQ);
+    const uint64_t k = kmajor(smem + C::kSmemK);
+    auto off = [](int tile, int bytes) { return static_cast<uint64_t>(tile * (bytes >> 4)); };
+    int done0 = 0, done1 = 0;  // scores of either warpgroup
+    int last = -1;             // whose were the last
+    walk_parts<C>(sh, wctx, [&](int items, int tiles, int steps) {
+        if (!mma_wait(&sh.q_full, items, wctx)) {
+            return false;
+        }
+#pragma unroll 1
+        for (int step = 0; step < steps; ++step) {
+            const int tile = tiles + (NR == 1 ? step : step >> 1);
+            const int w = step & 1;
+            if ((NR == 1 || w == 0) && !mma_wait(&sh.k_full[tile % C::kKStages], tile / C::kKStages, wctx)) {
+                return false;
+            }
+            if (last >= 0 && !mma_wait(&sh.s_free[last], (last == 0 ? done0 : done1) - 1, wctx)) {
+                return false;
+            }
+            if (elect_one()) {
+                issue_scores<C>(C::kTmemS, q + off(NR == 1 ? 0 : w, C::kQTile), k + off(tile % C::kKStages, C::kRaw));
+                umma_commit(smem_u32(&sh.s_full[w]));
+                if (NR == 1 || w == 1) {
+                    umma_commit(smem_u32(&sh.k_empty[tile % C::kKStages]));
+                }
+                if (step == steps - 1) {
+                    umma_commit(smem_u32(&sh.q_empty));
+                }
+            }
+            __syncwarp();
+            last = w;
+            done0 += 1 - w;
+            done1 += w;
+        }
+        return true;
+    });
     // Every product issued must be complete before tensor memory is released.
+    if (elect_one()) {
+        umma_commit(smem_u32(&sh.mma_idle));
+    }
+    __syncwarp();
+}
+
+template <class C>
+__device__ __forceinline__ void product_warp(Shared& sh, uint32_t smem, const WaitCtx& wctx) {
+    constexpr int NR = C::NR;
+    const uint64_t v = make_desc_mnmajor_sw128(smem + C::kSmemV, kBox);
+    int taken0 = 0, taken1 = 0;  // P of either warpgroup
+    walk_parts<C>(sh, wctx, [&](int items, int tiles, int steps) {
+        if (items > 0 && !mma_wait(&sh.o_free, items - 1, wctx)) {
+            return false;
+        }
+#pragma unroll 1
+        for (int step = 0; step < steps; ++step) {
+            const int tile = tiles + (NR == 1 ? step : step >> 1);
+            const int w = step & 1;
+            if ((NR == 1 || w == 0) && !mma_wait(&sh.v_full[tile % C::kVStages], tile / C::kVStages, wctx)) {
+                return false;
+            }
+            if (!mma_wait(&sh.p_full[w], w == 0 ? taken0++ : taken1++, wctx)) {
+                return false;
+            }
+            if (elect_one()) {
+                issue_product<C>(C::kTmemO + w * C::D, C::kTmemP + w * (kTile / 2),
+                                 v + static_cast<uint64_t>((tile % C::kVStages) * (C::kWide >> 4)), step < 2);
+                umma_commit(smem_u32(&sh.p_free[w]));
+                if (NR == 1 || w == 1) {
+                    umma_commit(smem_u32(&sh.v_empty[tile % C::kVStages]));
+                }
+                if (step == steps - 1) {
+                    umma_commit(smem_u32(&sh.done));
+                }
+            }
+            __syncwarp();
+        }
+        return true;
+    });
     if (elect_one()) {
         umma_commit(smem_u32(&sh.mma_idle));
     }
@@ -906,7 +966,6 @@ __device__ __forceinline__ void issue_products(Shared& sh, uint32_t smem, const 
 struct Row {
     bool real;          // a node's (else padding, or beyond the rows)
     int token;
-    uint32_t mask[kMaskWords];  // the node and its ancestors
     int first;          // first position of its window
     float factor;       // of a score, in log2 units
 };
@@ -1003,38 +1062,50 @@ __device__ __forceinline__ float bring_queries(const FaTreeParams& p, const uint
     return factor;
 }
 
-// 32 columns of scores, keys from kb on: those that the row does not see become -inf.
-template <class C>
-__device__ __forceinline__ uint32_t kept_columns(const FaTreeParams& p, const Part& s, const Row& row, int kb, uint32_t gone) {
-    uint32_t keep = bits_up_to(min(s.context - 1, s.last) - kb);
-    if (p.window > 0) {
-        keep &= ~bits_up_to(row.first - 1 - kb) | bits_up_to(p.sinks - 1 - kb);
-    }
-    const int node = kb - s.context;  // of the first column
-    if (node > -32 && node < kMostNodes) {
-        const int word = node >> 5;
-        uint32_t lo = 0, hi = 0;
+// A tile's columns that a row sees, as bits.
+__device__ __forceinline__ uint4 kept_columns(const FaTreeParams& p, const Part& s, const Row& row, int key0, uint32_t gone) {
+    uint32_t keep[4];
 #pragma unroll
-        for (int i = 0; i < kMaskWords; ++i) {
-            lo = i == word ? row.mask[i] : lo;
-            hi = i == word + 1 ? row.mask[i] : hi;
+    for (int i = 0; i < 4; ++i) {
+        const int kb = key0 + 32 * i;
+        keep[i] = bits_up_to(s.context - 1 - kb);
+        if (p.window > 0) {
+            keep[i] &= ~bits_up_to(row.first - 1 - kb) | bits_up_to(p.sinks - 1 - kb);
         }
-        keep |= __funnelshift_r(lo, hi, node & 31) & bits_up_to(s.last - kb);
     }
-    // 4 groups of 8 keys.
-    const uint32_t pages = ~gone;
-    keep &= ((pages & 1u) * 0xffu) | (((pages >> 1) & 1u) * 0xff00u) | (((pages >> 2) & 1u) * 0xff0000u) | (((pages >> 3) & 1u) * 0xff000000u);
-    return row.real ? keep : 0u;
+    if (key0 + kTile > s.context) {
+        const int column = s.context - key0;  // of node 0
+        for (int at = row.real ? row.token : -1; at >= 0;) {
+            const int low = s.low[at];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                keep[i] |= bits_up_to(column + at - 32 * i) & ~bits_up_to(column + low - 1 - 32 * i);
+            }
+            const int up = s.up[low];
+            at = up == 255 ? -1 : up;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        // 4 groups of 8 keys, and the end of the table.
+        const uint32_t pages = ~(gone >> (4 * i));
+        keep[i] &= bits_up_to(s.last - (key0 + 32 * i));
+        keep[i] &= ((pages & 1u) * 0xffu) | (((pages >> 1) & 1u) * 0xff00u) | (((pages >> 2) & 1u) * 0xff0000u) | (((pages >> 3) & 1u) * 0xff000000u);
+        keep[i] = row.real ? keep[i] : 0u;
+    }
+    return make_uint4(keep[0], keep[1], keep[2], keep[3]);
 }
 
-// One row's scores turned into P, in place: returns what the sums so far (and l, done here) shrink by. GROUP: keys that share
-// a page, and with it the scales.
-template <class C, int GROUP>
-__device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s, float factor, float& m, float& l) {
+// One row's scores turned into P: returns what the sums so far (and l, done here) shrink by. GROUP: keys that share a page,
+// and with it the scales. taken() once the scores are in registers, room() before P is stored.
+template <class C, int GROUP, class Taken, class Room>
+__device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s, uint32_t tmem_p, float factor, float& m, float& l, Taken taken,
+                                              Room room) {
     uint32_t x[128];
     tmem_ld64_of128<0>(tmem_s, x);
     tmem_ld64_of128<64>(tmem_s + 64, x);
     tmem_wait_ld();
+    taken();
     float top;
     if constexpr (C::E4M3) {
         top = -INFINITY;
@@ -1066,6 +1137,9 @@ __device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s
     }
     const float used = m == -INFINITY ? 0.0f : m;
     l *= alpha;
+    if (!room()) {
+        return alpha;
+    }
     __syncwarp();  // tensor memory is accessed by whole warps
 #pragma unroll
     for (int g = 0; g < kTile / GROUP; ++g) {
@@ -1096,14 +1170,14 @@ __device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s
             for (int i = 0; i < 16; ++i) {
                 packed[i] = pack2<C::kMmaBf16>(u2f(x[32 * g + 2 * i]), u2f(x[32 * g + 2 * i + 1]));
             }
-            tmem_st16(tmem_s + 16 * g, packed);
+            tmem_st16(tmem_p + 16 * g, packed);
         } else if (g % 4 == 3) {
             uint32_t packed[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 packed[i] = pack2<C::kMmaBf16>(u2f(x[8 * (g - 3) + 2 * i]), u2f(x[8 * (g - 3) + 2 * i + 1]));
             }
-            tmem_st16(tmem_s + 16 * (g / 4), packed);
+            tmem_st16(tmem_p + 16 * (g / 4), packed);
         }
     }
     return alpha;
@@ -1119,7 +1193,8 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, Shared& sh, Excha
     const int w = warp / 4;                  // warpgroup
     const int r = (warp % 4) * 32 + lane;    // row of its tile
     const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
-    const uint32_t tmem_s = lanes + C::kTmemS + w * kTile;
+    const uint32_t tmem_s = lanes + C::kTmemS;
+    const uint32_t tmem_p = lanes + C::kTmemP + w * (kTile / 2);
     const uint32_t tmem_o = lanes + C::kTmemO + w * D;
     const int group = p.heads / p.cache.kv_heads;
     const int rows = group * p.cache.tokens;
@@ -1180,21 +1255,18 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, Shared& sh, Excha
             }
             row.factor = ex.factor[items & 1][r];
         }
-        // The way up from the row's node.
-        int depth = 0;
-        int at = row.real ? row.token : -1;
-#pragma unroll
-        for (int i = kMaskWords - 1; i >= 0; --i) {
-            row.mask[i] = 0;
-            while (at >= 32 * i) {
-                row.mask[i] |= 1u << (at & 31);
-                ++depth;
-                const int up = s.up[at];
+        row.first = 0;
+        if (p.window > 0) {
+            int above = 0;  // ancestors
+            for (int at = row.real ? row.token : -1; at >= 0;) {
+                const int low = s.low[at];
+                const int up = s.up[low];
+                above += at - low + (up == 255 ? 0 : 1);
                 at = up == 255 ? -1 : up;
             }
+            row.first = window_first(max(s.context + above, 0), p.window);
+            __syncwarp();
         }
-        row.first = window_first(max(s.context + depth - 1, 0), p.window);
-        __syncwarp();
 
         float m = -INFINITY, l = 0.0f;
         int mine = 0;  // scores of this piece taken
@@ -1206,26 +1278,34 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, Shared& sh, Excha
             ++steps;
             const Listed& aux = sh.list[slot];
             if (aux.full == 0) {
-                const int key0 = aux.key0;
-                const uint32_t gone = aux.gone;
                 // What the row does not see becomes -inf.
+                const uint4 keep4 = kept_columns(p, s, row, aux.key0, aux.gone);
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     uint32_t x[32];
+                    __syncwarp();
                     tmem_ld32(tmem_s + 32 * c, x);
                     tmem_wait_ld();
-                    const uint32_t keep = kept_columns<C>(p, s, row, key0 + 32 * c, gone >> (4 * c));
+                    const uint32_t keep = c == 0 ? keep4.x : c == 1 ? keep4.y : c == 2 ? keep4.z : keep4.w;
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         x[i] = (keep >> i) & 1u ? x[i] : 0xff800000u;
                     }
-                    __syncwarp();
                     tmem_st32(tmem_s + 32 * c, x);
                 }
                 tmem_wait_st();
             }
-            const float alpha = C::E4M3 && !coarse ? exponentials<C, 8>(aux, tmem_s, row.factor, m, l)
-                                                   : exponentials<C, 32>(aux, tmem_s, row.factor, m, l);
+            bool ok = true;
+            auto taken = [&] {
+                tc_fence_before();
+                arrive(&sh.s_free[w]);
+            };
+            auto room = [&] { return ok = steps == 1 || wait(&sh.p_free[w], steps - 2); };
+            const float alpha = C::E4M3 && !coarse ? exponentials<C, 8>(aux, tmem_s, tmem_p, row.factor, m, l, taken, room)
+                                                   : exponentials<C, 32>(aux, tmem_s, tmem_p, row.factor, m, l, taken, room);
+            if (!ok) {
+                return;
+            }
             if (mine > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
@@ -1358,18 +1438,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         }
         for (int i = 0; i < kParts; ++i) {
             mbar_init(smem_u32(&sh.part_full[i]), 1);
-            mbar_init(smem_u32(&sh.part_empty[i]), kSoftmaxWarps + 1);
+            mbar_init(smem_u32(&sh.part_empty[i]), kSoftmaxWarps + 2);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&sh.s_full[i]), 1);
+            mbar_init(smem_u32(&sh.s_free[i]), kSoftmaxWarps / 2);
             mbar_init(smem_u32(&sh.p_full[i]), kSoftmaxWarps / 2);
+            mbar_init(smem_u32(&sh.p_free[i]), 1);
         }
         mbar_init(smem_u32(&sh.q_full), kSoftmaxWarps);
         mbar_init(smem_u32(&sh.q_empty), 1);
         mbar_init(smem_u32(&sh.done), 1);
         mbar_init(smem_u32(&sh.o_free), kSoftmaxWarps);
         mbar_init(smem_u32(&sh.ml_full), kSoftmaxWarps);
-        mbar_init(smem_u32(&sh.mma_idle), 1);
+        mbar_init(smem_u32(&sh.mma_idle), 2);
         mbar_fence_init();
     }
     if (warp == kMmaWarp) {
@@ -1394,12 +1476,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             softmax<C>(p, sh, *reinterpret_cast<Exchange*>(&sh + 1), smem_u32(smem), rec, wctx);
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-            if (warp < kMmaWarp) {
+            if (warp < kScoreWarp) {
                 ready_values<C>(p, sh, smem_u32(smem), wctx);
+            } else if (warp == kScoreWarp) {
+                score_warp<C>(sh, smem_u32(smem), wctx);
             } else if (warp == kMmaWarp) {
-                issue_products<C>(sh, smem_u32(smem), wctx);
-            } else if (warp == kPartWarp) {
-                list_parts(p, split, status, start_walk(p, split, range, static_cast<int>(blockIdx.x)), sh, wctx);
+                product_warp<C>(sh, smem_u32(smem), wctx);
             } else {
                 const Walk walk = start_walk(p, split, range, static_cast<int>(blockIdx.x));
                 list_tiles<C>(p, &tm_k, &tm_v, split, status, walk, sh, smem_u32(smem), warp - kListWarp, wctx);
@@ -1449,9 +1531,10 @@ __global__ void __launch_bounds__(kRowWarps * 32) tree_finish_kernel(const __gri
             return;
         }
         const Sequence s = sequence(p, range.found);
-        const long long item = (k * range.per - range.found_base) / s.tiles;
-        const long long start = range.found_base + item * s.tiles;
-        if (start == k * range.per || start / range.per != k - 1) {
+        const long long item = (k * range.per - range.found_base) / (s.tiles + kItemHead);
+        const long long head = range.found_base + item * (s.tiles + kItemHead);
+        const long long start = head + kItemHead;  // of its tiles
+        if (start >= k * range.per || start / range.per != k - 1) {
             return;
         }
         const int kvh = static_cast<int>(item / split.row_blocks);
@@ -1474,7 +1557,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) tree_finish_kernel(const __gri
 #pragma unroll 4
         for (long long c = c0; c <= c1; ++c) {
             // A CTA's first cut piece is its record 0; the item starts in c0, as its second unless there.
-            const long long record = 2 * c + (c * range.per >= start ? 0 : 1);
+            const long long record = 2 * c + (c * range.per >= head ? 0 : 1);
             odd = odd || (rec.odd != nullptr && rec.odd[c] != 0);
             const float2 ml = rec.ml[record * C::kRows + r];
             const float4* from = reinterpret_cast<const float4*>(rec.o) + (record * (D / 4) + 2 * eight) * C::kRows + r;
