@@ -467,6 +467,41 @@ __device__ __forceinline__ bool next_piece(const FaTreeParams& p, const Split& s
     return true;
 }
 
+// What a wait that was given up leaves word of.
+struct Waits {
+    volatile int* abort;  // of the CTA, in shared memory
+    unsigned* code;
+};
+
+// A bounded wait of a whole warp: 2^20 polls of at most a microsecond. In few instructions, for there are many of them and the
+// kernel's loops have to fit the instruction cache. False: given up, by this warp or another of the CTA.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, int phase, const Waits& waits, unsigned code) {
+    const uint32_t at = smem_u32(bar);
+    const uint32_t parity = static_cast<uint32_t>(phase) & 1u;
+    bool there = false;
+#pragma unroll 1
+    for (int i = 0; i < (1 << 20); ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(at), "r"(parity)
+            : "memory");
+        there = done != 0;
+        if (there || *waits.abort != 0) {
+            break;
+        }
+    }
+    there = __all_sync(0xffffffffu, there) != 0;
+    if (!there && *waits.abort == 0) {
+        *waits.abort = 1;
+        atomicOr(waits.code, code);
+    }
+    return there;
+}
+
 // Nonzero if a word of cache elements holds one that is not finite.
 template <class C>
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
@@ -510,11 +545,10 @@ __device__ __forceinline__ uint4 load_shared16(uint32_t at) {
 
 // A piece listed for the softmax and the products; n = 0: the end.
 __device__ __forceinline__ bool list_part(const FaTreeParams& p, DeviceStatus* status, Shared& sh, int part, const Piece& piece, const Sequence& s,
-                                          int n, const WaitCtx& wctx) {
+                                          int n, const Waits& waits) {
     const int lane = static_cast<int>(threadIdx.x) % 32;
     Part& to = sh.part[part % kParts];
-    const bool ok = mbar_wait(smem_u32(&sh.part_empty[part % kParts]), ((part / kParts) & 1) ^ 1, wctx, kStatusTimeoutProducer);
-    if (__all_sync(0xffffffffu, ok) == 0) {
+    if (!warp_wait(&sh.part_empty[part % kParts], part / kParts + 1, waits, kStatusTimeoutProducer)) {
         return false;
     }
     if (n > 0) {
@@ -569,7 +603,7 @@ __device__ __forceinline__ bool list_part(const FaTreeParams& p, DeviceStatus* s
 // that the loads of pages and scales of two tiles are on their way at once.
 template <class C>
 __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensorMap* tm_k, const CUtensorMap* tm_v, const Split& split,
-                                           DeviceStatus* status, Walk walk, Shared& sh, uint32_t smem, int which, const WaitCtx& wctx) {
+                                           DeviceStatus* status, Walk walk, Shared& sh, uint32_t smem, int which, const Waits& waits) {
     const FaCache& c = p.cache;
     const int lane = static_cast<int>(threadIdx.x) % 32;
     const int log2_page = 31 - __clz(c.page_size);
@@ -584,14 +618,14 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensor
     int turn = which;  // the tile that is this warp's
     int parts = 0;
     auto wait = [&](uint64_t* bar, int phase) {
-        return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), (phase & 1) ^ 1, wctx, kStatusTimeoutProducer)) != 0;
+        return warp_wait(bar, phase + 1, waits, kStatusTimeoutProducer);
     };
     while (true) {
         bool more = true;
         if (++v >= piece.v1) {
             more = next_piece(p, split, walk, piece, s);
             v = piece.v0;
-            if (which == 0 && !list_part(p, status, sh, parts++, piece, s, more ? piece.v1 - piece.v0 : 0, wctx)) {
+            if (which == 0 && !list_part(p, status, sh, parts++, piece, s, more ? piece.v1 - piece.v0 : 0, waits)) {
                 return;
             }
         }
@@ -701,14 +735,14 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensor
 // V's tiles made ready: e4m3 values widened to float16 and laid out for the product, rows that no row of the call sees made
 // zeros (0 times what lies there could be NaN), and what is not finite noticed where rows differ in what they see.
 template <class C>
-__device__ __forceinline__ void ready_values(const FaTreeParams& p, Shared& sh, uint32_t smem, const WaitCtx& wctx) {
+__device__ __forceinline__ void ready_values(const FaTreeParams& p, Shared& sh, uint32_t smem, const Waits& waits) {
     constexpr int kRing = C::E4M3 ? C::kRStages : C::kVStages;
     constexpr int kChunks = C::D * C::kElem / 16;  // 16-byte words of a row
     const int lt = static_cast<int>(threadIdx.x) % 128;
     const int lane = lt % 32;
     const int warp = lt / 32;
     auto wait = [&](uint64_t* bar, int phase) {
-        return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), phase & 1, wctx, kStatusTimeoutProducer)) != 0;
+        return warp_wait(bar, phase, waits, kStatusTimeoutProducer);
     };
     bool odd = false;
     for (int n = 0;; ++n) {
@@ -732,42 +766,45 @@ __device__ __forceinline__ void ready_values(const FaTreeParams& p, Shared& sh, 
             if (!wait(&sh.v_empty[n % C::kVStages], n / C::kVStages + 1)) {
                 break;
             }
+            if (mixed || !whole || tiny != 0) {
+                // The warp's rows as the cache holds them, in place (wherever the swizzle has a word in its row).
+                uint32_t any = 0;
+#pragma unroll 1
+                for (int i = warp * 32 * kChunks + lane; i < (warp + 1) * 32 * kChunks; i += 32) {
+                    const int r = i / kChunks;
+                    uint4 w = load_shared16(raw + i * 16);
+                    if (!((shown[r >> 5] >> (r & 31)) & 1u)) {
+                        w = make_uint4(0u, 0u, 0u, 0u);
+                    } else if ((tiny >> (r >> 3)) & 1u) {  // NaN stays
+                        w = make_uint4(w.x & (not_finite<C>(w.x) >> 7) * 255u, w.y & (not_finite<C>(w.y) >> 7) * 255u,
+                                       w.z & (not_finite<C>(w.z) >> 7) * 255u, w.w & (not_finite<C>(w.w) >> 7) * 255u);
+                    }
+                    any |= not_finite<C>(w.x) | not_finite<C>(w.y) | not_finite<C>(w.z) | not_finite<C>(w.w);
+                    store_shared16(raw + i * 16, w.x, w.y, w.z, w.w);
+                }
+                odd = odd || (mixed && any != 0);
+                __syncwarp();
+            }
             // Words of 8 lanes that load and store together: D = 128, half a row of rows r and r ^ 5, which the swizzles of
             // 128-byte rows (codes: by r, values: two chunks apart) put into different banks; D = 64, two rows.
             constexpr int kPasses = kTile * kChunks / 128;
-#pragma unroll
+#pragma unroll 1
             for (int i0 = 0; i0 < kPasses; i0 += 4) {
                 uint4 w[4];
-                int r[4], chunk;
+                uint32_t to[4];
+                const int chunk = C::D == 128 ? (lane & 3) + ((lane >> 1) & 4) : lane & 3;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int pass = i0 + i;
+                    int r;
                     if constexpr (C::D == 128) {
-                        const int a = 2 * (pass & 1) + (lane >> 4);
-                        r[i] = warp * 32 + (pass >> 1) * 8 + ((lane & 4) != 0 ? a ^ 5 : a);
-                        chunk = (lane & 3) + ((lane >> 1) & 4);
-                        w[i] = load_shared16(raw + code_offset<128>(r[i], chunk));
+                        const int a = 2 * (i & 1) + (lane >> 4);
+                        r = warp * 32 + ((i0 + i) >> 1) * 8 + ((lane & 4) != 0 ? a ^ 5 : a);
+                        w[i] = load_shared16(raw + code_offset<128>(r, chunk));
                     } else {
-                        r[i] = warp * 32 + pass * 8 + (lane >> 2);
-                        chunk = lane & 3;
-                        w[i] = load_shared16(raw + r[i] * 64 + chunk * 16);
+                        r = warp * 32 + (i0 + i) * 8 + (lane >> 2);
+                        w[i] = load_shared16(raw + r * 64 + chunk * 16);
                     }
-                }
-                if (mixed || !whole || tiny != 0) {
-                    uint32_t any = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (!((shown[r[i] >> 5] >> (r[i] & 31)) & 1u)) {
-                            w[i] = make_uint4(0u, 0u, 0u, 0u);
-                        } else if ((tiny >> (r[i] >> 3)) & 1u) {  // NaN stays
-                            w[i].x &= (not_finite<C>(w[i].x) >> 7) * 255u;
-                            w[i].y &= (not_finite<C>(w[i].y) >> 7) * 255u;
-                            w[i].z &= (not_finite<C>(w[i].z) >> 7) * 255u;
-                            w[i].w &= (not_finite<C>(w[i].w) >> 7) * 255u;
-                        }
-                        any |= not_finite<C>(w[i].x) | not_finite<C>(w[i].y) | not_finite<C>(w[i].z) | not_finite<C>(w[i].w);
-                    }
-                    odd = odd || (mixed && any != 0);
+                    to[i] = wide + tile_offset(r, 2 * chunk);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -776,8 +813,8 @@ __device__ __forceinline__ void ready_values(const FaTreeParams& p, Shared& sh, 
                     widen4(w[i].y, h[2], h[3]);
                     widen4(w[i].z, h[4], h[5]);
                     widen4(w[i].w, h[6], h[7]);
-                    store_shared16(wide + tile_offset(r[i], 2 * chunk), h[0], h[1], h[2], h[3]);
-                    store_shared16(wide + tile_offset(r[i], 2 * chunk + 1), h[4], h[5], h[6], h[7]);
+                    store_shared16(to[i], h[0], h[1], h[2], h[3]);
+                    store_shared16(to[i] ^ 16u, h[4], h[5], h[6], h[7]);  // the odd chunk of the pair
                 }
             }
             fence_proxy_async_smem();
@@ -846,9 +883,9 @@ __device__ __forceinline__ void issue_product(uint32_t acc, uint32_t w, uint64_t
 // memory, come to about 300 cycles even for what is there, so that one warp for both is what the kernel would wait for. Step
 // s is key tile s (NR 1) or row tile s % 2 of key tile s / 2 (NR 2), warpgroup s % 2's.
 template <class C, class Scores>
-__device__ __forceinline__ bool walk_parts(Shared& sh, const WaitCtx& wctx, Scores take) {
+__device__ __forceinline__ bool walk_parts(Shared& sh, const Waits& waits, Scores take) {
     for (int items = 0, tiles = 0;; ++items) {
-        if (__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.part_full[items % kParts]), (items / kParts) & 1, wctx, kStatusTimeoutMma)) == 0) {
+        if (!warp_wait(&sh.part_full[items % kParts], items / kParts, waits, kStatusTimeoutMma)) {
             return false;
         }
         const int n = sh.part[items % kParts].n;
@@ -867,14 +904,14 @@ __device__ __forceinline__ bool walk_parts(Shared& sh, const WaitCtx& wctx, Scor
     }
 }
 
-__device__ __forceinline__ bool mma_wait(uint64_t* bar, int parity, const WaitCtx& wctx) {
-    const bool there = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity & 1, wctx, kStatusTimeoutMma)) != 0;
+__device__ __forceinline__ bool mma_wait(uint64_t* bar, int parity, const Waits& waits) {
+    const bool there = warp_wait(bar, parity, waits, kStatusTimeoutMma);
     tc_fence_after();
     return there;
 }
 
 template <class C>
-__device__ __forceinline__ void score_warp(Shared& sh, uint32_t smem, const WaitCtx& wctx) {
+__device__ __forceinline__ void score_warp(Shared& sh, uint32_t smem, const Waits& waits) {
     constexpr int NR = C::NR;
     auto kmajor = [](uint32_t at) { return C::E4M3 && C::D == 64 ? make_desc_kmajor_sw64(at) : make_desc_kmajor_sw128(at); };
     const uint64_t q = kmajor(smem + C::kSmemQ);
@@ -882,18 +919,18 @@ __device__ __forceinline__ void score_warp(Shared& sh, uint32_t smem, const Wait
     auto off = [](int tile, int bytes) { return static_cast<uint64_t>(tile * (bytes >> 4)); };
     int done0 = 0, done1 = 0;  // scores of either warpgroup
     int last = -1;             // whose were the last
-    walk_parts<C>(sh, wctx, [&](int items, int tiles, int steps) {
-        if (!mma_wait(&sh.q_full, items, wctx)) {
+    walk_parts<C>(sh, waits, [&](int items, int tiles, int steps) {
+        if (!mma_wait(&sh.q_full, items, waits)) {
             return false;
         }
 #pragma unroll 1
         for (int step = 0; step < steps; ++step) {
             const int tile = tiles + (NR == 1 ? step : step >> 1);
             const int w = step & 1;
-            if ((NR == 1 || w == 0) && !mma_wait(&sh.k_full[tile % C::kKStages], tile / C::kKStages, wctx)) {
+            if ((NR == 1 || w == 0) && !mma_wait(&sh.k_full[tile % C::kKStages], tile / C::kKStages, waits)) {
                 return false;
             }
-            if (last >= 0 && !mma_wait(&sh.s_free[last], (last == 0 ? done0 : done1) - 1, wctx)) {
+            if (last >= 0 && !mma_wait(&sh.s_free[last], (last == 0 ? done0 : done1) - 1, waits)) {
                 return false;
             }
             if (elect_one()) {
@@ -921,22 +958,22 @@ __device__ __forceinline__ void score_warp(Shared& sh, uint32_t smem, const Wait
 }
 
 template <class C>
-__device__ __forceinline__ void product_warp(Shared& sh, uint32_t smem, const WaitCtx& wctx) {
+__device__ __forceinline__ void product_warp(Shared& sh, uint32_t smem, const Waits& waits) {
     constexpr int NR = C::NR;
     const uint64_t v = make_desc_mnmajor_sw128(smem + C::kSmemV, kBox);
     int taken0 = 0, taken1 = 0;  // P of either warpgroup
-    walk_parts<C>(sh, wctx, [&](int items, int tiles, int steps) {
-        if (items > 0 && !mma_wait(&sh.o_free, items - 1, wctx)) {
+    walk_parts<C>(sh, waits, [&](int items, int tiles, int steps) {
+        if (items > 0 && !mma_wait(&sh.o_free, items - 1, waits)) {
             return false;
         }
 #pragma unroll 1
         for (int step = 0; step < steps; ++step) {
             const int tile = tiles + (NR == 1 ? step : step >> 1);
             const int w = step & 1;
-            if ((NR == 1 || w == 0) && !mma_wait(&sh.v_full[tile % C::kVStages], tile / C::kVStages, wctx)) {
+            if ((NR == 1 || w == 0) && !mma_wait(&sh.v_full[tile % C::kVStages], tile / C::kVStages, waits)) {
                 return false;
             }
-            if (!mma_wait(&sh.p_full[w], w == 0 ? taken0++ : taken1++, wctx)) {
+            if (!mma_wait(&sh.p_full[w], w == 0 ? taken0++ : taken1++, waits)) {
                 return false;
             }
             if (elect_one()) {
@@ -958,7 +995,8 @@ __device__ __forceinline__ void product_warp(Shared& sh, uint32_t smem, const Wa
         umma_commit(smem_u32(&sh.mma_idle));
     }
     __syncwarp();
-    mbar_wait_drain(smem_u32(&sh.mma_idle), 0, wctx, kStatusTimeoutTeardown);
+    unsigned unused = 0;  // no other CTA listens
+    mbar_wait_drain(smem_u32(&sh.mma_idle), 0, WaitCtx{&sh.abort, waits.code, &unused, 0}, kStatusTimeoutTeardown);
     __syncwarp();
 }
 
@@ -1185,7 +1223,7 @@ __device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s
 
 template <class C>
 __device__ __forceinline__ void softmax(const FaTreeParams& p, Shared& sh, Exchange& ex, uint32_t smem, const Record& rec,
-                                        const WaitCtx& wctx) {
+                                        const Waits& waits) {
     constexpr int D = C::D;
     constexpr int NR = C::NR;
     const int lane = static_cast<int>(threadIdx.x) % 32;
@@ -1199,7 +1237,7 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, Shared& sh, Excha
     const int group = p.heads / p.cache.kv_heads;
     const int rows = group * p.cache.tokens;
     auto wait = [&](uint64_t* bar, int parity) {
-        const bool there = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity & 1, wctx, kStatusTimeoutSoftmax)) != 0;
+        const bool there = warp_wait(bar, parity, waits, kStatusTimeoutSoftmax);
         tc_fence_after();
         return there;
     };
@@ -1417,7 +1455,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     uint8_t* smem = raw;  // on 1024 bytes: a kernel without static shared memory has it from there
     Shared& sh = *reinterpret_cast<Shared*>(smem + C::kSmemShared);
     const int warp = static_cast<int>(threadIdx.x) / 32;
-    const WaitCtx wctx{&sh.abort, &status->code, &status->epoch_aborted, epoch};
+    const Waits waits{&sh.abort, &status->code};
     cudaTriggerProgrammaticLaunchCompletion();  // the second kernel's CTAs may take SMs as they get free
     if (threadIdx.x == 0) {
         sh.abort = 0;
@@ -1473,18 +1511,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     } else {
         if (warp < kSoftmaxWarps) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-            softmax<C>(p, sh, *reinterpret_cast<Exchange*>(&sh + 1), smem_u32(smem), rec, wctx);
+            softmax<C>(p, sh, *reinterpret_cast<Exchange*>(&sh + 1), smem_u32(smem), rec, waits);
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
             if (warp < kScoreWarp) {
-                ready_values<C>(p, sh, smem_u32(smem), wctx);
+                ready_values<C>(p, sh, smem_u32(smem), waits);
             } else if (warp == kScoreWarp) {
-                score_warp<C>(sh, smem_u32(smem), wctx);
+                score_warp<C>(sh, smem_u32(smem), waits);
             } else if (warp == kMmaWarp) {
-                product_warp<C>(sh, smem_u32(smem), wctx);
+                product_warp<C>(sh, smem_u32(smem), waits);
             } else {
                 const Walk walk = start_walk(p, split, range, static_cast<int>(blockIdx.x));
-                list_tiles<C>(p, &tm_k, &tm_v, split, status, walk, sh, smem_u32(smem), warp - kListWarp, wctx);
+                list_tiles<C>(p, &tm_k, &tm_v, split, status, walk, sh, smem_u32(smem), warp - kListWarp, waits);
                 // Copies in flight end by themselves; after a wait that was given up they get a millisecond.
                 if (sh.abort != 0) {
                     const unsigned long long t0 = globaltimer_ns();
