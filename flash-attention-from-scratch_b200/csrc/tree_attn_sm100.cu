@@ -1025,24 +1025,36 @@ __device__ __forceinline__ float bring_queries(const FaTreeParams& p, const uint
     const uint32_t sign = p.softmax_scale < 0.0f ? 0x80008000u : 0u;  // the factor stays positive
     const float scale = fmaxf(fabsf(p.softmax_scale) * kLog2e, kLeastFactor);
     float factor = scale;
-    uint4 word[kPasses][2];
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-        const uint64_t from = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(at), row0 + i * kAtOnce);
-        const bool there = __shfl_sync(0xffffffffu, static_cast<int>(real), row0 + i * kAtOnce) != 0;
+    uint4 word[2][2], next[2][2];
+    auto load = [&](int pass, uint4 (&to)[2]) {
+        const uint64_t from = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(at), (row0 + pass * kAtOnce) & 31);
+        const bool there = __shfl_sync(0xffffffffu, static_cast<int>(real), (row0 + pass * kAtOnce) & 31) != 0;
         const uint4* src = reinterpret_cast<const uint4*>(from) + 2 * part;
-        word[i][0] = there ? __ldg(src) : make_uint4(0u, 0u, 0u, 0u);
-        word[i][1] = there ? __ldg(src + 1) : make_uint4(0u, 0u, 0u, 0u);
-    }
+        to[0] = there ? __ldg(src) : make_uint4(0u, 0u, 0u, 0u);
+        to[1] = there ? __ldg(src + 1) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    load(0, next[0]);
+    load(1, next[1]);
     if (!ready()) {
         return factor;
     }
+#pragma unroll 1
+    for (int pass0 = 0; pass0 < kPasses; pass0 += 2) {
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
+        for (int e = 0; e < 2; ++e) {
+            word[e][0] = next[e][0];
+            word[e][1] = next[e][1];
+            if (pass0 + 2 < kPasses) {
+                load(pass0 + 2 + e, next[e]);
+            }
+        }
+#pragma unroll
+      for (int e2 = 0; e2 < 2; ++e2) {
+        const int i = pass0 + e2;
         const int owner = row0 + i * kAtOnce;
         const int r = quarter * 32 + owner;
-        const uint32_t x[8] = {word[i][0].x ^ sign, word[i][0].y ^ sign, word[i][0].z ^ sign, word[i][0].w ^ sign,
-                               word[i][1].x ^ sign, word[i][1].y ^ sign, word[i][1].z ^ sign, word[i][1].w ^ sign};
+        const uint32_t x[8] = {word[e2][0].x ^ sign, word[e2][0].y ^ sign, word[e2][0].z ^ sign, word[e2][0].w ^ sign,
+                               word[e2][1].x ^ sign, word[e2][1].y ^ sign, word[e2][1].z ^ sign, word[e2][1].w ^ sign};
         if constexpr (!C::E4M3) {
             store_shared16(tile + tile_offset(r, 2 * part), x[0], x[1], x[2], x[3]);
             store_shared16(tile + tile_offset(r, 2 * part + 1), x[4], x[5], x[6], x[7]);
@@ -1095,6 +1107,7 @@ __device__ __forceinline__ float bring_queries(const FaTreeParams& p, const uint
                 store_shared16(tile + term * C::kRaw + code_offset<C::D>(r, part), code[0], code[1], code[2], code[3]);
             }
         }
+      }
     }
     fence_proxy_async_smem();
     return factor;
@@ -1134,9 +1147,55 @@ __device__ __forceinline__ uint4 kept_columns(const FaTreeParams& p, const Part&
     return make_uint4(keep[0], keep[1], keep[2], keep[3]);
 }
 
-// One row's scores turned into P: returns what the sums so far (and l, done here) shrink by. GROUP: keys that share a page,
-// and with it the scales. taken() once the scores are in registers, room() before P is stored.
-template <class C, int GROUP, class Taken, class Room>
+// The largest of one group of GROUP scores.
+template <int GROUP, int N>
+__device__ __forceinline__ float group_most(const uint32_t (&x)[N], int at) {
+    float most[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        most[i] = fmax_nan(u2f(x[at + i]), u2f(x[at + 4 + i]));
+    }
+#pragma unroll
+    for (int j = 8; j < GROUP; j += 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            most[i] = fmax3(most[i], u2f(x[at + j + i]), u2f(x[at + j + 4 + i]));
+        }
+    }
+    return fmax_nan(fmax3(most[0], most[1], most[2]), most[3]);
+}
+
+// P of one group, in pairs of 16 bits, and its share of the sum.
+template <class C, int GROUP, int N>
+__device__ __forceinline__ void group_exponentials(const uint32_t (&x)[N], int at, uint32_t* packed, float f, float add, float inv, float& l) {
+    const float2 f2 = make_float2(f, f), add2 = make_float2(add, add);
+    float2 sum[4];
+#pragma unroll
+    for (int i = 0; i < GROUP / 2; ++i) {
+        float2 y = __ffma2_rn(make_float2(u2f(x[at + 2 * i]), u2f(x[at + 2 * i + 1])), f2, add2);
+        y = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+        sum[i & 3] = i < 4 ? y : __fadd2_rn(sum[i & 3], y);
+        packed[i] = pack2<C::kMmaBf16>(y.x, y.y);
+    }
+    const float2 all = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
+    l = fmaf(all.x + all.y, inv, l);
+}
+
+// The new maximum, and what the sums so far shrink by.
+__device__ __forceinline__ float raise(float top, float& m, float& l) {
+    float alpha = 1.0f;
+    if (!(top <= m + kLazy)) {  // NaN among it
+        alpha = ex2_approx(m - top);
+        m = top;
+    }
+    l *= alpha;
+    return alpha;
+}
+
+// One row's scores turned into P: returns what the sums so far shrink by (l is done here). taken() once the scores are in
+// registers for good, room() before P is stored. All 128 at once, so that the next tile's scores can follow, where 32 keys on
+// end share a page and its scales (or there are none).
+template <class C, class Taken, class Room>
 __device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s, uint32_t tmem_p, float factor, float& m, float& l, Taken taken,
                                               Room room) {
     uint32_t x[128];
@@ -1144,79 +1203,74 @@ __device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s
     tmem_ld64_of128<64>(tmem_s + 64, x);
     tmem_wait_ld();
     taken();
-    float top;
+    float top = -INFINITY;
     if constexpr (C::E4M3) {
-        top = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < kTile / GROUP; ++g) {
-            float most[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                most[i] = fmax_nan(u2f(x[GROUP * g + i]), u2f(x[GROUP * g + 4 + i]));
-            }
-#pragma unroll
-            for (int j = 8; j < GROUP; j += 8) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    most[i] = fmax3(most[i], u2f(x[GROUP * g + j + i]), u2f(x[GROUP * g + j + 4 + i]));
-                }
-            }
-            const float2 a = *reinterpret_cast<const float2*>(&aux.group[g * GROUP / 8]);
-            const float all = fmax_nan(fmax3(most[0], most[1], most[2]), most[3]);
-            top = fmax_nan(top, fmaf(all, fmaxf(factor * a.x, kLeastFactor), a.y));
+        for (int c = 0; c < 4; ++c) {
+            const float2 a = *reinterpret_cast<const float2*>(&aux.group[4 * c]);
+            top = fmax_nan(top, fmaf(group_most<32>(x, 32 * c), fmaxf(factor * a.x, kLeastFactor), a.y));
         }
     } else {
         top = row_extreme<true, 128>(x) * factor;
     }
-    float alpha = 1.0f;
-    if (!(top <= m + kLazy)) {  // NaN among it
-        alpha = ex2_approx(m - top);
-        m = top;
-    }
+    const float alpha = raise(top, m, l);
     const float used = m == -INFINITY ? 0.0f : m;
-    l *= alpha;
     if (!room()) {
         return alpha;
     }
     __syncwarp();  // tensor memory is accessed by whole warps
 #pragma unroll
-    for (int g = 0; g < kTile / GROUP; ++g) {
+    for (int c = 0; c < 4; ++c) {
         float f = factor, add = -used, inv = 1.0f;
         if constexpr (C::E4M3) {
-            const float4 a = aux.group[g * GROUP / 8];
+            const float4 a = aux.group[4 * c];
             f = fmaxf(f * a.x, kLeastFactor);
             add = a.y - used;
             inv = a.z;
         }
-        const float2 f2 = make_float2(f, f), add2 = make_float2(add, add);
-        float2 sum[4];
+        uint32_t packed[16];  // P of 32 keys takes 16 columns
+        group_exponentials<C, 32>(x, 32 * c, packed, f, add, inv, l);
+        tmem_st16(tmem_p + 16 * c, packed);
+    }
+    return alpha;
+}
+
+// The same over pages of 8 or 16 tokens, in few registers.
+template <class C, class Taken, class Room>
+__device__ __forceinline__ float exponentials_by_8(const Listed& aux, uint32_t tmem_s, uint32_t tmem_p, float factor, float& m, float& l, Taken taken,
+                                                   Room room) {
+    float top = -INFINITY;
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        uint32_t x[32];
+        tmem_ld32(tmem_s + 32 * c, x);
+        tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < GROUP / 2; ++i) {
-            uint32_t* at = &x[GROUP * g + 2 * i];
-            float2 y = __ffma2_rn(make_float2(u2f(at[0]), u2f(at[1])), f2, add2);
-            y = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-            sum[i & 3] = i < 4 ? y : __fadd2_rn(sum[i & 3], y);
-            at[0] = f2u(y.x);
-            at[1] = f2u(y.y);
+        for (int g = 0; g < 4; ++g) {
+            const float2 a = *reinterpret_cast<const float2*>(&aux.group[4 * c + g]);
+            top = fmax_nan(top, fmaf(group_most<8>(x, 8 * g), fmaxf(factor * a.x, kLeastFactor), a.y));
         }
-        const float2 all = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
-        l = fmaf(all.x + all.y, inv, l);
-        // P of 32 keys takes 16 columns.
-        if constexpr (GROUP == 32) {
-            uint32_t packed[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                packed[i] = pack2<C::kMmaBf16>(u2f(x[32 * g + 2 * i]), u2f(x[32 * g + 2 * i + 1]));
-            }
-            tmem_st16(tmem_p + 16 * g, packed);
-        } else if (g % 4 == 3) {
-            uint32_t packed[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                packed[i] = pack2<C::kMmaBf16>(u2f(x[8 * (g - 3) + 2 * i]), u2f(x[8 * (g - 3) + 2 * i + 1]));
-            }
-            tmem_st16(tmem_p + 16 * (g / 4), packed);
+    }
+    const float alpha = raise(top, m, l);
+    const float used = m == -INFINITY ? 0.0f : m;
+    if (!room()) {
+        return alpha;
+    }
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        uint32_t x[32], packed[16];
+        __syncwarp();
+        tmem_ld32(tmem_s + 32 * c, x);
+        tmem_wait_ld();
+        if (c == 3) {
+            taken();
         }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float4 a = aux.group[4 * c + g];
+            group_exponentials<C, 8>(x, 8 * g, packed + 4 * g, fmaxf(factor * a.x, kLeastFactor), a.y - used, a.z, l);
+        }
+        tmem_st16(tmem_p + 16 * c, packed);
     }
     return alpha;
 }
@@ -1339,8 +1393,8 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, Shared& sh, Excha
                 arrive(&sh.s_free[w]);
             };
             auto room = [&] { return ok = steps == 1 || wait(&sh.p_free[w], steps - 2); };
-            const float alpha = C::E4M3 && !coarse ? exponentials<C, 8>(aux, tmem_s, tmem_p, row.factor, m, l, taken, room)
-                                                   : exponentials<C, 32>(aux, tmem_s, tmem_p, row.factor, m, l, taken, room);
+            const float alpha = C::E4M3 && !coarse ? exponentials_by_8<C>(aux, tmem_s, tmem_p, row.factor, m, l, taken, room)
+                                                   : exponentials<C>(aux, tmem_s, tmem_p, row.factor, m, l, taken, room);
             if (!ok) {
                 return;
             }
