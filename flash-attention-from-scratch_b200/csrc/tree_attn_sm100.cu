@@ -1193,11 +1193,10 @@ __device__ __forceinline__ float raise(float top, float& m, float& l) {
 }
 
 // One row's scores turned into P: returns what the sums so far shrink by (l is done here). taken() once the scores are in
-// registers for good, room() before P is stored. All 128 at once, so that the next tile's scores can follow, where 32 keys on
+// registers for good. All 128 at once, so that the next tile's scores can follow, where 32 keys on
 // end share a page and its scales (or there are none).
-template <class C, class Taken, class Room>
-__device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s, uint32_t tmem_p, float factor, float& m, float& l, Taken taken,
-                                              Room room) {
+template <class C, class Taken>
+__device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s, uint32_t tmem_p, float factor, float& m, float& l, Taken taken) {
     uint32_t x[128];
     tmem_ld64_of128<0>(tmem_s, x);
     tmem_ld64_of128<64>(tmem_s + 64, x);
@@ -1215,9 +1214,6 @@ __device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s
     }
     const float alpha = raise(top, m, l);
     const float used = m == -INFINITY ? 0.0f : m;
-    if (!room()) {
-        return alpha;
-    }
     __syncwarp();  // tensor memory is accessed by whole warps
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -1236,9 +1232,8 @@ __device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s
 }
 
 // The same over pages of 8 or 16 tokens, in few registers.
-template <class C, class Taken, class Room>
-__device__ __forceinline__ float exponentials_by_8(const Listed& aux, uint32_t tmem_s, uint32_t tmem_p, float factor, float& m, float& l, Taken taken,
-                                                   Room room) {
+template <class C, class Taken>
+__device__ __forceinline__ float exponentials_by_8(const Listed& aux, uint32_t tmem_s, uint32_t tmem_p, float factor, float& m, float& l, Taken taken) {
     float top = -INFINITY;
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
@@ -1253,9 +1248,6 @@ __device__ __forceinline__ float exponentials_by_8(const Listed& aux, uint32_t t
     }
     const float alpha = raise(top, m, l);
     const float used = m == -INFINITY ? 0.0f : m;
-    if (!room()) {
-        return alpha;
-    }
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
         uint32_t x[32], packed[16];
@@ -1364,7 +1356,9 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, Shared& sh, Excha
         int mine = 0;  // scores of this piece taken
         for (int t = NR == 1 ? w : 0; t < n; t += NR == 1 ? 2 : 1, ++mine) {
             const int slot = (tiles + t) % kListed;
-            if (!wait(&sh.list_full[slot], (tiles + t) / kListed) || !wait(&sh.s_full[w], steps)) {
+            // P's place is free and the tile listed by the time its scores are there, most of the time.
+            if ((steps > 0 && !wait(&sh.p_free[w], steps - 1)) || !wait(&sh.s_full[w], steps) ||
+                !wait(&sh.list_full[slot], (tiles + t) / kListed)) {
                 return;
             }
             ++steps;
@@ -1387,17 +1381,12 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, Shared& sh, Excha
                 }
                 tmem_wait_st();
             }
-            bool ok = true;
             auto taken = [&] {
                 tc_fence_before();
                 arrive(&sh.s_free[w]);
             };
-            auto room = [&] { return ok = steps == 1 || wait(&sh.p_free[w], steps - 2); };
-            const float alpha = C::E4M3 && !coarse ? exponentials_by_8<C>(aux, tmem_s, tmem_p, row.factor, m, l, taken, room)
-                                                   : exponentials<C>(aux, tmem_s, tmem_p, row.factor, m, l, taken, room);
-            if (!ok) {
-                return;
-            }
+            const float alpha = C::E4M3 && !coarse ? exponentials_by_8<C>(aux, tmem_s, tmem_p, row.factor, m, l, taken)
+                                                   : exponentials<C>(aux, tmem_s, tmem_p, row.factor, m, l, taken);
             if (mine > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
