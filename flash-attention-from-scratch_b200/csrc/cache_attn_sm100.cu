@@ -85,9 +85,10 @@ __device__ __forceinline__ float not_finite_sum(const Apart& a, int row, int dim
 
 constexpr int kSmemCareful = kSmem + static_cast<int>(sizeof(Apart));
 
-template <int D_, bool BF16_, bool E4M3_, bool ONE_PAGE_>
+template <int D_, bool BF16_, bool E4M3_, bool ONE_PAGE_, bool TREE_ = false>
 struct Cfg {
     static constexpr bool ONE_PAGE = ONE_PAGE_;  // a key tile lies within one page
+    static constexpr bool TREE = TREE_;          // the new tokens are a tree's nodes, at most 32
     static constexpr int D = D_;
     static constexpr bool BF16 = BF16_;  // queries and output
     static constexpr bool E4M3 = E4M3_;
@@ -258,11 +259,46 @@ __device__ __forceinline__ Range locate(const FaCachedParams& p, int grid, At at
     return r;
 }
 
+// The tree's shape (TREE).
+struct Parents {
+    const int32_t* parents;
+    int64_t stride;  // from sequence to sequence
+};
+
+// A node and its ancestors, as bits.
+__device__ __forceinline__ uint32_t way_up(const Parents& tree, int b, int node, DeviceStatus* status) {
+    const int32_t* parents = tree.parents + b * tree.stride;
+    uint32_t bits = 0;
+    for (int at = node; at >= 0;) {
+        bits |= 1u << at;
+        int up = __ldg(parents + at);
+        if (up < -1 || up >= at) {
+            atomicOr(&status->code, kStatusBadPage);
+            up = -1;
+        }
+        at = up;
+    }
+    return bits;
+}
+
+// Whether a row sees a position: `pos` its own (-1: no query), `nodes` the nodes it sees (TREE; they are at pos0 and on).
+template <class C>
+__device__ __forceinline__ bool sees(const FaCachedParams& p, const Sequence& s, int pos, uint32_t nodes, int key) {
+    const int gap = pos - key;
+    if constexpr (C::TREE) {
+        const int node = key - s.pos0;
+        if (node >= 0) {
+            return node < 32 && ((nodes >> node) & 1u) != 0;
+        }
+    }
+    return gap >= 0 && (p.window == 0 || gap < p.window || key < p.sinks);
+}
+
 // Takes what is not finite out of 16 bytes `at` of a V tile (chunk `chunk` of the token at position `key`) and notes it for
 // the rows of the item that see it.
 template <class C>
-__device__ __forceinline__ void set_apart(const FaCachedParams& p, const Sequence& s, Apart& apart, uint8_t* at, int row0, int key,
-                                       int chunk) {
+__device__ __forceinline__ void set_apart(const FaCachedParams& p, const Parents& tree, DeviceStatus* status, const Sequence& s, Apart& apart,
+                                       uint8_t* at, int b, int row0, int key, int chunk) {
     const int rows = p.heads / p.cache.kv_heads * p.cache.tokens;
     for (int e = 0; e < 16 / C::kElem; ++e) {
         int kind = 0;
@@ -283,8 +319,16 @@ __device__ __forceinline__ void set_apart(const FaCachedParams& p, const Sequenc
         const int dim = chunk * (16 / C::kElem) + e;
         for (int row = 0; row < kRows && row0 + row < rows; ++row) {
             const int token = (row0 + row) % p.cache.tokens;
-            const int gap = s.pos0 + token - key;
-            if (token < s.count && gap >= 0 && (p.window == 0 || gap < p.window || key < p.sinks)) {
+            if (token >= s.count) {
+                continue;
+            }
+            int pos = s.pos0 + token;
+            uint32_t nodes = 0;
+            if constexpr (C::TREE) {
+                nodes = way_up(tree, b, token, status);
+                pos = s.pos0 + __popc(nodes) - 1;
+            }
+            if (sees<C>(p, s, pos, nodes, key)) {
                 atomicOr(&apart.bits[kind][row][dim / 32], 1u << (dim % 32));
             }
         }
@@ -305,7 +349,7 @@ struct Record {  // of a cut item's rows in the workspace
 // them when the rows are joined. (In this loop, which has no registers left, looking for them in every such tile, or
 // keeping rows apart in the product, cost drafted tokens 3 to 50%.)
 template <class C, bool CAREFUL>
-__device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* status, uint8_t* smem, const Sequence& s,
+__device__ __forceinline__ void attend(const FaCachedParams& p, const Parents& tree, DeviceStatus* status, uint8_t* smem, const Sequence& s,
                                        int b, int kvh, int row0, int v0, int v1, Record rec, long long record) {
     constexpr int D = C::D;
     const FaCache& c = p.cache;
@@ -441,6 +485,7 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
     uint32_t q[C::kSteps][4];
     float factor[2];  // scale * log2 e, and the row's power of two taken back
     int pos[2];
+    [[maybe_unused]] uint32_t nodes[2] = {0u, 0u};
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         const int r = row0 + g + 8 * half;
@@ -448,6 +493,10 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
         const int token = r - head * c.tokens;
         const bool real = r < rows && token < s.count;
         pos[half] = real ? s.pos0 + token : -1;
+        if constexpr (C::TREE) {
+            nodes[half] = real ? way_up(tree, b, token, status) : 0u;
+            pos[half] = real ? s.pos0 + __popc(nodes[half]) - 1 : -1;
+        }
         const uint16_t* src = static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] +
                               static_cast<int64_t>(kvh * group + head) * p.q_stride[1] + token * p.q_stride[2];
         float amax = 0.0f;
@@ -531,7 +580,7 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
         }
 
         // log2 of the weights, and what is hidden.
-        const bool whole = key0 + C::kKeys - 1 <= s.pos0 &&
+        const bool whole = key0 + C::kKeys - 1 <= s.pos0 - (C::TREE ? 1 : 0) &&
                            (p.window == 0 || s.pos0 + s.count - 1 - key0 < p.window || key0 + C::kKeys <= p.sinks);
         float inv_vs[C::kNTiles];
         float shrink = 1.0f;  // of P, for scales below 2^-60
@@ -560,9 +609,7 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
                     float y = fmaf(x[n][2 * half + e], f, lv);
                     if (!whole) {
                         const int key = key0 + 8 * n + 2 * t + e;
-                        const int gap = pos[half] - key;
-                        const bool seen = gap >= 0 && (p.window == 0 || gap < p.window || key < p.sinks);
-                        y = seen ? y : -INFINITY;
+                        y = sees<C>(p, s, pos[half], nodes[half], key) ? y : -INFINITY;
                     }
                     x[n][2 * half + e] = y;
                     top[half] = fmaxf(top[half], y);
@@ -620,7 +667,7 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, DeviceStatus* st
                 uint8_t* at = ring + stage * 2 * kTileBytes + kTileBytes + v_offset<C>(r, chunk);
                 const uint4 y = *reinterpret_cast<const uint4*>(at);
                 if ((not_finite<C>(y.x) | not_finite<C>(y.y) | not_finite<C>(y.z) | not_finite<C>(y.w)) != 0) {
-                    set_apart<C>(p, s, apart, at, row0, key0 + r, chunk);
+                    set_apart<C>(p, tree, status, s, apart, at, b, row0, key0 + r, chunk);
                 }
             }
             __syncwarp();
@@ -817,7 +864,7 @@ __device__ __forceinline__ void take_ranges(const FaCachedParams& p, const Recor
 
 // Items that are never cut, one a CTA.
 template <class C, bool CAREFUL>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) cached_whole_kernel(const __grid_constant__ FaCachedParams p,
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) cached_whole_kernel(const __grid_constant__ FaCachedParams p, Parents tree,
                                                                             DeviceStatus* status, Record rec, int ranges) {
     extern __shared__ __align__(128) uint8_t smem[];
     const int row_tiles = (p.heads / p.cache.kv_heads * p.cache.tokens + kRows - 1) / kRows;
@@ -826,12 +873,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cached_whole_kernel(cons
         const int b = range / items;
         const int item = range - b * items;
         const Sequence s = sequence<C>(p, b);
-        attend<C, CAREFUL>(p, status, smem, s, b, item / row_tiles, (item % row_tiles) * kRows, 0, s.tiles, rec, -1);
+        attend<C, CAREFUL>(p, tree, status, smem, s, b, item / row_tiles, (item % row_tiles) * kRows, 0, s.tiles, rec, -1);
     });
 }
 
 template <class C, bool CAREFUL>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) cached_kernel(const __grid_constant__ FaCachedParams p,
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) cached_kernel(const __grid_constant__ FaCachedParams p, Parents tree,
                                                                       DeviceStatus* status, Record rec, int ranges) {
     extern __shared__ __align__(128) uint8_t smem[];
     take_ranges<CAREFUL>(p, rec, ranges, [&](int cta) {
@@ -852,7 +899,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cached_kernel(const __gr
         while (at < end) {
             const int take = static_cast<int>(min(static_cast<long long>(s.tiles - v), end - at));
             const bool whole = v == 0 && take == s.tiles;
-            attend<C, CAREFUL>(p, status, smem, s, b, item / row_tiles, (item % row_tiles) * kRows, v, v + take, rec,
+            attend<C, CAREFUL>(p, tree, status, smem, s, b, item / row_tiles, (item % row_tiles) * kRows, v, v + take, rec,
                                whole ? -1 : 2ll * cta + (first ? 0 : 1));
             first = false;
             at += take;
@@ -1038,7 +1085,7 @@ cudaError_t launch_join(const FaCachedParams& p, const Record& rec, const Split&
 
 // All items or ranges; with several tokens, those that have to be taken carefully; the join of what was cut.
 template <class C, bool WHOLE>
-cudaError_t launch_kernels(const FaCachedParams& p, DeviceStatus* status, const Record& rec, const Split& split, int sm_count,
+cudaError_t launch_kernels(const FaCachedParams& p, const Parents& tree, DeviceStatus* status, const Record& rec, const Split& split, int sm_count,
                            cudaStream_t stream) {
     constexpr auto kernel = WHOLE ? cached_whole_kernel<C, false> : cached_kernel<C, false>;
     constexpr auto careful = WHOLE ? cached_whole_kernel<C, true> : cached_kernel<C, true>;
@@ -1050,13 +1097,13 @@ cudaError_t launch_kernels(const FaCachedParams& p, DeviceStatus* status, const 
     if (err != cudaSuccess) {
         return err;
     }
-    kernel<<<ranges, kThreads, kSmem, stream>>>(p, status, rec, ranges);
+    kernel<<<ranges, kThreads, kSmem, stream>>>(p, tree, status, rec, ranges);
     err = cudaGetLastError();
     if (err == cudaSuccess && p.cache.tokens > 1) {
         // Half as many CTAs as SMs: they find room while the first kernel's last ranges run, and the join's CTAs after
         // them (64 sequences x 4 tokens: 112.5 us, with a CTA for each range 115, without this kernel 110).
         err = launch_early(careful, dim3(static_cast<unsigned>(std::min(ranges, std::max(sm_count / 2, 1)))), kSmemCareful, stream,
-                           p, status, rec, ranges);
+                           p, tree, status, rec, ranges);
     }
     if (err == cudaSuccess && !WHOLE && ranges > 1) {
         err = launch_join<C>(p, rec, split, sm_count, stream);
@@ -1065,7 +1112,7 @@ cudaError_t launch_kernels(const FaCachedParams& p, DeviceStatus* status, const 
 }
 
 template <class C>
-cudaError_t launch(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
+cudaError_t launch(const FaCachedParams& p, const Parents& tree, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
     const Split split = split_for(p, sm_count);
     if (split.grid > 0x7fffffffLL) {
         return cudaErrorInvalidConfiguration;
@@ -1073,32 +1120,46 @@ cudaError_t launch(const FaCachedParams& p, DeviceStatus* status, void* workspac
     Record rec{};
     if (split.whole) {
         rec.odd = static_cast<int*>(workspace);
-        return launch_kernels<C, true>(p, status, rec, split, sm_count, stream);
+        return launch_kernels<C, true>(p, tree, status, rec, split, sm_count, stream);
     }
     const size_t rows = static_cast<size_t>(split.grid) * 2 * kRows;
     rec.o = static_cast<float*>(workspace);
     rec.ml = reinterpret_cast<float2*>(rec.o + rows * C::D);
     rec.odd = reinterpret_cast<int*>(rec.ml + rows);
-    return launch_kernels<C, false>(p, status, rec, split, sm_count, stream);
+    return launch_kernels<C, false>(p, tree, status, rec, split, sm_count, stream);
 }
 
-template <int D, bool ONE_PAGE>
-cudaError_t launch_pages(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count,
+template <int D, bool ONE_PAGE, bool TREE>
+cudaError_t launch_pages(const FaCachedParams& p, const Parents& tree, DeviceStatus* status, void* workspace, int sm_count,
                          cudaStream_t stream) {
     const bool bf16 = p.dtype == FA_DTYPE_BFLOAT16;
     if (p.cache.dtype == FA_DTYPE_FLOAT8_E4M3) {
-        return bf16 ? launch<Cfg<D, true, true, ONE_PAGE>>(p, status, workspace, sm_count, stream)
-                    : launch<Cfg<D, false, true, ONE_PAGE>>(p, status, workspace, sm_count, stream);
+        return bf16 ? launch<Cfg<D, true, true, ONE_PAGE, TREE>>(p, tree, status, workspace, sm_count, stream)
+                    : launch<Cfg<D, false, true, ONE_PAGE, TREE>>(p, tree, status, workspace, sm_count, stream);
     }
-    return bf16 ? launch<Cfg<D, true, false, ONE_PAGE>>(p, status, workspace, sm_count, stream)
-                : launch<Cfg<D, false, false, ONE_PAGE>>(p, status, workspace, sm_count, stream);
+    return bf16 ? launch<Cfg<D, true, false, ONE_PAGE, TREE>>(p, tree, status, workspace, sm_count, stream)
+                : launch<Cfg<D, false, false, ONE_PAGE, TREE>>(p, tree, status, workspace, sm_count, stream);
 }
 
-template <int D>
-cudaError_t launch_dim(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count,
-                       cudaStream_t stream) {
-    return p.cache.page_size >= tile_keys(p.cache) ? launch_pages<D, true>(p, status, workspace, sm_count, stream)
-                                                   : launch_pages<D, false>(p, status, workspace, sm_count, stream);
+template <int D, bool TREE>
+cudaError_t launch_dim(const FaCachedParams& p, const Parents& tree, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
+    return p.cache.page_size >= tile_keys(p.cache) ? launch_pages<D, true, TREE>(p, tree, status, workspace, sm_count, stream)
+                                                   : launch_pages<D, false, TREE>(p, tree, status, workspace, sm_count, stream);
+}
+
+// A tree's parameters as the cached attention's, whose kernel it is but for what a row sees.
+FaCachedParams as_cached(const FaTreeParams& t) {
+    FaCachedParams p{};
+    p.cache = t.cache;
+    p.q = t.q;
+    p.o = t.o;
+    std::copy(t.q_stride, t.q_stride + 3, p.q_stride);
+    p.heads = t.heads;
+    p.window = t.window;
+    p.sinks = t.sinks;
+    p.softmax_scale = t.softmax_scale;
+    p.dtype = t.dtype;
+    return p;
 }
 
 }  // namespace
@@ -1111,8 +1172,17 @@ unsigned long long cached_workspace_bytes(const FaCachedParams& p, int sm_count)
 
 cudaError_t launch_cached(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count,
                           cudaStream_t stream) {
-    return p.cache.head_dim == 64 ? launch_dim<64>(p, status, workspace, sm_count, stream)
-                                  : launch_dim<128>(p, status, workspace, sm_count, stream);
+    return p.cache.head_dim == 64 ? launch_dim<64, false>(p, {}, status, workspace, sm_count, stream)
+                                  : launch_dim<128, false>(p, {}, status, workspace, sm_count, stream);
+}
+
+unsigned long long small_tree_workspace_bytes(const FaTreeParams& t, int sm_count) { return cached_workspace_bytes(as_cached(t), sm_count); }
+
+cudaError_t launch_small_tree(const FaTreeParams& t, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
+    const FaCachedParams p = as_cached(t);
+    const Parents tree{t.parents, t.parent_stride};
+    return p.cache.head_dim == 64 ? launch_dim<64, true>(p, tree, status, workspace, sm_count, stream)
+                                  : launch_dim<128, true>(p, tree, status, workspace, sm_count, stream);
 }
 
 }  // namespace fa_sm100

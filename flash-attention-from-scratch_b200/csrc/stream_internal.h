@@ -30,6 +30,9 @@ unsigned long long cached_workspace_bytes(const FaCachedParams& p, int sm_count)
 cudaError_t launch_cached(const FaCachedParams& p, DeviceStatus* status, void* workspace, int sm_count,
                           cudaStream_t stream);
 
+// Trees of at most 32 nodes in the cached attention's kernel, 16 query rows at a time (cache_attn_sm100.cu).
+unsigned long long small_tree_workspace_bytes(const FaTreeParams& p, int sm_count);
+cudaError_t launch_small_tree(const FaTreeParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream);
 unsigned long long tree_workspace_bytes(const FaTreeParams& p, int sm_count);
 cudaError_t launch_tree(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count,
                         cudaStream_t stream);

@@ -473,23 +473,16 @@ struct Waits {
     unsigned* code;
 };
 
-// A bounded wait of a whole warp: 2^20 polls of at most a microsecond. In few instructions, for there are many of them and the
-// kernel's loops have to fit the instruction cache. False: given up, by this warp or another of the CTA.
+// A bounded wait of a whole warp: 2^20 polls, 20 ms at the least, where a healthy wait is a tile's time. In few instructions,
+// for there are many of them and the kernel's loops have to fit the instruction cache. False: given up, by this warp or another
+// of the CTA.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, int phase, const Waits& waits, unsigned code) {
     const uint32_t at = smem_u32(bar);
     const uint32_t parity = static_cast<uint32_t>(phase) & 1u;
     bool there = false;
 #pragma unroll 1
     for (int i = 0; i < (1 << 20); ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(at), "r"(parity)
-            : "memory");
-        there = done != 0;
+        there = mbar_try_wait(at, parity);
         if (there || *waits.abort != 0) {
             break;
         }
@@ -1741,6 +1734,10 @@ cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, cuda
 
 constexpr int kWholeTiles = 8;  // up to this many key tiles in the table's capacity items are not cut
 constexpr int kFixers = 64;
+constexpr int kFewRows = 16;
+
+// Whether a kv head's rows are better taken 16 at a time.
+bool few_rows(const FaTreeParams& p) { return p.heads / p.cache.kv_heads * p.cache.tokens <= kFewRows; }
 
 int row_tiles(const FaTreeParams& p) { return p.heads / p.cache.kv_heads * p.cache.tokens > kTile ? 2 : 1; }
 
@@ -1820,6 +1817,9 @@ cudaError_t launch_types(const FaTreeParams& p, DeviceStatus* status, unsigned e
 }  // namespace
 
 unsigned long long tree_workspace_bytes(const FaTreeParams& p, int sm_count) {
+    if (few_rows(p)) {
+        return small_tree_workspace_bytes(p, sm_count);
+    }
     const Split split = split_for(p, sm_count);
     const unsigned long long records =
         split.whole ? 0 : static_cast<unsigned long long>(split.grid) * 2 * row_tiles(p) * kTile * (p.cache.head_dim + 2) * 4;
@@ -1827,6 +1827,9 @@ unsigned long long tree_workspace_bytes(const FaTreeParams& p, int sm_count) {
 }
 
 cudaError_t launch_tree(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count, cudaStream_t stream) {
+    if (few_rows(p)) {
+        return launch_small_tree(p, status, workspace, sm_count, stream);
+    }
     return p.cache.head_dim == 64 ? launch_types<64>(p, status, epoch, workspace, sm_count, stream)
                                   : launch_types<128>(p, status, epoch, workspace, sm_count, stream);
 }
