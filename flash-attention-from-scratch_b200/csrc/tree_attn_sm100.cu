@@ -49,11 +49,12 @@ constexpr int kGroups = kTile / 8;   // keys that surely share a page
 constexpr int kMostStages = 4;
 constexpr int kParts = 2;  // pieces listed, the one at hand and the next
 
-template <int D_, bool BF16_, bool E4M3_, int NR_>
+template <int D_, bool BF16_, bool E4M3_, bool COARSE_, int NR_>
 struct Cfg {
     static constexpr int D = D_;
     static constexpr bool BF16 = BF16_;  // queries and output
     static constexpr bool E4M3 = E4M3_;
+    static constexpr bool COARSE = COARSE_;  // 32 keys on end share a page
     static constexpr int NR = NR_;  // row tiles of an item: 1 (key tiles alternate between the softmax warpgroups) or 2
     static constexpr bool kMmaBf16 = BF16 && !E4M3;  // type of P and V (and of Q and K, over a 16-bit cache)
     static constexpr int kElem = E4M3 ? 1 : 2;
@@ -1286,7 +1287,6 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, Shared& sh, Excha
             mbar_arrive(smem_u32(bar));
         }
     };
-    const bool coarse = p.cache.page_size >= 32;
     int tiles = 0;   // key tiles of the pieces before
     int steps = 0;   // scores taken
     float next_factor = 0.0f;
@@ -1378,8 +1378,12 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, Shared& sh, Excha
                 tc_fence_before();
                 arrive(&sh.s_free[w]);
             };
-            const float alpha = C::E4M3 && !coarse ? exponentials_by_8<C>(aux, tmem_s, tmem_p, row.factor, m, l, taken)
-                                                   : exponentials<C>(aux, tmem_s, tmem_p, row.factor, m, l, taken);
+            float alpha;
+            if constexpr (C::E4M3 && !C::COARSE) {
+                alpha = exponentials_by_8<C>(aux, tmem_s, tmem_p, row.factor, m, l, taken);
+            } else {
+                alpha = exponentials<C>(aux, tmem_s, tmem_p, row.factor, m, l, taken);
+            }
             if (mine > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
@@ -1797,21 +1801,27 @@ cudaError_t launch(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, 
     return err;
 }
 
-template <int D, bool BF16, bool E4M3>
+template <int D, bool BF16, bool E4M3, bool COARSE>
 cudaError_t launch_rows(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count, cudaStream_t stream) {
-    return row_tiles(p) == 1 ? launch<Cfg<D, BF16, E4M3, 1>>(p, status, epoch, workspace, sm_count, stream)
-                             : launch<Cfg<D, BF16, E4M3, 2>>(p, status, epoch, workspace, sm_count, stream);
+    return row_tiles(p) == 1 ? launch<Cfg<D, BF16, E4M3, COARSE, 1>>(p, status, epoch, workspace, sm_count, stream)
+                             : launch<Cfg<D, BF16, E4M3, COARSE, 2>>(p, status, epoch, workspace, sm_count, stream);
+}
+
+// Pages of 8 or 16 tokens matter to an e4m3 cache alone, by their scales. (One kernel for both took 271 us for 64 nodes on
+// 32 contexts where this takes 239: what it runs has to fit the instruction cache.)
+template <int D, bool BF16>
+cudaError_t launch_types(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count, cudaStream_t stream) {
+    if (p.cache.dtype != FA_DTYPE_FLOAT8_E4M3) {
+        return launch_rows<D, BF16, false, true>(p, status, epoch, workspace, sm_count, stream);
+    }
+    return p.cache.page_size >= 32 ? launch_rows<D, BF16, true, true>(p, status, epoch, workspace, sm_count, stream)
+                                   : launch_rows<D, BF16, true, false>(p, status, epoch, workspace, sm_count, stream);
 }
 
 template <int D>
-cudaError_t launch_types(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count, cudaStream_t stream) {
-    const bool bf16 = p.dtype == FA_DTYPE_BFLOAT16;
-    if (p.cache.dtype == FA_DTYPE_FLOAT8_E4M3) {
-        return bf16 ? launch_rows<D, true, true>(p, status, epoch, workspace, sm_count, stream)
-                    : launch_rows<D, false, true>(p, status, epoch, workspace, sm_count, stream);
-    }
-    return bf16 ? launch_rows<D, true, false>(p, status, epoch, workspace, sm_count, stream)
-                : launch_rows<D, false, false>(p, status, epoch, workspace, sm_count, stream);
+cudaError_t launch_dim(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count, cudaStream_t stream) {
+    return p.dtype == FA_DTYPE_BFLOAT16 ? launch_types<D, true>(p, status, epoch, workspace, sm_count, stream)
+                                        : launch_types<D, false>(p, status, epoch, workspace, sm_count, stream);
 }
 
 }  // namespace
@@ -1830,8 +1840,8 @@ cudaError_t launch_tree(const FaTreeParams& p, DeviceStatus* status, unsigned ep
     if (few_rows(p)) {
         return launch_small_tree(p, status, workspace, sm_count, stream);
     }
-    return p.cache.head_dim == 64 ? launch_types<64>(p, status, epoch, workspace, sm_count, stream)
-                                  : launch_types<128>(p, status, epoch, workspace, sm_count, stream);
+    return p.cache.head_dim == 64 ? launch_dim<64>(p, status, epoch, workspace, sm_count, stream)
+                                  : launch_dim<128>(p, status, epoch, workspace, sm_count, stream);
 }
 
 }  // namespace fa_sm100
