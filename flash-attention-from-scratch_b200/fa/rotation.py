@@ -113,13 +113,14 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dq, dk):
-        tables = ctx.saved_tensors
-        dq, dk = (None if g is None else _loadable(g) for g in (dq, dk))
+        # A gradient of the gradients asked for (create_graph): they are results of a rotation like any other.
+        turn = _Rotary.apply if torch.is_grad_enabled() else _run
+        dk = None if dk is None else _loadable(dk)
         if dq is None:
-            grads = (None, None) if dk is None else _Rotary.apply(dk, None, *tables, *ctx.how)[::-1]
+            grads = (None, None) if dk is None else turn(dk, None, *ctx.saved_tensors, *ctx.how)[::-1]
         else:
-            grads = _Rotary.apply(dq, dk, *tables, *ctx.how)
-        return (*grads, *(None,) * 6)
+            grads = turn(_loadable(dq), dk, *ctx.saved_tensors, *ctx.how)
+        return (*grads, None, None, None, None, None, None)
 
 
 def rotary(
