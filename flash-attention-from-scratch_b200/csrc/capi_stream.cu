@@ -201,6 +201,14 @@ int validate_tree(const FaTreeParams* p) {
     if (rc != FA_OK) {
         return rc;
     }
+    // Pages are read through tensor maps, which have no broadcast dims.
+    const FaCache& c = p->cache;
+    const int64_t most = (1ll << 40) / (c.dtype == FA_DTYPE_FLOAT8_E4M3 ? 1 : 2);
+    for (const int64_t* stride : {c.k_stride, c.v_stride}) {
+        if ((c.num_pages > 1 && (stride[0] <= 0 || stride[0] >= most)) || (c.kv_heads > 1 && (stride[1] <= 0 || stride[1] >= most))) {
+            return invalid(op, "the cache's strides must be positive and below 2^40 bytes");
+        }
+    }
     if (p->cache.tokens > kMostDrafted) {
         return invalid(op, "a tree has at most 256 nodes, got " + std::to_string(p->cache.tokens));
     }

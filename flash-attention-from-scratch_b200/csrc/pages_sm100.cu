@@ -320,40 +320,58 @@ __device__ __forceinline__ NewEntries new_entries(const FaPages& p, int b) {
     return e;
 }
 
-// Needs of all rows, then the free pages as far as they are needed, then the pages' new places: three passes with
-// CTA barriers between them, since needs and free pages are those that the call finds. Workspace: needs[batch]
-// (an entry's bit would not hold long prompts, so which entries need a page is a list of its own),
-// wanted[batch][entries], free[...].
+// The new entries of all rows, row after row, and for each the rank of the free page that it needs; then the free pages
+// as far as they are needed; then the pages' new places: three passes of one CTA with barriers between them, since needs and free
+// pages are those that the call finds. Entries are taken in order, four a thread, rows of any length alike. Workspace:
+// before[batch + 1] (needs of the rows before), rank[batch][entries] (-1: none needed), free[...].
 __global__ void __launch_bounds__(kReserveThreads) reserve_kernel(const __grid_constant__ FaPages p, DeviceStatus* status,
-                                                                  int32_t* before, uint8_t* wanted, int32_t* free_list) {
+                                                                  int32_t* before, int32_t* rank, int32_t* free_list) {
     const int entries = reserve_entries(p);
-    int need_total = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += kReserveThreads) {
-        const int b = b0 + static_cast<int>(threadIdx.x);
-        int need = 0;
-        if (b < p.batch) {
-            const NewEntries e = new_entries(p, b);
-            for (int i = e.first; i < e.end; ++i) {
-                const int id = p.table[b * p.table_stride + i];
-                const bool bad = id < -1 || id >= p.num_pages;
-                if (bad) {
-                    atomicOr(&status->code, kStatusBadPage);
+    const long long all = static_cast<long long>(p.batch) * entries;
+    int needed = 0;
+    for (long long at0 = 0; at0 < all; at0 += 4 * kReserveThreads) {
+        bool want[4];
+        int mine = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const long long at = at0 + 4 * static_cast<int>(threadIdx.x) + k;
+            want[k] = false;
+            if (at < all) {
+                const int b = static_cast<int>(at / entries);
+                const NewEntries e = new_entries(p, b);
+                const int i = e.first + static_cast<int>(at - static_cast<long long>(b) * entries);
+                if (i < e.end) {
+                    const int id = p.table[b * p.table_stride + i];
+                    const bool bad = id < -1 || id >= p.num_pages;
+                    if (bad) {
+                        atomicOr(&status->code, kStatusBadPage);
+                    }
+                    want[k] = id < 0 || bad || p.refs[id] > 1;
                 }
-                const bool want = id < 0 || bad || p.refs[id] > 1;
-                wanted[static_cast<int64_t>(b) * entries + i - e.first] = want;
-                need += want;
             }
+            mine += want[k];
         }
         int total;
-        const int prefix = block_prefix(need, total);
-        if (b < p.batch) {
-            before[b] = need_total + prefix;
+        int next = needed + block_prefix(mine, total);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const long long at = at0 + 4 * static_cast<int>(threadIdx.x) + k;
+            if (at < all) {
+                rank[at] = want[k] ? next : -1;
+                if (at % entries == 0) {
+                    before[at / entries] = next;
+                }
+            }
+            next += want[k];
         }
-        need_total += total;
+        needed += total;
+    }
+    if (threadIdx.x == 0) {
+        before[p.batch] = needed;
     }
     // Free pages in order, as many as are needed.
     int found = 0;
-    for (int i0 = 0; i0 < p.num_pages && found < need_total; i0 += 4 * kReserveThreads) {
+    for (int i0 = 0; i0 < p.num_pages && found < needed; i0 += 4 * kReserveThreads) {
         const int i = i0 + 4 * static_cast<int>(threadIdx.x);
         bool is_free[4];
         int mine = 0;
@@ -363,51 +381,47 @@ __global__ void __launch_bounds__(kReserveThreads) reserve_kernel(const __grid_c
             mine += is_free[k];
         }
         int total;
-        int rank = found + block_prefix(mine, total);
+        int next = found + block_prefix(mine, total);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             if (is_free[k]) {
-                if (rank < need_total) {
-                    free_list[rank] = i + k;
+                if (next < needed) {
+                    free_list[next] = i + k;
                 }
-                ++rank;
+                ++next;
             }
         }
         found += total;
     }
     __syncthreads();
-    for (int b = static_cast<int>(threadIdx.x); b < p.batch; b += kReserveThreads) {
+    for (long long at = threadIdx.x; at < all; at += kReserveThreads) {
+        const int b = static_cast<int>(at / entries);
+        const int nth = static_cast<int>(at - static_cast<long long>(b) * entries);
         const NewEntries e = new_entries(p, b);
-        const int rank0 = before[b];
-        const int end = b + 1 < p.batch ? before[b + 1] : need_total;
-        const bool granted = e.fits && (end == rank0 || end <= found);
-        if (!e.fits) {
-            atomicOr(&status->code, kStatusBadPage);
-        }
+        const bool granted = e.fits && (before[b + 1] == before[b] || before[b + 1] <= found);
         int src = -1, dst = -1;
-        if (granted) {
-            int rank = rank0;
-            for (int i = e.first; i < e.end; ++i) {
-                if (!wanted[static_cast<int64_t>(b) * entries + i - e.first]) {
-                    continue;
+        if (granted && rank[at] >= 0) {
+            int32_t* entry = p.table + b * p.table_stride + e.first + nth;
+            const int id = *entry;
+            const int page = free_list[rank[at]];
+            if (id >= 0 && id < p.num_pages) {
+                atomicSub(p.refs + id, 1);
+                if (nth == 0 && e.older) {
+                    src = id;
+                    dst = page;
                 }
-                int32_t* entry = p.table + b * p.table_stride + i;
-                const int id = *entry;
-                const int page = free_list[rank++];
-                if (id >= 0 && id < p.num_pages) {
-                    atomicSub(p.refs + id, 1);
-                    if (i == e.first && e.older) {
-                        src = id;
-                        dst = page;
-                    }
-                }
-                p.refs[page] = 1;
-                *entry = page;
             }
+            p.refs[page] = 1;
+            *entry = page;
         }
-        p.granted[b] = granted;
-        p.src[b] = src;
-        p.dst[b] = dst;
+        if (nth == 0) {
+            if (!e.fits) {
+                atomicOr(&status->code, kStatusBadPage);
+            }
+            p.granted[b] = granted;
+            p.src[b] = src;
+            p.dst[b] = dst;
+        }
     }
 }
 
@@ -454,16 +468,16 @@ cudaError_t launch_free_pages(const FaPages& p, DeviceStatus* status, cudaStream
 
 unsigned long long reserve_workspace_bytes(const FaPages& p) {
     const unsigned long long all = static_cast<unsigned long long>(p.batch) * reserve_entries(p);
-    return rounded(4ull * p.batch) + rounded(all) + 4ull * std::min<unsigned long long>(all, p.num_pages);
+    return rounded(4ull * (p.batch + 1ull)) + rounded(4ull * all) + 4ull * std::min<unsigned long long>(all, p.num_pages);
 }
 
 cudaError_t launch_reserve_pages(const FaPages& p, DeviceStatus* status, void* workspace, cudaStream_t stream) {
     uint8_t* at = static_cast<uint8_t*>(workspace);
     int32_t* before = reinterpret_cast<int32_t*>(at);
-    at += rounded(4ull * p.batch);
-    uint8_t* wanted = at;
-    at += rounded(static_cast<unsigned long long>(p.batch) * reserve_entries(p));
-    reserve_kernel<<<1, kReserveThreads, 0, stream>>>(p, status, before, wanted, reinterpret_cast<int32_t*>(at));
+    at += rounded(4ull * (p.batch + 1ull));
+    int32_t* rank = reinterpret_cast<int32_t*>(at);
+    at += rounded(4ull * p.batch * reserve_entries(p));
+    reserve_kernel<<<1, kReserveThreads, 0, stream>>>(p, status, before, rank, reinterpret_cast<int32_t*>(at));
     return cudaGetLastError();
 }
 

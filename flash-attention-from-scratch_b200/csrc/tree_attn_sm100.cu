@@ -716,8 +716,8 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensor
             to.gone = gone;
             to.tiny = tiny_bits;
             const int near = window_first(max(s.context, 0) + s.count, p.window);
-            to.mixed = c.tokens > 1 && (key0 + kTile > s.context || (p.window > 0 && key0 < near));
-            to.full = gone == 0 && key0 + kTile <= min(s.context, s.last + 1) && (p.window == 0 || key0 >= near || key0 + kTile <= p.sinks);
+            to.mixed = c.tokens > 1 && (key0 > s.context - kTile || (p.window > 0 && key0 < near));
+            to.full = gone == 0 && key0 <= min(s.context - 1, s.last) - (kTile - 1) && (p.window == 0 || key0 >= near || key0 <= p.sinks - kTile);
         }
         __syncwarp();
         if (lane == 0) {
@@ -1063,11 +1063,11 @@ __device__ __forceinline__ float bring_queries(const FaTreeParams& p, const uint
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
             }
             // 2^(8 - exponent of the largest), one less where that would pass 448, both it and its inverse normal; 1 for
-            // zeros, inf and NaN.
+            // zeros. A row with an infinity or NaN becomes NaN: e4m3 has no infinity.
             const uint32_t most = __float_as_uint(widen16<C::BF16>(static_cast<uint16_t>(top)));
             const int e = static_cast<int>(most >> 23);
             const int shift = (e == 0 || e == 255) ? 0 : min(max(135 - e - ((most & 0x7fffffu) > 0x600000u ? 1 : 0), -100), 100);
-            const float up = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+            const float up = e == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
             const float back = fmaxf(scale * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23), kLeastFactor);
             if constexpr (C::NR == 1) {
                 if (part == 0) {
@@ -1118,7 +1118,7 @@ __device__ __forceinline__ uint4 kept_columns(const FaTreeParams& p, const Part&
             keep[i] &= ~bits_up_to(row.first - 1 - kb) | bits_up_to(p.sinks - 1 - kb);
         }
     }
-    if (key0 + kTile > s.context) {
+    if (key0 > s.context - kTile) {
         const int column = s.context - key0;  // of node 0
         for (int at = row.real ? row.token : -1; at >= 0;) {
             const int low = s.low[at];

@@ -397,7 +397,8 @@ FA_API int fa_rotary(const FaRotaryParams* params, fa_stream_t stream);
  * hangs on the context. Anything else counts as -1 and sets bit 5 (32) of fa_device_status. Node t is
  * at position p = context + (number of its ancestors), context = lengths[b] - counts[b]. It sees
  * position j of the context when window == 0, or p - j < window, or j < sinks, and of the nodes its
- * ancestors and itself. window is 0 or at least `tokens`. */
+ * ancestors and itself. window is 0 or at least `tokens`. The cache's strides are positive, for dims of more than
+ * one element, and below 2^40 bytes. */
 typedef struct FaTreeParams {
     FaCache cache;
     const void* q;

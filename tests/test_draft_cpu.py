@@ -123,6 +123,7 @@ def test_rotary_refusals(change, match):
     ({"d": 80}, "head_dim"), ({"page": 12}, "power of two"), ({"cdtype": 1}, "tensors' type"), ({"ks": 0}, "scales"), ({"k": 8}, "16-byte aligned"),
     ({"window": -1}, "negative"), ({"sinks": -1}, "negative"), ({"window": 3}, "at least the number of nodes"), ({"scale": math.inf}, "finite"),
     ({"q": 0}, "must be present"), ({"o": 8}, "16-byte aligned"), ({"parents": 0}, "parents"), ({"pstride": -4}, "parents"), ({"dtype": 2}, "dtype"),
+    ({"k0": 0}, "strides"), ({"v1": 0}, "strides"), ({"v0": 1 << 40}, "2\\^40"),
 ])
 def test_tree_refusals(change, match):
     _refused("fa_tree_attention", _tree(**change), match, None, 0, None)

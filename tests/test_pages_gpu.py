@@ -196,6 +196,18 @@ def test_steps_of_many_sequences(seed, num_pages, batch, width, page, tokens):
     assert _C.device_status(0, clear=True) == 0
 
 
+def test_a_long_prompt():
+    """Thousands of entries of one row, some of them shared, beside rows that need one or none."""
+    refs, table = torch.zeros(9000, dtype=torch.int32, device=DEV), torch.full((3, 6500), -1, dtype=torch.int32, device=DEV)
+    refs[5], refs[7000], refs[17] = 2, 3, 1
+    table[1, 0], table[1, 6000], table[0, 0] = 5, 7000, 17
+    pages, rows, lengths, counts = oracle.Pages(refs.tolist()), table.tolist(), [9, 6400 * 8 + 3, 40], [1, 6400 * 8, 0]
+    got = fa.reserve_pages(refs, table, _ints(lengths), 6400 * 8, 8, counts=_ints(counts))
+    want = pages.reserve(rows, lengths, 6400 * 8, 8, counts)
+    assert [x.tolist() for x in got] == [*want] and all(want[0]) and want[1][1] == 5
+    _same(refs, pages, table, rows)
+
+
 def test_too_few_pages():
     refs, table = _ints([0, 1, 0, 0, 1]), _ints([[1, -1, -1], [4, -1, -1], [-1, -1, -1], [-1, -1, -1]])
     # Two pages, none, two of the one that is left, and one.

@@ -207,6 +207,37 @@ def test_infinite_and_nan_queries_stay_in_their_rows():
         assert torch.equal(out, clean)
 
 
+@pytest.mark.parametrize("dtype", [HALF, BF])
+@pytest.mark.parametrize("tokens", [3, 20, 60])
+def test_infinite_queries_over_an_e4m3_cache(tokens, dtype):
+    """e4m3 has no infinity: a row with one is NaN, as it is where the products are taken in 16 bits, and alone."""
+    gen = torch.Generator(DEV).manual_seed(9)
+    cache, table = _cache(gen, 1, 300, 16, 2, 128, E4M3)
+    q = torch.randn(1, 8, tokens, 128, generator=gen, device=DEV).to(dtype)
+    parents = _parents(1, tokens, 6, 3)
+    clean = fa.forward_tree(q, cache, table, _ints([300]), parents)
+    q[0, 1, 2, 5], q[0, 6, 1, 100], q[0, 7, 0, 0] = math.inf, -math.inf, math.nan
+    out = fa.forward_tree(q, cache, table, _ints([300]), parents)
+    for h, t in ((1, 2), (6, 1), (7, 0)):
+        assert torch.isnan(out[0, h, t]).all()
+        out[0, h, t] = clean[0, h, t]
+    assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("dtype,kind", KINDS)
+def test_tiny_and_zero_queries_and_scales(dtype, kind):
+    """Rows of zeros and of values at the small end of their type weigh what they see alike, or as little apart."""
+    gen = torch.Generator(DEV).manual_seed(10)
+    cache, table = _cache(gen, 1, 300, 32, 1, 64, kind)
+    for tokens in (4, 40):
+        q = torch.randn(1, 4, tokens, 64, generator=gen, device=DEV).to(dtype)
+        q[0, 0], q[0, 1, 0], q[0, 2] = 0.0, torch.finfo(dtype).tiny, q[0, 2] * 2.0**-12
+        if kind == E4M3:
+            cache.v_scale[int(table[0, 2])] = 0.0
+            cache.k_scale[int(table[0, 4])] = 0.0
+        _check(q, cache, table, _ints([300]), _parents(1, tokens, 3, 0))
+
+
 @pytest.mark.parametrize("tokens", [4, 50])
 def test_bad_parents_pages_and_lengths(tokens):
     gen = torch.Generator(DEV).manual_seed(10)
@@ -288,7 +319,9 @@ def test_empty_and_refused():
                        (lambda: fa.forward_tree(q.half(), cache, table, lengths, parents), "same dtype"), (lambda: fa.forward_tree(q, cache, table, lengths.long(), parents), "lengths")):
         with pytest.raises(RuntimeError, match=match):
             bad()
-    for bad, match in ((lambda: fa.forward_tree(q, cache, table, lengths, parents, window=2), "at least the number"), (lambda: fa.forward_tree(q[:, :3], cache, table, lengths, parents), "multiple of kv_heads"),
+    wide = fa.PagedKVCache(cache.k[:1].expand(3, 2, 16, 64), cache.v[:1].expand(3, 2, 16, 64))
+    for bad, match in ((lambda: fa.forward_tree(q, wide, table, lengths, parents), "strides must be positive"),
+                       (lambda: fa.forward_tree(q, cache, table, lengths, parents, window=2), "at least the number"), (lambda: fa.forward_tree(q[:, :3], cache, table, lengths, parents), "multiple of kv_heads"),
                        (lambda: fa.forward_tree(q, cache, table, lengths, parents, sinks=-1), "negative"), (lambda: fa.forward_tree(q, cache, table, lengths, parents, window=2**40), "32-bit"),
                        (lambda: fa.forward_tree(q.repeat(1, 1, 100, 1), cache, table, lengths, parents.repeat(1, 100)), "at most 256"),
                        (lambda: fa.forward_tree(q, cache, table, lengths, parents, softmax_scale=math.nan), "finite")):
