@@ -1349,14 +1349,18 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, Shared& sh, Excha
         int mine = 0;  // scores of this piece taken
         for (int t = NR == 1 ? w : 0; t < n; t += NR == 1 ? 2 : 1, ++mine) {
             const int slot = (tiles + t) % kListed;
-            // P's place is free and the tile listed by the time its scores are there, most of the time.
-            if ((steps > 0 && !wait(&sh.p_free[w], steps - 1)) || !wait(&sh.s_full[w], steps) ||
-                !wait(&sh.list_full[slot], (tiles + t) / kListed)) {
+            // P's place is free and the tile listed by the time its scores are there, most of the time. From the scores on it is
+            // a race: the next ones are not begun before these are in registers.
+            if ((steps > 0 && !wait(&sh.p_free[w], steps - 1)) || !wait(&sh.list_full[slot], (tiles + t) / kListed)) {
+                return;
+            }
+            const bool full = sh.list[slot].full != 0;
+            if (!wait(&sh.s_full[w], steps)) {
                 return;
             }
             ++steps;
             const Listed& aux = sh.list[slot];
-            if (aux.full == 0) {
+            if (!full) {
                 // What the row does not see becomes -inf.
                 const uint4 keep4 = kept_columns(p, s, row, aux.key0, aux.gone);
 #pragma unroll 1
