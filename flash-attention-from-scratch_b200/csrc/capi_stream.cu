@@ -344,7 +344,7 @@ int fa_tree_attention(const FaTreeParams* params, void* workspace, uint64_t work
     if (rc != FA_OK) {
         return rc;
     }
-    return done(fa_sm100::launch_tree(*params, status, fa_capi::next_epoch(), workspace, sms, reinterpret_cast<cudaStream_t>(stream)),
+    return done(fa_sm100::launch_tree(*params, status, workspace, sms, reinterpret_cast<cudaStream_t>(stream)),
                 "tree_attention launch");
 }
 

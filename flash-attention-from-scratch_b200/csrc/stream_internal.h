@@ -34,7 +34,7 @@ cudaError_t launch_cached(const FaCachedParams& p, DeviceStatus* status, void* w
 unsigned long long small_tree_workspace_bytes(const FaTreeParams& p, int sm_count);
 cudaError_t launch_small_tree(const FaTreeParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream);
 unsigned long long tree_workspace_bytes(const FaTreeParams& p, int sm_count);
-cudaError_t launch_tree(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count,
+cudaError_t launch_tree(const FaTreeParams& p, DeviceStatus* status, void* workspace, int sm_count,
                         cudaStream_t stream);
 
 cudaError_t launch_rotary(const FaRotaryParams& p, DeviceStatus* status, int sm_count, cudaStream_t stream);

@@ -2,6 +2,33 @@
 //
 //   O_t = sum_j e^(s_tj) v_j / sum_j e^(s_tj),   s_tj = scale q_t.k_j over the context (through a window and
 //   sinks) and those nodes that are t itself or its ancestors
+//
+// The rows of a kv head, its query heads times the nodes, share every key, so an item is (sequence, kv head, up to 256 rows) and
+// its keys come once: 128 at a time by TMA, a copy a page, whatever the pages' size. Up to 16 rows are a matrix instruction's
+// worth of rows for the cached attention's kernel, which takes them (kFewRows). More go to the tensor cores, 128 rows a product:
+// S = Q K^T in tensor memory, its rows' softmax in registers with a running maximum and sum, P back to tensor memory and
+// P V from there. Q, K and V of 16-bit caches are multiplied as they are. Over an e4m3 cache K's codes are multiplied as they are,
+// too, by queries that are taken apart into e4m3 terms (2 for bfloat16, 3 for float16), whose products tensor cores sum
+// in float32: 2 (3) products at twice the rate instead of a K that would have to be widened. V is widened to float16 by four
+// warps, exactly, since P has more bits than e4m3 holds. Scales join the scores: w = e^(s) v_scale is
+// 2^(factor k_scale x + log2 v_scale), so that the maximum that is subtracted bounds what is summed, and the sum takes w / v_scale.
+// P is rounded to 16 bits (float16 over an e4m3 cache, where it is at most 2^8; else the type of V), the sum is not.
+//
+// 16 warps: 2 x 4 softmax (a thread a row), 4 that ready V, one for S, one for P V, two that list key tiles and copy them. The
+// softmax warpgroups have a row tile each (more than 128 rows), or take key tiles in turn and join their sums at the
+// end. There is one S, which a warpgroup takes into registers at once: its place is free for the other's while it computes.
+//
+// What bounds it: a step (128 rows x 128 keys) takes 2100 to 2350 cycles, of which the tensor cores compute 35 to 45% (scores in
+// two or three e4m3 terms among it) and the exponentials' unit 47%; the rest is the chain scores -> registers -> P -> product,
+// which the two warpgroups take in turn. DRAM is a quarter to two thirds of the time (420 MB in 229 us below).
+// Items are laid end to end and cut into equal ranges, one an SM: a CTA that ends early would leave its SM idle, and a
+// cut costs a record of 128 or 256 rows (25 MB written and read for the second case below).
+//
+// Measured (D 128, bf16 queries, 32 heads on 8 kv heads, in a captured graph): over e4m3 pages of 64 tokens, 32 contexts
+// of 4096 to 8192 tokens: 8 nodes 138 us (62 for the cache's bytes), up to 64 nodes 229 to 238 (66; 80 for the products);
+// 4 contexts of 118000 to 131000, 32 nodes: 280 (155; 157). 16-bit pages of 32, 61 nodes on 16 contexts, window 4096: 107 (44; 40).
+// Scores and products issued by one warp: 203 us where two take 182. The wait for a step's list behind that for its
+// scores instead of before: 238 for 229, 298 for 290.
 
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -22,7 +49,8 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100: values of smaller scales (below 2^-91) count as zeros
 constexpr float kLeastFactor = 1e-37f;               // of a score: what is hidden (-inf) stays so
-constexpr float kLazy = 8.0f;                        // P is at most 2^this before O and the sum are rescaled
+// P is at most 2^this before O and the sum are rescaled: float16 holds that, and 2^15 was not faster.
+constexpr float kLazy = 8.0f;
 constexpr int kMostNodes = 256;
 constexpr int kMaskWords = kMostNodes / 32;
 
@@ -40,6 +68,7 @@ constexpr int kListWarps = 2;
 constexpr int kWarps = kScoreWarp + 4;  // whole warpgroups: registers are handed over between those
 constexpr int kThreads = kWarps * 32;
 // Registers: launched with 128 a thread, 512 for a lane of the four warpgroups.
+// 192 and 200 for the softmax were within 2%.
 constexpr int kRegsSoftmax = 184;
 constexpr int kRegsOther = 72;
 static_assert(2 * kRegsSoftmax + 2 * kRegsOther <= 4 * 128, "no more than the launch has");
@@ -320,7 +349,8 @@ __device__ __forceinline__ int tile_key(const Sequence& s, int v) { return (v < 
 
 // How a call is cut: items are (sequence, kv head, block of rows), each a list of key tiles. `whole`: an item a CTA. Else
 // the lists are laid end to end, each behind the few units that an item costs beside its tiles, and cut into equal ranges,
-// one a CTA; parts of cut items go to records, which a second kernel joins.
+// one a CTA; parts of cut items go to records, which a second kernel joins. Heads of 0, 4, 8 units: 8 nodes on 32 contexts 155,
+// 146, 147 us, 64 nodes 245, 238, 241, the window of 4096 108, 107, 115.
 constexpr int kItemHead = 4;
 
 struct Split {
@@ -330,9 +360,18 @@ struct Split {
     int items;  // of a sequence
 };
 
+// The item that a CTA's range begins within, for the join: pieces of it are records of CTAs c0 to c1. None (c1 = 0) where the
+// range begins with an item, or another CTA's range begins within the same one before.
+struct Cut {
+    int b, kvh, block;
+    int c0, c1;
+    int first;  // the record of c0
+};
+
 struct Record {
     float* o;    // [2 grid][D / 4][rows of an item][4]
     float2* ml;  // [2 grid][rows of an item]
+    Cut* cut;    // [grid]
     int* odd;    // [grid]: values that are not finite where some rows do not see them
 };
 
@@ -397,13 +436,33 @@ __device__ __forceinline__ Range locate(const FaTreeParams& p, const Split& spli
     return r;
 }
 
-// A CTA's range as pieces of items, in order. Every role walks it on its own.
+// A CTA's range as pieces of items, in order.
 struct Walk {
     Sequence s;
     int b, item, v;
     long long left;    // units from here on
     int record;        // of the next cut piece
 };
+
+// Found at the start of a CTA's range, by one thread.
+__device__ __forceinline__ Cut cut_at(const Split& split, const Range& range, const Walk& w, int cta) {
+    Cut cut{};
+    if (range.found >= 0 && w.left > 0 && w.v > 0) {
+        const long long head = range.found_base + static_cast<long long>(w.item) * (w.s.tiles + kItemHead);
+        const long long start = head + kItemHead;  // of its tiles
+        const int c0 = static_cast<int>(start / range.per);
+        if (c0 == cta - 1) {
+            cut.b = w.b;
+            cut.kvh = w.item / split.row_blocks;
+            cut.block = w.item - cut.kvh * split.row_blocks;
+            cut.c0 = c0;
+            cut.c1 = static_cast<int>((start + w.s.tiles - 1) / range.per);
+            // A CTA's first piece is its record 0, its last one its record 1.
+            cut.first = 2 * c0 + (c0 * range.per >= head ? 0 : 1);
+        }
+    }
+    return cut;
+}
 
 struct Piece {
     int b, kvh, block, v0, v1;
@@ -475,8 +534,8 @@ struct Waits {
 };
 
 // A bounded wait of a whole warp: 2^20 polls, 20 ms at the least, where a healthy wait is a tile's time. In few instructions,
-// for there are many of them and the kernel's loops have to fit the instruction cache. False: given up, by this warp or another
-// of the CTA.
+// for there are many of them and the kernel's loops have to fit the instruction cache (with a look at the clock in each,
+// 32 nodes on 4 long contexts took 411 us instead of 299). False: given up, by this warp or another of the CTA.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, int phase, const Waits& waits, unsigned code) {
     const uint32_t at = smem_u32(bar);
     const uint32_t parity = static_cast<uint32_t>(phase) & 1u;
@@ -1043,65 +1102,65 @@ __device__ __forceinline__ float bring_queries(const FaTreeParams& p, const uint
             }
         }
 #pragma unroll
-      for (int e2 = 0; e2 < 2; ++e2) {
-        const int i = pass0 + e2;
-        const int owner = row0 + i * kAtOnce;
-        const int r = quarter * 32 + owner;
-        const uint32_t x[8] = {word[e2][0].x ^ sign, word[e2][0].y ^ sign, word[e2][0].z ^ sign, word[e2][0].w ^ sign,
-                               word[e2][1].x ^ sign, word[e2][1].y ^ sign, word[e2][1].z ^ sign, word[e2][1].w ^ sign};
-        if constexpr (!C::E4M3) {
-            store_shared16(tile + tile_offset(r, 2 * part), x[0], x[1], x[2], x[3]);
-            store_shared16(tile + tile_offset(r, 2 * part + 1), x[4], x[5], x[6], x[7]);
-        } else {
-            uint32_t top = 0;  // of the values' bits without sign: their order is that of the sizes
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                top = max(top, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
-            }
-#pragma unroll
-            for (int o = 1; o < kLanes; o <<= 1) {
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-            }
-            // 2^(8 - exponent of the largest), one less where that would pass 448, both it and its inverse normal; 1 for
-            // zeros. A row with an infinity or NaN becomes NaN: e4m3 has no infinity.
-            const uint32_t most = __float_as_uint(widen16<C::BF16>(static_cast<uint16_t>(top)));
-            const int e = static_cast<int>(most >> 23);
-            const int shift = (e == 0 || e == 255) ? 0 : min(max(135 - e - ((most & 0x7fffffu) > 0x600000u ? 1 : 0), -100), 100);
-            const float up = e == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
-            const float back = fmaxf(scale * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23), kLeastFactor);
-            if constexpr (C::NR == 1) {
-                if (part == 0) {
-                    factors[r] = back;
-                }
+        for (int half = 0; half < 2; ++half) {
+            const int i = pass0 + half;
+            const int owner = row0 + i * kAtOnce;
+            const int r = quarter * 32 + owner;
+            const uint32_t x[8] = {word[half][0].x ^ sign, word[half][0].y ^ sign, word[half][0].z ^ sign, word[half][0].w ^ sign,
+                                   word[half][1].x ^ sign, word[half][1].y ^ sign, word[half][1].z ^ sign, word[half][1].w ^ sign};
+            if constexpr (!C::E4M3) {
+                store_shared16(tile + tile_offset(r, 2 * part), x[0], x[1], x[2], x[3]);
+                store_shared16(tile + tile_offset(r, 2 * part + 1), x[4], x[5], x[6], x[7]);
             } else {
-                const float rows_own = __shfl_sync(0xffffffffu, back, (lane % kAtOnce) * kLanes);
-                factor = lane / kAtOnce == i ? rows_own : factor;
-            }
-            float f[16];
+                uint32_t top = 0;  // of the values' bits without sign: their order is that of the sizes
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                f[2 * j] = widen16<C::BF16>(static_cast<uint16_t>(x[j] & 0xffffu)) * up;
-                f[2 * j + 1] = widen16<C::BF16>(static_cast<uint16_t>(x[j] >> 16)) * up;
-            }
-#pragma unroll
-            for (int term = 0; term < C::kTerms; ++term) {
-                uint32_t code[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t lo = pack_e4m3x2(f[4 * j], f[4 * j + 1]);
-                    const uint32_t hi = pack_e4m3x2(f[4 * j + 2], f[4 * j + 3]);
-                    code[j] = lo | (hi << 16);
-                    const float2 u = unpack_half2(e4m3x2_to_half2(lo));
-                    const float2 v = unpack_half2(e4m3x2_to_half2(hi));
-                    f[4 * j] -= u.x;
-                    f[4 * j + 1] -= u.y;
-                    f[4 * j + 2] -= v.x;
-                    f[4 * j + 3] -= v.y;
+                for (int e = 0; e < 8; ++e) {
+                    top = max(top, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
                 }
-                store_shared16(tile + term * C::kRaw + code_offset<C::D>(r, part), code[0], code[1], code[2], code[3]);
+#pragma unroll
+                for (int o = 1; o < kLanes; o <<= 1) {
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                }
+                // 2^(8 - exponent of the largest), one less where that would pass 448, both it and its inverse normal; 1 for
+                // zeros. A row with an infinity or NaN becomes NaN: e4m3 has no infinity.
+                const uint32_t most = __float_as_uint(widen16<C::BF16>(static_cast<uint16_t>(top)));
+                const int e = static_cast<int>(most >> 23);
+                const int shift = (e == 0 || e == 255) ? 0 : min(max(135 - e - ((most & 0x7fffffu) > 0x600000u ? 1 : 0), -100), 100);
+                const float up = e == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+                const float back = fmaxf(scale * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23), kLeastFactor);
+                if constexpr (C::NR == 1) {
+                    if (part == 0) {
+                        factors[r] = back;
+                    }
+                } else {
+                    const float rows_own = __shfl_sync(0xffffffffu, back, (lane % kAtOnce) * kLanes);
+                    factor = lane / kAtOnce == i ? rows_own : factor;
+                }
+                float f[16];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    f[2 * j] = widen16<C::BF16>(static_cast<uint16_t>(x[j] & 0xffffu)) * up;
+                    f[2 * j + 1] = widen16<C::BF16>(static_cast<uint16_t>(x[j] >> 16)) * up;
+                }
+#pragma unroll
+                for (int term = 0; term < C::kTerms; ++term) {
+                    uint32_t code[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t lo = pack_e4m3x2(f[4 * j], f[4 * j + 1]);
+                        const uint32_t hi = pack_e4m3x2(f[4 * j + 2], f[4 * j + 3]);
+                        code[j] = lo | (hi << 16);
+                        const float2 u = unpack_half2(e4m3x2_to_half2(lo));
+                        const float2 v = unpack_half2(e4m3x2_to_half2(hi));
+                        f[4 * j] -= u.x;
+                        f[4 * j + 1] -= u.y;
+                        f[4 * j + 2] -= v.x;
+                        f[4 * j + 3] -= v.y;
+                    }
+                    store_shared16(tile + term * C::kRaw + code_offset<C::D>(r, part), code[0], code[1], code[2], code[3]);
+                }
             }
         }
-      }
     }
     fence_proxy_async_smem();
     return factor;
@@ -1493,8 +1552,8 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, Shared& sh, Excha
 
 template <class C>
 __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ FaTreeParams p, const __grid_constant__ CUtensorMap tm_k,
-                                                           const __grid_constant__ CUtensorMap tm_v, DeviceStatus* status, unsigned epoch,
-                                                           Split split, Record rec) {
+                                                           const __grid_constant__ CUtensorMap tm_v, DeviceStatus* status, Split split,
+                                                           Record rec) {
     extern __shared__ uint8_t raw[];
     uint8_t* smem = raw;  // on 1024 bytes: a kernel without static shared memory has it from there
     Shared& sh = *reinterpret_cast<Shared*>(smem + C::kSmemShared);
@@ -1551,6 +1610,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     if (sh.tmem_base != 0 || (smem_u32(smem) & 1023u) != 0) {
         if (threadIdx.x == 0) {
             atomicOr(&status->code, kStatusTimeoutTeardown);
+            if (!split.whole) {
+                rec.cut[blockIdx.x] = Cut{};
+            }
         }
     } else {
         if (warp < kSoftmaxWarps) {
@@ -1566,6 +1628,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
                 product_warp<C>(sh, smem_u32(smem), waits);
             } else {
                 const Walk walk = start_walk(p, split, range, static_cast<int>(blockIdx.x));
+                if (!split.whole && warp == kListWarp && threadIdx.x % 32 == 0) {
+                    rec.cut[blockIdx.x] = cut_at(split, range, walk, static_cast<int>(blockIdx.x));
+                }
                 list_tiles<C>(p, &tm_k, &tm_v, split, status, walk, sh, smem_u32(smem), warp - kListWarp, waits);
                 // Copies in flight end by themselves; after a wait that was given up they get a millisecond.
                 if (sh.abort != 0) {
@@ -1588,9 +1653,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     }
 }
 
-// The second kernel. Its first CTAs join the records of cut items: CTA k those of the item that was cut at unit (k + 1) per, if
-// that is its first cut, always in the same order; a warp takes a row. The others, `fixers` of them, compute rows anew,
-// one by one, of items in whose tiles infinities or NaN are hidden from some rows (0 times them would be NaN there).
+// The second kernel. Its first CTAs join the records of cut items, always in the same order. The others, `fixers` of them,
+// compute rows anew, one by one, of items in whose tiles infinities or NaN are hidden from some rows (0 times them would be
+// NaN there).
 template <class C>
 __global__ void __launch_bounds__(kRowWarps * 32) tree_finish_kernel(const __grid_constant__ FaTreeParams p, DeviceStatus* status,
                                                                      Split split, Record rec, int joins, int fixers) {
@@ -1607,29 +1672,19 @@ __global__ void __launch_bounds__(kRowWarps * 32) tree_finish_kernel(const __gri
         cudaGridDependencySynchronize();
     }
     if (static_cast<int>(blockIdx.x) < joins) {
-        const long long k = blockIdx.x + 1;
-        const Range range = locate<kRowWarps>(p, split, warp_sum, &found_base, &found, [&](long long per) { return k * per; });
-        if (range.found < 0) {
+        cudaGridDependencySynchronize();  // the records are there
+        const Cut cut = rec.cut[blockIdx.x + 1];
+        // Out of range is what calls that share a workspace at a time make of it.
+        if (cut.c1 <= 0 || cut.c1 >= split.grid || cut.c0 < 0 || cut.first < 0 || cut.first >= 2 * split.grid || cut.b < 0 ||
+            cut.b >= p.cache.batch || cut.kvh < 0 || cut.kvh >= p.cache.kv_heads || cut.block < 0 || cut.block >= split.row_blocks) {
             return;
         }
-        const Sequence s = sequence(p, range.found);
-        const long long item = (k * range.per - range.found_base) / (s.tiles + kItemHead);
-        const long long head = range.found_base + item * (s.tiles + kItemHead);
-        const long long start = head + kItemHead;  // of its tiles
-        if (start >= k * range.per || start / range.per != k - 1) {
-            return;
-        }
-        const int kvh = static_cast<int>(item / split.row_blocks);
-        const int block = static_cast<int>(item - static_cast<long long>(kvh) * split.row_blocks);
         // A warp takes 32 rows and 8 columns, a lane a row.
         constexpr int kAcross = D / 8;
         const int unit = static_cast<int>(blockIdx.y) * kRowWarps + warp;
         const int r = unit / kAcross * 32 + lane;
         const int eight = unit % kAcross;
-        const int row_index = block * C::kRows + r;
-        const long long c0 = start / range.per;
-        const long long c1 = (start + s.tiles - 1) / range.per;
-        cudaGridDependencySynchronize();  // the records are there
+        const int row_index = cut.block * C::kRows + r;
         if (r >= C::kRows || row_index >= rows) {
             return;
         }
@@ -1637,9 +1692,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) tree_finish_kernel(const __gri
         float o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         bool odd = false;
 #pragma unroll 4
-        for (long long c = c0; c <= c1; ++c) {
-            // A CTA's first cut piece is its record 0; the item starts in c0, as its second unless there.
-            const long long record = 2 * c + (c * range.per >= head ? 0 : 1);
+        for (int c = cut.c0; c <= cut.c1; ++c) {
+            const int64_t record = c == cut.c0 ? cut.first : 2 * c;
             odd = odd || (rec.odd != nullptr && rec.odd[c] != 0);
             const float2 ml = rec.ml[record * C::kRows + r];
             const float4* from = reinterpret_cast<const float4*>(rec.o) + (record * (D / 4) + 2 * eight) * C::kRows + r;
@@ -1661,7 +1715,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) tree_finish_kernel(const __gri
             return;  // its rows are computed anew
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        uint16_t* out = static_cast<uint16_t*>(p.o) + ((static_cast<int64_t>(range.found) * p.heads + kvh * group) * p.cache.tokens + row_index) * D;
+        uint16_t* out = static_cast<uint16_t*>(p.o) + ((static_cast<int64_t>(cut.b) * p.heads + cut.kvh * group) * p.cache.tokens + row_index) * D;
         reinterpret_cast<uint4*>(out)[eight] = make_uint4(pack2<C::BF16>(o[0] * inv, o[1] * inv), pack2<C::BF16>(o[2] * inv, o[3] * inv),
                                                           pack2<C::BF16>(o[4] * inv, o[5] * inv), pack2<C::BF16>(o[6] * inv, o[7] * inv));
         return;
@@ -1740,37 +1794,55 @@ cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, cuda
     return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
-constexpr int kWholeTiles = 8;  // up to this many key tiles in the table's capacity items are not cut
 constexpr int kFixers = 64;
 constexpr int kFewRows = 16;
+constexpr int kShort = 16;     // key tiles of a short list
+constexpr int kJoinTiles = 5;  // what the records and their join cost, in key tiles of 1.15 us
 
-// Whether a kv head's rows are better taken 16 at a time.
+// Whether a kv head's rows are better taken 16 at a time, by warps of their own: 16 rows on one context of 777 tokens take 15.5 us
+// there and 17.1 here, 32 rows (8 nodes, above) 168 there and 141 here.
 bool few_rows(const FaTreeParams& p) { return p.heads / p.cache.kv_heads * p.cache.tokens <= kFewRows; }
 
-int row_tiles(const FaTreeParams& p) { return p.heads / p.cache.kv_heads * p.cache.tokens > kTile ? 2 : 1; }
+// Key tiles that a sequence has at most.
+long long most_tiles(const FaCache& c, int window, int sinks) {
+    long long shown = static_cast<long long>(c.max_pages) * c.page_size;
+    if (window > 0) {
+        shown = std::min<long long>(shown, static_cast<long long>(window) + sinks + c.tokens + 3 * kTile);
+    }
+    return (shown + kTile - 1) / kTile;
+}
 
-// `grid` is 0 for what no grid holds.
+// Two row tiles an item, for which a key tile is copied and widened once, or one, of which both softmax warpgroups work on key tiles
+// in turn. One where there are no more rows (32 nodes on 32 contexts of up to 8192 tokens: 148 us, padded to two 232), and where
+// lists are short and SMs would stay idle (64 nodes on 1000 tokens: 22.5 and 33); else two (64 nodes on 32 contexts: 248 and
+// 288; 128 nodes on 4, one item an SM either way: 86 and 88).
+int row_tiles(const FaTreeParams& p, int sm_count) {
+    const long long rows = static_cast<long long>(p.heads / p.cache.kv_heads) * p.cache.tokens;
+    const long long blocks = (rows + kTile - 1) / kTile;
+    const bool is_short = most_tiles(p.cache, p.window, p.sinks) <= kShort;
+    return blocks == 1 || (is_short && blocks * p.cache.kv_heads * p.cache.batch <= sm_count) ? 1 : 2;
+}
+
+// `grid` is 0 for what no grid holds. Short lists are not cut where every item has an SM and the cut would not pay for the records:
+// 16 nodes on 16 contexts of 1024 tokens 21.0 us whole and 30.5 cut, of 2048 30.2 and 39.6; on 4 of 512 15.8 and 16.9, of 1024
+// 20.1 and 19.2, of 2048 28.7 and 22.3; on one of 1024 20.2 and 16.5.
 Split split_for(const FaTreeParams& p, int sm_count) {
     const FaCache& c = p.cache;
     const long long rows = static_cast<long long>(p.heads / c.kv_heads) * c.tokens;
-    const long long block = static_cast<long long>(row_tiles(p)) * kTile;
+    const long long block = static_cast<long long>(row_tiles(p, sm_count)) * kTile;
     const long long row_blocks = (rows + block - 1) / block;
     const long long items = static_cast<long long>(c.kv_heads) * row_blocks;
-    long long shown = static_cast<long long>(c.max_pages) * c.page_size;
-    if (p.window > 0) {
-        shown = std::min<long long>(shown, static_cast<long long>(p.window) + p.sinks + c.tokens + 3 * kTile);
-    }
-    const long long tiles = (shown + kTile - 1) / kTile;
+    const long long tiles = most_tiles(c, p.window, p.sinks);
     Split s;
     s.row_blocks = static_cast<int>(row_blocks);
     s.items = static_cast<int>(items);
-    s.whole = tiles <= kWholeTiles && items * c.batch <= sm_count;
+    s.whole = tiles <= kShort && items * c.batch <= sm_count && (tiles - kJoinTiles) * sm_count <= items * c.batch * (tiles + kItemHead);
     s.grid = static_cast<int>(s.whole ? items * c.batch : std::min<long long>(sm_count, items * c.batch * tiles));
     return s;
 }
 
 template <class C>
-cudaError_t launch(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count, cudaStream_t stream) {
+cudaError_t launch(const FaTreeParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
     const Split split = split_for(p, sm_count);
     constexpr auto kernel = tree_kernel<C>;
     cudaError_t err = ensure_smem_limit<kernel>(smem_bytes<C>());
@@ -1783,7 +1855,8 @@ cudaError_t launch(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, 
         const size_t rows = static_cast<size_t>(split.grid) * 2 * C::kRows;
         rec.o = static_cast<float*>(workspace);
         rec.ml = reinterpret_cast<float2*>(rec.o + rows * C::D);
-        odd = reinterpret_cast<int*>(rec.ml + rows);
+        rec.cut = reinterpret_cast<Cut*>(rec.ml + rows);
+        odd = reinterpret_cast<int*>(rec.cut + split.grid);
     }
     rec.odd = p.cache.tokens > 1 ? odd : nullptr;
     CUtensorMap tm_k, tm_v;
@@ -1793,7 +1866,7 @@ cudaError_t launch(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, 
         encode_pool_map(&tm_v, p.cache, p.cache.v, p.cache.v_stride, C::BF16, raw_v) != CUDA_SUCCESS) {
         return cudaErrorInvalidValue;
     }
-    kernel<<<static_cast<unsigned>(split.grid), kThreads, smem_bytes<C>(), stream>>>(p, tm_k, tm_v, status, epoch, split, rec);
+    kernel<<<static_cast<unsigned>(split.grid), kThreads, smem_bytes<C>(), stream>>>(p, tm_k, tm_v, status, split, rec);
     err = cudaGetLastError();
     const int joins = split.whole ? 0 : split.grid - 1;
     const int fixers = rec.odd != nullptr ? kFixers : 0;
@@ -1806,26 +1879,26 @@ cudaError_t launch(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, 
 }
 
 template <int D, bool BF16, bool E4M3, bool COARSE>
-cudaError_t launch_rows(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count, cudaStream_t stream) {
-    return row_tiles(p) == 1 ? launch<Cfg<D, BF16, E4M3, COARSE, 1>>(p, status, epoch, workspace, sm_count, stream)
-                             : launch<Cfg<D, BF16, E4M3, COARSE, 2>>(p, status, epoch, workspace, sm_count, stream);
+cudaError_t launch_rows(const FaTreeParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
+    return row_tiles(p, sm_count) == 1 ? launch<Cfg<D, BF16, E4M3, COARSE, 1>>(p, status, workspace, sm_count, stream)
+                             : launch<Cfg<D, BF16, E4M3, COARSE, 2>>(p, status, workspace, sm_count, stream);
 }
 
 // Pages of 8 or 16 tokens matter to an e4m3 cache alone, by their scales. (One kernel for both took 271 us for 64 nodes on
 // 32 contexts where this takes 239: what it runs has to fit the instruction cache.)
 template <int D, bool BF16>
-cudaError_t launch_types(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count, cudaStream_t stream) {
+cudaError_t launch_types(const FaTreeParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
     if (p.cache.dtype != FA_DTYPE_FLOAT8_E4M3) {
-        return launch_rows<D, BF16, false, true>(p, status, epoch, workspace, sm_count, stream);
+        return launch_rows<D, BF16, false, true>(p, status, workspace, sm_count, stream);
     }
-    return p.cache.page_size >= 32 ? launch_rows<D, BF16, true, true>(p, status, epoch, workspace, sm_count, stream)
-                                   : launch_rows<D, BF16, true, false>(p, status, epoch, workspace, sm_count, stream);
+    return p.cache.page_size >= 32 ? launch_rows<D, BF16, true, true>(p, status, workspace, sm_count, stream)
+                                   : launch_rows<D, BF16, true, false>(p, status, workspace, sm_count, stream);
 }
 
 template <int D>
-cudaError_t launch_dim(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count, cudaStream_t stream) {
-    return p.dtype == FA_DTYPE_BFLOAT16 ? launch_types<D, true>(p, status, epoch, workspace, sm_count, stream)
-                                        : launch_types<D, false>(p, status, epoch, workspace, sm_count, stream);
+cudaError_t launch_dim(const FaTreeParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
+    return p.dtype == FA_DTYPE_BFLOAT16 ? launch_types<D, true>(p, status, workspace, sm_count, stream)
+                                        : launch_types<D, false>(p, status, workspace, sm_count, stream);
 }
 
 }  // namespace
@@ -1836,16 +1909,16 @@ unsigned long long tree_workspace_bytes(const FaTreeParams& p, int sm_count) {
     }
     const Split split = split_for(p, sm_count);
     const unsigned long long records =
-        split.whole ? 0 : static_cast<unsigned long long>(split.grid) * 2 * row_tiles(p) * kTile * (p.cache.head_dim + 2) * 4;
+        split.whole ? 0 : static_cast<unsigned long long>(split.grid) * (2ull * row_tiles(p, sm_count) * kTile * (p.cache.head_dim + 2) * 4 + sizeof(Cut));
     return records + (p.cache.tokens > 1 ? 4ull * split.grid : 0);
 }
 
-cudaError_t launch_tree(const FaTreeParams& p, DeviceStatus* status, unsigned epoch, void* workspace, int sm_count, cudaStream_t stream) {
+cudaError_t launch_tree(const FaTreeParams& p, DeviceStatus* status, void* workspace, int sm_count, cudaStream_t stream) {
     if (few_rows(p)) {
         return launch_small_tree(p, status, workspace, sm_count, stream);
     }
-    return p.cache.head_dim == 64 ? launch_dim<64>(p, status, epoch, workspace, sm_count, stream)
-                                  : launch_dim<128>(p, status, epoch, workspace, sm_count, stream);
+    return p.cache.head_dim == 64 ? launch_dim<64>(p, status, workspace, sm_count, stream)
+                                  : launch_dim<128>(p, status, workspace, sm_count, stream);
 }
 
 }  // namespace fa_sm100

@@ -2,6 +2,7 @@
 
 import math
 import random
+import sys
 
 import pytest
 import torch
@@ -26,10 +27,20 @@ def _parents(batch, tokens, span, seed):
     return _ints([[max(-1, i - rng.randint(1, span)) for i in range(tokens)] for _ in range(batch)])
 
 
+ROOM = 0  # tokens that tables have places for behind the pages that they hold
+
+
+@pytest.fixture(params=[0, 4200], ids=["short", "long"])
+def room(request, monkeypatch):
+    """What a table could hold decides how a call is cut and whether its rows come 128 or 256 at a time."""
+    monkeypatch.setattr(sys.modules[__name__], "ROOM", request.param)
+
+
 def _cache(gen, batch, most, page, heads, d, dtype, spare=2, low=0.004):
     per = max(1, -(-most // page))
     pages = batch * per + spare
     table = torch.randperm(pages, generator=gen, device=DEV)[: batch * per].to(torch.int32).view(batch, per)
+    table = torch.cat((table, table.new_full((batch, ROOM // page), -1)), dim=1)
     x = [torch.randn(pages, heads, page, d, generator=gen, device=DEV).to(HALF) for _ in "kv"]
     if dtype != E4M3:
         return fa.PagedKVCache(*(t.to(dtype) for t in x)), table
@@ -52,6 +63,7 @@ def _check(q, cache, table, lengths, parents, status=0, **how):
 KINDS = [(HALF, HALF), (BF, BF), (HALF, E4M3), (BF, E4M3)]
 
 
+@pytest.mark.usefixtures("room")
 @pytest.mark.parametrize("dtype,kind", KINDS)
 @pytest.mark.parametrize("group,hk,d,tokens,page,lengths,counts", [
     (1, 1, 64, 1, 16, [1, 2, 200], None),
@@ -73,10 +85,11 @@ def test_trees(group, hk, d, tokens, page, lengths, counts, dtype, kind):
         _check(q, cache, table, _ints(lengths), parents, counts=None if counts is None else _ints(counts))
 
 
+@pytest.mark.usefixtures("room")
 @pytest.mark.parametrize("dtype,kind", KINDS)
 @pytest.mark.parametrize("group,tokens,window,sinks,lengths", [
     (4, 7, 7, 0, [7, 20, 300, 1000]), (4, 32, 130, 4, [40, 129, 600, 3000]), (1, 20, 20, 300, [100, 700, 320]), (2, 128, 1000, 1, [1128, 4000, 128]),
-    (4, 64, 64, 17, [64, 65, 500, 81]), (2, 3, 1 << 30, 5, [800, 3]),
+    (4, 64, 64, 17, [64, 65, 500, 81]), (2, 3, 1 << 30, 5, [800, 3]), (3, 70, 2300, 130, [2500, 70, 4100, 2400]),
 ])
 def test_windows(group, tokens, window, sinks, lengths, dtype, kind):
     gen = torch.Generator(DEV).manual_seed(window)
@@ -94,6 +107,7 @@ def test_a_long_context(dtype, kind):
         _check(q, cache, table, _ints([40001, 29]), _parents(2, tokens, 5, 1), counts=_ints([tokens, min(tokens, 29)]))
 
 
+@pytest.mark.usefixtures("room")
 @pytest.mark.parametrize("dtype,kind", KINDS)
 def test_many_short_sequences(dtype, kind):
     gen = torch.Generator(DEV).manual_seed(3)
@@ -128,6 +142,7 @@ def test_strides_scales_and_one_tree_for_all():
         _check(q, cache, table, _ints([64, 33]), parents, scale=scale)
 
 
+@pytest.mark.usefixtures("room")
 @pytest.mark.parametrize("tokens", [3, 40])
 def test_scales_far_from_one(tokens):
     """Values' scales from 2^-100 to 2^60 in one sequence; the scores' stay where the softmax has a say."""
@@ -151,6 +166,7 @@ def test_large_scores(dtype, kind):
     _check(q, cache, table, _ints([500, 77]), _parents(2, 20, 4, 0))
 
 
+@pytest.mark.usefixtures("room")
 @pytest.mark.parametrize("dtype,kind", KINDS)
 @pytest.mark.parametrize("tokens,window", [(2, 0), (9, 16), (50, 0), (70, 128)])
 def test_hidden_values_have_no_part(dtype, kind, tokens, window):
@@ -191,6 +207,7 @@ def test_hidden_values_have_no_part(dtype, kind, tokens, window):
     stream_oracle.check(torch.where(odd, 0.0, out.double()), torch.where(odd, 0.0, want), torch.where(odd, 1.0, bound), "beside")
 
 
+@pytest.mark.usefixtures("room")
 def test_infinite_and_nan_queries_stay_in_their_rows():
     gen = torch.Generator(DEV).manual_seed(9)
     for tokens in (3, 60):
@@ -207,6 +224,7 @@ def test_infinite_and_nan_queries_stay_in_their_rows():
         assert torch.equal(out, clean)
 
 
+@pytest.mark.usefixtures("room")
 @pytest.mark.parametrize("dtype", [HALF, BF])
 @pytest.mark.parametrize("tokens", [3, 20, 60])
 def test_infinite_queries_over_an_e4m3_cache(tokens, dtype):
@@ -224,6 +242,7 @@ def test_infinite_queries_over_an_e4m3_cache(tokens, dtype):
     assert torch.equal(out, clean)
 
 
+@pytest.mark.usefixtures("room")
 @pytest.mark.parametrize("dtype,kind", KINDS)
 def test_tiny_and_zero_queries_and_scales(dtype, kind):
     """Rows of zeros and of values at the small end of their type weigh what they see alike, or as little apart."""
