@@ -3,30 +3,33 @@
 //   O_t = sum_j e^(s_tj) v_j / sum_j e^(s_tj),   s_tj = scale q_t.k_j over the context (through a window and
 //   sinks) and those nodes that are t itself or its ancestors
 //
-// The rows of a kv head, its query heads times the nodes, share every key, so an item is (sequence, kv head, up to 256 rows) and
-// its keys come once: 128 at a time by TMA, a copy a page, whatever the pages' size. Up to 16 rows are a matrix instruction's
-// worth of rows for the cached attention's kernel, which takes them (kFewRows). More go to the tensor cores, 128 rows a product:
-// S = Q K^T in tensor memory, its rows' softmax in registers with a running maximum and sum, P back to tensor memory and
-// P V from there. Q, K and V of 16-bit caches are multiplied as they are. Over an e4m3 cache K's codes are multiplied as they are,
-// too, by queries that are taken apart into e4m3 terms (2 for bfloat16, 3 for float16), whose products tensor cores sum
-// in float32: 2 (3) products at twice the rate instead of a K that would have to be widened. V is widened to float16 by four
-// warps, exactly, since P has more bits than e4m3 holds. Scales join the scores: w = e^(s) v_scale is
-// 2^(factor k_scale x + log2 v_scale), so that the maximum that is subtracted bounds what is summed, and the sum takes w / v_scale.
-// P is rounded to 16 bits (float16 over an e4m3 cache, where it is at most 2^8; else the type of V), the sum is not.
+// The rows of a kv head, its query heads times the nodes, share every key, so an item is (sequence, kv head, up to 256
+// rows) and its keys come once: 128 at a time by TMA, a copy a page, whatever the pages' size. Up to 16 rows are a matrix
+// instruction's worth of rows for the cached attention's kernel, which takes them (kFewRows). More go to the tensor cores,
+// 128 rows a product: S = Q K^T in tensor memory, its rows' softmax in registers with a running maximum and sum, P back to
+// tensor memory and P V from there. Q, K and V of 16-bit caches are multiplied as they are. Over an e4m3 cache K's codes
+// are multiplied as they are, too, by queries that are taken apart into e4m3 terms (2 for bfloat16, 3 for float16), whose
+// products the tensor cores sum in float32: 2 (3) products at twice the rate instead of a K that would have to be widened.
+// V is widened to float16 by four warps, exactly, since P has more bits than e4m3 holds. Scales join the scores:
+// w = e^(s) v_scale is 2^(factor k_scale x + log2 v_scale), so that the maximum that is subtracted bounds what is summed,
+// and the sum takes w / v_scale. P is rounded to 16 bits as a matrix operand (float16 over an e4m3 cache, where it is at
+// most 2^8; else the type of V), the sum is not.
 //
 // 16 warps: 2 x 4 softmax (a thread a row), 4 that ready V, one for S, one for P V, two that list key tiles and copy them. The
 // softmax warpgroups have a row tile each (more than 128 rows), or take key tiles in turn and join their sums at the
 // end. There is one S, which a warpgroup takes into registers at once: its place is free for the other's while it computes.
 //
-// What bounds it: a step (128 rows x 128 keys) takes 2100 to 2350 cycles, of which the tensor cores compute 35 to 45% (scores in
-// two or three e4m3 terms among it) and the exponentials' unit 47%; the rest is the chain scores -> registers -> P -> product,
-// which the two warpgroups take in turn. DRAM is a quarter to two thirds of the time (420 MB in 229 us below).
-// Items are laid end to end and cut into equal ranges, one an SM: a CTA that ends early would leave its SM idle, and a
-// cut costs a record of 128 or 256 rows (25 MB written and read for the second case below).
+// What bounds it: a step (128 rows x 128 keys) takes 2100 to 2350 cycles, of which the products need 1024 (scores in two
+// e4m3 terms, P V) and the exponentials, in a unit of their own, 1024 too. Two warpgroups take steps in turn, yet the chain
+// scores -> registers -> P -> product of one overlaps the other's only in part, with 40% of the issue slots taken and
+// many waits for instructions that are not in their cache.
+// DRAM takes a quarter to a half of the time. Items are laid end to end and cut into equal ranges, one an SM: an item a CTA
+// would leave SMs idle, and a cut costs a record of 128 or 256 rows (25 MB written and read for the second case below).
 //
 // Measured (D 128, bf16 queries, 32 heads on 8 kv heads, in a captured graph): over e4m3 pages of 64 tokens, 32 contexts
 // of 4096 to 8192 tokens: 8 nodes 138 us (62 for the cache's bytes), up to 64 nodes 229 to 238 (66; 80 for the products);
-// 4 contexts of 118000 to 131000, 32 nodes: 280 (155; 157). 16-bit pages of 32, 61 nodes on 16 contexts, window 4096: 107 (44; 40).
+// 4 contexts of 118000 to 131000, 32 nodes: 280 to 293 (155; 157). 16-bit pages of 32, 61 nodes on 16 contexts of 10000 to
+// 20000, window 4096: 100 (44; 40).
 // Scores and products issued by one warp: 203 us where two take 182. The wait for a step's list behind that for its
 // scores instead of before: 238 for 229, 298 for 290.
 
@@ -47,7 +50,7 @@ namespace fa_sm100 {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100: values of smaller scales (below 2^-91) count as zeros
+constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100: values of smaller scales, which are below 2^-91, count as zeros
 constexpr float kLeastFactor = 1e-37f;               // of a score: what is hidden (-inf) stays so
 // P is at most 2^this before O and the sum are rescaled: float16 holds that, and 2^15 was not faster.
 constexpr float kLazy = 8.0f;
@@ -1064,8 +1067,8 @@ struct Row {
 // A warp's rows of Q's tile (NR 1: half of its 32, the other warpgroup has the others), 16 dims a lane: as they are, or, over
 // an e4m3 cache, as sums of e4m3 terms (each the nearest to what the ones before leave), a row brought to [2^8, 448] by a
 // power of two that its factor takes back. The terms hold bfloat16 and float16 exactly, down to multiples of 2^-10 beside
-// that largest value. `at`, `real`: the lane's own row; ready() waits until the tile may be written. Returns the factor of the lane's
-// own row (NR 1: in `factors` by row, for both warpgroups).
+// that largest value. `at`, `real`: the lane's own row; ready() waits until the tile may be written. Returns the factor of
+// the lane's own row (NR 1: in `factors` by row, for both warpgroups).
 template <class C, class Ready>
 __device__ __forceinline__ float bring_queries(const FaTreeParams& p, const uint16_t* at, bool real, uint32_t tile, int quarter, int w,
                                                float* factors, Ready ready) {
@@ -1408,8 +1411,8 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, Shared& sh, Excha
         int mine = 0;  // scores of this piece taken
         for (int t = NR == 1 ? w : 0; t < n; t += NR == 1 ? 2 : 1, ++mine) {
             const int slot = (tiles + t) % kListed;
-            // P's place is free and the tile listed by the time its scores are there, most of the time. From the scores on it is
-            // a race: the next ones are not begun before these are in registers.
+            // P's place is free and the tile listed by the time its scores are there, most of the time. From the scores on
+            // every instruction counts: the next ones are not begun before these are in registers.
             if ((steps > 0 && !wait(&sh.p_free[w], steps - 1)) || !wait(&sh.list_full[slot], (tiles + t) / kListed)) {
                 return;
             }
@@ -1799,8 +1802,8 @@ constexpr int kFewRows = 16;
 constexpr int kShort = 16;     // key tiles of a short list
 constexpr int kJoinTiles = 5;  // what the records and their join cost, in key tiles of 1.15 us
 
-// Whether a kv head's rows are better taken 16 at a time, by warps of their own: 16 rows on one context of 777 tokens take 15.5 us
-// there and 17.1 here, 32 rows (8 nodes, above) 168 there and 141 here.
+// Whether a kv head's rows are better taken 16 at a time, by warps of their own: 16 rows on one context of 777 tokens take
+// 15.5 us there and 17.1 here, 32 rows (8 nodes, above) 168 there and 141 here.
 bool few_rows(const FaTreeParams& p) { return p.heads / p.cache.kv_heads * p.cache.tokens <= kFewRows; }
 
 // Key tiles that a sequence has at most.
@@ -1812,10 +1815,10 @@ long long most_tiles(const FaCache& c, int window, int sinks) {
     return (shown + kTile - 1) / kTile;
 }
 
-// Two row tiles an item, for which a key tile is copied and widened once, or one, of which both softmax warpgroups work on key tiles
-// in turn. One where there are no more rows (32 nodes on 32 contexts of up to 8192 tokens: 148 us, padded to two 232), and where
-// lists are short and SMs would stay idle (64 nodes on 1000 tokens: 22.5 and 33); else two (64 nodes on 32 contexts: 248 and
-// 288; 128 nodes on 4, one item an SM either way: 86 and 88).
+// Two row tiles an item, for which a key tile is copied and widened once, or one, of which both softmax warpgroups work on
+// key tiles in turn. One where there are no more rows (32 nodes on 32 contexts of up to 8192 tokens: 148 us, padded to two
+// 232), and where lists are short and SMs would stay idle (64 nodes on 1000 tokens: 19.6 and 25.1); else two (64 nodes on
+// 32 contexts: 248 and 288; 128 nodes on 4 of up to 8192, 86 and 88).
 int row_tiles(const FaTreeParams& p, int sm_count) {
     const long long rows = static_cast<long long>(p.heads / p.cache.kv_heads) * p.cache.tokens;
     const long long blocks = (rows + kTile - 1) / kTile;
@@ -1823,9 +1826,9 @@ int row_tiles(const FaTreeParams& p, int sm_count) {
     return blocks == 1 || (is_short && blocks * p.cache.kv_heads * p.cache.batch <= sm_count) ? 1 : 2;
 }
 
-// `grid` is 0 for what no grid holds. Short lists are not cut where every item has an SM and the cut would not pay for the records:
-// 16 nodes on 16 contexts of 1024 tokens 21.0 us whole and 30.5 cut, of 2048 30.2 and 39.6; on 4 of 512 15.8 and 16.9, of 1024
-// 20.1 and 19.2, of 2048 28.7 and 22.3; on one of 1024 20.2 and 16.5.
+// Short lists are not cut where every item has an SM and the cut would not pay for the records: 16 nodes on 16 contexts of
+// 1024 tokens 21.0 us whole and 30.5 cut, of 2048 30.2 and 39.6; on 4 of 512 15.8 and 16.9, of 1024 20.1 and 19.2, of 2048
+// 28.7 and 22.3; on one of 1024 20.2 and 16.5.
 Split split_for(const FaTreeParams& p, int sm_count) {
     const FaCache& c = p.cache;
     const long long rows = static_cast<long long>(p.heads / c.kv_heads) * c.tokens;

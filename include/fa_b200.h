@@ -398,7 +398,8 @@ FA_API int fa_rotary(const FaRotaryParams* params, fa_stream_t stream);
  * at position p = context + (number of its ancestors), context = lengths[b] - counts[b]. It sees
  * position j of the context when window == 0, or p - j < window, or j < sinks, and of the nodes its
  * ancestors and itself. window is 0 or at least `tokens`. The cache's strides are positive, for dims of more than
- * one element, and below 2^40 bytes. */
+ * one element, and below 2^40 bytes. Scales of an e4m3 cache are finite and not negative; values whose
+ * scale is below 2^-100 may count as zeros. */
 typedef struct FaTreeParams {
     FaCache cache;
     const void* q;
