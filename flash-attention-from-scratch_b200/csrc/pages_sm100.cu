@@ -275,8 +275,11 @@ __global__ void __launch_bounds__(kPageThreads) free_kernel(const __grid_constan
 
 constexpr int kReserveThreads = 1024;
 
-// Entries of a row that get new tokens: at most so many.
-__host__ __device__ __forceinline__ int reserve_entries(const FaPages& p) { return (p.tokens + p.page_size - 2) / p.page_size + 1; }
+// Entries of a row that get new tokens: at most so many, and no more than the row has.
+__host__ __device__ __forceinline__ int reserve_entries(const FaPages& p) {
+    const int most = (p.tokens + p.page_size - 2) / p.page_size + 1;
+    return most < p.width ? most : p.width;
+}
 
 // Exclusive prefix sum over the CTA and the total. All threads call.
 __device__ __forceinline__ int block_prefix(int mine, int& total) {

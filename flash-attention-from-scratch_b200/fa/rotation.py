@@ -132,5 +132,9 @@ def rotary(
     axes: Sequence[int] | None = None,
     interleaved: bool = False,
 ) -> tuple[torch.Tensor, torch.Tensor | None]:
-    """forward_rotary with a gradient in q and k (any number of times: a gradient is a rotation itself)."""
+    """forward_rotary with a gradient in q and k (any number of times: a gradient is a rotation itself).
+
+    A step captured in a CUDA graph may hold it as any operation of autograd: warmed up on a side stream, and with no
+    graph of the same leaves left from before the capture, which torch does not survive. forward_rotary and
+    backward_rotary have no such condition."""
     return _Rotary.apply(q, k, positions, cos, sin, axes, interleaved, False)

@@ -170,6 +170,41 @@ def test_graph_and_streams():
     assert torch.equal(out, oq)
 
 
+def test_a_training_step_in_a_graph():
+    """Forward and gradients captured, by the pair of calls and by autograd, and replayed on other values."""
+    gen = torch.Generator(DEV).manual_seed(9)
+    q, dq = (torch.randn(2, 4, 33, 128, generator=gen, device=DEV).to(BF) for _ in range(2))
+    k, dk = (torch.randn(2, 2, 33, 128, generator=gen, device=DEV).to(BF) for _ in range(2))
+    at = torch.randint(0, 50, (2, 33), generator=gen, device=DEV).to(torch.int32)
+    cos, sin = _tables(50, 32)
+
+    def step(q, k):
+        turned = fa.rotary(q, k, at, cos, sin)
+        return *turned, *torch.autograd.grad(turned, (q, k), (dq, dk))
+
+    def pair(q, k):
+        return *fa.forward_rotary(q, k, at, cos, sin), *fa.backward_rotary(dq, dk, at, cos, sin)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    q, k = q.requires_grad_(), k.requires_grad_()
+    with torch.cuda.stream(side):
+        step(q, k)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(q, k)
+        same = pair(q.detach(), k.detach())
+    for seed in (1, 2):
+        with torch.no_grad():
+            for t in (q, k, dq, dk):
+                t.copy_(torch.randn(t.shape, generator=gen, device=DEV))
+        at.copy_(torch.randint(0, 50, at.shape, generator=gen, device=DEV))
+        graph.replay()
+        for x, y, z in zip(out, same, pair(q.detach(), k.detach())):
+            assert torch.equal(x, z) and torch.equal(y, z)
+
+
 def test_empty_and_refused():
     cos, sin = _tables(9, 32)
     at = torch.zeros(0, 3, device=DEV, dtype=torch.int32)
