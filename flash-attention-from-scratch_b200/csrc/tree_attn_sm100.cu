@@ -24,12 +24,12 @@
 // scores -> registers -> P -> product of one overlaps the other's only in part, with 40% of the issue slots taken and
 // many waits for instructions that are not in their cache.
 // DRAM takes a quarter to a half of the time. Items are laid end to end and cut into equal ranges, one an SM: an item a CTA
-// would leave SMs idle, and a cut costs a record of 128 or 256 rows (25 MB written and read for the second case below).
+// would leave SMs idle, and a cut costs a record of 128 or 256 rows (22 MB written and read for the second case below).
 //
 // Measured (D 128, bf16 queries, 32 heads on 8 kv heads, in a captured graph): over e4m3 pages of 64 tokens, 32 contexts
-// of 4096 to 8192 tokens: 8 nodes 138 us (62 for the cache's bytes), up to 64 nodes 229 to 238 (66; 80 for the products);
-// 4 contexts of 118000 to 131000, 32 nodes: 280 to 293 (155; 157). 16-bit pages of 32, 61 nodes on 16 contexts of 10000 to
-// 20000, window 4096: 100 (44; 40).
+// of 4096 to 8192 tokens: 8 nodes 130 us (62 for the cache's bytes), up to 64 nodes 217 (66; 80 for the products);
+// 4 contexts of 118000 to 131000, 32 nodes: 287 (155; 157). 16-bit pages of 32, 61 nodes on 16 contexts of 10000 to
+// 20000, window 4096: 98 (44; 40).
 // Scores and products issued by one warp: 203 us where two take 182. The wait for a step's list behind that for its
 // scores instead of before: 238 for 229, 298 for 290.
 
@@ -1631,10 +1631,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
                 product_warp<C>(sh, smem_u32(smem), waits);
             } else {
                 const Walk walk = start_walk(p, split, range, static_cast<int>(blockIdx.x));
-                if (!split.whole && warp == kListWarp && threadIdx.x % 32 == 0) {
-                    rec.cut[blockIdx.x] = cut_at(split, range, walk, static_cast<int>(blockIdx.x));
-                }
                 list_tiles<C>(p, &tm_k, &tm_v, split, status, walk, sh, smem_u32(smem), warp - kListWarp, waits);
+                // Behind the list, not before it: 217 us for 240 of 64 nodes on 32 contexts.
+                if (!split.whole && warp == kListWarp && threadIdx.x % 32 == 0) {
+                    const Walk start = start_walk(p, split, range, static_cast<int>(blockIdx.x));
+                    rec.cut[blockIdx.x] = cut_at(split, range, start, static_cast<int>(blockIdx.x));
+                }
                 // Copies in flight end by themselves; after a wait that was given up they get a millisecond.
                 if (sh.abort != 0) {
                     const unsigned long long t0 = globaltimer_ns();
