@@ -13,7 +13,7 @@
 // V is widened to float16 by four warps, exactly, since P has more bits than e4m3 holds. Scales join the scores:
 // w = e^(s) v_scale is 2^(factor k_scale x + log2 v_scale), so that the maximum that is subtracted bounds what is summed,
 // and the sum takes w / v_scale. P is rounded to 16 bits as a matrix operand (float16 over an e4m3 cache, where it is at
-// most 2^8; else the type of V), the sum is not.
+// most 2^15; else the type of V), the sum is not.
 //
 // 16 warps: 2 x 4 softmax (a thread a row), 4 that ready V, one for S, one for P V, two that list key tiles and copy them. The
 // softmax warpgroups have a row tile each (more than 128 rows), or take key tiles in turn and join their sums at the
@@ -52,7 +52,8 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100: values of smaller scales, which are below 2^-91, count as zeros
 constexpr float kLeastFactor = 1e-37f;               // of a score: what is hidden (-inf) stays so
-// P is at most 2^this before O and the sum are rescaled: float16 holds that, and 2^15 was not faster.
+// A weight is at most 2^this, relative to the maximum in use, before O and the sum are rescaled. 2^6 took 221 us for 64 nodes on
+// 32 contexts where this takes 217; 2^15 was not faster.
 constexpr float kLazy = 8.0f;
 constexpr int kMostNodes = 256;
 constexpr int kMaskWords = kMostNodes / 32;
@@ -89,6 +90,13 @@ struct Cfg {
     static constexpr bool COARSE = COARSE_;  // 32 keys on end share a page
     static constexpr int NR = NR_;  // row tiles of an item: 1 (key tiles alternate between the softmax warpgroups) or 2
     static constexpr bool kMmaBf16 = BF16 && !E4M3;  // type of P and V (and of Q and K, over a 16-bit cache)
+    // P is 2^kUp times a weight. float16's steps end at 2^-24, so a weight is off by 2^-32 of the largest at most: a flat tail of
+    // 2^20 keys beside an attention sink is there to float16's own precision. Weights as they are (kUp 0) made 0.0078 of a tail's
+    // share of 0.0054 (131000 keys 17 nats below the sink) and 0 of 0.0036 (17.4 nats). Same time.
+    static constexpr float kUp = kMmaBf16 ? 0.0f : 7.0f;
+    // What the sum takes of P: over an e4m3 cache, where P / v_scale may be large, the weight itself.
+    static constexpr float kDown = E4M3 ? 1.0f / 128.0f : 1.0f;
+    static_assert(!E4M3 || kUp == 7.0f, "kDown undoes kUp");
     static constexpr int kElem = E4M3 ? 1 : 2;
     // e4m3 terms that a query is the sum of: bfloat16 has 8 bits, float16 11, a term 4.
     static constexpr int kTerms = E4M3 ? (BF16 ? 2 : 3) : 1;
@@ -114,7 +122,7 @@ struct Cfg {
 };
 
 struct Listed {             // a key tile
-    float4 group[kGroups];  // e4m3: K's scale, log2 of V's, 1 / V's
+    float4 group[kGroups];  // e4m3: K's scale, log2 of V's, kDown / V's
     uint4 shown;            // bits of the rows that some row of the call sees and that have a page
     int key0;               // first position; -1: the list's end
     uint32_t gone;          // bits of groups that are shown and have no page
@@ -589,6 +597,19 @@ __device__ __forceinline__ uint32_t code_offset(int r, int c) {
     return D == 128 ? static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4)) : static_cast<uint32_t>(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
 
+// Two of P: at most 2^(kLazy + kUp), which float16 holds twice over; more where scores pass 2^23 and the maximum is rounded to
+// whole powers of two, and then float16's largest value rather than infinity.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
+    if constexpr (BF16) {
+        return pack_bf162(lo, hi);
+    } else {
+        uint32_t r;
+        asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+}
+
 __device__ __forceinline__ void store_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -758,7 +779,7 @@ __device__ __forceinline__ void list_tiles(const FaTreeParams& p, const CUtensor
             tiny = vs < kMinScale;
             const float used = tiny ? kMinScale : vs;
             if (lane < kGroups) {
-                to.group[lane] = make_float4(ks, __log2f(used), __fdividef(1.0f, used), 0.0f);
+                to.group[lane] = make_float4(ks, __log2f(used), __fdividef(C::kDown, used), 0.0f);
             }
         }
         const uint32_t paged = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
@@ -1231,7 +1252,7 @@ __device__ __forceinline__ void group_exponentials(const uint32_t (&x)[N], int a
         float2 y = __ffma2_rn(make_float2(u2f(x[at + 2 * i]), u2f(x[at + 2 * i + 1])), f2, add2);
         y = make_float2(ex2_approx(y.x), ex2_approx(y.y));
         sum[i & 3] = i < 4 ? y : __fadd2_rn(sum[i & 3], y);
-        packed[i] = pack2<C::kMmaBf16>(y.x, y.y);
+        packed[i] = pack_weights<C::kMmaBf16>(y.x, y.y);
     }
     const float2 all = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
     l = fmaf(all.x + all.y, inv, l);
@@ -1269,7 +1290,7 @@ __device__ __forceinline__ float exponentials(const Listed& aux, uint32_t tmem_s
         top = row_extreme<true, 128>(x) * factor;
     }
     const float alpha = raise(top, m, l);
-    const float used = m == -INFINITY ? 0.0f : m;
+    const float used = (m == -INFINITY ? 0.0f : m) - C::kUp;
     __syncwarp();  // tensor memory is accessed by whole warps
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -1303,7 +1324,7 @@ __device__ __forceinline__ float exponentials_by_8(const Listed& aux, uint32_t t
         }
     }
     const float alpha = raise(top, m, l);
-    const float used = m == -INFINITY ? 0.0f : m;
+    const float used = (m == -INFINITY ? 0.0f : m) - C::kUp;
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
         uint32_t x[32], packed[16];
@@ -1495,7 +1516,7 @@ __device__ __forceinline__ void softmax(const FaTreeParams& p, Shared& sh, Excha
         const bool self = NR == 2 || w == 0 || n > 1;     // this one does
         const bool in_rows = row_index < rows;
         const int record = s.record;
-        const float inv = record >= 0 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+        const float inv = (record >= 0 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l)) * C::kDown;
         own_weight = row.real ? own_weight * inv : 0.0f;
         other_weight = row.real ? other_weight * inv : 0.0f;
         // Rows of an item lie one after another in the output. In a record four columns of all rows do, so that the

@@ -15,6 +15,7 @@ import fa
 import fa.draft
 import fa.pages
 import fa.rotation
+import tree_bound
 from fa import _C
 
 REPO = Path(__file__).resolve().parent.parent
@@ -226,3 +227,16 @@ def test_oracle_of_the_pages():
     assert pages.reserve(table, [34, 10], 1, 16)[0] == [True, False]
     pages.free(fork, [1, 0, 0])
     assert fork == [[3, -1, -1], [-1, -1, -1], [-1, -1, -1]]
+
+
+def test_the_derived_bound_by_hand():
+    """Two keys, one a sink; what tree_bound allows is above the rounding of P and of the output and below twice their sum."""
+    cache = type("Cache", (), dict(k=torch.zeros(1, 1, 8, 64), v=torch.ones(1, 1, 8, 64), k_scale=None, v_scale=None, num_pages=1, page_size=8, kv_heads=1))
+    cache.k, cache.v = cache.k.half(), cache.v.half()
+    cache.k[0, 0, 0] = 1.0
+    cache.v[0, 0, 0] = 0.0
+    q, lengths = torch.full((1, 1, 1, 64), 2.0, dtype=torch.float16), torch.tensor([2], dtype=torch.int32)
+    o, bound = tree_bound.tree(q, cache, torch.tensor([[0]]), lengths, torch.tensor([[-1]]), scale=1 / 64)
+    want = 1 / (1 + math.exp(2))
+    assert abs(o[0, 0, 0, 0].item() - want) < 1e-12
+    assert 2 * 2.0**-11 * want < bound[0, 0, 0, 0].item() < 4 * 2.0**-11 * want
