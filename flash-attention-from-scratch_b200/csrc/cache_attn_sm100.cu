@@ -38,7 +38,7 @@
 //
 // e4m3's value scales. With w_j = e^(s_j) vs_j (vs_j: the scale of j's page) O = sum w_j c_j / sum
 // (w_j / vs_j) over the codes c_j. The running maximum is taken over log2 w_j = s_j log2 e + log2
-// vs_j, so P <= 1 keeps its 11 bits where the output comes from, whatever the scales of other
+// vs_j, so P (at most 2^kUp) keeps its 11 bits where the output comes from, whatever the scales of other
 // pages; the sum takes P / vs_j in fp32. Scales below 2^-60 (0 among them) enter as 2^-60 with P
 // scaled down.
 
@@ -93,6 +93,10 @@ struct Cfg {
     static constexpr bool BF16 = BF16_;  // queries and output
     static constexpr bool E4M3 = E4M3_;
     static constexpr bool kMmaBf16 = BF16 && !E4M3;
+    // P, its sum and O are 2^kUp times what they stand for. float16's steps end at 2^-24: with P <= 1 a flat tail 17 nats below
+    // an attention sink counted half as much again in the sink's warp, from 17.4 on not at all. With 2^7 a weight is off by 2^-32
+    // of the largest at most. A power that the maximum's own rounding (to whole numbers from 2^24 on) makes 2^8 at most.
+    static constexpr float kUp = kMmaBf16 ? 0.0f : 7.0f;
     static constexpr int kElem = E4M3 ? 1 : 2;
     static constexpr int kRowBytes = D * kElem;
     static constexpr int kKeys = kTileBytes / kRowBytes;  // 16, 32 or 64
@@ -618,7 +622,7 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, const Parents& t
                 }
             }
         }
-        float used[2];
+        float base[2];  // of the exponents
         bool grew = false;
         float alpha[2];
 #pragma unroll
@@ -626,8 +630,9 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, const Parents& t
             top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
             top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
             const float now = fmaxf(m[half], top[half]);
-            used[half] = now == -INFINITY ? 0.0f : now;
-            alpha[half] = ex2_approx(m[half] - used[half]);
+            const float used = now == -INFINITY ? 0.0f : now;
+            base[half] = used - C::kUp;
+            alpha[half] = ex2_approx(m[half] - used);
             grew = grew || now > m[half];
             m[half] = now;
         }
@@ -646,8 +651,8 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, const Parents& t
         for (int n = 0; n < C::kNTiles; ++n) {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const float p0 = ex2_approx(x[n][2 * half] - used[half]);
-                const float p1 = ex2_approx(x[n][2 * half + 1] - used[half]);
+                const float p0 = ex2_approx(x[n][2 * half] - base[half]);
+                const float p1 = ex2_approx(x[n][2 * half + 1] - base[half]);
                 l[half] = C::E4M3 ? fmaf(p0 + p1, inv_vs[n], l[half]) : l[half] + (p0 + p1);
                 x[n][2 * half] = p0;
                 x[n][2 * half + 1] = p1;

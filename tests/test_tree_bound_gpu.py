@@ -76,12 +76,19 @@ def _check_many(q, cache, table, length, parents, scale):
     out = fa.forward_tree(of_all[0], cache, *of_all[1:], softmax_scale=scale)
     for b in range(MANY):
         stream_oracle.check(out[b : b + 1], want, bound, f"sequence {b}")
+    tokens = q.shape[2]
+    if tokens <= 4:
+        chain = torch.arange(-1, tokens - 1, device=DEV, dtype=torch.int32)[None]
+        want, bound = tree_bound.tree(q, cache, table, _ints([length]), chain, scale=scale)
+        out = fa.forward_cached(of_all[0], cache, *of_all[1:3], softmax_scale=scale)
+        for b in range(MANY):
+            stream_oracle.check(out[b : b + 1], want, bound, f"cached, sequence {b}")
     assert _C.device_status(0, clear=True) == 0
     return want
 
 
 @pytest.mark.parametrize("dtype,kind", KINDS)
-@pytest.mark.parametrize("tokens", NODES[1:])
+@pytest.mark.parametrize("tokens", [1, 2] + NODES[1:])
 def test_a_long_tail_beside_a_sink(tokens, dtype, kind):
     """One key, whose value is 0, outweighs every other by 14 to 17 nats; 33000 of those together are the answer."""
     gen = torch.Generator(DEV).manual_seed(2)
@@ -103,7 +110,7 @@ def test_a_long_tail_beside_a_sink(tokens, dtype, kind):
     assert (want > 4e-4).all() and (want < 0.1).all()
 
 
-@pytest.mark.parametrize("tokens", NODES[1:])
+@pytest.mark.parametrize("tokens", NODES)
 def test_a_tail_of_other_scales(tokens):
     """The same where the tail's pages have smaller and larger value scales than the sink's."""
     gen = torch.Generator(DEV).manual_seed(3)
