@@ -1145,11 +1145,12 @@ __device__ __forceinline__ float bring_queries(const FaTreeParams& p, const uint
                 for (int o = 1; o < kLanes; o <<= 1) {
                     top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
                 }
-                // 2^(8 - exponent of the largest), one less where that would pass 448, both it and its inverse normal; 1 for
-                // zeros. A row with an infinity or NaN becomes NaN: e4m3 has no infinity.
+                // 2^(8 - exponent of the largest), one less where that would pass 448: from 2^-120 on, and to 2^100, so that the
+                // factor, which takes it back, stays above kLeastFactor; 1 for zeros. A row with an infinity or NaN becomes NaN:
+                // e4m3 has no infinity.
                 const uint32_t most = __float_as_uint(widen16<C::BF16>(static_cast<uint16_t>(top)));
                 const int e = static_cast<int>(most >> 23);
-                const int shift = (e == 0 || e == 255) ? 0 : min(max(135 - e - ((most & 0x7fffffu) > 0x600000u ? 1 : 0), -100), 100);
+                const int shift = (e == 0 || e == 255) ? 0 : min(135 - e - ((most & 0x7fffffu) > 0x600000u ? 1 : 0), 100);
                 const float up = e == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
                 const float back = fmaxf(scale * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23), kLeastFactor);
                 if constexpr (C::NR == 1) {

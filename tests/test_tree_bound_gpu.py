@@ -144,3 +144,16 @@ def test_scores_beyond_whole_numbers(tokens, dtype, kind):
     for power in range(10, 23):
         out = fa.forward_tree(q, cache, table, lengths, parents, softmax_scale=2.0**power)
         stream_oracle.check(out[clear], want[clear], 2.0**-7 * want[clear].abs() + 1e-6, f"2^{power}")
+
+
+@pytest.mark.parametrize("kind", [BF, E4M3])
+@pytest.mark.parametrize("tokens", NODES[1:])
+def test_bfloat16_queries_far_beyond_float16(tokens, kind):
+    """Largest elements from 2^100 to 2^121 in rows whose scores are about 1: the others are beside them as they are."""
+    gen = torch.Generator(DEV).manual_seed(4)
+    cache, table = _cache(gen, 1, 500, 16, 1, 64, kind)
+    x = torch.randn(1, 4, tokens, 64, generator=gen, device=DEV).clamp(-3.9, 3.9)
+    for power in (100, 108, 112, 119):
+        q = (x * 2.0**power).to(BF)
+        q[..., ::7] *= 2.0**-8
+        _check(q, cache, table, _ints([500]), _parents(1, tokens, 3, 0), f"2^{power}", scale=2.0 ** (-power - 2))
