@@ -521,9 +521,9 @@ __device__ __forceinline__ void attend(const FaCachedParams& p, const Parents& t
         if constexpr (C::E4M3 && C::BF16) {
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            // 2^(13 - exponent of amax), both it and its inverse normal; 1 for zeros, inf and NaN.
+            // 2^(13 - exponent of amax), from 2^-114 to 2^100, both it and its inverse normal; 1 for zeros, inf and NaN.
             const int e = static_cast<int>(__float_as_uint(amax) >> 23);
-            const int shift = (e == 0 || e == 255) ? 0 : min(max(140 - e, -100), 100);
+            const int shift = (e == 0 || e == 255) ? 0 : min(140 - e, 100);
             const float up = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
             factor[half] *= __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
 #pragma unroll

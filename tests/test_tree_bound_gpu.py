@@ -147,7 +147,7 @@ def test_scores_beyond_whole_numbers(tokens, dtype, kind):
 
 
 @pytest.mark.parametrize("kind", [BF, E4M3])
-@pytest.mark.parametrize("tokens", NODES[1:])
+@pytest.mark.parametrize("tokens", [1] + NODES)
 def test_bfloat16_queries_far_beyond_float16(tokens, kind):
     """Largest elements from 2^100 to 2^121 in rows whose scores are about 1: the others are beside them as they are."""
     gen = torch.Generator(DEV).manual_seed(4)
@@ -157,3 +157,8 @@ def test_bfloat16_queries_far_beyond_float16(tokens, kind):
         q = (x * 2.0**power).to(BF)
         q[..., ::7] *= 2.0**-8
         _check(q, cache, table, _ints([500]), _parents(1, tokens, 3, 0), f"2^{power}", scale=2.0 ** (-power - 2))
+        if tokens < 20:
+            chain = torch.arange(-1, tokens - 1, device=DEV, dtype=torch.int32)[None]
+            want, bound = tree_bound.tree(q, cache, table, _ints([500]), chain, scale=2.0 ** (-power - 2))
+            out = fa.forward_cached(q, cache, table, _ints([500]), softmax_scale=2.0 ** (-power - 2))
+            stream_oracle.check(out, want, bound, f"cached 2^{power}")
