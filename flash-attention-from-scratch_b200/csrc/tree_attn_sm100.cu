@@ -92,8 +92,10 @@ struct Cfg {
     static constexpr bool kMmaBf16 = BF16 && !E4M3;  // type of P and V (and of Q and K, over a 16-bit cache)
     // P is 2^kUp times a weight. float16's steps end at 2^-24, so a weight is off by 2^-32 of the largest at most: a flat tail of
     // 2^20 keys beside an attention sink is there to float16's own precision. Weights as they are (kUp 0) made 0.0078 of a tail's
-    // share of 0.0054 (131000 keys 17 nats below the sink) and 0 of 0.0036 (17.4 nats). Same time.
-    static constexpr float kUp = kMmaBf16 ? 0.0f : 7.0f;
+    // share of 0.0054 (131000 keys 17 nats below the sink) and 0 of 0.0036 (17.4 nats). Same time. bfloat16 has float32's range
+    // at the small end and needs it at the large one: P is at most 1, so that the unnormalised O of values near the end of that
+    // range does not overflow by P.
+    static constexpr float kUp = kMmaBf16 ? -kLazy : 7.0f;
     // What the sum takes of P: over an e4m3 cache, where P / v_scale may be large, the weight itself.
     static constexpr float kDown = E4M3 ? 1.0f / 128.0f : 1.0f;
     static_assert(!E4M3 || kUp == 7.0f, "kDown undoes kUp");

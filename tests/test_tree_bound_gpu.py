@@ -162,3 +162,17 @@ def test_bfloat16_queries_far_beyond_float16(tokens, kind):
             want, bound = tree_bound.tree(q, cache, table, _ints([500]), chain, scale=2.0 ** (-power - 2))
             out = fa.forward_cached(q, cache, table, _ints([500]), softmax_scale=2.0 ** (-power - 2))
             stream_oracle.check(out, want, bound, f"cached 2^{power}")
+
+
+@pytest.mark.parametrize("tokens", NODES)
+def test_large_values_of_bfloat16(tokens):
+    """Values of 2^117, the later ones 2^7 times as heavy as the first: a sum of weights up to 1 times them is in range."""
+    gen = torch.Generator(DEV).manual_seed(7)
+    cache, table = _cache(gen, 1, 400, 16, 1, 64, BF)
+    cache.k.fill_(0.0)
+    for i in range(25):
+        cache.k[int(table[0, i]), ..., 0] = 1.0 if i >= 8 else 0.0
+    cache.v.copy_(2.0**117 * (1 + torch.rand(cache.v.shape, generator=gen, device=DEV)))
+    q = torch.zeros(1, 4, tokens, 64, device=DEV, dtype=BF)
+    q[..., 0] = 7 * math.log(2)
+    _check(q, cache, table, _ints([400]), _parents(1, tokens, 3, 0), scale=1.0)
