@@ -137,4 +137,5 @@ def rotary(
     A step captured in a CUDA graph may hold it as any operation of autograd: warmed up on a side stream, and with no
     graph of the same leaves left from before the capture, which torch does not survive. forward_rotary and
     backward_rotary have no such condition."""
-    return _Rotary.apply(q, k, positions, cos, sin, axes, interleaved, False)
+    # As bytes: the gradients turn by what is in the sequence now, whatever becomes of it.
+    return _Rotary.apply(q, k, positions, cos, sin, None if axes is None else bytes(tuple(axes)), interleaved, False)

@@ -223,3 +223,18 @@ def test_empty_and_refused():
                        (lambda: fa.forward_rotary(torch.zeros(2, 4, 3, 68, device=DEV, dtype=HALF)[..., :64], None, at, cos, sin), "multiples of 8")):
         with pytest.raises(ValueError, match=match):
             bad()
+
+
+def test_axes_edited_between_forward_and_backward():
+    """The gradient turns by the axes that the forward turned by, whatever becomes of the caller's list."""
+    gen = torch.Generator(DEV).manual_seed(10)
+    q, k = (torch.randn(2, n, 7, 64, generator=gen, device=DEV).to(BF).requires_grad_() for n in (4, 1))
+    positions = torch.randint(0, 9, (2, 2, 7), generator=gen, device=DEV, dtype=torch.int32)
+    cos, sin = _tables(9, 32)
+    axes = [i % 2 for i in range(32)]
+    turned = fa.rotary(q, k, positions, cos, sin, axes=axes)
+    dq, dk = (torch.randn(t.shape, generator=gen, device=DEV).to(BF) for t in turned)
+    want = fa.backward_rotary(dq, dk, positions, cos, sin, axes=axes)
+    axes[:] = [0] * 32
+    got = torch.autograd.grad(turned, (q, k), (dq, dk))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
