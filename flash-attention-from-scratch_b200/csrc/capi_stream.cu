@@ -277,6 +277,9 @@ int validate_pages(const FaPages* p, const char* op) {
     if (p->batch <= 0 || p->batch > 65535 || p->width <= 0 || p->num_pages <= 0 || p->table_stride < p->width) {
         return invalid(op, "batch (<= 65535), width and num_pages must be positive, rows at least a row apart");
     }
+    if (p->num_pages > (1 << 30)) {  // fa_reserve_pages steps over them 4096 at a time, in 32 bits
+        return invalid(op, "num_pages must be <= 2^30, got " + std::to_string(p->num_pages));
+    }
     if (p->refs == nullptr || p->table == nullptr) {
         return invalid(op, "refs and table must be given");
     }

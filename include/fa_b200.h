@@ -489,7 +489,7 @@ typedef struct FaPages {
     int32_t* dst;
     int64_t table_stride;
     int64_t from_stride;
-    int32_t num_pages;
+    int32_t num_pages; /* up to 2^30 */
     int32_t batch;
     int32_t width; /* width * page_size < 2^31 */
     int32_t from_batch;

@@ -240,3 +240,10 @@ def test_the_derived_bound_by_hand():
     want = 1 / (1 + math.exp(2))
     assert abs(o[0, 0, 0, 0].item() - want) < 1e-12
     assert 2 * 2.0**-11 * want < bound[0, 0, 0, 0].item() < 4 * 2.0**-11 * want
+
+
+def test_pools_beyond_the_kernels_indexes_are_refused():
+    for entry in ("fork", "free"):
+        _refused(f"fa_{entry}_pages", _pages(pages=(1 << 30) + 1), "num_pages", None)
+    _refused("fa_reserve_workspace_size", _pages(pages=(1 << 30) + 1), "num_pages", None)
+    _refused("fa_reserve_pages", _pages(pages=2**31 - 1), "num_pages", None, 0, None)
