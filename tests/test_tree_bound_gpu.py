@@ -176,3 +176,35 @@ def test_large_values_of_bfloat16(tokens):
     q = torch.zeros(1, 4, tokens, 64, device=DEV, dtype=BF)
     q[..., 0] = 7 * math.log(2)
     _check(q, cache, table, _ints([400]), _parents(1, tokens, 3, 0), scale=1.0)
+
+
+@pytest.mark.parametrize("dtype,kind", KINDS)
+@pytest.mark.parametrize("tokens", NODES)
+def test_queries_with_one_large_channel(tokens, dtype, kind):
+    """One channel 2^3 to 2^10 times the others, where the keys have next to nothing."""
+    gen = torch.Generator(DEV).manual_seed(5)
+    cache, table = _cache(gen, 2, 400, 32, 1, 128, kind)
+    if kind == E4M3:
+        cache.k.view(torch.uint8)[..., 77] &= 0x87  # subnormal codes
+    else:
+        cache.k[..., 77] *= 2.0**-8
+    q = torch.randn(2, 4, tokens, 128, generator=gen, device=DEV)
+    for power in (3, 6, 9):
+        q[..., 77] = 2.0**power * (1 + torch.rand(2, 4, tokens, generator=gen, device=DEV))
+        _check(q.to(dtype), cache, table, _ints([400, 111]), _parents(2, tokens, 3, 0), f"2^{power}", scale=0.02)
+
+
+@pytest.mark.parametrize("dtype,kind", KINDS)
+@pytest.mark.parametrize("tokens", NODES)
+def test_scales_of_any_sign_and_strided_pools(tokens, dtype, kind):
+    gen = torch.Generator(DEV).manual_seed(6)
+    plain, table = _cache(gen, 2, 300, 16, 2, 64, kind)
+    # [pages][k, v][slots][heads] of another pool's pages: page and head strides of their own.
+    raw = torch.uint8 if kind == E4M3 else kind
+    both = torch.zeros(plain.num_pages, 3, 2, 16, 64, device=DEV, dtype=raw)
+    both[:, 0], both[:, 2] = plain.k.view(raw), plain.v.view(raw)
+    cache = fa.PagedKVCache(both[:, 0].view(kind), both[:, 2].view(kind), plain.k_scale, plain.v_scale)
+    q = torch.randn(2, tokens, 8, 64, generator=gen, device=DEV).to(dtype).transpose(1, 2)
+    for scale in (0.0, -0.125, -0.4, 0.3):
+        out = _check(q, cache, table, _ints([300, 200]), _parents(2, tokens, 3, 0), f"scale {scale}", scale=scale)
+        assert torch.equal(out, fa.forward_tree(q, plain, table, _ints([300, 200]), _parents(2, tokens, 3, 0), softmax_scale=scale))
