@@ -264,7 +264,8 @@ __device__ __forceinline__ Range locate(const FaCachedParams& p, int grid, At at
 }
 
 // Trees of few rows: 16 of a kv head's rows, query heads times nodes, are one matrix instruction's worth of rows here, where
-// the tensor cores' kernel would pad them to 128 (6 nodes of one sequence of 777 tokens, 16 heads: 15.5 us, 17.1 there). What
+// the tensor cores' kernel would pad them to 128 (16 nodes of one sequence of 777 tokens, 16 heads: 15.5 us, 17.1
+// there; 4 nodes on 32 contexts of 4096 to 8192, 32 heads on 8, e4m3, 90 us, 61 for the cache's bytes). What
 // differs is what a row sees: a node's ancestors are bits of a word, its position is their number behind the context.
 struct Parents {
     const int32_t* parents;

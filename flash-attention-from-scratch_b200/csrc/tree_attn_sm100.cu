@@ -29,7 +29,8 @@
 // Measured (D 128, bf16 queries, 32 heads on 8 kv heads, in a captured graph): over e4m3 pages of 64 tokens, 32 contexts
 // of 4096 to 8192 tokens: 8 nodes 130 us (62 for the cache's bytes), up to 64 nodes 217 (66; 80 for the products);
 // 4 contexts of 118000 to 131000, 32 nodes: 287 (155; 157). 16-bit pages of 32, 61 nodes on 16 contexts of 10000 to
-// 20000, window 4096: 98 (44; 40).
+// 20000, window 4096: 98 (44; 40). Other forms of the first two: float16 queries (three terms) 142 and 243, pages of 16 or 8
+// (scores read twice) 175 and 342, both 210 and 386; 16-bit caches 140 to 144 (122) and 215 to 221 (127; 80).
 // Scores and products issued by one warp: 203 us where two take 182. The wait for a step's list behind that for its
 // scores instead of before: 238 for 229, 298 for 290.
 
@@ -1089,8 +1090,8 @@ struct Row {
 
 // A warp's rows of Q's tile (NR 1: half of its 32, the other warpgroup has the others), 16 dims a lane: as they are, or, over
 // an e4m3 cache, as sums of e4m3 terms (each the nearest to what the ones before leave), a row brought to [2^8, 448] by a
-// power of two that its factor takes back. The terms hold bfloat16 and float16 exactly, down to multiples of 2^-10 beside
-// that largest value. `at`, `real`: the lane's own row; ready() waits until the tile may be written. Returns the factor of
+// power of two that its factor takes back. e4m3's steps end at 2^-9: two terms hold bfloat16 exactly down to 2^-10 of the row's
+// largest value, three float16 down to 2^-7 of it, and what is smaller is off by 2^-18 of the largest at most. `at`, `real`: the lane's own row; ready() waits until the tile may be written. Returns the factor of
 // the lane's own row (NR 1: in `factors` by row, for both warpgroups).
 template <class C, class Ready>
 __device__ __forceinline__ float bring_queries(const FaTreeParams& p, const uint16_t* at, bool real, uint32_t tile, int quarter, int w,
@@ -1854,7 +1855,8 @@ int row_tiles(const FaTreeParams& p, int sm_count) {
 
 // Short lists are not cut where every item has an SM and the cut would not pay for the records: 16 nodes on 16 contexts of
 // 1024 tokens 21.0 us whole and 30.5 cut, of 2048 30.2 and 39.6; on 4 of 512 15.8 and 16.9, of 1024 20.1 and 19.2, of 2048
-// 28.7 and 22.3; on one of 1024 20.2 and 16.5.
+// 28.7 and 22.3; on one of 1024 20.2 and 16.5. Lengths are on the device, so a list is as short as the table is narrow: behind a
+// table of 131072 places 16 nodes on 16 contexts of 1024 take 30.6 us (21.5 behind one of 1024), 64 nodes on 1000 26.4 (19.7).
 Split split_for(const FaTreeParams& p, int sm_count) {
     const FaCache& c = p.cache;
     const long long rows = static_cast<long long>(p.heads / c.kv_heads) * c.tokens;
